@@ -1012,6 +1012,238 @@ int gemma_hip_prefill_attention(float *out, const float *q, int q_stride, const 
   return 0;
 }
 
+/* ---- batches of sequences: 8-bit paged cache, attention over it, sampling - */
+
+}  // extern "C"
+
+namespace {
+
+// The kernels run on the library's GPU; memory and streams of another one are
+// not theirs.
+int need_device(const char *name) {
+  if (need_init()) return 1;
+  int dev = -1;
+  GH_CHECK(name, hipGetDevice(&dev));
+  if (dev != g.device)
+    return fail("%s: the current device is %d, the library's is %d", name, dev, g.device);
+  return 0;
+}
+
+bool aligned16(const void *p) { return (uintptr_t)p % 16 == 0; }
+
+// A cache and a batch as the kernels take them; 1 and a message where their sizes
+// don't fit.
+int kv_args(const char *name, const gemma_hip_cache *cache, const gemma_hip_batch *batch,
+            gh::KvCache *c, gh::KvBatch *b) {
+  if (cache == nullptr || batch == nullptr) return fail("%s: null pointer", name);
+  const int page = cache->page;
+  if (cache->type != GEMMA_HIP_CACHE_I8 && cache->type != GEMMA_HIP_CACHE_E4M3)
+    return fail("%s: unknown cache type %d", name, cache->type);
+  if ((cache->hdim != 128 && cache->hdim != 256) || cache->nkv < 1 || cache->nkv > 1024)
+    return fail("%s: unsupported cache of %d heads of %d", name, cache->nkv, cache->hdim);
+  if (page < 16 || (page & (page - 1)) != 0 || page > (1 << 24) || cache->npages < 1)
+    return fail("%s: %d pages of %d positions (a power of two from 16 to 2^24)", name,
+                cache->npages, page);
+  if (batch->batch < 0 || batch->batch > 65535 || batch->rows < 0 || batch->max_rows < 0 ||
+      batch->max_rows > batch->rows || batch->max_pages < 0 || batch->max_len < 0 ||
+      batch->max_len > (1 << 30) || (long)batch->max_pages * page < batch->max_len)
+    return fail("%s: bad batch: %d sequences, %d rows (%d at most), %d positions in %d pages of %d",
+                name, batch->batch, batch->rows, batch->max_rows, batch->max_len,
+                batch->max_pages, page);
+  int shift = 0;
+  while ((1 << shift) < page) ++shift;
+  *c = gh::KvCache{(uint8_t *)cache->k, (uint8_t *)cache->v, cache->ks, cache->vs,
+                   cache->type == GEMMA_HIP_CACHE_I8 ? gh::kKvI8 : gh::kKvE4m3,
+                   cache->npages, shift, cache->nkv, cache->hdim};
+  *b = gh::KvBatch{batch->pages, batch->len, batch->row0, batch->batch, batch->max_pages,
+                   batch->rows, batch->max_rows, batch->max_len};
+  return 0;
+}
+
+// ... and their pointers, where there is something to do.
+int kv_pointers(const char *name, const gh::KvCache &c, const gh::KvBatch &b) {
+  if (!c.k || !c.v || !c.ks || !c.vs || !b.len || !b.row0 || (!b.pages && b.width > 0))
+    return fail("%s: null pointer", name);
+  if (!aligned16(c.k) || !aligned16(c.v) || !aligned16(c.ks) || !aligned16(c.vs))
+    return fail("%s: the cache's arrays must be 16-byte aligned", name);
+  return 0;
+}
+
+// Rows of fp32 that the kernels read and write 16 bytes at a time.
+int kv_rows(const char *name, const void *p, int *stride, long width) {
+  if (p == nullptr) return fail("%s: null pointer", name);
+  if (*stride == 0) *stride = (int)width;
+  if (*stride < width || *stride % 4 != 0 || !aligned16(p))
+    return fail("%s: rows of %ld floats need a stride of at least that and a multiple of 4, "
+                "16-byte aligned (got %d)", name, width, *stride);
+  return 0;
+}
+
+int attn_args(const char *name, const gemma_hip_cache *cache, const gemma_hip_batch *batch,
+              int n_heads, int slide, int shared, gh::KvAttn *a) {
+  if (kv_args(name, cache, batch, &a->c, &a->b)) return 1;
+  if (n_heads < 1 || n_heads > 1024 || n_heads % a->c.nkv != 0)
+    return fail("%s: %d heads over %d key/value heads", name, n_heads, a->c.nkv);
+  if (slide < 0 || shared < 0 || shared > a->b.max_len)
+    return fail("%s: bad window %d or shared prefix %d (of %d positions)", name, slide, shared,
+                a->b.max_len);
+  if ((long)a->b.max_rows * n_heads > (1l << 30))
+    return fail("%s: too many rows", name);
+  a->n_heads = n_heads;
+  a->slide = slide;
+  a->shared = shared;
+  return 0;
+}
+
+// The workspace of a call: the caller's, or the one kept for the stream.
+int call_workspace(const char *name, size_t need, void *work, size_t work_bytes, hipStream_t s,
+                   AttnHold *hold, char **out) {
+  *out = (char *)work;
+  if (need == 0) return 0;
+  if (work != nullptr) {
+    if (work_bytes < need || (uintptr_t)work % 256 != 0)
+      return fail("%s: the workspace must be 256-byte aligned and hold %zu bytes (got %zu)", name,
+                  need, work_bytes);
+    return 0;
+  }
+  if (capturing(s))
+    return fail("%s: a call that is captured needs a workspace of its own (%zu bytes)", name, need);
+  GH_CHECK(name, hold->get(need, out));
+  return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int gemma_hip_cache_write(const gemma_hip_cache *cache, const gemma_hip_batch *batch,
+                          const float *k, int k_stride, const float *v, int v_stride,
+                          void *stream) {
+  const char *name = "gemma_hip_cache_write";
+  gh::KvCache c;
+  gh::KvBatch b;
+  if (kv_args(name, cache, batch, &c, &b)) return 1;
+  const bool any = b.batch > 0 && b.max_rows > 0;
+  const long width = (long)c.nkv * c.hdim;
+  if (any && (kv_pointers(name, c, b) || kv_rows(name, k, &k_stride, width) ||
+              kv_rows(name, v, &v_stride, width)))
+    return 1;
+  if (need_device(name)) return 1;
+  if (!any) return 0;
+  PerfScope perf(kOpQuantizeAct, pick_stream(stream));
+  GH_CHECK("gemma_hip_cache_write: launch",
+           gh::launch_kv_write(c, b, k, k_stride, v, v_stride, pick_stream(stream)));
+  return 0;
+}
+
+int gemma_hip_cache_read(const gemma_hip_cache *cache, const gemma_hip_batch *batch, float *k,
+                         int k_stride, float *v, int v_stride, void *stream) {
+  const char *name = "gemma_hip_cache_read";
+  gh::KvCache c;
+  gh::KvBatch b;
+  if (kv_args(name, cache, batch, &c, &b)) return 1;
+  const bool any = b.batch > 0 && b.max_rows > 0;
+  const long width = (long)c.nkv * c.hdim;
+  if (any && (kv_pointers(name, c, b) || kv_rows(name, k, &k_stride, width) ||
+              kv_rows(name, v, &v_stride, width)))
+    return 1;
+  if (need_device(name)) return 1;
+  if (!any) return 0;
+  PerfScope perf(kOpQuantizeAct, pick_stream(stream));
+  GH_CHECK("gemma_hip_cache_read: launch",
+           gh::launch_kv_read(c, b, k, k_stride, v, v_stride, pick_stream(stream)));
+  return 0;
+}
+
+int gemma_hip_cache_attention(float *out, const float *q, int q_stride,
+                              const gemma_hip_cache *cache, const gemma_hip_batch *batch,
+                              int n_heads, int slide, float asc, float sc_att, int dense,
+                              int shared, void *work, size_t work_bytes, void *stream) {
+  const char *name = "gemma_hip_cache_attention";
+  gh::KvAttn a{};
+  if (attn_args(name, cache, batch, n_heads, slide, shared, &a)) return 1;
+  const bool any = a.b.batch > 0 && a.b.max_rows > 0;
+  if (any &&
+      (kv_pointers(name, a.c, a.b) || kv_rows(name, q, &q_stride, (long)n_heads * a.c.hdim)))
+    return 1;
+  if (any && (out == nullptr || !aligned16(out)))
+    return fail("%s: out must be there and 16-byte aligned", name);
+  if (need_device(name)) return 1;
+  if (!any) return 0;
+  a.out = out;
+  a.q = q;
+  a.q_stride = q_stride;
+  a.dense = dense != 0;
+  a.asc = asc;
+  a.cap = sc_att;
+  hipStream_t s = pick_stream(stream);
+  AttnHold hold(s);
+  if (call_workspace(name, gh::kv_attention_work(a, g.info), work, work_bytes, s, &hold, &a.work))
+    return 1;
+  {
+    PerfScope perf(kOpSoftmax, s);
+    GH_CHECK("gemma_hip_cache_attention: launch", gh::launch_kv_attention(a, g.info, s));
+  }
+  GH_CHECK("gemma_hip_cache_attention", hold.done());
+  return 0;
+}
+
+size_t gemma_hip_cache_attention_work(const gemma_hip_cache *cache, const gemma_hip_batch *batch,
+                                      int n_heads, int slide, int shared) {
+  const char *name = "gemma_hip_cache_attention_work";
+  gh::KvAttn a{};
+  if (attn_args(name, cache, batch, n_heads, slide, shared, &a) || need_init()) return (size_t)-1;
+  return gh::kv_attention_work(a, g.info);
+}
+
+}  // extern "C"
+
+namespace {
+int sample_args(const char *name, int rows, int vocab) {
+  if (rows < 0 || rows > 65535 || vocab < 1 || vocab > gh::kSampleMaxVocab)
+    return fail("%s: unsupported shape: %d rows of %d (at most 65535 of %d)", name, rows, vocab,
+                gh::kSampleMaxVocab);
+  return 0;
+}
+}  // namespace
+
+extern "C" {
+
+int gemma_hip_sample(int *tokens, float *probs, const float *logits, int stride, int rows,
+                     int vocab, const gemma_hip_sampling *settings, const float *u, void *work,
+                     size_t work_bytes, void *stream) {
+  const char *name = "gemma_hip_sample";
+  if (sample_args(name, rows, vocab)) return 1;
+  if (rows > 0 && (!tokens || !logits || !u)) return fail("%s: null pointer", name);
+  if (stride == 0) stride = vocab;
+  if (stride < vocab) return fail("%s: stride %d smaller than a row of %d", name, stride, vocab);
+  if (need_device(name)) return 1;
+  if (rows == 0) return 0;
+  gh::Sample a{tokens, probs, logits, (size_t)stride, rows, vocab, nullptr, nullptr, nullptr,
+               nullptr, u, nullptr};
+  if (settings != nullptr) {
+    a.temperature = settings->temperature;
+    a.top_k = settings->top_k;
+    a.top_p = settings->top_p;
+    a.min_p = settings->min_p;
+  }
+  hipStream_t s = pick_stream(stream);
+  AttnHold hold(s);
+  if (call_workspace(name, gh::sample_work(rows, vocab), work, work_bytes, s, &hold, &a.work))
+    return 1;
+  {
+    PerfScope perf(kOpSample, s);
+    GH_CHECK("gemma_hip_sample: launch", gh::launch_sample(a, s));
+  }
+  GH_CHECK("gemma_hip_sample", hold.done());
+  return 0;
+}
+
+size_t gemma_hip_sample_work(int rows, int vocab) {
+  if (sample_args("gemma_hip_sample_work", rows, vocab)) return (size_t)-1;
+  return gh::sample_work(rows, vocab);
+}
+
 /* ---- host drop-ins ------------------------------------------------------ */
 
 // Inputs up to this size are read by the kernels straight from pinned host

@@ -10,6 +10,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "kv_cache.h"
+
 namespace gh {
 
 constexpr int kMaxJobs = 4;  // Pick4 (gh_arith.h) selects among exactly four
@@ -395,5 +397,45 @@ hipError_t launch_vis_pool(const VisPool &a, int ntok, hipStream_t stream);
 // h [n][mlp] = gelu(h + bias) in place (the fp32-weight tower, where no
 // quantize follows); mlp % 4 == 0
 hipError_t launch_vis_bias_gelu(float *h, const float *bias, int n, int mlp, hipStream_t stream);
+
+// kv_cache.hip: the batch's new rows of k and v (head h at column h * hdim) into
+// the cache, and out of it
+hipError_t launch_kv_write(const KvCache &c, const KvBatch &b, const float *k, int k_stride,
+                           const float *v, int v_stride, hipStream_t stream);
+hipError_t launch_kv_read(const KvCache &c, const KvBatch &b, float *k, int k_stride, float *v,
+                          int v_stride, hipStream_t stream);
+
+// kv_attention.hip: attention of the batch's new rows over the cache.  q rows
+// [n_heads][hdim], q_stride apart; out [rows][n_heads * hdim]; scores q.k * asc,
+// capped by cap (0: not); positions below `shared` lie in the same pages for all
+// sequences; work: kv_attention_work() bytes.
+struct KvAttn {
+  float *out;
+  const float *q;
+  int q_stride, n_heads, slide, dense, shared;
+  float asc, cap;
+  KvCache c;
+  KvBatch b;
+  char *work;
+};
+size_t kv_attention_work(const KvAttn &a, const DeviceInfo &dev);
+hipError_t launch_kv_attention(const KvAttn &a, const DeviceInfo &dev, hipStream_t stream);
+
+// sample.hip: one token per row of logits.  Settings are device arrays of a value
+// per row, or null.
+constexpr int kSampleMaxVocab = 1 << 19;
+struct Sample {
+  int *tokens;
+  float *probs;  // or null
+  const float *logits;
+  size_t stride;
+  int rows, vocab;
+  const float *temperature;
+  const int *top_k;
+  const float *top_p, *min_p, *u;
+  char *work;
+};
+size_t sample_work(int rows, int vocab);
+hipError_t launch_sample(const Sample &a, hipStream_t stream);
 
 }  // namespace gh

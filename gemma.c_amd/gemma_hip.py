@@ -124,12 +124,34 @@ class VisionLayerF32(ctypes.Structure):
         "bq", "bk", "bv", "bo", "b1", "b2", "n1", "n1_b", "n2", "n2_b")]
 
 
+class Cache(ctypes.Structure):
+    """gemma_hip_cache: one layer's keys and values in 8-bit pages."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "ks", "vs")] + \
+               [(n, ctypes.c_int) for n in ("type", "npages", "page", "nkv", "hdim")]
+
+
+class Batch(ctypes.Structure):
+    """gemma_hip_batch: the sequences of a call and their new rows."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("pages", "len", "row0")] + \
+               [(n, ctypes.c_int) for n in ("batch", "max_pages", "rows", "max_rows", "max_len")]
+
+
+class Sampling(ctypes.Structure):
+    """gemma_hip_sampling: the settings of gemma_hip_sample, a value per row."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("temperature", "top_k", "top_p", "min_p")]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 
 # attention arithmetic of the prompt passes and the vision tower
 # (GEMMA_HIP_ATTN_*): fp32 (the default) or fp64 matrix cores (verification)
 ATTN_F64, ATTN_F32 = 0, 1
+# what a paged cache's codes are (GEMMA_HIP_CACHE_*)
+CACHE_I8, CACHE_E4M3 = 0, 1
 _SIGS = {
     "gemma_hip_init": (_I, [_I]),
     "gemma_hip_shutdown": (None, []),
@@ -148,6 +170,18 @@ _SIGS = {
     "gemma_hip_matmul_cols": (_I, [_P, _I, ctypes.POINTER(Job), _I, _P, _I, _P, _I, _I, _P]),
     "gemma_hip_prefill_attention": (_I, [_P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I,
                                          ctypes.c_float, ctypes.c_float, _I, _I, _P]),
+    "gemma_hip_cache_write": (_I, [ctypes.POINTER(Cache), ctypes.POINTER(Batch), _P, _I, _P, _I,
+                                   _P]),
+    "gemma_hip_cache_read": (_I, [ctypes.POINTER(Cache), ctypes.POINTER(Batch), _P, _I, _P, _I,
+                                  _P]),
+    "gemma_hip_cache_attention": (_I, [_P, _P, _I, ctypes.POINTER(Cache), ctypes.POINTER(Batch),
+                                       _I, _I, ctypes.c_float, ctypes.c_float, _I, _I, _P,
+                                       ctypes.c_size_t, _P]),
+    "gemma_hip_cache_attention_work": (ctypes.c_size_t, [ctypes.POINTER(Cache),
+                                                         ctypes.POINTER(Batch), _I, _I, _I]),
+    "gemma_hip_sample": (_I, [_P, _P, _P, _I, _I, _I, ctypes.POINTER(Sampling), _P, _P,
+                              ctypes.c_size_t, _P]),
+    "gemma_hip_sample_work": (ctypes.c_size_t, [_I, _I]),
     "gemma_hip_matmul_multi": (_I, [ctypes.POINTER(Job), _I, _P, _P, _I, _P]),
     "gemma_hip_quantize_matmul": (_I, [ctypes.POINTER(Job), _I, _P, _I, _P, _P, _P]),
     "gemma_hip_matmul_f32": (_I, [_P, _I, _P, _I, _P, _I, _I, _I, _I, _P]),
@@ -213,6 +247,35 @@ def _addr(x) -> int | None:
     if hasattr(x, "ctypes"):
         return x.ctypes.data
     raise TypeError(f"cannot take the address of {type(x)}")
+
+
+def _nbytes(t) -> int:
+    """Bytes of a workspace (None: the library's own)."""
+    return 0 if t is None else t.numel() * t.element_size()
+
+
+def _kept(cls, buffers, *sizes):
+    """A structure of buffers' addresses and sizes that keeps the buffers alive."""
+    s = cls(*(_addr(x) for x in buffers), *(int(n) for n in sizes))
+    s.buffers = buffers
+    return s
+
+
+def cache(k, v, ks, vs, type, npages, page, nkv, hdim) -> Cache:
+    """A paged cache over device buffers k, v [npages][nkv][page][hdim] (8-bit
+    codes) and ks, vs [npages][nkv][page]; type CACHE_I8 or CACHE_E4M3."""
+    return _kept(Cache, (k, v, ks, vs), type, npages, page, nkv, hdim)
+
+
+def batch(pages, len, row0, batch, max_pages, rows, max_rows, max_len) -> Batch:
+    """A batch over device int32 arrays pages [batch][max_pages], len [batch] and
+    row0 [batch + 1]; rows, max_rows and max_len bound what these say."""
+    return _kept(Batch, (pages, len, row0), batch, max_pages, rows, max_rows, max_len)
+
+
+def sampling(temperature=None, top_k=None, top_p=None, min_p=None) -> Sampling:
+    """Settings of GemmaHip.sample: device arrays of a value per row, or None."""
+    return _kept(Sampling, (temperature, top_k, top_p, min_p))
 
 
 class GemmaHip:
@@ -325,6 +388,47 @@ class GemmaHip:
         self._check(self.lib.gemma_hip_vision_attention(_addr(out), _addr(qkv), _addr(bias), n,
                                                         n_heads, dim, mode,
                                                         stream))
+
+    # batches of sequences over a paged 8-bit cache ----------------------------
+    def cache_write(self, cache, batch, k, k_stride, v, v_stride, stream=None):
+        """gemma_hip_cache_write: the batch's new rows of k and v into the cache."""
+        self._check(self.lib.gemma_hip_cache_write(cache, batch, _addr(k), k_stride, _addr(v),
+                                                   v_stride, stream))
+
+    def cache_read(self, cache, batch, k, k_stride, v, v_stride, stream=None):
+        """gemma_hip_cache_read: ... and the values of the batch's rows out of it."""
+        self._check(self.lib.gemma_hip_cache_read(cache, batch, _addr(k), k_stride, _addr(v),
+                                                  v_stride, stream))
+
+    def cache_attention(self, out, q, q_stride, cache, batch, n_heads, slide, asc, sc_att, dense,
+                        shared, work=None, stream=None):
+        """gemma_hip_cache_attention on device pointers; work: a tensor of
+        cache_attention_work() bytes, or None for the library's own."""
+        self._check(self.lib.gemma_hip_cache_attention(
+            _addr(out), _addr(q), q_stride, cache, batch, n_heads, slide, float(asc),
+            float(sc_att), 1 if dense else 0, shared, _addr(work), _nbytes(work), stream))
+
+    def _size(self, n: int) -> int:
+        if n == ctypes.c_size_t(-1).value:
+            self._check(1)
+        return n
+
+    def cache_attention_work(self, cache, batch, n_heads, slide, shared) -> int:
+        """Bytes of cache_attention's workspace."""
+        return self._size(self.lib.gemma_hip_cache_attention_work(cache, batch, n_heads, slide,
+                                                                  shared))
+
+    def sample(self, tokens, probs, logits, stride, rows, vocab, settings, u, work=None,
+               stream=None):
+        """gemma_hip_sample on device pointers (probs and settings nullable); work:
+        a tensor of sample_work() bytes, or None for the library's own."""
+        self._check(self.lib.gemma_hip_sample(_addr(tokens), _addr(probs), _addr(logits), stride,
+                                              rows, vocab, settings, _addr(u), _addr(work),
+                                              _nbytes(work), stream))
+
+    def sample_work(self, rows: int, vocab: int) -> int:
+        """Bytes of sample's workspace."""
+        return self._size(self.lib.gemma_hip_sample_work(rows, vocab))
 
     def register_weights(self, host, nbytes: int):
         self._check(self.lib.gemma_hip_register_weights(_addr(host), nbytes))

@@ -552,6 +552,115 @@ int gemma_hip_prefill_attention(float *out, const float *q, int q_stride, const 
 int gemma_hip_gemma_image(gemma_hip_decoder *dec, gemma_hip_vision *vis, const float *img,
                           int *pos, float *logits, int *next);
 
+/* ---- batches of sequences: 8-bit paged cache, attention over it, sampling --- */
+/* No counterpart in the reference, which runs one sequence with an fp32 cache
+ * (gemma.c:4776-4858, 5152-5293) and samples on the host (5596-5949).  These entry
+ * points take device buffers and enqueue on `stream`; none of them allocates when
+ * its workspace is given, and all of them may be captured into a graph then: what
+ * changes from step to step (lengths, page ids, rows, settings) lies in device
+ * memory. */
+
+/* The keys and values of one layer in 8 bits, in pages of `page` positions (a
+ * power of two of at least 16; a contiguous cache is one page per sequence).
+ * k, v: codes [npages][nkv][page][hdim]; ks, vs: fp32 scales [npages][nkv][page];
+ * all 16-byte aligned.  hdim is 128 or 256.  A value is code * scale, one scale
+ * per position and head:
+ *   GEMMA_HIP_CACHE_I8    int8 codes as gemma_hip_quantize makes them,
+ *   GEMMA_HIP_CACHE_E4M3  8-bit floats (4 exponent, 3 mantissa bits, largest 448):
+ *                         scale = amax (1/448), code = x (448/amax) rounded to
+ *                         nearest even.
+ * A row of zeros has scale 0.  A row with a NaN or an infinity has codes of 0 and
+ * a NaN scale: it reads back as NaN, and makes those rows NaN that see it, no
+ * others.  The e4m3 code of a NaN (0x7f, 0xff) is not for callers to write. */
+#define GEMMA_HIP_CACHE_I8 0
+#define GEMMA_HIP_CACHE_E4M3 1
+typedef struct {
+  void *k, *v;
+  float *ks, *vs;
+  int type, npages, page, nkv, hdim;
+} gemma_hip_cache;
+
+/* A batch of sequences, each with some new rows.  Device memory: pages
+ * [batch][max_pages], the ids of each sequence's pages in order; len [batch], its
+ * positions, the new rows among them; row0 [batch + 1], rising: rows row0[b] ..
+ * row0[b+1] - 1 of the call's buffers are sequence b's last positions, len[b] -
+ * (row0[b+1] - row0[b]) and up.  A sequence may have no rows, or no positions.
+ * Sizes that the host knows: `rows`, the rows of the call's buffers (at least
+ * row0[batch]; those from row0[batch] on are left as they are); max_rows and
+ * max_len, at least every sequence's rows and len (max_len <= max_pages * page).
+ * Lengths and rows are cut to these bounds, and a page id outside the cache stands
+ * for positions that aren't there: not written, read as zeros, not attended to. */
+typedef struct {
+  const int *pages, *len, *row0;
+  int batch, max_pages, rows, max_rows, max_len;
+} gemma_hip_batch;
+
+/* Quantises the batch's new rows into the cache: k and v rows of k_stride and
+ * v_stride floats (multiples of 4, 16-byte aligned; 0: dense), head h at column
+ * h * hdim, after the k norm and RoPE (gemma.c:4800-4830).  Two rows of one call
+ * must not lie at the same place of the cache. */
+int gemma_hip_cache_write(const gemma_hip_cache *cache, const gemma_hip_batch *batch,
+                          const float *k, int k_stride, const float *v, int v_stride,
+                          void *stream);
+
+/* Reads the keys and values of the batch's rows back, as the fp32 values that the
+ * codes stand for (zeros for positions that aren't there). */
+int gemma_hip_cache_read(const gemma_hip_cache *cache, const gemma_hip_batch *batch, float *k,
+                         int k_stride, float *v, int v_stride, void *stream);
+
+/* Attention of the batch's new rows over their sequences: gemma_hip_prefill_attention
+ * (gemma.c:5152-5293) for any number of sequences and for single tokens, over the
+ * cache as it stands (gemma_hip_cache_write goes before).  q [rows][q_stride] (head
+ * h at column h * hdim; 16-byte aligned, q_stride a multiple of 4, 0: dense); out
+ * [rows][n_heads * hdim], 16-byte aligned; n_heads a multiple of nkv.  The row at
+ * position p sees keys max(0, p + 1 - slide) .. p (slide 0: no window; dense != 0:
+ * every key of its sequence); scores are q.k * asc, capped as tanh(s / sc_att) *
+ * sc_att when sc_att != 0.  A row that sees nothing is zeros.
+ * shared: the first `shared` positions lie in the same pages for every sequence (a
+ * common prefix; 0: none).  Each sequence's table lists them; the first one's is
+ * read, and their keys and values are read once for all rows.
+ * work: gemma_hip_cache_attention_work() bytes of device memory for these sizes,
+ * 256-byte aligned, which one call at a time may use; NULL takes the workspace
+ * that the library keeps for the stream (not while it is being captured). */
+int gemma_hip_cache_attention(float *out, const float *q, int q_stride,
+                              const gemma_hip_cache *cache, const gemma_hip_batch *batch,
+                              int n_heads, int slide, float asc, float sc_att, int dense,
+                              int shared, void *work, size_t work_bytes, void *stream);
+
+/* Bytes of gemma_hip_cache_attention's workspace (0: none), from the sizes alone: the
+ * device tables are not read.  (size_t)-1 for arguments that call refuses. */
+size_t gemma_hip_cache_attention_work(const gemma_hip_cache *cache, const gemma_hip_batch *batch,
+                                      int n_heads, int slide, int shared);
+
+/* Settings of gemma_hip_sample: device arrays of a value per row, each nullable
+ * (temperature 1, nothing filtered).  temperature 0 (or below, or NaN) takes the
+ * largest logit, the lowest index among equals; top_k <= 0, top_p >= 1 or NaN and
+ * min_p <= 0 or NaN filter nothing. */
+typedef struct {
+  const float *temperature;
+  const int *top_k;
+  const float *top_p, *min_p;
+} gemma_hip_sampling;
+
+/* The next token of every row of logits [rows][stride] (vocab columns, vocab <=
+ * 524288; stride 0: dense) from given uniform random numbers u [rows] in [0, 1):
+ * what the reference's sample_from_logits (gemma.c:5769-5948) does after its
+ * repetition penalty, with min-p.  With w = exp((l - max l) / temperature), tokens
+ * in the order of falling logit, equals by index: kept are the first top_k, of
+ * these the fewest whose w sum to at least top_p of theirs, of these those with w
+ * >= min_p; the token is the first whose running sum exceeds u times the sum of the
+ * kept ones.  NaN logits count as -inf, which is never drawn; +inf ones take all.
+ * tokens [rows] (-1 where no logit is above -inf) and probs [rows] (nullable, the
+ * token's share of the kept sum).  Weights are 64-bit and their sums exact to 2^-44
+ * of the largest, in any order of the work: equal calls draw equal tokens.
+ * work: gemma_hip_sample_work() bytes, as above. */
+int gemma_hip_sample(int *tokens, float *probs, const float *logits, int stride, int rows,
+                     int vocab, const gemma_hip_sampling *settings, const float *u, void *work,
+                     size_t work_bytes, void *stream);
+
+/* Bytes of gemma_hip_sample's workspace ((size_t)-1 for sizes it refuses). */
+size_t gemma_hip_sample_work(int rows, int vocab);
+
 #ifdef __cplusplus
 }
 #endif
