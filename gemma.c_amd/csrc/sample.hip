@@ -1,12 +1,24 @@
 // sample.hip -- the next token of each row of logits: temperature, top-k, top-p
 // and min-p, from a given uniform random number.
 //
+// Let z = l log2(e) / temperature be a token's logit in octaves, w = 2^z its weight.
 // The kept tokens are a prefix of the row in the order of falling logit (ties by
 // rising index), and so is what each filter keeps and what lies before the token
-// drawn: every step finds the first token of that order up to which a running
-// count or a running weight reaches a target.  Weights exp((l - max l) / T) are
-// taken in fp64 and held as whole multiples of 2^-44, so that their sums are exact
-// whatever their order.
+// drawn: each step finds the first token of that order up to which a running
+// count or a running weight reaches a target.  No row is sorted for that: tokens
+// are counted, and weighed, in 256 bins of 1/8 octave below the row's largest (the
+// last bin holds all the rest), and only the bins in which a target may be reached
+// are looked into.
+//
+// Weights are fp64.  Sums inside a bin of a workgroup are of whole multiples of a
+// power of two, and so exact in any order; sums over bins and workgroups are fp64 in
+// one order.  So equal calls give equal bits.
+//
+// Up to kWholeVocab columns a workgroup does a row by itself.  Longer rows take four
+// launches: each 4096-column chunk's bins, relative to its own largest logit so
+// that one reading does (sample_bins_kernel); their sum and the bins that matter
+// (sample_decide_kernel); these bins' tokens (sample_collect_kernel; chunks that
+// hold none are not read again); and the targets inside them (sample_pick_kernel).
 #include <float.h>
 #include <limits.h>
 
@@ -18,192 +30,856 @@ namespace gh {
 namespace {
 
 typedef unsigned long long u64;
-constexpr int kThreads = 1024;
-constexpr int kMassBits = 44;  // of the largest weight; times 2^19 tokens: 63
 
-// A token's place in the order: rising.  NaN and -inf have none (kNoPlace).
-constexpr u64 kNoPlace = ~0ull;
+constexpr int kBins = 256;
+constexpr double kPerOctave = 8.0;
+constexpr int kChunk = 4096;       // columns of a workgroup of the long rows' kernels
+constexpr int kChunkThreads = 256;
+constexpr int kPer = kChunk / kChunkThreads;
+constexpr int kThreads = 1024;     // ... of the kernels that see whole rows
+constexpr int kWholeVocab = 16384;
+constexpr int kRanked = 256;       // tokens that are put in order by comparing all pairs
+constexpr int kSubs = 1024;        // parts of a bin with more
+constexpr int kList = 16384;       // tokens of a row's bins that are collected, at most
+constexpr int kUnit = 44;          // a weight's units within its bin: 2^-44 of the bin's octave
+constexpr double kInfZ = 0x1p1000;  // an infinite logit, far above any other's octaves
+
+// A token's place in the order: rising.  NaN and -inf have none.
+__device__ __forceinline__ bool has_place(float l) { return l > -INFINITY; }
 __device__ __forceinline__ u64 place(float l, int index) {
-  if (!(l > -INFINITY)) return kNoPlace;
   const uint32_t b = l == 0.0f ? 0u : __float_as_uint(l);
   const uint32_t up = b & 0x80000000u ? ~b : b | 0x80000000u;
   return (u64)~up << 32 | (uint32_t)index;
 }
+__device__ __forceinline__ float logit_at(u64 place) {
+  const uint32_t up = ~(uint32_t)(place >> 32);
+  return __uint_as_float(up & 0x80000000u ? up & 0x7fffffffu : ~up);
+}
 
-struct Found {
-  u64 at;            // the token's place
-  u64 before, mass;  // the weights before it, and its own
+__device__ __forceinline__ double octaves(float l, double c) {
+  return l == INFINITY ? kInfZ : (double)l * c;
+}
+
+// 2^x in fp64 for x <= 0 (0 below -1000): x = e + j / 128 + r, the table's 2^(j/128)
+// (exp_tab_load) and the Taylor polynomial of 2^r, |r| <= 2^-8 (truncation below
+// 2e-18).
+__device__ __forceinline__ double pow2(double x, const double *tab) {
+  x = fmax(x, -1000.0);
+  const double kf = rint(x * 128.0);
+  const double r = fma(kf, -0x1p-7, x);
+  double p = fma(r, 0x1.5d87fe78a6731p-10, 0x1.3b2ab6fba4e77p-7);  // (ln 2)^i / i!
+  p = fma(r, p, 0x1.c6b08d704a0c0p-5);
+  p = fma(r, p, 0x1.ebfbdff82c58fp-3);
+  p = fma(r, p, 0x1.62e42fefa39efp-1);
+  p = fma(r, p, 1.0);
+  const int k = (int)kf;
+  return ldexp(tab[k & 127] * p, k >> 7);
+}
+// ... rounded to a whole number of units 2^-bits, bits <= 51
+__device__ __forceinline__ u64 units(double w, int bits) {
+  const double magic = 0x1p52;
+  return (u64)(__double_as_longlong(ldexp(w, bits) + magic) - __double_as_longlong(magic));
+}
+
+// A row's settings; a temperature of 0 is top-k 1.
+struct Settings {
+  double c;  // octaves of a logit
+  int k;     // 0: all
+  double p;  // 1: all
+  double m;  // 0: all
+  double u;
 };
-
-struct Lds {
-  u64 mass[256];
-  uint32_t count[256];
-  double tab[128];
-  u64 red[kThreads / 64];
-  u64 pick[3];
-};
-
-// The first token, among those at places up to `last`, up to which the running
-// count (BY_COUNT) or weight reaches target >= 1; the last one where none does.
-// One digit of the place at a time: eight bits of the logit, then of the index.
-template <bool BY_COUNT, class W>
-__device__ Found select(const float *l, int vocab, u64 last, u64 target, W &&weight, Lds &s) {
-  const int tid = threadIdx.x, lane = tid & 63;
-  u64 prefix = 0, before = 0;
-  u64 gone = 0;  // count or weight before the prefix
-  for (int shift = 56; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += kThreads) s.mass[i] = s.count[i] = 0;
-    __syncthreads();
-    for (int i = tid; i < vocab; i += kThreads) {
-      const u64 p = place(l[i], i);
-      if (p > last || p == kNoPlace || (shift < 56 && (p >> (shift + 8)) != prefix)) continue;
-      const int d = (int)(p >> shift) & 255;
-      atomicAdd(&s.count[d], 1u);
-      atomicAdd(&s.mass[d], weight(l[i]));
-    }
-    __syncthreads();
-    if (tid < 64) {  // four digits a lane
-      u64 c[4], m[4], sum = 0, msum = 0;
-      for (int e = 0; e < 4; ++e) {
-        c[e] = BY_COUNT ? s.count[4 * lane + e] : s.mass[4 * lane + e];
-        m[e] = s.mass[4 * lane + e];
-        sum += c[e];
-        msum += m[e];
-      }
-      u64 at = sum, mat = msum;
-      for (int off = 1; off < 64; off <<= 1) {
-        const u64 t = __shfl_up(at, off, 64), mt = __shfl_up(mat, off, 64);
-        if (lane >= off) {
-          at += t;
-          mat += mt;
-        }
-      }
-      at += gone - sum;  // before this lane's digits
-      mat += before - msum;
-      // the digit in which the target is reached, or the last one that isn't empty
-      int hit = -1, some = -1;
-      u64 hg = 0, hb = 0, sg = 0, sb = 0;
-      for (int e = 0; e < 4; ++e) {
-        if (s.count[4 * lane + e] != 0) {
-          some = 4 * lane + e;
-          sg = at;
-          sb = mat;
-          if (hit < 0 && at + c[e] >= target) {
-            hit = some;
-            hg = at;
-            hb = mat;
-          }
-        }
-        at += c[e];
-        mat += m[e];
-      }
-      const u64 hits = __ballot(hit >= 0), somes = __ballot(some >= 0);
-      const int who = hits ? __ffsll(hits) - 1 : somes ? 63 - __clzll(somes) : 0;
-      if (lane == who) {
-        s.pick[0] = hits ? hit : some < 0 ? 0 : some;
-        s.pick[1] = hits ? hg : sg;
-        s.pick[2] = hits ? hb : sb;
-      }
-    }
-    __syncthreads();
-    prefix = prefix << 8 | s.pick[0];
-    gone = s.pick[1];
-    before = s.pick[2];
-    __syncthreads();
+__device__ __forceinline__ double octave_scale(const Sample &a, int row) {
+  constexpr double log2e = 0x1.71547652b82fep+0;
+  const float t = a.temperature != nullptr ? a.temperature[row] : 1.0f;
+  return t > 0.0f ? log2e / (double)t : log2e;
+}
+__device__ Settings settings(const Sample &a, int row) {
+  Settings s;
+  const float t = a.temperature != nullptr ? a.temperature[row] : 1.0f;
+  s.c = octave_scale(a, row);
+  s.k = a.top_k != nullptr ? max(a.top_k[row], 0) : 0;
+  const float p = a.top_p != nullptr ? a.top_p[row] : 1.0f;
+  s.p = p < 1.0f ? (double)p : 1.0;
+  const float m = a.min_p != nullptr ? a.min_p[row] : 0.0f;
+  s.m = m > 0.0f ? (double)m : 0.0;
+  const float u = a.u[row];
+  s.u = u > 0.0f ? fmin((double)u, 1.0) : 0.0;
+  if (!(t > 0.0f)) {
+    s.k = 1;
+    s.p = 1.0;
+    s.m = 0.0;
   }
-  const int index = (int)(uint32_t)prefix;
-  return Found{prefix, before, weight(l[index < vocab ? index : 0])};
+  return s;
 }
 
-__device__ u64 block_sum(u64 v, Lds &s) {
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) s.red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  u64 t = 0;
-  for (int w = 0; w < kThreads / 64; ++w) t += s.red[w];
-  return t;
+// Where bins lie: bin i holds 8 z in [gmax - i, gmax - i + 1), the last one all below;
+// weights are relative to 2^e.
+struct Grid {
+  double gmax, e;
+};
+__device__ __forceinline__ Grid grid_of(float most, double c) {
+  const double z = octaves(most, c);
+  return {floor(z * kPerOctave), ceil(z)};
+}
+__device__ __forceinline__ int bin_of(double z, double gmax) {
+  const double d = gmax - floor(z * kPerOctave);
+  return d >= kBins - 1 ? kBins - 1 : (int)d;
+}
+// The power of two that no weight of a bin exceeds, relative to the row's.
+__device__ __forceinline__ double bin_top(int bin, const Grid &g) {
+  return ceil((g.gmax - bin + 1.0) / kPerOctave);
 }
 
-// One workgroup per row.
-__global__ __launch_bounds__(kThreads) void sample_kernel(Sample a) {
+// A row's bins, running sums from the largest logits down, and where the tokens of
+// the bins that matter have been collected.
+struct Row {
+  Grid g;
+  double zmax;
+  u64 sum_m[kBins];  // (doubles) running weight ...
+  uint32_t sum_c[kBins];  // ... and count, each bin's own included
+  uint32_t at[kBins];     // list position of the bin's tokens, kNone: not collected
+  uint32_t fill[kBins];   // tokens of the bin in the list so far
+  uint32_t listed;        // whether the bins that matter fit the list
+  uint32_t pad;
+  __device__ double weight(int i) const { return __longlong_as_double((long long)sum_m[i]); }
+  __device__ double weight_before(int i) const { return i > 0 ? weight(i - 1) : 0.0; }
+  __device__ uint32_t count_before(int i) const { return i > 0 ? sum_c[i - 1] : 0u; }
+  __device__ uint32_t count_of(int i) const { return sum_c[i] - count_before(i); }
+};
+constexpr uint32_t kNone = ~0u;
+
+// The first bin with tokens for which f holds, the last one with tokens if none: by
+// each wave on its own.
+template <class F>
+__device__ __forceinline__ int first_bin(const Row &r, F &&f) {
+  const int lane = threadIdx.x & 63;
+  int hit = kBins, some = -1;
+#pragma unroll
+  for (int e = 3; e >= 0; --e) {
+    const int i = 4 * lane + e;
+    if (r.count_of(i) == 0) continue;
+    some = max(some, i);
+    if (f(i)) hit = i;
+  }
+  const u64 any = __ballot(hit < kBins), full = __ballot(some >= 0);
+  if (any != 0) return __shfl(hit, __ffsll(any) - 1, 64);
+  return full != 0 ? __shfl(some, 63 - __clzll(full), 64) : 0;
+}
+
+__device__ __forceinline__ int bin_by_weight(const Row &r, double target) {
+  return first_bin(r, [&](int i) { return r.weight(i) >= target; });
+}
+__device__ __forceinline__ int bin_past_weight(const Row &r, double target) {
+  return first_bin(r, [&](int i) { return r.weight(i) > target; });
+}
+__device__ __forceinline__ int bin_by_count(const Row &r, uint32_t target) {
+  return first_bin(r, [&](int i) { return r.sum_c[i] >= target; });
+}
+// Bins in which min-p's border may lie: [0], the first of them, to [1].
+__device__ __forceinline__ void min_p_bins(const Row &r, double m, int (&b)[2]) {
+  const double z = r.zmax + log2(m);
+  const double slack = 1e-9 * (1.0 + fabs(r.zmax));
+  b[0] = z + slack >= r.zmax ? 0 : bin_of(z + slack, r.g.gmax);
+  b[1] = z - slack >= r.zmax ? 0 : bin_of(z - slack, r.g.gmax);
+}
+
+// Running sums over the bins, by wave 0 (count, then weight).
+__device__ void sum_bins(const uint32_t *count, const double *mass, Row &r) {
+  const int lane = threadIdx.x;
+  if (lane >= 64) return;
+  uint32_t c[4], cs = 0;
+  double m[4], ms = 0.0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    c[e] = cs += count[4 * lane + e];
+    m[e] = ms += mass[4 * lane + e];
+  }
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const uint32_t ct = __shfl_up(cs, off, 64);
+    const double mt = __shfl_up(ms, off, 64);
+    if (lane >= off) {
+      cs += ct;
+      ms += mt;
+    }
+  }
+  const uint32_t cb = cs - c[3];
+  const double before = __shfl_up(ms, 1, 64);  // not ms less the own: sums must not fall
+  const double mb = lane > 0 ? before : 0.0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    r.sum_c[4 * lane + e] = cb + c[e];
+    r.sum_m[4 * lane + e] = (u64)__double_as_longlong(fmin(mb + m[e], ms));
+  }
+}
+
+// Marks the bins that pick() may look into, by wave 0.  A target that is a share of
+// a sum which itself depends on a border inside a bin lies between the shares of
+// that bin's ends.
+__device__ void decide(const Settings &st, Row &r) {
+  const int lane = threadIdx.x;
+  if (lane >= 64) return;
+  const uint32_t n = r.sum_c[kBins - 1];
+  bool need[4] = {};
+  auto mark = [&](int lo, int hi) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) need[e] = need[e] || (4 * lane + e >= lo && 4 * lane + e <= hi);
+  };
+  int cut_lo = kBins - 1, cut_hi = kBins - 1;
+  double s_lo = r.weight(kBins - 1), s_hi = s_lo;
+  if (st.k > 0 && (uint32_t)st.k < n) {
+    cut_lo = cut_hi = bin_by_count(r, st.k);
+    s_hi = r.weight(cut_hi);
+    s_lo = r.weight_before(cut_lo);
+    if (r.sum_c[cut_hi] == (uint32_t)st.k)
+      s_lo = s_hi;
+    else
+      mark(cut_lo, cut_hi);
+  }
+  if (st.p < 1.0) {
+    const int lo = bin_by_weight(r, st.p * s_lo), hi = bin_by_weight(r, st.p * s_hi);
+    mark(min(lo, cut_lo), min(hi, cut_hi));
+    cut_lo = min(cut_lo, lo);
+    cut_hi = min(cut_hi, hi);
+    s_lo = fmin(s_lo, r.weight_before(cut_lo));
+    s_hi = fmin(s_hi, r.weight(cut_hi));
+  }
+  if (st.m > 0.0) {
+    int b[2];
+    min_p_bins(r, st.m, b);
+    if (b[0] <= cut_hi) {
+      mark(b[0], min(b[1], cut_hi));
+      cut_lo = min(cut_lo, b[0]);
+      cut_hi = min(cut_hi, b[1]);
+      s_lo = fmin(s_lo, r.weight_before(cut_lo));
+      s_hi = fmin(s_hi, r.weight(cut_hi));
+    }
+  }
+  mark(bin_past_weight(r, st.u * s_lo), min(bin_past_weight(r, st.u * s_hi), cut_hi));
+  // list positions
+  uint32_t own[4], sum = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    own[e] = sum;
+    sum += need[e] ? r.count_of(4 * lane + e) : 0u;
+  }
+  uint32_t run = sum;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const uint32_t t = __shfl_up(run, off, 64);
+    if (lane >= off) run += t;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    r.at[4 * lane + e] = need[e] ? run - sum + own[e] : kNone;
+    r.fill[4 * lane + e] = 0;
+  }
+  if (lane == 63) r.listed = run <= kList;
+}
+
+// Working memory of pick() and of what it calls.
+struct Lds {
+  Row row;
+  double tab[128];
+  u64 mass[kSubs];
+  uint32_t count[kSubs];
+  u64 place[kRanked], sorted[kRanked];
+  double weight[kRanked];
+  double wred[kThreads / 64];
+  u64 red[3];
+  uint32_t n;
+};
+
+// A token found: how many tokens of its bin come before it, the weight of the bin up
+// to and with it, and its own.
+struct Found {
+  u64 place;
+  uint32_t before;
+  double upto, own;
+};
+
+// Calls f(place) for the tokens of a bin: from the list, or from the row itself.
+template <class F>
+__device__ __forceinline__ void each_of_bin(const Sample &a, int row, const Settings &st,
+                                            const u64 *list, const Row &r, int bin, F &&f) {
+  if (list != nullptr && r.listed && r.at[bin] != kNone) {
+    const uint32_t n = r.count_of(bin);
+    for (uint32_t i = threadIdx.x; i < n; i += kThreads) f(list[r.at[bin] + i]);
+  } else {
+    const float *l = a.logits + row * a.stride;
+    for (int i = threadIdx.x; i < a.vocab; i += kThreads) {
+      const float x = l[i];
+      if (has_place(x) && bin_of(octaves(x, st.c), r.g.gmax) == bin) f(place(x, i));
+    }
+  }
+}
+
+// The first part of an array of counts and weights (units) at which the running count
+// or weight reaches the target, or the last that isn't empty: into red[] as part,
+// count before, weight before.  By wave 0; barriers around it are the caller's.
+template <int N>
+__device__ void find_part(Lds &s, bool by_count, double target, bool strict, double unit,
+                          uint32_t count0, u64 mass0) {
+  const int lane = threadIdx.x;
+  if (lane >= 64) return;
+  constexpr int P = N / 64;
+  uint32_t c = 0;
+  u64 m = 0;
+  for (int e = 0; e < P; ++e) {
+    c += s.count[P * lane + e];
+    m += s.mass[P * lane + e];
+  }
+  uint32_t cs = c;
+  u64 ms = m;
+  for (int off = 1; off < 64; off <<= 1) {
+    const uint32_t ct = __shfl_up(cs, off, 64);
+    const u64 mt = __shfl_up(ms, off, 64);
+    if (lane >= off) {
+      cs += ct;
+      ms += mt;
+    }
+  }
+  cs += count0 - c;  // before this lane's parts
+  ms += mass0 - m;
+  int hit = -1, some = -1;
+  uint32_t hc = 0, sc = 0;
+  u64 hm = 0, sm = 0;
+  for (int e = 0; e < P; ++e) {
+    const uint32_t ce = s.count[P * lane + e];
+    const u64 me = s.mass[P * lane + e];
+    if (ce != 0) {
+      some = P * lane + e;
+      sc = cs;
+      sm = ms;
+      const double v = by_count ? (double)(cs + ce) : (double)(ms + me) * unit;
+      if (hit < 0 && (strict ? v > target : v >= target)) {
+        hit = some;
+        hc = cs;
+        hm = ms;
+      }
+    }
+    cs += ce;
+    ms += me;
+  }
+  const u64 hits = __ballot(hit >= 0), somes = __ballot(some >= 0);
+  const int who = hits ? __ffsll(hits) - 1 : somes ? 63 - __clzll(somes) : 0;
+  if (lane == who) {
+    s.red[0] = hits ? hit : some < 0 ? 0 : some;
+    s.red[1] = hits ? hc : sc;
+    s.red[2] = hits ? hm : sm;
+  }
+}
+
+// The first token of a bin up to which the bin's running count, or `base` plus its
+// running weight, reaches (strict: exceeds) the target; its last one where none
+// does.  By the whole workgroup.
+//  - Up to 256 tokens: all pairs compared.
+//  - More: counted and weighed in 1024 parts of the bin, then the part's tokens.
+//  - Where a part has more than that (equal logits): digit by digit of the place.
+__device__ Found locate(const Sample &a, int row, const Settings &st, const u64 *list, Lds &s,
+                        int bin, bool by_count, double target, bool strict, double base) {
+  const Row &r = s.row;
+  const int tid = threadIdx.x;
+  const double top = bin_top(bin, r.g);
+  const double unit = ldexp(1.0, (int)fmax(top - r.g.e, -1000.0) - kUnit);
+  if (!by_count) target -= base;
+  auto weigh = [&](u64 p) { return pow2(octaves(logit_at(p), st.c) - top, s.tab); };
+  const double edge = r.g.gmax - bin;  // 8 z of the bin's lower end
+  auto part = [&](u64 p) {
+    const double y = octaves(logit_at(p), st.c) * kPerOctave - edge;  // in [0, 1); the last: < 1
+    const double d = bin < kBins - 1 ? (1.0 - y) * kSubs : 1.0 - y;
+    return min(kSubs - 1, max(0, (int)fmin(d, 1e6)));
+  };
+  int only = -1;  // the part to look at, all if -1
+  uint32_t count0 = 0;
+  u64 mass0 = 0;
+  uint32_t n = r.count_of(bin);
+  __syncthreads();
+  if (n > kRanked) {
+    for (int i = tid; i < kSubs; i += kThreads) s.count[i] = s.mass[i] = 0;
+    __syncthreads();
+    each_of_bin(a, row, st, list, r, bin, [&](u64 p) {
+      const int i = part(p);
+      atomicAdd(&s.count[i], 1u);
+      atomicAdd(&s.mass[i], units(weigh(p), kUnit));
+    });
+    __syncthreads();
+    find_part<kSubs>(s, by_count, target, strict, unit, 0, 0);
+    __syncthreads();
+    only = (int)s.red[0];
+    count0 = (uint32_t)s.red[1];
+    mass0 = s.red[2];
+    n = s.count[only];
+  }
+  if (n > kRanked) {
+    u64 prefix = 0;
+    for (int shift = 56; shift >= 0; shift -= 8) {
+      __syncthreads();
+      for (int i = tid; i < 256; i += kThreads) s.count[i] = s.mass[i] = 0;
+      __syncthreads();
+      each_of_bin(a, row, st, list, r, bin, [&](u64 p) {
+        if (part(p) != only || (shift < 56 && (p >> (shift + 8)) != prefix)) return;
+        const int d = (int)(p >> shift) & 255;
+        atomicAdd(&s.count[d], 1u);
+        atomicAdd(&s.mass[d], units(weigh(p), kUnit));
+      });
+      __syncthreads();
+      find_part<256>(s, by_count, target, strict, unit, count0, mass0);
+      __syncthreads();
+      prefix = prefix << 8 | s.red[0];
+      count0 = (uint32_t)s.red[1];
+      mass0 = s.red[2];
+    }
+    const double w = weigh(prefix);
+    return Found{prefix, count0, base + (double)(mass0 + units(w, kUnit)) * unit,
+                 w * ldexp(unit, kUnit)};
+  }
+  // gather, rank, sum in order
+  if (tid == 0) s.n = 0;
+  __syncthreads();
+  each_of_bin(a, row, st, list, r, bin, [&](u64 p) {
+    if (only >= 0 && part(p) != only) return;
+    const uint32_t i = atomicAdd(&s.n, 1u);
+    if (i < kRanked) s.place[i] = p;
+  });
+  if (tid < kRanked) s.count[tid] = 0;
+  __syncthreads();
+  n = min(s.n, (uint32_t)kRanked);
+  {
+    constexpr int S = kThreads / kRanked;
+    const uint32_t i = tid % kRanked, q = tid / kRanked;
+    if (i < n) {
+      const u64 mine = s.place[i];
+      uint32_t rank = 0;
+      for (uint32_t e = q; e < n; e += S) rank += s.place[e] < mine;
+      atomicAdd(&s.count[i], rank);
+    }
+  }
+  __syncthreads();
+  if (tid < kRanked) s.weight[tid] = 0.0;
+  __syncthreads();
+  if (tid < (int)n) {
+    const uint32_t at = s.count[tid];
+    s.sorted[at] = s.place[tid];
+    s.weight[at] = (double)units(weigh(s.place[tid]), kUnit) * unit;
+  }
+  __syncthreads();
+  if (tid < 64) {
+    constexpr int P = kRanked / 64;
+    double w[P], sum = 0.0;
+    for (int e = 0; e < P; ++e) sum += w[e] = s.weight[P * tid + e];
+    double run = sum;
+    for (int off = 1; off < 64; off <<= 1) {
+      const double t = __shfl_up(run, off, 64);
+      if (tid >= off) run += t;
+    }
+    const double prev = __shfl_up(run, 1, 64);
+    run = (double)mass0 * unit + (tid > 0 ? prev : 0.0);
+    int hit = -1;
+    double upto = 0.0;
+    for (int e = 0; e < P; ++e) {
+      const int i = P * tid + e;
+      run += w[e];
+      if (hit >= 0 || i >= (int)n) continue;
+      const double v = by_count ? (double)(count0 + i + 1) : run;
+      if (strict ? v > target : v >= target) {
+        hit = i;
+        upto = run;
+      } else if (i == (int)n - 1) {
+        upto = run;  // the last one, for want of another
+      }
+    }
+    const u64 hits = __ballot(hit >= 0);
+    const int who = hits ? __ffsll(hits) - 1 : (int)(n - 1) / P;
+    if (tid == who) {
+      s.red[0] = hits ? hit : (int)n - 1;
+      s.wred[0] = upto;
+    }
+  }
+  __syncthreads();
+  const uint32_t at = (uint32_t)s.red[0];
+  return Found{s.sorted[at], count0 + at, base + s.wred[0], weigh(s.sorted[at]) * ldexp(unit, kUnit)};
+}
+
+// The token, from the row's bins.
+__device__ void pick(const Sample &a, int row, const Settings &st, const u64 *list, Lds &s) {
+  const Row &r = s.row;
+  const uint32_t total = r.sum_c[kBins - 1];
+  uint32_t n = total;  // what is kept: so many, weighing so much
+  double sum = r.weight(kBins - 1);
+  // sums stay between the bins' own, whatever they were rounded to
+  auto within = [&](double w, int bin) { return fmin(fmax(w, r.weight_before(bin)), r.weight(bin)); };
+  auto in_bin = [&](int bin, bool by_count, double target, bool strict) {
+    Found f = locate(a, row, st, list, s, bin, by_count, target, strict, r.weight_before(bin));
+    f.upto = within(f.upto, bin);
+    return f;
+  };
+  if (st.k > 0 && (uint32_t)st.k < n) {
+    n = st.k;
+    const int bin = bin_by_count(r, n);
+    sum = r.sum_c[bin] == n ? r.weight(bin)
+                            : in_bin(bin, true, n - r.count_before(bin), false).upto;
+  }
+  if (st.p < 1.0) {
+    const double target = st.p * sum;
+    const int bin = bin_by_weight(r, target);
+    const Found f = in_bin(bin, false, target, false);
+    const uint32_t np = r.count_before(bin) + f.before + 1;
+    if (np < n) {
+      n = np;
+      sum = f.upto;
+    }
+  }
+  if (st.m > 0.0) {
+    int b[2];
+    min_p_bins(r, st.m, b);
+    for (int bin = b[0]; bin <= b[1] && r.count_before(bin) < n; ++bin) {
+      const double top = bin_top(bin, r.g);
+      const double unit = ldexp(1.0, (int)fmax(top - r.g.e, -1000.0) - kUnit);
+      uint32_t c = 0;
+      u64 w = 0;
+      if (r.count_of(bin) != 0)
+        each_of_bin(a, row, st, list, r, bin, [&](u64 p) {
+          const double z = octaves(logit_at(p), st.c);
+          if (z < r.zmax && pow2(z - r.zmax, s.tab) < st.m) return;
+          ++c;
+          w += units(pow2(z - top, s.tab), kUnit);
+        });
+      __syncthreads();
+      if (threadIdx.x == 0) s.red[0] = s.red[1] = 0;
+      __syncthreads();
+      atomicAdd(&s.red[0], (u64)c);
+      atomicAdd(&s.red[1], w);
+      __syncthreads();
+      const uint32_t kept = (uint32_t)s.red[0];
+      const double weight = r.weight_before(bin) + (double)s.red[1] * unit;
+      __syncthreads();
+      if (kept == r.count_of(bin) && bin < b[1]) continue;
+      if (r.count_before(bin) + kept < n) {  // at least the largest logit is
+        n = r.count_before(bin) + kept;
+        sum = within(weight, bin);
+      }
+      break;
+    }
+  }
+  const double target = st.u * sum;
+  int bin = bin_past_weight(r, target);
+  const int last = bin_by_count(r, n);
+  bin = min(bin, last);
+  Found f = in_bin(bin, false, target, true);
+  if (r.count_before(bin) + f.before + 1 > n)  // by a rounding: the last one kept
+    f = in_bin(bin, true, n - r.count_before(bin), false);
+  if (threadIdx.x == 0) {
+    a.tokens[row] = (int)(uint32_t)f.place;
+    if (a.probs != nullptr) a.probs[row] = (float)(f.own / sum);
+  }
+}
+
+__device__ void pick_none(const Sample &a, int row) {
+  if (threadIdx.x == 0) {
+    a.tokens[row] = -1;
+    if (a.probs != nullptr) a.probs[row] = 0.0f;
+  }
+}
+
+// The largest of a workgroup's values (-inf: none), by waves through red[].
+template <int NT>
+__device__ float block_most(float v, float *red) {
+  v = wave_max_dpp(v);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  float m = red[0];
+#pragma unroll
+  for (int w = 1; w < NT / 64; ++w) m = fmaxf(m, red[w]);
+  return m;
+}
+
+// Counts and weighs tokens into bins; the last bin's, which most tokens of a peaked
+// row share, in registers first.
+struct Binner {
+  uint32_t *count;
+  u64 *mass;
+  uint32_t rest_c = 0;
+  u64 rest_m = 0;
+  __device__ __forceinline__ Binner(uint32_t *c, u64 *m) : count(c), mass(m) {}
+  __device__ __forceinline__ void add(float l, double c, const Grid &g, int bits,
+                                      const double *tab) {
+    if (!has_place(l)) return;
+    const double z = octaves(l, c), x = z - g.e;
+    const int i = bin_of(z, g.gmax);
+    const u64 w = x > -64.0 ? units(pow2(x, tab), bits) : 0;
+    if (i < kBins - 1) {
+      atomicAdd(&count[i], 1u);
+      atomicAdd(&mass[i], w);
+    } else {
+      ++rest_c;
+      rest_m += w;
+    }
+  }
+  __device__ __forceinline__ void finish() {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+      rest_c += __shfl_xor(rest_c, off, 64);
+      rest_m += __shfl_xor(rest_m, off, 64);
+    }
+    if ((threadIdx.x & 63) == 0 && rest_c != 0) {
+      atomicAdd(&count[kBins - 1], rest_c);
+      atomicAdd(&mass[kBins - 1], rest_m);
+    }
+  }
+};
+
+// ---- short rows: a workgroup each -----------------------------------------------
+
+__global__ __launch_bounds__(kThreads) void sample_whole_kernel(Sample a) {
   __shared__ Lds s;
+  __shared__ float red[kThreads / 64];
+  __shared__ double mass[kBins];
   const int row = blockIdx.x, tid = threadIdx.x;
   const float *l = a.logits + row * a.stride;
+  const Settings st = settings(a, row);
   exp_tab_load(s.tab);
-  const ExpConsts ec = exp_consts();
-  u64 first = kNoPlace;
-  for (int i = tid; i < a.vocab; i += kThreads) first = min(first, place(l[i], i));
-  for (int off = 32; off > 0; off >>= 1) first = min(first, (u64)__shfl_xor(first, off, 64));
-  if ((tid & 63) == 0) s.red[tid >> 6] = first;
-  __syncthreads();
-  for (int w = 0; w < kThreads / 64; ++w) first = min(first, s.red[w]);
-  if (first == kNoPlace) {
-    if (tid == 0) {
-      a.tokens[row] = -1;
-      if (a.probs != nullptr) a.probs[row] = 0.0f;
-    }
-    return;
-  }
-  const float t = a.temperature != nullptr ? a.temperature[row] : 1.0f;
-  if (!(t > 0.0f)) {
-    if (tid == 0) {
-      a.tokens[row] = (int)(uint32_t)first;
-      if (a.probs != nullptr) a.probs[row] = 1.0f;
-    }
-    return;
-  }
-  const float top = l[(uint32_t)first];
-  auto w64 = [&](float x) {  // x has a place
-    return x == top ? 1.0 : exp_tab(((double)x - (double)top) / (double)t, s.tab, ec);
-  };
-  auto weight = [&](float x) { return (u64)rint(ldexp(w64(x), kMassBits)); };
-  const float min_p = a.min_p != nullptr ? a.min_p[row] : 0.0f;
-  const int k = a.top_k != nullptr ? a.top_k[row] : 0;
-  const float top_p = a.top_p != nullptr ? a.top_p[row] : 1.0f;
-  u64 last = kNoPlace - 1;
-  auto kept = [&]() {  // the weight of what is kept
-    u64 sum = 0;
-    for (int i = tid; i < a.vocab; i += kThreads) {
-      const u64 p = place(l[i], i);
-      if (p <= last && p != kNoPlace) sum += weight(l[i]);
-    }
-    return block_sum(sum, s);
-  };
-  if (k > 0 && k < a.vocab) last = select<true>(l, a.vocab, last, k, weight, s).at;
-  if (top_p < 1.0f) {
-    const double at_least = ceil((double)top_p * (double)kept());
-    last = select<false>(l, a.vocab, last, at_least >= 1.0 ? (u64)at_least : 1, weight, s).at;
-  }
-  if (min_p > 0.0f) {  // the last one whose weight is large enough
-    u64 most = first;
-    for (int i = tid; i < a.vocab; i += kThreads) {
-      const u64 p = place(l[i], i);
-      if (p <= last && p != kNoPlace && w64(l[i]) >= (double)min_p) most = max(most, p);
-    }
-    for (int off = 32; off > 0; off >>= 1) most = max(most, (u64)__shfl_xor(most, off, 64));
-    __syncthreads();
-    if ((tid & 63) == 0) s.red[tid >> 6] = most;
-    __syncthreads();
-    for (int w = 0; w < kThreads / 64; ++w) most = max(most, s.red[w]);
-    last = most;
-  }
-  const u64 sum = kept();
-  const float u = a.u[row];
-  const double over = floor((u > 0.0f ? fmin((double)u, 1.0) : 0.0) * (double)sum);
-  const Found f = select<false>(l, a.vocab, last, (u64)over + 1, weight, s);
+  if (tid < kBins) s.count[tid] = s.mass[tid] = 0;
+  float most = -INFINITY;
+  for (int i = tid; i < a.vocab; i += kThreads) most = fmaxf(most, l[i]);
+  most = block_most<kThreads>(most, red);
+  if (!has_place(most)) return pick_none(a, row);
+  const Grid g = grid_of(most, st.c);
+  Binner bins(s.count, s.mass);
+  for (int i = tid; i < a.vocab; i += kThreads) bins.add(l[i], st.c, g, kUnit, s.tab);
+  bins.finish();
   if (tid == 0) {
-    a.tokens[row] = (int)(uint32_t)f.at;
-    if (a.probs != nullptr) a.probs[row] = (float)((double)f.mass / (double)sum);
+    s.row.g = g;
+    s.row.zmax = octaves(most, st.c);
+    s.row.listed = 0;
+  }
+  __syncthreads();
+  if (tid < kBins) mass[tid] = ldexp((double)s.mass[tid], -kUnit);
+  __syncthreads();
+  sum_bins(s.count, mass, s.row);
+  __syncthreads();
+  pick(a, row, st, nullptr, s);
+}
+
+// ---- long rows --------------------------------------------------------------------
+
+// A chunk's bins, relative to its own largest logit.
+struct Chunk {
+  Grid g;     // gmax -inf: no token
+  double zmax;
+  double pad;
+  u64 mass[kBins];
+  uint32_t count[kBins];
+};
+constexpr int kChunkUnit = 50;  // 2^-50 of the chunk's octave: 4096 of them fit 64 bits
+
+struct Work {
+  Chunk *chunks;  // [rows][nchunk]
+  Row *rows;      // [rows]
+  u64 *list;      // [rows][kList]
+};
+__host__ __device__ inline int chunks_of(int vocab) { return (vocab + kChunk - 1) / kChunk; }
+
+__device__ __forceinline__ void load_chunk(const Sample &a, int row, float (&x)[kPer]) {
+  const float *l = a.logits + row * a.stride;
+  const int base = blockIdx.x * kChunk + threadIdx.x;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) {
+    const int i = base + e * kChunkThreads;
+    x[e] = l[min(i, a.vocab - 1)];
+    x[e] = i < a.vocab ? x[e] : -INFINITY;
   }
 }
+
+__global__ __launch_bounds__(kChunkThreads) void sample_bins_kernel(Sample a, Work w) {
+  __shared__ double tab[128];
+  __shared__ uint32_t count[kBins];
+  __shared__ u64 mass[kBins];
+  __shared__ float red[kChunkThreads / 64];
+  const int row = blockIdx.y, tid = threadIdx.x;
+  float x[kPer];
+  load_chunk(a, row, x);
+  const double c = octave_scale(a, row);
+  exp_tab_load(tab);
+  count[tid] = 0;
+  mass[tid] = 0;
+  float most = -INFINITY;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) most = fmaxf(most, x[e]);
+  most = block_most<kChunkThreads>(most, red);
+  Chunk *out = w.chunks + (size_t)row * gridDim.x + blockIdx.x;
+  if (!has_place(most)) {
+    if (tid == 0) out->g.gmax = -INFINITY;
+    return;
+  }
+  const Grid g = grid_of(most, c);
+  Binner bins(count, mass);
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) bins.add(x[e], c, g, kChunkUnit, tab);
+  bins.finish();
+  __syncthreads();
+  out->count[tid] = count[tid];
+  out->mass[tid] = mass[tid];
+  if (tid == 0) {
+    out->g = g;
+    out->zmax = octaves(most, c);
+  }
+}
+
+// The chunks' bins summed into the row's.  Thread (bin, part) sums its bin over a
+// quarter of the chunks; a chunk's bins that fall into the row's last one are summed in
+// units.
+__global__ __launch_bounds__(kThreads) void sample_decide_kernel(Sample a, Work w, int nchunk) {
+  constexpr int kParts = kThreads / kBins;
+  __shared__ Row r;
+  __shared__ uint32_t count[kBins];
+  __shared__ double mass[kParts][kBins];
+  __shared__ u64 rest;
+  __shared__ double zred[kThreads / 64];
+  const int row = blockIdx.x, tid = threadIdx.x, bin = tid % kBins, part = tid / kBins;
+  const Chunk *ch = w.chunks + (size_t)row * nchunk;
+  double z = -INFINITY;
+  for (int c = tid; c < nchunk; c += kThreads)
+    if (ch[c].g.gmax > -INFINITY) z = fmax(z, ch[c].zmax);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) z = fmax(z, __shfl_xor(z, off, 64));
+  if ((tid & 63) == 0) zred[tid >> 6] = z;
+  if (tid < kBins) count[tid] = 0;
+  if (tid == 0) rest = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kThreads / 64; ++i) z = fmax(z, zred[i]);
+  Row *out = w.rows + row;
+  if (!(z > -INFINITY)) {
+    if (tid == 0) out->zmax = -INFINITY;
+    return;
+  }
+  const Grid g{floor(z * kPerOctave), ceil(z)};
+  uint32_t n = 0, rest_n = 0;
+  double m = 0.0;
+  u64 rest_m = 0;
+  for (int c = part; c < nchunk; c += kParts) {
+    const Grid cg = ch[c].g;
+    if (!(cg.gmax > -INFINITY)) continue;
+    const int shift = (int)fmin(g.gmax - cg.gmax, (double)kBins);
+    const int down = (int)fmin(g.e - cg.e, 64.0);
+    if (bin < kBins - 1 && bin >= shift) {
+      n += ch[c].count[bin - shift];
+      m += ldexp((double)ch[c].mass[bin - shift], -kChunkUnit - down);
+    }
+    if (bin + shift >= kBins - 1) {
+      rest_n += ch[c].count[bin];
+      rest_m += down < 64 ? ch[c].mass[bin] >> down : 0;
+    }
+  }
+  mass[part][bin] = m;
+  if (n != 0) atomicAdd(&count[bin], n);
+  if (rest_n != 0) {
+    atomicAdd(&count[kBins - 1], rest_n);
+    atomicAdd(&rest, rest_m);
+  }
+  __syncthreads();
+  if (tid < kBins) {
+    double sum = mass[0][tid];
+#pragma unroll
+    for (int i = 1; i < kParts; ++i) sum += mass[i][tid];
+    mass[0][tid] = tid < kBins - 1 ? sum : ldexp((double)rest, -kChunkUnit);
+  }
+  if (tid == 0) {
+    r.g = g;
+    r.zmax = z;
+  }
+  __syncthreads();
+  sum_bins(count, mass[0], r);
+  __syncthreads();
+  decide(settings(a, row), r);
+  __syncthreads();
+  for (int i = tid; i < (int)(sizeof(Row) / 8); i += kThreads) ((u64 *)out)[i] = ((u64 *)&r)[i];
+}
+
+// The tokens of the bins that matter, into the row's list: each workgroup takes room
+// for a bin's at once.
+__global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(Sample a, Work w) {
+  __shared__ uint32_t at[kBins], count[kBins];
+  const int row = blockIdx.y, tid = threadIdx.x;
+  Row *r = w.rows + row;
+  const Chunk *ch = w.chunks + (size_t)row * gridDim.x + blockIdx.x;
+  const Grid g = r->g;
+  const double cmax = ch->g.gmax;
+  if (!(r->zmax > -INFINITY) || !(cmax > -INFINITY) || !r->listed) return;
+  at[tid] = r->at[tid];
+  count[tid] = 0;
+  __syncthreads();
+  // whether the chunk has any of them
+  const int shift = (int)fmin(g.gmax - cmax, (double)kBins);
+  const bool here = ch->count[tid] != 0 && at[min(tid + shift, kBins - 1)] != kNone;
+  if (!__syncthreads_or(here)) return;
+  float x[kPer];
+  load_chunk(a, row, x);
+  const double c = octave_scale(a, row);
+  int bin[kPer];
+  uint32_t slot[kPer];
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) {
+    bin[e] = -1;
+    if (!has_place(x[e])) continue;
+    const int i = bin_of(octaves(x[e], c), g.gmax);
+    if (at[i] == kNone) continue;
+    bin[e] = i;
+    slot[e] = atomicAdd(&count[i], 1u);
+  }
+  __syncthreads();
+  if (count[tid] != 0) at[tid] += atomicAdd(&r->fill[tid], count[tid]);
+  __syncthreads();
+  u64 *list = w.list + (size_t)row * kList;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) {
+    if (bin[e] < 0) continue;
+    const uint32_t i = at[bin[e]] + slot[e];
+    if (i < kList) list[i] = place(x[e], blockIdx.x * kChunk + tid + e * kChunkThreads);
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void sample_pick_kernel(Sample a, Work w) {
+  __shared__ Lds s;
+  const int row = blockIdx.x, tid = threadIdx.x;
+  const Row *r = w.rows + row;
+  if (!(r->zmax > -INFINITY)) return pick_none(a, row);
+  exp_tab_load(s.tab);
+  for (int i = tid; i < (int)(sizeof(Row) / 8); i += kThreads)
+    ((u64 *)&s.row)[i] = ((const u64 *)r)[i];
+  __syncthreads();
+  pick(a, row, settings(a, row), w.list + (size_t)row * kList, s);
+}
+
+static_assert(sizeof(Row) % 8 == 0 && kBins == kChunkThreads, "layout");
+
+size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
 }  // namespace
 
-size_t sample_work(int, int) { return 0; }
+size_t sample_work(int rows, int vocab) {
+  if (vocab <= kWholeVocab) return 0;
+  return align256((size_t)rows * chunks_of(vocab) * sizeof(Chunk)) +
+         align256((size_t)rows * sizeof(Row)) + align256((size_t)rows * kList * 8);
+}
 
 hipError_t launch_sample(const Sample &a, hipStream_t stream) {
-  sample_kernel<<<a.rows, kThreads, 0, stream>>>(a);
+  if (a.vocab <= kWholeVocab) {
+    sample_whole_kernel<<<a.rows, kThreads, 0, stream>>>(a);
+    return hipGetLastError();
+  }
+  const int n = chunks_of(a.vocab);
+  Work w;
+  w.chunks = (Chunk *)a.work;
+  w.rows = (Row *)(a.work + align256((size_t)a.rows * n * sizeof(Chunk)));
+  w.list = (u64 *)((char *)w.rows + align256((size_t)a.rows * sizeof(Row)));
+  const dim3 grid(n, a.rows);
+  sample_bins_kernel<<<grid, kChunkThreads, 0, stream>>>(a, w);
+  sample_decide_kernel<<<a.rows, kThreads, 0, stream>>>(a, w, n);
+  sample_collect_kernel<<<grid, kChunkThreads, 0, stream>>>(a, w);
+  sample_pick_kernel<<<a.rows, kThreads, 0, stream>>>(a, w);
   return hipGetLastError();
 }
 
