@@ -30,6 +30,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "gh_arith.h"
 #include "gh_kernels.h"
@@ -49,6 +50,7 @@ constexpr float kLog2e = 1.44269502162933349609375f;
 // workspace by it, and in the kernels.
 struct KvPlan {
   int group;                    // heads per kv head
+  uint32_t inv_group;           // 2^21 / group, rounded up
   int step, step_ns, step_tpc;  // single tokens: on or off, key chunks, tiles of a chunk
   int step_rows;                // query vectors of a sequence and kv head, at most
   int rows_ns, rows_tpc;        // prompt rows (0 chunks: off)
@@ -99,33 +101,41 @@ __device__ __forceinline__ h8 codes8(uint32_t a, uint32_t b) {
     return join(from_e4m3<false>(a), from_e4m3<true>(a), from_e4m3<false>(b), from_e4m3<true>(b));
   }
 }
-// x: a dword (four dims) of each of eight keys; f[i]: dim i of the eight keys
-template <int TYPE>
-__device__ __forceinline__ void codes_t(const uint32_t (&x)[8], h8 (&f)[4]) {
+// A dword (four dims) of each of eight keys, transposed: dim(i) is dim i of the eight
+// keys.  Two keys at a time.
+struct Transposed {
   h2 p[4][4];  // [dim][pair of keys]
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    uint32_t a = x[2 * j], b = x[2 * j + 1];
-    if (TYPE == kKvI8) {
-      a = flip(a);
-      b = flip(b);
-    }
-    const uint32_t lo = __builtin_amdgcn_perm(b, a, 0x05010400u);  // a0 b0 a1 b1
-    const uint32_t hi = __builtin_amdgcn_perm(b, a, 0x07030602u);  // a2 b2 a3 b3
-    if constexpr (TYPE == kKvI8) {
-      p[0][j] = magic<0x04010400u>(lo);
-      p[1][j] = magic<0x04030402u>(lo);
-      p[2][j] = magic<0x04010400u>(hi);
-      p[3][j] = magic<0x04030402u>(hi);
-    } else {
-      p[0][j] = from_e4m3<false>(lo);
-      p[1][j] = from_e4m3<true>(lo);
-      p[2][j] = from_e4m3<false>(hi);
-      p[3][j] = from_e4m3<true>(hi);
-    }
+  __device__ __forceinline__ h8 dim(int i) const { return join(p[i][0], p[i][1], p[i][2], p[i][3]); }
+};
+template <int TYPE, int J>
+__device__ __forceinline__ void transpose_pair(const uint32_t (&x)[8], Transposed &t) {
+  uint32_t a = x[2 * J], b = x[2 * J + 1];
+  if (TYPE == kKvI8) {
+    a = flip(a);
+    b = flip(b);
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) f[i] = join(p[i][0], p[i][1], p[i][2], p[i][3]);
+  const uint32_t lo = __builtin_amdgcn_perm(b, a, 0x05010400u);  // a0 b0 a1 b1
+  const uint32_t hi = __builtin_amdgcn_perm(b, a, 0x07030602u);  // a2 b2 a3 b3
+  if constexpr (TYPE == kKvI8) {
+    t.p[0][J] = magic<0x04010400u>(lo);
+    t.p[1][J] = magic<0x04030402u>(lo);
+    t.p[2][J] = magic<0x04010400u>(hi);
+    t.p[3][J] = magic<0x04030402u>(hi);
+  } else {
+    t.p[0][J] = from_e4m3<false>(lo);
+    t.p[1][J] = from_e4m3<true>(lo);
+    t.p[2][J] = from_e4m3<false>(hi);
+    t.p[3][J] = from_e4m3<true>(hi);
+  }
+}
+
+// f(0) .. f(N - 1), the numbers as constants.
+template <int N, int I = 0, class F>
+__device__ __forceinline__ void each(F &&f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    each<N, I + 1>(f);
+  }
 }
 
 __device__ __forceinline__ v4f mma(h8 a, h8 b, v4f c) {
@@ -138,9 +148,13 @@ struct KvSee {
 };
 
 // The scales of a lane's eight keys of a tile: keys 16 u + 4 g + i.
+typedef float v8f __attribute__((ext_vector_type(8)));
 struct Scales {
-  v4f k[2], v[2];
+  v8f k, v;
 };
+__device__ __forceinline__ v8f eight(v4f a, v4f b) {
+  return v8f{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+}
 
 // The running softmax of a query: M, and the sum of the weights of the keys that
 // the lane has.
@@ -148,46 +162,47 @@ struct Soft {
   float m, l;
 };
 
-// A query of HD dims in operand order (dims 64 j + 16 g + 8 h .. + 7 are piece
-// number 2 j + h), in two f16 pieces; the exponent it was scaled by comes back.
+// A query of HD dims in operand order (dims 64 j + 16 g + 8 h .. + 7 are step 2 j + h).
 template <int HD>
-__device__ __forceinline__ int load_q(const float *row, int g, h8 (&hi)[HD / 32],
-                                      h8 (&lo)[HD / 32]) {
-  float x[HD / 32][8], amax = 0.0f;
+struct Query {
+  v4f x[HD / 16];
+  __device__ __forceinline__ void load(const float *row, int g) {
 #pragma unroll
-  for (int s = 0; s < HD / 32; ++s)
+    for (int e = 0; e < HD / 16; ++e)
+      x[e] = *reinterpret_cast<const v4f *>(row + 64 * (e / 4) + 16 * g + 4 * (e % 4));
+  }
+  // in two f16 pieces; the exponent that it was scaled by comes back
+  __device__ __forceinline__ int split(h8 (&hi)[HD / 32], h8 (&lo)[HD / 32]) const {
+    float amax = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 8; e += 4) {
-      const v4f t =
-          *reinterpret_cast<const v4f *>(row + 64 * (s / 2) + 16 * g + 8 * (s % 2) + e);
+    for (int e = 0; e < HD / 16; ++e)
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        x[s][e + u] = t[u];
-        amax = fmaxf(amax, finite_abs(t[u]));
+      for (int u = 0; u < 4; ++u) amax = fmaxf(amax, finite_abs(x[e][u]));
+    amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
+    amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
+    const int eq = amax > 0.0f ? max(ilogbf(amax) - 14, -126) : 0;
+    const float down = ldexpf(1.0f, -eq);
+#pragma unroll
+    for (int s = 0; s < HD / 32; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const float a = x[2 * s + e / 4][e % 4] * down, b = x[2 * s + e / 4][e % 4 + 1] * down;
+        const h2 p = cvt_pk_f16(a, b);
+        const h2 r = cvt_pk_f16(a - (float)p[0], b - (float)p[1]);
+        hi[s][e] = p[0];
+        hi[s][e + 1] = p[1];
+        lo[s][e] = r[0];
+        lo[s][e + 1] = r[1];
       }
-    }
-  amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
-  amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
-  const int eq = amax > 0.0f ? ilogbf(amax) - 14 : 0;
-#pragma unroll
-  for (int s = 0; s < HD / 32; ++s)
-#pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-      const float a = ldexpf(x[s][e], -eq), b = ldexpf(x[s][e + 1], -eq);
-      const h2 p = cvt_pk_f16(a, b);
-      const h2 r = cvt_pk_f16(a - (float)p[0], b - (float)p[1]);
-      hi[s][e] = p[0];
-      hi[s][e + 1] = p[1];
-      lo[s][e] = r[0];
-      lo[s][e + 1] = r[1];
-    }
-  return eq;
-}
+    return eq;
+  }
+};
 
 // A query's score scale: raw dot products times c times a key's scale are octaves;
 // with a cap, z times the key's scale goes through the tanh.
 struct Score {
   float c, z, cap;
+  Score() = default;
   __device__ __forceinline__ Score(float asc, float sc_att, int eq) {
     z = ldexpf(asc, eq) / (sc_att != 0.0f ? sc_att : 1.0f);
     c = ldexpf(asc * kLog2e, eq);
@@ -195,68 +210,68 @@ struct Score {
   }
 };
 
-// Scores of a tile to weights.  d: raw dot products; p: the weights' pieces.
-// live: bit 4 u + i is set where the key is seen (used when some isn't).
-template <bool CAP, class F>
-__device__ __forceinline__ void weights(const v4f (&d)[2], const Scales &sc, const Score &q,
-                                        bool masked, unsigned live, Soft &s, h8 &phi, h8 &plo,
-                                        F &&rescale) {
-  float x[8], a[8], vs[8];
-  float top = -INFINITY;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float ks = sc.k[e / 4][e % 4];
-    vs[e] = sc.v[e / 4][e % 4];
-    if constexpr (CAP) {
-      x[e] = tanh32(d[e / 4][e % 4] * (q.z * ks));
-      a[e] = q.cap;
-    } else {
-      x[e] = d[e / 4][e % 4];
-      a[e] = q.c * ks;
-    }
-  }
-  float t[8];
+// Octaves that the values of a lane's eight keys may add to a weight.
+__device__ __forceinline__ void scale_octaves(const v8f &vs, float (&lv)[8]) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const int ev = (int)(__float_as_uint(vs[e]) >> 23 & 255) - 127;
-    t[e] = fmaf(x[e], a[e], fmaxf((float)ev, kLeastVs));
+    lv[e] = fmaxf((float)ev, kLeastVs);
   }
+}
+
+// A raw dot product to a score in octaves.
+template <bool CAP>
+__device__ __forceinline__ float score_of(float x, float ks, const Score &q) {
+  return CAP ? tanh32(x * (q.z * ks)) * q.cap : x * (q.c * ks);
+}
+// The scores of keys that aren't seen (live: a bit per key) become -inf; the largest
+// s + log2 vs of the lane's keys comes back.
+__device__ __forceinline__ float top_of(v4f (&d)[2], const float (&lv)[8], bool masked,
+                                        unsigned live) {
   if (masked) {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (!(live >> e & 1)) {
-        t[e] = -INFINITY;
-        x[e] = -INFINITY;
-        a[e] = 1.0f;
-        vs[e] = 0.0f;
-      }
+      if (!(live >> e & 1)) d[e / 4][e % 4] = -INFINITY;
   }
+  float top = -INFINITY;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) top = fmaxf(top, t[e]);
-  if (__any(top > s.m + kSlack)) {
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    const float m = top > s.m + kSlack ? ceilf(top) - kSet : s.m;
-    const float f = __builtin_amdgcn_exp2f(s.m - m);
-    s.m = m;
-    s.l *= f;
-    rescale(f);
-  }
-  float sum = 0.0f;
-#pragma unroll
-  for (int e = 0; e < 8; e += 2) {
-    const float p0 = __builtin_amdgcn_exp2f(fmaf(x[e], a[e], -s.m));
-    const float p1 = __builtin_amdgcn_exp2f(fmaf(x[e + 1], a[e + 1], -s.m));
-    sum += p0 + p1;
-    const float w0 = p0 * vs[e], w1 = p1 * vs[e + 1];
-    const h2 h = cvt_pk_f16(w0, w1);
-    const h2 r = cvt_pk_f16(w0 - (float)h[0], w1 - (float)h[1]);
-    phi[e] = h[0];
-    phi[e + 1] = h[1];
-    plo[e] = r[0];
-    plo[e + 1] = r[1];
-  }
-  s.l += sum;
+  for (int e = 0; e < 8; ++e) top = fmaxf(top, d[e / 4][e % 4] + lv[e]);
+  return top;
+}
+
+// Moves a query's M where the tile's largest weight needs it.
+template <class F>
+__device__ __forceinline__ void settle(float top, Soft &s, F &&rescale) {
+  if (!__any(top > s.m + kSlack)) return;
+  top = fmaxf(top, __shfl_xor(top, 16, 64));
+  top = fmaxf(top, __shfl_xor(top, 32, 64));
+  const float m = top > s.m + kSlack ? ceilf(top) - kSet : s.m;
+  const float f = __builtin_amdgcn_exp2f(s.m - m);
+  s.m = m;
+  s.l *= f;
+  rescale(f);
+}
+
+// a b, 0 where a is 0, whatever b (v_mul_legacy_f32; as the compiler's own
+// instruction, so that it keeps its distance from the exponential before it).
+__device__ float mul_legacy(float a, float b) __asm("llvm.amdgcn.fmul.legacy");
+
+// Scores 2 j and 2 j + 1 to weights' pieces.  The product by a value's scale is 0 for
+// a weight of 0, whatever the scale.
+__device__ __forceinline__ void weigh(int j, const v4f (&x)[2], const v8f &vs, Soft &s, h8 &phi,
+                                      h8 &plo) {
+  const int e = 2 * j;
+  const float p0 = __builtin_amdgcn_exp2f(x[e / 4][e % 4] - s.m);
+  const float p1 = __builtin_amdgcn_exp2f(x[e / 4][e % 4 + 1] - s.m);
+  s.l += p0 + p1;
+  const float w0 = mul_legacy(p0, vs[e]);
+  const float w1 = mul_legacy(p1, vs[e + 1]);
+  const h2 h = cvt_pk_f16(w0, w1);
+  const h2 r = cvt_pk_f16(w0 - (float)h[0], w1 - (float)h[1]);
+  phi[e] = h[0];
+  phi[e + 1] = h[1];
+  plo[e] = r[0];
+  plo[e + 1] = r[1];
 }
 
 // Which of a lane's eight keys of the tile at key0 are seen.
@@ -270,20 +285,79 @@ __device__ __forceinline__ unsigned seen(int key0, int g, KvSee see, bool ok0, b
   return live;
 }
 
-// Where the two halves of the tile at key0 lie (wave-uniform): pages hold whole
-// halves.  A half that isn't there (past the end, or on a bad page) reads page 0.
-struct Half {
-  size_t slot;
-  bool ok;
+// Where the halves (16 keys) of a tile lie, wave-uniform: pages hold whole halves.  One
+// that isn't there (past the end, or on a bad page) reads page 0.
+struct Halves {
+  size_t slot0, slot1;
+  bool ok0, ok1;
 };
-__device__ __forceinline__ Half half_at(const KvCache &c, const int *pages, int width, int key,
-                                        int len, int hk) {
-  const int id = pages[min(key >> c.shift, width - 1)];
-  Half h;
-  h.ok = key < len && (unsigned)id < (unsigned)c.npages;
-  const int page = h.ok ? id : 0;
-  h.slot = (((size_t)page * c.nkv + hk) << c.shift) + (key & ((1 << c.shift) - 1));
-  return h;
+
+// The halves of a wave's tiles first, first + step, ... in turn.  Page ids come 64 at a
+// time, one a lane, the next ones ahead of their use, and by vector loads: waits for
+// a scalar load would be waits for all of the wave's LDS reads as well.
+struct Pager {
+  const int *pages;
+  int width, shift, npages, nkv, hk, len, first, step;
+  int ids, next;
+  __device__ __forceinline__ Pager(const KvAttn &a, int seq, int length, int head, int t0, int dt)
+      : pages(a.b.pages + (size_t)seq * a.b.width), width(a.b.width), shift(a.c.shift),
+        npages(a.c.npages), nkv(a.c.nkv), hk(head), len(length), first(t0), step(dt) {
+    ids = load(0);
+    next = load(32);
+  }
+  __device__ __forceinline__ int load(int from) const {
+    const int lane = threadIdx.x & 63, key = kTile * (first + step * (from + lane / 2)) + 16 * (lane & 1);
+    return pages[min(key >> shift, width - 1)];
+  }
+  __device__ __forceinline__ size_t slot(int id, int key, bool *ok) const {
+    *ok = key < len && (unsigned)id < (unsigned)npages;
+    return (((size_t)(*ok ? id : 0) * nkv + hk) << shift) + (key & ((1 << shift) - 1));
+  }
+  // the j-th tile's halves; j counts up from 0
+  __device__ __forceinline__ Halves get(int j) {
+    if ((j & 31) == 0 && j > 0) {
+      ids = next;
+      next = load(j + 32);
+    }
+    const int key = kTile * (first + step * j);
+    Halves h;
+    h.slot0 = slot(__builtin_amdgcn_readlane(ids, 2 * (j & 31)), key, &h.ok0);
+    h.slot1 = slot(__builtin_amdgcn_readlane(ids, 2 * (j & 31) + 1), key + 16, &h.ok1);
+    return h;
+  }
+};
+
+// The lane's value at a wave-uniform address and an offset of its own, in bytes.
+template <class T, class P>
+__device__ __forceinline__ T at_offset(const P *base, uint32_t off) {
+  return *reinterpret_cast<const T *>(reinterpret_cast<const char *>(base) + off);
+}
+
+// One load from memory straight to LDS: each lane's 16 bytes at base + off land at lds +
+// 16 lane (base and lds wave-uniform).  The compiler doesn't see it: who reads it waits
+// first (dma_wait).  m0 has no other user in the kernel that calls this.
+__device__ __forceinline__ void dma16(const void *base, uint32_t off, const void *lds) {
+  const uint32_t m = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char *)lds;
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m), "v"(off),
+               "s"(base)
+               : "memory", "m0");
+#pragma clang diagnostic pop
+}
+// ... from an address of each lane's own
+__device__ __forceinline__ void dma16_at(const void *src, const void *lds) {
+  const uint32_t m = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char *)lds;
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(m), "v"(src)
+               : "memory", "m0");
+#pragma clang diagnostic pop
+}
+// Waits until at most N of the wave's loads, the newest, are under way.
+template <int N>
+__device__ __forceinline__ void dma_wait() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
 __device__ __forceinline__ int wave_max_all(int v) {
@@ -336,8 +410,9 @@ __global__ __launch_bounds__(64 * kStepWaves, 2) void kv_step_kernel(KvAttn a, K
   const KvSee see{max(span.lo, a.shared), span.hi};
   const int f_lo = wave_max_all(see.lo), f_hi = -wave_max_all(-see.hi);
   h8 qhi[KS], qlo[KS];
-  const int eq = load_q<HD>(a.q + (size_t)row * a.q_stride + head * HD, g, qhi, qlo);
-  const Score score(a.asc, a.cap, eq);
+  Query<HD> raw;
+  raw.load(a.q + (size_t)row * a.q_stride + head * HD, g);
+  const Score score(a.asc, a.cap, raw.split(qhi, qlo));
 
   v4f o[ND];
 #pragma unroll
@@ -345,43 +420,37 @@ __global__ __launch_bounds__(64 * kStepWaves, 2) void kv_step_kernel(KvAttn a, K
   Soft soft{kFloor, 0.0f};
 
   typedef uint32_t vreg __attribute__((ext_vector_type(VW)));
-  const int *pages = a.b.pages + (size_t)b * a.b.width;
+  const uint32_t koff = n * HD + 16 * g, voff = 4 * g * HD + (HD / 16) * n, soff = 16 * g;
   u4 kreg[2][NJ];
   vreg vval[2][4];
   Scales sc;
-  auto halves = [&](int t, Half (&h)[2]) {
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-      h[u] = half_at(a.c, pages, a.b.width, kTile * t + 16 * u, s.len, hk);
-  };
-  auto load_k = [&](const Half (&h)[2]) {
+  auto load_k = [&](const Halves &h) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const uint8_t *p = a.c.k + (h[u].slot + n) * HD + 16 * g;
 #pragma unroll
-      for (int i = 0; i < NJ; ++i) kreg[u][i] = *reinterpret_cast<const u4 *>(p + 64 * i);
-      sc.k[u] = *reinterpret_cast<const v4f *>(a.c.ks + h[u].slot + 4 * g);
+      for (int i = 0; i < NJ; ++i)
+        kreg[u][i] = at_offset<u4>(a.c.k + (u ? h.slot1 : h.slot0) * HD + 64 * i, koff);
     }
+    sc.k = eight(at_offset<v4f>(a.c.ks + h.slot0, soff), at_offset<v4f>(a.c.ks + h.slot1, soff));
   };
-  auto load_v = [&](const Half (&h)[2]) {
+  auto load_v = [&](const Halves &h) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const uint8_t *p = a.c.v + (h[u].slot + 4 * g) * HD + (HD / 16) * n;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) vval[u][i] = *reinterpret_cast<const vreg *>(p + HD * i);
-      sc.v[u] = *reinterpret_cast<const v4f *>(a.c.vs + h[u].slot + 4 * g);
+      for (int i = 0; i < 4; ++i)
+        vval[u][i] = at_offset<vreg>(a.c.v + ((u ? h.slot1 : h.slot0) + i) * HD, voff);
     }
+    sc.v = eight(at_offset<v4f>(a.c.vs + h.slot0, soff), at_offset<v4f>(a.c.vs + h.slot1, soff));
   };
 
   int t = t0 + wave;
   if (t < t1) {
-    Half cur[2], nxt[2];
-    halves(t, cur);
+    Pager pager(a, b, s.len, hk, t, kStepWaves);
+    Halves cur = pager.get(0);
     load_k(cur);
     load_v(cur);
-    for (; t < t1; t += kStepWaves) {
-      const int tn = min(t + kStepWaves, t1 - 1);  // past the last: loaded, not used
-      halves(tn, nxt);
+    for (int k = 1; t < t1; t += kStepWaves, ++k) {
+      const Halves nxt = pager.get(k);  // past the last: of this sequence or page 0, loaded and not used
       v4f dh[2] = {}, dl[2] = {};
 #pragma unroll
       for (int i = 0; i < KS; ++i)
@@ -392,46 +461,52 @@ __global__ __launch_bounds__(64 * kStepWaves, 2) void kv_step_kernel(KvAttn a, K
           dl[u] = mma(f, qlo[i], dl[u]);
           dh[u] = mma(f, qhi[i], dh[u]);
         }
-      const v4f d[2] = {dh[0] + dl[0], dh[1] + dl[1]};
-      Scales now = sc;
+      v4f d[2] = {dh[0] + dl[0], dh[1] + dl[1]};
+      const Scales now = sc;
       __builtin_amdgcn_sched_barrier(0);
       load_k(nxt);
       __builtin_amdgcn_sched_barrier(0);
       const int key0 = kTile * t;
       const bool masked =
-          key0 < f_lo || key0 + kTile - 1 > f_hi || !cur[0].ok || !cur[1].ok;  // wave-uniform
+          key0 < f_lo || key0 + kTile - 1 > f_hi || !cur.ok0 || !cur.ok1;  // wave-uniform
       unsigned live = 0xff;
       if (masked) {
-        live = seen(key0, g, see, cur[0].ok, cur[1].ok);
+        live = seen(key0, g, see, cur.ok0, cur.ok1);
         // what lies past a sequence's end may be a NaN's code, times a weight of 0
         if (TYPE == kKvE4m3)
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            if (key0 + 16 * (e / 4) + 4 * g + e % 4 >= s.len || !cur[e / 4].ok)
+            if (key0 + 16 * (e / 4) + 4 * g + e % 4 >= s.len ||
+                !(e < 4 ? cur.ok0 : cur.ok1))
               vval[e / 4][e % 4] = vreg(0u);
       }
-      h8 phi, plo;
-      weights<CAP>(d, now, score, masked, live, soft, phi, plo, [&](float f) {
+      float lv[8];
+      scale_octaves(now.v, lv);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        d[e / 4][e % 4] = score_of<CAP>(d[e / 4][e % 4], now.k[e], score);
+      settle(top_of(d, lv, masked, live), soft, [&](float f) {
 #pragma unroll
         for (int i = 0; i < ND; ++i) o[i] *= f;
       });
+      h8 phi, plo;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) weigh(j, d, now.v, soft, phi, plo);
 #pragma unroll
       for (int w = 0; w < VW; ++w) {
         uint32_t x[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = vval[e / 4][e % 4][w];
-        h8 f[4];
-        codes_t<TYPE>(x, f);
+        Transposed v;
+        each<4>([&](auto J) { transpose_pair<TYPE, J>(x, v); });
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          o[4 * w + i] = mma(f[i], plo, o[4 * w + i]);
-          o[4 * w + i] = mma(f[i], phi, o[4 * w + i]);
-        }
+        for (int i = 0; i < 4; ++i) o[4 * w + i] = mma(v.dim(i), plo, o[4 * w + i]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[4 * w + i] = mma(v.dim(i), phi, o[4 * w + i]);
       }
       __builtin_amdgcn_sched_barrier(0);
       load_v(nxt);
-      cur[0] = nxt[0];
-      cur[1] = nxt[1];
+      cur = nxt;
     }
   }
 
@@ -484,15 +559,23 @@ __global__ __launch_bounds__(64 * kStepWaves, 2) void kv_step_kernel(KvAttn a, K
 // A workgroup takes 64 QB query vectors of a kv head, 16 QB a wave, and a chunk of
 // their keys; PRE: the rows of all sequences, over the shared prefix.  Each tile's
 // codes are made f16 once, a share by each wave, and reach the others through LDS in
-// operand order.
+// operand order (16-byte reads of 64 lanes in a row: no conflicts).
+//
+// Tiles are pipelined so that the vector unit works while the matrix cores do: the
+// scores of tile t + 1 run with the weights of tile t, the value products of tile t with
+// the conversion of K of tile t + 2 and of V of tile t + 1, whose codes were loaded an
+// iteration before.  One barrier a tile; K and V each have two buffers.
 
 template <int HD, int TYPE, bool CAP, int QB, bool PRE>
 __global__ __launch_bounds__(256) void kv_rows_kernel(KvAttn a, KvPlan pl) {
   constexpr int KS = HD / 32, ND = HD / 16;
-  constexpr int TR = 64 * QB;
-  __shared__ h8 kf[2 * KS][64], vf[ND][64];
+  constexpr int TR = 64 * QB, VP = 4;  // VP: value fragments read ahead
+  __shared__ h8 kf[2][2 * KS][64], vf[2][ND][64];
+  __shared__ v4f scales[4][4][16];
+  __shared__ u4 raw_k[4][3][HD / 128][64], raw_v[4][3][2][64];
   const int ns = PRE ? pl.pre_ns : pl.rows_ns, tpc = PRE ? pl.pre_tpc : pl.rows_tpc;
-  const int chunk = blockIdx.x % ns, tile = blockIdx.x / ns, hk = blockIdx.y;
+  // the last rows, which see most, first
+  const int chunk = blockIdx.x % ns, tile = gridDim.x / ns - 1 - blockIdx.x / ns, hk = blockIdx.y;
   const int b = PRE ? 0 : blockIdx.z;
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -508,44 +591,56 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(KvAttn a, KvPlan pl) {
   const int rows = s.n * pl.group, at = tile * TR;
   if (at >= rows) return;
 
-  // the lane's queries
+  // the rows' sequences are looked up in LDS, where the table fits: a search in memory is
+  // as many round trips as it has steps
+  constexpr int kFind = (int)(sizeof(kf) / 4);
+  int *const row0 = reinterpret_cast<int *>(&kf[0][0][0]);
+  if (PRE && a.b.batch < kFind) {
+    for (int i = threadIdx.x; i <= a.b.batch; i += 256) row0[i] = a.b.row0[i];
+    __syncthreads();
+  }
+
+  // the lane's queries: loads first
   KvSee see[QB];
   int qrow[QB], qhead[QB];
-  h8 qhi[QB][KS], qlo[QB][KS];
-  float cq[QB], zq[QB];
-  int f_lo = 0, f_hi = INT_MAX, any_lo = INT_MAX, any_hi = -1;
+  Query<HD> raw[QB];
+  const int base_row = at / pl.group, base_head = at % pl.group;
 #pragma unroll
   for (int q = 0; q < QB; ++q) {
-    const int j = at + 16 * (QB * wave + q) + n;
-    const int jj = min(j, rows - 1);
-    qrow[q] = s.r0 + jj / pl.group;
-    qhead[q] = hk * pl.group + jj % pl.group;
-    KvSpan span{0, -1};
+    const int j = base_head + min(16 * (QB * wave + q) + n, rows - 1 - at);
+    const int i = (int)((uint32_t)j * pl.inv_group >> 21);  // j / group: j is below group + 128
+    qrow[q] = s.r0 + base_row + i;
+    qhead[q] = hk * pl.group + j - i * pl.group;
+    raw[q].load(a.q + (size_t)qrow[q] * a.q_stride + qhead[q] * HD, g);
+  }
+  int f_lo = 0, f_hi = INT_MAX;
+#pragma unroll
+  for (int q = 0; q < QB; ++q) {
     if (PRE) {
-      const int i = kv_find(a.b.row0, a.b.batch, qrow[q]);
+      KvSpan span{0, -1};
+      const int i = a.b.batch < kFind ? kv_find(row0, a.b.batch, qrow[q])
+                                      : kv_find(a.b.row0, a.b.batch, qrow[q]);
       if (i >= 0) {
         const KvSeq o = kv_seq(a.b, i);
         span = kv_span(o.len - o.n + (qrow[q] - o.r0), o.len, a.slide, a.dense);
       }
       see[q] = {span.lo, min(span.hi, a.shared - 1)};
     } else {
-      span = kv_span(s.len - s.n + jj / pl.group, s.len, a.slide, a.dense);
+      const KvSpan span = kv_span(s.len - s.n + qrow[q] - s.r0, s.len, a.slide, a.dense);
       see[q] = {max(span.lo, a.shared), span.hi};
-    }
-    if (see[q].hi >= see[q].lo) {
-      any_lo = min(any_lo, see[q].lo);
-      any_hi = max(any_hi, see[q].hi);
     }
     f_lo = max(f_lo, see[q].lo);
     f_hi = min(f_hi, see[q].hi);
-    const int eq = load_q<HD>(a.q + (size_t)qrow[q] * a.q_stride + qhead[q] * HD, g, qhi[q],
-                              qlo[q]);
-    const Score sc(a.asc, a.cap, eq);
-    cq[q] = sc.c;
-    zq[q] = sc.z;
   }
+  h8 qhi[QB][KS], qlo[QB][KS];
+  Score score[QB];
+  auto split_queries = [&]() {
+#pragma unroll
+    for (int q = 0; q < QB; ++q) score[q] = Score(a.asc, a.cap, raw[q].split(qhi[q], qlo[q]));
+  };
   f_lo = wave_max_all(f_lo);
   f_hi = -wave_max_all(-f_hi);
+  if (PRE) __syncthreads();  // the search is over, its table goes
   int t0, t1;
   if (PRE) {  // chunks of the whole prefix
     t0 = chunk * tpc;
@@ -567,70 +662,230 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(KvAttn a, KvPlan pl) {
 #pragma unroll
     for (int i = 0; i < ND; ++i) o[q][i] = v4f{};
   }
-  const int *pages = a.b.pages + (size_t)b * a.b.width;
-  for (int t = t0; t < t1; ++t) {
-    Half h[2];
+  // A wave's share of a tile: KU of K's half tiles by 64 dims (of 128 dims one, of 256
+  // both halves of 64) and 64 dims of V (with 128 dims waves 2 and 3 load what 0 and 1 do,
+  // and leave it), and all of the scales (K's, then V's).  Codes wait in LDS, three tiles
+  // of them, for the wave that loaded them: in registers, two tiles ahead, they don't fit.
+  constexpr int KU = HD / 128, LOADS = KU + 3;
+  const bool has_v = HD == 256 || wave < HD / 64;
+  const int vblock = wave % (HD / 64);
+  const uint32_t koff = n * HD + 16 * g;
+  // row r of 16 lanes' LDS holds key 4 (r % 4) + r / 4, so that the four lane groups, which
+  // read keys 4 g + e at a time, meet different banks
+  const uint32_t voff = (4 * (lane >> 2 & 3) + (lane >> 4)) * HD + 16 * (lane & 3);
+  auto load_k = [&](int t, const Halves &h) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-      h[u] = half_at(a.c, pages, a.b.width, kTile * t + 16 * u, len, hk);
-    Scales sc;
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      sc.k[u] = *reinterpret_cast<const v4f *>(a.c.ks + h[u].slot + 4 * g);
-      sc.v[u] = *reinterpret_cast<const v4f *>(a.c.vs + h[u].slot + 4 * g);
+    for (int i = 0; i < KU; ++i) {
+      const size_t slot = (KU == 2 ? i : wave >> 1) != 0 ? h.slot1 : h.slot0;
+      dma16(a.c.k + slot * HD + 64 * (wave % (HD / 64)), koff, raw_k[wave][t % 3][i]);
     }
-    __syncthreads();
-    for (int f = wave; f < HD / 32; f += 4) {  // halves and 64-dim blocks of K
-      const int u = f % 2, jc = f / 2;
-      const u4 x = *reinterpret_cast<const u4 *>(a.c.k + (h[u].slot + n) * HD + 64 * jc + 16 * g);
-      kf[u * KS + 2 * jc][lane] = codes8<TYPE>(x[0], x[1]);
-      kf[u * KS + 2 * jc + 1][lane] = codes8<TYPE>(x[2], x[3]);
-    }
-    for (int f = wave; f < HD / 64; f += 4) {  // 64-dim blocks of V
-      uint32_t x[8];
+  };
+  auto load_v = [&](int t, size_t slot0, size_t slot1) {
+    dma16(a.c.v + slot0 * HD + 64 * vblock, voff, raw_v[wave][t % 3][0]);
+    dma16(a.c.v + slot1 * HD + 64 * vblock, voff, raw_v[wave][t % 3][1]);
+  };
+  const float *const scale_base = (lane & 8 ? a.c.vs : a.c.ks) + 4 * (lane & 3);
+  auto load_scales = [&](int t, size_t slot0, size_t slot1) {
+    if (lane < 16) dma16_at(scale_base + (lane & 4 ? slot1 : slot0), scales[wave][t & 3]);
+  };
+  auto scales_k = [&](int t) { return eight(scales[wave][t & 3][g], scales[wave][t & 3][4 + g]); };
+  auto scales_v = [&](int t) {
+    return eight(scales[wave][t & 3][8 + g], scales[wave][t & 3][12 + g]);
+  };
+  auto store_k = [&](int t, int i, int half) {
+    const int u = KU == 2 ? i : wave >> 1;
+    const u2 r = reinterpret_cast<const u2 *>(raw_k[wave][t % 3][i])[2 * lane + half];
+    kf[t & 1][u * KS + 2 * (wave % (HD / 64)) + half][lane] = codes8<TYPE>(r[0], r[1]);
+  };
+  // what lies past the end may be a NaN's code, times a weight of 0 (ok: bits 0 and 1, the
+  // halves that are there)
+  auto read_v = [&](int t, int ok, uint32_t (&r)[8]) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] = *reinterpret_cast<const uint32_t *>(
-            a.c.v + (h[e / 4].slot + 4 * g + e % 4) * HD + 64 * f + 4 * (4 * (n & 3) + (n >> 2)));
-        if (kTile * t + 16 * (e / 4) + 4 * g + e % 4 >= len || !h[e / 4].ok) x[e] = 0;
-      }
-      h8 fr[4];
-      codes_t<TYPE>(x, fr);
+    for (int e = 0; e < 8; ++e)
+      r[e] = reinterpret_cast<const uint32_t *>(
+          raw_v[wave][t % 3][e / 4])[16 * (4 * (e % 4) + g) + 4 * (n & 3) + (n >> 2)];
+    if (TYPE == kKvE4m3 && (kTile * (t0 + t) + kTile > len || (ok & 3) != 3))
 #pragma unroll
-      for (int i = 0; i < 4; ++i) vf[4 * f + i][lane] = fr[i];
-    }
-    __syncthreads();
-    const int key0 = kTile * t;
-    const bool masked = key0 < f_lo || key0 + kTile - 1 > f_hi || !h[0].ok || !h[1].ok;
-    h8 phi[QB], plo[QB];
+      for (int e = 0; e < 8; ++e)
+        if (kTile * (t0 + t) + 16 * (e / 4) + 4 * g + e % 4 >= len || !(ok >> (e / 4) & 1))
+          r[e] = 0;
+  };
+  // step i of the scores; f: K's fragments
+  auto score_step = [&](auto I, const h8 (&f)[2], v4f (&d)[QB][2]) {
 #pragma unroll
-    for (int q = 0; q < QB; ++q) {
-      v4f dh[2] = {}, dl[2] = {};
+    for (int q = 0; q < QB; ++q)
 #pragma unroll
-      for (int i = 0; i < KS; ++i)
+      for (int u = 0; u < 2; ++u) d[q][u] = mma(f[u], qlo[q][I], d[q][u]);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          dl[u] = mma(kf[u * KS + i][lane], qlo[q][i], dl[u]);
-          dh[u] = mma(kf[u * KS + i][lane], qhi[q][i], dh[u]);
+    for (int q = 0; q < QB; ++q)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) d[q][u] = mma(f[u], qhi[q][I], d[q][u]);
+  };
+
+  if (t0 < t1) {
+    Pager pager(a, b, len, hk, t0, 1);  // tiles past the last are loaded and not used
+    int there = 0;  // bits 2 i and 2 i + 1: the halves of tile t + i that are there
+    size_t v_slot0, v_slot1;  // where tile t + 3 lies
+    {
+      const Halves h0 = pager.get(0), h1 = pager.get(1), h2 = pager.get(2), h3 = pager.get(3);
+      there = h0.ok0 | h0.ok1 << 1 | h1.ok0 << 2 | h1.ok1 << 3 | h2.ok0 << 4 | h2.ok1 << 5 |
+              h3.ok0 << 6 | h3.ok1 << 7;
+      v_slot0 = h3.slot0;
+      v_slot1 = h3.slot1;
+      load_k(0, h0);
+      load_v(0, h0.slot0, h0.slot1);
+      load_scales(0, h0.slot0, h0.slot1);
+      load_k(1, h1);
+      load_scales(1, h1.slot0, h1.slot1);
+      load_k(2, h2);
+      load_v(1, h1.slot0, h1.slot1);
+      split_queries();
+      dma_wait<LOADS - 1>();
+#pragma unroll
+      for (int i = 0; i < KU; ++i)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          store_k(0, i, half);
+          store_k(1, i, half);
         }
-      const v4f d[2] = {dh[0] + dl[0], dh[1] + dl[1]};
-      Score score(0.0f, a.cap, 0);
-      score.c = cq[q];
-      score.z = zq[q];
-      const unsigned live = masked ? seen(key0, g, see[q], h[0].ok, h[1].ok) : 0xff;
-      weights<CAP>(d, sc, score, masked, live, soft[q], phi[q], plo[q], [&](float f) {
-#pragma unroll
-        for (int i = 0; i < ND; ++i) o[q][i] *= f;
-      });
+      if (has_v) {
+        uint32_t r[8];
+        Transposed v;
+        read_v(0, there, r);
+        each<4>([&](auto J) { transpose_pair<TYPE, J>(r, v); });
+        each<4>([&](auto I) { vf[0][4 * wave + I][lane] = v.dim(I); });
+      }
+      lds_barrier();
+      load_k(3, h3);
+      load_v(2, h2.slot0, h2.slot1);
+      load_scales(2, h2.slot0, h2.slot1);
     }
-#pragma unroll
-    for (int i = 0; i < ND; ++i) {
-      const h8 f = vf[i][lane];
+    v4f d[QB][2] = {};
+    each<KS>([&](auto I) {
+      const h8 f[2] = {kf[0][I][lane], kf[0][KS + I][lane]};
+      score_step(I, f, d);
+    });
+    float lv[8], top[QB];
+    auto score_all = [&](int t) {
+      const v8f ks = scales_k(t);
+      scale_octaves(scales_v(t), lv);
 #pragma unroll
       for (int q = 0; q < QB; ++q) {
-        o[q][i] = mma(f, plo[q], o[q][i]);
-        o[q][i] = mma(f, phi[q], o[q][i]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          d[q][e / 4][e % 4] = score_of<CAP>(d[q][e / 4][e % 4], ks[e], score[q]);
+        top[q] = top_of(d[q], lv, false, 0);
       }
+    };
+    score_all(0);
+    lds_barrier();
+    int t = 0;  // from t0 on
+    // Hides what queries of tile t don't see; whether some query's M has to move.  That
+    // rarely happens, and lies outside the inner loop: in it the value sums are touched by
+    // the matrix cores alone and stay in the accumulation registers.
+    auto begin = [&]() {
+      const int key0 = kTile * (t0 + t);
+      if (key0 < f_lo || key0 + kTile - 1 > f_hi || (there & 3) != 3) {  // wave-uniform
+        scale_octaves(scales_v(t), lv);
+#pragma unroll
+        for (int q = 0; q < QB; ++q)
+          top[q] = top_of(d[q], lv, true, seen(key0, g, see[q], there & 1, there & 2));
+      }
+      bool moves = false;
+#pragma unroll
+      for (int q = 0; q < QB; ++q) moves = moves || top[q] > soft[q].m + kSlack;
+      return __any(moves);
+    };
+    auto tile = [&]() {
+      const int cur = t & 1, nxt = cur ^ 1;
+      // what was loaded two iterations ago is in; the buffers of an iteration ago are free
+      dma_wait<LOADS>();
+      const Halves h4 = pager.get(t + 4);
+      load_k(t + 4, h4);
+      load_v(t + 3, v_slot0, v_slot1);
+      load_scales(t + 3, v_slot0, v_slot1);
+      h8 phi[QB], plo[QB], kpre[2] = {kf[nxt][0][lane], kf[nxt][KS][lane]}, vpre[VP];
+      v4f dn[QB][2] = {};
+      const v8f vs = scales_v(t);
+      uint32_t rv[8];
+      read_v(t + 1, there >> 2, rv);
+      __builtin_amdgcn_sched_barrier(0);
+      // scores of tile t + 1, weights of tile t, V of tile t + 1
+      Transposed v;
+      each<KS>([&](auto I) {
+        constexpr int i = I;
+        const h8 f[2] = {kpre[0], kpre[1]};
+        if constexpr (i + 1 < KS) {
+          kpre[0] = kf[nxt][i + 1][lane];
+          kpre[1] = kf[nxt][KS + i + 1][lane];
+        } else {
+          each<VP>([&](auto V) { vpre[V] = vf[cur][V][lane]; });
+        }
+        score_step(I, f, dn);
+        constexpr int j0 = 4 * QB * i / KS, j1 = 4 * QB * (i + 1) / KS;
+        each<j1 - j0>([&](auto J) {
+          constexpr int j = j0 + J, q = j / 4;
+          weigh(j % 4, d[q], vs, soft[q], phi[q], plo[q]);
+        });
+        constexpr int v0 = 4 * i / KS, v1 = 4 * (i + 1) / KS;
+        each<v1 - v0>([&](auto J) { transpose_pair<TYPE, v0 + J>(rv, v); });
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      // value products of tile t, V and K of tiles t + 1 and t + 2 into LDS, scores
+      if (has_v) each<4>([&](auto I) { vf[nxt][4 * wave + I][lane] = v.dim(I); });
+      const v8f ks = scales_k(t + 1);
+      scale_octaves(scales_v(t + 1), lv);
+      constexpr int NC = ND / 2;  // chunks of two blocks of dims
+      each<NC>([&](auto I) {
+        constexpr int i = I;
+        const h8 f[2] = {vpre[2 * i % VP], vpre[(2 * i + 1) % VP]};
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (2 * i + e + VP < ND) vpre[(2 * i + e) % VP] = vf[cur][2 * i + e + VP][lane];
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int q = 0; q < QB; ++q) o[q][2 * i + e] = mma(f[e], plo[q], o[q][2 * i + e]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int q = 0; q < QB; ++q) o[q][2 * i + e] = mma(f[e], phi[q], o[q][2 * i + e]);
+        constexpr int k0 = 2 * KU * i / (NC / 2), k1 = 2 * KU * (i + 1) / (NC / 2);
+        if constexpr (i < NC / 2)
+          each<k1 - k0>([&](auto J) {
+            constexpr int j = k0 + J;
+            store_k(t + 2, j / 2, j % 2);
+          });
+        constexpr int e0 = 8 * QB * i / NC, e1 = 8 * QB * (i + 1) / NC;
+        each<e1 - e0>([&](auto E) {
+          constexpr int e = (e0 + E) % 8, q = (e0 + E) / 8;
+          d[q][e / 4][e % 4] = score_of<CAP>(dn[q][e / 4][e % 4], ks[e], score[q]);
+          const float x = d[q][e / 4][e % 4] + lv[e];
+          top[q] = e == 0 ? x : fmaxf(top[q], x);
+        });
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      there = there >> 2 | h4.ok0 << 6 | h4.ok1 << 7;
+      v_slot0 = h4.slot0;
+      v_slot1 = h4.slot1;
+      lds_barrier();
+    };
+    const int nt = t1 - t0;
+    begin();
+    for (;;) {
+#pragma unroll
+      for (int q = 0; q < QB; ++q)
+        settle(top[q], soft[q], [&](float f) {
+#pragma unroll
+          for (int i = 0; i < ND; ++i) o[q][i] *= f;
+        });
+      bool moves = false;
+      do {
+        tile();
+        if (++t == nt) break;
+        moves = begin();
+      } while (!moves);
+      if (t == nt) break;
     }
   }
 #pragma unroll
@@ -747,8 +1002,11 @@ __global__ __launch_bounds__(1024) void kv_merge_kernel(KvAttn a, KvPlan pl) {
 KvPlan plan(const KvAttn &a, const DeviceInfo &dev) {
   KvPlan p{};
   p.group = a.n_heads / a.c.nkv;
+  p.inv_group = ((1 << 21) + p.group - 1) / p.group;
   const int most = a.b.max_rows * p.group;  // query vectors of a sequence and kv head
-  p.step = p.group <= kStepRows && (most <= kStepRows || a.b.batch > 1);
+  // (a batch whose rows add up to max_rows of each has no single tokens)
+  p.step = p.group <= kStepRows &&
+           (most <= kStepRows || a.b.rows < (long)a.b.batch * a.b.max_rows);
   const bool rows = !p.step || most > kStepRows;
   // tiles that a sequence's rows see behind the prefix: by the window where there is one
   const int own = a.b.max_len - a.shared;
