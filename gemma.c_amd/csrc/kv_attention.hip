@@ -9,11 +9,11 @@
 // score, V's into its weight.
 //
 // With c = asc log2 e, s the scaled score in octaves, and a whole number M per
-// query: w = 2^(s - M) vs, l = sum 2^(s - M), out = sum w code / l.  M follows the
-// largest s + log2 vs, not the largest s: what must fit f16 is w.  It has some
-// octaves of slack, so that the sums are rescaled rarely and by powers of two.
-// Weights are kept to 2^-31 of the largest beside them and have all their 22 bits
-// down to 2^-20 of it.
+// query: p = 2^(s - M), w = p vs 2^-24, l = sum p, out = 2^24 sum w code / l.  M follows
+// the largest s + log2 vs, not the largest s: what must fit f16 is w.  It has twelve
+// octaves of slack, so that the sums are rescaled rarely and by powers of two.  A weight
+// is off by at most 2^-25 where the largest is 2 or more: 2^-26 of that one, below the
+// rounding of an fp32 sum that it is part of.
 //
 // A wave computes S^T = K Q^T (rows: 16 keys, columns: 16 queries) and O^T = V^T
 // P^T (rows: 16 dims) with 16x16x32 products.  Operand layout: lane l holds row (or
@@ -41,9 +41,12 @@ namespace {
 constexpr int kTile = 32;             // keys of a tile
 constexpr int kStepRows = 16;         // query vectors (rows x heads of a kv head) of a step tile
 constexpr float kFloor = -0x1p55f;    // M of a query that has seen no key
-constexpr float kSlack = 14.0f;       // weights stay below 2^15 ...
-constexpr float kSet = 7.0f;          // ... and a moved M puts the largest at 2^6 .. 2^8
-constexpr float kLeastVs = -60.0f;    // octaves that a scale counts at least
+constexpr float kVsUnit = 0x1p-24f;   // V's scales enter the weights in units of 2^24, so that
+constexpr float kVsOctaves = 24.0f;   // l keeps its terms beside the largest scales
+constexpr float kSlack = 14.0f + kVsOctaves;  // weights stay below 2^15 ...
+constexpr float kSet = 2.0f + kVsOctaves;     // ... and a moved M puts the largest at 2 .. 2^3
+constexpr float kLeastVs = -60.0f;    // octaves that a scale counts at least ...
+constexpr float kMostVs = 121.0f;     // ... and at most (its own largest; for a NaN)
 constexpr float kLog2e = 1.44269502162933349609375f;
 
 // How a call is cut into workgroups: the same on the host, which sizes the
@@ -210,12 +213,13 @@ struct Score {
   }
 };
 
-// Octaves that the values of a lane's eight keys may add to a weight.
+// Octaves that the values of a lane's eight keys may add to a weight, from their scales in
+// units of 2^24.
 __device__ __forceinline__ void scale_octaves(const v8f &vs, float (&lv)[8]) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const int ev = (int)(__float_as_uint(vs[e]) >> 23 & 255) - 127;
-    lv[e] = fmaxf((float)ev, kLeastVs);
+    const int ev = (int)(__float_as_uint(vs[e]) >> 23 & 255) - 127 + (int)kVsOctaves;
+    lv[e] = fminf(fmaxf((float)ev, kLeastVs), kMostVs);
   }
 }
 
@@ -275,55 +279,63 @@ __device__ __forceinline__ void weigh(int j, const v4f (&x)[2], const v8f &vs, S
 }
 
 // Which of a lane's eight keys of the tile at key0 are seen.
-__device__ __forceinline__ unsigned seen(int key0, int g, KvSee see, bool ok0, bool ok1) {
+__device__ __forceinline__ unsigned seen(int key0, int g, KvSee see, int ok) {
   unsigned live = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const int key = key0 + 16 * (e / 4) + 4 * g + e % 4;
-    if (key >= see.lo && key <= see.hi && (e < 4 ? ok0 : ok1)) live |= 1u << e;
+    if (key >= see.lo && key <= see.hi && (ok >> (e / 4) & 1)) live |= 1u << e;
   }
   return live;
 }
 
-// Where the halves (16 keys) of a tile lie, wave-uniform: pages hold whole halves.  One
-// that isn't there (past the end, or on a bad page) reads page 0.
+// Where the halves (16 keys) of a tile lie: number of the first position's row in the
+// cache, wave-uniform (pages hold whole halves).  One that isn't there (past the end, or on
+// a bad page) reads page 0.
 struct Halves {
   size_t slot0, slot1;
-  bool ok0, ok1;
+  int ok;  // bits 0 and 1: the halves that are there
 };
 
-// The halves of a wave's tiles first, first + step, ... in turn.  Page ids come 64 at a
-// time, one a lane, the next ones ahead of their use, and by vector loads: waits for
-// a scalar load would be waits for all of the wave's LDS reads as well.
+// The halves of a wave's tiles first, first + step, ... in turn.  Lane i works out half i
+// of 32 tiles at a time, the next ones' page ids loaded ahead of their use; by vector
+// loads, since waits for a scalar load would be waits for all of the wave's LDS reads too.
 struct Pager {
   const int *pages;
   int width, shift, npages, nkv, hk, len, first, step;
-  int ids, next;
+  int next, slot_lo, slot_hi;
+  unsigned long long there;
   __device__ __forceinline__ Pager(const KvAttn &a, int seq, int length, int head, int t0, int dt)
       : pages(a.b.pages + (size_t)seq * a.b.width), width(a.b.width), shift(a.c.shift),
         npages(a.c.npages), nkv(a.c.nkv), hk(head), len(length), first(t0), step(dt) {
-    ids = load(0);
-    next = load(32);
+    next = load(0);
+    place(0);
+  }
+  __device__ __forceinline__ int key(int from) const {
+    const int lane = threadIdx.x & 63;
+    return kTile * (first + step * (from + lane / 2)) + 16 * (lane & 1);
   }
   __device__ __forceinline__ int load(int from) const {
-    const int lane = threadIdx.x & 63, key = kTile * (first + step * (from + lane / 2)) + 16 * (lane & 1);
-    return pages[min(key >> shift, width - 1)];
+    return pages[min(key(from) >> shift, width - 1)];
   }
-  __device__ __forceinline__ size_t slot(int id, int key, bool *ok) const {
-    *ok = key < len && (unsigned)id < (unsigned)npages;
-    return (((size_t)(*ok ? id : 0) * nkv + hk) << shift) + (key & ((1 << shift) - 1));
+  __device__ __forceinline__ void place(int from) {
+    const int k = key(from);
+    const bool ok = k < len && (unsigned)next < (unsigned)npages;
+    const size_t slot = (((size_t)(ok ? next : 0) * nkv + hk) << shift) + (k & ((1 << shift) - 1));
+    slot_lo = (int)slot;
+    slot_hi = (int)(slot >> 32);
+    there = __ballot(ok);
+    next = load(from + 32);
+  }
+  __device__ __forceinline__ size_t slot(int i) const {
+    return (size_t)(uint32_t)__builtin_amdgcn_readlane(slot_hi, i) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane(slot_lo, i);
   }
   // the j-th tile's halves; j counts up from 0
   __device__ __forceinline__ Halves get(int j) {
-    if ((j & 31) == 0 && j > 0) {
-      ids = next;
-      next = load(j + 32);
-    }
-    const int key = kTile * (first + step * j);
-    Halves h;
-    h.slot0 = slot(__builtin_amdgcn_readlane(ids, 2 * (j & 31)), key, &h.ok0);
-    h.slot1 = slot(__builtin_amdgcn_readlane(ids, 2 * (j & 31) + 1), key + 16, &h.ok1);
-    return h;
+    if ((j & 31) == 0 && j > 0) place(j);
+    const int i = 2 * (j & 31);
+    return Halves{slot(i), slot(i + 1), (int)(there >> i) & 3};
   }
 };
 
@@ -462,22 +474,23 @@ __global__ __launch_bounds__(64 * kStepWaves, 2) void kv_step_kernel(KvAttn a, K
           dh[u] = mma(f, qhi[i], dh[u]);
         }
       v4f d[2] = {dh[0] + dl[0], dh[1] + dl[1]};
-      const Scales now = sc;
+      Scales now = sc;
+      now.v *= kVsUnit;
       __builtin_amdgcn_sched_barrier(0);
       load_k(nxt);
       __builtin_amdgcn_sched_barrier(0);
       const int key0 = kTile * t;
       const bool masked =
-          key0 < f_lo || key0 + kTile - 1 > f_hi || !cur.ok0 || !cur.ok1;  // wave-uniform
+          key0 < f_lo || key0 + kTile - 1 > f_hi || cur.ok != 3;  // wave-uniform
       unsigned live = 0xff;
       if (masked) {
-        live = seen(key0, g, see, cur.ok0, cur.ok1);
+        live = seen(key0, g, see, cur.ok);
         // what lies past a sequence's end may be a NaN's code, times a weight of 0
         if (TYPE == kKvE4m3)
 #pragma unroll
           for (int e = 0; e < 8; ++e)
             if (key0 + 16 * (e / 4) + 4 * g + e % 4 >= s.len ||
-                !(e < 4 ? cur.ok0 : cur.ok1))
+                !(cur.ok >> (e / 4) & 1))
               vval[e / 4][e % 4] = vreg(0u);
       }
       float lv[8];
@@ -546,7 +559,7 @@ __global__ __launch_bounds__(64 * kStepWaves, 2) void kv_step_kernel(KvAttn a, K
     if (pl.step_ns == 1 && pl.pre_ns == 0) {
       float *out = a.out + ((size_t)(s.r0 + q / pl.group) * a.n_heads + hk * pl.group +
                             q % pl.group) * HD + d;
-      *reinterpret_cast<v4f *>(out) = l != 0.0f ? x / l : v4f{};
+      *reinterpret_cast<v4f *>(out) = l != 0.0f ? x / (l * kVsUnit) : v4f{};
     } else {
       const size_t at = (((size_t)b * a.c.nkv + hk) * pl.step_ns + chunk) * pl.step_rows + q;
       *reinterpret_cast<v4f *>((float *)(a.work + pl.step_o) + at * HD + d) = x;
@@ -673,16 +686,17 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(KvAttn a, KvPlan pl) {
   // row r of 16 lanes' LDS holds key 4 (r % 4) + r / 4, so that the four lane groups, which
   // read keys 4 g + e at a time, meet different banks
   const uint32_t voff = (4 * (lane >> 2 & 3) + (lane >> 4)) * HD + 16 * (lane & 3);
-  auto load_k = [&](int t, const Halves &h) {
+  const uint8_t *const k_base = a.c.k + 64 * (wave % (HD / 64)), *const v_base = a.c.v + 64 * vblock;
+  auto load_k = [&](int r, const Halves &h) {  // r: the buffer, tile modulo 3
 #pragma unroll
     for (int i = 0; i < KU; ++i) {
       const size_t slot = (KU == 2 ? i : wave >> 1) != 0 ? h.slot1 : h.slot0;
-      dma16(a.c.k + slot * HD + 64 * (wave % (HD / 64)), koff, raw_k[wave][t % 3][i]);
+      dma16(k_base + slot * HD, koff, raw_k[wave][r][i]);
     }
   };
-  auto load_v = [&](int t, size_t slot0, size_t slot1) {
-    dma16(a.c.v + slot0 * HD + 64 * vblock, voff, raw_v[wave][t % 3][0]);
-    dma16(a.c.v + slot1 * HD + 64 * vblock, voff, raw_v[wave][t % 3][1]);
+  auto load_v = [&](int r, size_t slot0, size_t slot1) {
+    dma16(v_base + slot0 * HD, voff, raw_v[wave][r][0]);
+    dma16(v_base + slot1 * HD, voff, raw_v[wave][r][1]);
   };
   const float *const scale_base = (lane & 8 ? a.c.vs : a.c.ks) + 4 * (lane & 3);
   auto load_scales = [&](int t, size_t slot0, size_t slot1) {
@@ -690,25 +704,30 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(KvAttn a, KvPlan pl) {
   };
   auto scales_k = [&](int t) { return eight(scales[wave][t & 3][g], scales[wave][t & 3][4 + g]); };
   auto scales_v = [&](int t) {
-    return eight(scales[wave][t & 3][8 + g], scales[wave][t & 3][12 + g]);
+    return eight(scales[wave][t & 3][8 + g], scales[wave][t & 3][12 + g]) * kVsUnit;
   };
-  auto store_k = [&](int t, int i, int half) {
+  auto read_k = [&](int r, u4 (&x)[KU]) {
+#pragma unroll
+    for (int i = 0; i < KU; ++i) x[i] = raw_k[wave][r][i][lane];
+  };
+  auto store_k = [&](int buf, int i, int half, const u4 (&x)[KU]) {
     const int u = KU == 2 ? i : wave >> 1;
-    const u2 r = reinterpret_cast<const u2 *>(raw_k[wave][t % 3][i])[2 * lane + half];
-    kf[t & 1][u * KS + 2 * (wave % (HD / 64)) + half][lane] = codes8<TYPE>(r[0], r[1]);
+    kf[buf][u * KS + 2 * (wave % (HD / 64)) + half][lane] =
+        codes8<TYPE>(x[i][2 * half], x[i][2 * half + 1]);
+  };
+  auto read_v = [&](int r, uint32_t (&x)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      x[e] = reinterpret_cast<const uint32_t *>(
+          raw_v[wave][r][e / 4])[16 * (4 * (e % 4) + g) + 4 * (n & 3) + (n >> 2)];
   };
   // what lies past the end may be a NaN's code, times a weight of 0 (ok: bits 0 and 1, the
   // halves that are there)
-  auto read_v = [&](int t, int ok, uint32_t (&r)[8]) {
+  auto clear_v = [&](int t, int ok, uint32_t (&x)[8]) {
+    if (TYPE != kKvE4m3 || (kTile * (t0 + t) + kTile <= len && (ok & 3) == 3)) return;
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      r[e] = reinterpret_cast<const uint32_t *>(
-          raw_v[wave][t % 3][e / 4])[16 * (4 * (e % 4) + g) + 4 * (n & 3) + (n >> 2)];
-    if (TYPE == kKvE4m3 && (kTile * (t0 + t) + kTile > len || (ok & 3) != 3))
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (kTile * (t0 + t) + 16 * (e / 4) + 4 * g + e % 4 >= len || !(ok >> (e / 4) & 1))
-          r[e] = 0;
+      if (kTile * (t0 + t) + 16 * (e / 4) + 4 * g + e % 4 >= len || !(ok >> (e / 4) & 1)) x[e] = 0;
   };
   // step i of the scores; f: K's fragments
   auto score_step = [&](auto I, const h8 (&f)[2], v4f (&d)[QB][2]) {
@@ -726,10 +745,10 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(KvAttn a, KvPlan pl) {
     Pager pager(a, b, len, hk, t0, 1);  // tiles past the last are loaded and not used
     int there = 0;  // bits 2 i and 2 i + 1: the halves of tile t + i that are there
     size_t v_slot0, v_slot1;  // where tile t + 3 lies
+    uint32_t rv[8];  // codes of V of tile t + 1
     {
       const Halves h0 = pager.get(0), h1 = pager.get(1), h2 = pager.get(2), h3 = pager.get(3);
-      there = h0.ok0 | h0.ok1 << 1 | h1.ok0 << 2 | h1.ok1 << 3 | h2.ok0 << 4 | h2.ok1 << 5 |
-              h3.ok0 << 6 | h3.ok1 << 7;
+      there = h0.ok | h1.ok << 2 | h2.ok << 4 | h3.ok << 6;
       v_slot0 = h3.slot0;
       v_slot1 = h3.slot1;
       load_k(0, h0);
@@ -741,34 +760,39 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(KvAttn a, KvPlan pl) {
       load_v(1, h1.slot0, h1.slot1);
       split_queries();
       dma_wait<LOADS - 1>();
+      u4 rk[KU];
 #pragma unroll
-      for (int i = 0; i < KU; ++i)
+      for (int t = 0; t < 2; ++t) {
+        read_k(t, rk);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          store_k(0, i, half);
-          store_k(1, i, half);
+        for (int i = 0; i < KU; ++i) {
+          store_k(t, i, 0, rk);
+          store_k(t, i, 1, rk);
         }
-      if (has_v) {
-        uint32_t r[8];
-        Transposed v;
-        read_v(0, there, r);
-        each<4>([&](auto J) { transpose_pair<TYPE, J>(r, v); });
-        each<4>([&](auto I) { vf[0][4 * wave + I][lane] = v.dim(I); });
       }
+      read_v(0, rv);
+      clear_v(0, there, rv);
+      Transposed v;
+      each<4>([&](auto J) { transpose_pair<TYPE, J>(rv, v); });
+      if (has_v) each<4>([&](auto I) { vf[0][4 * wave + I][lane] = v.dim(I); });
       lds_barrier();
-      load_k(3, h3);
+      load_k(0, h3);
       load_v(2, h2.slot0, h2.slot1);
       load_scales(2, h2.slot0, h2.slot1);
+      dma_wait<LOADS>();
+      read_v(1, rv);
     }
     v4f d[QB][2] = {};
     each<KS>([&](auto I) {
       const h8 f[2] = {kf[0][I][lane], kf[0][KS + I][lane]};
       score_step(I, f, d);
     });
-    float lv[8], top[QB];
-    auto score_all = [&](int t) {
-      const v8f ks = scales_k(t);
-      scale_octaves(scales_v(t), lv);
+    float top[QB];
+    v8f vs = scales_v(0);
+    {
+      const v8f ks = scales_k(0);
+      float lv[8];
+      scale_octaves(vs, lv);
 #pragma unroll
       for (int q = 0; q < QB; ++q) {
 #pragma unroll
@@ -776,42 +800,39 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(KvAttn a, KvPlan pl) {
           d[q][e / 4][e % 4] = score_of<CAP>(d[q][e / 4][e % 4], ks[e], score[q]);
         top[q] = top_of(d[q], lv, false, 0);
       }
-    };
-    score_all(0);
+    }
     lds_barrier();
-    int t = 0;  // from t0 on
+    int t = 0, r = 0;  // the tile, from t0 on; its number modulo 3
     // Hides what queries of tile t don't see; whether some query's M has to move.  That
     // rarely happens, and lies outside the inner loop: in it the value sums are touched by
     // the matrix cores alone and stay in the accumulation registers.
     auto begin = [&]() {
       const int key0 = kTile * (t0 + t);
       if (key0 < f_lo || key0 + kTile - 1 > f_hi || (there & 3) != 3) {  // wave-uniform
-        scale_octaves(scales_v(t), lv);
+        float lv[8];
+        scale_octaves(vs, lv);
 #pragma unroll
         for (int q = 0; q < QB; ++q)
-          top[q] = top_of(d[q], lv, true, seen(key0, g, see[q], there & 1, there & 2));
+          top[q] = top_of(d[q], lv, true, seen(key0, g, see[q], there));
       }
+      clear_v(t + 1, there >> 2, rv);
       bool moves = false;
 #pragma unroll
       for (int q = 0; q < QB; ++q) moves = moves || top[q] > soft[q].m + kSlack;
       return __any(moves);
     };
+    // One tile.  Each chunk of products takes its share of the vector work; what a later
+    // chunk reads from LDS is asked for one or two chunks before.
     auto tile = [&]() {
-      const int cur = t & 1, nxt = cur ^ 1;
-      // what was loaded two iterations ago is in; the buffers of an iteration ago are free
-      dma_wait<LOADS>();
-      const Halves h4 = pager.get(t + 4);
-      load_k(t + 4, h4);
-      load_v(t + 3, v_slot0, v_slot1);
-      load_scales(t + 3, v_slot0, v_slot1);
+      const int cur = t & 1, nxt = cur ^ 1, r1 = r == 2 ? 0 : r + 1, r2 = 3 - r - r1;
       h8 phi[QB], plo[QB], kpre[2] = {kf[nxt][0][lane], kf[nxt][KS][lane]}, vpre[VP];
       v4f dn[QB][2] = {};
-      const v8f vs = scales_v(t);
-      uint32_t rv[8];
-      read_v(t + 1, there >> 2, rv);
-      __builtin_amdgcn_sched_barrier(0);
-      // scores of tile t + 1, weights of tile t, V of tile t + 1
+      u4 rk[KU];
+      v8f ks, vn;
       Transposed v;
+      Halves h4;
+      // scores of tile t + 1; weights of tile t, V of tile t + 1, loads of tiles t + 3 and
+      // t + 4 (into the buffers that the iteration before was done with)
       each<KS>([&](auto I) {
         constexpr int i = I;
         const h8 f[2] = {kpre[0], kpre[1]};
@@ -819,7 +840,10 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(KvAttn a, KvPlan pl) {
           kpre[0] = kf[nxt][i + 1][lane];
           kpre[1] = kf[nxt][KS + i + 1][lane];
         } else {
+          read_k(r2, rk);
           each<VP>([&](auto V) { vpre[V] = vf[cur][V][lane]; });
+          ks = scales_k(t + 1);
+          vn = scales_v(t + 1);
         }
         score_step(I, f, dn);
         constexpr int j0 = 4 * QB * i / KS, j1 = 4 * QB * (i + 1) / KS;
@@ -827,15 +851,25 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(KvAttn a, KvPlan pl) {
           constexpr int j = j0 + J, q = j / 4;
           weigh(j % 4, d[q], vs, soft[q], phi[q], plo[q]);
         });
-        constexpr int v0 = 4 * i / KS, v1 = 4 * (i + 1) / KS;
-        each<v1 - v0>([&](auto J) { transpose_pair<TYPE, v0 + J>(rv, v); });
+        if constexpr (KS == 8) {
+          if constexpr (i < 4)
+            transpose_pair<TYPE, i>(rv, v);
+          else if (has_v)
+            vf[nxt][4 * wave + i - 4][lane] = v.dim(i - 4);
+        } else {
+          transpose_pair<TYPE, i>(rv, v);
+          if constexpr (i == KS - 1)
+            if (has_v) each<4>([&](auto D) { vf[nxt][4 * wave + D][lane] = v.dim(D); });
+        }
+        if constexpr (i == KS / 2 - 2) h4 = pager.get(t + 4);
+        if constexpr (i == KS / 2 - 1) load_k(r1, h4);
+        if constexpr (i == KS / 2) load_v(r, v_slot0, v_slot1);
+        if constexpr (i == KS / 2 + 1) load_scales(t + 3, v_slot0, v_slot1);
         __builtin_amdgcn_sched_barrier(0);
       });
-      // value products of tile t, V and K of tiles t + 1 and t + 2 into LDS, scores
-      if (has_v) each<4>([&](auto I) { vf[nxt][4 * wave + I][lane] = v.dim(I); });
-      const v8f ks = scales_k(t + 1);
-      scale_octaves(scales_v(t + 1), lv);
+      // value products of tile t; scores and K of tiles t + 1 and t + 2
       constexpr int NC = ND / 2;  // chunks of two blocks of dims
+      float lv[8];
       each<NC>([&](auto I) {
         constexpr int i = I;
         const h8 f[2] = {vpre[2 * i % VP], vpre[(2 * i + 1) % VP]};
@@ -850,24 +884,34 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(KvAttn a, KvPlan pl) {
         for (int e = 0; e < 2; ++e)
 #pragma unroll
           for (int q = 0; q < QB; ++q) o[q][2 * i + e] = mma(f[e], phi[q], o[q][2 * i + e]);
-        constexpr int k0 = 2 * KU * i / (NC / 2), k1 = 2 * KU * (i + 1) / (NC / 2);
-        if constexpr (i < NC / 2)
-          each<k1 - k0>([&](auto J) {
-            constexpr int j = k0 + J;
-            store_k(t + 2, j / 2, j % 2);
-          });
-        constexpr int e0 = 8 * QB * i / NC, e1 = 8 * QB * (i + 1) / NC;
+        if constexpr (i == 0) scale_octaves(vn, lv);
+        constexpr int k0 = 2 * KU * i / NC, k1 = 2 * KU * (i + 1) / NC;
+        each<k1 - k0>([&](auto J) {
+          constexpr int j = k0 + J;
+          store_k(cur, j / 2, j % 2, rk);
+        });
+        constexpr int e0 = i > 0 ? 8 * QB * (i - 1) / (NC - 1) : 0, e1 = 8 * QB * i / (NC - 1);
         each<e1 - e0>([&](auto E) {
           constexpr int e = (e0 + E) % 8, q = (e0 + E) / 8;
-          d[q][e / 4][e % 4] = score_of<CAP>(dn[q][e / 4][e % 4], ks[e], score[q]);
-          const float x = d[q][e / 4][e % 4] + lv[e];
-          top[q] = e == 0 ? x : fmaxf(top[q], x);
+          float x = score_of<CAP>(dn[q][e / 4][e % 4], ks[e], score[q]);
+          asm volatile("" : "+v"(x));  // here, not behind the barrier
+          d[q][e / 4][e % 4] = x;
+          top[q] = e == 0 ? x + lv[e] : fmaxf(top[q], x + lv[e]);
         });
+        if constexpr (i == NC - 2) {
+          // what was loaded an iteration ago is in
+          dma_wait<LOADS>();
+          read_v(r2, rv);
+        }
         __builtin_amdgcn_sched_barrier(0);
       });
-      there = there >> 2 | h4.ok0 << 6 | h4.ok1 << 7;
+#pragma unroll
+      for (int q = 0; q < QB; ++q) asm volatile("" : "+v"(top[q]));
+      vs = vn;
+      there = there >> 2 | h4.ok << 6;
       v_slot0 = h4.slot0;
       v_slot1 = h4.slot1;
+      r = r1;
       lds_barrier();
     };
     const int nt = t1 - t0;
@@ -898,7 +942,7 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(KvAttn a, KvPlan pl) {
     const size_t pt = (size_t)chunk * a.b.rows * a.n_heads + vec;
     float *dst = whole ? a.out + vec * HD
                        : (float *)(a.work + (PRE ? pl.pre_o : pl.rows_o)) + pt * HD;
-    const float f = !whole ? 1.0f : soft[q].l != 0.0f ? 1.0f / soft[q].l : 0.0f;
+    const float f = !whole ? 1.0f : soft[q].l != 0.0f ? 1.0f / (soft[q].l * kVsUnit) : 0.0f;
     // o[4 w + i][r]: dim 64 w + 16 r + 4 g + i
 #pragma unroll
     for (int w = 0; w < HD / 64; ++w)
@@ -996,7 +1040,7 @@ __global__ __launch_bounds__(1024) void kv_merge_kernel(KvAttn a, KvPlan pl) {
     ll += sl[w] * f;
     sum += so[w][threadIdx.x] * f;
   }
-  a.out[vec * HD + threadIdx.x] = ll != 0.0f ? sum / ll : 0.0f;
+  a.out[vec * HD + threadIdx.x] = ll != 0.0f ? sum / (ll * kVsUnit) : 0.0f;
 }
 
 KvPlan plan(const KvAttn &a, const DeviceInfo &dev) {
