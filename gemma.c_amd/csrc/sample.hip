@@ -6,17 +6,18 @@
 // rising index), and so is what each filter keeps and what lies before the token
 // drawn: each step finds the first token of that order up to which a running
 // count or a running weight reaches a target.  No row is sorted for that: tokens
-// are counted, and weighed, in 256 bins of 1/8 octave below the row's largest (the
+// are counted, and weighed, in 512 bins of 1/16 octave below the row's largest (the
 // last bin holds all the rest), and only the bins in which a target may be reached
 // are looked into.
 //
-// Weights are fp64.  Sums inside a bin of a workgroup are of whole multiples of a
-// power of two, and so exact in any order; sums over bins and workgroups are fp64 in
-// one order.  So equal calls give equal bits.
+// Weights are fp64.  A bin's tokens weigh 1 to 1.044 times its lower end: what a token
+// adds is 1 and a fraction in whole multiples of 2^-39, count and fraction in one
+// 64-bit sum, exact in any order.  Sums over bins and workgroups are fp64 in one order.
+// So equal calls give equal bits.
 //
 // Up to kWholeVocab columns a workgroup does a row by itself.  Longer rows take four
-// launches: each 4096-column chunk's bins, relative to its own largest logit so
-// that one reading does (sample_bins_kernel); their sum and the bins that matter
+// launches: each 8192-column chunk's bins, from its own largest logit down so that one
+// reading does (sample_bins_kernel); their sum and the bins that matter
 // (sample_decide_kernel); these bins' tokens (sample_collect_kernel; chunks that
 // hold none are not read again); and the targets inside them (sample_pick_kernel).
 #include <float.h>
@@ -31,16 +32,18 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int kBins = 256;
-constexpr double kPerOctave = 8.0;
-constexpr int kChunk = 4096;       // columns of a workgroup of the long rows' kernels
-constexpr int kChunkThreads = 256;
+constexpr int kBins = 512;
+constexpr double kPerOctave = 16.0;
+constexpr int kChunk = 8192;       // columns of a workgroup of the long rows' kernels
+constexpr int kChunkThreads = 512;
 constexpr int kPer = kChunk / kChunkThreads;
 constexpr int kThreads = 1024;     // ... of the kernels that see whole rows
 constexpr int kWholeVocab = 16384;
 constexpr int kRanked = 256;       // tokens that are put in order by comparing all pairs
 constexpr int kSubs = 1024;        // parts of a bin with more
-constexpr int kList = 16384;       // tokens of a row's bins that are collected, at most
+constexpr int kList = 32768;       // tokens of a row's bins that are collected, at most
+constexpr int kFrac = 39;          // a bin's sum: fractions in 2^-39 below, the count above
+constexpr int kCountAt = 49;       // (2^14 tokens of fractions below 0.0443 stay below 2^49)
 constexpr int kUnit = 44;          // a weight's units within its bin: 2^-44 of the bin's octave
 constexpr double kInfZ = 0x1p1000;  // an infinite logit, far above any other's octaves
 
@@ -113,7 +116,7 @@ __device__ Settings settings(const Sample &a, int row) {
   return s;
 }
 
-// Where bins lie: bin i holds 8 z in [gmax - i, gmax - i + 1), the last one all below;
+// Where bins lie: bin i holds 16 z in [gmax - i, gmax - i + 1), the last one all below;
 // weights are relative to 2^e.
 struct Grid {
   double gmax, e;
@@ -148,6 +151,7 @@ struct Row {
   __device__ uint32_t count_of(int i) const { return sum_c[i] - count_before(i); }
 };
 constexpr uint32_t kNone = ~0u;
+constexpr int kPerLane = kBins / 64;
 
 // The first bin with tokens for which f holds, the last one with tokens if none: by
 // each wave on its own.
@@ -156,8 +160,8 @@ __device__ __forceinline__ int first_bin(const Row &r, F &&f) {
   const int lane = threadIdx.x & 63;
   int hit = kBins, some = -1;
 #pragma unroll
-  for (int e = 3; e >= 0; --e) {
-    const int i = 4 * lane + e;
+  for (int e = kPerLane - 1; e >= 0; --e) {
+    const int i = kPerLane * lane + e;
     if (r.count_of(i) == 0) continue;
     some = max(some, i);
     if (f(i)) hit = i;
@@ -188,12 +192,12 @@ __device__ __forceinline__ void min_p_bins(const Row &r, double m, int (&b)[2]) 
 __device__ void sum_bins(const uint32_t *count, const double *mass, Row &r) {
   const int lane = threadIdx.x;
   if (lane >= 64) return;
-  uint32_t c[4], cs = 0;
-  double m[4], ms = 0.0;
+  uint32_t c[kPerLane], cs = 0;
+  double m[kPerLane], ms = 0.0;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    c[e] = cs += count[4 * lane + e];
-    m[e] = ms += mass[4 * lane + e];
+  for (int e = 0; e < kPerLane; ++e) {
+    c[e] = cs += count[kPerLane * lane + e];
+    m[e] = ms += mass[kPerLane * lane + e];
   }
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
@@ -204,13 +208,13 @@ __device__ void sum_bins(const uint32_t *count, const double *mass, Row &r) {
       ms += mt;
     }
   }
-  const uint32_t cb = cs - c[3];
+  const uint32_t cb = cs - c[kPerLane - 1];
   const double before = __shfl_up(ms, 1, 64);  // not ms less the own: sums must not fall
   const double mb = lane > 0 ? before : 0.0;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    r.sum_c[4 * lane + e] = cb + c[e];
-    r.sum_m[4 * lane + e] = (u64)__double_as_longlong(fmin(mb + m[e], ms));
+  for (int e = 0; e < kPerLane; ++e) {
+    r.sum_c[kPerLane * lane + e] = cb + c[e];
+    r.sum_m[kPerLane * lane + e] = (u64)__double_as_longlong(fmin(mb + m[e], ms));
   }
 }
 
@@ -221,10 +225,10 @@ __device__ void decide(const Settings &st, Row &r) {
   const int lane = threadIdx.x;
   if (lane >= 64) return;
   const uint32_t n = r.sum_c[kBins - 1];
-  bool need[4] = {};
+  bool need[kPerLane] = {};
   auto mark = [&](int lo, int hi) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) need[e] = need[e] || (4 * lane + e >= lo && 4 * lane + e <= hi);
+    for (int e = 0; e < kPerLane; ++e) need[e] = need[e] || (kPerLane * lane + e >= lo && kPerLane * lane + e <= hi);
   };
   int cut_lo = kBins - 1, cut_hi = kBins - 1;
   double s_lo = r.weight(kBins - 1), s_hi = s_lo;
@@ -258,11 +262,11 @@ __device__ void decide(const Settings &st, Row &r) {
   }
   mark(bin_past_weight(r, st.u * s_lo), min(bin_past_weight(r, st.u * s_hi), cut_hi));
   // list positions
-  uint32_t own[4], sum = 0;
+  uint32_t own[kPerLane], sum = 0;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
+  for (int e = 0; e < kPerLane; ++e) {
     own[e] = sum;
-    sum += need[e] ? r.count_of(4 * lane + e) : 0u;
+    sum += need[e] ? r.count_of(kPerLane * lane + e) : 0u;
   }
   uint32_t run = sum;
 #pragma unroll
@@ -271,9 +275,9 @@ __device__ void decide(const Settings &st, Row &r) {
     if (lane >= off) run += t;
   }
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    r.at[4 * lane + e] = need[e] ? run - sum + own[e] : kNone;
-    r.fill[4 * lane + e] = 0;
+  for (int e = 0; e < kPerLane; ++e) {
+    r.at[kPerLane * lane + e] = need[e] ? run - sum + own[e] : kNone;
+    r.fill[kPerLane * lane + e] = 0;
   }
   if (lane == 63) r.listed = run <= kList;
 }
@@ -385,7 +389,7 @@ __device__ Found locate(const Sample &a, int row, const Settings &st, const u64 
   const double unit = ldexp(1.0, (int)fmax(top - r.g.e, -1000.0) - kUnit);
   if (!by_count) target -= base;
   auto weigh = [&](u64 p) { return pow2(octaves(logit_at(p), st.c) - top, s.tab); };
-  const double edge = r.g.gmax - bin;  // 8 z of the bin's lower end
+  const double edge = r.g.gmax - bin;  // 16 z of the bin's lower end
   auto part = [&](u64 p) {
     const double y = octaves(logit_at(p), st.c) * kPerOctave - edge;  // in [0, 1); the last: < 1
     const double d = bin < kBins - 1 ? (1.0 - y) * kSubs : 1.0 - y;
@@ -595,26 +599,41 @@ __device__ float block_most(float v, float *red) {
   return m;
 }
 
+// 2^x - 1 in units of 2^-kFrac, 0 <= x < 1/16: the Taylor polynomial (what it leaves out
+// is below 2^-51).
+__device__ __forceinline__ u64 fraction(double x) {
+  const double y = x * 0x1.62e42fefa39efp-1;
+  double p = fma(y, 1.0 / 5040.0, 1.0 / 720.0);
+  p = fma(y, p, 1.0 / 120.0);
+  p = fma(y, p, 1.0 / 24.0);
+  p = fma(y, p, 1.0 / 6.0);
+  p = fma(y, p, 0.5);
+  p = fma(y, p, 1.0);
+  return units(y * p, kFrac);
+}
+
 // Counts and weighs tokens into bins; the last bin's, which most tokens of a peaked
-// row share, in registers first.
+// row share, in registers first (weights of all sizes: count, and units of 2^-kUnit of
+// the bin's octave).
+struct Rest {
+  u64 mass;
+  uint32_t count;
+};
 struct Binner {
-  uint32_t *count;
-  u64 *mass;
+  u64 *bins;
+  Rest *rest;
   uint32_t rest_c = 0;
   u64 rest_m = 0;
-  __device__ __forceinline__ Binner(uint32_t *c, u64 *m) : count(c), mass(m) {}
-  __device__ __forceinline__ void add(float l, double c, const Grid &g, int bits,
-                                      const double *tab) {
+  __device__ __forceinline__ Binner(u64 *b, Rest *r) : bins(b), rest(r) {}
+  __device__ __forceinline__ void add(float l, double c, const Grid &g, const double *tab) {
     if (!has_place(l)) return;
-    const double z = octaves(l, c), x = z - g.e;
-    const int i = bin_of(z, g.gmax);
-    const u64 w = x > -64.0 ? units(pow2(x, tab), bits) : 0;
-    if (i < kBins - 1) {
-      atomicAdd(&count[i], 1u);
-      atomicAdd(&mass[i], w);
+    const double z = octaves(l, c), y = z * kPerOctave, f = floor(y), d = g.gmax - f;
+    if (d < kBins - 1) {
+      atomicAdd(&bins[(int)d], (1ull << kCountAt) + fraction((y - f) * (1.0 / kPerOctave)));
     } else {
       ++rest_c;
-      rest_m += w;
+      const double x = z - bin_top(kBins - 1, g);
+      if (x > -64.0) rest_m += units(pow2(x, tab), kUnit);
     }
   }
   __device__ __forceinline__ void finish() {
@@ -624,11 +643,24 @@ struct Binner {
       rest_m += __shfl_xor(rest_m, off, 64);
     }
     if ((threadIdx.x & 63) == 0 && rest_c != 0) {
-      atomicAdd(&count[kBins - 1], rest_c);
-      atomicAdd(&mass[kBins - 1], rest_m);
+      atomicAdd(&rest->count, rest_c);
+      atomicAdd(&rest->mass, rest_m);
     }
   }
 };
+__device__ __forceinline__ uint32_t bin_count(u64 b) { return (uint32_t)(b >> kCountAt); }
+// ... and weight, relative to the bin's lower end
+__device__ __forceinline__ double bin_weight(u64 b) {
+  return (double)bin_count(b) + ldexp((double)(b & ((1ull << kCountAt) - 1)), -kFrac);
+}
+// The last bin's weight, relative to 2^e.
+__device__ __forceinline__ double rest_weight(const Rest &r, const Grid &g) {
+  return ldexp((double)r.mass, (int)fmax(bin_top(kBins - 1, g) - g.e, -1000.0) - kUnit);
+}
+// A bin's lower end, relative to 2^e.
+__device__ __forceinline__ double bin_end(int bin, const Grid &g, const double *tab) {
+  return pow2((g.gmax - bin) * (1.0 / kPerOctave) - g.e, tab);
+}
 
 // ---- short rows: a workgroup each -----------------------------------------------
 
@@ -636,18 +668,20 @@ __global__ __launch_bounds__(kThreads) void sample_whole_kernel(Sample a) {
   __shared__ Lds s;
   __shared__ float red[kThreads / 64];
   __shared__ double mass[kBins];
+  __shared__ Rest rest;
   const int row = blockIdx.x, tid = threadIdx.x;
   const float *l = a.logits + row * a.stride;
   const Settings st = settings(a, row);
   exp_tab_load(s.tab);
-  if (tid < kBins) s.count[tid] = s.mass[tid] = 0;
+  if (tid < kBins) s.mass[tid] = 0;
+  if (tid == 0) rest = Rest{0, 0};
   float most = -INFINITY;
   for (int i = tid; i < a.vocab; i += kThreads) most = fmaxf(most, l[i]);
   most = block_most<kThreads>(most, red);
   if (!has_place(most)) return pick_none(a, row);
   const Grid g = grid_of(most, st.c);
-  Binner bins(s.count, s.mass);
-  for (int i = tid; i < a.vocab; i += kThreads) bins.add(l[i], st.c, g, kUnit, s.tab);
+  Binner bins(s.mass, &rest);
+  for (int i = tid; i < a.vocab; i += kThreads) bins.add(l[i], st.c, g, s.tab);
   bins.finish();
   if (tid == 0) {
     s.row.g = g;
@@ -655,7 +689,11 @@ __global__ __launch_bounds__(kThreads) void sample_whole_kernel(Sample a) {
     s.row.listed = 0;
   }
   __syncthreads();
-  if (tid < kBins) mass[tid] = ldexp((double)s.mass[tid], -kUnit);
+  if (tid < kBins) {
+    s.count[tid] = tid < kBins - 1 ? bin_count(s.mass[tid]) : rest.count;
+    mass[tid] = tid < kBins - 1 ? bin_weight(s.mass[tid]) * bin_end(tid, g, s.tab)
+                                : rest_weight(rest, g);
+  }
   __syncthreads();
   sum_bins(s.count, mass, s.row);
   __syncthreads();
@@ -664,15 +702,13 @@ __global__ __launch_bounds__(kThreads) void sample_whole_kernel(Sample a) {
 
 // ---- long rows --------------------------------------------------------------------
 
-// A chunk's bins, relative to its own largest logit.
+// A chunk's bins, from its own largest logit down.
 struct Chunk {
-  Grid g;     // gmax -inf: no token
+  Grid g;  // gmax -inf: no token
   double zmax;
-  double pad;
-  u64 mass[kBins];
-  uint32_t count[kBins];
+  Rest rest;
+  u64 bins[kBins];
 };
-constexpr int kChunkUnit = 50;  // 2^-50 of the chunk's octave: 4096 of them fit 64 bits
 
 struct Work {
   Chunk *chunks;  // [rows][nchunk]
@@ -694,8 +730,8 @@ __device__ __forceinline__ void load_chunk(const Sample &a, int row, float (&x)[
 
 __global__ __launch_bounds__(kChunkThreads) void sample_bins_kernel(Sample a, Work w) {
   __shared__ double tab[128];
-  __shared__ uint32_t count[kBins];
-  __shared__ u64 mass[kBins];
+  __shared__ u64 count[kBins];
+  __shared__ Rest rest;
   __shared__ float red[kChunkThreads / 64];
   const int row = blockIdx.y, tid = threadIdx.x;
   float x[kPer];
@@ -703,7 +739,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_bins_kernel(Sample a, Wo
   const double c = octave_scale(a, row);
   exp_tab_load(tab);
   count[tid] = 0;
-  mass[tid] = 0;
+  if (tid == 0) rest = Rest{0, 0};
   float most = -INFINITY;
 #pragma unroll
   for (int e = 0; e < kPer; ++e) most = fmaxf(most, x[e]);
@@ -714,77 +750,108 @@ __global__ __launch_bounds__(kChunkThreads) void sample_bins_kernel(Sample a, Wo
     return;
   }
   const Grid g = grid_of(most, c);
-  Binner bins(count, mass);
+  Binner bins(count, &rest);
 #pragma unroll
-  for (int e = 0; e < kPer; ++e) bins.add(x[e], c, g, kChunkUnit, tab);
+  for (int e = 0; e < kPer; ++e) bins.add(x[e], c, g, tab);
   bins.finish();
   __syncthreads();
-  out->count[tid] = count[tid];
-  out->mass[tid] = mass[tid];
+  out->bins[tid] = count[tid];
   if (tid == 0) {
     out->g = g;
     out->zmax = octaves(most, c);
+    out->rest = rest;
   }
 }
 
-// The chunks' bins summed into the row's.  Thread (bin, part) sums its bin over a
-// quarter of the chunks; a chunk's bins that fall into the row's last one are summed in
-// units.
+// The chunks' bins summed into the row's: thread (bin, part) sums its bin over its part of
+// the chunks.  A chunk's bins that fall into the row's last one are summed in units, as
+// its own last one is.
+constexpr int kMaxChunks = (kSampleMaxVocab + kChunk - 1) / kChunk;
 __global__ __launch_bounds__(kThreads) void sample_decide_kernel(Sample a, Work w, int nchunk) {
-  constexpr int kParts = kThreads / kBins;
+  constexpr int kParts = kThreads / kBins, kAhead = 8;
+  static_assert(kMaxChunks <= 64, "a lane per chunk");
   __shared__ Row r;
+  __shared__ double tab[128];
   __shared__ uint32_t count[kBins];
   __shared__ double mass[kParts][kBins];
-  __shared__ u64 rest;
-  __shared__ double zred[kThreads / 64];
+  __shared__ Rest rest;
+  __shared__ int shift[64];
   const int row = blockIdx.x, tid = threadIdx.x, bin = tid % kBins, part = tid / kBins;
+  const int lane = tid & 63;
   const Chunk *ch = w.chunks + (size_t)row * nchunk;
-  double z = -INFINITY;
-  for (int c = tid; c < nchunk; c += kThreads)
-    if (ch[c].g.gmax > -INFINITY) z = fmax(z, ch[c].zmax);
+  exp_tab_load(tab);
+  const Chunk *mine = ch + min(lane, nchunk - 1);
+  const double gm = mine->g.gmax;
+  double z = gm > -INFINITY ? mine->zmax : -INFINITY;
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) z = fmax(z, __shfl_xor(z, off, 64));
-  if ((tid & 63) == 0) zred[tid >> 6] = z;
-  if (tid < kBins) count[tid] = 0;
-  if (tid == 0) rest = 0;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kThreads / 64; ++i) z = fmax(z, zred[i]);
   Row *out = w.rows + row;
   if (!(z > -INFINITY)) {
     if (tid == 0) out->zmax = -INFINITY;
     return;
   }
   const Grid g{floor(z * kPerOctave), ceil(z)};
-  uint32_t n = 0, rest_n = 0;
+  // chunks without a token, and past the last, are shifted out
+  if (tid < 64)
+    shift[tid] = tid < nchunk && gm > -INFINITY ? (int)fmin(g.gmax - gm, (double)kBins) : 2 * kBins;
+  if (tid < kBins) count[tid] = 0;
+  if (tid == 0) rest = Rest{0, 0};
+  __syncthreads();
+  uint32_t n = 0;
   double m = 0.0;
-  u64 rest_m = 0;
-  for (int c = part; c < nchunk; c += kParts) {
-    const Grid cg = ch[c].g;
-    if (!(cg.gmax > -INFINITY)) continue;
-    const int shift = (int)fmin(g.gmax - cg.gmax, (double)kBins);
-    const int down = (int)fmin(g.e - cg.e, 64.0);
-    if (bin < kBins - 1 && bin >= shift) {
-      n += ch[c].count[bin - shift];
-      m += ldexp((double)ch[c].mass[bin - shift], -kChunkUnit - down);
-    }
-    if (bin + shift >= kBins - 1) {
-      rest_n += ch[c].count[bin];
-      rest_m += down < 64 ? ch[c].mass[bin] >> down : 0;
+  const int per = (nchunk + kParts - 1) / kParts, c0 = part * per, c1 = min(nchunk, c0 + per);
+  for (int c = c0; c < c1; c += kAhead) {
+    u64 b[kAhead];
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e)
+      b[e] = ch[min(c + e, nchunk - 1)].bins[max(bin - shift[min(c + e, 63)], 0)];
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) {
+      if (c + e >= c1 || bin < shift[c + e] || bin >= kBins - 1) continue;
+      n += bin_count(b[e]);
+      m += bin_weight(b[e]);
     }
   }
   mass[part][bin] = m;
   if (n != 0) atomicAdd(&count[bin], n);
-  if (rest_n != 0) {
-    atomicAdd(&count[kBins - 1], rest_n);
-    atomicAdd(&rest, rest_m);
+  // the last bin: one chunk a wave
+  const double top = bin_top(kBins - 1, g);
+  for (int c = tid >> 6; c < nchunk; c += kThreads / 64) {
+    if (shift[c] > kBins) continue;
+    uint32_t rc = 0;
+    u64 rm = 0;
+    const Grid cg = ch[c].g;
+    for (int i = kBins - 1 - shift[c] + lane; i < kBins - 1; i += 64) {
+      if (i < 0) continue;
+      const u64 b = ch[c].bins[i];
+      const double end = (cg.gmax - i) * (1.0 / kPerOctave) - top;
+      rc += bin_count(b);
+      // (more than units() takes: up to 2^14 weights)
+      if (end > -64.0) rm += (u64)rint(ldexp(bin_weight(b) * pow2(end, tab), kUnit));
+    }
+    if (lane == 0) {
+      const Rest cr = ch[c].rest;
+      const double down = top - bin_top(kBins - 1, cg);
+      rc += cr.count;
+      rm += down < 64.0 ? cr.mass >> (int)down : 0;
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+      rc += __shfl_xor(rc, off, 64);
+      rm += __shfl_xor(rm, off, 64);
+    }
+    if (lane == 0 && rc != 0) {
+      atomicAdd(&rest.count, rc);
+      atomicAdd(&rest.mass, rm);
+    }
   }
   __syncthreads();
   if (tid < kBins) {
     double sum = mass[0][tid];
 #pragma unroll
     for (int i = 1; i < kParts; ++i) sum += mass[i][tid];
-    mass[0][tid] = tid < kBins - 1 ? sum : ldexp((double)rest, -kChunkUnit);
+    mass[0][tid] = tid < kBins - 1 ? sum * bin_end(tid, g, tab) : rest_weight(rest, g);
+    if (tid == kBins - 1) count[tid] = rest.count;
   }
   if (tid == 0) {
     r.g = g;
@@ -813,7 +880,8 @@ __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(Sample a,
   __syncthreads();
   // whether the chunk has any of them
   const int shift = (int)fmin(g.gmax - cmax, (double)kBins);
-  const bool here = ch->count[tid] != 0 && at[min(tid + shift, kBins - 1)] != kNone;
+  const bool here = (tid < kBins - 1 ? bin_count(ch->bins[tid]) : ch->rest.count) != 0 &&
+                    at[min(tid + shift, kBins - 1)] != kNone;
   if (!__syncthreads_or(here)) return;
   float x[kPer];
   load_chunk(a, row, x);
