@@ -134,6 +134,8 @@ __device__ __forceinline__ double bin_top(int bin, const Grid &g) {
   return ceil((g.gmax - bin + 1.0) / kPerOctave);
 }
 
+constexpr uint32_t kNone = ~0u;
+constexpr int kPerLane = kBins / 64;
 // A row's bins, running sums from the largest logits down, and where the tokens of
 // the bins that matter have been collected.
 struct Row {
@@ -143,43 +145,55 @@ struct Row {
   uint32_t sum_c[kBins];  // ... and count, each bin's own included
   uint32_t at[kBins];     // list position of the bin's tokens, kNone: not collected
   uint32_t fill[kBins];   // tokens of the bin in the list so far
-  uint32_t listed;        // whether the bins that matter fit the list
+  uint32_t listed;        // tokens of the bins that matter, kNone: more than the list takes
   uint32_t pad;
   __device__ double weight(int i) const { return __longlong_as_double((long long)sum_m[i]); }
   __device__ double weight_before(int i) const { return i > 0 ? weight(i - 1) : 0.0; }
   __device__ uint32_t count_before(int i) const { return i > 0 ? sum_c[i - 1] : 0u; }
   __device__ uint32_t count_of(int i) const { return sum_c[i] - count_before(i); }
 };
-constexpr uint32_t kNone = ~0u;
-constexpr int kPerLane = kBins / 64;
 
-// The first bin with tokens for which f holds, the last one with tokens if none: by
-// each wave on its own.
-template <class F>
-__device__ __forceinline__ int first_bin(const Row &r, F &&f) {
-  const int lane = threadIdx.x & 63;
-  int hit = kBins, some = -1;
+// A row's running sums, a lane's bins in its registers: each wave searches them alone.
+struct Bins {
+  uint32_t before, c[kPerLane];  // count before the lane's bins, and up to each
+  double w[kPerLane];
+  __device__ __forceinline__ explicit Bins(const Row &r) {
+    const int lane = threadIdx.x & 63;
+    before = r.count_before(kPerLane * lane);
 #pragma unroll
-  for (int e = kPerLane - 1; e >= 0; --e) {
-    const int i = kPerLane * lane + e;
-    if (r.count_of(i) == 0) continue;
-    some = max(some, i);
-    if (f(i)) hit = i;
+    for (int e = 0; e < kPerLane; ++e) {
+      c[e] = r.sum_c[kPerLane * lane + e];
+      w[e] = r.weight(kPerLane * lane + e);
+    }
   }
-  const u64 any = __ballot(hit < kBins), full = __ballot(some >= 0);
-  if (any != 0) return __shfl(hit, __ffsll(any) - 1, 64);
-  return full != 0 ? __shfl(some, 63 - __clzll(full), 64) : 0;
-}
-
-__device__ __forceinline__ int bin_by_weight(const Row &r, double target) {
-  return first_bin(r, [&](int i) { return r.weight(i) >= target; });
-}
-__device__ __forceinline__ int bin_past_weight(const Row &r, double target) {
-  return first_bin(r, [&](int i) { return r.weight(i) > target; });
-}
-__device__ __forceinline__ int bin_by_count(const Row &r, uint32_t target) {
-  return first_bin(r, [&](int i) { return r.sum_c[i] >= target; });
-}
+  // the first bin with tokens for which f holds, the last one with tokens if none
+  template <class F>
+  __device__ __forceinline__ int first(F &&f) const {
+    int hit = kPerLane, some = -1;
+#pragma unroll
+    for (int e = kPerLane - 1; e >= 0; --e) {
+      if (c[e] == (e > 0 ? c[e > 0 ? e - 1 : 0] : before)) continue;
+      some = max(some, e);
+      if (f(c[e], w[e])) hit = e;
+    }
+    const u64 any = __ballot(hit < kPerLane), full = __ballot(some >= 0);
+    if (any != 0) {
+      const int l = __ffsll(any) - 1;
+      return kPerLane * l + __shfl(hit, l, 64);
+    }
+    const int l = full != 0 ? 63 - __clzll(full) : 0;
+    return kPerLane * l + max(0, __shfl(some, l, 64));
+  }
+  __device__ __forceinline__ int by_weight(double target) const {
+    return first([&](uint32_t, double x) { return x >= target; });
+  }
+  __device__ __forceinline__ int past_weight(double target) const {
+    return first([&](uint32_t, double x) { return x > target; });
+  }
+  __device__ __forceinline__ int by_count(uint32_t target) const {
+    return first([&](uint32_t x, double) { return x >= target; });
+  }
+};
 // Bins in which min-p's border may lie: [0], the first of them, to [1].
 __device__ __forceinline__ void min_p_bins(const Row &r, double m, int (&b)[2]) {
   const double z = r.zmax + log2(m);
@@ -224,6 +238,7 @@ __device__ void sum_bins(const uint32_t *count, const double *mass, Row &r) {
 __device__ void decide(const Settings &st, Row &r) {
   const int lane = threadIdx.x;
   if (lane >= 64) return;
+  const Bins bins(r);
   const uint32_t n = r.sum_c[kBins - 1];
   bool need[kPerLane] = {};
   auto mark = [&](int lo, int hi) {
@@ -233,7 +248,7 @@ __device__ void decide(const Settings &st, Row &r) {
   int cut_lo = kBins - 1, cut_hi = kBins - 1;
   double s_lo = r.weight(kBins - 1), s_hi = s_lo;
   if (st.k > 0 && (uint32_t)st.k < n) {
-    cut_lo = cut_hi = bin_by_count(r, st.k);
+    cut_lo = cut_hi = bins.by_count(st.k);
     s_hi = r.weight(cut_hi);
     s_lo = r.weight_before(cut_lo);
     if (r.sum_c[cut_hi] == (uint32_t)st.k)
@@ -242,7 +257,7 @@ __device__ void decide(const Settings &st, Row &r) {
       mark(cut_lo, cut_hi);
   }
   if (st.p < 1.0) {
-    const int lo = bin_by_weight(r, st.p * s_lo), hi = bin_by_weight(r, st.p * s_hi);
+    const int lo = bins.by_weight(st.p * s_lo), hi = bins.by_weight(st.p * s_hi);
     mark(min(lo, cut_lo), min(hi, cut_hi));
     cut_lo = min(cut_lo, lo);
     cut_hi = min(cut_hi, hi);
@@ -260,7 +275,7 @@ __device__ void decide(const Settings &st, Row &r) {
       s_hi = fmin(s_hi, r.weight(cut_hi));
     }
   }
-  mark(bin_past_weight(r, st.u * s_lo), min(bin_past_weight(r, st.u * s_hi), cut_hi));
+  mark(bins.past_weight(st.u * s_lo), min(bins.past_weight(st.u * s_hi), cut_hi));
   // list positions
   uint32_t own[kPerLane], sum = 0;
 #pragma unroll
@@ -279,7 +294,7 @@ __device__ void decide(const Settings &st, Row &r) {
     r.at[kPerLane * lane + e] = need[e] ? run - sum + own[e] : kNone;
     r.fill[kPerLane * lane + e] = 0;
   }
-  if (lane == 63) r.listed = run <= kList;
+  if (lane == 63) r.listed = run <= kList ? run : kNone;
 }
 
 // Working memory of pick() and of what it calls.
@@ -307,7 +322,7 @@ struct Found {
 template <class F>
 __device__ __forceinline__ void each_of_bin(const Sample &a, int row, const Settings &st,
                                             const u64 *list, const Row &r, int bin, F &&f) {
-  if (list != nullptr && r.listed && r.at[bin] != kNone) {
+  if (list != nullptr && r.listed != kNone && r.at[bin] != kNone) {
     const uint32_t n = r.count_of(bin);
     for (uint32_t i = threadIdx.x; i < n; i += kThreads) f(list[r.at[bin] + i]);
   } else {
@@ -506,28 +521,108 @@ __device__ Found locate(const Sample &a, int row, const Settings &st, const u64 
   return Found{s.sorted[at], count0 + at, base + s.wred[0], weigh(s.sorted[at]) * ldexp(unit, kUnit)};
 }
 
+// Where a bin's tokens are put in order once for all targets: those of all bins that
+// matter, up to kRanked, in s.sorted with running weights (over all of them) in s.weight.
+__device__ void rank_all(const Sample &a, int row, const Settings &st, const u64 *list, Lds &s) {
+  const Row &r = s.row;
+  const uint32_t n = r.listed, tid = threadIdx.x;
+  if (tid < kRanked) {
+    s.place[tid] = tid < n ? list[tid] : ~0ull;
+    s.count[tid] = 0;
+  }
+  __syncthreads();
+  constexpr uint32_t S = kThreads / kRanked, E = kRanked / S;  // parts of the pairs, tokens of one
+  const uint32_t i = tid % kRanked, q = tid / kRanked;
+  if (i < n && q * E < n) {
+    const u64 mine = s.place[i];
+    uint32_t rank = 0;
+#pragma unroll 8
+    for (uint32_t e = q * E; e < (q + 1) * E; ++e) rank += s.place[e] < mine;
+    atomicAdd(&s.count[i], rank);
+  }
+  __syncthreads();
+  if (tid < n) {
+    const u64 p = s.place[tid];
+    s.sorted[s.count[tid]] = p;
+    s.weight[s.count[tid]] = pow2(octaves(logit_at(p), st.c) - r.g.e, s.tab);
+  } else if (tid < kRanked) {
+    s.weight[tid] = 0.0;
+  }
+  __syncthreads();
+  if (tid < 64) {
+    constexpr int P = kRanked / 64;
+    double w[P], sum = 0.0;
+#pragma unroll
+    for (int e = 0; e < P; ++e) w[e] = sum += s.weight[P * tid + e];
+    double run = sum;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const double t = __shfl_up(run, off, 64);
+      if ((int)tid >= off) run += t;
+    }
+    const double before = __shfl_up(run, 1, 64);
+#pragma unroll
+    for (int e = 0; e < P; ++e) s.weight[P * tid + e] = (tid > 0 ? before : 0.0) + w[e];
+  }
+  __syncthreads();
+}
+
+// locate() among ranked tokens, by each wave alone.
+__device__ __forceinline__ Found locate_ranked(const Settings &st, const Lds &s, int bin,
+                                               bool by_count, double target, bool strict,
+                                               double base) {
+  const Row &r = s.row;
+  const int lane = threadIdx.x & 63;
+  const uint32_t from = r.at[bin], n = r.count_of(bin);
+  const double start = from > 0 ? s.weight[from - 1] : 0.0;
+  uint32_t at = n - 1;
+  if (by_count) {
+    at = min(n, (uint32_t)target) - 1;
+  } else {
+    uint32_t hit = kNone;
+    for (uint32_t i = lane; i < n; i += 64) {
+      const double v = base + (s.weight[from + i] - start);
+      if (strict ? v > target : v >= target) {
+        hit = i;
+        break;
+      }
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) hit = min(hit, (uint32_t)__shfl_xor((int)hit, off, 64));
+    at = min(at, hit);
+  }
+  const u64 p = s.sorted[from + at];
+  return Found{p, at, base + (s.weight[from + at] - start),
+               pow2(octaves(logit_at(p), st.c) - r.g.e, s.tab)};
+}
+
 // The token, from the row's bins.
 __device__ void pick(const Sample &a, int row, const Settings &st, const u64 *list, Lds &s) {
   const Row &r = s.row;
+  const Bins bins(r);
   const uint32_t total = r.sum_c[kBins - 1];
   uint32_t n = total;  // what is kept: so many, weighing so much
   double sum = r.weight(kBins - 1);
+  const bool ranked = list != nullptr && r.listed <= kRanked;
+  if (ranked) rank_all(a, row, st, list, s);
   // sums stay between the bins' own, whatever they were rounded to
   auto within = [&](double w, int bin) { return fmin(fmax(w, r.weight_before(bin)), r.weight(bin)); };
   auto in_bin = [&](int bin, bool by_count, double target, bool strict) {
-    Found f = locate(a, row, st, list, s, bin, by_count, target, strict, r.weight_before(bin));
+    Found f = ranked && r.at[bin] != kNone
+                  ? locate_ranked(st, s, bin, by_count, target, strict, r.weight_before(bin))
+                  : locate(a, row, st, list, s, bin, by_count, target, strict, r.weight_before(bin));
     f.upto = within(f.upto, bin);
     return f;
   };
   if (st.k > 0 && (uint32_t)st.k < n) {
     n = st.k;
-    const int bin = bin_by_count(r, n);
+    const int bin = bins.by_count(n);
     sum = r.sum_c[bin] == n ? r.weight(bin)
                             : in_bin(bin, true, n - r.count_before(bin), false).upto;
   }
   if (st.p < 1.0) {
     const double target = st.p * sum;
-    const int bin = bin_by_weight(r, target);
+    const int bin = bins.by_weight(target);
     const Found f = in_bin(bin, false, target, false);
     const uint32_t np = r.count_before(bin) + f.before + 1;
     if (np < n) {
@@ -539,27 +634,40 @@ __device__ void pick(const Sample &a, int row, const Settings &st, const u64 *li
     int b[2];
     min_p_bins(r, st.m, b);
     for (int bin = b[0]; bin <= b[1] && r.count_before(bin) < n; ++bin) {
-      const double top = bin_top(bin, r.g);
-      const double unit = ldexp(1.0, (int)fmax(top - r.g.e, -1000.0) - kUnit);
-      uint32_t c = 0;
-      u64 w = 0;
-      if (r.count_of(bin) != 0)
+      uint32_t kept = 0;
+      double weight = r.weight_before(bin);
+      const uint32_t in = r.count_of(bin);
+      auto enough = [&](u64 p) {
+        const double z = octaves(logit_at(p), st.c);
+        return z >= r.zmax || pow2(z - r.zmax, s.tab) >= st.m;
+      };
+      if (in != 0 && ranked && r.at[bin] != kNone) {
+        const uint32_t from = r.at[bin];
+        for (uint32_t i = threadIdx.x & 63; i < (in + 63) / 64 * 64; i += 64)
+          kept += __popcll(__ballot(i < in && enough(s.sorted[from + min(i, in - 1)])));
+        if (kept > 0)
+          weight += s.weight[from + kept - 1] - (from > 0 ? s.weight[from - 1] : 0.0);
+      } else if (in != 0) {
+        const double top = bin_top(bin, r.g);
+        const double unit = ldexp(1.0, (int)fmax(top - r.g.e, -1000.0) - kUnit);
+        uint32_t c = 0;
+        u64 w = 0;
         each_of_bin(a, row, st, list, r, bin, [&](u64 p) {
-          const double z = octaves(logit_at(p), st.c);
-          if (z < r.zmax && pow2(z - r.zmax, s.tab) < st.m) return;
+          if (!enough(p)) return;
           ++c;
-          w += units(pow2(z - top, s.tab), kUnit);
+          w += units(pow2(octaves(logit_at(p), st.c) - top, s.tab), kUnit);
         });
-      __syncthreads();
-      if (threadIdx.x == 0) s.red[0] = s.red[1] = 0;
-      __syncthreads();
-      atomicAdd(&s.red[0], (u64)c);
-      atomicAdd(&s.red[1], w);
-      __syncthreads();
-      const uint32_t kept = (uint32_t)s.red[0];
-      const double weight = r.weight_before(bin) + (double)s.red[1] * unit;
-      __syncthreads();
-      if (kept == r.count_of(bin) && bin < b[1]) continue;
+        __syncthreads();
+        if (threadIdx.x == 0) s.red[0] = s.red[1] = 0;
+        __syncthreads();
+        atomicAdd(&s.red[0], (u64)c);
+        atomicAdd(&s.red[1], w);
+        __syncthreads();
+        kept = (uint32_t)s.red[0];
+        weight += (double)s.red[1] * unit;
+        __syncthreads();
+      }
+      if (kept == in && bin < b[1]) continue;
       if (r.count_before(bin) + kept < n) {  // at least the largest logit is
         n = r.count_before(bin) + kept;
         sum = within(weight, bin);
@@ -568,9 +676,7 @@ __device__ void pick(const Sample &a, int row, const Settings &st, const u64 *li
     }
   }
   const double target = st.u * sum;
-  int bin = bin_past_weight(r, target);
-  const int last = bin_by_count(r, n);
-  bin = min(bin, last);
+  const int bin = min(bins.past_weight(target), bins.by_count(n));
   Found f = in_bin(bin, false, target, true);
   if (r.count_before(bin) + f.before + 1 > n)  // by a rounding: the last one kept
     f = in_bin(bin, true, n - r.count_before(bin), false);
@@ -599,17 +705,21 @@ __device__ float block_most(float v, float *red) {
   return m;
 }
 
-// 2^x - 1 in units of 2^-kFrac, 0 <= x < 1/16: the Taylor polynomial (what it leaves out
-// is below 2^-51).
-__device__ __forceinline__ u64 fraction(double x) {
-  const double y = x * 0x1.62e42fefa39efp-1;
-  double p = fma(y, 1.0 / 5040.0, 1.0 / 720.0);
-  p = fma(y, p, 1.0 / 120.0);
-  p = fma(y, p, 1.0 / 24.0);
-  p = fma(y, p, 1.0 / 6.0);
-  p = fma(y, p, 0.5);
-  p = fma(y, p, 1.0);
-  return units(y * p, kFrac);
+// What a token r of a bin's width above the bin's lower end adds to the bin's sum: 1 and
+// 2^(r / 16) - 1 in units of 2^-kFrac, by its Taylor polynomial (what it leaves out is below
+// 2^-43), whose coefficients hold the units and whose last step rounds to a whole number.
+__device__ __forceinline__ u64 bin_term(double r) {
+  constexpr double q = 0x1.62e42fefa39efp-5;  // ln 2 / 16
+  constexpr double unit = (double)(1ull << kFrac);
+  constexpr double c1 = q * unit, c2 = c1 * q / 2.0, c3 = c2 * q / 3.0, c4 = c3 * q / 4.0,
+                   c5 = c4 * q / 5.0, c6 = c5 * q / 6.0;
+  double p = fma(r, c6, c5);
+  p = fma(r, p, c4);
+  p = fma(r, p, c3);
+  p = fma(r, p, c2);
+  p = fma(r, p, c1);
+  p = fma(r, p, 0x1p52);
+  return ((u64)__double_as_longlong(p) & ((1ull << kCountAt) - 1)) | 1ull << kCountAt;
 }
 
 // Counts and weighs tokens into bins; the last bin's, which most tokens of a peaked
@@ -629,7 +739,7 @@ struct Binner {
     if (!has_place(l)) return;
     const double z = octaves(l, c), y = z * kPerOctave, f = floor(y), d = g.gmax - f;
     if (d < kBins - 1) {
-      atomicAdd(&bins[(int)d], (1ull << kCountAt) + fraction((y - f) * (1.0 / kPerOctave)));
+      atomicAdd(&bins[(int)d], bin_term(y - f));
     } else {
       ++rest_c;
       const double x = z - bin_top(kBins - 1, g);
@@ -686,7 +796,7 @@ __global__ __launch_bounds__(kThreads) void sample_whole_kernel(Sample a) {
   if (tid == 0) {
     s.row.g = g;
     s.row.zmax = octaves(most, st.c);
-    s.row.listed = 0;
+    s.row.listed = kNone;
   }
   __syncthreads();
   if (tid < kBins) {
@@ -780,6 +890,7 @@ __global__ __launch_bounds__(kThreads) void sample_decide_kernel(Sample a, Work 
   const int lane = tid & 63;
   const Chunk *ch = w.chunks + (size_t)row * nchunk;
   exp_tab_load(tab);
+  const Settings st = settings(a, row);
   const Chunk *mine = ch + min(lane, nchunk - 1);
   const double gm = mine->g.gmax;
   double z = gm > -INFINITY ? mine->zmax : -INFINITY;
@@ -860,7 +971,7 @@ __global__ __launch_bounds__(kThreads) void sample_decide_kernel(Sample a, Work 
   __syncthreads();
   sum_bins(count, mass[0], r);
   __syncthreads();
-  decide(settings(a, row), r);
+  decide(st, r);
   __syncthreads();
   for (int i = tid; i < (int)(sizeof(Row) / 8); i += kThreads) ((u64 *)out)[i] = ((u64 *)&r)[i];
 }
@@ -874,7 +985,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(Sample a,
   const Chunk *ch = w.chunks + (size_t)row * gridDim.x + blockIdx.x;
   const Grid g = r->g;
   const double cmax = ch->g.gmax;
-  if (!(r->zmax > -INFINITY) || !(cmax > -INFINITY) || !r->listed) return;
+  if (!(r->zmax > -INFINITY) || !(cmax > -INFINITY) || r->listed == kNone) return;
   at[tid] = r->at[tid];
   count[tid] = 0;
   __syncthreads();
@@ -913,12 +1024,13 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(Sample a, Work w)
   __shared__ Lds s;
   const int row = blockIdx.x, tid = threadIdx.x;
   const Row *r = w.rows + row;
+  const Settings st = settings(a, row);
   if (!(r->zmax > -INFINITY)) return pick_none(a, row);
   exp_tab_load(s.tab);
   for (int i = tid; i < (int)(sizeof(Row) / 8); i += kThreads)
     ((u64 *)&s.row)[i] = ((const u64 *)r)[i];
   __syncthreads();
-  pick(a, row, settings(a, row), w.list + (size_t)row * kList, s);
+  pick(a, row, st, w.list + (size_t)row * kList, s);
 }
 
 static_assert(sizeof(Row) % 8 == 0 && kBins == kChunkThreads, "layout");
