@@ -136,21 +136,25 @@ __device__ __forceinline__ double bin_top(int bin, const Grid &g) {
 
 constexpr uint32_t kNone = ~0u;
 constexpr int kPerLane = kBins / 64;
+// Arrays of which a lane reads neighbouring entries have a gap after every eight: without
+// them all lanes would meet in one LDS bank.
+__device__ __forceinline__ constexpr int gap(int i) { return i + (i >> 3); }
+constexpr int kBinsGap = kBins + kBins / 8, kSubsGap = kSubs + kSubs / 8;
 // A row's bins, running sums from the largest logits down, and where the tokens of
 // the bins that matter have been collected.
 struct Row {
   Grid g;
   double zmax;
-  u64 sum_m[kBins];  // (doubles) running weight ...
-  uint32_t sum_c[kBins];  // ... and count, each bin's own included
-  uint32_t at[kBins];     // list position of the bin's tokens, kNone: not collected
-  uint32_t fill[kBins];   // tokens of the bin in the list so far
+  u64 sum_m[kBinsGap];       // (doubles) running weight ...
+  uint32_t sum_c[kBinsGap];  // ... and count, each bin's own included
+  uint32_t at[kBinsGap];     // list position of the bin's tokens, kNone: not collected
+  uint32_t fill[kBinsGap];   // tokens of the bin in the list so far
   uint32_t listed;        // tokens of the bins that matter, kNone: more than the list takes
   uint32_t pad;
-  __device__ double weight(int i) const { return __longlong_as_double((long long)sum_m[i]); }
+  __device__ double weight(int i) const { return __longlong_as_double((long long)sum_m[gap(i)]); }
   __device__ double weight_before(int i) const { return i > 0 ? weight(i - 1) : 0.0; }
-  __device__ uint32_t count_before(int i) const { return i > 0 ? sum_c[i - 1] : 0u; }
-  __device__ uint32_t count_of(int i) const { return sum_c[i] - count_before(i); }
+  __device__ uint32_t count_before(int i) const { return i > 0 ? sum_c[gap(i - 1)] : 0u; }
+  __device__ uint32_t count_of(int i) const { return sum_c[gap(i)] - count_before(i); }
 };
 
 // A row's running sums, a lane's bins in its registers: each wave searches them alone.
@@ -162,7 +166,7 @@ struct Bins {
     before = r.count_before(kPerLane * lane);
 #pragma unroll
     for (int e = 0; e < kPerLane; ++e) {
-      c[e] = r.sum_c[kPerLane * lane + e];
+      c[e] = r.sum_c[gap(kPerLane * lane + e)];
       w[e] = r.weight(kPerLane * lane + e);
     }
   }
@@ -210,8 +214,8 @@ __device__ void sum_bins(const uint32_t *count, const double *mass, Row &r) {
   double m[kPerLane], ms = 0.0;
 #pragma unroll
   for (int e = 0; e < kPerLane; ++e) {
-    c[e] = cs += count[kPerLane * lane + e];
-    m[e] = ms += mass[kPerLane * lane + e];
+    c[e] = cs += count[gap(kPerLane * lane + e)];
+    m[e] = ms += mass[gap(kPerLane * lane + e)];
   }
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
@@ -227,8 +231,8 @@ __device__ void sum_bins(const uint32_t *count, const double *mass, Row &r) {
   const double mb = lane > 0 ? before : 0.0;
 #pragma unroll
   for (int e = 0; e < kPerLane; ++e) {
-    r.sum_c[kPerLane * lane + e] = cb + c[e];
-    r.sum_m[kPerLane * lane + e] = (u64)__double_as_longlong(fmin(mb + m[e], ms));
+    r.sum_c[gap(kPerLane * lane + e)] = cb + c[e];
+    r.sum_m[gap(kPerLane * lane + e)] = (u64)__double_as_longlong(fmin(mb + m[e], ms));
   }
 }
 
@@ -239,7 +243,7 @@ __device__ void decide(const Settings &st, Row &r) {
   const int lane = threadIdx.x;
   if (lane >= 64) return;
   const Bins bins(r);
-  const uint32_t n = r.sum_c[kBins - 1];
+  const uint32_t n = r.sum_c[gap(kBins - 1)];
   bool need[kPerLane] = {};
   auto mark = [&](int lo, int hi) {
 #pragma unroll
@@ -251,7 +255,7 @@ __device__ void decide(const Settings &st, Row &r) {
     cut_lo = cut_hi = bins.by_count(st.k);
     s_hi = r.weight(cut_hi);
     s_lo = r.weight_before(cut_lo);
-    if (r.sum_c[cut_hi] == (uint32_t)st.k)
+    if (r.sum_c[gap(cut_hi)] == (uint32_t)st.k)
       s_lo = s_hi;
     else
       mark(cut_lo, cut_hi);
@@ -291,8 +295,8 @@ __device__ void decide(const Settings &st, Row &r) {
   }
 #pragma unroll
   for (int e = 0; e < kPerLane; ++e) {
-    r.at[kPerLane * lane + e] = need[e] ? run - sum + own[e] : kNone;
-    r.fill[kPerLane * lane + e] = 0;
+    r.at[gap(kPerLane * lane + e)] = need[e] ? run - sum + own[e] : kNone;
+    r.fill[gap(kPerLane * lane + e)] = 0;
   }
   if (lane == 63) r.listed = run <= kList ? run : kNone;
 }
@@ -301,8 +305,8 @@ __device__ void decide(const Settings &st, Row &r) {
 struct Lds {
   Row row;
   double tab[128];
-  u64 mass[kSubs];
-  uint32_t count[kSubs];
+  u64 mass[kSubsGap];
+  uint32_t count[kSubsGap];
   u64 place[kRanked], sorted[kRanked];
   double weight[kRanked];
   double wred[kThreads / 64];
@@ -318,13 +322,41 @@ struct Found {
   double upto, own;
 };
 
-// Calls f(place) for the tokens of a bin: from the list, or from the row itself.
+// Where pick() finds the tokens of the bins that matter: in the row's list, of which one
+// bin at a time is brought to LDS; null: in the row alone.
+constexpr int kStaged = 8192;
+struct Source {
+  const u64 *list;
+  u64 *staged;  // LDS
+};
+
+// Brings a bin's tokens to LDS, if they are listed and fit: then true (barriers around it
+// are the caller's).
+__device__ __forceinline__ bool stage(const Source &src, const Row &r, int bin) {
+  constexpr int kAhead = 8;
+  const uint32_t n = r.count_of(bin);
+  if (src.list == nullptr || r.listed == kNone || r.at[gap(bin)] == kNone || n > kStaged) return false;
+  const u64 *from = src.list + r.at[gap(bin)];
+  u64 p[kAhead];
+#pragma unroll
+  for (int e = 0; e < kAhead; ++e) p[e] = from[min(threadIdx.x + e * kThreads, n - 1)];
+#pragma unroll
+  for (int e = 0; e < kAhead; ++e)
+    if (threadIdx.x + e * kThreads < n) src.staged[threadIdx.x + e * kThreads] = p[e];
+  static_assert(kAhead * kThreads == kStaged, "all of it");
+  return true;
+}
+
+// Calls f(place) for the tokens of a bin.
 template <class F>
 __device__ __forceinline__ void each_of_bin(const Sample &a, int row, const Settings &st,
-                                            const u64 *list, const Row &r, int bin, F &&f) {
-  if (list != nullptr && r.listed != kNone && r.at[bin] != kNone) {
-    const uint32_t n = r.count_of(bin);
-    for (uint32_t i = threadIdx.x; i < n; i += kThreads) f(list[r.at[bin] + i]);
+                                            const Source &src, const Row &r, int bin, bool staged,
+                                            F &&f) {
+  const uint32_t n = r.count_of(bin);
+  if (staged) {
+    for (uint32_t i = threadIdx.x; i < n; i += kThreads) f(src.staged[i]);
+  } else if (src.list != nullptr && r.listed != kNone && r.at[gap(bin)] != kNone) {
+    for (uint32_t i = threadIdx.x; i < n; i += kThreads) f(src.list[r.at[gap(bin)] + i]);
   } else {
     const float *l = a.logits + row * a.stride;
     for (int i = threadIdx.x; i < a.vocab; i += kThreads) {
@@ -336,7 +368,8 @@ __device__ __forceinline__ void each_of_bin(const Sample &a, int row, const Sett
 
 // The first part of an array of counts and weights (units) at which the running count
 // or weight reaches the target, or the last that isn't empty: into red[] as part,
-// count before, weight before.  By wave 0; barriers around it are the caller's.
+// count before, weight before.  By wave 0, first over N / 64 parts a lane, then over those
+// of the lane found, one each; barriers around it are the caller's.
 template <int N>
 __device__ void find_part(Lds &s, bool by_count, double target, bool strict, double unit,
                           uint32_t count0, u64 mass0) {
@@ -345,48 +378,40 @@ __device__ void find_part(Lds &s, bool by_count, double target, bool strict, dou
   constexpr int P = N / 64;
   uint32_t c = 0;
   u64 m = 0;
+#pragma unroll
   for (int e = 0; e < P; ++e) {
-    c += s.count[P * lane + e];
-    m += s.mass[P * lane + e];
+    c += s.count[gap(P * lane + e)];
+    m += s.mass[gap(P * lane + e)];
   }
-  uint32_t cs = c;
-  u64 ms = m;
-  for (int off = 1; off < 64; off <<= 1) {
-    const uint32_t ct = __shfl_up(cs, off, 64);
-    const u64 mt = __shfl_up(ms, off, 64);
-    if (lane >= off) {
-      cs += ct;
-      ms += mt;
-    }
-  }
-  cs += count0 - c;  // before this lane's parts
-  ms += mass0 - m;
-  int hit = -1, some = -1;
-  uint32_t hc = 0, sc = 0;
-  u64 hm = 0, sm = 0;
-  for (int e = 0; e < P; ++e) {
-    const uint32_t ce = s.count[P * lane + e];
-    const u64 me = s.mass[P * lane + e];
-    if (ce != 0) {
-      some = P * lane + e;
-      sc = cs;
-      sm = ms;
-      const double v = by_count ? (double)(cs + ce) : (double)(ms + me) * unit;
-      if (hit < 0 && (strict ? v > target : v >= target)) {
-        hit = some;
-        hc = cs;
-        hm = ms;
+  // the lane found; then c and m are the sums before its own
+  auto first = [&]() {
+    uint32_t cs = c;
+    u64 ms = m;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const uint32_t ct = __shfl_up(cs, off, 64);
+      const u64 mt = __shfl_up(ms, off, 64);
+      if (lane >= off) {
+        cs += ct;
+        ms += mt;
       }
     }
-    cs += ce;
-    ms += me;
-  }
-  const u64 hits = __ballot(hit >= 0), somes = __ballot(some >= 0);
-  const int who = hits ? __ffsll(hits) - 1 : somes ? 63 - __clzll(somes) : 0;
-  if (lane == who) {
-    s.red[0] = hits ? hit : some < 0 ? 0 : some;
-    s.red[1] = hits ? hc : sc;
-    s.red[2] = hits ? hm : sm;
+    const double v = by_count ? (double)(count0 + cs) : (double)(mass0 + ms) * unit;
+    const u64 some = __ballot(c != 0);
+    const u64 hits = __ballot(c != 0 && (strict ? v > target : v >= target));
+    const int who = hits ? __ffsll(hits) - 1 : some ? 63 - __clzll(some) : 0;
+    count0 += __shfl(cs - c, who, 64);
+    mass0 += __shfl(ms - m, who, 64);
+    return who;
+  };
+  const int lot = first();
+  c = lane < P ? s.count[gap(P * lot + lane % P)] : 0;
+  m = lane < P ? s.mass[gap(P * lot + lane % P)] : 0;
+  const int at = first();
+  if (lane == 0) {
+    s.red[0] = P * lot + at;
+    s.red[1] = count0;
+    s.red[2] = mass0;
   }
 }
 
@@ -396,7 +421,7 @@ __device__ void find_part(Lds &s, bool by_count, double target, bool strict, dou
 //  - Up to 256 tokens: all pairs compared.
 //  - More: counted and weighed in 1024 parts of the bin, then the part's tokens.
 //  - Where a part has more than that (equal logits): digit by digit of the place.
-__device__ Found locate(const Sample &a, int row, const Settings &st, const u64 *list, Lds &s,
+__device__ Found locate(const Sample &a, int row, const Settings &st, const Source &src, Lds &s,
                         int bin, bool by_count, double target, bool strict, double base) {
   const Row &r = s.row;
   const int tid = threadIdx.x;
@@ -404,6 +429,8 @@ __device__ Found locate(const Sample &a, int row, const Settings &st, const u64 
   const double unit = ldexp(1.0, (int)fmax(top - r.g.e, -1000.0) - kUnit);
   if (!by_count) target -= base;
   auto weigh = [&](u64 p) { return pow2(octaves(logit_at(p), st.c) - top, s.tab); };
+  // the part of the bin that a token falls into: any that falls as logits rise does; of the
+  // last bin, 1/16 octave each
   const double edge = r.g.gmax - bin;  // 16 z of the bin's lower end
   auto part = [&](u64 p) {
     const double y = octaves(logit_at(p), st.c) * kPerOctave - edge;  // in [0, 1); the last: < 1
@@ -415,11 +442,12 @@ __device__ Found locate(const Sample &a, int row, const Settings &st, const u64 
   u64 mass0 = 0;
   uint32_t n = r.count_of(bin);
   __syncthreads();
+  const bool staged = stage(src, r, bin);
   if (n > kRanked) {
-    for (int i = tid; i < kSubs; i += kThreads) s.count[i] = s.mass[i] = 0;
+    for (int i = tid; i < kSubsGap; i += kThreads) s.count[i] = s.mass[i] = 0;
     __syncthreads();
-    each_of_bin(a, row, st, list, r, bin, [&](u64 p) {
-      const int i = part(p);
+    each_of_bin(a, row, st, src, r, bin, staged, [&](u64 p) {
+      const int i = gap(part(p));
       atomicAdd(&s.count[i], 1u);
       atomicAdd(&s.mass[i], units(weigh(p), kUnit));
     });
@@ -429,17 +457,17 @@ __device__ Found locate(const Sample &a, int row, const Settings &st, const u64 
     only = (int)s.red[0];
     count0 = (uint32_t)s.red[1];
     mass0 = s.red[2];
-    n = s.count[only];
+    n = s.count[gap(only)];
   }
   if (n > kRanked) {
     u64 prefix = 0;
     for (int shift = 56; shift >= 0; shift -= 8) {
       __syncthreads();
-      for (int i = tid; i < 256; i += kThreads) s.count[i] = s.mass[i] = 0;
+      for (int i = tid; i < gap(256); i += kThreads) s.count[i] = s.mass[i] = 0;
       __syncthreads();
-      each_of_bin(a, row, st, list, r, bin, [&](u64 p) {
+      each_of_bin(a, row, st, src, r, bin, staged, [&](u64 p) {
         if (part(p) != only || (shift < 56 && (p >> (shift + 8)) != prefix)) return;
-        const int d = (int)(p >> shift) & 255;
+        const int d = gap((int)(p >> shift) & 255);
         atomicAdd(&s.count[d], 1u);
         atomicAdd(&s.mass[d], units(weigh(p), kUnit));
       });
@@ -456,8 +484,8 @@ __device__ Found locate(const Sample &a, int row, const Settings &st, const u64 
   }
   // gather, rank, sum in order
   if (tid == 0) s.n = 0;
-  __syncthreads();
-  each_of_bin(a, row, st, list, r, bin, [&](u64 p) {
+  __syncthreads();  // (what was staged is there, too)
+  each_of_bin(a, row, st, src, r, bin, staged, [&](u64 p) {
     if (only >= 0 && part(p) != only) return;
     const uint32_t i = atomicAdd(&s.n, 1u);
     if (i < kRanked) s.place[i] = p;
@@ -523,11 +551,11 @@ __device__ Found locate(const Sample &a, int row, const Settings &st, const u64 
 
 // Where a bin's tokens are put in order once for all targets: those of all bins that
 // matter, up to kRanked, in s.sorted with running weights (over all of them) in s.weight.
-__device__ void rank_all(const Sample &a, int row, const Settings &st, const u64 *list, Lds &s) {
+__device__ void rank_all(const Settings &st, u64 mine_, Lds &s) {
   const Row &r = s.row;
   const uint32_t n = r.listed, tid = threadIdx.x;
   if (tid < kRanked) {
-    s.place[tid] = tid < n ? list[tid] : ~0ull;
+    s.place[tid] = tid < n ? mine_ : ~0ull;
     s.count[tid] = 0;
   }
   __syncthreads();
@@ -573,7 +601,7 @@ __device__ __forceinline__ Found locate_ranked(const Settings &st, const Lds &s,
                                                double base) {
   const Row &r = s.row;
   const int lane = threadIdx.x & 63;
-  const uint32_t from = r.at[bin], n = r.count_of(bin);
+  const uint32_t from = r.at[gap(bin)], n = r.count_of(bin);
   const double start = from > 0 ? s.weight[from - 1] : 0.0;
   uint32_t at = n - 1;
   if (by_count) {
@@ -597,28 +625,31 @@ __device__ __forceinline__ Found locate_ranked(const Settings &st, const Lds &s,
 }
 
 // The token, from the row's bins.
-__device__ void pick(const Sample &a, int row, const Settings &st, const u64 *list, Lds &s) {
+// listed: the list's threadIdx.x-th.
+__device__ void pick(const Sample &a, int row, const Settings &st, const Source &src, u64 listed,
+                     Lds &s) {
   const Row &r = s.row;
   const Bins bins(r);
-  const uint32_t total = r.sum_c[kBins - 1];
+  const uint32_t total = r.sum_c[gap(kBins - 1)];
   uint32_t n = total;  // what is kept: so many, weighing so much
   double sum = r.weight(kBins - 1);
-  const bool ranked = list != nullptr && r.listed <= kRanked;
-  if (ranked) rank_all(a, row, st, list, s);
+  const bool ranked = src.list != nullptr && r.listed <= kRanked;
+  if (ranked) rank_all(st, listed, s);
   // sums stay between the bins' own, whatever they were rounded to
   auto within = [&](double w, int bin) { return fmin(fmax(w, r.weight_before(bin)), r.weight(bin)); };
   auto in_bin = [&](int bin, bool by_count, double target, bool strict) {
-    Found f = ranked && r.at[bin] != kNone
-                  ? locate_ranked(st, s, bin, by_count, target, strict, r.weight_before(bin))
-                  : locate(a, row, st, list, s, bin, by_count, target, strict, r.weight_before(bin));
+    const double base = r.weight_before(bin);
+    Found f = ranked && r.at[gap(bin)] != kNone
+                  ? locate_ranked(st, s, bin, by_count, target, strict, base)
+                  : locate(a, row, st, src, s, bin, by_count, target, strict, base);
     f.upto = within(f.upto, bin);
     return f;
   };
   if (st.k > 0 && (uint32_t)st.k < n) {
     n = st.k;
     const int bin = bins.by_count(n);
-    sum = r.sum_c[bin] == n ? r.weight(bin)
-                            : in_bin(bin, true, n - r.count_before(bin), false).upto;
+    sum = r.sum_c[gap(bin)] == n ? r.weight(bin)
+                                 : in_bin(bin, true, n - r.count_before(bin), false).upto;
   }
   if (st.p < 1.0) {
     const double target = st.p * sum;
@@ -641,8 +672,8 @@ __device__ void pick(const Sample &a, int row, const Settings &st, const u64 *li
         const double z = octaves(logit_at(p), st.c);
         return z >= r.zmax || pow2(z - r.zmax, s.tab) >= st.m;
       };
-      if (in != 0 && ranked && r.at[bin] != kNone) {
-        const uint32_t from = r.at[bin];
+      if (in != 0 && ranked && r.at[gap(bin)] != kNone) {
+        const uint32_t from = r.at[gap(bin)];
         for (uint32_t i = threadIdx.x & 63; i < (in + 63) / 64 * 64; i += 64)
           kept += __popcll(__ballot(i < in && enough(s.sorted[from + min(i, in - 1)])));
         if (kept > 0)
@@ -652,7 +683,7 @@ __device__ void pick(const Sample &a, int row, const Settings &st, const u64 *li
         const double unit = ldexp(1.0, (int)fmax(top - r.g.e, -1000.0) - kUnit);
         uint32_t c = 0;
         u64 w = 0;
-        each_of_bin(a, row, st, list, r, bin, [&](u64 p) {
+        each_of_bin(a, row, st, src, r, bin, false, [&](u64 p) {
           if (!enough(p)) return;
           ++c;
           w += units(pow2(octaves(logit_at(p), st.c) - top, s.tab), kUnit);
@@ -676,10 +707,13 @@ __device__ void pick(const Sample &a, int row, const Settings &st, const u64 *li
     }
   }
   const double target = st.u * sum;
-  const int bin = min(bins.past_weight(target), bins.by_count(n));
+  int bin = min(bins.past_weight(target), bins.by_count(n));
   Found f = in_bin(bin, false, target, true);
-  if (r.count_before(bin) + f.before + 1 > n)  // by a rounding: the last one kept
+  // where a rounding took the draw past the last token kept
+  if (r.count_before(bin) + f.before + 1 > n) {
+    bin = bins.by_count(n);
     f = in_bin(bin, true, n - r.count_before(bin), false);
+  }
   if (threadIdx.x == 0) {
     a.tokens[row] = (int)(uint32_t)f.place;
     if (a.probs != nullptr) a.probs[row] = (float)(f.own / sum);
@@ -777,7 +811,7 @@ __device__ __forceinline__ double bin_end(int bin, const Grid &g, const double *
 __global__ __launch_bounds__(kThreads) void sample_whole_kernel(Sample a) {
   __shared__ Lds s;
   __shared__ float red[kThreads / 64];
-  __shared__ double mass[kBins];
+  __shared__ double mass[kBinsGap];
   __shared__ Rest rest;
   const int row = blockIdx.x, tid = threadIdx.x;
   const float *l = a.logits + row * a.stride;
@@ -786,12 +820,21 @@ __global__ __launch_bounds__(kThreads) void sample_whole_kernel(Sample a) {
   if (tid < kBins) s.mass[tid] = 0;
   if (tid == 0) rest = Rest{0, 0};
   float most = -INFINITY;
-  for (int i = tid; i < a.vocab; i += kThreads) most = fmaxf(most, l[i]);
+  constexpr int kWhole = kWholeVocab / kThreads;
+  float x[kWhole];
+#pragma unroll
+  for (int e = 0; e < kWhole; ++e) {
+    x[e] = l[min(tid + e * kThreads, a.vocab - 1)];
+    if (tid + e * kThreads >= a.vocab) x[e] = -INFINITY;
+  }
+#pragma unroll
+  for (int e = 0; e < kWhole; ++e) most = fmaxf(most, x[e]);
   most = block_most<kThreads>(most, red);
   if (!has_place(most)) return pick_none(a, row);
   const Grid g = grid_of(most, st.c);
   Binner bins(s.mass, &rest);
-  for (int i = tid; i < a.vocab; i += kThreads) bins.add(l[i], st.c, g, s.tab);
+#pragma unroll
+  for (int e = 0; e < kWhole; ++e) bins.add(x[e], st.c, g, s.tab);
   bins.finish();
   if (tid == 0) {
     s.row.g = g;
@@ -800,14 +843,14 @@ __global__ __launch_bounds__(kThreads) void sample_whole_kernel(Sample a) {
   }
   __syncthreads();
   if (tid < kBins) {
-    s.count[tid] = tid < kBins - 1 ? bin_count(s.mass[tid]) : rest.count;
-    mass[tid] = tid < kBins - 1 ? bin_weight(s.mass[tid]) * bin_end(tid, g, s.tab)
-                                : rest_weight(rest, g);
+    s.count[gap(tid)] = tid < kBins - 1 ? bin_count(s.mass[tid]) : rest.count;
+    mass[gap(tid)] = tid < kBins - 1 ? bin_weight(s.mass[tid]) * bin_end(tid, g, s.tab)
+                                     : rest_weight(rest, g);
   }
   __syncthreads();
   sum_bins(s.count, mass, s.row);
   __syncthreads();
-  pick(a, row, st, nullptr, s);
+  pick(a, row, st, Source{nullptr, nullptr}, 0, s);
 }
 
 // ---- long rows --------------------------------------------------------------------
@@ -873,27 +916,39 @@ __global__ __launch_bounds__(kChunkThreads) void sample_bins_kernel(Sample a, Wo
   }
 }
 
-// The chunks' bins summed into the row's: thread (bin, part) sums its bin over its part of
-// the chunks.  A chunk's bins that fall into the row's last one are summed in units, as
-// its own last one is.
+// The chunks' bins summed into the row's: thread (bin, part) takes one bin of each chunk of
+// its part, all loaded before the row's largest logit is known.  Counts and fractions are
+// whole numbers and their sums exact in any order; so are those of bins that fall into
+// the row's last one, in units.
 constexpr int kMaxChunks = (kSampleMaxVocab + kChunk - 1) / kChunk;
 __global__ __launch_bounds__(kThreads) void sample_decide_kernel(Sample a, Work w, int nchunk) {
-  constexpr int kParts = kThreads / kBins, kAhead = 8;
+  constexpr int kParts = kThreads / kBins, kAhead = 16;
   static_assert(kMaxChunks <= 64, "a lane per chunk");
   __shared__ Row r;
-  __shared__ double tab[128];
-  __shared__ uint32_t count[kBins];
-  __shared__ double mass[kParts][kBins];
+  __shared__ double tab[128], mass[kBinsGap];
+  __shared__ uint32_t count[kBinsGap];
+  __shared__ u64 frac[kBins];
   __shared__ Rest rest;
-  __shared__ int shift[64];
-  const int row = blockIdx.x, tid = threadIdx.x, bin = tid % kBins, part = tid / kBins;
-  const int lane = tid & 63;
+  const int row = blockIdx.x, tid = threadIdx.x, bin = tid % kBins, lane = tid & 63;
+  const int part = __builtin_amdgcn_readfirstlane(tid / kBins);
   const Chunk *ch = w.chunks + (size_t)row * nchunk;
-  exp_tab_load(tab);
+  const Chunk *mine = ch + min(lane, nchunk - 1);  // a lane per chunk
+  const double gm = mine->g.gmax, zm = mine->zmax;
+  const Rest mr = mine->rest;
   const Settings st = settings(a, row);
-  const Chunk *mine = ch + min(lane, nchunk - 1);
-  const double gm = mine->g.gmax;
-  double z = gm > -INFINITY ? mine->zmax : -INFINITY;
+  u64 b[kAhead];
+  auto load = [&](int c) {
+#pragma unroll
+    for (int e = 0; e < kAhead; ++e) b[e] = ch[min(c + kParts * e, nchunk - 1)].bins[bin];
+  };
+  load(part);
+  exp_tab_load(tab);
+  if (tid < kBins) {
+    count[gap(tid)] = 0;
+    frac[tid] = 0;
+  }
+  if (tid == 0) rest = Rest{0, 0};
+  double z = gm > -INFINITY ? zm : -INFINITY;
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) z = fmax(z, __shfl_xor(z, off, 64));
   Row *out = w.rows + row;
@@ -902,74 +957,61 @@ __global__ __launch_bounds__(kThreads) void sample_decide_kernel(Sample a, Work 
     return;
   }
   const Grid g{floor(z * kPerOctave), ceil(z)};
+  const double top = bin_top(kBins - 1, g);
   // chunks without a token, and past the last, are shifted out
-  if (tid < 64)
-    shift[tid] = tid < nchunk && gm > -INFINITY ? (int)fmin(g.gmax - gm, (double)kBins) : 2 * kBins;
-  if (tid < kBins) count[tid] = 0;
-  if (tid == 0) rest = Rest{0, 0};
+  const int shift =
+      lane < nchunk && gm > -INFINITY ? (int)fmin(g.gmax - gm, (double)kBins) : 2 * kBins;
   __syncthreads();
-  uint32_t n = 0;
-  double m = 0.0;
-  const int per = (nchunk + kParts - 1) / kParts, c0 = part * per, c1 = min(nchunk, c0 + per);
-  for (int c = c0; c < c1; c += kAhead) {
-    u64 b[kAhead];
-#pragma unroll
-    for (int e = 0; e < kAhead; ++e)
-      b[e] = ch[min(c + e, nchunk - 1)].bins[max(bin - shift[min(c + e, 63)], 0)];
+  uint32_t rest_n = 0;
+  u64 rest_m = 0;
+  for (int c = part; c < nchunk; c += kParts * kAhead) {
+    if (c != part) load(c);
 #pragma unroll
     for (int e = 0; e < kAhead; ++e) {
-      if (c + e >= c1 || bin < shift[c + e] || bin >= kBins - 1) continue;
-      n += bin_count(b[e]);
-      m += bin_weight(b[e]);
+      const int i = c + kParts * e;
+      if (i >= nchunk || bin >= kBins - 1 || b[e] == 0) continue;
+      const int s = __builtin_amdgcn_readlane(shift, i);
+      if (s > kBins) continue;
+      if (bin + s < kBins - 1) {
+        atomicAdd(&count[gap(bin + s)], bin_count(b[e]));
+        atomicAdd(&frac[bin + s], b[e] & ((1ull << kCountAt) - 1));
+      } else {
+        const double end = (readlane_f64(gm, i) - bin) * (1.0 / kPerOctave) - top;
+        // (more than units() takes: up to 2^14 weights)
+        rest_n += bin_count(b[e]);
+        if (end > -64.0)
+          rest_m += (u64)rint(ldexp(bin_weight(b[e]) * pow2(end, tab), kUnit));
+      }
     }
   }
-  mass[part][bin] = m;
-  if (n != 0) atomicAdd(&count[bin], n);
-  // the last bin: one chunk a wave
-  const double top = bin_top(kBins - 1, g);
-  for (int c = tid >> 6; c < nchunk; c += kThreads / 64) {
-    if (shift[c] > kBins) continue;
-    uint32_t rc = 0;
-    u64 rm = 0;
-    const Grid cg = ch[c].g;
-    for (int i = kBins - 1 - shift[c] + lane; i < kBins - 1; i += 64) {
-      if (i < 0) continue;
-      const u64 b = ch[c].bins[i];
-      const double end = (cg.gmax - i) * (1.0 / kPerOctave) - top;
-      rc += bin_count(b);
-      // (more than units() takes: up to 2^14 weights)
-      if (end > -64.0) rm += (u64)rint(ldexp(bin_weight(b) * pow2(end, tab), kUnit));
-    }
-    if (lane == 0) {
-      const Rest cr = ch[c].rest;
-      const double down = top - bin_top(kBins - 1, cg);
-      rc += cr.count;
-      rm += down < 64.0 ? cr.mass >> (int)down : 0;
-    }
+  if (tid < nchunk && shift <= kBins && mr.count != 0) {
+    const double down = top - ceil((gm - (kBins - 1) + 1.0) / kPerOctave);
+    rest_n += mr.count;
+    rest_m += down < 64.0 ? mr.mass >> (int)down : 0;
+  }
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-      rc += __shfl_xor(rc, off, 64);
-      rm += __shfl_xor(rm, off, 64);
-    }
-    if (lane == 0 && rc != 0) {
-      atomicAdd(&rest.count, rc);
-      atomicAdd(&rest.mass, rm);
-    }
+  for (int off = 32; off > 0; off >>= 1) {
+    rest_n += __shfl_xor(rest_n, off, 64);
+    rest_m += __shfl_xor(rest_m, off, 64);
+  }
+  if (lane == 0 && rest_n != 0) {
+    atomicAdd(&rest.count, rest_n);
+    atomicAdd(&rest.mass, rest_m);
   }
   __syncthreads();
-  if (tid < kBins) {
-    double sum = mass[0][tid];
-#pragma unroll
-    for (int i = 1; i < kParts; ++i) sum += mass[i][tid];
-    mass[0][tid] = tid < kBins - 1 ? sum * bin_end(tid, g, tab) : rest_weight(rest, g);
-    if (tid == kBins - 1) count[tid] = rest.count;
+  if (tid < kBins - 1) {
+    mass[gap(tid)] =
+        ((double)count[gap(tid)] + ldexp((double)frac[tid], -kFrac)) * bin_end(tid, g, tab);
+  } else if (tid == kBins - 1) {
+    mass[gap(tid)] = rest_weight(rest, g);
+    count[gap(tid)] = rest.count;
   }
   if (tid == 0) {
     r.g = g;
     r.zmax = z;
   }
   __syncthreads();
-  sum_bins(count, mass[0], r);
+  sum_bins(count, mass, r);
   __syncthreads();
   decide(st, r);
   __syncthreads();
@@ -986,7 +1028,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(Sample a,
   const Grid g = r->g;
   const double cmax = ch->g.gmax;
   if (!(r->zmax > -INFINITY) || !(cmax > -INFINITY) || r->listed == kNone) return;
-  at[tid] = r->at[tid];
+  at[tid] = r->at[gap(tid)];
   count[tid] = 0;
   __syncthreads();
   // whether the chunk has any of them
@@ -1009,7 +1051,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(Sample a,
     slot[e] = atomicAdd(&count[i], 1u);
   }
   __syncthreads();
-  if (count[tid] != 0) at[tid] += atomicAdd(&r->fill[tid], count[tid]);
+  if (count[tid] != 0) at[tid] += atomicAdd(&r->fill[gap(tid)], count[tid]);
   __syncthreads();
   u64 *list = w.list + (size_t)row * kList;
 #pragma unroll
@@ -1022,15 +1064,24 @@ __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(Sample a,
 
 __global__ __launch_bounds__(kThreads) void sample_pick_kernel(Sample a, Work w) {
   __shared__ Lds s;
+  __shared__ u64 staged[kStaged];
   const int row = blockIdx.x, tid = threadIdx.x;
   const Row *r = w.rows + row;
+  const u64 *list = w.list + (size_t)row * kList;
   const Settings st = settings(a, row);
-  if (!(r->zmax > -INFINITY)) return pick_none(a, row);
+  const u64 listed = list[min(tid, kRanked - 1)];  // before it is known how many there are
+  const double zmax = r->zmax;
+  u64 x[(sizeof(Row) / 8 + kThreads - 1) / kThreads];
+#pragma unroll
+  for (int e = 0; e < (int)(sizeof(x) / 8); ++e)
+    x[e] = ((const u64 *)r)[min(tid + e * kThreads, (int)(sizeof(Row) / 8) - 1)];
   exp_tab_load(s.tab);
-  for (int i = tid; i < (int)(sizeof(Row) / 8); i += kThreads)
-    ((u64 *)&s.row)[i] = ((const u64 *)r)[i];
+  if (!(zmax > -INFINITY)) return pick_none(a, row);
+#pragma unroll
+  for (int e = 0; e < (int)(sizeof(x) / 8); ++e)
+    if (tid + e * kThreads < (int)(sizeof(Row) / 8)) ((u64 *)&s.row)[tid + e * kThreads] = x[e];
   __syncthreads();
-  pick(a, row, st, w.list + (size_t)row * kList, s);
+  pick(a, row, st, Source{list, staged}, listed, s);
 }
 
 static_assert(sizeof(Row) % 8 == 0 && kBins == kChunkThreads, "layout");
