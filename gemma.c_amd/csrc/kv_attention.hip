@@ -39,6 +39,7 @@ namespace gh {
 namespace {
 
 constexpr int kTile = 32;             // keys of a tile
+constexpr int kLongRun = 20;          // tiles by 64 query vectors of a compute unit: see plan()
 constexpr int kStepRows = 16;         // query vectors (rows x heads of a kv head) of a step tile
 constexpr float kFloor = -0x1p55f;    // M of a query that has seen no key
 constexpr float kVsUnit = 0x1p-24f;   // V's scales enter the weights in units of 2^24, so that
@@ -58,7 +59,7 @@ struct KvPlan {
   int step_rows;                // query vectors of a sequence and kv head, at most
   int rows_ns, rows_tpc;        // prompt rows (0 chunks: off)
   int pre_ns, pre_tpc;          // shared prefix (0: none)
-  int qb;                       // 16-query blocks of a wave of the prompt kernel
+  int qb, pre_qb;               // 16-query blocks of a wave of the prompt kernel
   size_t step_o, step_m, rows_o, rows_m, pre_o, pre_m, bytes;  // workspace
 };
 
@@ -958,29 +959,33 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(KvAttn a, KvPlan pl) {
 }
 
 // ---- the chunks' sums together ------------------------------------------------------
-// One workgroup per row and head, its waves sharing out the chunks.
+// SHARE waves take a query vector and share out its chunks; STEP: vectors of single tokens,
+// else of prompt rows, which may have very different numbers of both.  Bound by the partial
+// sums' bytes where there are many vectors.
 
-template <int HD>
-__global__ __launch_bounds__(1024) void kv_merge_kernel(KvAttn a, KvPlan pl) {
-  constexpr int E = HD / 64;
-  __shared__ float so[16][HD], sm[16], sl[16];
-  const int b = blockIdx.z, lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
+constexpr int kMergeWaves = 4;  // of a workgroup, at least
+
+template <int HD, int SHARE, bool STEP>
+__global__ __launch_bounds__(64 * (SHARE > kMergeWaves ? SHARE : kMergeWaves)) void kv_merge_kernel(
+    KvAttn a, KvPlan pl) {
+  constexpr int E = HD / 64, W = SHARE > kMergeWaves ? SHARE : kMergeWaves;
+  __shared__ float so[SHARE][HD], sm[SHARE], sl[SHARE];
+  const int b = blockIdx.y, lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave % SHARE;
   const KvSeq s = kv_seq(a.b, b);
-  const int i = blockIdx.x, head = blockIdx.y;
-  if (i >= s.n) return;
-  const int hk = head / pl.group, j = i * pl.group + head % pl.group, p0 = s.len - s.n;
+  const int v = blockIdx.x * (W / SHARE) + wave / SHARE, i = v / a.n_heads, head = v % a.n_heads;
   const bool step = pl.step && s.n * pl.group <= kStepRows;
+  if (i >= s.n || step != STEP) return;  // (a whole workgroup's, where its waves share)
+  const int hk = head / pl.group, j = i * pl.group + head % pl.group, p0 = s.len - s.n;
   const size_t vec = (size_t)(s.r0 + i) * a.n_heads + head;
   // this row's own chunks: number, first partial and the step to the next
   int n;
   size_t first, stride;
   const float *po;
   const float2 *pm;
-  if (step) {
+  if (STEP) {
     const KvRange kr = key_range(p0, s.len - 1, s.len, a.slide, a.dense, a.shared);
     n = max(1, ceil_div(kr.t1 - kr.t0, pl.step_tpc));
-    if (pl.step_ns == 1 && pl.pre_ns == 0) return;
     first = ((size_t)b * a.c.nkv + hk) * pl.step_ns * pl.step_rows + j;
     stride = pl.step_rows;
     po = (const float *)(a.work + pl.step_o);
@@ -990,7 +995,6 @@ __global__ __launch_bounds__(1024) void kv_merge_kernel(KvAttn a, KvPlan pl) {
     const int i0 = at / pl.group, i1 = min(s.n - 1, (at + tr - 1) / pl.group);
     const KvRange kr = key_range(p0 + i0, p0 + i1, s.len, a.slide, a.dense, a.shared);
     n = max(1, ceil_div(kr.t1 - kr.t0, pl.rows_tpc));
-    if (pl.rows_ns == 1 && pl.pre_ns == 0) return;
     first = vec;
     stride = (size_t)a.b.rows * a.n_heads;
     po = (const float *)(a.work + pl.rows_o);
@@ -1012,35 +1016,52 @@ __global__ __launch_bounds__(1024) void kv_merge_kernel(KvAttn a, KvPlan pl) {
     return v;
   };
   float m = kFloor, l = 0.0f, x[E] = {};
-  for (int c = wave; c < total; c += nw) {
-    const float *o;
-    const float2 v = where(c, &o);
-    float y[E];
+  constexpr int A = 4;  // chunks loaded at a time
+  for (int c = part; c < total; c += A * SHARE) {
+    float2 v[A];
+    float y[A][E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) y[e] = o[E * lane + e];
-    const float mn = fmaxf(m, v.x);
-    const float f = __builtin_amdgcn_exp2f(m - mn), h = __builtin_amdgcn_exp2f(v.x - mn);
-    m = mn;
-    l = l * f + v.y * h;
+    for (int u = 0; u < A; ++u) {
+      const float *o;
+      v[u] = where(min(c + u * SHARE, total - 1), &o);
 #pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = x[e] * f + y[e] * h;
-  }
-  if (lane == 0) {
-    sm[wave] = m;
-    sl[wave] = l;
-  }
+      for (int e = 0; e < E; ++e) y[u][e] = o[E * lane + e];
+    }
 #pragma unroll
-  for (int e = 0; e < E; ++e) so[wave][E * lane + e] = x[e];
-  __syncthreads();
-  if (threadIdx.x >= HD) return;
-  float mm = kFloor, ll = 0.0f, sum = 0.0f;
-  for (int w = 0; w < nw; ++w) mm = fmaxf(mm, sm[w]);
-  for (int w = 0; w < nw; ++w) {
-    const float f = __builtin_amdgcn_exp2f(sm[w] - mm);
-    ll += sl[w] * f;
-    sum += so[w][threadIdx.x] * f;
+    for (int u = 0; u < A; ++u) {
+      if (c + u * SHARE >= total) break;
+      const float mn = fmaxf(m, v[u].x);
+      const float f = __builtin_amdgcn_exp2f(m - mn), h = __builtin_amdgcn_exp2f(v[u].x - mn);
+      m = mn;
+      l = l * f + v[u].y * h;
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] = x[e] * f + y[u][e] * h;
+    }
   }
-  a.out[vec * HD + threadIdx.x] = ll != 0.0f ? sum / (ll * kVsUnit) : 0.0f;
+  if constexpr (SHARE == 1) {
+    const float unit = l * kVsUnit;
+#pragma unroll
+    for (int e = 0; e < E; ++e) a.out[vec * HD + E * lane + e] = l != 0.0f ? x[e] / unit : 0.0f;
+  } else {
+    if (lane == 0) {
+      sm[part] = m;
+      sl[part] = l;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) so[part][E * lane + e] = x[e];
+    __syncthreads();
+    if (threadIdx.x >= HD) return;
+    float mm = kFloor, ll = 0.0f, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < SHARE; ++w) mm = fmaxf(mm, sm[w]);
+#pragma unroll
+    for (int w = 0; w < SHARE; ++w) {
+      const float f = __builtin_amdgcn_exp2f(sm[w] - mm);
+      ll += sl[w] * f;
+      sum += so[w][threadIdx.x] * f;
+    }
+    a.out[vec * HD + threadIdx.x] = ll != 0.0f ? sum / (ll * kVsUnit) : 0.0f;
+  }
 }
 
 KvPlan plan(const KvAttn &a, const DeviceInfo &dev) {
@@ -1073,15 +1094,30 @@ KvPlan plan(const KvAttn &a, const DeviceInfo &dev) {
   if (p.step) {
     p.step_rows = std::min(kStepRows, most);
     const int n = std::min(a.b.max_rows, kStepRows / p.group);
-    cut(tiles(n), 4 * dev.cus / std::max(1, a.b.batch * a.c.nkv), kStepWaves, &p.step_ns,
+    // two workgroups a compute unit are resident: more than that is rounds of them.  32
+    // sequences of up to 8192 keys and 4 kv heads: 72 us with 2, 73 with 1, 82 with 4
+    cut(tiles(n), 2 * dev.cus / std::max(1, a.b.batch * a.c.nkv), kStepWaves, &p.step_ns,
         &p.step_tpc);
   }
-  p.qb = (long)a.b.rows * p.group > 64 ? 2 : 1;
-  const int blocks = (int)std::max<long>(1, ((long)a.b.rows * p.group + 64 * p.qb - 1) /
-                                                (64 * p.qb)) * a.c.nkv;
-  if (rows) cut(tiles(ceil_div(64 * p.qb, p.group) + 1), dev.cus / blocks, 4, &p.rows_ns, &p.rows_tpc);
-  if (a.shared > 0)
-    cut(ceil_div(a.shared, kTile), dev.cus / blocks, 4, &p.pre_ns, &p.pre_tpc);
+  const long vecs_kv = (long)a.b.rows * p.group;  // query vectors of a kv head
+  auto blocks = [&](int qb) {
+    return (int)std::max<long>(1, (vecs_kv + 64 * qb - 1) / (64 * qb)) * a.c.nkv;
+  };
+  // A workgroup of 128 vectors takes 4500 cycles a tile and 27000 to begin, one of 64 3080
+  // and 16000, and writes half as much for the merge where there are chunks: short runs take
+  // 64.  Of gemma-3-1b over 16384 keys, merge included: 256 vectors 31 us and 37 (128), 512
+  // vectors 44 and 46, four prompts of 512 behind 1536 85 and 80
+  auto block_rows = [&](int tiles) {
+    return vecs_kv > 64 && (long)blocks(1) * tiles > (long)kLongRun * dev.cus ? 2 : 1;
+  };
+  auto rows_tiles = [&](int qb) { return tiles(ceil_div(64 * qb, p.group) + 1); };
+  p.qb = block_rows(rows_tiles(1));
+  if (rows) cut(rows_tiles(p.qb), dev.cus / blocks(p.qb), 4, &p.rows_ns, &p.rows_tpc);
+  if (a.shared > 0) {
+    const int all = ceil_div(a.shared, kTile);
+    p.pre_qb = block_rows(all);
+    cut(all, dev.cus / blocks(p.pre_qb), 4, &p.pre_ns, &p.pre_tpc);
+  }
   if (p.step && (p.step_ns > 1 || p.pre_ns > 0)) {
     const size_t n = (size_t)a.b.batch * a.c.nkv * p.step_ns * p.step_rows;
     p.step_o = take(n * a.c.hdim * 4);
@@ -1105,33 +1141,47 @@ KvPlan plan(const KvAttn &a, const DeviceInfo &dev) {
   return p;
 }
 
+// Waves share a vector where it has many chunks: 2452 vectors of 6 chunks take 6.5 us with a
+// wave each and 8.4 with four, 256 of 64 chunks 6.1 with 16.
+template <int HD, bool STEP>
+void launch_merge(const KvAttn &a, const KvPlan &p, int chunks, int rows, hipStream_t stream) {
+  const int vecs = rows * a.n_heads, batch = a.b.batch;
+  if (chunks > 16)
+    kv_merge_kernel<HD, 16, STEP><<<dim3(vecs, batch), 1024, 0, stream>>>(a, p);
+  else if (chunks > 8)
+    kv_merge_kernel<HD, 4, STEP><<<dim3(vecs, batch), 64 * kMergeWaves, 0, stream>>>(a, p);
+  else if (chunks > 1)
+    kv_merge_kernel<HD, 1, STEP>
+        <<<dim3(ceil_div(vecs, kMergeWaves), batch), 64 * kMergeWaves, 0, stream>>>(a, p);
+}
+
 template <int HD, int TYPE, bool CAP>
 void launch_typed(const KvAttn &a, const KvPlan &p, hipStream_t stream) {
   const int nkv = a.c.nkv, batch = a.b.batch;
   if (p.step)
     kv_step_kernel<HD, TYPE, CAP>
         <<<dim3(p.step_ns, nkv, batch), 64 * kStepWaves, 0, stream>>>(a, p);
-  auto rows = [&](auto kernel, int vecs, int ns, int z) {
-    kernel<<<dim3(ceil_div(vecs, 64 * p.qb) * ns, nkv, z), 256, 0, stream>>>(a, p);
+  auto rows = [&](auto kernel, int vecs, int qb, int ns, int z) {
+    kernel<<<dim3(ceil_div(vecs, 64 * qb) * ns, nkv, z), 256, 0, stream>>>(a, p);
   };
   if (p.rows_ns > 0) {
     const int vecs = a.b.max_rows * p.group;
     if (p.qb == 2)
-      rows(kv_rows_kernel<HD, TYPE, CAP, 2, false>, vecs, p.rows_ns, batch);
+      rows(kv_rows_kernel<HD, TYPE, CAP, 2, false>, vecs, 2, p.rows_ns, batch);
     else
-      rows(kv_rows_kernel<HD, TYPE, CAP, 1, false>, vecs, p.rows_ns, batch);
+      rows(kv_rows_kernel<HD, TYPE, CAP, 1, false>, vecs, 1, p.rows_ns, batch);
   }
   if (p.pre_ns > 0) {
     const int vecs = a.b.rows * p.group;
-    if (p.qb == 2)
-      rows(kv_rows_kernel<HD, TYPE, CAP, 2, true>, vecs, p.pre_ns, 1);
+    if (p.pre_qb == 2)
+      rows(kv_rows_kernel<HD, TYPE, CAP, 2, true>, vecs, 2, p.pre_ns, 1);
     else
-      rows(kv_rows_kernel<HD, TYPE, CAP, 1, true>, vecs, p.pre_ns, 1);
+      rows(kv_rows_kernel<HD, TYPE, CAP, 1, true>, vecs, 1, p.pre_ns, 1);
   }
-  const int most = std::max(p.step ? p.step_ns : 0, p.rows_ns) + p.pre_ns;
-  if (most > 1)
-    kv_merge_kernel<HD><<<dim3(a.b.max_rows, a.n_heads, batch), most > 16 ? 1024 : 256, 0, stream>>>(
-        a, p);
+  if (p.step)
+    launch_merge<HD, true>(a, p, p.step_ns + p.pre_ns, std::min(a.b.max_rows, kStepRows / p.group),
+                           stream);
+  if (p.rows_ns > 0) launch_merge<HD, false>(a, p, p.rows_ns + p.pre_ns, a.b.max_rows, stream);
 }
 
 template <int HD>
