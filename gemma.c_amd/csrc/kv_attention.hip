@@ -309,8 +309,7 @@ struct Pager {
   __device__ __forceinline__ Pager(const KvAttn &a, int seq, int length, int head, int t0, int dt)
       : pages(a.b.pages + (size_t)seq * a.b.width), width(a.b.width), shift(a.c.shift),
         npages(a.c.npages), nkv(a.c.nkv), hk(head), len(length), first(t0), step(dt) {
-    next = load(0);
-    place(0);
+    next = load(0);  // place(0) waits for it
   }
   __device__ __forceinline__ int key(int from) const {
     const int lane = threadIdx.x & 63;
@@ -422,10 +421,12 @@ __global__ __launch_bounds__(64 * kStepWaves, 2) void kv_step_kernel(KvAttn a, K
   const KvSpan span = kv_span(p0 + j / pl.group, s.len, a.slide, a.dense);
   const KvSee see{max(span.lo, a.shared), span.hi};
   const int f_lo = wave_max_all(see.lo), f_hi = -wave_max_all(-see.hi);
+  // (page ids, then the query, then codes are under way before the first of them is waited for)
+  int t = t0 + wave;
+  Pager pager(a, b, s.len, hk, t, kStepWaves);
   h8 qhi[KS], qlo[KS];
   Query<HD> raw;
   raw.load(a.q + (size_t)row * a.q_stride + head * HD, g);
-  const Score score(a.asc, a.cap, raw.split(qhi, qlo));
 
   v4f o[ND];
 #pragma unroll
@@ -456,12 +457,12 @@ __global__ __launch_bounds__(64 * kStepWaves, 2) void kv_step_kernel(KvAttn a, K
     sc.v = eight(at_offset<v4f>(a.c.vs + h.slot0, soff), at_offset<v4f>(a.c.vs + h.slot1, soff));
   };
 
-  int t = t0 + wave;
   if (t < t1) {
-    Pager pager(a, b, s.len, hk, t, kStepWaves);
+    pager.place(0);
     Halves cur = pager.get(0);
     load_k(cur);
     load_v(cur);
+    const Score score(a.asc, a.cap, raw.split(qhi, qlo));
     for (int k = 1; t < t1; t += kStepWaves, ++k) {
       const Halves nxt = pager.get(k);  // past the last: of this sequence or page 0, loaded and not used
       v4f dh[2] = {}, dl[2] = {};
@@ -744,6 +745,7 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(KvAttn a, KvPlan pl) {
 
   if (t0 < t1) {
     Pager pager(a, b, len, hk, t0, 1);  // tiles past the last are loaded and not used
+    pager.place(0);
     int there = 0;  // bits 2 i and 2 i + 1: the halves of tile t + i that are there
     size_t v_slot0, v_slot1;  // where tile t + 3 lies
     uint32_t rv[8];  // codes of V of tile t + 1
