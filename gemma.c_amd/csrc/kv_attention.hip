@@ -581,13 +581,16 @@ __global__ __launch_bounds__(64 * kStepWaves, 2) void kv_step_kernel(KvAttn a, K
 // the conversion of K of tile t + 2 and of V of tile t + 1, whose codes were loaded an
 // iteration before.  One barrier a tile; K and V each have two buffers.
 
-template <int HD, int TYPE, bool CAP, int QB, bool PRE>
-__global__ __launch_bounds__(256) void kv_rows_kernel(KvAttn a, KvPlan pl) {
+template <int HD, int TYPE, bool CAP, int QB, int NW, bool PRE>
+__global__ __launch_bounds__(64 * NW) void kv_rows_kernel(KvAttn a, KvPlan pl) {
   constexpr int KS = HD / 32, ND = HD / 16;
-  constexpr int TR = 64 * QB, VP = 4;  // VP: value fragments read ahead
+  constexpr int TR = 16 * NW * QB, VP = 4;  // VP: value fragments read ahead
+  constexpr int NB = HD / 64;  // blocks of 64 dims
+  // K's half tiles by 64 dims of a wave: both halves of a block, one, or none for some waves
+  constexpr int KU = NW == NB ? 2 : 1;
   __shared__ h8 kf[2][2 * KS][64], vf[2][ND][64];
-  __shared__ v4f scales[4][4][16];
-  __shared__ u4 raw_k[4][3][HD / 128][64], raw_v[4][3][2][64];
+  __shared__ v4f scales[NW][4][16];
+  __shared__ u4 raw_k[NW][3][KU][64], raw_v[NB][3][2][64];
   const int ns = PRE ? pl.pre_ns : pl.rows_ns, tpc = PRE ? pl.pre_tpc : pl.rows_tpc;
   // the last rows, which see most, first
   const int chunk = blockIdx.x % ns, tile = gridDim.x / ns - 1 - blockIdx.x / ns, hk = blockIdx.y;
@@ -611,7 +614,7 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(KvAttn a, KvPlan pl) {
   constexpr int kFind = (int)(sizeof(kf) / 4);
   int *const row0 = reinterpret_cast<int *>(&kf[0][0][0]);
   if (PRE && a.b.batch < kFind) {
-    for (int i = threadIdx.x; i <= a.b.batch; i += 256) row0[i] = a.b.row0[i];
+    for (int i = threadIdx.x; i <= a.b.batch; i += 64 * NW) row0[i] = a.b.row0[i];
     __syncthreads();
   }
 
@@ -677,29 +680,41 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(KvAttn a, KvPlan pl) {
 #pragma unroll
     for (int i = 0; i < ND; ++i) o[q][i] = v4f{};
   }
-  // A wave's share of a tile: KU of K's half tiles by 64 dims (of 128 dims one, of 256
-  // both halves of 64) and 64 dims of V (with 128 dims waves 2 and 3 load what 0 and 1 do,
-  // and leave it), and all of the scales (K's, then V's).  Codes wait in LDS, three tiles
-  // of them, for the wave that loaded them: in registers, two tiles ahead, they don't fit.
-  constexpr int KU = HD / 128, LOADS = KU + 3;
-  const bool has_v = HD == 256 || wave < HD / 64;
-  const int vblock = wave % (HD / 64);
+  // A wave's share of a tile: KU of K's half tiles by 64 dims, 64 dims of V (waves that
+  // there are no dims for have none), and all of the scales (K's, then V's).  Codes wait in
+  // LDS, three tiles of them, for the wave that loaded them: in registers, two tiles ahead,
+  // they don't fit.
+  const bool has_k = NW <= 2 * NB || wave < 2 * NB, has_v = NW == NB || wave < NB;
+  const int block = wave % NB, khalf = KU == 2 ? 0 : wave / NB & 1;
   const uint32_t koff = n * HD + 16 * g;
   // row r of 16 lanes' LDS holds key 4 (r % 4) + r / 4, so that the four lane groups, which
   // read keys 4 g + e at a time, meet different banks
   const uint32_t voff = (4 * (lane >> 2 & 3) + (lane >> 4)) * HD + 16 * (lane & 3);
-  const uint8_t *const k_base = a.c.k + 64 * (wave % (HD / 64)), *const v_base = a.c.v + 64 * vblock;
+  const uint8_t *const k_base = a.c.k + 64 * block, *const v_base = a.c.v + 64 * block;
   auto load_k = [&](int r, const Halves &h) {  // r: the buffer, tile modulo 3
 #pragma unroll
     for (int i = 0; i < KU; ++i) {
-      const size_t slot = (KU == 2 ? i : wave >> 1) != 0 ? h.slot1 : h.slot0;
-      dma16(k_base + slot * HD, koff, raw_k[wave][r][i]);
+      const size_t slot = khalf + i != 0 ? h.slot1 : h.slot0;
+      if (has_k) dma16(k_base + slot * HD, koff, raw_k[wave][r][i]);
     }
   };
   auto load_v = [&](int r, size_t slot0, size_t slot1) {
-    dma16(v_base + slot0 * HD, voff, raw_v[wave][r][0]);
-    dma16(v_base + slot1 * HD, voff, raw_v[wave][r][1]);
+    if (!has_v) return;
+    dma16(v_base + slot0 * HD, voff, raw_v[block][r][0]);
+    dma16(v_base + slot1 * HD, voff, raw_v[block][r][1]);
   };
+  // until only the newest loads of a tile, its scales (or not) and codes, are under way
+  auto wait = [&](auto S) {
+    constexpr int N = S;
+    if (has_v)
+      dma_wait<N + KU + 2>();
+    else if (has_k)
+      dma_wait<N + KU>();
+    else
+      dma_wait<N>();
+  };
+  typedef std::integral_constant<int, 1> with_scales;
+  typedef std::integral_constant<int, 0> but_scales;
   const float *const scale_base = (lane & 8 ? a.c.vs : a.c.ks) + 4 * (lane & 3);
   auto load_scales = [&](int t, size_t slot0, size_t slot1) {
     if (lane < 16) dma16_at(scale_base + (lane & 4 ? slot1 : slot0), scales[wave][t & 3]);
@@ -713,15 +728,15 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(KvAttn a, KvPlan pl) {
     for (int i = 0; i < KU; ++i) x[i] = raw_k[wave][r][i][lane];
   };
   auto store_k = [&](int buf, int i, int half, const u4 (&x)[KU]) {
-    const int u = KU == 2 ? i : wave >> 1;
-    kf[buf][u * KS + 2 * (wave % (HD / 64)) + half][lane] =
-        codes8<TYPE>(x[i][2 * half], x[i][2 * half + 1]);
+    if (has_k)
+      kf[buf][(khalf + i) * KS + 2 * block + half][lane] =
+          codes8<TYPE>(x[i][2 * half], x[i][2 * half + 1]);
   };
   auto read_v = [&](int r, uint32_t (&x)[8]) {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       x[e] = reinterpret_cast<const uint32_t *>(
-          raw_v[wave][r][e / 4])[16 * (4 * (e % 4) + g) + 4 * (n & 3) + (n >> 2)];
+          raw_v[block][r][e / 4])[16 * (4 * (e % 4) + g) + 4 * (n & 3) + (n >> 2)];
   };
   // what lies past the end may be a NaN's code, times a weight of 0 (ok: bits 0 and 1, the
   // halves that are there)
@@ -762,7 +777,7 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(KvAttn a, KvPlan pl) {
       load_k(2, h2);
       load_v(1, h1.slot0, h1.slot1);
       split_queries();
-      dma_wait<LOADS - 1>();
+      wait(but_scales());
       u4 rk[KU];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
@@ -782,7 +797,7 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(KvAttn a, KvPlan pl) {
       load_k(0, h3);
       load_v(2, h2.slot0, h2.slot1);
       load_scales(2, h2.slot0, h2.slot1);
-      dma_wait<LOADS>();
+      wait(with_scales());
       read_v(1, rv);
     }
     v4f d[QB][2] = {};
@@ -855,9 +870,9 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(KvAttn a, KvPlan pl) {
           weigh(j % 4, d[q], vs, soft[q], phi[q], plo[q]);
         });
         if constexpr (KS == 8) {
-          if constexpr (i < 4)
-            transpose_pair<TYPE, i>(rv, v);
-          else if (has_v)
+          if constexpr (i < 4) {
+            if (has_v) transpose_pair<TYPE, i>(rv, v);
+          } else if (has_v)
             vf[nxt][4 * wave + i - 4][lane] = v.dim(i - 4);
         } else {
           transpose_pair<TYPE, i>(rv, v);
@@ -903,8 +918,8 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(KvAttn a, KvPlan pl) {
         });
         if constexpr (i == NC - 2) {
           // what was loaded an iteration ago is in
-          dma_wait<LOADS>();
-          read_v(r2, rv);
+          wait(with_scales());
+          if (has_v) read_v(r2, rv);
         }
         __builtin_amdgcn_sched_barrier(0);
       });
@@ -1157,28 +1172,31 @@ void launch_merge(const KvAttn &a, const KvPlan &p, int chunks, int rows, hipStr
         <<<dim3(ceil_div(vecs, kMergeWaves), batch), 64 * kMergeWaves, 0, stream>>>(a, p);
 }
 
+// 64 B query vectors a workgroup.
+template <int HD, int TYPE, bool CAP, int B, bool PRE>
+void launch_rows(const KvAttn &a, const KvPlan &p, int rows, int ns, int z, hipStream_t stream) {
+  constexpr int NW = B == 2 && HD == 256 ? 8 : 4, QB = B * 4 / NW;
+  kv_rows_kernel<HD, TYPE, CAP, QB, NW, PRE>
+      <<<dim3(ceil_div(rows * p.group, 64 * B) * ns, a.c.nkv, z), 64 * NW, 0, stream>>>(a, p);
+}
+
 template <int HD, int TYPE, bool CAP>
 void launch_typed(const KvAttn &a, const KvPlan &p, hipStream_t stream) {
   const int nkv = a.c.nkv, batch = a.b.batch;
   if (p.step)
     kv_step_kernel<HD, TYPE, CAP>
         <<<dim3(p.step_ns, nkv, batch), 64 * kStepWaves, 0, stream>>>(a, p);
-  auto rows = [&](auto kernel, int vecs, int qb, int ns, int z) {
-    kernel<<<dim3(ceil_div(vecs, 64 * qb) * ns, nkv, z), 256, 0, stream>>>(a, p);
-  };
   if (p.rows_ns > 0) {
-    const int vecs = a.b.max_rows * p.group;
     if (p.qb == 2)
-      rows(kv_rows_kernel<HD, TYPE, CAP, 2, false>, vecs, 2, p.rows_ns, batch);
+      launch_rows<HD, TYPE, CAP, 2, false>(a, p, a.b.max_rows, p.rows_ns, batch, stream);
     else
-      rows(kv_rows_kernel<HD, TYPE, CAP, 1, false>, vecs, 1, p.rows_ns, batch);
+      launch_rows<HD, TYPE, CAP, 1, false>(a, p, a.b.max_rows, p.rows_ns, batch, stream);
   }
   if (p.pre_ns > 0) {
-    const int vecs = a.b.rows * p.group;
     if (p.pre_qb == 2)
-      rows(kv_rows_kernel<HD, TYPE, CAP, 2, true>, vecs, 2, p.pre_ns, 1);
+      launch_rows<HD, TYPE, CAP, 2, true>(a, p, a.b.rows, p.pre_ns, 1, stream);
     else
-      rows(kv_rows_kernel<HD, TYPE, CAP, 1, true>, vecs, 1, p.pre_ns, 1);
+      launch_rows<HD, TYPE, CAP, 1, true>(a, p, a.b.rows, p.pre_ns, 1, stream);
   }
   if (p.step)
     launch_merge<HD, true>(a, p, p.step_ns + p.pre_ns, std::min(a.b.max_rows, kStepRows / p.group),
