@@ -113,14 +113,12 @@ struct Transposed {
 };
 template <int TYPE, int J>
 __device__ __forceinline__ void transpose_pair(const uint32_t (&x)[8], Transposed &t) {
-  uint32_t a = x[2 * J], b = x[2 * J + 1];
-  if (TYPE == kKvI8) {
-    a = flip(a);
-    b = flip(b);
-  }
-  const uint32_t lo = __builtin_amdgcn_perm(b, a, 0x05010400u);  // a0 b0 a1 b1
-  const uint32_t hi = __builtin_amdgcn_perm(b, a, 0x07030602u);  // a2 b2 a3 b3
+  const uint32_t a = x[2 * J], b = x[2 * J + 1];
+  uint32_t lo = __builtin_amdgcn_perm(b, a, 0x05010400u);  // a0 b0 a1 b1
+  uint32_t hi = __builtin_amdgcn_perm(b, a, 0x07030602u);  // a2 b2 a3 b3
   if constexpr (TYPE == kKvI8) {
+    lo = flip(lo);
+    hi = flip(hi);
     t.p[0][J] = magic<0x04010400u>(lo);
     t.p[1][J] = magic<0x04030402u>(lo);
     t.p[2][J] = magic<0x04010400u>(hi);
@@ -130,6 +128,26 @@ __device__ __forceinline__ void transpose_pair(const uint32_t (&x)[8], Transpose
     t.p[1][J] = from_e4m3<true>(lo);
     t.p[2][J] = from_e4m3<false>(hi);
     t.p[3][J] = from_e4m3<true>(hi);
+  }
+}
+
+// ... of two of the four dims, by sel
+struct TransposedHalf {
+  h2 p[2][4];
+  __device__ __forceinline__ h8 dim(int i) const { return join(p[i][0], p[i][1], p[i][2], p[i][3]); }
+};
+constexpr uint32_t kDims01 = 0x05010400u, kDims23 = 0x07030602u;
+template <int TYPE, int J>
+__device__ __forceinline__ void transpose_pair(const uint32_t (&x)[8], uint32_t sel,
+                                               TransposedHalf &t) {
+  uint32_t a = __builtin_amdgcn_perm(x[2 * J + 1], x[2 * J], sel);
+  if constexpr (TYPE == kKvI8) {
+    a = flip(a);
+    t.p[0][J] = magic<0x04010400u>(a);
+    t.p[1][J] = magic<0x04030402u>(a);
+  } else {
+    t.p[0][J] = from_e4m3<false>(a);
+    t.p[1][J] = from_e4m3<true>(a);
   }
 }
 
@@ -272,7 +290,7 @@ __device__ __forceinline__ void weigh(int j, const v4f (&x)[2], const v8f &vs, S
   const float w0 = mul_legacy(p0, vs[e]);
   const float w1 = mul_legacy(p1, vs[e + 1]);
   const h2 h = cvt_pk_f16(w0, w1);
-  const h2 r = cvt_pk_f16(w0 - (float)h[0], w1 - (float)h[1]);
+  const h2 r = cvt_pk_f16(fmaf((float)h[0], -1.0f, w0), fmaf((float)h[1], -1.0f, w1));
   phi[e] = h[0];
   phi[e + 1] = h[1];
   plo[e] = r[0];
@@ -331,9 +349,11 @@ struct Pager {
     return (size_t)(uint32_t)__builtin_amdgcn_readlane(slot_hi, i) << 32 |
            (uint32_t)__builtin_amdgcn_readlane(slot_lo, i);
   }
-  // the j-th tile's halves; j counts up from 0
-  __device__ __forceinline__ Halves get(int j) {
+  // the j-th tile's halves; prepare() is called before, for each j from 0 up
+  __device__ __forceinline__ void prepare(int j) {
     if ((j & 31) == 0 && j > 0) place(j);
+  }
+  __device__ __forceinline__ Halves get(int j) const {
     const int i = 2 * (j & 31);
     return Halves{slot(i), slot(i + 1), (int)(there >> i) & 3};
   }
@@ -464,6 +484,7 @@ __global__ __launch_bounds__(64 * kStepWaves, 2) void kv_step_kernel(KvAttn a, K
     load_v(cur);
     const Score score(a.asc, a.cap, raw.split(qhi, qlo));
     for (int k = 1; t < t1; t += kStepWaves, ++k) {
+      pager.prepare(k);
       const Halves nxt = pager.get(k);  // past the last: of this sequence or page 0, loaded and not used
       v4f dh[2] = {}, dl[2] = {};
 #pragma unroll
@@ -586,11 +607,14 @@ __global__ __launch_bounds__(64 * NW) void kv_rows_kernel(KvAttn a, KvPlan pl) {
   constexpr int KS = HD / 32, ND = HD / 16;
   constexpr int TR = 16 * NW * QB, VP = 4;  // VP: value fragments read ahead
   constexpr int NB = HD / 64;  // blocks of 64 dims
-  // K's half tiles by 64 dims of a wave: both halves of a block, one, or none for some waves
-  constexpr int KU = NW == NB ? 2 : 1;
+  // A wave's share of a tile: K's half tiles by 64 dims, both of a block or one; 64 dims of
+  // V or 32, of which a lane transposes VD
+  static_assert(NW == NB || NW == 2 * NB, "shares");
+  constexpr int KU = NW == NB ? 2 : 1, VD = NW == NB ? 4 : 2, VL = VD / 2;
+  constexpr int LOADS = KU + VL + 1;
   __shared__ h8 kf[2][2 * KS][64], vf[2][ND][64];
-  __shared__ v4f scales[NW][4][16];
-  __shared__ u4 raw_k[NW][3][KU][64], raw_v[NB][3][2][64];
+  __shared__ v4f scales[4][64];  // of which the first 16 are read; all waves write the same
+  __shared__ u4 raw_k[NW][3][KU][64], raw_v[NW][3][VL][64];
   const int ns = PRE ? pl.pre_ns : pl.rows_ns, tpc = PRE ? pl.pre_tpc : pl.rows_tpc;
   // the last rows, which see most, first
   const int chunk = blockIdx.x % ns, tile = gridDim.x / ns - 1 - blockIdx.x / ns, hk = blockIdx.y;
@@ -680,64 +704,68 @@ __global__ __launch_bounds__(64 * NW) void kv_rows_kernel(KvAttn a, KvPlan pl) {
 #pragma unroll
     for (int i = 0; i < ND; ++i) o[q][i] = v4f{};
   }
-  // A wave's share of a tile: KU of K's half tiles by 64 dims, 64 dims of V (waves that
-  // there are no dims for have none), and all of the scales (K's, then V's).  Codes wait in
-  // LDS, three tiles of them, for the wave that loaded them: in registers, two tiles ahead,
-  // they don't fit.
-  const bool has_k = NW <= 2 * NB || wave < 2 * NB, has_v = NW == NB || wave < NB;
-  const int block = wave % NB, khalf = KU == 2 ? 0 : wave / NB & 1;
+  // Codes wait in LDS, three tiles of them, for the wave that loaded them: in registers, two
+  // tiles ahead, they don't fit.
+  const int block = wave % NB, part = wave / NB, khalf = KU == 2 ? 0 : part;
   const uint32_t koff = n * HD + 16 * g;
   // row r of 16 lanes' LDS holds key 4 (r % 4) + r / 4, so that the four lane groups, which
   // read keys 4 g + e at a time, meet different banks
-  const uint32_t voff = (4 * (lane >> 2 & 3) + (lane >> 4)) * HD + 16 * (lane & 3);
-  const uint8_t *const k_base = a.c.k + 64 * block, *const v_base = a.c.v + 64 * block;
+  const int vrow = VD == 4 ? lane >> 2 : lane >> 1 & 15;
+  const uint32_t voff = (4 * (vrow & 3) + (vrow >> 2)) * HD + 16 * (lane & (VD - 1));
+  const uint8_t *const k_base = a.c.k + 64 * block, *const v_base = a.c.v + 64 * block + (VD == 4 ? 0 : 32 * part);
   auto load_k = [&](int r, const Halves &h) {  // r: the buffer, tile modulo 3
 #pragma unroll
     for (int i = 0; i < KU; ++i) {
       const size_t slot = khalf + i != 0 ? h.slot1 : h.slot0;
-      if (has_k) dma16(k_base + slot * HD, koff, raw_k[wave][r][i]);
+      dma16(k_base + slot * HD, koff, raw_k[wave][r][i]);
     }
   };
   auto load_v = [&](int r, size_t slot0, size_t slot1) {
-    if (!has_v) return;
-    dma16(v_base + slot0 * HD, voff, raw_v[block][r][0]);
-    dma16(v_base + slot1 * HD, voff, raw_v[block][r][1]);
+    if constexpr (VD == 4) {
+      dma16(v_base + slot0 * HD, voff, raw_v[wave][r][0]);
+      dma16(v_base + slot1 * HD, voff, raw_v[wave][r][VL - 1]);
+    } else {
+      dma16_at(v_base + (lane < 32 ? slot0 : slot1) * HD + voff, raw_v[wave][r][0]);
+    }
   };
-  // until only the newest loads of a tile, its scales (or not) and codes, are under way
-  auto wait = [&](auto S) {
-    constexpr int N = S;
-    if (has_v)
-      dma_wait<N + KU + 2>();
-    else if (has_k)
-      dma_wait<N + KU>();
-    else
-      dma_wait<N>();
-  };
-  typedef std::integral_constant<int, 1> with_scales;
-  typedef std::integral_constant<int, 0> but_scales;
   const float *const scale_base = (lane & 8 ? a.c.vs : a.c.ks) + 4 * (lane & 3);
   auto load_scales = [&](int t, size_t slot0, size_t slot1) {
-    if (lane < 16) dma16_at(scale_base + (lane & 4 ? slot1 : slot0), scales[wave][t & 3]);
+    dma16_at(scale_base + (lane & 4 ? slot1 : slot0), scales[t & 3]);
   };
-  auto scales_k = [&](int t) { return eight(scales[wave][t & 3][g], scales[wave][t & 3][4 + g]); };
+  auto scales_k = [&](int t) { return eight(scales[t & 3][g], scales[t & 3][4 + g]); };
   auto scales_v = [&](int t) {
-    return eight(scales[wave][t & 3][8 + g], scales[wave][t & 3][12 + g]) * kVsUnit;
+    return eight(scales[t & 3][8 + g], scales[t & 3][12 + g]) * kVsUnit;
   };
   auto read_k = [&](int r, u4 (&x)[KU]) {
 #pragma unroll
     for (int i = 0; i < KU; ++i) x[i] = raw_k[wave][r][i][lane];
   };
   auto store_k = [&](int buf, int i, int half, const u4 (&x)[KU]) {
-    if (has_k)
-      kf[buf][(khalf + i) * KS + 2 * block + half][lane] =
-          codes8<TYPE>(x[i][2 * half], x[i][2 * half + 1]);
+    kf[buf][(khalf + i) * KS + 2 * block + half][lane] =
+        codes8<TYPE>(x[i][2 * half], x[i][2 * half + 1]);
   };
+  // A lane of 64 dims: the four of row n of its block's fragments; of 32: two of four, so
+  // that lanes n and n + 8 share dims
+  const int vquad = VD == 4 ? 4 * (n & 3) + (n >> 2) : n & 7;
+  const uint32_t vsel = n < 8 ? kDims01 : kDims23;
   auto read_v = [&](int r, uint32_t (&x)[8]) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      x[e] = reinterpret_cast<const uint32_t *>(
-          raw_v[block][r][e / 4])[16 * (4 * (e % 4) + g) + 4 * (n & 3) + (n >> 2)];
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t *raw = reinterpret_cast<const uint32_t *>(raw_v[wave][r][VD == 4 ? e / 4 : 0]);
+      x[e] = VD == 4 ? raw[16 * (4 * (e % 4) + g) + vquad]
+                     : raw[8 * (16 * (e / 4) + 4 * (e % 4) + g) + vquad];
+    }
   };
+  typedef std::conditional_t<VD == 4, Transposed, TransposedHalf> VT;
+  auto turn = [&](auto J, const uint32_t (&x)[8], VT &v) {
+    if constexpr (VD == 4)
+      transpose_pair<TYPE, J>(x, v);
+    else
+      transpose_pair<TYPE, J>(x, vsel, v);
+  };
+  const int vfrag = 4 * block + (VD == 4 ? 0 : 2 * (n >> 3));
+  const int vlane = VD == 4 ? lane : 16 * g + 4 * (n & 3) + 2 * part + (n >> 2 & 1);
+  auto store_v = [&](int buf, int i, const VT &v) { vf[buf][vfrag + i][vlane] = v.dim(i); };
   // what lies past the end may be a NaN's code, times a weight of 0 (ok: bits 0 and 1, the
   // halves that are there)
   auto clear_v = [&](int t, int ok, uint32_t (&x)[8]) {
@@ -777,7 +805,7 @@ __global__ __launch_bounds__(64 * NW) void kv_rows_kernel(KvAttn a, KvPlan pl) {
       load_k(2, h2);
       load_v(1, h1.slot0, h1.slot1);
       split_queries();
-      wait(but_scales());
+      dma_wait<LOADS - 1>();
       u4 rk[KU];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
@@ -790,14 +818,14 @@ __global__ __launch_bounds__(64 * NW) void kv_rows_kernel(KvAttn a, KvPlan pl) {
       }
       read_v(0, rv);
       clear_v(0, there, rv);
-      Transposed v;
-      each<4>([&](auto J) { transpose_pair<TYPE, J>(rv, v); });
-      if (has_v) each<4>([&](auto I) { vf[0][4 * wave + I][lane] = v.dim(I); });
+      VT v;
+      each<4>([&](auto J) { turn(J, rv, v); });
+      each<VD>([&](auto I) { store_v(0, I, v); });
       lds_barrier();
       load_k(0, h3);
       load_v(2, h2.slot0, h2.slot1);
       load_scales(2, h2.slot0, h2.slot1);
-      wait(with_scales());
+      dma_wait<LOADS>();
       read_v(1, rv);
     }
     v4f d[QB][2] = {};
@@ -825,8 +853,10 @@ __global__ __launch_bounds__(64 * NW) void kv_rows_kernel(KvAttn a, KvPlan pl) {
     // rarely happens, and lies outside the inner loop: in it the value sums are touched by
     // the matrix cores alone and stay in the accumulation registers.
     auto begin = [&]() {
-      const int key0 = kTile * (t0 + t);
+      int key0 = kTile * (t0 + t);
+      pager.prepare(t + 4);
       if (key0 < f_lo || key0 + kTile - 1 > f_hi || (there & 3) != 3) {  // wave-uniform
+        asm volatile("" : "+s"(key0));  // the compiler would have all tiles work out the masks
         float lv[8];
         scale_octaves(vs, lv);
 #pragma unroll
@@ -847,8 +877,8 @@ __global__ __launch_bounds__(64 * NW) void kv_rows_kernel(KvAttn a, KvPlan pl) {
       v4f dn[QB][2] = {};
       u4 rk[KU];
       v8f ks, vn;
-      Transposed v;
-      Halves h4;
+      VT v;
+      const Halves h4 = pager.get(t + 4);
       // scores of tile t + 1; weights of tile t, V of tile t + 1, loads of tiles t + 3 and
       // t + 4 (into the buffers that the iteration before was done with)
       each<KS>([&](auto I) {
@@ -870,16 +900,14 @@ __global__ __launch_bounds__(64 * NW) void kv_rows_kernel(KvAttn a, KvPlan pl) {
           weigh(j % 4, d[q], vs, soft[q], phi[q], plo[q]);
         });
         if constexpr (KS == 8) {
-          if constexpr (i < 4) {
-            if (has_v) transpose_pair<TYPE, i>(rv, v);
-          } else if (has_v)
-            vf[nxt][4 * wave + i - 4][lane] = v.dim(i - 4);
+          if constexpr (i < 4)
+            turn(I, rv, v);
+          else if constexpr (i - 4 < VD)
+            store_v(nxt, i - 4, v);
         } else {
-          transpose_pair<TYPE, i>(rv, v);
-          if constexpr (i == KS - 1)
-            if (has_v) each<4>([&](auto D) { vf[nxt][4 * wave + D][lane] = v.dim(D); });
+          turn(I, rv, v);
+          if constexpr (i == KS - 1) each<VD>([&](auto D) { store_v(nxt, D, v); });
         }
-        if constexpr (i == KS / 2 - 2) h4 = pager.get(t + 4);
         if constexpr (i == KS / 2 - 1) load_k(r1, h4);
         if constexpr (i == KS / 2) load_v(r, v_slot0, v_slot1);
         if constexpr (i == KS / 2 + 1) load_scales(t + 3, v_slot0, v_slot1);
@@ -918,8 +946,8 @@ __global__ __launch_bounds__(64 * NW) void kv_rows_kernel(KvAttn a, KvPlan pl) {
         });
         if constexpr (i == NC - 2) {
           // what was loaded an iteration ago is in
-          wait(with_scales());
-          if (has_v) read_v(r2, rv);
+          dma_wait<LOADS>();
+          read_v(r2, rv);
         }
         __builtin_amdgcn_sched_barrier(0);
       });
