@@ -1031,6 +1031,10 @@ int need_device(const char *name) {
 
 bool aligned16(const void *p) { return (uintptr_t)p % 16 == 0; }
 
+// Rows times heads of a call of the cache's, at most: what a grid's threads and the kernels'
+// 32-bit counts of query vectors hold, with room.
+constexpr long kKvMostVecs = 1l << 25;
+
 // A cache and a batch as the kernels take them; 1 and a message where their sizes
 // don't fit.
 int kv_args(const char *name, const gemma_hip_cache *cache, const gemma_hip_batch *batch,
@@ -1050,6 +1054,8 @@ int kv_args(const char *name, const gemma_hip_cache *cache, const gemma_hip_batc
     return fail("%s: bad batch: %d sequences, %d rows (%d at most), %d positions in %d pages of %d",
                 name, batch->batch, batch->rows, batch->max_rows, batch->max_len,
                 batch->max_pages, page);
+  if ((long)batch->max_rows * cache->nkv > kKvMostVecs)
+    return fail("%s: too many rows: %d of %d heads", name, batch->max_rows, cache->nkv);
   int shift = 0;
   while ((1 << shift) < page) ++shift;
   *c = gh::KvCache{(uint8_t *)cache->k, (uint8_t *)cache->v, cache->ks, cache->vs,
@@ -1087,8 +1093,8 @@ int attn_args(const char *name, const gemma_hip_cache *cache, const gemma_hip_ba
   if (slide < 0 || shared < 0 || shared > a->b.max_len)
     return fail("%s: bad window %d or shared prefix %d (of %d positions)", name, slide, shared,
                 a->b.max_len);
-  if ((long)a->b.max_rows * n_heads > (1l << 30))
-    return fail("%s: too many rows", name);
+  if ((long)a->b.rows * n_heads > kKvMostVecs)
+    return fail("%s: too many rows: %d of %d heads", name, a->b.rows, n_heads);
   a->n_heads = n_heads;
   a->slide = slide;
   a->shared = shared;

@@ -441,12 +441,7 @@ __global__ __launch_bounds__(64 * kStepWaves, 2) void kv_step_kernel(KvAttn a, K
   const KvSpan span = kv_span(p0 + j / pl.group, s.len, a.slide, a.dense);
   const KvSee see{max(span.lo, a.shared), span.hi};
   const int f_lo = wave_max_all(see.lo), f_hi = -wave_max_all(-see.hi);
-  // (page ids, then the query, then codes are under way before the first of them is waited for)
-  int t = t0 + wave;
-  Pager pager(a, b, s.len, hk, t, kStepWaves);
   h8 qhi[KS], qlo[KS];
-  Query<HD> raw;
-  raw.load(a.q + (size_t)row * a.q_stride + head * HD, g);
 
   v4f o[ND];
 #pragma unroll
@@ -477,7 +472,12 @@ __global__ __launch_bounds__(64 * kStepWaves, 2) void kv_step_kernel(KvAttn a, K
     sc.v = eight(at_offset<v4f>(a.c.vs + h.slot0, soff), at_offset<v4f>(a.c.vs + h.slot1, soff));
   };
 
-  if (t < t1) {
+  int t = t0 + wave;
+  if (t < t1) {  // (there may be no page table where there is no key)
+    // page ids, then the query, then codes are asked for before the first of them is needed
+    Pager pager(a, b, s.len, hk, t, kStepWaves);
+    Query<HD> raw;
+    raw.load(a.q + (size_t)row * a.q_stride + head * HD, g);
     pager.place(0);
     Halves cur = pager.get(0);
     load_k(cur);

@@ -105,7 +105,9 @@ int gemma_hip_sync(void *stream);
  * gate|up one launch each), "gemv_fpx" (with 'U' weights the decode GEMVs,
  * their norm-fused forms, GELU fused, and the LM head) and
  * "sample_from_logits" (softcap + argmax,
- * counted in the decode phase as the reference does).  They set the phase
+ * counted in the decode phase as the reference does).  Of the entry points for
+ * batches, cache_write and cache_read count as "quantize_act", cache_attention as
+ * "softmax" and gemma_hip_sample as "sample_from_logits".  They set the phase
  * themselves as the reference's forward_gemma_* do: decoder_prefill and
  * prefill_rows with mask != 0 prefill; decoder_step and decoder_generate
  * decode (run eagerly, not as the captured graph, while timing is on);
@@ -588,6 +590,8 @@ typedef struct {
  * Sizes that the host knows: `rows`, the rows of the call's buffers (at least
  * row0[batch]; those from row0[batch] on are left as they are); max_rows and
  * max_len, at least every sequence's rows and len (max_len <= max_pages * page).
+ * Rows times heads are 2^25 at most (of the longest sequence for cache_write and
+ * cache_read, of all for cache_attention).
  * Lengths and rows are cut to these bounds, and a page id outside the cache stands
  * for positions that aren't there: not written, read as zeros, not attended to. */
 typedef struct {
@@ -615,7 +619,7 @@ int gemma_hip_cache_read(const gemma_hip_cache *cache, const gemma_hip_batch *ba
  * [rows][n_heads * hdim], 16-byte aligned; n_heads a multiple of nkv.  The row at
  * position p sees keys max(0, p + 1 - slide) .. p (slide 0: no window; dense != 0:
  * every key of its sequence); scores are q.k * asc, capped as tanh(s / sc_att) *
- * sc_att when sc_att != 0.  A row that sees nothing is zeros.
+ * sc_att when sc_att != 0.  A row that sees nothing is zeros.  out and q do not overlap.
  * shared: the first `shared` positions lie in the same pages for every sequence (a
  * common prefix; 0: none).  Each sequence's table lists them; the first one's is
  * read, and their keys and values are read once for all rows.
@@ -651,8 +655,9 @@ typedef struct {
  * >= min_p; the token is the first whose running sum exceeds u times the sum of the
  * kept ones.  NaN logits count as -inf, which is never drawn; +inf ones take all.
  * tokens [rows] (-1 where no logit is above -inf) and probs [rows] (nullable, the
- * token's share of the kept sum).  Weights are 64-bit and their sums exact to 2^-44
- * of the largest, in any order of the work: equal calls draw equal tokens.
+ * token's share of the kept sum).  Weights are 64-bit, off by at most 2^-39 of
+ * themselves in the sums, which no order of the work changes: equal calls draw equal
+ * tokens.
  * work: gemma_hip_sample_work() bytes, as above. */
 int gemma_hip_sample(int *tokens, float *probs, const float *logits, int stride, int rows,
                      int vocab, const gemma_hip_sampling *settings, const float *u, void *work,

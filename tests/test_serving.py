@@ -4,8 +4,8 @@
 (gemma_hip_sample), against plain numpy in 64 bits.
 
 Bars.  Codes, scales and read values follow a definition of single fp32 roundings:
-equal to the bit.  Tokens: equal (the weights' sums are exact to 2^-44 of the
-largest; a random number falls that close to a border once in 10^8 draws).
+equal to the bit.  Tokens: equal (a weight in a sum is off by at most 2^-39 of itself,
+and a random number falls that close to a border once in 10^8 draws).
 Attention, relative to the largest |v| that a row sees: scores up to about 10 are
 fp32 sums whose 16 or so roundings leave 1e-6, which is the weights' relative error
 and at most that of the output, and the value sums' own roundings leave about as
@@ -308,6 +308,19 @@ def test_bad_caches_and_batches_are_refused(what, field, value, word):
         assert name in msg and word in msg, msg
     if word not in ("null", "aligned"):
         assert lib.gemma_hip_cache_attention_work(c, b, 4, 0, 0) == ctypes.c_size_t(-1).value
+
+
+def test_more_rows_than_the_kernels_count_are_refused():
+    lib = gemma_hip.load()
+    c, b = good()
+    b.rows = b.max_rows = 1 << 26
+    assert lib.gemma_hip_cache_write(c, b, fake(), 256, fake(), 256, None) == 1
+    assert "too many rows" in lib.gemma_hip_last_error().decode()
+    b.max_rows = 1  # few of each sequence, but the shared prefix is read by all of them
+    assert lib.gemma_hip_cache_attention(fake(), fake(), 512, c, b, 4, 0, 1.0, 0.0, 0, 0, None, 0,
+                                         None) == 1
+    assert "too many rows" in lib.gemma_hip_last_error().decode()
+    assert lib.gemma_hip_cache_attention_work(c, b, 4, 0, 0) == ctypes.c_size_t(-1).value
 
 
 def test_bad_rows_and_settings_are_refused():
@@ -666,6 +679,44 @@ def test_attention_long_prompt_and_prefix(gh):
     check_attention(gh, p, 4, 0, 0.0, False, 2048, 0.0625, rng, step=7)
     check_attention(gh, p, 4, 512, 0.0, False, 2048, 0.0625, rng, step=7)
     check_attention(gh, p, 4, 0, 0.0, False, 0, 0.0625, rng, step=7)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,hdim,kind,slide,cap,shared", [
+    (4, 1, 256, "i8", 0, 0.0, 0), (4, 1, 256, "e4m3", 0, 30.0, 1200), (4, 1, 256, "i8", 1500, 0.0, 0),
+    (4, 1, 256, "e4m3", 1501, 0.0, 1216), (4, 1, 256, "i8", 0, 0.0, 1296),
+    (8, 2, 128, "i8", 0, 0.0, 1200), (8, 2, 128, "e4m3", 1500, 30.0, 0)])
+def test_attention_many_rows_over_many_keys(gh, heads, kv, hdim, kind, slide, cap, shared):
+    """Enough of both (more than 20 tiles of 32 keys by 64 query vectors for each of the
+    card's 256 compute units) that a workgroup takes 128 vectors, prefixes included."""
+    rng = np.random.default_rng(19)
+    p = Paged([(1300, 2600), (1, 1390), (901, 1400), (0, 1300)], kv, hdim, 16, KINDS[kind], rng,
+              shared=shared)
+    p.fill(rng)
+    check_attention(gh, p, heads, slide, cap, False, shared, 0.0625, rng, step=53)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hdim", [128, 256])
+def test_rows_without_a_page_table(gh, hdim):
+    """Sequences of rows and no positions need no pages: nothing is written, and what is
+    read or attended to is zeros."""
+    import torch
+
+    p = Paged([(1, 20)], 1, hdim, 16, CACHE_I8, np.random.default_rng(20))
+    c = p.device()
+    for n in ([1, 1], [40, 1]):
+        rows = sum(n)
+        b = gemma_hip.batch(None, cuda(np.zeros(2, np.int32)),
+                            cuda(np.array([0, n[0], rows], np.int32)), 2, 0, rows, max(n), 0)
+        x = torch.randn(rows, 4 * hdim, device="cuda")
+        k, v = torch.ones(rows, hdim, device="cuda"), torch.ones(rows, hdim, device="cuda")
+        gh.cache_write(c, b, k, 0, v, 0, stream())
+        gh.cache_read(c, b, k, 0, v, 0, stream())
+        out = torch.ones(rows, 4 * hdim, device="cuda")
+        gh.cache_attention(out, x, 0, c, b, 4, 0, 1.0, 0.0, False, 0, None, stream())
+        torch.cuda.synchronize()
+        assert not k.any() and not v.any() and not out.any()
 
 
 @pytest.mark.gpu
