@@ -39,7 +39,7 @@ namespace gh {
 namespace {
 
 constexpr int kTile = 32;             // keys of a tile
-constexpr int kLongRun = 20;          // tiles by 64 query vectors of a compute unit: see plan()
+constexpr int kLongRun = 16;          // tiles by 64 query vectors of a compute unit: see plan()
 constexpr int kStepRows = 16;         // query vectors (rows x heads of a kv head) of a step tile
 constexpr float kFloor = -0x1p55f;    // M of a query that has seen no key
 constexpr float kVsUnit = 0x1p-24f;   // V's scales enter the weights in units of 2^24, so that

@@ -107,8 +107,8 @@ int gemma_hip_sync(void *stream);
  * "sample_from_logits" (softcap + argmax,
  * counted in the decode phase as the reference does).  Of the entry points for
  * batches, cache_write and cache_read count as "quantize_act", cache_attention as
- * "softmax" and gemma_hip_sample as "sample_from_logits".  They set the phase
- * themselves as the reference's forward_gemma_* do: decoder_prefill and
+ * "softmax" and gemma_hip_sample as "sample_from_logits".  The decoder and the
+ * tower set the phase themselves as the reference's forward_gemma_* do: decoder_prefill and
  * prefill_rows with mask != 0 prefill; decoder_step and decoder_generate
  * decode (run eagerly, not as the captured graph, while timing is on);
  * vision_forward, gemma_image and prefill_rows with mask == 0 vision.
