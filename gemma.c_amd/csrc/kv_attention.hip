@@ -40,6 +40,8 @@ namespace {
 
 constexpr int kTile = 32;             // keys of a tile
 constexpr int kLongRun = 16;          // tiles by 64 query vectors of a compute unit: see plan()
+constexpr int kBothTiles = 64;         // tiles of own keys, at most, of single tokens that share
+                                      // a launch with their prefix
 constexpr int kStepRows = 16;         // query vectors (rows x heads of a kv head) of a step tile
 constexpr float kFloor = -0x1p55f;    // M of a query that has seen no key
 constexpr float kVsUnit = 0x1p-24f;   // V's scales enter the weights in units of 2^24, so that
@@ -59,6 +61,8 @@ struct KvPlan {
   int step_rows;                // query vectors of a sequence and kv head, at most
   int rows_ns, rows_tpc;        // prompt rows (0 chunks: off)
   int pre_ns, pre_tpc;          // shared prefix (0: none)
+  int pre_blocks;               // its tiles of rows, where one launch takes it and the single
+                                // tokens (0: not)
   int qb, pre_qb;               // 16-query blocks of a wave of the prompt kernel
   size_t step_o, step_m, rows_o, rows_m, pre_o, pre_m, bytes;  // workspace
 };
@@ -419,13 +423,19 @@ __device__ __forceinline__ KvRange key_range(int first_pos, int last_pos, int le
 
 constexpr int kStepWaves = 4;
 
+template <int HD>
+struct StepLds {
+  float part[kStepWaves][kStepRows][HD + 4];
+  float sm[kStepWaves][kStepRows], sl[kStepWaves][kStepRows];
+};
+
 template <int HD, int TYPE, bool CAP>
-__global__ __launch_bounds__(64 * kStepWaves, 2) void kv_step_kernel(KvAttn a, KvPlan pl) {
+__device__ __forceinline__ void step_keys(const KvAttn &a, const KvPlan &pl, int chunk, int hk,
+                                          int b, StepLds<HD> &lds) {
   constexpr int KS = HD / 32, ND = HD / 16, NJ = HD / 64, VW = HD / 64;
-  constexpr int LS = HD + 4;  // floats of a query in LDS
-  __shared__ float part[kStepWaves][kStepRows][LS];
-  __shared__ float sm[kStepWaves][kStepRows], sl[kStepWaves][kStepRows];
-  const int chunk = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
+  auto &part = lds.part;
+  auto &sm = lds.sm;
+  auto &sl = lds.sl;
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const KvSeq s = kv_seq(a.b, b);
@@ -591,6 +601,12 @@ __global__ __launch_bounds__(64 * kStepWaves, 2) void kv_step_kernel(KvAttn a, K
   }
 }
 
+template <int HD, int TYPE, bool CAP>
+__global__ __launch_bounds__(64 * kStepWaves, 2) void kv_step_kernel(KvAttn a, KvPlan pl) {
+  __shared__ StepLds<HD> lds;
+  step_keys<HD, TYPE, CAP>(a, pl, blockIdx.x, blockIdx.y, blockIdx.z, lds);
+}
+
 // ---- prompt rows and shared prefixes ---------------------------------------------
 // A workgroup takes 64 QB query vectors of a kv head, 16 QB a wave, and a chunk of
 // their keys; PRE: the rows of all sequences, over the shared prefix.  Each tile's
@@ -602,23 +618,35 @@ __global__ __launch_bounds__(64 * kStepWaves, 2) void kv_step_kernel(KvAttn a, K
 // the conversion of K of tile t + 2 and of V of tile t + 1, whose codes were loaded an
 // iteration before.  One barrier a tile; K and V each have two buffers.
 
-template <int HD, int TYPE, bool CAP, int QB, int NW, bool PRE>
-__global__ __launch_bounds__(64 * NW) void kv_rows_kernel(KvAttn a, KvPlan pl) {
-  constexpr int KS = HD / 32, ND = HD / 16;
-  constexpr int TR = 16 * NW * QB, VP = 4;  // VP: value fragments read ahead
-  constexpr int NB = HD / 64;  // blocks of 64 dims
-  // A wave's share of a tile: K's half tiles by 64 dims, both of a block or one; 64 dims of
-  // V or 32, of which a lane transposes VD
+// A wave's share of a tile: K's half tiles by 64 dims, both of a block or one; 64 dims of
+// V or 32, of which a lane transposes VD.
+template <int HD, int NW>
+struct RowsLds {
+  static constexpr int NB = HD / 64;  // blocks of 64 dims
   static_assert(NW == NB || NW == 2 * NB, "shares");
-  constexpr int KU = NW == NB ? 2 : 1, VD = NW == NB ? 4 : 2, VL = VD / 2;
+  static constexpr int KS = HD / 32, ND = HD / 16, KU = NW == NB ? 2 : 1, VD = NW == NB ? 4 : 2,
+                       VL = VD / 2;
+  h8 kf[2][2 * KS][64], vf[2][ND][64];
+  v4f scales[4][64];  // of which the first 16 are read; all waves write the same
+  u4 raw_k[NW][3][KU][64], raw_v[NW][3][VL][64];
+};
+
+// block: of nblocks, chunks of a tile of rows in a row.
+template <int HD, int TYPE, bool CAP, int QB, int NW, bool PRE>
+__device__ __forceinline__ void rows_keys(const KvAttn &a, const KvPlan &pl, int block_x,
+                                          int nblocks, int hk, int b, RowsLds<HD, NW> &lds) {
+  typedef RowsLds<HD, NW> L;
+  constexpr int NB = L::NB, KS = L::KS, ND = L::ND, KU = L::KU, VD = L::VD, VL = L::VL;
+  constexpr int TR = 16 * NW * QB, VP = 4;  // VP: value fragments read ahead
   constexpr int LOADS = KU + VL + 1;
-  __shared__ h8 kf[2][2 * KS][64], vf[2][ND][64];
-  __shared__ v4f scales[4][64];  // of which the first 16 are read; all waves write the same
-  __shared__ u4 raw_k[NW][3][KU][64], raw_v[NW][3][VL][64];
+  auto &kf = lds.kf;
+  auto &vf = lds.vf;
+  auto &scales = lds.scales;
+  auto &raw_k = lds.raw_k;
+  auto &raw_v = lds.raw_v;
   const int ns = PRE ? pl.pre_ns : pl.rows_ns, tpc = PRE ? pl.pre_tpc : pl.rows_tpc;
   // the last rows, which see most, first
-  const int chunk = blockIdx.x % ns, tile = gridDim.x / ns - 1 - blockIdx.x / ns, hk = blockIdx.y;
-  const int b = PRE ? 0 : blockIdx.z;
+  const int chunk = block_x % ns, tile = nblocks / ns - 1 - block_x / ns;
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   KvSeq s = kv_seq(a.b, b);
@@ -1003,6 +1031,32 @@ __global__ __launch_bounds__(64 * NW) void kv_rows_kernel(KvAttn a, KvPlan pl) {
   }
 }
 
+template <int HD, int TYPE, bool CAP, int QB, int NW, bool PRE>
+__global__ __launch_bounds__(64 * NW) void kv_rows_kernel(KvAttn a, KvPlan pl) {
+  __shared__ RowsLds<HD, NW> lds;
+  rows_keys<HD, TYPE, CAP, QB, NW, PRE>(a, pl, blockIdx.x, gridDim.x, blockIdx.y,
+                                        PRE ? 0 : blockIdx.z, lds);
+}
+
+// The shared prefix and what single tokens' sequences have of their own in one launch: each
+// leaves most of its time to latencies, and neither fills the card for long.  The prefix's
+// workgroups, which take longest, come first.
+template <int HD, int TYPE, bool CAP>
+__global__ __launch_bounds__(64 * kStepWaves) void kv_both_kernel(KvAttn a, KvPlan pl) {
+  constexpr int NW = kStepWaves;
+  __shared__ union {
+    RowsLds<HD, NW> rows;
+    StepLds<HD> step;
+  } lds;
+  const int blocks = pl.pre_blocks * pl.pre_ns, id = blockIdx.x;
+  if (id < blocks * a.c.nkv) {
+    rows_keys<HD, TYPE, CAP, 1, NW, true>(a, pl, id % blocks, blocks, id / blocks, 0, lds.rows);
+  } else {
+    const int i = id - blocks * a.c.nkv;  // one chunk
+    step_keys<HD, TYPE, CAP>(a, pl, 0, i % a.c.nkv, i / a.c.nkv, lds.step);
+  }
+}
+
 // ---- the chunks' sums together ------------------------------------------------------
 // SHARE waves take a query vector and share out its chunks; STEP: vectors of single tokens,
 // else of prompt rows, which may have very different numbers of both.  Bound by the partial
@@ -1155,13 +1209,36 @@ KvPlan plan(const KvAttn &a, const DeviceInfo &dev) {
   auto block_rows = [&](int tiles) {
     return vecs_kv > 64 && (long)blocks(1) * tiles > (long)kLongRun * dev.cus ? 2 : 1;
   };
+  const int own_tiles = tiles(std::min(a.b.max_rows, kStepRows / std::min(p.group, kStepRows)));
   auto rows_tiles = [&](int qb) { return tiles(ceil_div(64 * qb, p.group) + 1); };
   p.qb = block_rows(rows_tiles(1));
   if (rows) cut(rows_tiles(p.qb), dev.cus / blocks(p.qb), 4, &p.rows_ns, &p.rows_tpc);
   if (a.shared > 0) {
     const int all = ceil_div(a.shared, kTile);
     p.pre_qb = block_rows(all);
-    cut(all, dev.cus / blocks(p.pre_qb), 4, &p.pre_ns, &p.pre_tpc);
+    int ns = dev.cus / blocks(p.pre_qb);
+    const long seqs = (long)a.b.batch * a.c.nkv;
+    if (p.step && !rows && p.pre_qb == 1 && own_tiles <= kBothTiles && seqs <= 2 * dev.cus) {
+      // One launch for both, one workgroup a compute unit at a time.  In 1000 cycles a
+      // prefix's takes 16 and 3 a tile, a sequence's (in one chunk) 18 and 1 / 2: chunks such
+      // that the sequences find room beside the prefix
+      long best = LONG_MAX;
+      const int most_ns = std::max(1, std::min({dev.cus / blocks(1), ceil_div(all, 4), 256}));
+      for (int n = 1; n <= most_ns; ++n) {
+        const long room = dev.cus - (long)n * blocks(1), pre = 16 + 3 * ceil_div(all, n);
+        const long step = 18 + own_tiles / 2;
+        const long t = room > 0 ? std::max(pre, (seqs + room - 1) / room * step)
+                                : pre + (seqs + dev.cus - 1) / dev.cus * step;
+        if (t < best) {
+          best = t;
+          ns = n;
+        }
+      }
+      p.pre_blocks = blocks(1) / a.c.nkv;
+      p.step_ns = 1;
+      p.step_tpc = ceil_div(own_tiles, kStepWaves) * kStepWaves;
+    }
+    cut(all, ns, p.pre_blocks > 0 ? 1 : 4, &p.pre_ns, &p.pre_tpc);
   }
   if (p.step && (p.step_ns > 1 || p.pre_ns > 0)) {
     const size_t n = (size_t)a.b.batch * a.c.nkv * p.step_ns * p.step_rows;
@@ -1211,7 +1288,10 @@ void launch_rows(const KvAttn &a, const KvPlan &p, int rows, int ns, int z, hipS
 template <int HD, int TYPE, bool CAP>
 void launch_typed(const KvAttn &a, const KvPlan &p, hipStream_t stream) {
   const int nkv = a.c.nkv, batch = a.b.batch;
-  if (p.step)
+  if (p.pre_blocks > 0)
+    kv_both_kernel<HD, TYPE, CAP>
+        <<<(p.pre_blocks * p.pre_ns + batch) * nkv, 64 * kStepWaves, 0, stream>>>(a, p);
+  else if (p.step)
     kv_step_kernel<HD, TYPE, CAP>
         <<<dim3(p.step_ns, nkv, batch), 64 * kStepWaves, 0, stream>>>(a, p);
   if (p.rows_ns > 0) {
@@ -1220,7 +1300,7 @@ void launch_typed(const KvAttn &a, const KvPlan &p, hipStream_t stream) {
     else
       launch_rows<HD, TYPE, CAP, 1, false>(a, p, a.b.max_rows, p.rows_ns, batch, stream);
   }
-  if (p.pre_ns > 0) {
+  if (p.pre_ns > 0 && p.pre_blocks == 0) {
     if (p.pre_qb == 2)
       launch_rows<HD, TYPE, CAP, 2, true>(a, p, a.b.rows, p.pre_ns, 1, stream);
     else
