@@ -405,9 +405,12 @@ __device__ __forceinline__ int wave_max_all(int v) {
 // ---- single tokens ------------------------------------------------------------
 // A workgroup takes up to 16 query vectors of one sequence and kv head, and a chunk
 // of its keys, whose tiles its four waves share out.  Codes go straight from memory
-// to registers, a tile ahead of their use; 24 KB and more in flight a wave.  Bound by
-// the cache's bytes: per 32 keys (16 KB) a wave spends about 1000 cycles of products and
-// 1500 of vector work on what takes 1200 to arrive at the card's rate.
+// to registers, a tile (16 KB of 256 dims) ahead of their use.  Bound by the cache's bytes
+// where there are many: 32 gemma-3-4b tokens of up to 8192 int8 positions (335 MB) take 72
+// us, 4.7 TB/s of the 5.1 that a large copy reaches; two gemma-3-1b ones of 131072 e4m3
+// positions (136 MB) 30 us.  Few keys are a chain of round trips to memory (tables, page ids,
+// the query and codes, each about a microsecond) and code fetched cold: one token of 1001
+// positions takes 9 to 10 us.
 
 // The keys that a sequence's rows see: tiles t0 .. t1 - 1, from `from` on.
 struct KvRange {
@@ -608,10 +611,15 @@ __global__ __launch_bounds__(64 * kStepWaves, 2) void kv_step_kernel(KvAttn a, K
 }
 
 // ---- prompt rows and shared prefixes ---------------------------------------------
-// A workgroup takes 64 QB query vectors of a kv head, 16 QB a wave, and a chunk of
-// their keys; PRE: the rows of all sequences, over the shared prefix.  Each tile's
-// codes are made f16 once, a share by each wave, and reach the others through LDS in
-// operand order (16-byte reads of 64 lanes in a row: no conflicts).
+// A workgroup of NW waves takes 16 NW QB query vectors of a kv head, 16 QB a wave, and a
+// chunk of their keys; PRE: the rows of all sequences, over the shared prefix.  Each
+// tile's codes are made f16 once, a share by each wave, and reach the others through LDS in
+// operand order (16-byte reads of 64 lanes in a row: no conflicts).  128 vectors of 256
+// dims are eight waves of 16: two a SIMD hide more of each other's waits than one of 32
+// vectors (two 2048-token gemma-3-4b prompts in a window of 1024: 85 us, 93 with four waves).
+// Their 4100 cycles a tile are 2050 of products, about 2600 of LDS traffic (every wave
+// reads all of a tile's fragments) and 1800 of vector work, which overlap in part; a third
+// of the whole is the card's wait for the workgroups that have the most keys.
 //
 // Tiles are pipelined so that the vector unit works while the matrix cores do: the
 // scores of tile t + 1 run with the weights of tile t, the value products of tile t with
@@ -1202,10 +1210,11 @@ KvPlan plan(const KvAttn &a, const DeviceInfo &dev) {
   auto blocks = [&](int qb) {
     return (int)std::max<long>(1, (vecs_kv + 64 * qb - 1) / (64 * qb)) * a.c.nkv;
   };
-  // A workgroup of 128 vectors takes 4500 cycles a tile and 27000 to begin, one of 64 3080
-  // and 16000, and writes half as much for the merge where there are chunks: short runs take
-  // 64.  Of gemma-3-1b over 16384 keys, merge included: 256 vectors 31 us and 37 (128), 512
-  // vectors 44 and 46, four prompts of 512 behind 1536 85 and 80
+  // A workgroup of 128 vectors of 256 dims takes 4100 cycles a tile and 25000 to begin, one
+  // of 64 3000 and 16000, and writes half as much for the merge where there are chunks:
+  // short runs take 64.  gemma-3-1b behind 16384 positions, merge included: 256 vectors (8
+  // tiles by 64 vectors a compute unit) 30 us with 64 and 35 with 128, 512 vectors (16) 42
+  // and 42; a 613-row chunk (10) 39 and 44, 1024 rows of gemma-3-4b (16) 46 and 44
   auto block_rows = [&](int tiles) {
     return vecs_kv > 64 && (long)blocks(1) * tiles > (long)kLongRun * dev.cus ? 2 : 1;
   };

@@ -9,7 +9,9 @@
 //
 // One group of hdim / 4 lanes per row and head, 16 bytes a lane: each value is
 // read once and stays in registers between the maximum and the codes.  Bound by
-// memory for prompts (9 bytes move per value), by the launch for single tokens.
+// memory for prompts (5 bytes and a part of a scale move per value, each way): four of up to
+// 4096 rows of gemma-3-4b are written in 26 us and read in 21, 3.7 and 4.6 TB/s of the 5.1
+// that a large copy reaches; by the launch for single tokens (3 us each).
 #include "gh_arith.h"
 #include "gh_kernels.h"
 
