@@ -1123,14 +1123,15 @@ __global__ __launch_bounds__(64 * (SHARE > kMergeWaves ? SHARE : kMergeWaves)) v
     return v;
   };
   float m = kFloor, l = 0.0f, x[E] = {};
-  constexpr int A = 4;  // chunks loaded at a time
+  constexpr int A = SHARE == 16 ? 8 : 4;  // chunks loaded at a time
   for (int c = part; c < total; c += A * SHARE) {
     float2 v[A];
     float y[A][E];
 #pragma unroll
     for (int u = 0; u < A; ++u) {
+      if (c + u * SHARE >= total) break;
       const float *o;
-      v[u] = where(min(c + u * SHARE, total - 1), &o);
+      v[u] = where(c + u * SHARE, &o);
 #pragma unroll
       for (int e = 0; e < E; ++e) y[u][e] = o[E * lane + e];
     }
