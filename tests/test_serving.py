@@ -697,6 +697,22 @@ def test_attention_many_rows_over_many_keys(gh, heads, kv, hdim, kind, slide, ca
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("hdim,kind", [(128, "e4m3"), (256, "i8")])
+def test_attention_prefix_beside_long_or_many_sequences(gh, hdim, kind):
+    """Single tokens behind a prefix in launches of their own: one with more than 64 tiles of
+    keys of its own, and more than 512 sequences by key/value heads."""
+    rng = np.random.default_rng(21)
+    p = Paged([(1, 3500), (2, 1300), (1, 900), (0, 1100), (1, 1025)], 1, hdim, 32, KINDS[kind],
+              rng, shared=1024)
+    p.fill(rng)
+    check_attention(gh, p, 4, 0, 0.0, False, 1024, 0.0625, rng)
+    check_attention(gh, p, 4, 700, 20.0, False, 1024, 0.0625, rng)
+    p = Paged([(i % 3, 64 + i % 70) for i in range(301)], 2, hdim, 16, KINDS[kind], rng, shared=64)
+    p.fill(rng)
+    check_attention(gh, p, 4, 0, 0.0, False, 64, 0.0625, rng)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("hdim", [128, 256])
 def test_rows_without_a_page_table(gh, hdim):
     """Sequences of rows and no positions need no pages: nothing is written, and what is
