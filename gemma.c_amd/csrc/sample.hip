@@ -67,6 +67,12 @@ __device__ __forceinline__ float logit_at(u64 place) {
 __device__ __forceinline__ double octaves(float l, double c) {
   return l == INFINITY ? kInfZ : (double)l * c;
 }
+// ... times kPerOctave (c16 is c times that, a power of two: the same to the bit); INF: some
+// logit may be infinite
+template <bool INF>
+__device__ __forceinline__ double steps(float l, double c16) {
+  return INF && l == INFINITY ? kInfZ * kPerOctave : (double)l * c16;
+}
 
 // 2^x in fp64 for x <= 0 (0 below -1000): x = e + j / 128 + r, the table's 2^(j/128)
 // (exp_tab_load) and the Taylor polynomial of 2^r, |r| <= 2^-8 (truncation below
@@ -130,9 +136,12 @@ __device__ __forceinline__ Grid grid_of(float most, double c) {
   const double z = octaves(most, c);
   return {floor(z * kPerOctave), ceil(z)};
 }
-__device__ __forceinline__ int bin_of(double z, double gmax) {
-  const double d = gmax - floor(z * kPerOctave);
+__device__ __forceinline__ int bin_at(double y, double gmax) {  // y: z kPerOctave
+  const double d = gmax - floor(y);
   return d >= kBins - 1 ? kBins - 1 : (int)d;
+}
+__device__ __forceinline__ int bin_of(double z, double gmax) {
+  return bin_at(z * kPerOctave, gmax);
 }
 // The power of two that no weight of a bin exceeds, relative to the row's.
 __device__ __forceinline__ double bin_top(int bin, const Grid &g) {
@@ -155,7 +164,7 @@ struct Row {
   uint32_t at[kBinsGap];     // list position of the bin's tokens, kNone: not collected
   uint32_t fill[kBinsGap];   // tokens of the bin in the list so far
   uint32_t listed;        // tokens of the bins that matter, kNone: more than the list takes
-  uint32_t pad;
+  uint32_t last;          // the last of them
   __device__ double weight(int i) const { return __longlong_as_double((long long)sum_m[gap(i)]); }
   __device__ double weight_before(int i) const { return i > 0 ? weight(i - 1) : 0.0; }
   __device__ uint32_t count_before(int i) const { return i > 0 ? sum_c[gap(i - 1)] : 0u; }
@@ -303,7 +312,16 @@ __device__ void decide(const Settings &st, Row &r) {
     r.at[gap(kPerLane * lane + e)] = need[e] ? run - sum + own[e] : kNone;
     r.fill[gap(kPerLane * lane + e)] = 0;
   }
-  if (lane == 63) r.listed = run <= kList ? run : kNone;
+  int last = 0;
+#pragma unroll
+  for (int e = 0; e < kPerLane; ++e)
+    if (need[e]) last = kPerLane * lane + e;
+  const u64 some = __ballot(last > 0);
+  last = __shfl(last, some != 0 ? 63 - __clzll(some) : 0, 64);
+  if (lane == 63) {
+    r.listed = run <= kList ? run : kNone;
+    r.last = last;
+  }
 }
 
 // Working memory of pick() and of what it calls.
@@ -774,15 +792,29 @@ struct Binner {
   uint32_t rest_c = 0;
   u64 rest_m = 0;
   __device__ __forceinline__ Binner(u64 *b, Rest *r) : bins(b), rest(r) {}
-  __device__ __forceinline__ void add(float l, double c, const Grid &g, const double *tab) {
+  template <bool INF>
+  __device__ __forceinline__ void add(float l, double c16, const Grid &g, const double *tab) {
     if (!has_place(l)) return;
-    const double z = octaves(l, c), y = z * kPerOctave, f = floor(y), d = g.gmax - f;
+    const double y = steps<INF>(l, c16), f = floor(y), d = g.gmax - f;
     if (d < kBins - 1) {
       atomicAdd(&bins[(int)d], bin_term(y - f));
     } else {
       ++rest_c;
-      const double x = z - bin_top(kBins - 1, g);
+      const double x = y * (1.0 / kPerOctave) - bin_top(kBins - 1, g);
       if (x > -64.0) rest_m += units(pow2(x, tab), kUnit);
+    }
+  }
+  // a thread's logits, of which `most` is the workgroup's largest
+  template <int N>
+  __device__ __forceinline__ void add_all(const float (&x)[N], float most, double c, const Grid &g,
+                                          const double *tab) {
+    const double c16 = c * kPerOctave;
+    if (most == INFINITY) {
+#pragma unroll 1
+      for (int e = 0; e < N; ++e) add<true>(x[e], c16, g, tab);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) add<false>(x[e], c16, g, tab);
     }
   }
   __device__ __forceinline__ void finish() {
@@ -838,8 +870,7 @@ __global__ __launch_bounds__(kThreads) void sample_whole_kernel(Sample a) {
   if (!has_place(most)) return pick_none(a, row);
   const Grid g = grid_of(most, st.c);
   Binner bins(s.mass, &rest);
-#pragma unroll
-  for (int e = 0; e < kWhole; ++e) bins.add(x[e], st.c, g, s.tab);
+  bins.add_all(x, most, st.c, g, s.tab);
   bins.finish();
   if (tid == 0) {
     s.row.g = g;
@@ -909,8 +940,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_bins_kernel(Sample a, Wo
   }
   const Grid g = grid_of(most, c);
   Binner bins(count, &rest);
-#pragma unroll
-  for (int e = 0; e < kPer; ++e) bins.add(x[e], c, g, tab);
+  bins.add_all(x, most, c, g, tab);
   bins.finish();
   __syncthreads();
   out->bins[tid] = count[tid];
@@ -1043,14 +1073,18 @@ __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(Sample a,
   if (!__syncthreads_or(here)) return;
   float x[kPer];
   load_chunk(a, row, x);
-  const double c = octave_scale(a, row);
+  // logits below the last of these bins are most of a row's: told by a bound a little lower
+  const double c16 = octave_scale(a, row) * kPerOctave;
+  const uint32_t last = r->last;
+  const double end = (g.gmax - last) / c16;  // (0 / 0 of a row of equal weights: no bound)
+  const float least = last < kBins - 1 ? (float)(end - fabs(end) * 0x1p-22) : -INFINITY;
   int bin[kPer];
   uint32_t slot[kPer];
 #pragma unroll
   for (int e = 0; e < kPer; ++e) {
     bin[e] = -1;
-    if (!has_place(x[e])) continue;
-    const int i = bin_of(octaves(x[e], c), g.gmax);
+    if (!has_place(x[e]) || x[e] < least) continue;
+    const int i = bin_at(steps<true>(x[e], c16), g.gmax);
     if (at[i] == kNone) continue;
     bin[e] = i;
     slot[e] = atomicAdd(&count[i], 1u);
