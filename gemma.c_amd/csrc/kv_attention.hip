@@ -1204,8 +1204,12 @@ KvPlan plan(const KvAttn &a, const DeviceInfo &dev) {
     const int n = std::min(a.b.max_rows, kStepRows / p.group);
     // two workgroups a compute unit are resident: more than that is rounds of them.  32
     // sequences of up to 8192 keys and 4 kv heads: 72 us with 2, 73 with 1, 82 with 4
-    cut(tiles(n), 2 * dev.cus / std::max(1, a.b.batch * a.c.nkv), kStepWaves, &p.step_ns,
-        &p.step_tpc);
+    // ... and few keys are one chunk, without a merge: a tile more a wave is 0.85 us of 256 dims,
+    // the merge about 2.  A token over 200 positions 10.2 us and 10.7 (split), over 330 11.8
+    // and 11.2; of 128 dims over 330 7.2 and 7.8, over 460 8.1 and 7.6 (int8; e4m3 7.5 and 7.7)
+    const bool few = tiles(n) * a.c.hdim <= 8 * 256;
+    cut(tiles(n), few ? 1 : 2 * dev.cus / std::max(1, a.b.batch * a.c.nkv), kStepWaves,
+        &p.step_ns, &p.step_tpc);
   }
   const long vecs_kv = (long)a.b.rows * p.group;  // query vectors of a kv head
   auto blocks = [&](int qb) {
