@@ -15,15 +15,16 @@
 // 64-bit sum, exact in any order.  Sums over bins and workgroups are fp64 in one order.
 // So equal calls give equal bits.
 //
-// Up to kWholeVocab columns a workgroup does a row by itself.  Longer rows take four
+// Up to kWholeVocab columns a workgroup does a row by itself, from registers.  Longer rows take four
 // launches: each 8192-column chunk's bins, from its own largest logit down so that one
 // reading does (sample_bins_kernel); their sum and the bins that matter
 // (sample_decide_kernel); these bins' tokens (sample_collect_kernel; chunks that
 // hold none are not read again); and the targets inside them (sample_pick_kernel).
 //
-// Of 262144 columns, us: one row by top-k 64 and top-p 0.95 8 + 13 + 6 + 8, four chains of
-// round trips and of code fetched cold; 64 rows with settings of all kinds (67 MB) 28 + 13 +
-// 18 + 27: the first by its vector work and the LDS's 64-bit sums (2.4 TB/s), the last by the
+// Of 16000 columns one row by top-k 64 and top-p 0.95 takes 17 us, 64 rows with settings of
+// all kinds 22 (24 and 37 when the bins' tokens are looked for in the row, not in a list).
+// Of 262144 columns, us: the one row 8 + 13 + 5 + 8, four chains of round trips and of code
+// fetched cold; the 64 rows (67 MB) 26 + 13 + 18 + 28: the first by its vector work and the LDS's 64-bit sums (2.4 TB/s), the last by the
 // rows that cut deep into a flat part, a workgroup each.
 #include <float.h>
 #include <limits.h>
@@ -44,6 +45,7 @@ constexpr int kChunkThreads = 512;
 constexpr int kPer = kChunk / kChunkThreads;
 constexpr int kThreads = 1024;     // ... of the kernels that see whole rows
 constexpr int kWholeVocab = 16384;
+constexpr int kWholeList = 4096;   // their tokens that are put into LDS, at most
 constexpr int kRanked = 256;       // tokens that are put in order by comparing all pairs
 constexpr int kSubs = 1024;        // parts of a bin with more
 constexpr int kList = 32768;       // tokens of a row's bins that are collected, at most
@@ -346,7 +348,8 @@ struct Found {
 };
 
 // Where pick() finds the tokens of the bins that matter: in the row's list, of which one
-// bin at a time is brought to LDS; null: in the row alone.
+// bin at a time is brought to LDS (staged; null: the list is there already); null: in the
+// row alone.
 constexpr int kStaged = 8192;
 struct Source {
   const u64 *list;
@@ -358,7 +361,7 @@ struct Source {
 __device__ __forceinline__ bool stage(const Source &src, const Row &r, int bin) {
   constexpr int kAhead = 8;
   const uint32_t n = r.count_of(bin);
-  if (src.list == nullptr || r.listed == kNone || r.at[gap(bin)] == kNone || n > kStaged) return false;
+  if (src.staged == nullptr || r.listed == kNone || r.at[gap(bin)] == kNone || n > kStaged) return false;
   const u64 *from = src.list + r.at[gap(bin)];
   u64 p[kAhead];
 #pragma unroll
@@ -850,6 +853,7 @@ __global__ __launch_bounds__(kThreads) void sample_whole_kernel(Sample a) {
   __shared__ float red[kThreads / 64];
   __shared__ double mass[kBinsGap];
   __shared__ Rest rest;
+  __shared__ u64 list[kWholeList];
   const int row = blockIdx.x, tid = threadIdx.x;
   const float *l = a.logits + row * a.stride;
   const Settings st = settings(a, row);
@@ -875,7 +879,6 @@ __global__ __launch_bounds__(kThreads) void sample_whole_kernel(Sample a) {
   if (tid == 0) {
     s.row.g = g;
     s.row.zmax = octaves(most, st.c);
-    s.row.listed = kNone;
   }
   __syncthreads();
   if (tid < kBins) {
@@ -886,7 +889,20 @@ __global__ __launch_bounds__(kThreads) void sample_whole_kernel(Sample a) {
   __syncthreads();
   sum_bins(s.count, mass, s.row);
   __syncthreads();
-  pick(a, row, st, Source{nullptr, nullptr}, 0, s);
+  decide(st, s.row);
+  __syncthreads();
+  const bool fits = s.row.listed <= kWholeList;
+  if (fits) {
+#pragma unroll
+    for (int e = 0; e < kWhole; ++e) {
+      if (!has_place(x[e])) continue;
+      const int bin = gap(bin_of(octaves(x[e], st.c), g.gmax));
+      if (s.row.at[bin] != kNone)
+        list[s.row.at[bin] + atomicAdd(&s.row.fill[bin], 1u)] = place(x[e], tid + e * kThreads);
+    }
+  }
+  __syncthreads();
+  pick(a, row, st, Source{fits ? list : nullptr, nullptr}, list[min(tid, kRanked - 1)], s);
 }
 
 // ---- long rows --------------------------------------------------------------------
