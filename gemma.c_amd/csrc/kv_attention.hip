@@ -639,10 +639,51 @@ struct RowsLds {
   u4 raw_k[NW][3][KU][64], raw_v[NW][3][VL][64];
 };
 
-// block: of nblocks, chunks of a tile of rows in a row.
+// Prompt rows are cut into tiles of tr query vectors, sequence by sequence and the last rows,
+// which see most, first.  Where the id-th lies; false past the last.  By each wave, 64
+// sequences at a time: a grid of all sequences by the longest one's tiles would be mostly
+// workgroups that find nothing to do (a 2048-row prompt beside 200 single tokens: 255 us).
+__device__ __forceinline__ bool find_tile(const KvAttn &a, const KvPlan &pl, int tr, int id, int *b,
+                                          int *tile) {
+  const int lane = threadIdx.x & 63;
+  for (int base = 0; base < a.b.batch; base += 64) {
+    int sum = 0;
+    if (base + lane < a.b.batch) {
+      const int rows = kv_seq(a.b, base + lane).n * pl.group;
+      sum = pl.step && rows <= kStepRows ? 0 : (rows + tr - 1) / tr;
+    }
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int t = __shfl_up(sum, off, 64);
+      if (lane >= off) sum += t;
+    }
+    const unsigned long long past = __ballot(sum > id);
+    if (past != 0) {
+      const int l = __builtin_amdgcn_readfirstlane(__ffsll(past) - 1);
+      *b = base + l;
+      *tile = __builtin_amdgcn_readlane(sum, l) - 1 - id;
+      return true;
+    }
+    id -= __builtin_amdgcn_readlane(sum, 63);
+  }
+  return false;
+}
+// The sequence that row r is in, if it is in one.
+__device__ __forceinline__ int find_row(const KvBatch &b, int r) {
+  const int lane = threadIdx.x & 63;
+  int last = 0;
+  for (int base = 0; base < b.batch; base += 64) {
+    const unsigned long long from = __ballot(base + lane < b.batch && b.row0[min(base + lane, b.batch)] <= r);
+    if (from != 0) last = base + __popcll(from) - 1;
+    if (from != ~0ull) break;
+  }
+  return __builtin_amdgcn_readfirstlane(last);
+}
+
+// block_x: of nblocks, the chunks of a tile of rows one after the other.
 template <int HD, int TYPE, bool CAP, int QB, int NW, bool PRE>
 __device__ __forceinline__ void rows_keys(const KvAttn &a, const KvPlan &pl, int block_x,
-                                          int nblocks, int hk, int b, RowsLds<HD, NW> &lds) {
+                                          int nblocks, int hk, RowsLds<HD, NW> &lds) {
   typedef RowsLds<HD, NW> L;
   constexpr int NB = L::NB, KS = L::KS, ND = L::ND, KU = L::KU, VD = L::VD, VL = L::VL;
   constexpr int TR = 16 * NW * QB, VP = 4;  // VP: value fragments read ahead
@@ -653,8 +694,9 @@ __device__ __forceinline__ void rows_keys(const KvAttn &a, const KvPlan &pl, int
   auto &raw_k = lds.raw_k;
   auto &raw_v = lds.raw_v;
   const int ns = PRE ? pl.pre_ns : pl.rows_ns, tpc = PRE ? pl.pre_tpc : pl.rows_tpc;
-  // the last rows, which see most, first
-  const int chunk = block_x % ns, tile = nblocks / ns - 1 - block_x / ns;
+  const int chunk = block_x % ns;
+  int b = 0, tile = nblocks / ns - 1 - block_x / ns;
+  if (!PRE && !find_tile(a, pl, TR, block_x / ns, &b, &tile)) return;
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   KvSeq s = kv_seq(a.b, b);
@@ -663,8 +705,6 @@ __device__ __forceinline__ void rows_keys(const KvAttn &a, const KvPlan &pl, int
     s.r0 = kv_clamp(a.b.row0[0], 0, a.b.rows);
     s.n = kv_clamp(a.b.row0[a.b.batch], s.r0, a.b.rows) - s.r0;
     len = a.shared;
-  } else if (pl.step && s.n * pl.group <= kStepRows) {
-    return;
   }
   const int rows = s.n * pl.group, at = tile * TR;
   if (at >= rows) return;
@@ -1042,8 +1082,7 @@ __device__ __forceinline__ void rows_keys(const KvAttn &a, const KvPlan &pl, int
 template <int HD, int TYPE, bool CAP, int QB, int NW, bool PRE>
 __global__ __launch_bounds__(64 * NW) void kv_rows_kernel(KvAttn a, KvPlan pl) {
   __shared__ RowsLds<HD, NW> lds;
-  rows_keys<HD, TYPE, CAP, QB, NW, PRE>(a, pl, blockIdx.x, gridDim.x, blockIdx.y,
-                                        PRE ? 0 : blockIdx.z, lds);
+  rows_keys<HD, TYPE, CAP, QB, NW, PRE>(a, pl, blockIdx.x, gridDim.x, blockIdx.y, lds);
 }
 
 // The shared prefix and what single tokens' sequences have of their own in one launch: each
@@ -1058,7 +1097,7 @@ __global__ __launch_bounds__(64 * kStepWaves) void kv_both_kernel(KvAttn a, KvPl
   } lds;
   const int blocks = pl.pre_blocks * pl.pre_ns, id = blockIdx.x;
   if (id < blocks * a.c.nkv) {
-    rows_keys<HD, TYPE, CAP, 1, NW, true>(a, pl, id % blocks, blocks, id / blocks, 0, lds.rows);
+    rows_keys<HD, TYPE, CAP, 1, NW, true>(a, pl, id % blocks, blocks, id / blocks, lds.rows);
   } else {
     const int i = id - blocks * a.c.nkv;  // one chunk
     step_keys<HD, TYPE, CAP>(a, pl, 0, i % a.c.nkv, i / a.c.nkv, lds.step);
@@ -1077,12 +1116,15 @@ __global__ __launch_bounds__(64 * (SHARE > kMergeWaves ? SHARE : kMergeWaves)) v
     KvAttn a, KvPlan pl) {
   constexpr int E = HD / 64, W = SHARE > kMergeWaves ? SHARE : kMergeWaves;
   __shared__ float so[SHARE][HD], sm[SHARE], sl[SHARE];
-  const int b = blockIdx.y, lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave % SHARE;
+  // single tokens: of sequence blockIdx.y; prompt rows: of all sequences, one after the other
+  const int v = blockIdx.x * (W / SHARE) + wave / SHARE, head = v % a.n_heads;
+  const int b = STEP ? blockIdx.y : find_row(a.b, v / a.n_heads);
   const KvSeq s = kv_seq(a.b, b);
-  const int v = blockIdx.x * (W / SHARE) + wave / SHARE, i = v / a.n_heads, head = v % a.n_heads;
+  const int i = v / a.n_heads - (STEP ? 0 : s.r0);
   const bool step = pl.step && s.n * pl.group <= kStepRows;
-  if (i >= s.n || step != STEP) return;  // (a whole workgroup's, where its waves share)
+  if (i < 0 || i >= s.n || step != STEP) return;  // (a whole workgroup's, where its waves share)
   const int hk = head / pl.group, j = i * pl.group + head % pl.group, p0 = s.len - s.n;
   const size_t vec = (size_t)(s.r0 + i) * a.n_heads + head;
   // this row's own chunks: number, first partial and the step to the next
@@ -1281,7 +1323,7 @@ KvPlan plan(const KvAttn &a, const DeviceInfo &dev) {
 // wave each and 8.4 with four, 256 of 64 chunks 6.1 with 16.
 template <int HD, bool STEP>
 void launch_merge(const KvAttn &a, const KvPlan &p, int chunks, int rows, hipStream_t stream) {
-  const int vecs = rows * a.n_heads, batch = a.b.batch;
+  const int vecs = rows * a.n_heads, batch = STEP ? a.b.batch : 1;
   if (chunks > 16)
     kv_merge_kernel<HD, 16, STEP><<<dim3(vecs, batch), 1024, 0, stream>>>(a, p);
   else if (chunks > 8)
@@ -1293,10 +1335,15 @@ void launch_merge(const KvAttn &a, const KvPlan &p, int chunks, int rows, hipStr
 
 // 64 B query vectors a workgroup.
 template <int HD, int TYPE, bool CAP, int B, bool PRE>
-void launch_rows(const KvAttn &a, const KvPlan &p, int rows, int ns, int z, hipStream_t stream) {
+void launch_rows(const KvAttn &a, const KvPlan &p, hipStream_t stream) {
   constexpr int NW = B == 2 && HD == 256 ? 8 : 4, QB = B * 4 / NW;
-  kv_rows_kernel<HD, TYPE, CAP, QB, NW, PRE>
-      <<<dim3(ceil_div(rows * p.group, 64 * B) * ns, a.c.nkv, z), 64 * NW, 0, stream>>>(a, p);
+  const int vecs = a.b.rows * p.group;
+  // tiles: one more than the whole ones for each sequence, of which there are so many
+  const int tiles = PRE ? ceil_div(vecs, 64 * B)
+                        : vecs / (64 * B) + std::min(a.b.batch, vecs / (p.step ? kStepRows + 1 : p.group));
+  if (tiles > 0)
+    kv_rows_kernel<HD, TYPE, CAP, QB, NW, PRE>
+        <<<dim3(tiles * (PRE ? p.pre_ns : p.rows_ns), a.c.nkv), 64 * NW, 0, stream>>>(a, p);
 }
 
 template <int HD, int TYPE, bool CAP>
@@ -1310,20 +1357,20 @@ void launch_typed(const KvAttn &a, const KvPlan &p, hipStream_t stream) {
         <<<dim3(p.step_ns, nkv, batch), 64 * kStepWaves, 0, stream>>>(a, p);
   if (p.rows_ns > 0) {
     if (p.qb == 2)
-      launch_rows<HD, TYPE, CAP, 2, false>(a, p, a.b.max_rows, p.rows_ns, batch, stream);
+      launch_rows<HD, TYPE, CAP, 2, false>(a, p, stream);
     else
-      launch_rows<HD, TYPE, CAP, 1, false>(a, p, a.b.max_rows, p.rows_ns, batch, stream);
+      launch_rows<HD, TYPE, CAP, 1, false>(a, p, stream);
   }
   if (p.pre_ns > 0 && p.pre_blocks == 0) {
     if (p.pre_qb == 2)
-      launch_rows<HD, TYPE, CAP, 2, true>(a, p, a.b.rows, p.pre_ns, 1, stream);
+      launch_rows<HD, TYPE, CAP, 2, true>(a, p, stream);
     else
-      launch_rows<HD, TYPE, CAP, 1, true>(a, p, a.b.rows, p.pre_ns, 1, stream);
+      launch_rows<HD, TYPE, CAP, 1, true>(a, p, stream);
   }
   if (p.step)
     launch_merge<HD, true>(a, p, p.step_ns + p.pre_ns, std::min(a.b.max_rows, kStepRows / p.group),
                            stream);
-  if (p.rows_ns > 0) launch_merge<HD, false>(a, p, p.rows_ns + p.pre_ns, a.b.max_rows, stream);
+  if (p.rows_ns > 0) launch_merge<HD, false>(a, p, p.rows_ns + p.pre_ns, a.b.rows, stream);
 }
 
 template <int HD>
