@@ -1054,8 +1054,8 @@ int kv_args(const char *name, const gemma_hip_cache *cache, const gemma_hip_batc
     return fail("%s: bad batch: %d sequences, %d rows (%d at most), %d positions in %d pages of %d",
                 name, batch->batch, batch->rows, batch->max_rows, batch->max_len,
                 batch->max_pages, page);
-  if ((long)batch->max_rows * cache->nkv > kKvMostVecs)
-    return fail("%s: too many rows: %d of %d heads", name, batch->max_rows, cache->nkv);
+  if ((long)batch->rows * cache->nkv > kKvMostVecs)
+    return fail("%s: too many rows: %d of %d heads", name, batch->rows, cache->nkv);
   int shift = 0;
   while ((1 << shift) < page) ++shift;
   *c = gh::KvCache{(uint8_t *)cache->k, (uint8_t *)cache->v, cache->ks, cache->vs,

@@ -668,17 +668,6 @@ __device__ __forceinline__ bool find_tile(const KvAttn &a, const KvPlan &pl, int
   }
   return false;
 }
-// The sequence that row r is in, if it is in one.
-__device__ __forceinline__ int find_row(const KvBatch &b, int r) {
-  const int lane = threadIdx.x & 63;
-  int last = 0;
-  for (int base = 0; base < b.batch; base += 64) {
-    const unsigned long long from = __ballot(base + lane < b.batch && b.row0[min(base + lane, b.batch)] <= r);
-    if (from != 0) last = base + __popcll(from) - 1;
-    if (from != ~0ull) break;
-  }
-  return __builtin_amdgcn_readfirstlane(last);
-}
 
 // block_x: of nblocks, the chunks of a tile of rows one after the other.
 template <int HD, int TYPE, bool CAP, int QB, int NW, bool PRE>
@@ -1120,7 +1109,7 @@ __global__ __launch_bounds__(64 * (SHARE > kMergeWaves ? SHARE : kMergeWaves)) v
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave % SHARE;
   // single tokens: of sequence blockIdx.y; prompt rows: of all sequences, one after the other
   const int v = blockIdx.x * (W / SHARE) + wave / SHARE, head = v % a.n_heads;
-  const int b = STEP ? blockIdx.y : find_row(a.b, v / a.n_heads);
+  const int b = STEP ? blockIdx.y : kv_find_wave(a.b, v / a.n_heads);
   const KvSeq s = kv_seq(a.b, b);
   const int i = v / a.n_heads - (STEP ? 0 : s.r0);
   const bool step = pl.step && s.n * pl.group <= kStepRows;

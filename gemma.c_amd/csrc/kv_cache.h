@@ -74,6 +74,21 @@ GH_HD int kv_find(const int *row0, int batch, int r) {
   return lo;
 }
 
+#ifdef __HIPCC__
+// The sequence that row r is in if it is in one, else any; by a whole wave, for one row.
+__device__ __forceinline__ int kv_find_wave(const KvBatch &b, int r) {
+  const int lane = threadIdx.x & 63;
+  int last = 0;
+  for (int base = 0; base < b.batch; base += 64) {
+    const bool from = base + lane < b.batch && b.row0[base + lane] <= r;
+    const unsigned long long all = __ballot(from);
+    if (all != 0) last = base + __popcll(all) - 1;
+    if (all != ~0ull) break;
+  }
+  return __builtin_amdgcn_readfirstlane(last);
+}
+#endif
+
 // Keys that a row at position pos sees: lo .. hi (hi < lo: none).
 struct KvSpan {
   int lo, hi;

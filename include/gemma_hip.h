@@ -590,8 +590,7 @@ typedef struct {
  * Sizes that the host knows: `rows`, the rows of the call's buffers (at least
  * row0[batch]; those from row0[batch] on are left as they are); max_rows and
  * max_len, at least every sequence's rows and len (max_len <= max_pages * page).
- * Rows times heads are 2^25 at most (of the longest sequence for cache_write and
- * cache_read, of all for cache_attention).
+ * Rows times heads are 2^25 at most.
  * Lengths and rows are cut to these bounds, and a page id outside the cache stands
  * for positions that aren't there: not written, read as zeros, not attended to. */
 typedef struct {

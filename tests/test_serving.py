@@ -453,6 +453,7 @@ WRITES = {  # sequences (new rows, positions), kv heads, head dim, page
     "prompts": ([(33, 33), (5, 70), (0, 12), (128, 131), (1, 1), (0, 0)], 4, 256, 32),
     "hd128": ([(19, 40), (64, 64), (1, 65)], 3, 128, 64),
     "one_page": ([(7, 300)], 2, 128, 512),
+    "many": ([(i % 3, 3 + i % 40) for i in range(100)] + [(90, 100), (0, 7), (3, 60)], 1, 128, 16),
     "ahead": ([(5, 3), (2, 2)], 2, 256, 16),  # rows before position 0: nowhere
 }
 
@@ -554,6 +555,10 @@ ATTN = {
     "step_24": ([(1, 90), (1, 31)], 24, 2, 256, 16, 0, 0.0, False, 0),
     "few_rows": ([(3, 90), (2, 31), (4, 4)], 4, 1, 256, 16, 0, 0.0, False, 0),
     "prompt": ([(70, 70)], 4, 1, 256, 16, 0, 0.0, False, 0),
+    "many_mixed": ([(i % 3, 3 + i % 40) for i in range(70)] + [(90, 100), (0, 7), (40, 300)] +
+                   [(1 + i % 7, 80 + i) for i in range(60)], 4, 1, 256, 16, 0, 0.0, False, 0),
+    "many_prompts": ([(17 + i % 9, 30 + i) for i in range(67)] + [(0, 0), (70, 900)], 4, 2, 128, 16,
+                     0, 0.0, False, 0),
     "prompt_behind": ([(45, 200), (7, 130)], 8, 4, 256, 64, 0, 0.0, False, 0),
     "prompt_window": ([(130, 220)], 4, 2, 128, 32, 33, 0.0, False, 0),
     "prompt_window_1": ([(40, 50)], 4, 2, 128, 32, 1, 0.0, False, 0),
