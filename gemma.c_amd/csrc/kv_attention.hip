@@ -57,10 +57,10 @@ constexpr float kLog2e = 1.44269502162933349609375f;
 struct KvPlan {
   int group;                    // heads per kv head
   uint32_t inv_group;           // 2^21 / group, rounded up
-  int step, step_ns, step_tpc;  // single tokens: on or off, key chunks, tiles of a chunk
+  int step, step_ns;            // single tokens: on or off, key chunks at most
   int step_rows;                // query vectors of a sequence and kv head, at most
-  int rows_ns, rows_tpc;        // prompt rows (0 chunks: off)
-  int pre_ns, pre_tpc;          // shared prefix (0: none)
+  int rows_ns;                  // prompt rows (0 chunks: off)
+  int pre_ns, pre_tpc;          // shared prefix (0: none), tiles of a chunk
   int pre_blocks;               // its tiles of rows, where one launch takes it and the single
                                 // tokens (0: not)
   int qb, pre_qb;               // 16-query blocks of a wave of the prompt kernel
@@ -68,6 +68,15 @@ struct KvPlan {
 };
 
 __host__ __device__ inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+// Tiles of a chunk, at least, and the whole number of them that a chunk has: what rows see is
+// cut evenly into ns chunks or fewer, by the lengths on the device, of which the host only
+// knows a bound.
+constexpr int kChunkTiles = 4;
+__host__ __device__ inline int chunk_tiles(int tiles, int ns) {
+  const int n = ceil_div(ceil_div(tiles, ns), kChunkTiles) * kChunkTiles;
+  return n > 0 ? n : kChunkTiles;
+}
 
 // tanh(x) to about an ulp: its odd series below 0.35, else from e^-2|x|.
 __device__ __forceinline__ float tanh32(float x) {
@@ -446,7 +455,8 @@ __device__ __forceinline__ void step_keys(const KvAttn &a, const KvPlan &pl, int
   if (s.n == 0 || rows > kStepRows) return;
   const int p0 = s.len - s.n;
   const KvRange kr = key_range(p0, s.len - 1, s.len, a.slide, a.dense, a.shared);
-  const int t0 = kr.t0 + chunk * pl.step_tpc, t1 = min(kr.t1, t0 + pl.step_tpc);
+  const int tpc = chunk_tiles(kr.t1 - kr.t0, pl.step_ns);
+  const int t0 = kr.t0 + chunk * tpc, t1 = min(kr.t1, t0 + tpc);
   if (t0 >= t1 && chunk > 0) return;
 
   // the lane's query
@@ -682,7 +692,7 @@ __device__ __forceinline__ void rows_keys(const KvAttn &a, const KvPlan &pl, int
   auto &scales = lds.scales;
   auto &raw_k = lds.raw_k;
   auto &raw_v = lds.raw_v;
-  const int ns = PRE ? pl.pre_ns : pl.rows_ns, tpc = PRE ? pl.pre_tpc : pl.rows_tpc;
+  const int ns = PRE ? pl.pre_ns : pl.rows_ns;
   const int chunk = block_x % ns;
   int b = 0, tile = nblocks / ns - 1 - block_x / ns;
   if (!PRE && !find_tile(a, pl, TR, block_x / ns, &b, &tile)) return;
@@ -750,12 +760,13 @@ __device__ __forceinline__ void rows_keys(const KvAttn &a, const KvPlan &pl, int
   if (PRE) __syncthreads();  // the search is over, its table goes
   int t0, t1;
   if (PRE) {  // chunks of the whole prefix
-    t0 = chunk * tpc;
-    t1 = min(ceil_div(a.shared, kTile), t0 + tpc);
+    t0 = chunk * pl.pre_tpc;
+    t1 = min(ceil_div(a.shared, kTile), t0 + pl.pre_tpc);
   } else {
     const int i0 = at / pl.group, i1 = min(s.n - 1, (at + TR - 1) / pl.group);
     const KvRange kr = key_range(s.len - s.n + i0, s.len - s.n + i1, s.len, a.slide, a.dense,
                                  a.shared);
+    const int tpc = chunk_tiles(kr.t1 - kr.t0, ns);
     t0 = kr.t0 + chunk * tpc;
     t1 = min(kr.t1, t0 + tpc);
     if (t0 >= t1 && chunk > 0) return;
@@ -1123,7 +1134,7 @@ __global__ __launch_bounds__(64 * (SHARE > kMergeWaves ? SHARE : kMergeWaves)) v
   const float2 *pm;
   if (STEP) {
     const KvRange kr = key_range(p0, s.len - 1, s.len, a.slide, a.dense, a.shared);
-    n = max(1, ceil_div(kr.t1 - kr.t0, pl.step_tpc));
+    n = max(1, ceil_div(kr.t1 - kr.t0, chunk_tiles(kr.t1 - kr.t0, pl.step_ns)));
     first = ((size_t)b * a.c.nkv + hk) * pl.step_ns * pl.step_rows + j;
     stride = pl.step_rows;
     po = (const float *)(a.work + pl.step_o);
@@ -1132,7 +1143,7 @@ __global__ __launch_bounds__(64 * (SHARE > kMergeWaves ? SHARE : kMergeWaves)) v
     const int tr = 64 * pl.qb, at = j / tr * tr;
     const int i0 = at / pl.group, i1 = min(s.n - 1, (at + tr - 1) / pl.group);
     const KvRange kr = key_range(p0 + i0, p0 + i1, s.len, a.slide, a.dense, a.shared);
-    n = max(1, ceil_div(kr.t1 - kr.t0, pl.rows_tpc));
+    n = max(1, ceil_div(kr.t1 - kr.t0, chunk_tiles(kr.t1 - kr.t0, pl.rows_ns)));
     first = vec;
     stride = (size_t)a.b.rows * a.n_heads;
     po = (const float *)(a.work + pl.rows_o);
@@ -1218,10 +1229,9 @@ KvPlan plan(const KvAttn &a, const DeviceInfo &dev) {
     const int keys = a.slide > 0 ? (int)std::min<long>(own, (long)a.slide + n) : own;
     return std::max(1, ceil_div(keys, kTile) + 1);
   };
-  auto cut = [](int tiles, int ns, int unit, int *out_ns, int *out_tpc) {
-    ns = std::max(1, std::min({ns, ceil_div(tiles, unit), 256}));
-    *out_tpc = ceil_div(ceil_div(tiles, ns), unit) * unit;
-    *out_ns = ceil_div(tiles, *out_tpc);
+  // chunks: so many, if there are tiles enough
+  auto cut = [](int tiles, int ns) {
+    return std::max(1, std::min({ns, ceil_div(tiles, kChunkTiles), 256}));
   };
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -1239,8 +1249,7 @@ KvPlan plan(const KvAttn &a, const DeviceInfo &dev) {
     // the merge about 2.  A token over 200 positions 10.2 us and 10.7 (split), over 330 11.8
     // and 11.2; of 128 dims over 330 7.2 and 7.8, over 460 8.1 and 7.6 (int8; e4m3 7.5 and 7.7)
     const bool few = tiles(n) * a.c.hdim <= 8 * 256;
-    cut(tiles(n), few ? 1 : 2 * dev.cus / std::max(1, a.b.batch * a.c.nkv), kStepWaves,
-        &p.step_ns, &p.step_tpc);
+    p.step_ns = cut(tiles(n), few ? 1 : 2 * dev.cus / std::max(1, a.b.batch * a.c.nkv));
   }
   const long vecs_kv = (long)a.b.rows * p.group;  // query vectors of a kv head
   auto blocks = [&](int qb) {
@@ -1257,19 +1266,18 @@ KvPlan plan(const KvAttn &a, const DeviceInfo &dev) {
   const int own_tiles = tiles(std::min(a.b.max_rows, kStepRows / std::min(p.group, kStepRows)));
   auto rows_tiles = [&](int qb) { return tiles(ceil_div(64 * qb, p.group) + 1); };
   p.qb = block_rows(rows_tiles(1));
-  if (rows) cut(rows_tiles(p.qb), dev.cus / blocks(p.qb), 4, &p.rows_ns, &p.rows_tpc);
+  if (rows) p.rows_ns = cut(rows_tiles(p.qb), dev.cus / blocks(p.qb));
   if (a.shared > 0) {
     const int all = ceil_div(a.shared, kTile);
     p.pre_qb = block_rows(all);
-    int ns = dev.cus / blocks(p.pre_qb);
+    int ns = cut(all, dev.cus / blocks(p.pre_qb));
     const long seqs = (long)a.b.batch * a.c.nkv;
     if (p.step && !rows && p.pre_qb == 1 && own_tiles <= kBothTiles && seqs <= 2 * dev.cus) {
       // One launch for both, one workgroup a compute unit at a time.  In 1000 cycles a
       // prefix's takes 16 and 3 a tile, a sequence's (in one chunk) 18 and 1 / 2: chunks such
       // that the sequences find room beside the prefix
       long best = LONG_MAX;
-      const int most_ns = std::max(1, std::min({dev.cus / blocks(1), ceil_div(all, 4), 256}));
-      for (int n = 1; n <= most_ns; ++n) {
+      for (int n = 1, most_ns = ns; n <= most_ns; ++n) {
         const long room = dev.cus - (long)n * blocks(1), pre = 16 + 3 * ceil_div(all, n);
         const long step = 18 + own_tiles / 2;
         const long t = room > 0 ? std::max(pre, (seqs + room - 1) / room * step)
@@ -1281,9 +1289,9 @@ KvPlan plan(const KvAttn &a, const DeviceInfo &dev) {
       }
       p.pre_blocks = blocks(1) / a.c.nkv;
       p.step_ns = 1;
-      p.step_tpc = ceil_div(own_tiles, kStepWaves) * kStepWaves;
     }
-    cut(all, ns, p.pre_blocks > 0 ? 1 : 4, &p.pre_ns, &p.pre_tpc);
+    p.pre_tpc = ceil_div(all, ns);
+    p.pre_ns = ceil_div(all, p.pre_tpc);
   }
   if (p.step && (p.step_ns > 1 || p.pre_ns > 0)) {
     const size_t n = (size_t)a.b.batch * a.c.nkv * p.step_ns * p.step_rows;
@@ -1299,12 +1307,6 @@ KvPlan plan(const KvAttn &a, const DeviceInfo &dev) {
     p.pre_m = take(p.pre_ns * vecs * 8);
   }
   p.bytes = at;
-  // every key of a dense row, in as many chunks
-  if (a.dense && a.slide > 0) {
-    const int all = std::max(1, ceil_div(own, kTile) + 1);
-    if (p.step) p.step_tpc = ceil_div(ceil_div(all, p.step_ns), kStepWaves) * kStepWaves;
-    if (p.rows_ns) p.rows_tpc = ceil_div(all, p.rows_ns);
-  }
   return p;
 }
 

@@ -581,7 +581,7 @@ ATTN = {
 
 
 def check_attention(gh, p, heads, slide, cap, dense, shared, asc, rng, q=None, qpad=8, work=None,
-                    rows=None, step=1):
+                    rows=None, step=1, max_len=None):
     """Runs the call and compares every row (or every step-th) with attend()."""
     import torch
 
@@ -591,8 +591,8 @@ def check_attention(gh, p, heads, slide, cap, dense, shared, asc, rng, q=None, q
         q = rng.standard_normal((rows, heads * hd + qpad)).astype(F32)
     c = p.device()
     out = torch.full((rows, heads * hd), 3.0, device="cuda")
-    gh.cache_attention(out, cuda(q), q.shape[1], c, p.batch(rows), heads, slide, asc, cap, dense,
-                       shared, work, stream())
+    gh.cache_attention(out, cuda(q), q.shape[1], c, p.batch(rows, max_len=max_len), heads, slide, asc,
+                       cap, dense, shared, work, stream())
     torch.cuda.synchronize()
     got = out.cpu().numpy().reshape(rows, heads, hd)
     worst = 0.0
@@ -715,6 +715,21 @@ def test_attention_prefix_beside_long_or_many_sequences(gh, hdim, kind):
     p = Paged([(i % 3, 64 + i % 70) for i in range(301)], 2, hdim, 16, KINDS[kind], rng, shared=64)
     p.fill(rng)
     check_attention(gh, p, 4, 0, 0.0, False, 64, 0.0625, rng)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("slide,dense,shared", [(0, False, 0), (90, False, 0), (90, True, 0),
+                                                (0, False, 64), (300, True, 64)])
+def test_attention_lengths_far_below_their_bound(gh, slide, dense, shared):
+    """As a captured step has them: the host knows that no sequence passes 131072."""
+    rng = np.random.default_rng(22)
+    p = Paged([(1, 700), (3, 130), (1, 66), (50, 400)], 1, 256, 64, CACHE_E4M3, rng, shared=shared,
+              width=2048)
+    p.fill(rng)
+    check_attention(gh, p, 4, slide, 0.0, dense, shared, 0.0625, rng, max_len=131072)
+    p = Paged([(1, 700), (3, 130), (1, 66)], 2, 128, 64, CACHE_I8, rng, shared=shared, width=2048)
+    p.fill(rng)
+    check_attention(gh, p, 4, slide, 0.0, dense, shared, 0.0625, rng, max_len=131072)
 
 
 @pytest.mark.gpu
