@@ -415,8 +415,8 @@ __device__ __forceinline__ int wave_max_all(int v) {
 // A workgroup takes up to 16 query vectors of one sequence and kv head, and a chunk
 // of its keys, whose tiles its four waves share out.  Codes go straight from memory
 // to registers, a tile (16 KB of 256 dims) ahead of their use.  Bound by the cache's bytes
-// where there are many: 32 gemma-3-4b tokens of up to 8192 int8 positions (335 MB) take 72
-// us, 4.7 TB/s of the 5.1 that a large copy reaches; two gemma-3-1b ones of 131072 e4m3
+// where there are many: 32 gemma-3-4b tokens of up to 8192 int8 positions (335 MB) take 75
+// us, 4.5 TB/s of the 5.1 that a large copy reaches; two gemma-3-1b ones of 131072 e4m3
 // positions (136 MB) 30 us.  Few keys are a chain of round trips to memory (tables, page ids,
 // the query and codes, each about a microsecond) and code fetched cold: one token of 1001
 // positions takes 9 to 10 us.
