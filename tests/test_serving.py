@@ -552,6 +552,9 @@ ATTN = {
     "step_cap": ([(1, 77), (1, 300)], 4, 2, 128, 16, 0, 5.0, False, 0),
     "step_no_gqa": ([(1, 60), (1, 61)], 3, 3, 128, 16, 0, 0.0, False, 0),
     "step_wide": ([(1, 90), (1, 31)], 32, 1, 128, 16, 0, 0.0, False, 0),
+    "wide_prefix": ([(1, 90), (3, 131), (0, 70), (1, 64)], 32, 1, 128, 16, 0, 0.0, False, 64),
+    "widest": ([(1, 40), (2, 33)], 1024, 1, 128, 16, 0, 0.0, False, 0),
+    "widest_prefix": ([(1, 40), (1, 33)], 1024, 2, 128, 16, 20, 0.0, False, 32),
     "step_24": ([(1, 90), (1, 31)], 24, 2, 256, 16, 0, 0.0, False, 0),
     "few_rows": ([(3, 90), (2, 31), (4, 4)], 4, 1, 256, 16, 0, 0.0, False, 0),
     "prompt": ([(70, 70)], 4, 1, 256, 16, 0, 0.0, False, 0),
