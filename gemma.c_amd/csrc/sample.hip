@@ -897,8 +897,9 @@ __global__ __launch_bounds__(kThreads) void sample_whole_kernel(Sample a) {
     for (int e = 0; e < kWhole; ++e) {
       if (!has_place(x[e])) continue;
       const int bin = gap(bin_of(octaves(x[e], st.c), g.gmax));
-      if (s.row.at[bin] != kNone)
-        list[s.row.at[bin] + atomicAdd(&s.row.fill[bin], 1u)] = place(x[e], tid + e * kThreads);
+      if (s.row.at[bin] == kNone) continue;
+      const uint32_t i = s.row.at[bin] + atomicAdd(&s.row.fill[bin], 1u);
+      if (i < kWholeList) list[i] = place(x[e], tid + e * kThreads);
     }
   }
   __syncthreads();
