@@ -788,7 +788,8 @@ __device__ __forceinline__ void rows_keys(const KvAttn &a, const KvPlan &pl, int
   // read keys 4 g + e at a time, meet different banks
   const int vrow = VD == 4 ? lane >> 2 : lane >> 1 & 15;
   const uint32_t voff = (4 * (vrow & 3) + (vrow >> 2)) * HD + 16 * (lane & (VD - 1));
-  const uint8_t *const k_base = a.c.k + 64 * block, *const v_base = a.c.v + 64 * block + (VD == 4 ? 0 : 32 * part);
+  const uint8_t *const k_base = a.c.k + 64 * block;
+  const uint8_t *const v_base = a.c.v + 64 * block + (VD == 4 ? 0 : 32 * part);
   auto load_k = [&](int r, const Halves &h) {  // r: the buffer, tile modulo 3
 #pragma unroll
     for (int i = 0; i < KU; ++i) {
@@ -1331,7 +1332,8 @@ void launch_rows(const KvAttn &a, const KvPlan &p, hipStream_t stream) {
   const int vecs = a.b.rows * p.group;
   // tiles: one more than the whole ones for each sequence, of which there are so many
   const int tiles = PRE ? ceil_div(vecs, 64 * B)
-                        : vecs / (64 * B) + std::min(a.b.batch, vecs / (p.step ? kStepRows + 1 : p.group));
+                        : vecs / (64 * B) +
+                              std::min(a.b.batch, vecs / (p.step ? kStepRows + 1 : p.group));
   if (tiles > 0)
     kv_rows_kernel<HD, TYPE, CAP, QB, NW, PRE>
         <<<dim3(tiles * (PRE ? p.pre_ns : p.rows_ns), a.c.nkv), 64 * NW, 0, stream>>>(a, p);

@@ -15,17 +15,18 @@
 // 64-bit sum, exact in any order.  Sums over bins and workgroups are fp64 in one order.
 // So equal calls give equal bits.
 //
-// Up to kWholeVocab columns a workgroup does a row by itself, from registers.  Longer rows take four
-// launches: each 8192-column chunk's bins, from its own largest logit down so that one
-// reading does (sample_bins_kernel); their sum and the bins that matter
-// (sample_decide_kernel); these bins' tokens (sample_collect_kernel; chunks that
-// hold none are not read again); and the targets inside them (sample_pick_kernel).
+// Up to kWholeVocab columns a workgroup does a row by itself, from registers.  Longer rows
+// take four launches: each 8192-column chunk's bins, from its own largest logit down so that
+// one reading does (sample_bins_kernel); their sum and the bins that matter
+// (sample_decide_kernel); these bins' tokens (sample_collect_kernel; chunks that hold none
+// are not read again); and the targets inside them (sample_pick_kernel).
 //
 // Of 16000 columns one row by top-k 64 and top-p 0.95 takes 17 us, 64 rows with settings of
 // all kinds 22 (24 and 37 when the bins' tokens are looked for in the row, not in a list).
 // Of 262144 columns, us: the one row 8 + 13 + 5 + 8, four chains of round trips and of code
-// fetched cold; the 64 rows (67 MB) 26 + 13 + 18 + 28: the first by its vector work and the LDS's 64-bit sums (2.4 TB/s), the last by the
-// rows that cut deep into a flat part, a workgroup each.
+// fetched cold; the 64 rows (67 MB) 26 + 13 + 18 + 28: the first by its fp64 work (2.6 TB/s;
+// copies of the bins, for fewer lanes in one, change nothing), the last by the rows that cut
+// deep into a flat part, a workgroup each.
 #include <float.h>
 #include <limits.h>
 
