@@ -11,9 +11,10 @@
 // With c = asc log2 e, s the scaled score in octaves, and a whole number M per
 // query: p = 2^(s - M), w = p vs 2^-24, l = sum p, out = 2^24 sum w code / l.  M follows
 // the largest s + log2 vs, not the largest s: what must fit f16 is w.  It has twelve
-// octaves of slack, so that the sums are rescaled rarely and by powers of two.  A weight
-// is off by at most 2^-25 where the largest is 2 or more: 2^-26 of that one, below the
-// rounding of an fp32 sum that it is part of.
+// octaves of slack, so that the sums are rescaled rarely and by powers of two.  A weight w
+// in its two pieces is off by at most 2^-23 of itself, or by 2^-25 where that is more, and the
+// largest of a query is 2 or more.  Where it may not be (M doesn't follow scales below 2^-60)
+// the query is done over in 64 bits: wide_query().
 //
 // A wave computes S^T = K Q^T (rows: 16 keys, columns: 16 queries) and O^T = V^T
 // P^T (rows: 16 dims) with 16x16x32 products.  Operand layout: lane l holds row (or
@@ -411,6 +412,143 @@ __device__ __forceinline__ int wave_max_all(int v) {
   return __builtin_amdgcn_readfirstlane(v);
 }
 
+// ---- queries whose weights f16 doesn't hold ----------------------------------------
+// Whether the sums of a query may have lost what counts, from its l.  M lies 25 to 38 octaves
+// below the largest s + log2 vs of its keys.  Where that key's log2 vs is its own, its w is 2
+// or more; where it is kLeastVs instead, its p = 2^(s - M) is 2^85 or more, and so is l.  (l is
+// that large, too, where scales are below 2^-45 or so: for nothing, but right.)  The inner
+// loops pay nothing for it; a test of w itself, for each key, made them 2 to 5% slower.
+//
+// Such a query is done over by whoever has its sums last: the merge, for a chunk, or the kernel
+// where there is no merge.
+__device__ __forceinline__ bool lost(float l) { return l >= 0x1p84f; }
+
+// Whether any of a sequence's keys first .. last has a value that isn't a row of zeros; by a
+// whole wave.  Without one (nothing was written there yet) there is nothing to do over.
+__device__ bool any_value(const KvAttn &a, int b, int hk, int first, int last) {
+  const int lane = threadIdx.x & 63;
+  for (int base = first; base <= last; base += 64) {
+    const int key = base + lane;
+    const long slot = key <= last ? kv_slot(a.c, a.b, b, key, hk) : -1;
+    if (__any(slot >= 0 && a.c.vs[max(slot, 0l)] != 0.0f)) return true;
+  }
+  return false;
+}
+
+__device__ __forceinline__ double wave_max_f64(double v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v = fmax(v, __shfl_xor(v, off, 64));
+  return v;
+}
+__device__ __forceinline__ double wave_sum_f64(double v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  return v;
+}
+
+template <int TYPE>
+__device__ __forceinline__ void codes4(uint32_t x, float (&f)[4]) {
+  if constexpr (TYPE == kKvI8) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = (float)(int8_t)(x >> (8 * e));
+  } else {
+    f[0] = __builtin_amdgcn_cvt_f32_fp8(x, 0);
+    f[1] = __builtin_amdgcn_cvt_f32_fp8(x, 1);
+    f[2] = __builtin_amdgcn_cvt_f32_fp8(x, 2);
+    f[3] = __builtin_amdgcn_cvt_f32_fp8(x, 3);
+  }
+}
+
+// A query's softmax sums in fp64: the largest score in octaves, and, by that, the sum of
+// weights and the lane's dims (HD / 64 lane and up) of the sum of weighted values.
+template <int HD>
+struct Wide {
+  double m = -INFINITY, l = 0.0, x[HD / 64] = {};
+};
+
+// One query over keys lo .. hi of sequence b, all in fp64, whose exponents hold any weight times
+// any scale; by a whole wave: a key a lane for the scores, HD / 64 dims a lane for the values.
+template <int HD, int TYPE>
+__device__ Wide<HD> wide_query(const KvAttn &a, int b, int hk, const float *q, int lo, int hi) {
+  constexpr int E = HD / 64;
+  constexpr double log2e = 0x1.71547652b82fep+0;
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));  // nothing of this is worked out ahead, beside an inner loop
+  Wide<HD> r;
+  for (int base = lo; base <= hi; base += 64) {
+    const int key = base + lane;
+    const long slot = key <= hi ? kv_slot(a.c, a.b, b, key, hk) : -1;
+    unsigned long long live = __ballot(slot >= 0);
+    if (live == 0) continue;
+    double s = -INFINITY, vs = 0.0;
+    if (slot >= 0) {
+      const uint32_t *codes = reinterpret_cast<const uint32_t *>(a.c.k + (size_t)slot * HD);
+      double dot = 0.0;
+#pragma unroll 1  // (and below: registers count here, time doesn't)
+      for (int d = 0; d < HD; d += 4) {
+        float f[4];
+        codes4<TYPE>(codes[d / 4], f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dot = fma((double)q[d + e], (double)f[e], dot);
+      }
+      s = dot * (double)a.c.ks[slot] * (double)a.asc;
+      if (a.cap != 0.0f) s = tanh(s / (double)a.cap) * (double)a.cap;
+      s *= log2e;
+      if (!(fabs(s) < INFINITY)) s = NAN;
+      vs = (double)a.c.vs[slot];
+    }
+    const double m = fmax(r.m, wave_max_f64(s)), f = exp2(r.m - m);
+    const double p = slot >= 0 ? exp2(s - m) : 0.0, w = slot >= 0 ? p * vs : 0.0;
+    r.m = m;
+    r.l = r.l * f + wave_sum_f64(p);
+#pragma unroll
+    for (int e = 0; e < E; ++e) r.x[e] *= f;
+#pragma unroll 1
+    for (; live != 0; live &= live - 1) {
+      const int i = __ffsll(live) - 1;
+      const double wi = readlane_f64(w, i);
+      const size_t at = (size_t)__builtin_amdgcn_readlane((int)(slot >> 32), i) << 32 |
+                        (uint32_t)__builtin_amdgcn_readlane((int)slot, i);
+      const uint8_t *codes = a.c.v + at * HD + E * lane;
+      float c[4];
+      if constexpr (E == 4)
+        codes4<TYPE>(*reinterpret_cast<const uint32_t *>(codes), c);
+      else
+        codes4<TYPE>(*reinterpret_cast<const uint16_t *>(codes), c);
+#pragma unroll
+      for (int e = 0; e < E; ++e) r.x[e] = fma(wi, (double)c[e], r.x[e]);
+    }
+  }
+  return r;
+}
+
+// ... to an output row.
+template <int HD>
+__device__ __forceinline__ void wide_out(const Wide<HD> &r, float *out) {
+  constexpr int E = HD / 64;
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    out[E * (threadIdx.x & 63) + e] = r.l != 0.0 ? (float)(r.x[e] / r.l) : 0.0f;
+}
+
+// ... to a chunk's sums, by an M that keeps both of them in fp32: l and the largest of the
+// others at equal distances from 1.
+template <int HD>
+__device__ __forceinline__ float2 wide_part(const Wide<HD> &r, float (&x)[HD / 64]) {
+  double most = 0.0;
+#pragma unroll
+  for (int e = 0; e < HD / 64; ++e) most = fmax(most, fabs(r.x[e]));
+  most = wave_max_f64(most);
+  const bool both = most > 0.0 && r.l > 0.0;
+  const double by = both ? rint(0.5 * (kVsOctaves - log2(r.l) - log2(most))) : 0.0;
+  const float m = fabs(r.m) < INFINITY ? (float)(r.m - by) : kFloor;
+  double up = r.m - (double)m;
+  if (!(fabs(up - by) < 32.0)) up = by;  // (none seen, or fp32 has no octaves left at M)
+#pragma unroll
+  for (int e = 0; e < HD / 64; ++e) x[e] = (float)(r.x[e] * exp2(up - kVsOctaves));
+  return float2{m, (float)(r.l * exp2(up))};
+}
+
 // ---- single tokens ------------------------------------------------------------
 // A workgroup takes up to 16 query vectors of one sequence and kv head, and a chunk
 // of its keys, whose tiles its four waves share out.  Codes go straight from memory
@@ -441,7 +579,8 @@ struct StepLds {
   float sm[kStepWaves][kStepRows], sl[kStepWaves][kStepRows];
 };
 
-template <int HD, int TYPE, bool CAP>
+// WHOLE: one chunk and no prefix, so that what comes out is the output.
+template <int HD, int TYPE, bool CAP, bool WHOLE>
 __device__ __forceinline__ void step_keys(const KvAttn &a, const KvPlan &pl, int chunk, int hk,
                                           int b, StepLds<HD> &lds) {
   constexpr int KS = HD / 32, ND = HD / 16, NJ = HD / 64, VW = HD / 64;
@@ -591,8 +730,20 @@ __device__ __forceinline__ void step_keys(const KvAttn &a, const KvPlan &pl, int
             v4f{o[i][r], o[i + 1][r], o[i + 2][r], o[i + 3][r]} * f;
   }
   __syncthreads();
+  auto out_of = [&](int q) {
+    return a.out + ((size_t)(s.r0 + q / pl.group) * a.n_heads + hk * pl.group + q % pl.group) * HD;
+  };
+  unsigned again = 0;  // a bit for each query of which a wave has lost something
+  if (WHOLE) {
+    static_assert(kStepWaves * kStepRows == 64, "a lane each");
+    const unsigned long long marks = __ballot(lost((&sl[0][0])[lane]));
+    again = (unsigned)(marks | marks >> 32);
+    again = (again | again >> 16) & ((1u << rows) - 1);
+    if (again != 0 && !any_value(a, b, hk, kTile * kr.t0, s.len - 1)) again = 0;
+  }
   for (int e = threadIdx.x; e < rows * (HD / 4); e += 64 * kStepWaves) {
     const int q = e / (HD / 4), d = 4 * (e % (HD / 4));
+    if (WHOLE && (again >> q & 1)) continue;
     float m = kFloor, l = 0.0f;
 #pragma unroll
     for (int w = 0; w < kStepWaves; ++w) m = fmaxf(m, sm[w][q]);
@@ -602,22 +753,28 @@ __device__ __forceinline__ void step_keys(const KvAttn &a, const KvPlan &pl, int
       l += sl[w][q] * __builtin_amdgcn_exp2f(sm[w][q] - m);
       x += *reinterpret_cast<const v4f *>(&part[w][q][d]);
     }
-    if (pl.step_ns == 1 && pl.pre_ns == 0) {
-      float *out = a.out + ((size_t)(s.r0 + q / pl.group) * a.n_heads + hk * pl.group +
-                            q % pl.group) * HD + d;
-      *reinterpret_cast<v4f *>(out) = l != 0.0f ? x / (l * kVsUnit) : v4f{};
+    if (WHOLE) {
+      *reinterpret_cast<v4f *>(out_of(q) + d) = l != 0.0f ? x / (l * kVsUnit) : v4f{};
     } else {
       const size_t at = (((size_t)b * a.c.nkv + hk) * pl.step_ns + chunk) * pl.step_rows + q;
       *reinterpret_cast<v4f *>((float *)(a.work + pl.step_o) + at * HD + d) = x;
       if (d == 0) ((float2 *)(a.work + pl.step_m))[at] = float2{m, l};
     }
   }
+  if (WHOLE && again != 0)
+    for (int q = wave; q < rows; q += kStepWaves) {
+      if (!(again >> q & 1)) continue;
+      const KvSpan sees = kv_span(p0 + q / pl.group, s.len, a.slide, a.dense);
+      const float *from = a.q + (size_t)(s.r0 + q / pl.group) * a.q_stride +
+                          (hk * pl.group + q % pl.group) * HD;
+      wide_out(wide_query<HD, TYPE>(a, b, hk, from, sees.lo, sees.hi), out_of(q));
+    }
 }
 
-template <int HD, int TYPE, bool CAP>
+template <int HD, int TYPE, bool CAP, bool WHOLE>
 __global__ __launch_bounds__(64 * kStepWaves, 2) void kv_step_kernel(KvAttn a, KvPlan pl) {
   __shared__ StepLds<HD> lds;
-  step_keys<HD, TYPE, CAP>(a, pl, blockIdx.x, blockIdx.y, blockIdx.z, lds);
+  step_keys<HD, TYPE, CAP, WHOLE>(a, pl, blockIdx.x, blockIdx.y, blockIdx.z, lds);
 }
 
 // ---- prompt rows and shared prefixes ---------------------------------------------
@@ -1059,9 +1216,24 @@ __device__ __forceinline__ void rows_keys(const KvAttn &a, const KvPlan &pl, int
   for (int q = 0; q < QB; ++q) {
     soft[q].l += __shfl_xor(soft[q].l, 16, 64);
     soft[q].l += __shfl_xor(soft[q].l, 32, 64);
-    if (at + 16 * (QB * wave + q) + n >= rows) continue;
-    const size_t vec = (size_t)qrow[q] * a.n_heads + qhead[q];
+    const bool there = at + 16 * (QB * wave + q) + n < rows;
     const bool whole = !PRE && ns == 1 && pl.pre_ns == 0;
+    unsigned again = 0;  // a bit for each query that has lost something
+    if (!PRE && whole) {
+      again = (unsigned)__ballot(there && lost(soft[q].l)) & 0xffff;
+      if (again != 0 && !any_value(a, b, hk, kTile * t0, min(kTile * t1, len) - 1)) again = 0;
+    }
+    for (unsigned rest = again; rest != 0; rest &= rest - 1) {
+      const int i = __ffs(rest) - 1;
+      const size_t row = __builtin_amdgcn_readlane(qrow[q], i);
+      const int head = __builtin_amdgcn_readlane(qhead[q], i);
+      wide_out(wide_query<HD, TYPE>(a, b, hk, a.q + row * a.q_stride + head * HD,
+                                    __builtin_amdgcn_readlane(see[q].lo, i),
+                                    __builtin_amdgcn_readlane(see[q].hi, i)),
+               a.out + (row * a.n_heads + head) * HD);
+    }
+    if (!there || (again >> n & 1)) continue;
+    const size_t vec = (size_t)qrow[q] * a.n_heads + qhead[q];
     const size_t pt = (size_t)chunk * a.b.rows * a.n_heads + vec;
     float *dst = whole ? a.out + vec * HD
                        : (float *)(a.work + (PRE ? pl.pre_o : pl.rows_o)) + pt * HD;
@@ -1101,7 +1273,7 @@ __global__ __launch_bounds__(64 * kStepWaves) void kv_both_kernel(KvAttn a, KvPl
     rows_keys<HD, TYPE, CAP, 1, NW, true>(a, pl, id % blocks, blocks, id / blocks, lds.rows);
   } else {
     const int i = id - blocks * a.c.nkv;  // one chunk
-    step_keys<HD, TYPE, CAP>(a, pl, 0, i % a.c.nkv, i / a.c.nkv, lds.step);
+    step_keys<HD, TYPE, CAP, false>(a, pl, 0, i % a.c.nkv, i / a.c.nkv, lds.step);
   }
 }
 
@@ -1112,7 +1284,7 @@ __global__ __launch_bounds__(64 * kStepWaves) void kv_both_kernel(KvAttn a, KvPl
 
 constexpr int kMergeWaves = 4;  // of a workgroup, at least
 
-template <int HD, int SHARE, bool STEP>
+template <int HD, int TYPE, int SHARE, bool STEP>
 __global__ __launch_bounds__(64 * (SHARE > kMergeWaves ? SHARE : kMergeWaves)) void kv_merge_kernel(
     KvAttn a, KvPlan pl) {
   constexpr int E = HD / 64, W = SHARE > kMergeWaves ? SHARE : kMergeWaves;
@@ -1128,14 +1300,16 @@ __global__ __launch_bounds__(64 * (SHARE > kMergeWaves ? SHARE : kMergeWaves)) v
   if (i < 0 || i >= s.n || step != STEP) return;  // (a whole workgroup's, where its waves share)
   const int hk = head / pl.group, j = i * pl.group + head % pl.group, p0 = s.len - s.n;
   const size_t vec = (size_t)(s.r0 + i) * a.n_heads + head;
-  // this row's own chunks: number, first partial and the step to the next
-  int n;
+  // this row's own chunks: number, first partial and the step to the next; their tiles
+  int n, t0, tpc;
   size_t first, stride;
   const float *po;
   const float2 *pm;
   if (STEP) {
     const KvRange kr = key_range(p0, s.len - 1, s.len, a.slide, a.dense, a.shared);
-    n = max(1, ceil_div(kr.t1 - kr.t0, chunk_tiles(kr.t1 - kr.t0, pl.step_ns)));
+    tpc = chunk_tiles(kr.t1 - kr.t0, pl.step_ns);
+    t0 = kr.t0;
+    n = max(1, ceil_div(kr.t1 - kr.t0, tpc));
     first = ((size_t)b * a.c.nkv + hk) * pl.step_ns * pl.step_rows + j;
     stride = pl.step_rows;
     po = (const float *)(a.work + pl.step_o);
@@ -1144,7 +1318,9 @@ __global__ __launch_bounds__(64 * (SHARE > kMergeWaves ? SHARE : kMergeWaves)) v
     const int tr = 64 * pl.qb, at = j / tr * tr;
     const int i0 = at / pl.group, i1 = min(s.n - 1, (at + tr - 1) / pl.group);
     const KvRange kr = key_range(p0 + i0, p0 + i1, s.len, a.slide, a.dense, a.shared);
-    n = max(1, ceil_div(kr.t1 - kr.t0, chunk_tiles(kr.t1 - kr.t0, pl.rows_ns)));
+    tpc = chunk_tiles(kr.t1 - kr.t0, pl.rows_ns);
+    t0 = kr.t0;
+    n = max(1, ceil_div(kr.t1 - kr.t0, tpc));
     first = vec;
     stride = (size_t)a.b.rows * a.n_heads;
     po = (const float *)(a.work + pl.rows_o);
@@ -1166,6 +1342,15 @@ __global__ __launch_bounds__(64 * (SHARE > kMergeWaves ? SHARE : kMergeWaves)) v
     return v;
   };
   float m = kFloor, l = 0.0f, x[E] = {};
+  auto add = [&](float2 v, const float (&y)[E]) {
+    const float mn = fmaxf(m, v.x);
+    const float f = __builtin_amdgcn_exp2f(m - mn), h = __builtin_amdgcn_exp2f(v.x - mn);
+    m = mn;
+    l = l * f + v.y * h;
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = x[e] * f + y[e] * h;
+  };
+  bool some = false;  // chunks that have lost something are left for later
   constexpr int A = SHARE == 16 ? 8 : 4;  // chunks loaded at a time
   for (int c = part; c < total; c += A * SHARE) {
     float2 v[A];
@@ -1181,12 +1366,30 @@ __global__ __launch_bounds__(64 * (SHARE > kMergeWaves ? SHARE : kMergeWaves)) v
 #pragma unroll
     for (int u = 0; u < A; ++u) {
       if (c + u * SHARE >= total) break;
-      const float mn = fmaxf(m, v[u].x);
-      const float f = __builtin_amdgcn_exp2f(m - mn), h = __builtin_amdgcn_exp2f(v[u].x - mn);
-      m = mn;
-      l = l * f + v[u].y * h;
+      if (lost(v[u].y))
+        some = true;
+      else
+        add(v[u], y[u]);
+    }
+  }
+  if (__any(some)) {
+    const float *from = a.q + (size_t)(s.r0 + i) * a.q_stride + head * HD;
+    const KvSpan sees = kv_span(p0 + i, s.len, a.slide, a.dense);
+    for (int c = part; c < total; c += SHARE) {
+      const float *o;
+      float2 v = where(c, &o);
+      if (!lost(v.y)) continue;
+      const bool own = c < n;
+      const int first = kTile * (own ? t0 + c * tpc : (c - n) * pl.pre_tpc);
+      const int lo = max(own ? max(sees.lo, a.shared) : sees.lo, first);
+      const int hi = min(own ? sees.hi : min(sees.hi, a.shared - 1),
+                         first + kTile * (own ? tpc : pl.pre_tpc) - 1);
+      float y[E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) x[e] = x[e] * f + y[u][e] * h;
+      for (int e = 0; e < E; ++e) y[e] = o[E * lane + e];
+      if (any_value(a, own ? b : 0, hk, lo, hi))
+        v = wide_part(wide_query<HD, TYPE>(a, own ? b : 0, hk, from, lo, hi), y);
+      add(v, y);
     }
   }
   if constexpr (SHARE == 1) {
@@ -1313,15 +1516,15 @@ KvPlan plan(const KvAttn &a, const DeviceInfo &dev) {
 
 // Waves share a vector where it has many chunks: 2452 vectors of 6 chunks take 6.5 us with a
 // wave each and 8.4 with four, 256 of 64 chunks 6.1 with 16.
-template <int HD, bool STEP>
+template <int HD, int TYPE, bool STEP>
 void launch_merge(const KvAttn &a, const KvPlan &p, int chunks, int rows, hipStream_t stream) {
   const int vecs = rows * a.n_heads, batch = STEP ? a.b.batch : 1;
   if (chunks > 16)
-    kv_merge_kernel<HD, 16, STEP><<<dim3(vecs, batch), 1024, 0, stream>>>(a, p);
+    kv_merge_kernel<HD, TYPE, 16, STEP><<<dim3(vecs, batch), 1024, 0, stream>>>(a, p);
   else if (chunks > 8)
-    kv_merge_kernel<HD, 4, STEP><<<dim3(vecs, batch), 64 * kMergeWaves, 0, stream>>>(a, p);
+    kv_merge_kernel<HD, TYPE, 4, STEP><<<dim3(vecs, batch), 64 * kMergeWaves, 0, stream>>>(a, p);
   else if (chunks > 1)
-    kv_merge_kernel<HD, 1, STEP>
+    kv_merge_kernel<HD, TYPE, 1, STEP>
         <<<dim3(ceil_div(vecs, kMergeWaves), batch), 64 * kMergeWaves, 0, stream>>>(a, p);
 }
 
@@ -1345,8 +1548,11 @@ void launch_typed(const KvAttn &a, const KvPlan &p, hipStream_t stream) {
   if (p.pre_blocks > 0)
     kv_both_kernel<HD, TYPE, CAP>
         <<<(p.pre_blocks * p.pre_ns + batch) * nkv, 64 * kStepWaves, 0, stream>>>(a, p);
+  else if (p.step && p.step_ns == 1 && p.pre_ns == 0)
+    kv_step_kernel<HD, TYPE, CAP, true>
+        <<<dim3(1, nkv, batch), 64 * kStepWaves, 0, stream>>>(a, p);
   else if (p.step)
-    kv_step_kernel<HD, TYPE, CAP>
+    kv_step_kernel<HD, TYPE, CAP, false>
         <<<dim3(p.step_ns, nkv, batch), 64 * kStepWaves, 0, stream>>>(a, p);
   if (p.rows_ns > 0) {
     if (p.qb == 2)
@@ -1361,9 +1567,9 @@ void launch_typed(const KvAttn &a, const KvPlan &p, hipStream_t stream) {
       launch_rows<HD, TYPE, CAP, 1, true>(a, p, stream);
   }
   if (p.step)
-    launch_merge<HD, true>(a, p, p.step_ns + p.pre_ns, std::min(a.b.max_rows, kStepRows / p.group),
-                           stream);
-  if (p.rows_ns > 0) launch_merge<HD, false>(a, p, p.rows_ns + p.pre_ns, a.b.rows, stream);
+    launch_merge<HD, TYPE, true>(a, p, p.step_ns + p.pre_ns,
+                                 std::min(a.b.max_rows, kStepRows / p.group), stream);
+  if (p.rows_ns > 0) launch_merge<HD, TYPE, false>(a, p, p.rows_ns + p.pre_ns, a.b.rows, stream);
 }
 
 template <int HD>
