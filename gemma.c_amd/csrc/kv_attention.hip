@@ -13,8 +13,8 @@
 // the largest s + log2 vs, not the largest s: what must fit f16 is w.  It has twelve
 // octaves of slack, so that the sums are rescaled rarely and by powers of two.  A weight w
 // in its two pieces is off by at most 2^-23 of itself, or by 2^-25 where that is more, and the
-// largest of a query is 2 or more.  Where it may not be (M doesn't follow scales below 2^-60)
-// the query is done over in 64 bits: wide_query().
+// largest of a query is 2 or more.  Where it may not be (M doesn't follow scales below 2^-60,
+// nor scores past 2^23 octaves) the query is done over in 64 bits: wide_query().
 //
 // A wave computes S^T = K Q^T (rows: 16 keys, columns: 16 queries) and O^T = V^T
 // P^T (rows: 16 dims) with 16x16x32 products.  Operand layout: lane l holds row (or
@@ -44,7 +44,8 @@ constexpr int kLongRun = 16;          // tiles by 64 query vectors of a compute 
 constexpr int kBothTiles = 64;         // tiles of own keys, at most, of single tokens that share
                                       // a launch with their prefix
 constexpr int kStepRows = 16;         // query vectors (rows x heads of a kv head) of a step tile
-constexpr float kFloor = -0x1p55f;    // M of a query that has seen no key
+constexpr float kFloor = -0x1p126f;   // M of a query that has seen no key
+constexpr float kFar = 0x1p23f;       // |M| from which on fp32 can't hold M and M + kSlack apart
 constexpr float kVsUnit = 0x1p-24f;   // V's scales enter the weights in units of 2^24, so that
 constexpr float kVsOctaves = 24.0f;   // l keeps its terms beside the largest scales
 constexpr float kSlack = 14.0f + kVsOctaves;  // weights stay below 2^15 ...
@@ -276,7 +277,10 @@ __device__ __forceinline__ float top_of(v4f (&d)[2], const float (&lv)[8], bool 
   return top;
 }
 
-// Moves a query's M where the tile's largest weight needs it.
+__device__ __forceinline__ bool far(float m) { return fabsf(m) >= kFar && m > kFloor; }
+
+// Moves a query's M where the tile's largest weight needs it.  An M that was too far out leaves
+// an infinite l: the sums may be anything.
 template <class F>
 __device__ __forceinline__ void settle(float top, Soft &s, F &&rescale) {
   if (!__any(top > s.m + kSlack)) return;
@@ -284,8 +288,8 @@ __device__ __forceinline__ void settle(float top, Soft &s, F &&rescale) {
   top = fmaxf(top, __shfl_xor(top, 32, 64));
   const float m = top > s.m + kSlack ? ceilf(top) - kSet : s.m;
   const float f = __builtin_amdgcn_exp2f(s.m - m);
+  s.l = (m != s.m && far(s.m)) || s.l == INFINITY ? INFINITY : s.l * f;
   s.m = m;
-  s.l *= f;
   rescale(f);
 }
 
@@ -413,7 +417,8 @@ __device__ __forceinline__ int wave_max_all(int v) {
 }
 
 // ---- queries whose weights f16 doesn't hold ----------------------------------------
-// Whether the sums of a query may have lost what counts, from its l.  M lies 25 to 38 octaves
+// Whether the sums of a query may have lost what counts, from its l (infinite where M is or was
+// far).  M lies 25 to 38 octaves
 // below the largest s + log2 vs of its keys.  Where that key's log2 vs is its own, its w is 2
 // or more; where it is kLeastVs instead, its p = 2^(s - M) is 2^85 or more, and so is l.  (l is
 // that large, too, where scales are below 2^-45 or so: for nothing, but right.)  The inner
@@ -532,18 +537,19 @@ __device__ __forceinline__ void wide_out(const Wide<HD> &r, float *out) {
 }
 
 // ... to a chunk's sums, by an M that keeps both of them in fp32: l and the largest of the
-// others at equal distances from 1.
+// others at equal distances from 1.  Past 2^29 octaves fp32 has no M for that and past 2^30 none
+// for the score either: chunks are then weighed by what their largest scores round to.
 template <int HD>
 __device__ __forceinline__ float2 wide_part(const Wide<HD> &r, float (&x)[HD / 64]) {
   double most = 0.0;
 #pragma unroll
   for (int e = 0; e < HD / 64; ++e) most = fmax(most, fabs(r.x[e]));
   most = wave_max_f64(most);
-  const bool both = most > 0.0 && r.l > 0.0;
+  const bool both = most > 0.0 && r.l > 0.0 && fabs(r.m) < 0x1p29;
   const double by = both ? rint(0.5 * (kVsOctaves - log2(r.l) - log2(most))) : 0.0;
   const float m = fabs(r.m) < INFINITY ? (float)(r.m - by) : kFloor;
   double up = r.m - (double)m;
-  if (!(fabs(up - by) < 32.0)) up = by;  // (none seen, or fp32 has no octaves left at M)
+  if (!(fabs(up - by) <= 32.0)) up = by;
 #pragma unroll
   for (int e = 0; e < HD / 64; ++e) x[e] = (float)(r.x[e] * exp2(up - kVsOctaves));
   return float2{m, (float)(r.l * exp2(up))};
@@ -713,7 +719,7 @@ __device__ __forceinline__ void step_keys(const KvAttn &a, const KvPlan &pl, int
   soft.l += __shfl_xor(soft.l, 32, 64);
   if (g == 0) {
     sm[wave][n] = soft.m;
-    sl[wave][n] = soft.l;
+    sl[wave][n] = far(soft.m) ? INFINITY : soft.l;
   }
   __syncthreads();
   if (n < rows) {
@@ -750,7 +756,8 @@ __device__ __forceinline__ void step_keys(const KvAttn &a, const KvPlan &pl, int
     v4f x = {};
 #pragma unroll
     for (int w = 0; w < kStepWaves; ++w) {
-      l += sl[w][q] * __builtin_amdgcn_exp2f(sm[w][q] - m);
+      const float own = sl[w][q];  // (an infinite one, which is a mark, stays so)
+      l += own == INFINITY ? own : own * __builtin_amdgcn_exp2f(sm[w][q] - m);
       x += *reinterpret_cast<const v4f *>(&part[w][q][d]);
     }
     if (WHOLE) {
@@ -1216,6 +1223,7 @@ __device__ __forceinline__ void rows_keys(const KvAttn &a, const KvPlan &pl, int
   for (int q = 0; q < QB; ++q) {
     soft[q].l += __shfl_xor(soft[q].l, 16, 64);
     soft[q].l += __shfl_xor(soft[q].l, 32, 64);
+    if (far(soft[q].m)) soft[q].l = INFINITY;
     const bool there = at + 16 * (QB * wave + q) + n < rows;
     const bool whole = !PRE && ns == 1 && pl.pre_ns == 0;
     unsigned again = 0;  // a bit for each query that has lost something
@@ -1387,7 +1395,7 @@ __global__ __launch_bounds__(64 * (SHARE > kMergeWaves ? SHARE : kMergeWaves)) v
       float y[E];
 #pragma unroll
       for (int e = 0; e < E; ++e) y[e] = o[E * lane + e];
-      if (any_value(a, own ? b : 0, hk, lo, hi))
+      if (v.y == INFINITY || any_value(a, own ? b : 0, hk, lo, hi))
         v = wide_part(wide_query<HD, TYPE>(a, own ? b : 0, hk, from, lo, hi), y);
       add(v, y);
     }

@@ -136,3 +136,76 @@ def test_small_values_beside_zeros_and_unseen_large_ones(gh, rows, cap):
     check(gh, p, q, 4, 0.1, 9, cap)
     p.scales["v"][:], p.codes["v"][:] = 0.0, 0
     check(gh, p, q, 4, 0.1, 9, cap)
+
+
+def scored_cache(name, kind, octaves, sign):
+    """Keys that differ in their first dim alone: scores of exactly sign 2^octaves by asc 1 (q is
+    a power of two in that dim, the rest meets codes of 0)."""
+    p, q, rng = cache_of(name, kind, 6)
+    a = octaves // 2
+    q[:, ::p.hd] = F32(2.0) ** a
+    code = 64 if kind == "i8" else 0x38
+    live = np.isfinite(p.scales["k"])
+    p.codes["k"][live] = 0
+    p.codes["k"][..., 0][live] = code
+    unit = F32(sign * 2.0 ** (octaves - a) / (64 if kind == "i8" else 1))
+    p.scales["k"] = np.where(live, unit, np.nan).astype(F32)
+    return p, q
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", sorted(KINDS))
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("octaves", [10, 23, 27, 30, 60, 100])
+@pytest.mark.parametrize("name", ["step", "step_128", "step_long", "prompt", "prompt_128", "prefix",
+                                  "prefix_mixed"])
+def test_equal_scores_of_any_size(gh, name, octaves, sign, kind):
+    """Every key scores the same, however much that is: the values' mean."""
+    _, heads, _, hd, slide, shared, step = SHAPES[name]
+    p, q = scored_cache(name, kind, octaves, sign)
+    check(gh, p, q, heads, 1.0, slide, 0.0, shared, step, exact=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", sorted(KINDS))
+@pytest.mark.parametrize("octaves", [22, 24, 25, 26, 27, 28, 29, 31, 40])
+@pytest.mark.parametrize("name", ["step", "prompt", "prefix"])
+def test_scores_that_rise_by_their_last_place(gh, name, octaves, kind):
+    """From tile to tile by 2^-23 of themselves, which is octaves where they are large."""
+    _, heads, _, hd, slide, shared, step = SHAPES[name]
+    p, q = scored_cache(name, kind, octaves, 1.0)
+    for b, ln in enumerate(p.len):
+        for pos in range(ln):
+            page = p.table[b, pos // 16]
+            unit = np.abs(p.scales["k"][page, :, pos % 16])
+            up = F32(1.0 + (pos // 32) * 2.0 ** -23)
+            p.scales["k"][page, :, pos % 16] = 2.0 ** np.floor(np.log2(unit)) * up
+    check(gh, p, q, heads, 1.0, slide, 0.0, shared, step)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", sorted(KINDS))
+@pytest.mark.parametrize("octaves", [25, 27, 30, 60])
+@pytest.mark.parametrize("name", ["step", "step_128", "step_long", "prompt", "prompt_128", "prefix",
+                                  "prefix_mixed"])
+def test_scores_that_come_from_far(gh, name, octaves, kind):
+    """A sequence's first keys score -2^octaves and count for nothing beside the rest's 0: what
+    their sums may have become is gone without a trace, but for a NaN among them."""
+    import torch
+
+    seqs, heads, _, hd, slide, shared, step = SHAPES[name]
+    p, q = scored_cache(name, kind, octaves, -1.0)
+    for b, ln in enumerate(p.len):
+        for pos in range(ln // 2 if not shared else shared // 2, ln):
+            p.scales["k"][p.table[b, pos // 16], :, pos % 16] = 0.0
+    check(gh, p, q, heads, 1.0, slide, 0.0, shared, step, exact=True)
+    if slide:
+        return
+    p.scales["k"][p.table[0, 0], :, 1] = np.nan  # seen by every row of the first sequence
+    c = p.device()
+    out = torch.zeros((p.rows, heads * hd), device="cuda")
+    gh.cache_attention(out, cuda(q), 0, c, p.batch(), heads, 0, 1.0, 0.0, False, shared, None,
+                       stream())
+    torch.cuda.synchronize()
+    sees = out[:p.n[0]].cpu().numpy()[[p.len[0] - p.n[0] + i >= 1 for i in range(p.n[0])]]
+    assert np.isnan(sees).all()
