@@ -74,6 +74,19 @@ GH_HD int kv_find(const int *row0, int batch, int r) {
   return lo;
 }
 
+// The grid of a launch that needs `blocks` workgroups for each of `batch` sequences: x and z for
+// the former, as a grid takes 2^32 - 1 threads a dimension at most; kv_block() is a
+// workgroup's number.
+constexpr long kKvMostX = 1l << 22;  // (of 256 threads)
+struct KvGrid {
+  unsigned x, y, z;
+};
+GH_HD KvGrid kv_grid_of(long blocks, int batch) {
+  const long z = (blocks + kKvMostX - 1) / kKvMostX;
+  return KvGrid{(unsigned)(z > 1 ? kKvMostX : blocks), (unsigned)batch, (unsigned)(z > 1 ? z : 1)};
+}
+GH_HD long kv_block(unsigned x, unsigned z) { return (long)z * kKvMostX + x; }
+
 #ifdef __HIPCC__
 // The sequence that row r is in if it is in one, else any; by a whole wave, for one row.
 __device__ __forceinline__ int kv_find_wave(const KvBatch &b, int r) {

@@ -35,7 +35,7 @@ template <int HD, bool FLAT>
 __device__ __forceinline__ bool kv_unit(const KvCache &c, const KvBatch &b, KvUnit *u) {
   constexpr int G = HD / 4;  // lanes of a unit
   const int per = 2 * c.nkv;
-  const long unit = (long)blockIdx.x * (kThreads / G) + threadIdx.x / G;
+  const long unit = kv_block(blockIdx.x, blockIdx.z) * (kThreads / G) + threadIdx.x / G;
   int i = (int)(unit / per);
   const int j = (int)(unit % per);
   static_assert(64 / G <= 2, "a wave's units are of one row, of which there are 2 nkv");
@@ -124,7 +124,8 @@ bool kv_flat(const KvBatch &b) { return (long)b.batch * b.max_rows > 2l * b.rows
 dim3 kv_grid(const KvCache &c, const KvBatch &b) {
   const long units = (kv_flat(b) ? (long)b.rows : b.max_rows) * 2 * c.nkv;
   const long per = kThreads / (c.hdim / 4);
-  return dim3((unsigned)((units + per - 1) / per), kv_flat(b) ? 1 : b.batch);
+  const KvGrid g = kv_grid_of((units + per - 1) / per, kv_flat(b) ? 1 : b.batch);
+  return dim3(g.x, g.y, g.z);
 }
 
 // Calls go(hdim, type, flat) with the constants that fit.
