@@ -19,6 +19,7 @@
 #include <cstring>
 #include <map>
 #include <mutex>
+#include <optional>
 #include <string>
 #include <vector>
 
@@ -1101,9 +1102,10 @@ int attn_args(const char *name, const gemma_hip_cache *cache, const gemma_hip_ba
   return 0;
 }
 
-// The workspace of a call: the caller's, or the one kept for the stream.
+// The workspace of a call: the caller's, or the one kept for the stream, which alone is held:
+// a call that needs none, or has its own, waits for no other thread's.
 int call_workspace(const char *name, size_t need, void *work, size_t work_bytes, hipStream_t s,
-                   AttnHold *hold, char **out) {
+                   std::optional<AttnHold> *hold, char **out) {
   *out = (char *)work;
   if (need == 0) return 0;
   if (work != nullptr) {
@@ -1114,7 +1116,8 @@ int call_workspace(const char *name, size_t need, void *work, size_t work_bytes,
   }
   if (capturing(s))
     return fail("%s: a call that is captured needs a workspace of its own (%zu bytes)", name, need);
-  GH_CHECK(name, hold->get(need, out));
+  hold->emplace(s);
+  GH_CHECK(name, (*hold)->get(need, out));
   return 0;
 }
 
@@ -1183,14 +1186,14 @@ int gemma_hip_cache_attention(float *out, const float *q, int q_stride,
   a.asc = asc;
   a.cap = sc_att;
   hipStream_t s = pick_stream(stream);
-  AttnHold hold(s);
+  std::optional<AttnHold> hold;
   if (call_workspace(name, gh::kv_attention_work(a, g.info), work, work_bytes, s, &hold, &a.work))
     return 1;
   {
     PerfScope perf(kOpSoftmax, s);
     GH_CHECK("gemma_hip_cache_attention: launch", gh::launch_kv_attention(a, g.info, s));
   }
-  GH_CHECK("gemma_hip_cache_attention", hold.done());
+  if (hold) GH_CHECK("gemma_hip_cache_attention", hold->done());
   return 0;
 }
 
@@ -1234,14 +1237,14 @@ int gemma_hip_sample(int *tokens, float *probs, const float *logits, int stride,
     a.min_p = settings->min_p;
   }
   hipStream_t s = pick_stream(stream);
-  AttnHold hold(s);
+  std::optional<AttnHold> hold;
   if (call_workspace(name, gh::sample_work(rows, vocab), work, work_bytes, s, &hold, &a.work))
     return 1;
   {
     PerfScope perf(kOpSample, s);
     GH_CHECK("gemma_hip_sample: launch", gh::launch_sample(a, s));
   }
-  GH_CHECK("gemma_hip_sample", hold.done());
+  if (hold) GH_CHECK("gemma_hip_sample", hold->done());
   return 0;
 }
 

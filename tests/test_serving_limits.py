@@ -5,13 +5,14 @@ from __future__ import annotations
 
 import ctypes
 import subprocess
+import threading
 
 import numpy as np
 import pytest
 
 import gemma_hip
-from gemma_hip import CACHE_I8
-from test_serving import CSRC, F32, cuda, quantise, stream, values
+from gemma_hip import CACHE_E4M3, CACHE_I8
+from test_serving import CSRC, F32, Paged, cuda, quantise, stream, values
 
 
 def test_grids_of_the_cache_are_launchable(tmp_path):
@@ -70,3 +71,75 @@ def test_as_many_rows_as_there_may_be(gh, flat):
         assert not t[:4].any() and not t[rows // 2:rows // 2 + 4].any() and not t[-ln - 4:-ln].any()
     del k, v
     torch.cuda.empty_cache()
+
+
+def attention_call(gh, seed, lens, heads=4, kv=1, hd=256):
+    """A call of single tokens, and how many bytes its workspace takes."""
+    import torch
+
+    rng = np.random.default_rng(seed)
+    p = Paged([(1, n) for n in lens], kv, hd, 64, CACHE_E4M3, rng)
+    p.fill(rng)
+    c, b = p.device(), p.batch()
+    q = torch.randn((p.rows, heads * hd), device="cuda")
+    out = torch.zeros_like(q)
+
+    def call(work, s):
+        gh.cache_attention(out, q, 0, c, b, heads, 0, 0.0625, 0.0, False, 0, work, s)
+
+    call.out, call.keep = out, p
+    return call, gh.cache_attention_work(c, b, heads, 0, 0)
+
+
+@pytest.mark.gpu
+def test_calls_with_workspaces_do_not_wait_for_those_without(gh):
+    """A thread whose stream's workspace grows waits for that stream; one that brings a
+    workspace of its own goes on meanwhile, and so does one that samples short rows."""
+    import torch
+
+    small, need0 = attention_call(gh, 1, [3000])
+    large, need1 = attention_call(gh, 2, [4000] * 40)
+    mine, need2 = attention_call(gh, 3, [3000])
+    assert 0 < need0 < need1
+    work = torch.empty(need2, dtype=torch.uint8, device="cuda")
+    busy, free = torch.cuda.Stream(), torch.cuda.Stream()
+    logits, u = torch.randn((1, 1000), device="cuda"), torch.rand(1, device="cuda")
+    tokens = torch.empty(1, dtype=torch.int32, device="cuda")
+    m = torch.randn((8192, 8192), device="cuda")
+    to = torch.empty_like(m)
+    torch.mm(m, m, out=to)
+    small(None, busy.cuda_stream)
+    mine(work, free.cuda_stream)
+    torch.cuda.synchronize()
+    want = mine.out.clone()
+    mine.out.zero_()
+    torch.cuda.synchronize()
+    begun, errors = threading.Event(), []
+
+    def grow():
+        try:
+            begun.set()
+            large(None, busy.cuda_stream)
+        except Exception as e:  # (shown by the main thread)
+            errors.append(e)
+
+    with torch.cuda.stream(busy):
+        for _ in range(200):
+            torch.mm(m, m, out=to)
+        done = torch.cuda.Event()
+        done.record()
+    t = threading.Thread(target=grow)
+    t.start()
+    begun.wait()
+    t.join(0.2)  # time to take the lock and to wait
+    waiting = t.is_alive()
+    mine(work, free.cuda_stream)
+    gh.sample(tokens, None, logits, 0, 1, 1000, None, u, None, free.cuda_stream)
+    early = not done.query()
+    free.synchronize()
+    t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    assert waiting, "the other thread's call was not waiting: this shows nothing"
+    assert early, "a call with a workspace of its own waited for another thread's"
+    assert torch.equal(mine.out, want)
