@@ -143,3 +143,77 @@ def test_calls_with_workspaces_do_not_wait_for_those_without(gh):
     assert waiting, "the other thread's call was not waiting: this shows nothing"
     assert early, "a call with a workspace of its own waited for another thread's"
     assert torch.equal(mine.out, want)
+
+
+def clamped(lens, row0, rows, max_rows, max_len):
+    """(first row, rows, length) of every sequence, cut to the call's bounds."""
+    out = []
+    for i, ln in enumerate(lens):
+        r0 = min(max(row0[i], 0), rows)
+        out.append((r0, min(min(max(row0[i + 1], r0), rows) - r0, max_rows),
+                    min(max(ln, 0), max_len)))
+    return out
+
+
+LIES = {  # lengths, first rows: of five rows, three a sequence at most, in 64 positions
+    "few": ([2 ** 31 - 1, -5, 64], [0, 900, 2, 5]),
+    "falling": ([70, 64, -2 ** 31], [4, 3, 1, -9]),
+    "many": ([9, 64, 0, 2 ** 31 - 1, 33, -1, 64], [-7, 2, 2, 1, 2 ** 31 - 1, 3, 0, 5]),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", sorted(LIES))
+@pytest.mark.parametrize("shared", [0, 16])
+def test_tables_that_lie_lead_nowhere_else(gh, case, shared):
+    """Whatever lengths, first rows and page ids say, cache_write touches no place but those
+    that they name within the call's bounds, cache_read and attention no row but the call's
+    sequences', and nothing beside any of the buffers."""
+    import torch
+
+    lens, row0 = LIES[case]
+    rows, max_rows, max_len, hd, kv, page, npages, heads = 5, 3, 64, 128, 2, 16, 9, 4
+    rng = np.random.default_rng(7)
+    batch = len(lens)
+    table = rng.permutation(np.arange(batch * 4) % (npages + 3)).reshape(batch, 4).astype(np.int32)
+    table[0, 0], table[-1, -1], table[1, 3] = npages, -1, -2 ** 31
+    pad = 4096  # before and behind every buffer
+
+    def fenced(n, dtype, value):
+        whole = torch.full((n + 2 * pad,), value, dtype=dtype, device="cuda")
+        return whole, whole[pad:pad + n]
+
+    ncode, nscale = npages * kv * page * hd, npages * kv * page
+    codes = [fenced(ncode, torch.int8, 3) for _ in "kv"]
+    scales = [fenced(nscale, torch.float32, 0.5) for _ in "kv"]
+    reads = [fenced(rows * kv * hd, torch.float32, 7.0) for _ in "kv"]
+    outs = fenced(rows * heads * hd, torch.float32, 7.0)
+    every = codes + scales + reads + [outs]
+    c = gemma_hip.cache(codes[0][1], codes[1][1], scales[0][1], scales[1][1], CACHE_I8, npages,
+                        page, kv, hd)
+    b = gemma_hip.batch(cuda(table), cuda(np.array(lens, np.int32)), cuda(np.array(row0, np.int32)),
+                        batch, 4, rows, max_rows, max_len)
+    x = torch.randn((rows, kv * hd), device="cuda")
+    q = torch.randn((rows, heads * hd), device="cuda")
+    gh.cache_write(c, b, x, 0, x, 0, stream())
+    gh.cache_read(c, b, reads[0][1], 0, reads[1][1], 0, stream())
+    gh.cache_attention(outs[1], q, 0, c, b, heads, 0, 0.1, 0.0, False, shared, None, stream())
+    torch.cuda.synchronize()
+
+    for whole, inner in every:
+        edge = torch.cat([whole[:pad], whole[pad + inner.numel():]])
+        assert (edge == edge[0]).all() and float(edge[0]) in (3.0, 0.5, 7.0)
+    named, ours = np.zeros((npages, page), bool), np.zeros(rows, bool)
+    for i, (r0, n, ln) in enumerate(clamped(lens, row0, rows, max_rows, max_len)):
+        ours[r0:r0 + n] = True
+        for pos in range(max(0, ln - n), ln):
+            if 0 <= table[i, pos // page] < npages:
+                named[table[i, pos // page], pos % page] = True
+    for (_, code), (_, scale) in zip(codes, scales):
+        same = (code.view(npages, kv, page, hd) == 3).all(3).all(1).cpu().numpy()
+        assert same[~named].all() and (not named.any() or not same[named].all())
+        same = (scale.view(npages, kv, page) == 0.5).all(1).cpu().numpy()
+        assert same[~named].all()
+    for _, inner in reads + [outs]:
+        same = (inner.view(rows, -1) == 7.0).all(1).cpu().numpy()
+        assert same[~ours].all()
