@@ -211,7 +211,7 @@ def test_tables_that_lie_lead_nowhere_else(gh, case, shared):
                 named[table[i, pos // page], pos % page] = True
     for (_, code), (_, scale) in zip(codes, scales):
         same = (code.view(npages, kv, page, hd) == 3).all(3).all(1).cpu().numpy()
-        assert same[~named].all() and (not named.any() or not same[named].all())
+        assert same[~named].all() and (case != "few" or not same[named].any())
         same = (scale.view(npages, kv, page) == 0.5).all(1).cpu().numpy()
         assert same[~named].all()
     for _, inner in reads + [outs]:
