@@ -417,27 +417,33 @@ __device__ __forceinline__ int wave_max_all(int v) {
 }
 
 // ---- queries whose weights f16 doesn't hold ----------------------------------------
-// Whether the sums of a query may have lost what counts, from its l (infinite where M is or was
-// far).  M lies 25 to 38 octaves
-// below the largest s + log2 vs of its keys.  Where that key's log2 vs is its own, its w is 2
-// or more; where it is kLeastVs instead, its p = 2^(s - M) is 2^85 or more, and so is l.  (l is
-// that large, too, where scales are below 2^-45 or so: for nothing, but right.)  The inner
-// loops pay nothing for it; a test of w itself, for each key, made them 2 to 5% slower.
-//
-// Such a query is done over by whoever has its sums last: the merge, for a chunk, or the kernel
-// where there is no merge.
-__device__ __forceinline__ bool lost(float l) { return l >= 0x1p84f; }
-
-// Whether any of a sequence's keys first .. last has a value that isn't a row of zeros; by a
-// whole wave.  Without one (nothing was written there yet) there is nothing to do over.
-__device__ bool any_value(const KvAttn &a, int b, int hk, int first, int last) {
-  const int lane = threadIdx.x & 63;
-  for (int base = first; base <= last; base += 64) {
-    const int key = base + lane;
-    const long slot = key <= last ? kv_slot(a.c, a.b, b, key, hk) : -1;
-    if (__any(slot >= 0 && a.c.vs[max(slot, 0l)] != 0.0f)) return true;
+// Whether any of a sequence's keys first .. last has a scale that counted as kLeastVs for more than
+// it is; by a whole wave.
+__device__ bool any_small(const KvAttn &a, int b, int hk, int first, int last) {
+  bool small = false;
+  for (int key = first + (threadIdx.x & 63); key <= last; key += 64) {
+    const long slot = kv_slot(a.c, a.b, b, key, hk);
+    const float vs = slot >= 0 ? fabsf(a.c.vs[slot]) : 0.0f;
+    small = small || (vs > 0.0f && vs < 0x1p-60f);
   }
-  return false;
+  return __any(small);
+}
+
+// A query's l, infinite where its sums have lost what counts: M is far, or has been, or was set
+// by a key of a small scale among the wave's first .. last.  M lies 25 to 38 octaves below the
+// largest s + log2 vs of its keys.  Where that key's log2 vs is its own, its w is 2 or more; where
+// it is kLeastVs instead, its p = 2^(s - M) is 2^85 or more, and so is l.  (l is that large, too,
+// where all scales are below 2^-45 or so, or 0.)  The inner loops pay nothing for it; a test of w
+// itself, for each key, made them 2 to 5% slower.
+//
+// A query with an infinite l is done over by whoever has its sums last: the merge, for a chunk,
+// or the kernel where there is no merge.
+__device__ __forceinline__ float marked(const KvAttn &a, const Soft &s, int b, int hk, int first,
+                                        int last) {
+  float l = far(s.m) ? INFINITY : s.l;
+  const bool large = l >= 0x1p84f;
+  if (__any(large && l < INFINITY) && any_small(a, b, hk, first, last) && large) l = INFINITY;
+  return l;
 }
 
 __device__ __forceinline__ double wave_max_f64(double v) {
@@ -483,18 +489,22 @@ __device__ Wide<HD> wide_query(const KvAttn &a, int b, int hk, const float *q, i
   for (int base = lo; base <= hi; base += 64) {
     const int key = base + lane;
     const long slot = key <= hi ? kv_slot(a.c, a.b, b, key, hk) : -1;
-    unsigned long long live = __ballot(slot >= 0);
+    const unsigned long long live = __ballot(slot >= 0);
     if (live == 0) continue;
     double s = -INFINITY, vs = 0.0;
     if (slot >= 0) {
       const uint32_t *codes = reinterpret_cast<const uint32_t *>(a.c.k + (size_t)slot * HD);
       double dot = 0.0;
-#pragma unroll 1  // (and below: registers count here, time doesn't)
-      for (int d = 0; d < HD; d += 4) {
-        float f[4];
-        codes4<TYPE>(codes[d / 4], f);
+#pragma unroll 1  // (registers count here, time less)
+      for (int d = 0; d < HD; d += 16) {
+        const u4 x = *reinterpret_cast<const u4 *>(codes + d / 4);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) dot = fma((double)q[d + e], (double)f[e], dot);
+        for (int u = 0; u < 4; ++u) {
+          float f[4];
+          codes4<TYPE>(x[u], f);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dot = fma((double)q[d + 4 * u + e], (double)f[e], dot);
+        }
       }
       s = dot * (double)a.c.ks[slot] * (double)a.asc;
       if (a.cap != 0.0f) s = tanh(s / (double)a.cap) * (double)a.cap;
@@ -509,19 +519,25 @@ __device__ Wide<HD> wide_query(const KvAttn &a, int b, int hk, const float *q, i
 #pragma unroll
     for (int e = 0; e < E; ++e) r.x[e] *= f;
 #pragma unroll 1
-    for (; live != 0; live &= live - 1) {
-      const int i = __ffsll(live) - 1;
-      const double wi = readlane_f64(w, i);
-      const size_t at = (size_t)__builtin_amdgcn_readlane((int)(slot >> 32), i) << 32 |
-                        (uint32_t)__builtin_amdgcn_readlane((int)slot, i);
-      const uint8_t *codes = a.c.v + at * HD + E * lane;
-      float c[4];
-      if constexpr (E == 4)
-        codes4<TYPE>(*reinterpret_cast<const uint32_t *>(codes), c);
-      else
-        codes4<TYPE>(*reinterpret_cast<const uint16_t *>(codes), c);
+    for (int i0 = 0; i0 < 64; i0 += 4) {
+      typedef std::conditional_t<E == 4, uint32_t, uint16_t> T;
+      T v[4];
 #pragma unroll
-      for (int e = 0; e < E; ++e) r.x[e] = fma(wi, (double)c[e], r.x[e]);
+      for (int u = 0; u < 4; ++u) {  // (a key that isn't there: any row, not used)
+        const long at = max(slot, 0l);
+        const size_t row = (size_t)__builtin_amdgcn_readlane((int)(at >> 32), i0 + u) << 32 |
+                           (uint32_t)__builtin_amdgcn_readlane((int)at, i0 + u);
+        v[u] = *reinterpret_cast<const T *>(a.c.v + row * HD + E * lane);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (!(live >> (i0 + u) & 1)) continue;
+        const double wi = readlane_f64(w, i0 + u);
+        float c[4];
+        codes4<TYPE>(v[u], c);
+#pragma unroll
+        for (int e = 0; e < E; ++e) r.x[e] = fma(wi, (double)c[e], r.x[e]);
+      }
     }
   }
   return r;
@@ -717,9 +733,10 @@ __device__ __forceinline__ void step_keys(const KvAttn &a, const KvPlan &pl, int
   // the waves' sums, by the largest M
   soft.l += __shfl_xor(soft.l, 16, 64);
   soft.l += __shfl_xor(soft.l, 32, 64);
+  soft.l = marked(a, soft, b, hk, kTile * t0, min(kTile * t1, s.len) - 1);
   if (g == 0) {
     sm[wave][n] = soft.m;
-    sl[wave][n] = far(soft.m) ? INFINITY : soft.l;
+    sl[wave][n] = soft.l;
   }
   __syncthreads();
   if (n < rows) {
@@ -739,13 +756,12 @@ __device__ __forceinline__ void step_keys(const KvAttn &a, const KvPlan &pl, int
   auto out_of = [&](int q) {
     return a.out + ((size_t)(s.r0 + q / pl.group) * a.n_heads + hk * pl.group + q % pl.group) * HD;
   };
-  unsigned again = 0;  // a bit for each query of which a wave has lost something
+  unsigned again = 0;  // a bit for each query that is done over here
   if (WHOLE) {
     static_assert(kStepWaves * kStepRows == 64, "a lane each");
-    const unsigned long long marks = __ballot(lost((&sl[0][0])[lane]));
+    const unsigned long long marks = __ballot((&sl[0][0])[lane] == INFINITY);
     again = (unsigned)(marks | marks >> 32);
     again = (again | again >> 16) & ((1u << rows) - 1);
-    if (again != 0 && !any_value(a, b, hk, kTile * kr.t0, s.len - 1)) again = 0;
   }
   for (int e = threadIdx.x; e < rows * (HD / 4); e += 64 * kStepWaves) {
     const int q = e / (HD / 4), d = 4 * (e % (HD / 4));
@@ -756,7 +772,7 @@ __device__ __forceinline__ void step_keys(const KvAttn &a, const KvPlan &pl, int
     v4f x = {};
 #pragma unroll
     for (int w = 0; w < kStepWaves; ++w) {
-      const float own = sl[w][q];  // (an infinite one, which is a mark, stays so)
+      const float own = sl[w][q];  // (an infinite one, the mark, stays so)
       l += own == INFINITY ? own : own * __builtin_amdgcn_exp2f(sm[w][q] - m);
       x += *reinterpret_cast<const v4f *>(&part[w][q][d]);
     }
@@ -1223,16 +1239,31 @@ __device__ __forceinline__ void rows_keys(const KvAttn &a, const KvPlan &pl, int
   for (int q = 0; q < QB; ++q) {
     soft[q].l += __shfl_xor(soft[q].l, 16, 64);
     soft[q].l += __shfl_xor(soft[q].l, 32, 64);
-    if (far(soft[q].m)) soft[q].l = INFINITY;
+    soft[q].l = marked(a, soft[q], b, hk, kTile * t0, min(kTile * t1, len) - 1);
     const bool there = at + 16 * (QB * wave + q) + n < rows;
     const bool whole = !PRE && ns == 1 && pl.pre_ns == 0;
-    unsigned again = 0;  // a bit for each query that has lost something
-    if (!PRE && whole) {
-      again = (unsigned)__ballot(there && lost(soft[q].l)) & 0xffff;
-      if (again != 0 && !any_value(a, b, hk, kTile * t0, min(kTile * t1, len) - 1)) again = 0;
+    unsigned again = 0;  // a bit for each query that is done over here
+    if (!PRE && whole) again = (unsigned)__ballot(there && soft[q].l == INFINITY) & 0xffff;
+    if (there && !(again >> n & 1)) {
+      const size_t vec = (size_t)qrow[q] * a.n_heads + qhead[q];
+      const size_t pt = (size_t)chunk * a.b.rows * a.n_heads + vec;
+      float *dst = whole ? a.out + vec * HD
+                         : (float *)(a.work + (PRE ? pl.pre_o : pl.rows_o)) + pt * HD;
+      const float f = !whole ? 1.0f : soft[q].l != 0.0f ? 1.0f / (soft[q].l * kVsUnit) : 0.0f;
+      // o[4 w + i][r]: dim 64 w + 16 r + 4 g + i
+#pragma unroll
+      for (int w = 0; w < HD / 64; ++w)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          v4f x = v4f{o[q][4 * w][r], o[q][4 * w + 1][r], o[q][4 * w + 2][r], o[q][4 * w + 3][r]};
+          x = f != 0.0f ? x * f : v4f{};
+          *reinterpret_cast<v4f *>(dst + 64 * w + 16 * r + 4 * g) = x;
+        }
+      if (!whole && g == 0)
+        ((float2 *)(a.work + (PRE ? pl.pre_m : pl.rows_m)))[pt] = float2{soft[q].m, soft[q].l};
     }
-    for (unsigned rest = again; rest != 0; rest &= rest - 1) {
-      const int i = __ffs(rest) - 1;
+    for (; again != 0; again &= again - 1) {
+      const int i = __ffs(again) - 1;
       const size_t row = __builtin_amdgcn_readlane(qrow[q], i);
       const int head = __builtin_amdgcn_readlane(qhead[q], i);
       wide_out(wide_query<HD, TYPE>(a, b, hk, a.q + row * a.q_stride + head * HD,
@@ -1240,23 +1271,6 @@ __device__ __forceinline__ void rows_keys(const KvAttn &a, const KvPlan &pl, int
                                     __builtin_amdgcn_readlane(see[q].hi, i)),
                a.out + (row * a.n_heads + head) * HD);
     }
-    if (!there || (again >> n & 1)) continue;
-    const size_t vec = (size_t)qrow[q] * a.n_heads + qhead[q];
-    const size_t pt = (size_t)chunk * a.b.rows * a.n_heads + vec;
-    float *dst = whole ? a.out + vec * HD
-                       : (float *)(a.work + (PRE ? pl.pre_o : pl.rows_o)) + pt * HD;
-    const float f = !whole ? 1.0f : soft[q].l != 0.0f ? 1.0f / (soft[q].l * kVsUnit) : 0.0f;
-    // o[4 w + i][r]: dim 64 w + 16 r + 4 g + i
-#pragma unroll
-    for (int w = 0; w < HD / 64; ++w)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        v4f x = v4f{o[q][4 * w][r], o[q][4 * w + 1][r], o[q][4 * w + 2][r], o[q][4 * w + 3][r]};
-        x = f != 0.0f ? x * f : v4f{};
-        *reinterpret_cast<v4f *>(dst + 64 * w + 16 * r + 4 * g) = x;
-      }
-    if (!whole && g == 0)
-      ((float2 *)(a.work + (PRE ? pl.pre_m : pl.rows_m)))[pt] = float2{soft[q].m, soft[q].l};
   }
 }
 
@@ -1358,7 +1372,6 @@ __global__ __launch_bounds__(64 * (SHARE > kMergeWaves ? SHARE : kMergeWaves)) v
 #pragma unroll
     for (int e = 0; e < E; ++e) x[e] = x[e] * f + y[e] * h;
   };
-  bool some = false;  // chunks that have lost something are left for later
   constexpr int A = SHARE == 16 ? 8 : 4;  // chunks loaded at a time
   for (int c = part; c < total; c += A * SHARE) {
     float2 v[A];
@@ -1374,29 +1387,31 @@ __global__ __launch_bounds__(64 * (SHARE > kMergeWaves ? SHARE : kMergeWaves)) v
 #pragma unroll
     for (int u = 0; u < A; ++u) {
       if (c + u * SHARE >= total) break;
-      if (lost(v[u].y))
-        some = true;
-      else
-        add(v[u], y[u]);
+      add(v[u], y[u]);
     }
   }
-  if (__any(some)) {
+  if (__any(!(l < INFINITY))) {  // some chunk is to be done over: all once more
+    m = kFloor;
+    l = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = 0.0f;
     const float *from = a.q + (size_t)(s.r0 + i) * a.q_stride + head * HD;
     const KvSpan sees = kv_span(p0 + i, s.len, a.slide, a.dense);
     for (int c = part; c < total; c += SHARE) {
       const float *o;
       float2 v = where(c, &o);
-      if (!lost(v.y)) continue;
-      const bool own = c < n;
-      const int first = kTile * (own ? t0 + c * tpc : (c - n) * pl.pre_tpc);
-      const int lo = max(own ? max(sees.lo, a.shared) : sees.lo, first);
-      const int hi = min(own ? sees.hi : min(sees.hi, a.shared - 1),
-                         first + kTile * (own ? tpc : pl.pre_tpc) - 1);
       float y[E];
-#pragma unroll
-      for (int e = 0; e < E; ++e) y[e] = o[E * lane + e];
-      if (v.y == INFINITY || any_value(a, own ? b : 0, hk, lo, hi))
+      if (v.y == INFINITY) {
+        const bool own = c < n;
+        const int first = kTile * (own ? t0 + c * tpc : (c - n) * pl.pre_tpc);
+        const int lo = max(own ? max(sees.lo, a.shared) : sees.lo, first);
+        const int hi = min(own ? sees.hi : min(sees.hi, a.shared - 1),
+                           first + kTile * (own ? tpc : pl.pre_tpc) - 1);
         v = wide_part(wide_query<HD, TYPE>(a, own ? b : 0, hk, from, lo, hi), y);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[e] = o[E * lane + e];
+      }
       add(v, y);
     }
   }
