@@ -417,24 +417,25 @@ __device__ __forceinline__ int wave_max_all(int v) {
 }
 
 // ---- queries whose weights f16 doesn't hold ----------------------------------------
-// Whether any of a sequence's keys first .. last has a scale that counted as kLeastVs for more than
-// it is; by a whole wave.
+// Whether, of a sequence's keys first .. last, any has a scale that counted as kLeastVs for more
+// than it is, and any a value (not so: nothing but zeros was written there); by a whole wave.
 __device__ bool any_small(const KvAttn &a, int b, int hk, int first, int last) {
-  bool small = false;
+  bool small = false, value = false;
   for (int key = first + (threadIdx.x & 63); key <= last; key += 64) {
     const long slot = kv_slot(a.c, a.b, b, key, hk);
-    const float vs = slot >= 0 ? fabsf(a.c.vs[slot]) : 0.0f;
-    small = small || (vs > 0.0f && vs < 0x1p-60f);
+    const float vs = slot >= 0 ? fabsf(a.c.vs[slot]) : 1.0f;
+    small = small || vs < 0x1p-60f;
+    value = value || (slot >= 0 && vs != 0.0f);
   }
-  return __any(small);
+  return __any(small) && __any(value);
 }
 
 // A query's l, infinite where its sums have lost what counts: M is far, or has been, or was set
-// by a key of a small scale among the wave's first .. last.  M lies 25 to 38 octaves below the
-// largest s + log2 vs of its keys.  Where that key's log2 vs is its own, its w is 2 or more; where
-// it is kLeastVs instead, its p = 2^(s - M) is 2^85 or more, and so is l.  (l is that large, too,
-// where all scales are below 2^-45 or so, or 0.)  The inner loops pay nothing for it; a test of w
-// itself, for each key, made them 2 to 5% slower.
+// by a key of a small scale, or of zeros, among the wave's first .. last.  M lies 25 to 38
+// octaves below the largest s + log2 vs of its keys.  Where that key's log2 vs is its own, its w
+// is 2 or more; where it is kLeastVs instead, its p = 2^(s - M) is 2^85 or more, and so is l.
+// (l is that large, too, where all scales are below 2^-45 or so, or 0.)  The inner loops pay
+// nothing for it; a test of w itself, for each key, made them 2 to 5% slower.
 //
 // A query with an infinite l is done over by whoever has its sums last: the merge, for a chunk,
 // or the kernel where there is no merge.
@@ -562,7 +563,9 @@ __device__ __forceinline__ float2 wide_part(const Wide<HD> &r, float (&x)[HD / 6
   for (int e = 0; e < HD / 64; ++e) most = fmax(most, fabs(r.x[e]));
   most = wave_max_f64(most);
   const bool both = most > 0.0 && r.l > 0.0 && fabs(r.m) < 0x1p29;
-  const double by = both ? rint(0.5 * (kVsOctaves - log2(r.l) - log2(most))) : 0.0;
+  // (past 2^-90 of l the others round to zeros, which is what they are beside it)
+  const double by =
+      both ? fmin(rint(0.5 * (kVsOctaves - log2(r.l) - log2(most))), 90.0) : 0.0;
   const float m = fabs(r.m) < INFINITY ? (float)(r.m - by) : kFloor;
   double up = r.m - (double)m;
   if (!(fabs(up - by) <= 32.0)) up = by;
@@ -577,7 +580,9 @@ __device__ __forceinline__ float2 wide_part(const Wide<HD> &r, float (&x)[HD / 6
 // to registers, a tile (16 KB of 256 dims) ahead of their use.  Bound by the cache's bytes
 // where there are many: 32 gemma-3-4b tokens of up to 8192 int8 positions (335 MB) take 75
 // us, 4.5 TB/s of the 5.1 that a large copy reaches; two gemma-3-1b ones of 131072 e4m3
-// positions (136 MB) 30 us.  Few keys are a chain of round trips to memory (tables, page ids,
+// positions (136 MB) 30 us.  256 dims take all of the 256 registers that two workgroups a
+// compute unit leave a lane, and 13 to 28 more that wait in scratch, most of them read outside
+// the inner loop.  Few keys are a chain of round trips to memory (tables, page ids,
 // the query and codes, each about a microsecond) and code fetched cold: one token of 1001
 // positions takes 9 to 10 us.
 
@@ -806,7 +811,8 @@ __global__ __launch_bounds__(64 * kStepWaves, 2) void kv_step_kernel(KvAttn a, K
 // tile's codes are made f16 once, a share by each wave, and reach the others through LDS in
 // operand order (16-byte reads of 64 lanes in a row: no conflicts).  128 vectors of 256
 // dims are eight waves of 16: two a SIMD hide more of each other's waits than one of 32
-// vectors (two 2048-token gemma-3-4b prompts in a window of 1024: 85 us, 93 with four waves).
+// vectors (two 2048-token gemma-3-4b prompts in a window of 1024: 85 us, 93 with four waves, both
+// in a kernel trace, under which this kernel takes a tenth longer: calls in turn 75 us).
 // Their 4100 cycles a tile are 2050 of products, about 2600 of LDS traffic (every wave
 // reads all of a tile's fragments) and 1800 of vector work, which overlap in part; a third
 // of the whole is the card's wait for the workgroups that have the most keys.
@@ -1482,6 +1488,8 @@ KvPlan plan(const KvAttn &a, const DeviceInfo &dev) {
   auto blocks = [&](int qb) {
     return (int)std::max<long>(1, (vecs_kv + 64 * qb - 1) / (64 * qb)) * a.c.nkv;
   };
+  // (All figures are of 256 dims; 128 take the same rules, not measured on both sides, though two
+  // of their workgroups of 64 vectors fit a compute unit.)
   // A workgroup of 128 vectors of 256 dims takes 4100 cycles a tile and 25000 to begin, one
   // of 64 3000 and 16000, and writes half as much for the merge where there are chunks:
   // short runs take 64.  gemma-3-1b behind 16384 positions, merge included: 256 vectors (8

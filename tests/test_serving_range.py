@@ -209,3 +209,28 @@ def test_scores_that_come_from_far(gh, name, octaves, kind):
     torch.cuda.synchronize()
     sees = out[:p.n[0]].cpu().numpy()[[p.len[0] - p.n[0] + i >= 1 for i in range(p.n[0])]]
     assert np.isnan(sees).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", sorted(KINDS))
+@pytest.mark.parametrize("octaves", [0, -70])
+@pytest.mark.parametrize("ahead", [80, 1000])
+@pytest.mark.parametrize("name", ["step", "step_long", "prompt", "prompt_large", "prefix",
+                                  "prefix_mixed"])
+def test_positions_of_zeros_with_the_most_weight(gh, name, ahead, octaves, kind):
+    """A position of zeros scores so many octaves above the others that these are 2^-80 of the
+    sum, or nothing; then one further on scores above both."""
+    _, heads, _, hd, slide, shared, step = SHAPES[name]
+    p, q = scored_cache(name, kind, 0, 1.0)
+    p.scales["v"] *= F32(2.0) ** octaves
+    p.scales["k"] = np.where(np.isfinite(p.scales["k"]), 0, np.nan).astype(F32)
+    unit = np.log(2.0) * ahead / (64 if kind == "i8" else 1)
+    for b, ln in enumerate(p.len):
+        if ln > 20:
+            at = p.table[b, 1], slice(None), 3  # (position 19)
+            p.scales["k"][at], p.scales["v"][at], p.codes["v"][at] = unit, 0.0, 0
+    check(gh, p, q, heads, 1.0, slide, 0.0, shared, step)
+    for b, ln in enumerate(p.len):
+        if ln > 60:
+            p.scales["k"][p.table[b, (ln - 5) // 16], :, (ln - 5) % 16] = 2.0 * unit
+    check(gh, p, q, heads, 1.0, slide, 0.0, shared, step)
