@@ -12,7 +12,9 @@
 //
 // Weights are fp64.  A bin's tokens weigh 1 to 1.044 times its lower end: what a token
 // adds is 1 and a fraction in whole multiples of 2^-39, count and fraction in one
-// 64-bit sum, exact in any order.  Sums over bins and workgroups are fp64 in one order.
+// 64-bit sum, exact in any order.  What the last bin's add is whole multiples of 2^-44 of the
+// bin's upper end, some 2^-75 of the row's largest weight.  Sums over bins and workgroups are
+// fp64 in one order.
 // So equal calls give equal bits.
 //
 // Up to kWholeVocab columns a workgroup does a row by itself, from registers.  Longer rows
@@ -24,9 +26,10 @@
 // Of 16000 columns one row by top-k 64 and top-p 0.95 takes 17 us, 64 rows with settings of
 // all kinds 22 (24 and 37 when the bins' tokens are looked for in the row, not in a list).
 // Of 262144 columns, us: the one row 8 + 13 + 5 + 8, four chains of round trips and of code
-// fetched cold; the 64 rows (67 MB) 26 + 13 + 18 + 28: the first by its fp64 work (2.6 TB/s;
-// copies of the bins, for fewer lanes in one, change nothing), the last by the rows that cut
-// deep into a flat part, a workgroup each.
+// fetched cold; the 64 rows (67 MB) 26 + 13 + 18 + 28: the first by its vector instructions (47
+// a logit, a fifth of them fp64 arithmetic, keep the vector units busy for three quarters of
+// the time and more; LDS, conflicts included, for a third; 2.6 TB/s), the last by the rows that
+// cut deep into a flat part, a workgroup each.
 #include <float.h>
 #include <limits.h>
 

@@ -619,9 +619,16 @@ int gemma_hip_cache_read(const gemma_hip_cache *cache, const gemma_hip_batch *ba
  * position p sees keys max(0, p + 1 - slide) .. p (slide 0: no window; dense != 0:
  * every key of its sequence); scores are q.k * asc, capped as tanh(s / sc_att) *
  * sc_att when sc_att != 0.  A row that sees nothing is zeros.  out and q do not overlap.
+ * Arithmetic: codes are exact; q's values and the softmax weights are off by at most 2^-23 of
+ * themselves (small ones of q by 2^-39 of the head's largest, weights far below the largest
+ * by 2^-26 of it), sums are fp32.  Rows whose weight lies on values with scales below 2^-60,
+ * or whose scores pass 2^23 octaves, are computed in 64 bits, which takes some tens of times
+ * longer (rows of zeros don't).
  * shared: the first `shared` positions lie in the same pages for every sequence (a
  * common prefix; 0: none).  Each sequence's table lists them; the first one's is
- * read, and their keys and values are read once for all rows.
+ * read, and their keys and values are read once for all rows.  All of them are, whether a
+ * window lets a row see them or not: in layers whose window ends in or behind the prefix, 0 is
+ * the faster of two right answers.
  * work: gemma_hip_cache_attention_work() bytes of device memory for these sizes,
  * 256-byte aligned, which one call at a time may use; NULL takes the workspace
  * that the library keeps for the stream (not while it is being captured). */
@@ -654,9 +661,9 @@ typedef struct {
  * >= min_p; the token is the first whose running sum exceeds u times the sum of the
  * kept ones.  NaN logits count as -inf, which is never drawn; +inf ones take all.
  * tokens [rows] (-1 where no logit is above -inf) and probs [rows] (nullable, the
- * token's share of the kept sum).  Weights are 64-bit, off by at most 2^-39 of
- * themselves in the sums, which no order of the work changes: equal calls draw equal
- * tokens.
+ * token's share of the kept sum).  Weights are 64-bit.  In the sums, which no order of
+ * the work changes (equal calls draw equal tokens), one is off by at most 2^-39 of itself,
+ * or, where it is below 2^-30 of the row's largest, by 2^-74 of that one.
  * work: gemma_hip_sample_work() bytes, as above. */
 int gemma_hip_sample(int *tokens, float *probs, const float *logits, int stride, int rows,
                      int vocab, const gemma_hip_sampling *settings, const float *u, void *work,
