@@ -28,7 +28,7 @@
 // Of 262144 columns, us: the one row 8 + 13 + 5 + 8, four chains of round trips and of code
 // fetched cold; the 64 rows (67 MB) 26 + 13 + 18 + 28: the first by its vector instructions (47
 // a logit, a fifth of them fp64 arithmetic, keep the vector units busy for three quarters of
-// the time and more; LDS, conflicts included, for a third; 2.6 TB/s), the last by the rows that
+// the time and more; LDS, conflicts included, for two fifths; 2.6 TB/s), the last by the rows that
 // cut deep into a flat part, a workgroup each.
 #include <float.h>
 #include <limits.h>
