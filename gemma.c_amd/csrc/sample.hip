@@ -15,7 +15,9 @@
 // 64-bit sum, exact in any order.  What the last bin's add is whole multiples of 2^-44 of the
 // bin's upper end, some 2^-75 of the row's largest weight.  Sums over bins and workgroups are
 // fp64 in one order.
-// So equal calls give equal bits.
+// So equal calls give equal bits.  What a token adds is the same wherever it is summed, so that
+// sums over equal logits meet a target (top-p's, the draw's) where exact ones do: at or past it
+// within kTie.
 //
 // Up to kWholeVocab columns a workgroup does a row by itself, from registers.  Longer rows
 // take four launches: each 8192-column chunk's bins, from its own largest logit down so that
@@ -56,6 +58,7 @@ constexpr int kList = 32768;       // tokens of a row's bins that are collected,
 constexpr int kFrac = 39;          // a bin's sum: fractions in 2^-39 below, the count above
 constexpr int kCountAt = 49;       // (2^14 tokens of fractions below 0.0443 stay below 2^49)
 constexpr int kUnit = 44;          // a weight's units within its bin: 2^-44 of the bin's octave
+constexpr double kTie = 0x1p-46;   // of a target: sums as near count as equal to it
 constexpr double kInfZ = 0x1p1000;  // an infinite logit, far above any other's octaves
 
 // A token's place in the order: rising.  NaN and -inf have none.
@@ -114,7 +117,7 @@ __device__ __forceinline__ double octave_scale(const Sample &a, int row) {
   const float t = a.temperature != nullptr ? a.temperature[row] : 1.0f;
   return t > 0.0f ? log2e / (double)t : log2e;
 }
-__device__ Settings settings(const Sample &a, int row) {
+__device__ __forceinline__ Settings settings(const Sample &a, int row) {
   Settings s;
   const float t = a.temperature != nullptr ? a.temperature[row] : 1.0f;
   s.c = octave_scale(a, row);
@@ -134,14 +137,11 @@ __device__ Settings settings(const Sample &a, int row) {
 }
 
 // Where bins lie: bin i holds 16 z in [gmax - i, gmax - i + 1), the last one all below;
-// weights are relative to 2^e.
+// weights are relative to the first one's lower end.
 struct Grid {
-  double gmax, e;
+  double gmax;
 };
-__device__ __forceinline__ Grid grid_of(float most, double c) {
-  const double z = octaves(most, c);
-  return {floor(z * kPerOctave), ceil(z)};
-}
+__device__ __forceinline__ Grid grid_of(double zmax) { return {floor(zmax * kPerOctave)}; }
 __device__ __forceinline__ int bin_at(double y, double gmax) {  // y: z kPerOctave
   const double d = gmax - floor(y);
   return d >= kBins - 1 ? kBins - 1 : (int)d;
@@ -149,10 +149,40 @@ __device__ __forceinline__ int bin_at(double y, double gmax) {  // y: z kPerOcta
 __device__ __forceinline__ int bin_of(double z, double gmax) {
   return bin_at(z * kPerOctave, gmax);
 }
-// The power of two that no weight of a bin exceeds, relative to the row's.
-__device__ __forceinline__ double bin_top(int bin, const Grid &g) {
-  return ceil((g.gmax - bin + 1.0) / kPerOctave);
+// The power of two that no weight of the last bin exceeds.
+__device__ __forceinline__ double rest_top(const Grid &g) {
+  return ceil((g.gmax - (kBins - 1) + 1.0) / kPerOctave);
 }
+
+// What a token r of a bin's width above the bin's lower end adds to the bin's sum: 1 and
+// 2^(r / 16) - 1 in units of 2^-kFrac, by its Taylor polynomial (what it leaves out is below
+// 2^-43), whose coefficients hold the units and whose last step rounds to a whole number.
+__device__ __forceinline__ u64 bin_term(double r) {
+  constexpr double q = 0x1.62e42fefa39efp-5;  // ln 2 / 16
+  constexpr double unit = (double)(1ull << kFrac);
+  constexpr double c1 = q * unit, c2 = c1 * q / 2.0, c3 = c2 * q / 3.0, c4 = c3 * q / 4.0,
+                   c5 = c4 * q / 5.0, c6 = c5 * q / 6.0;
+  double p = fma(r, c6, c5);
+  p = fma(r, p, c4);
+  p = fma(r, p, c3);
+  p = fma(r, p, c2);
+  p = fma(r, p, c1);
+  p = fma(r, p, 0x1p52);
+  return ((u64)__double_as_longlong(p) & ((1ull << kCountAt) - 1)) | 1ull << kCountAt;
+}
+
+// What a token of a bin (its z kPerOctave: y) adds to the bin's sum, in the bin's units ...
+__device__ __forceinline__ u64 token_units(double y, int bin, const Grid &g, const double *tab) {
+  if (bin < kBins - 1) return (bin_term(y - floor(y)) & ((1ull << kCountAt) - 1)) + (1ull << kFrac);
+  const double x = y * (1.0 / kPerOctave) - rest_top(g);
+  return x > -64.0 ? units(pow2(x, tab), kUnit) : 0;
+}
+// ... and these units.
+__device__ __forceinline__ double bin_unit(int bin, const Grid &g, const double *tab) {
+  return bin < kBins - 1 ? pow2(bin * (-1.0 / kPerOctave), tab) * 0x1p-39
+                         : pow2(rest_top(g) - g.gmax * (1.0 / kPerOctave), tab) * 0x1p-44;
+}
+static_assert(kFrac == 39 && kUnit == 44, "bin_unit's");
 
 constexpr uint32_t kNone = ~0u;
 constexpr int kPerLane = kBins / 64;
@@ -226,8 +256,12 @@ __device__ __forceinline__ void min_p_bins(const Row &r, double m, int (&b)[2]) 
   b[1] = z - slack >= r.zmax ? 0 : bin_of(z - slack, r.g.gmax);
 }
 
+// What a running sum has to reach to be at least t, or to exceed it.
+__device__ __forceinline__ double at_least(double t) { return t - t * kTie; }
+__device__ __forceinline__ double past(double t) { return t + t * kTie; }
+
 // Running sums over the bins, by wave 0 (count, then weight).
-__device__ void sum_bins(const uint32_t *count, const double *mass, Row &r) {
+__device__ __forceinline__ void sum_bins(const uint32_t *count, const double *mass, Row &r) {
   const int lane = threadIdx.x;
   if (lane >= 64) return;
   uint32_t c[kPerLane], cs = 0;
@@ -259,7 +293,7 @@ __device__ void sum_bins(const uint32_t *count, const double *mass, Row &r) {
 // Marks the bins that pick() may look into, by wave 0.  A target that is a share of
 // a sum which itself depends on a border inside a bin lies between the shares of
 // that bin's ends.
-__device__ void decide(const Settings &st, Row &r) {
+__device__ __forceinline__ void decide(const Settings &st, Row &r) {
   const int lane = threadIdx.x;
   if (lane >= 64) return;
   const Bins bins(r);
@@ -281,7 +315,8 @@ __device__ void decide(const Settings &st, Row &r) {
       mark(cut_lo, cut_hi);
   }
   if (st.p < 1.0) {
-    const int lo = bins.by_weight(st.p * s_lo), hi = bins.by_weight(st.p * s_hi);
+    const int lo = bins.by_weight(at_least(st.p * s_lo));
+    const int hi = bins.by_weight(at_least(st.p * s_hi));
     mark(min(lo, cut_lo), min(hi, cut_hi));
     cut_lo = min(cut_lo, lo);
     cut_hi = min(cut_hi, hi);
@@ -299,7 +334,7 @@ __device__ void decide(const Settings &st, Row &r) {
       s_hi = fmin(s_hi, r.weight(cut_hi));
     }
   }
-  mark(bins.past_weight(st.u * s_lo), min(bins.past_weight(st.u * s_hi), cut_hi));
+  mark(bins.past_weight(past(st.u * s_lo)), min(bins.past_weight(past(st.u * s_hi)), cut_hi));
   // list positions
   uint32_t own[kPerLane], sum = 0;
 #pragma unroll
@@ -342,6 +377,12 @@ struct Lds {
   u64 red[3];
   uint32_t n;
 };
+
+// A token's weight, relative to the first bin's lower end.
+__device__ __forceinline__ double weight_of(const Settings &st, const Row &r, u64 place,
+                                            const double *tab) {
+  return pow2(octaves(logit_at(place), st.c) - r.g.gmax * (1.0 / kPerOctave), tab);
+}
 
 // A token found: how many tokens of its bin come before it, the weight of the bin up
 // to and with it, and its own.
@@ -401,8 +442,8 @@ __device__ __forceinline__ void each_of_bin(const Sample &a, int row, const Sett
 // count before, weight before.  By wave 0, first over N / 64 parts a lane, then over those
 // of the lane found, one each; barriers around it are the caller's.
 template <int N>
-__device__ void find_part(Lds &s, bool by_count, double target, bool strict, double unit,
-                          uint32_t count0, u64 mass0) {
+__device__ __forceinline__ void find_part(Lds &s, bool by_count, double target, bool strict,
+                                          double unit, uint32_t count0, u64 mass0) {
   const int lane = threadIdx.x;
   if (lane >= 64) return;
   constexpr int P = N / 64;
@@ -451,14 +492,16 @@ __device__ void find_part(Lds &s, bool by_count, double target, bool strict, dou
 //  - Up to 256 tokens: all pairs compared.
 //  - More: counted and weighed in 1024 parts of the bin, then the part's tokens.
 //  - Where a part has more than that (equal logits): digit by digit of the place.
-__device__ Found locate(const Sample &a, int row, const Settings &st, const Source &src, Lds &s,
-                        int bin, bool by_count, double target, bool strict, double base) {
+__device__ __forceinline__ Found locate(const Sample &a, int row, const Settings &st,
+                                        const Source &src, Lds &s, int bin, bool by_count,
+                                        double target, bool strict, double base) {
   const Row &r = s.row;
   const int tid = threadIdx.x;
-  const double top = bin_top(bin, r.g);
-  const double unit = ldexp(1.0, (int)fmax(top - r.g.e, -1000.0) - kUnit);
+  const double unit = bin_unit(bin, r.g, s.tab);
   if (!by_count) target -= base;
-  auto weigh = [&](u64 p) { return pow2(octaves(logit_at(p), st.c) - top, s.tab); };
+  auto weigh = [&](u64 p) {
+    return token_units(octaves(logit_at(p), st.c) * kPerOctave, bin, r.g, s.tab);
+  };
   // the part of the bin that a token falls into: any that falls as logits rise does; of the
   // last bin, 1/16 octave each
   const double edge = r.g.gmax - bin;  // 16 z of the bin's lower end
@@ -479,7 +522,7 @@ __device__ Found locate(const Sample &a, int row, const Settings &st, const Sour
     each_of_bin(a, row, st, src, r, bin, staged, [&](u64 p) {
       const int i = gap(part(p));
       atomicAdd(&s.count[i], 1u);
-      atomicAdd(&s.mass[i], units(weigh(p), kUnit));
+      atomicAdd(&s.mass[i], weigh(p));
     });
     __syncthreads();
     find_part<kSubs>(s, by_count, target, strict, unit, 0, 0);
@@ -499,7 +542,7 @@ __device__ Found locate(const Sample &a, int row, const Settings &st, const Sour
         if (part(p) != only || (shift < 56 && (p >> (shift + 8)) != prefix)) return;
         const int d = gap((int)(p >> shift) & 255);
         atomicAdd(&s.count[d], 1u);
-        atomicAdd(&s.mass[d], units(weigh(p), kUnit));
+        atomicAdd(&s.mass[d], weigh(p));
       });
       __syncthreads();
       find_part<256>(s, by_count, target, strict, unit, count0, mass0);
@@ -508,9 +551,8 @@ __device__ Found locate(const Sample &a, int row, const Settings &st, const Sour
       count0 = (uint32_t)s.red[1];
       mass0 = s.red[2];
     }
-    const double w = weigh(prefix);
-    return Found{prefix, count0, base + (double)(mass0 + units(w, kUnit)) * unit,
-                 w * ldexp(unit, kUnit)};
+    return Found{prefix, count0, base + (double)(mass0 + weigh(prefix)) * unit,
+                 weight_of(st, r, prefix, s.tab)};
   }
   // gather, rank, sum in order
   if (tid == 0) s.n = 0;
@@ -539,7 +581,7 @@ __device__ Found locate(const Sample &a, int row, const Settings &st, const Sour
   if (tid < (int)n) {
     const uint32_t at = s.count[tid];
     s.sorted[at] = s.place[tid];
-    s.weight[at] = (double)units(weigh(s.place[tid]), kUnit) * unit;
+    s.weight[at] = (double)weigh(s.place[tid]) * unit;
   }
   __syncthreads();
   if (tid < 64) {
@@ -576,12 +618,13 @@ __device__ Found locate(const Sample &a, int row, const Settings &st, const Sour
   }
   __syncthreads();
   const uint32_t at = (uint32_t)s.red[0];
-  return Found{s.sorted[at], count0 + at, base + s.wred[0], weigh(s.sorted[at]) * ldexp(unit, kUnit)};
+  return Found{s.sorted[at], count0 + at, base + s.wred[0],
+               weight_of(st, r, s.sorted[at], s.tab)};
 }
 
 // Where a bin's tokens are put in order once for all targets: those of all bins that
 // matter, up to kRanked, in s.sorted with running weights (over all of them) in s.weight.
-__device__ void rank_all(const Settings &st, u64 mine_, Lds &s) {
+__device__ __forceinline__ void rank_all(const Settings &st, u64 mine_, Lds &s) {
   const Row &r = s.row;
   const uint32_t n = r.listed, tid = threadIdx.x;
   if (tid < kRanked) {
@@ -601,8 +644,11 @@ __device__ void rank_all(const Settings &st, u64 mine_, Lds &s) {
   __syncthreads();
   if (tid < n) {
     const u64 p = s.place[tid];
+    const double y = octaves(logit_at(p), st.c) * kPerOctave;
+    const int bin = bin_at(y, r.g.gmax);
     s.sorted[s.count[tid]] = p;
-    s.weight[s.count[tid]] = pow2(octaves(logit_at(p), st.c) - r.g.e, s.tab);
+    s.weight[s.count[tid]] =
+        (double)token_units(y, bin, r.g, s.tab) * bin_unit(bin, r.g, s.tab);
   } else if (tid < kRanked) {
     s.weight[tid] = 0.0;
   }
@@ -650,14 +696,15 @@ __device__ __forceinline__ Found locate_ranked(const Settings &st, const Lds &s,
     at = min(at, hit);
   }
   const u64 p = s.sorted[from + at];
-  return Found{p, at, base + (s.weight[from + at] - start),
-               pow2(octaves(logit_at(p), st.c) - r.g.e, s.tab)};
+  return Found{p, at, base + (s.weight[from + at] - start), weight_of(st, r, p, s.tab)};
 }
 
 // The token, from the row's bins.
 // listed: the list's threadIdx.x-th.
-__device__ void pick(const Sample &a, int row, const Settings &st, const Source &src, u64 listed,
-                     Lds &s) {
+// (Inlined, as all that it calls and decide() are: calls would go through scratch, 8 to 45% of a
+// short row.)
+__device__ __forceinline__ void pick(const Sample &a, int row, const Settings &st,
+                                     const Source &src, u64 listed, Lds &s) {
   const Row &r = s.row;
   const Bins bins(r);
   const uint32_t total = r.sum_c[gap(kBins - 1)];
@@ -667,7 +714,8 @@ __device__ void pick(const Sample &a, int row, const Settings &st, const Source 
   if (ranked) rank_all(st, listed, s);
   // sums stay between the bins' own, whatever they were rounded to
   auto within = [&](double w, int bin) { return fmin(fmax(w, r.weight_before(bin)), r.weight(bin)); };
-  auto in_bin = [&](int bin, bool by_count, double target, bool strict) {
+  auto in_bin = [&](int bin, bool by_count, double target, bool strict)
+      __attribute__((always_inline)) {
     const double base = r.weight_before(bin);
     Found f = ranked && r.at[gap(bin)] != kNone
                   ? locate_ranked(st, s, bin, by_count, target, strict, base)
@@ -682,7 +730,7 @@ __device__ void pick(const Sample &a, int row, const Settings &st, const Source 
                                  : in_bin(bin, true, n - r.count_before(bin), false).upto;
   }
   if (st.p < 1.0) {
-    const double target = st.p * sum;
+    const double target = at_least(st.p * sum);
     const int bin = bins.by_weight(target);
     const Found f = in_bin(bin, false, target, false);
     const uint32_t np = r.count_before(bin) + f.before + 1;
@@ -709,14 +757,12 @@ __device__ void pick(const Sample &a, int row, const Settings &st, const Source 
         if (kept > 0)
           weight += s.weight[from + kept - 1] - (from > 0 ? s.weight[from - 1] : 0.0);
       } else if (in != 0) {
-        const double top = bin_top(bin, r.g);
-        const double unit = ldexp(1.0, (int)fmax(top - r.g.e, -1000.0) - kUnit);
         uint32_t c = 0;
         u64 w = 0;
         each_of_bin(a, row, st, src, r, bin, false, [&](u64 p) {
           if (!enough(p)) return;
           ++c;
-          w += units(pow2(octaves(logit_at(p), st.c) - top, s.tab), kUnit);
+          w += token_units(octaves(logit_at(p), st.c) * kPerOctave, bin, r.g, s.tab);
         });
         __syncthreads();
         if (threadIdx.x == 0) s.red[0] = s.red[1] = 0;
@@ -725,7 +771,7 @@ __device__ void pick(const Sample &a, int row, const Settings &st, const Source 
         atomicAdd(&s.red[1], w);
         __syncthreads();
         kept = (uint32_t)s.red[0];
-        weight += (double)s.red[1] * unit;
+        weight += (double)s.red[1] * bin_unit(bin, r.g, s.tab);
         __syncthreads();
       }
       if (kept == in && bin < b[1]) continue;
@@ -736,7 +782,7 @@ __device__ void pick(const Sample &a, int row, const Settings &st, const Source 
       break;
     }
   }
-  const double target = st.u * sum;
+  const double target = past(st.u * sum);
   int bin = min(bins.past_weight(target), bins.by_count(n));
   Found f = in_bin(bin, false, target, true);
   // where a rounding took the draw past the last token kept
@@ -750,7 +796,7 @@ __device__ void pick(const Sample &a, int row, const Settings &st, const Source 
   }
 }
 
-__device__ void pick_none(const Sample &a, int row) {
+__device__ __forceinline__ void pick_none(const Sample &a, int row) {
   if (threadIdx.x == 0) {
     a.tokens[row] = -1;
     if (a.probs != nullptr) a.probs[row] = 0.0f;
@@ -759,7 +805,7 @@ __device__ void pick_none(const Sample &a, int row) {
 
 // The largest of a workgroup's values (-inf: none), by waves through red[].
 template <int NT>
-__device__ float block_most(float v, float *red) {
+__device__ __forceinline__ float block_most(float v, float *red) {
   v = wave_max_dpp(v);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
@@ -767,23 +813,6 @@ __device__ float block_most(float v, float *red) {
 #pragma unroll
   for (int w = 1; w < NT / 64; ++w) m = fmaxf(m, red[w]);
   return m;
-}
-
-// What a token r of a bin's width above the bin's lower end adds to the bin's sum: 1 and
-// 2^(r / 16) - 1 in units of 2^-kFrac, by its Taylor polynomial (what it leaves out is below
-// 2^-43), whose coefficients hold the units and whose last step rounds to a whole number.
-__device__ __forceinline__ u64 bin_term(double r) {
-  constexpr double q = 0x1.62e42fefa39efp-5;  // ln 2 / 16
-  constexpr double unit = (double)(1ull << kFrac);
-  constexpr double c1 = q * unit, c2 = c1 * q / 2.0, c3 = c2 * q / 3.0, c4 = c3 * q / 4.0,
-                   c5 = c4 * q / 5.0, c6 = c5 * q / 6.0;
-  double p = fma(r, c6, c5);
-  p = fma(r, p, c4);
-  p = fma(r, p, c3);
-  p = fma(r, p, c2);
-  p = fma(r, p, c1);
-  p = fma(r, p, 0x1p52);
-  return ((u64)__double_as_longlong(p) & ((1ull << kCountAt) - 1)) | 1ull << kCountAt;
 }
 
 // Counts and weighs tokens into bins; the last bin's, which most tokens of a peaked
@@ -807,8 +836,7 @@ struct Binner {
       atomicAdd(&bins[(int)d], bin_term(y - f));
     } else {
       ++rest_c;
-      const double x = y * (1.0 / kPerOctave) - bin_top(kBins - 1, g);
-      if (x > -64.0) rest_m += units(pow2(x, tab), kUnit);
+      rest_m += token_units(y, kBins - 1, g, tab);
     }
   }
   // a thread's logits, of which `most` is the workgroup's largest
@@ -841,13 +869,9 @@ __device__ __forceinline__ uint32_t bin_count(u64 b) { return (uint32_t)(b >> kC
 __device__ __forceinline__ double bin_weight(u64 b) {
   return (double)bin_count(b) + ldexp((double)(b & ((1ull << kCountAt) - 1)), -kFrac);
 }
-// The last bin's weight, relative to 2^e.
-__device__ __forceinline__ double rest_weight(const Rest &r, const Grid &g) {
-  return ldexp((double)r.mass, (int)fmax(bin_top(kBins - 1, g) - g.e, -1000.0) - kUnit);
-}
-// A bin's lower end, relative to 2^e.
-__device__ __forceinline__ double bin_end(int bin, const Grid &g, const double *tab) {
-  return pow2((g.gmax - bin) * (1.0 / kPerOctave) - g.e, tab);
+// A bin's lower end, relative to the first one's.
+__device__ __forceinline__ double bin_end(int bin, const double *tab) {
+  return pow2(bin * (-1.0 / kPerOctave), tab);
 }
 
 // ---- short rows: a workgroup each -----------------------------------------------
@@ -876,7 +900,7 @@ __global__ __launch_bounds__(kThreads) void sample_whole_kernel(Sample a) {
   for (int e = 0; e < kWhole; ++e) most = fmaxf(most, x[e]);
   most = block_most<kThreads>(most, red);
   if (!has_place(most)) return pick_none(a, row);
-  const Grid g = grid_of(most, st.c);
+  const Grid g = grid_of(octaves(most, st.c));
   Binner bins(s.mass, &rest);
   bins.add_all(x, most, st.c, g, s.tab);
   bins.finish();
@@ -887,8 +911,8 @@ __global__ __launch_bounds__(kThreads) void sample_whole_kernel(Sample a) {
   __syncthreads();
   if (tid < kBins) {
     s.count[gap(tid)] = tid < kBins - 1 ? bin_count(s.mass[tid]) : rest.count;
-    mass[gap(tid)] = tid < kBins - 1 ? bin_weight(s.mass[tid]) * bin_end(tid, g, s.tab)
-                                     : rest_weight(rest, g);
+    mass[gap(tid)] = tid < kBins - 1 ? bin_weight(s.mass[tid]) * bin_end(tid, s.tab)
+                                     : (double)rest.mass * bin_unit(tid, g, s.tab);
   }
   __syncthreads();
   sum_bins(s.count, mass, s.row);
@@ -959,7 +983,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_bins_kernel(Sample a, Wo
     if (tid == 0) out->g.gmax = -INFINITY;
     return;
   }
-  const Grid g = grid_of(most, c);
+  const Grid g = grid_of(octaves(most, c));
   Binner bins(count, &rest);
   bins.add_all(x, most, c, g, tab);
   bins.finish();
@@ -1012,8 +1036,8 @@ __global__ __launch_bounds__(kThreads) void sample_decide_kernel(Sample a, Work 
     if (tid == 0) out->zmax = -INFINITY;
     return;
   }
-  const Grid g{floor(z * kPerOctave), ceil(z)};
-  const double top = bin_top(kBins - 1, g);
+  const Grid g = grid_of(z);
+  const double top = rest_top(g);
   // chunks without a token, and past the last, are shifted out
   const int shift =
       lane < nchunk && gm > -INFINITY ? (int)fmin(g.gmax - gm, (double)kBins) : 2 * kBins;
@@ -1041,7 +1065,7 @@ __global__ __launch_bounds__(kThreads) void sample_decide_kernel(Sample a, Work 
     }
   }
   if (tid < nchunk && shift <= kBins && mr.count != 0) {
-    const double down = top - ceil((gm - (kBins - 1) + 1.0) / kPerOctave);
+    const double down = top - rest_top(Grid{gm});
     rest_n += mr.count;
     rest_m += down < 64.0 ? mr.mass >> (int)down : 0;
   }
@@ -1057,9 +1081,9 @@ __global__ __launch_bounds__(kThreads) void sample_decide_kernel(Sample a, Work 
   __syncthreads();
   if (tid < kBins - 1) {
     mass[gap(tid)] =
-        ((double)count[gap(tid)] + ldexp((double)frac[tid], -kFrac)) * bin_end(tid, g, tab);
+        ((double)count[gap(tid)] + ldexp((double)frac[tid], -kFrac)) * bin_end(tid, tab);
   } else if (tid == kBins - 1) {
-    mass[gap(tid)] = rest_weight(rest, g);
+    mass[gap(tid)] = (double)rest.mass * bin_unit(tid, g, tab);
     count[gap(tid)] = rest.count;
   }
   if (tid == 0) {

@@ -663,7 +663,8 @@ typedef struct {
  * tokens [rows] (-1 where no logit is above -inf) and probs [rows] (nullable, the
  * token's share of the kept sum).  Weights are 64-bit.  In the sums, which no order of
  * the work changes (equal calls draw equal tokens), one is off by at most 2^-39 of itself,
- * or, where it is below 2^-30 of the row's largest, by 2^-74 of that one.
+ * or, where it is below 2^-30 of the row's largest, by 2^-74 of that one; equal logits
+ * weigh the same, and sums within 2^-46 of a target count as equal to it.
  * work: gemma_hip_sample_work() bytes, as above. */
 int gemma_hip_sample(int *tokens, float *probs, const float *logits, int stride, int rows,
                      int vocab, const gemma_hip_sampling *settings, const float *u, void *work,
