@@ -277,6 +277,12 @@ __device__ __forceinline__ float top_of(v4f (&d)[2], const float (&lv)[8], bool 
   return top;
 }
 
+// l by another M, `by` octaves above its own (a whole number, 0 or below).  In one step: beside
+// values of very different sizes l may be 2^98 where 2^by alone is 0.  An infinite l stays so.
+__device__ __forceinline__ float lowered(float l, float by) {
+  return ldexpf(l, (int)fmaxf(by, -400.0f));
+}
+
 __device__ __forceinline__ bool far(float m) { return fabsf(m) >= kFar && m > kFloor; }
 
 // Moves a query's M where the tile's largest weight needs it.  An M that was too far out leaves
@@ -288,7 +294,7 @@ __device__ __forceinline__ void settle(float top, Soft &s, F &&rescale) {
   top = fmaxf(top, __shfl_xor(top, 32, 64));
   const float m = top > s.m + kSlack ? ceilf(top) - kSet : s.m;
   const float f = __builtin_amdgcn_exp2f(s.m - m);
-  s.l = (m != s.m && far(s.m)) || s.l == INFINITY ? INFINITY : s.l * f;
+  s.l = m != s.m && far(s.m) ? INFINITY : lowered(s.l, s.m - m);
   s.m = m;
   rescale(f);
 }
@@ -566,7 +572,7 @@ __device__ __forceinline__ float2 wide_part(const Wide<HD> &r, float (&x)[HD / 6
   // (past 2^-90 of l the others round to zeros, which is what they are beside it)
   const double by =
       both ? fmin(rint(0.5 * (kVsOctaves - log2(r.l) - log2(most))), 90.0) : 0.0;
-  const float m = fabs(r.m) < INFINITY ? (float)(r.m - by) : kFloor;
+  const float m = fabs(r.m) < INFINITY ? (float)rint(r.m - by) : kFloor;
   double up = r.m - (double)m;
   if (!(fabs(up - by) <= 32.0)) up = by;
 #pragma unroll
@@ -777,8 +783,7 @@ __device__ __forceinline__ void step_keys(const KvAttn &a, const KvPlan &pl, int
     v4f x = {};
 #pragma unroll
     for (int w = 0; w < kStepWaves; ++w) {
-      const float own = sl[w][q];  // (an infinite one, the mark, stays so)
-      l += own == INFINITY ? own : own * __builtin_amdgcn_exp2f(sm[w][q] - m);
+      l += lowered(sl[w][q], sm[w][q] - m);
       x += *reinterpret_cast<const v4f *>(&part[w][q][d]);
     }
     if (WHOLE) {
@@ -1373,8 +1378,8 @@ __global__ __launch_bounds__(64 * (SHARE > kMergeWaves ? SHARE : kMergeWaves)) v
   auto add = [&](float2 v, const float (&y)[E]) {
     const float mn = fmaxf(m, v.x);
     const float f = __builtin_amdgcn_exp2f(m - mn), h = __builtin_amdgcn_exp2f(v.x - mn);
+    l = lowered(l, m - mn) + lowered(v.y, v.x - mn);
     m = mn;
-    l = l * f + v.y * h;
 #pragma unroll
     for (int e = 0; e < E; ++e) x[e] = x[e] * f + y[e] * h;
   };
@@ -1440,7 +1445,7 @@ __global__ __launch_bounds__(64 * (SHARE > kMergeWaves ? SHARE : kMergeWaves)) v
 #pragma unroll
     for (int w = 0; w < SHARE; ++w) {
       const float f = __builtin_amdgcn_exp2f(sm[w] - mm);
-      ll += sl[w] * f;
+      ll += lowered(sl[w], sm[w] - mm);
       sum += so[w][threadIdx.x] * f;
     }
     a.out[vec * HD + threadIdx.x] = ll != 0.0f ? sum / (ll * kVsUnit) : 0.0f;

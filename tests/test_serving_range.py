@@ -234,3 +234,20 @@ def test_positions_of_zeros_with_the_most_weight(gh, name, ahead, octaves, kind)
         if ln > 60:
             p.scales["k"][p.table[b, (ln - 5) // 16], :, (ln - 5) % 16] = 2.0 * unit
     check(gh, p, q, heads, 1.0, slide, 0.0, shared, step)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", sorted(KINDS))
+@pytest.mark.parametrize("low,high", [(-55, 75), (-100, 100), (-44, 110), (-59, 119)])
+@pytest.mark.parametrize("name", sorted(SHAPES))
+def test_small_values_first(gh, name, low, high, kind):
+    """Scores near zero: the first keys' values are of 2^low, those from some key on of 2^high,
+    beside whose M the sum of the first ones' weights, as large as those of the others, is still
+    to be counted."""
+    _, heads, _, hd, slide, shared, step = SHAPES[name]
+    p, q, _ = cache_of(name, kind, 8)
+    for b, ln in enumerate(p.len):
+        for pos in range(ln):
+            up = pos >= (shared or ln) * 2 // 3
+            p.scales["v"][p.table[b, pos // 16], :, pos % 16] = F32(2.0) ** (high if up else low) / 127
+    check(gh, p, q, heads, hd ** -0.5, 0, 0.0, shared, step)
