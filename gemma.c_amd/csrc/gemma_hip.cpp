@@ -1253,6 +1253,312 @@ size_t gemma_hip_sample_work(int rows, int vocab) {
   return gh::sample_work(rows, vocab);
 }
 
+/* ---- between the products of a served batch --------------------------------- */
+
+}  // extern "C"
+
+namespace {
+
+// A rotation as the kernels take it, for heads of hdim values.
+int rotary_args(const char *name, const gemma_hip_rotary *r, int hdim, gh::Rotary *out) {
+  *out = gh::Rotary{nullptr, 0, 0, 0, 1.0f};
+  if (r == nullptr || r->rot == 0) return 0;
+  if (r->rot < 0 || r->rot % 4 != 0 || r->rot > hdim)
+    return fail("%s: %d turning values of %d (a multiple of 4)", name, r->rot, hdim);
+  if (r->layout != GEMMA_HIP_ROPE_HALF && r->layout != GEMMA_HIP_ROPE_PAIRS)
+    return fail("%s: unknown layout %d", name, r->layout);
+  if (r->freq == nullptr || (uintptr_t)r->freq % 8 != 0)
+    return fail("%s: the frequencies must be there and 8-byte aligned", name);
+  *out = gh::Rotary{r->freq, r->rot, r->layout == GEMMA_HIP_ROPE_PAIRS, r->angle32 != 0,
+                    r->amp == 0.0f ? 1.0f : r->amp};
+  return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int gemma_hip_rotary_freqs(double *freq, float *amp, int rot, double theta, int scaling,
+                           double factor, double original, double low, double high) {
+  const char *name = "gemma_hip_rotary_freqs";
+  if (rot < 4 || rot % 4 != 0 || rot > 65536 || !(theta > 1.0) || std::isinf(theta) ||
+      freq == nullptr)
+    return fail("%s: bad arguments (%d turning values, theta %g)", name, rot, theta);
+  if (scaling < GEMMA_HIP_ROPE_NONE || scaling > GEMMA_HIP_ROPE_YARN)
+    return fail("%s: unknown scaling %d", name, scaling);
+  if (scaling != GEMMA_HIP_ROPE_NONE && !(factor >= 1.0 && factor <= 1e9))
+    return fail("%s: bad factor %g", name, factor);
+  const bool by_turns = scaling == GEMMA_HIP_ROPE_BANDS || scaling == GEMMA_HIP_ROPE_YARN;
+  if (by_turns && !(original >= 1.0 && original <= 1e12 && low > 0.0 && low < high && high <= 1e12))
+    return fail("%s: bad bounds: %g to %g turns in %g positions", name, low, high, original);
+  const double two_pi = 0x1.921fb54442d18p+2;
+  if (scaling == GEMMA_HIP_ROPE_NTK) theta *= pow(factor, rot / (rot - 2.0));
+  const auto pair_of = [&](double turns) {
+    return rot * log(original / (turns * two_pi)) / (2.0 * log(theta));
+  };
+  double from = 0.0, to = 0.0;
+  if (scaling == GEMMA_HIP_ROPE_YARN) {
+    from = std::min(std::max(floor(pair_of(high)), 0.0), rot - 1.0);
+    to = std::min(std::max(ceil(pair_of(low)), 0.0), rot - 1.0);
+  }
+  for (int j = 0; j < rot / 2; ++j) {
+    const double f = pow(theta, -2.0 * j / rot);
+    freq[j] = f;
+    if (scaling == GEMMA_HIP_ROPE_LINEAR) freq[j] = f / factor;
+    if (scaling == GEMMA_HIP_ROPE_BANDS) {
+      const double s = (original * f / two_pi - low) / (high - low);
+      freq[j] = s >= 1.0 ? f : s <= 0.0 ? f / factor : f * ((1.0 - s) / factor + s);
+    }
+    if (scaling == GEMMA_HIP_ROPE_YARN) {
+      const double s = std::min(std::max((j - from) / std::max(to - from, 0.001), 0.0), 1.0);
+      freq[j] = f * (s / factor + 1.0 - s);
+    }
+  }
+  if (amp != nullptr)
+    *amp = scaling == GEMMA_HIP_ROPE_YARN ? (float)(0.1 * log(factor) + 1.0) : 1.0f;
+  return 0;
+}
+
+int gemma_hip_rope(float *dst, int dst_stride, const float *src, int src_stride, int rows,
+                   int heads, int hdim, const int *pos, const float *norm, float eps,
+                   const gemma_hip_rotary *rotary, void *stream) {
+  const char *name = "gemma_hip_rope";
+  if (rows < 0 || heads < 1 || heads > 65536 || hdim < 4 || hdim % 4 != 0 || hdim > 256 ||
+      (long)rows * heads > kKvMostVecs)
+    return fail("%s: unsupported shape: %d rows of %d heads of %d", name, rows, heads, hdim);
+  gh::RopeRows a{};
+  if (rotary_args(name, rotary, hdim, &a.rot)) return 1;
+  const long width = (long)heads * hdim;
+  if (rows > 0 &&
+      (kv_rows(name, src, &src_stride, width) || kv_rows(name, dst, &dst_stride, width)))
+    return 1;
+  if (rows > 0 && (pos == nullptr || !aligned16(norm)))
+    return fail("%s: positions must be there, the norm's weights 16-byte aligned", name);
+  if (need_device(name)) return 1;
+  if (rows == 0) return 0;
+  const gh::Rotary rot = a.rot;
+  a = gh::RopeRows{dst, src, pos, norm, dst_stride, src_stride, rows, heads, hdim, eps, rot};
+  PerfScope perf(kOpRope, pick_stream(stream));
+  GH_CHECK("gemma_hip_rope: launch", gh::launch_rope(a, pick_stream(stream)));
+  return 0;
+}
+
+int gemma_hip_cache_append(const gemma_hip_cache *cache, const gemma_hip_batch *batch,
+                           const gemma_hip_heads *heads, void *stream) {
+  const char *name = "gemma_hip_cache_append";
+  gh::KvAppend a{};
+  if (heads == nullptr) return fail("%s: null pointer", name);
+  if (kv_args(name, cache, batch, &a.c, &a.b) ||
+      rotary_args(name, &heads->rotary, a.c.hdim, &a.rot))
+    return 1;
+  const bool queries = heads->q != nullptr || heads->q_out != nullptr;
+  const int nq = queries ? heads->n_heads : 0;
+  if (queries && (nq < 1 || nq > 1024))
+    return fail("%s: unsupported number of heads: %d", name, nq);
+  if ((long)a.b.rows * (nq + 2 * a.c.nkv) > 2 * kKvMostVecs)
+    return fail("%s: too many rows: %d of %d heads", name, a.b.rows, nq + 2 * a.c.nkv);
+  int qs = heads->q_stride, os = heads->q_out_stride, ks = heads->k_stride, vs = heads->v_stride;
+  const bool any = a.b.batch > 0 && a.b.max_rows > 0;
+  const long width = (long)a.c.nkv * a.c.hdim, q_width = (long)nq * a.c.hdim;
+  if (any && (kv_pointers(name, a.c, a.b) || kv_rows(name, heads->k, &ks, width) ||
+              kv_rows(name, heads->v, &vs, width)))
+    return 1;
+  if (any && queries &&
+      (kv_rows(name, heads->q, &qs, q_width) || kv_rows(name, heads->q_out, &os, q_width)))
+    return 1;
+  if (!aligned16(heads->nq) || !aligned16(heads->nk))
+    return fail("%s: the norms' weights must be 16-byte aligned", name);
+  if (need_device(name)) return 1;
+  if (!any) return 0;
+  a.q = heads->q, a.k = heads->k, a.v = heads->v, a.q_out = heads->q_out;
+  a.q_stride = qs, a.k_stride = ks, a.v_stride = vs, a.out_stride = os;
+  a.n_heads = nq, a.nq = heads->nq, a.nk = heads->nk, a.eps = heads->eps;
+  PerfScope perf(kOpRope, pick_stream(stream));
+  GH_CHECK("gemma_hip_cache_append: launch", gh::launch_kv_append(a, pick_stream(stream)));
+  return 0;
+}
+
+}  // extern "C"
+
+namespace {
+
+int norm_args(const char *name, const gemma_hip_norm &n, gh::NormOf *out) {
+  if (n.kind < GEMMA_HIP_NORM_NONE || n.kind > GEMMA_HIP_NORM_LAYER)
+    return fail("%s: unknown norm %d", name, n.kind);
+  if (!aligned16(n.w) || !aligned16(n.b))
+    return fail("%s: a norm's weights must be 16-byte aligned", name);
+  *out = gh::NormOf{n.kind, n.w, n.b, n.offset, n.eps};
+  return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int gemma_hip_norm_residual(const gemma_hip_residual *residual, int rows, int dim, void *stream) {
+  const char *name = "gemma_hip_norm_residual";
+  if (residual == nullptr) return fail("%s: null pointer", name);
+  gemma_hip_residual v = *residual;
+  if (rows < 0 || dim < 4 || dim % 4 != 0 || dim > gh::kNormMaxDim)
+    return fail("%s: unsupported shape: %d rows of %d", name, rows, dim);
+  gh::NormResidual a{};
+  if (norm_args(name, v.after, &a.after) || norm_args(name, v.before, &a.before)) return 1;
+  if ((v.hq == nullptr) != (v.hs == nullptr))
+    return fail("%s: codes and their scales go together", name);
+  if (rows > 0) {
+    if (kv_rows(name, v.x, &v.x_stride, dim)) return 1;
+    if (v.y != nullptr && kv_rows(name, v.y, &v.y_stride, dim)) return 1;
+    if (v.gate != nullptr && kv_rows(name, v.gate, &v.gate_stride, dim)) return 1;
+    if (v.x_out != nullptr && kv_rows(name, v.x_out, &v.x_out_stride, dim)) return 1;
+    if (v.h != nullptr && kv_rows(name, v.h, &v.h_stride, dim)) return 1;
+    if (v.hq_stride == 0) v.hq_stride = dim;
+    if (v.hq != nullptr && (v.hq_stride < dim || v.hq_stride % 4 != 0 || (uintptr_t)v.hq % 4 != 0))
+      return fail("%s: codes need a stride of at least %d and a multiple of 4, 4-byte aligned",
+                  name, dim);
+  }
+  if (need_device(name)) return 1;
+  if (rows == 0) return 0;
+  a.x = v.x, a.y = v.y, a.gate = v.gate;
+  a.x_stride = v.x_stride, a.y_stride = v.y_stride, a.out_stride = v.x_out_stride;
+  a.gate_stride = v.gate_one ? 0 : v.gate_stride;
+  a.h_stride = v.h_stride, a.hq_stride = v.hq_stride;
+  a.cx = v.x_scale, a.cy = v.y_scale;
+  a.x_out = v.x_out, a.h = v.h, a.hq = v.hq, a.hs = v.hs;
+  a.rows = rows, a.dim = dim;
+  const bool layer = v.before.kind == GEMMA_HIP_NORM_LAYER || v.after.kind == GEMMA_HIP_NORM_LAYER;
+  PerfScope perf(layer ? kOpLayernorm : kOpRmsnorm, pick_stream(stream));
+  GH_CHECK("gemma_hip_norm_residual: launch", gh::launch_norm_residual(a, pick_stream(stream)));
+  return 0;
+}
+
+}  // extern "C"
+
+namespace {
+
+// Rows times columns, or times values of u, of a call of the adapters', at most.
+constexpr long kAdapterMostRows = 1l << 22;
+
+int adapter_args(const char *name, const gemma_hip_adapters *ad, int njobs, int k) {
+  if (ad == nullptr) return fail("%s: null pointer", name);
+  if (njobs < 1 || njobs > gh::kAdapterMaxJobs || k < 8 || k % 8 != 0 || k > (1 << 20))
+    return fail("%s: unsupported shape: %d projections of %d inputs (a multiple of 8)", name,
+                njobs, k);
+  if (ad->rank < 8 || ad->rank % 8 != 0 || ad->rank > gh::kAdapterMaxRank)
+    return fail("%s: unsupported rank %d (a multiple of 8 up to %d)", name, ad->rank,
+                gh::kAdapterMaxRank);
+  if (ad->type < GEMMA_HIP_ADAPTER_F32 || ad->type > GEMMA_HIP_ADAPTER_F16)
+    return fail("%s: unknown type %d", name, ad->type);
+  if (ad->batch < 0 || ad->batch > 65535 || ad->rows < 0 || ad->rows > kAdapterMostRows ||
+      ad->max_rows < 0 || ad->max_rows > ad->rows || ad->count < 0)
+    return fail("%s: bad batch: %d sequences, %d rows (%d at most), %d adapters", name, ad->batch,
+                ad->rows, ad->max_rows, ad->count);
+  return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int gemma_hip_adapters_add(float *dst, int dstr, const float *base, int bstr,
+                           const gemma_hip_adapters *adapters, const gemma_hip_adapter_job *jobs,
+                           int njobs, const float *src, int sstr, int k, void *work,
+                           size_t work_bytes, void *stream) {
+  const char *name = "gemma_hip_adapters_add";
+  if (adapter_args(name, adapters, njobs, k)) return 1;
+  if (jobs == nullptr) return fail("%s: null pointer", name);
+  gh::Adapters a{};
+  long n = 0;
+  for (int j = 0; j < njobs; ++j) {
+    if (jobs[j].n < 1 || jobs[j].n > (1 << 20))
+      return fail("%s: unsupported shape: %d outputs", name, jobs[j].n);
+    if (adapters->count > 0 && (!jobs[j].a || !jobs[j].b)) return fail("%s: null pointer", name);
+    if (!aligned16(jobs[j].a) || !aligned16(jobs[j].b))
+      return fail("%s: the matrices must be 16-byte aligned", name);
+    n += jobs[j].n;
+    a.a[j] = jobs[j].a, a.b[j] = jobs[j].b, a.end[j] = (int)n;
+  }
+  const bool any = adapters->batch > 0 && adapters->max_rows > 0;
+  if (any && (!adapters->row0 || !adapters->ids || !dst || !base))
+    return fail("%s: null pointer", name);
+  if (dstr == 0) dstr = (int)n;
+  if (bstr == 0) bstr = (int)n;
+  if (dstr < n || bstr < n)
+    return fail("%s: strides %d and %d smaller than a row of %ld", name, dstr, bstr, n);
+  if (any && kv_rows(name, src, &sstr, k)) return 1;
+  if (need_device(name)) return 1;
+  if (!any) return 0;
+  a.dst = dst, a.base = base, a.src = src;
+  a.dst_stride = dstr, a.base_stride = bstr, a.src_stride = sstr;
+  a.njobs = njobs, a.k = k, a.rank = adapters->rank, a.count = adapters->count;
+  a.type = adapters->type, a.ids = adapters->ids, a.scale = adapters->scale;
+  a.seq = gh::KvBatch{nullptr, nullptr, adapters->row0, adapters->batch, 0, adapters->rows,
+                      adapters->max_rows, 0};
+  hipStream_t s = pick_stream(stream);
+  std::optional<AttnHold> hold;
+  if (call_workspace(name, gh::adapters_work(adapters->rows, njobs, adapters->rank), work,
+                     work_bytes, s, &hold, &a.work))
+    return 1;
+  {
+    PerfScope perf(adapters->max_rows > 1 ? kOpGemmFpx : kOpGemvFpx, s);
+    GH_CHECK("gemma_hip_adapters_add: launch", gh::launch_adapters(a, g.info, s));
+  }
+  if (hold) GH_CHECK("gemma_hip_adapters_add", hold->done());
+  return 0;
+}
+
+size_t gemma_hip_adapters_work(const gemma_hip_adapters *adapters, int njobs, int k) {
+  if (adapter_args("gemma_hip_adapters_work", adapters, njobs, k)) return (size_t)-1;
+  return gh::adapters_work(adapters->rows, njobs, adapters->rank);
+}
+
+}  // extern "C"
+
+namespace {
+int logprobs_args(const char *name, int rows, int vocab, int targets, int ntop) {
+  if (rows < 0 || rows > 65535 || vocab < 1 || vocab > gh::kSampleMaxVocab)
+    return fail("%s: unsupported shape: %d rows of %d (at most 65535 of %d)", name, rows, vocab,
+                gh::kSampleMaxVocab);
+  if (targets < 0 || targets > gh::kLogprobsMaxTargets || ntop < 0 ||
+      ntop > gh::kLogprobsMaxTop)
+    return fail("%s: %d given tokens and %d likeliest ones (at most %d and %d)", name, targets,
+                ntop, gh::kLogprobsMaxTargets, gh::kLogprobsMaxTop);
+  return 0;
+}
+}  // namespace
+
+extern "C" {
+
+int gemma_hip_logprobs(const gemma_hip_scores *scores, const float *logits, int stride, int rows,
+                       int vocab, const float *temperature, const int *ids, int targets, int ntop,
+                       void *work, size_t work_bytes, void *stream) {
+  const char *name = "gemma_hip_logprobs";
+  if (scores == nullptr) return fail("%s: null pointer", name);
+  if (logprobs_args(name, rows, vocab, targets, ntop)) return 1;
+  if (rows > 0 && (!logits || (targets > 0 && !ids))) return fail("%s: null pointer", name);
+  if (stride == 0) stride = vocab;
+  if (stride < vocab) return fail("%s: stride %d smaller than a row of %d", name, stride, vocab);
+  if (need_device(name)) return 1;
+  if (rows == 0) return 0;
+  gh::Logprobs a{scores->logp, scores->rank, scores->entropy, scores->top, scores->top_logp,
+                 logits, (size_t)stride, rows, vocab, temperature, ids, targets, ntop, nullptr};
+  hipStream_t s = pick_stream(stream);
+  std::optional<AttnHold> hold;
+  if (call_workspace(name, gh::logprobs_work(rows, vocab, targets, ntop), work, work_bytes, s,
+                     &hold, &a.work))
+    return 1;
+  {
+    PerfScope perf(kOpSample, s);
+    GH_CHECK("gemma_hip_logprobs: launch", gh::launch_logprobs(a, s));
+  }
+  if (hold) GH_CHECK("gemma_hip_logprobs", hold->done());
+  return 0;
+}
+
+size_t gemma_hip_logprobs_work(int rows, int vocab, int targets, int ntop) {
+  if (logprobs_args("gemma_hip_logprobs_work", rows, vocab, targets, ntop)) return (size_t)-1;
+  return gh::logprobs_work(rows, vocab, targets, ntop);
+}
+
 /* ---- host drop-ins ------------------------------------------------------ */
 
 // Inputs up to this size are read by the kernels straight from pinned host

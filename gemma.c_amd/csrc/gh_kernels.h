@@ -421,6 +421,101 @@ struct KvAttn {
 size_t kv_attention_work(const KvAttn &a, const DeviceInfo &dev);
 hipError_t launch_kv_attention(const KvAttn &a, const DeviceInfo &dev, hipStream_t stream);
 
+// rope.hip: heads by their positions.  freq [rot / 2] radians a position (null: none turn), pairs
+// (j, j + rot/2) or, with `pairs`, (2j, 2j + 1); angle32: the angle, its cosine and sine rounded
+// to fp32 first
+struct Rotary {
+  const double *freq;
+  int rot, pairs, angle32;
+  float amp;
+};
+// dst row r, head h = src's through the norm of weights w + 1 (null: none) and the turn
+struct RopeRows {
+  float *dst;
+  const float *src;
+  const int *pos;
+  const float *w;
+  long dst_stride, src_stride;
+  int rows, heads, hdim;
+  float eps;
+  Rotary rot;
+};
+hipError_t launch_rope(const RopeRows &a, hipStream_t stream);
+// the batch's new rows of q into q_out, of k and v into the cache, q by the norm of nq and the
+// turn, k by those of nk; q may be null
+struct KvAppend {
+  const float *q, *k, *v;
+  float *q_out;
+  long q_stride, k_stride, v_stride, out_stride;
+  int n_heads;
+  const float *nq, *nk;
+  float eps;
+  Rotary rot;
+  KvCache c;
+  KvBatch b;
+};
+hipError_t launch_kv_append(const KvAppend &a, hipStream_t stream);
+
+// norm.hip: per row x' = clamp(cx x + cy gate after(y)), h = before(x') as fp32 and, when hq is
+// given, as codes.  A norm's kind: 0 none, 1 by the root of the mean square, 2 with the mean taken
+// off; weights (null: 1) w + offset, b (null: 0) added.  y, gate, x_out and h may be null.
+struct NormOf {
+  int kind;
+  const float *w, *b;
+  float offset, eps;
+};
+struct NormResidual {
+  const float *x, *y, *gate;
+  long x_stride, y_stride, gate_stride, out_stride, h_stride, hq_stride;
+  float cx, cy;
+  NormOf after, before;
+  float *x_out, *h;
+  int8_t *hq;
+  float *hs;
+  int rows, dim;
+};
+constexpr int kNormMaxDim = 24576;
+hipError_t launch_norm_residual(const NormResidual &a, hipStream_t stream);
+
+// adapters.hip: dst row = base row + scale[id] B[id] (A[id] src row), id that of the row's
+// sequence; rows whose id is none of 0 .. count - 1 are base.  Job j: a [count][rank][k],
+// b [count][n][rank], columns behind the jobs' before it.
+constexpr int kAdapterF32 = 0, kAdapterBf16 = 1, kAdapterF16 = 2;  // GEMMA_HIP_ADAPTER_*
+constexpr int kAdapterMaxJobs = 3, kAdapterMaxRank = 128;
+struct Adapters {
+  float *dst;
+  const float *base, *src;
+  long dst_stride, base_stride, src_stride;
+  const void *a[kAdapterMaxJobs], *b[kAdapterMaxJobs];
+  int end[kAdapterMaxJobs];  // a job's columns end here
+  int njobs, k, rank, count, type;
+  const int *ids;
+  const float *scale;
+  KvBatch seq;  // without pages and lengths
+  char *work;
+};
+size_t adapters_work(int rows, int njobs, int rank);
+hipError_t launch_adapters(const Adapters &a, const DeviceInfo &dev, hipStream_t stream);
+
+// logprobs.hip: what logits say of given tokens, and the likeliest ones.
+constexpr int kLogprobsMaxTop = 64, kLogprobsMaxTargets = 64;
+struct Logprobs {
+  float *logp;      // [rows][targets]
+  int *rank;        // [rows][targets]
+  float *entropy;   // [rows]
+  int *top;         // [rows][ntop]
+  float *top_logp;  // [rows][ntop]; each of the five may be null
+  const float *logits;
+  size_t stride;
+  int rows, vocab;
+  const float *temperature;  // [rows] or null
+  const int *ids;            // [rows][targets]
+  int targets, ntop;
+  char *work;
+};
+size_t logprobs_work(int rows, int vocab, int targets, int ntop);
+hipError_t launch_logprobs(const Logprobs &a, hipStream_t stream);
+
 // sample.hip: one token per row of logits.  Settings are device arrays of a value
 // per row, or null.
 constexpr int kSampleMaxVocab = 1 << 19;

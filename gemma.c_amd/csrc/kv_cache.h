@@ -102,6 +102,38 @@ __device__ __forceinline__ int kv_find_wave(const KvBatch &b, int r) {
 }
 #endif
 
+#ifdef __HIPCC__
+// Where row r lies: sequence i, its position (rows behind their sequences' starts have negative
+// ones); i -1: in none.  By a whole wave, for one row: one load for up to 63 sequences, two for
+// up to 3969 and so on, their lengths' among them.
+struct KvRow {
+  int i, pos;
+};
+template <bool POS>
+__device__ __forceinline__ KvRow kv_row_wave(const KvBatch &b, int r) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, n = b.batch;  // it is one of lo .. lo + n - 1
+  while (n > 63) {
+    const int step = (n + 62) / 63, at = lane * step;
+    const int before = __popcll(__ballot(at < n && b.row0[lo + (at < n ? at : 0)] <= r));
+    const int skip = (before > 0 ? before - 1 : 0) * step;
+    lo += skip;
+    n = n - skip < step ? n - skip : step;
+  }
+  const int at = lo + (lane < n ? lane : n);  // row0[lo + n] is there too
+  const int first = b.row0[at];
+  const int len = POS ? b.len[at < b.batch ? at : b.batch - 1] : 0;
+  const int before = __popcll(__ballot(lane < n && first <= r));
+  const int j = before > 0 ? before - 1 : 0;
+  const int r0 = kv_clamp(__builtin_amdgcn_readlane(first, j), 0, b.rows);
+  int rows = kv_clamp(__builtin_amdgcn_readlane(first, j + 1), r0, b.rows) - r0;
+  if (rows > b.max_rows) rows = b.max_rows;
+  const bool in = r >= r0 && r - r0 < rows;
+  const int ln = POS ? kv_clamp(__builtin_amdgcn_readlane(len, j), 0, b.max_len) : 0;
+  return KvRow{in ? lo + j : -1, ln - rows + (r - r0)};
+}
+#endif
+
 // Keys that a row at position pos sees: lo .. hi (hi < lo: none).
 struct KvSpan {
   int lo, hi;

@@ -1,0 +1,315 @@
+// logprobs.hip -- what rows of logits say: log probabilities and ranks of given tokens, the
+// entropy, and the likeliest tokens.
+//
+// Let z = l log2(e) / temperature.  With any reference m, S = sum 2^(z - m), T = sum (z - m)
+// 2^(z - m): log2 p = z - m - log2 S, and the entropy is log2 S - T / S octaves; sums by
+// different references join when one is moved to the other's.  A token's rank is 1 and the
+// count of those above it.  The n likeliest lie in the n runs of 64 columns with the largest
+// largest logits (equals by index): a token of another run has n above it.
+//
+// So one reading does: a wave takes 2048 columns, 32 a lane in registers, and leaves S and T by
+// its own largest logit (fp32, the exponents' errors below 2^-22), the given tokens' counts and its 32
+// runs' largest logits.  A second launch joins a row's (fp64) and looks into the n runs that
+// matter.
+#include <float.h>
+#include <type_traits>
+
+#include "dec_common.h"
+#include "gh_arith.h"
+#include "gh_kernels.h"
+
+namespace gh {
+namespace {
+
+typedef unsigned long long u64;
+
+constexpr int kRun = 64;                  // columns of a run
+constexpr int kLoads = 8;                 // 256 columns each
+constexpr int kTile = 256 * kLoads;       // columns of a wave
+constexpr int kTileRuns = kTile / kRun;
+constexpr int kThreads = 256;
+constexpr int kMaxTiles = (kSampleMaxVocab + kTile - 1) / kTile;
+constexpr int kMost = kMaxTiles * kTileRuns;  // runs of a row
+constexpr float kFar = -160.0f;  // octaves; a weight there is 0 in fp32
+
+// rows of logits may begin anywhere
+typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));
+
+// What a wave leaves: its largest logit, S and T by it.
+struct Part {
+  float m, s, t;
+};
+
+// A row's parts, runs and counts in the workspace.
+struct Layout {
+  size_t parts, runs, counts, all;
+};
+__host__ __device__ inline int tiles_of(int vocab) { return (vocab + kTile - 1) / kTile; }
+__host__ __device__ inline Layout layout_of(int rows, int vocab, int targets, int ntop) {
+  const size_t tiles = (size_t)rows * tiles_of(vocab);
+  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  Layout l;
+  l.parts = 0;
+  l.runs = up(tiles * sizeof(Part));
+  l.counts = l.runs + (ntop > 0 ? up(tiles * kTileRuns * 4) : 0);
+  l.all = l.counts + up(tiles * targets * 4);
+  return l;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float no_nan(float l) { return fmaxf(l, -INFINITY); }
+
+// log2(e) / temperature; 0 where the temperature is 0 or none: all on the largest
+__device__ __forceinline__ float octaves_of(const float *temperature, int r) {
+  const float t = temperature != nullptr ? temperature[r] : 1.0f;
+  return t > 0.0f ? (float)fmin(0x1.71547652b82fep+0 / (double)t, (double)FLT_MAX) : 0.0f;
+}
+
+// The least float above l (l not NaN); of +inf: NaN, which nothing reaches.
+__device__ __forceinline__ float next_up(float l) {
+  if (l == 0.0f) return __int_as_float(1);
+  const int b = __float_as_int(l);
+  return __int_as_float(b > 0 ? b + 1 : b - 1);
+}
+
+template <bool TOP>
+__global__ __launch_bounds__(kThreads) void logprobs_scan_kernel(Logprobs a, Layout at) {
+  const int lane = threadIdx.x & 63, tiles = tiles_of(a.vocab);
+  const long unit = (long)blockIdx.x * (kThreads / 64) +
+                    __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int r = (int)(unit / tiles), tile = (int)(unit % tiles), c0 = tile * kTile;
+  if (r >= a.rows) return;
+  const float *row = a.logits + r * a.stride;
+  float l[kLoads][4];
+  if (c0 + kTile <= a.vocab) {
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const v4f_any v = *reinterpret_cast<const v4f_any *>(row + c0 + 256 * j + 4 * lane);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) l[j][e] = v[e];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int c = c0 + 256 * j + 4 * lane + e;
+        l[j][e] = c < a.vocab ? row[c] : -INFINITY;
+      }
+  }
+  const float c = octaves_of(a.temperature, r);
+  float m = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < kLoads; ++j) {
+    float top = fmaxf(fmaxf(no_nan(l[j][0]), l[j][1]), fmaxf(no_nan(l[j][2]), l[j][3]));
+    m = fmaxf(m, top);
+    if (TOP) {  // 16 lanes' columns are a run
+      top = fmaxf(top, dpp_f32<kDppXor1>(top));
+      top = fmaxf(top, dpp_f32<kDppXor2>(top));
+      top = fmaxf(top, dpp_f32<kDppHalfMirror>(top));
+      top = fmaxf(top, dpp_f32<kDppMirror>(top));
+      if ((lane & 15) == 0)
+        reinterpret_cast<float *>(a.work + at.runs)[unit * kTileRuns + 4 * j + lane / 16] = top;
+    }
+  }
+  // S and T of a lane by its largest, then of the wave by the wave's
+  float s = 0.0f, t = 0.0f;
+#pragma unroll
+  for (int j = 0; j < kLoads; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float x = fmaxf((l[j][e] - m) * c, kFar);  // NaN and -inf are far off
+      const float w = exp2_fast(x);
+      s += w;
+      t = fmaf(w, x, t);
+    }
+  const float top = wave_max_dpp(m);
+  if (top == INFINITY) {  // infinite logits share everything
+    s = t = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s += l[j][e] == INFINITY ? 1.0f : 0.0f;
+  } else {
+    const float x = fmaxf((m - top) * c, kFar);
+    const float w = exp2_fast(x);
+    t = w * fmaf(s, x, t);
+    s = w * s;
+  }
+  s = group_sum_f32<64>(s);
+  t = group_sum_f32<64>(t);
+  if (lane == 0) reinterpret_cast<Part *>(a.work + at.parts)[unit] = Part{top, s, t};
+  for (int k = 0; k < a.targets; ++k) {
+    const int id = a.ids[(size_t)r * a.targets + k];
+    int above = 0;
+    if ((unsigned)id < (unsigned)a.vocab) {
+      const float mine = no_nan(row[id]), more = next_up(mine);
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        const int first = c0 + 256 * j;
+        if (id < first || id >= first + 256) {
+          const float least = id < first ? more : mine;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) above += __popcll(__ballot(no_nan(l[j][e]) >= least));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            above += __popcll(
+                __ballot(no_nan(l[j][e]) >= (first + 4 * lane + e < id ? mine : more)));
+        }
+      }
+    }
+    if (lane == 0) reinterpret_cast<int *>(a.work + at.counts)[unit * a.targets + k] = above;
+  }
+}
+
+// Tokens and runs in the order of falling logit, then rising index, as falling whole numbers;
+// 0: none.
+__device__ __forceinline__ u64 key_of(float l, int index) {
+  if (!(l > -INFINITY)) return 0;
+  const uint32_t b = l == 0.0f ? 0u : __float_as_uint(l);
+  const uint32_t up = b & 0x80000000u ? ~b : b | 0x80000000u;
+  return (u64)up << 32 | (uint32_t)~index;
+}
+__device__ __forceinline__ int index_of(u64 key) { return (int)~(uint32_t)key; }
+__device__ __forceinline__ float logit_of(u64 key) {
+  const uint32_t up = (uint32_t)(key >> 32);
+  return __uint_as_float(up & 0x80000000u ? up & 0x7fffffffu : ~up);
+}
+
+constexpr int kKeys = kMost / kThreads;  // of a thread, at most
+struct TopShared {
+  u64 most[kThreads];
+  u64 list[kKeys * kLogprobsMaxTop];
+  u64 best[kLogprobsMaxTop];
+  int count;
+};
+
+// The n largest of the threads' keys (no two alike but 0), in order, 0 where there are fewer,
+// into sh.best: threads' largest are ranked, those that reach the n-th of them are listed, and
+// the list is ranked.  A thread that reaches it has `per` keys at most, and n threads do.
+template <class K>
+__device__ void top_of(TopShared &sh, int n, int per, K &&key) {
+  const int tid = threadIdx.x;
+  u64 most = 0;
+  for (int j = 0; j < per; ++j) most = max(most, key(j));
+  __syncthreads();
+  sh.most[tid] = most;
+  if (tid < n) sh.best[tid] = 0;
+  if (tid == 0) sh.count = 0;
+  __syncthreads();
+  int above = 0;
+  for (int j = 0; j < kThreads; ++j) above += sh.most[j] > most;
+  if (most != 0 && above < n)
+    for (int j = 0; j < per; ++j) {
+      const u64 k = key(j);
+      if (k != 0) sh.list[atomicAdd(&sh.count, 1)] = k;
+    }
+  __syncthreads();
+  const int count = sh.count;
+  for (int i = tid; i < count; i += kThreads) {
+    const u64 mine = sh.list[i];
+    int rank = 0;
+    for (int j = 0; j < count; ++j) rank += sh.list[j] > mine;
+    if (rank < n) sh.best[rank] = mine;
+  }
+  __syncthreads();
+}
+
+__global__ __launch_bounds__(kThreads) void logprobs_join_kernel(Logprobs a, Layout at) {
+  __shared__ TopShared sh;
+  __shared__ double red[kThreads / 64];
+  __shared__ float redf[kThreads / 64];
+  const int r = blockIdx.x, tid = threadIdx.x, tiles = tiles_of(a.vocab);
+  const float *row = a.logits + r * a.stride;
+  const Part *parts = reinterpret_cast<const Part *>(a.work + at.parts) + (size_t)r * tiles;
+  const float temp = a.temperature != nullptr ? a.temperature[r] : 1.0f;
+  const bool drawn = temp > 0.0f;
+  const double c = drawn ? fmin(0x1.71547652b82fep+0 / (double)temp, (double)FLT_MAX) : 0.0;
+  const bool in = tid < tiles;  // one part a thread
+  static_assert(kMaxTiles <= kThreads, "a thread a part");
+  const Part p = in ? parts[tid] : Part{-INFINITY, 0.0f, 0.0f};
+  const float top = block_max<kThreads>(p.m, redf);
+  double s = 0.0, t = 0.0;
+  if (p.m > -INFINITY) {
+    const double x = top == p.m ? 0.0 : ((double)p.m - (double)top) * c;  // (-inf below +inf)
+    const double w = x > -1000.0 ? exp2(x) : 0.0;
+    s = w * (double)p.s;
+    t = w > 0.0 ? w * ((double)p.t + (double)p.s * x) : 0.0;
+  }
+  s = block_sum<kThreads>(s, red);
+  t = block_sum<kThreads>(t, red);
+  const double ln2 = 0x1.62e42fefa39efp-1, logs = log(s);
+  // log p of a logit that isn't NaN; first: whether it is the row's first largest
+  auto logp = [&](float l, bool first) -> float {
+    if (!(l > -INFINITY)) return -INFINITY;
+    if (!drawn) return first ? 0.0f : -INFINITY;
+    if (l == top) return (float)(0.0 - logs);
+    return (float)(((double)l - (double)top) / (double)temp - logs);
+  };
+  if (tid == 0 && a.entropy != nullptr)
+    a.entropy[r] = drawn && top > -INFINITY ? (float)fmax(0.0, logs - ln2 * t / s) : 0.0f;
+  const int *counts = reinterpret_cast<const int *>(a.work + at.counts) +
+                      (size_t)r * tiles * a.targets;
+  for (int k = tid / 64; k < a.targets; k += kThreads / 64) {  // a wave a token
+    int above = 0;
+    for (int j = tid & 63; j < tiles; j += 64) above += counts[(size_t)j * a.targets + k];
+    above = group_sum_i32<64>(above);
+    if ((tid & 63) != 0) continue;
+    const size_t to = (size_t)r * a.targets + k;
+    const int id = a.ids[to];
+    const bool there = (unsigned)id < (unsigned)a.vocab;
+    if (a.rank != nullptr) a.rank[to] = there ? above + 1 : 0;
+    if (a.logp != nullptr) a.logp[to] = there ? logp(no_nan(row[id]), above == 0) : -INFINITY;
+  }
+  if (a.ntop == 0) return;
+  const float *runs = reinterpret_cast<const float *>(a.work + at.runs) +
+                      (size_t)r * tiles * kTileRuns;
+  const int nruns = (a.vocab + kRun - 1) / kRun;
+  top_of(sh, a.ntop, (nruns + kThreads - 1) / kThreads, [&](int j) -> u64 {
+    const int i = tid + j * kThreads;
+    return i < nruns ? key_of(runs[i], i) : 0;
+  });
+  // a wave a run: its columns in their threads' keys
+  u64 mine[kLogprobsMaxTop / (kThreads / 64)];
+  const int per = (a.ntop + kThreads / 64 - 1) / (kThreads / 64);
+#pragma unroll
+  for (int j = 0; j < kLogprobsMaxTop / (kThreads / 64); ++j) {
+    mine[j] = 0;
+    const int i = j * (kThreads / 64) + tid / 64;
+    if (i >= a.ntop || sh.best[i] == 0) continue;
+    const int col = index_of(sh.best[i]) * kRun + (tid & 63);
+    if (col < a.vocab) mine[j] = key_of(row[col], col);
+  }
+  top_of(sh, a.ntop, per, [&](int j) -> u64 {
+    u64 k = 0;
+#pragma unroll
+    for (int i = 0; i < kLogprobsMaxTop / (kThreads / 64); ++i) k = i == j ? mine[i] : k;
+    return k;
+  });
+  if (tid < a.ntop) {
+    const u64 k = sh.best[tid];
+    const size_t to = (size_t)r * a.ntop + tid;
+    if (a.top != nullptr) a.top[to] = k != 0 ? index_of(k) : -1;
+    if (a.top_logp != nullptr)
+      a.top_logp[to] = k != 0 ? logp(logit_of(k), tid == 0) : -INFINITY;
+  }
+}
+
+}  // namespace
+
+size_t logprobs_work(int rows, int vocab, int targets, int ntop) {
+  return layout_of(rows, vocab, targets, ntop).all;
+}
+
+hipError_t launch_logprobs(const Logprobs &a, hipStream_t stream) {
+  const Layout at = layout_of(a.rows, a.vocab, a.targets, a.ntop);
+  const long units = (long)a.rows * tiles_of(a.vocab);
+  const unsigned grid = (unsigned)((units + 3) / 4);
+  a.ntop > 0 ? logprobs_scan_kernel<true><<<grid, kThreads, 0, stream>>>(a, at)
+             : logprobs_scan_kernel<false><<<grid, kThreads, 0, stream>>>(a, at);
+  logprobs_join_kernel<<<a.rows, kThreads, 0, stream>>>(a, at);
+  return hipGetLastError();
+}
+
+}  // namespace gh

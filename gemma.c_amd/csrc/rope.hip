@@ -1,0 +1,345 @@
+// rope.hip -- rotary positions, by themselves and on the way into the paged cache.
+//
+// Pair j of a head's first `rot` values (x, y) becomes (x c - y s, y c + x s), c and s amp times
+// the cosine and sine of pos f_j; the others stay.  Before that comes, if asked for, the head's
+// norm x / sqrt(mean x^2 + eps) (w + 1).  Both in fp64, rounded to fp32 once: a far position's
+// angle needs more than fp32, and the keys' codes that follow are then the exact ones but where
+// a border between two codes is hit to 1e-15 (an fp32 rounding in between moves one in 10^5).
+//
+// A head is hdim / 4 lanes' (16, 32 or 64 of them), four values a lane: pairs 2l and 2l + 1 of
+// lane l, then what doesn't turn.  A lane's two angles are those of every head of its row.
+#include <type_traits>
+
+#include "dec_common.h"
+#include "gh_arith.h"
+#include "gh_kernels.h"
+
+namespace gh {
+namespace {
+
+constexpr int kThreads = 256;
+
+typedef float v2f __attribute__((ext_vector_type(2)));
+
+// Sum and largest over each aligned group of G lanes, the same in all of them.
+template <int G>
+__device__ __forceinline__ double group_sum_f64(double v) {
+  if (G == 64) return wave_sum_f64(v);
+  v += dpp_f64<kDppXor1>(v);
+  v += dpp_f64<kDppXor2>(v);
+  v += dpp_f64<kDppHalfMirror>(v);
+  v += dpp_f64<kDppMirror>(v);
+  if (G == 32) v += __shfl_xor(v, 16, 64);
+  return v;
+}
+template <int G>
+__device__ __forceinline__ int group_max_i32(int v) {
+#pragma unroll
+  for (int off = G / 2; off > 0; off >>= 1) v = max(v, __shfl_xor(v, off, 64));
+  return v;
+}
+
+// 1 / sqrt(v) for v > 0: the instruction's approximation and a step of third order
+__device__ __forceinline__ double rsqrt_f64(double v) {
+  const double y = __builtin_amdgcn_rsq(v);
+  const double e = fma(-v * y, y, 1.0);
+  return v < INFINITY ? fma(y * e, fma(e, 0.375, 0.5), y) : y;
+}
+
+// Cosine and sine of an angle of up to some 2^40, to fp64 rounding: the nearest multiple of pi/2
+// taken off (in two parts), Taylor polynomials of degree 15 and 16 on what is left, at most pi/4
+// (the terms left out are below 7e-17).
+__device__ __forceinline__ void cos_sin(double angle, double *c, double *s) {
+  const double shift = fma(angle, 0x1.45f306dc9c883p-1, 0x1.8p52);  // 2 / pi
+  const double k = shift - 0x1.8p52;
+  double r = fma(-k, 0x1.921fb54442d18p0, angle);
+  r = fma(-k, 0x1.1a62633145c07p-54, r);
+  const double z = r * r;
+  double p = fma(z, -1.0 / 1307674368000.0, 1.0 / 6227020800.0);
+  p = fma(z, p, -1.0 / 39916800.0);
+  p = fma(z, p, 1.0 / 362880.0);
+  p = fma(z, p, -1.0 / 5040.0);
+  p = fma(z, p, 1.0 / 120.0);
+  p = fma(z, p, -1.0 / 6.0);
+  const double sine = fma(r * z, p, r);
+  double q = fma(z, 1.0 / 20922789888000.0, -1.0 / 87178291200.0);
+  q = fma(z, q, 1.0 / 479001600.0);
+  q = fma(z, q, -1.0 / 3628800.0);
+  q = fma(z, q, 1.0 / 40320.0);
+  q = fma(z, q, -1.0 / 720.0);
+  q = fma(z, q, 1.0 / 24.0);
+  q = fma(z, q, -0.5);
+  const double cosine = fma(z, q, 1.0);
+  const int turn = (int)__double_as_longlong(shift) & 3;
+  const double a = turn & 1 ? sine : cosine, b = turn & 1 ? cosine : sine;
+  *c = turn == 1 || turn == 2 ? -a : a;
+  *s = turn & 2 ? -b : b;
+}
+
+// Where a lane's four values lie in its head: two and two neighbours at `a` and `b`, or, with
+// PAIRS, four from `a`; turns: they are pairs f and f + 1.
+struct Place {
+  int a, b, f;
+  bool there, turns;
+};
+template <bool PAIRS>
+__device__ __forceinline__ Place place_of(int lane, int hdim, int rot) {
+  Place p;
+  p.there = 4 * lane < hdim;
+  p.turns = 4 * lane < rot;
+  p.f = 2 * lane;
+  p.a = PAIRS ? 4 * lane : p.turns ? 2 * lane : 4 * lane;
+  p.b = PAIRS ? 4 * lane + 2 : p.turns ? rot / 2 + 2 * lane : 4 * lane + 2;
+  return p;
+}
+
+// x[0], x[2] and x[1], x[3] are the lane's pairs
+template <bool PAIRS>
+__device__ __forceinline__ void head_load(const float *p, const Place &at, float (&x)[4]) {
+  if (PAIRS) {
+    const v4f v = *reinterpret_cast<const v4f *>(p + at.a);
+    x[0] = v[0], x[2] = v[1], x[1] = v[2], x[3] = v[3];
+  } else {
+    const v2f a = *reinterpret_cast<const v2f *>(p + at.a);
+    const v2f b = *reinterpret_cast<const v2f *>(p + at.b);
+    x[0] = a[0], x[1] = a[1], x[2] = b[0], x[3] = b[1];
+  }
+}
+template <bool PAIRS>
+__device__ __forceinline__ void head_store(float *p, const Place &at, const float (&x)[4]) {
+  if (PAIRS) {
+    *reinterpret_cast<v4f *>(p + at.a) = v4f{x[0], x[2], x[1], x[3]};
+  } else {
+    *reinterpret_cast<v2f *>(p + at.a) = v2f{x[0], x[1]};
+    *reinterpret_cast<v2f *>(p + at.b) = v2f{x[2], x[3]};
+  }
+}
+
+// A lane's cosines and sines at a position.
+struct Turn {
+  double c[2], s[2];
+};
+__device__ __forceinline__ Turn turn_at(const Rotary &r, const Place &at, const double (&f)[2],
+                                        int pos) {
+  Turn t = {{1.0, 1.0}, {0.0, 0.0}};
+  if (!at.turns) return t;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    double angle = f[e] * (double)pos;
+    if (r.angle32) angle = (double)((float)f[e] * (float)pos);
+    cos_sin(angle, &t.c[e], &t.s[e]);
+    if (r.angle32) t.c[e] = (double)(float)t.c[e], t.s[e] = (double)(float)t.s[e];
+    t.c[e] *= (double)r.amp;
+    t.s[e] *= (double)r.amp;
+  }
+  return t;
+}
+
+// The norm (weights w1 are w + 1), where the lane's group has one (some: any group has), and the
+// turn of a lane's values.
+template <int G>
+__device__ __forceinline__ void head_turn(float (&x)[4], bool some, bool norm,
+                                          const double (&w1)[4], int hdim, float eps, bool turns,
+                                          const Turn &t) {
+  double d[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) d[e] = (double)x[e];
+  if (some) {
+    const double ss = fma(d[0], d[0], d[1] * d[1]) + fma(d[2], d[2], d[3] * d[3]);
+    const double m = rsqrt_f64(group_sum_f64<G>(ss) / (double)hdim + (double)eps);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) d[e] = norm ? d[e] * (m * w1[e]) : d[e];
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const double a = d[e], b = d[e + 2];
+    x[e] = (float)(turns ? a * t.c[e] - b * t.s[e] : a);
+    x[e + 2] = (float)(turns ? b * t.c[e] + a * t.s[e] : b);
+  }
+}
+
+template <bool PAIRS>
+__device__ __forceinline__ void weights_load(const float *w, const Place &at, double (&w1)[4]) {
+  float x[4] = {};
+  if (w != nullptr && at.there) head_load<PAIRS>(w, at, x);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w1[e] = (double)x[e] + 1.0;
+}
+__device__ __forceinline__ void freq_load(const Rotary &r, const Place &at, double (&f)[2]) {
+  f[0] = f[1] = 0.0;
+  if (at.turns) f[0] = r.freq[at.f], f[1] = r.freq[at.f + 1];
+}
+
+// H heads of a row for each group of G lanes; a wave's groups take neighbouring ones
+template <int G, bool PAIRS, int H>
+__global__ __launch_bounds__(kThreads) void rope_kernel(RopeRows a) {
+  constexpr int PER = 64 / G * H;  // heads of a wave
+  const int lane = threadIdx.x % G, group = threadIdx.x % 64 / G;
+  const int parts = (a.heads + PER - 1) / PER;
+  const long unit = (long)blockIdx.x * (kThreads / 64) +
+                    __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int r = (int)(unit / parts), h0 = (int)(unit % parts) * PER + group;
+  if (r >= a.rows) return;
+  const Place at = place_of<PAIRS>(lane, a.hdim, a.rot.rot);
+  float x[H][4];
+#pragma unroll
+  for (int j = 0; j < H; ++j) {
+    const int h = min(h0 + j * (64 / G), a.heads - 1);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[j][e] = 0.0f;
+    if (at.there) head_load<PAIRS>(a.src + r * a.src_stride + h * a.hdim, at, x[j]);
+  }
+  double w1[4], f[2];
+  weights_load<PAIRS>(a.w, at, w1);
+  freq_load(a.rot, at, f);
+  const Turn t = turn_at(a.rot, at, f, a.pos[r]);
+#pragma unroll
+  for (int j = 0; j < H; ++j) {
+    const int h = h0 + j * (64 / G);
+    head_turn<G>(x[j], a.w != nullptr, a.w != nullptr, w1, a.hdim, a.eps, at.turns, t);
+    if (at.there && h < a.heads)
+      head_store<PAIRS>(a.dst + r * a.dst_stride + h * a.hdim, at, x[j]);
+  }
+}
+
+// A head of a row, its values at their places in x, as codes and a scale: cache_write's arithmetic.
+template <int G, int TYPE, bool PAIRS>
+__device__ __forceinline__ void head_code(const KvCache &c, bool isv, long slot, const Place &at,
+                                          const float (&x)[4], int lane) {
+  int top = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) top = max(top, __float_as_int(x[e]) & 0x7fffffff);
+  top = group_max_i32<G>(top);
+  if (slot < 0) return;
+  const bool finite = top < 0x7f800000;
+  const float amax = finite ? daz(__int_as_float(top)) : 0.0f;
+  uint32_t q = 0;  // codes of x[0], x[1], x[2], x[3]
+  float scale = 0.0f;
+  if (amax > 0.0f) {
+    if (TYPE == kKvI8) {
+      const QuantParams qp = quant_params(amax);
+      scale = qp.scale;
+      q = pack4(quant_one(x[0], qp.inv), quant_one(x[1], qp.inv), quant_one(x[2], qp.inv),
+                quant_one(x[3], qp.inv));
+    } else {
+      scale = mul_ftz(amax, 1.0f / 448.0f);
+      const float inv = (float)(448.0 / (double)amax);
+      float y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = fmaxf(-448.0f, fminf(448.0f, daz(x[e]) * inv));
+      const int t = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+      q = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], t, true);
+    }
+  }
+  uint8_t *dst = (isv ? c.v : c.k) + (size_t)slot * (4 * G);
+  if (PAIRS) {
+    *reinterpret_cast<uint32_t *>(dst + at.a) = __builtin_amdgcn_perm(q, q, 0x03010200u);
+  } else {
+    *reinterpret_cast<uint16_t *>(dst + at.a) = (uint16_t)q;
+    *reinterpret_cast<uint16_t *>(dst + at.b) = (uint16_t)(q >> 16);
+  }
+  if (lane == 0) (isv ? c.vs : c.ks)[slot] = finite ? scale : __int_as_float(0x7fc00000);
+}
+
+// H of a row's heads (q's, then k's, then v's) for each group of G lanes
+template <int G, int TYPE, bool PAIRS, int H>
+__global__ __launch_bounds__(kThreads) void kv_append_kernel(KvAppend a) {
+  constexpr int PER = 64 / G * H, HD = 4 * G;
+  const int lane = threadIdx.x % G, group = threadIdx.x % 64 / G;
+  const int nq = a.q != nullptr ? a.n_heads : 0, nk = a.c.nkv, all = nq + 2 * nk;
+  const int parts = (all + PER - 1) / PER;
+  const long unit = (long)blockIdx.x * (kThreads / 64) +
+                    __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int r = (int)(unit / parts), h0 = (int)(unit % parts) * PER + group;
+  if (r >= a.b.rows) return;
+  const Place at = place_of<PAIRS>(lane, HD, a.rot.rot);
+  float x[H][4];
+#pragma unroll
+  for (int j = 0; j < H; ++j) {
+    const int h = min(h0 + j * (64 / G), all - 1);
+    const float *row = h < nq        ? a.q + r * a.q_stride + h * HD
+                       : h < nq + nk ? a.k + r * a.k_stride + (h - nq) * HD
+                                     : a.v + r * a.v_stride + (h - nq - nk) * HD;
+    head_load<PAIRS>(row, at, x[j]);
+  }
+  double wq[4], wk[4], f[2];
+  weights_load<PAIRS>(a.nq, at, wq);
+  weights_load<PAIRS>(a.nk, at, wk);
+  freq_load(a.rot, at, f);
+  const KvRow row = kv_row_wave<true>(a.b, r);
+  if (row.i < 0) return;
+  const Turn t = turn_at(a.rot, at, f, row.pos);
+#pragma unroll
+  for (int j = 0; j < H; ++j) {
+    const int h = h0 + j * (64 / G);
+    const bool isq = h < nq, isk = !isq && h < nq + nk, there = h < all;
+    if (__any(isq || isk)) {
+      double w1[4];
+      float y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w1[e] = isq ? wq[e] : wk[e], y[e] = x[j][e];
+      head_turn<G>(y, a.nq != nullptr || a.nk != nullptr, isq ? a.nq != nullptr : a.nk != nullptr,
+                   w1, HD, a.eps, at.turns, t);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[j][e] = isq || isk ? y[e] : x[j][e];
+    }
+    if (isq) head_store<PAIRS>(a.q_out + r * a.out_stride + h * HD, at, x[j]);
+    if (__any(!isq && there)) {
+      const bool isv = !isq && !isk;
+      const int kv = isv ? h - nq - nk : h - nq;
+      const long slot = isq || !there || row.pos < 0 ? -1 : kv_slot(a.c, a.b, row.i, row.pos, kv);
+      head_code<G, TYPE, PAIRS>(a.c, isv, slot, at, x[j], lane);
+    }
+  }
+}
+
+// Heads a group of lanes does one after the other: one while that leaves the card room, so that a
+// few rows take one trip to memory, else four, which share the row's angles and table look-ups.
+constexpr long kFewHeads = 16384;
+
+}  // namespace
+
+hipError_t launch_rope(const RopeRows &a, hipStream_t stream) {
+  auto go = [&](auto g, auto pairs, auto h) {
+    constexpr int PER = 64 / g() * h();
+    const long units = (long)a.rows * ((a.heads + PER - 1) / PER);
+    rope_kernel<g(), pairs(), h()><<<(unsigned)((units + 3) / 4), kThreads, 0, stream>>>(a);
+  };
+  auto heads = [&](auto g, auto pairs) {
+    (long)a.rows * a.heads <= kFewHeads ? go(g, pairs, std::integral_constant<int, 1>())
+                                        : go(g, pairs, std::integral_constant<int, 4>());
+  };
+  auto pairs = [&](auto g) {
+    a.rot.pairs ? heads(g, std::true_type()) : heads(g, std::false_type());
+  };
+  a.hdim <= 64    ? pairs(std::integral_constant<int, 16>())
+  : a.hdim <= 128 ? pairs(std::integral_constant<int, 32>())
+                  : pairs(std::integral_constant<int, 64>());
+  return hipGetLastError();
+}
+
+hipError_t launch_kv_append(const KvAppend &a, hipStream_t stream) {
+  const int all = (a.q != nullptr ? a.n_heads : 0) + 2 * a.c.nkv;
+  auto go = [&](auto g, auto type, auto pairs, auto h) {
+    constexpr int PER = 64 / g() * h();
+    const long units = (long)a.b.rows * ((all + PER - 1) / PER);
+    kv_append_kernel<g(), type(), pairs(), h()>
+        <<<(unsigned)((units + 3) / 4), kThreads, 0, stream>>>(a);
+  };
+  auto heads = [&](auto g, auto type, auto pairs) {
+    (long)a.b.rows * all <= kFewHeads ? go(g, type, pairs, std::integral_constant<int, 1>())
+                                      : go(g, type, pairs, std::integral_constant<int, 4>());
+  };
+  auto pairs = [&](auto g, auto type) {
+    a.rot.pairs ? heads(g, type, std::true_type()) : heads(g, type, std::false_type());
+  };
+  auto type = [&](auto g) {
+    a.c.type == kKvI8 ? pairs(g, std::integral_constant<int, kKvI8>())
+                      : pairs(g, std::integral_constant<int, kKvE4m3>());
+  };
+  a.c.hdim == 256 ? type(std::integral_constant<int, 64>())
+                  : type(std::integral_constant<int, 32>());
+  return hipGetLastError();
+}
+
+}  // namespace gh

@@ -144,14 +144,77 @@ class Sampling(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in ("temperature", "top_k", "top_p", "min_p")]
 
 
+class Rotary(ctypes.Structure):
+    """gemma_hip_rotary: how heads turn with their positions."""
+
+    _fields_ = [("freq", ctypes.c_void_p)] + \
+               [(n, ctypes.c_int) for n in ("rot", "layout", "angle32")] + [("amp", ctypes.c_float)]
+
+
+class Heads(ctypes.Structure):
+    """gemma_hip_heads: a layer's q, k and v rows on their way into its attention."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "v", "q_out")] + \
+               [(n, ctypes.c_int) for n in ("q_stride", "k_stride", "v_stride", "q_out_stride",
+                                            "n_heads")] + \
+               [(n, ctypes.c_void_p) for n in ("nq", "nk")] + [("eps", ctypes.c_float),
+                                                               ("rotary", Rotary)]
+
+
+class Norm(ctypes.Structure):
+    """gemma_hip_norm: a norm of rows."""
+
+    _fields_ = [("kind", ctypes.c_int), ("w", ctypes.c_void_p), ("b", ctypes.c_void_p),
+                ("offset", ctypes.c_float), ("eps", ctypes.c_float)]
+
+
+class Residual(ctypes.Structure):
+    """gemma_hip_residual: what lies between two blocks."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "y", "gate")] + \
+               [(n, ctypes.c_int) for n in ("x_stride", "y_stride", "gate_stride", "gate_one")] + \
+               [(n, ctypes.c_float) for n in ("x_scale", "y_scale")] + \
+               [("after", Norm), ("before", Norm)] + \
+               [(n, ctypes.c_void_p) for n in ("x_out", "h", "hq", "hs")] + \
+               [(n, ctypes.c_int) for n in ("x_out_stride", "h_stride", "hq_stride")]
+
+
+class Adapters(ctypes.Structure):
+    """gemma_hip_adapters: low-rank adapters and the requests that use them."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("row0", "ids", "scale")] + \
+               [(n, ctypes.c_int) for n in ("batch", "rows", "max_rows", "count", "rank", "type")]
+
+
+class AdapterJob(ctypes.Structure):
+    """gemma_hip_adapter_job: the adapters of one projection."""
+
+    _fields_ = [("a", ctypes.c_void_p), ("b", ctypes.c_void_p), ("n", ctypes.c_int)]
+
+
+class Scores(ctypes.Structure):
+    """gemma_hip_scores: what GemmaHip.logprobs answers."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("logp", "rank", "entropy", "top", "top_logp")]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
+_F = ctypes.c_float
+_D = ctypes.c_double
 
 # attention arithmetic of the prompt passes and the vision tower
 # (GEMMA_HIP_ATTN_*): fp32 (the default) or fp64 matrix cores (verification)
 ATTN_F64, ATTN_F32 = 0, 1
 # what a paged cache's codes are (GEMMA_HIP_CACHE_*)
 CACHE_I8, CACHE_E4M3 = 0, 1
+# which values of a head turn together, and how frequencies follow longer contexts
+# (GEMMA_HIP_ROPE_*)
+ROPE_HALF, ROPE_PAIRS = 0, 1
+ROPE_NONE, ROPE_LINEAR, ROPE_NTK, ROPE_BANDS, ROPE_YARN = range(5)
+# norms (GEMMA_HIP_NORM_*) and adapters' types (GEMMA_HIP_ADAPTER_*)
+NORM_NONE, NORM_RMS, NORM_LAYER = range(3)
+ADAPTER_F32, ADAPTER_BF16, ADAPTER_F16 = range(3)
 _SIGS = {
     "gemma_hip_init": (_I, [_I]),
     "gemma_hip_shutdown": (None, []),
@@ -182,6 +245,18 @@ _SIGS = {
     "gemma_hip_sample": (_I, [_P, _P, _P, _I, _I, _I, ctypes.POINTER(Sampling), _P, _P,
                               ctypes.c_size_t, _P]),
     "gemma_hip_sample_work": (ctypes.c_size_t, [_I, _I]),
+    "gemma_hip_rotary_freqs": (_I, [_P, ctypes.POINTER(_F), _I, _D, _I, _D, _D, _D, _D]),
+    "gemma_hip_rope": (_I, [_P, _I, _P, _I, _I, _I, _I, _P, _P, _F, ctypes.POINTER(Rotary), _P]),
+    "gemma_hip_cache_append": (_I, [ctypes.POINTER(Cache), ctypes.POINTER(Batch),
+                                    ctypes.POINTER(Heads), _P]),
+    "gemma_hip_norm_residual": (_I, [ctypes.POINTER(Residual), _I, _I, _P]),
+    "gemma_hip_adapters_add": (_I, [_P, _I, _P, _I, ctypes.POINTER(Adapters),
+                                    ctypes.POINTER(AdapterJob), _I, _P, _I, _I, _P,
+                                    ctypes.c_size_t, _P]),
+    "gemma_hip_adapters_work": (ctypes.c_size_t, [ctypes.POINTER(Adapters), _I, _I]),
+    "gemma_hip_logprobs": (_I, [ctypes.POINTER(Scores), _P, _I, _I, _I, _P, _P, _I, _I, _P,
+                                ctypes.c_size_t, _P]),
+    "gemma_hip_logprobs_work": (ctypes.c_size_t, [_I, _I, _I, _I]),
     "gemma_hip_matmul_multi": (_I, [ctypes.POINTER(Job), _I, _P, _P, _I, _P]),
     "gemma_hip_quantize_matmul": (_I, [ctypes.POINTER(Job), _I, _P, _I, _P, _P, _P]),
     "gemma_hip_matmul_f32": (_I, [_P, _I, _P, _I, _P, _I, _I, _I, _I, _P]),
@@ -276,6 +351,75 @@ def batch(pages, len, row0, batch, max_pages, rows, max_rows, max_len) -> Batch:
 def sampling(temperature=None, top_k=None, top_p=None, min_p=None) -> Sampling:
     """Settings of GemmaHip.sample: device arrays of a value per row, or None."""
     return _kept(Sampling, (temperature, top_k, top_p, min_p))
+
+
+def rotary(freq, rot, layout=ROPE_HALF, amp=1.0, angle32=False) -> Rotary:
+    """A rotation of heads' first `rot` values by a device array of rot / 2 float64
+    radians a position (rotary_freqs)."""
+    s = Rotary(_addr(freq), int(rot), int(layout), int(bool(angle32)), float(amp))
+    s.buffers = (freq,)
+    return s
+
+
+def rotary_freqs(rot, theta, scaling=ROPE_NONE, factor=1.0, original=0.0, low=1.0, high=32.0):
+    """gemma_hip_rotary_freqs: (float64 numpy array of rot / 2 frequencies, amplitude)."""
+    import numpy as np
+
+    lib = load()
+    freq, amp = np.empty(max(0, int(rot)) // 2), ctypes.c_float(1.0)
+    if lib.gemma_hip_rotary_freqs(freq.ctypes.data, ctypes.byref(amp), rot, theta, scaling, factor,
+                                  original, low, high) != 0:
+        raise GemmaHipError(lib.gemma_hip_last_error().decode())
+    return freq, amp.value
+
+
+def heads(q, q_stride, k, k_stride, v, v_stride, q_out, q_out_stride, n_heads, nq=None, nk=None,
+          eps=1e-6, rotary=None) -> Heads:
+    """Rows of q (or None), k and v for GemmaHip.cache_append, with the norms' weights
+    (stored as w, applied as w + 1) and the rotation."""
+    s = Heads(_addr(q), _addr(k), _addr(v), _addr(q_out), int(q_stride), int(k_stride),
+              int(v_stride), int(q_out_stride), int(n_heads), _addr(nq), _addr(nk), float(eps),
+              rotary if rotary is not None else Rotary())
+    s.buffers = (q, k, v, q_out, nq, nk, rotary)
+    return s
+
+
+def norm(kind, w=None, b=None, offset=0.0, eps=1e-6) -> Norm:
+    """A norm of rows: NORM_RMS or NORM_LAYER, times w + offset, plus b."""
+    s = Norm(int(kind), _addr(w), _addr(b), float(offset), float(eps))
+    s.buffers = (w, b)
+    return s
+
+
+def residual(x, y=None, gate=None, x_scale=1.0, y_scale=1.0, after=None, before=None, x_out=None,
+             h=None, hq=None, hs=None, x_stride=0, y_stride=0, gate_stride=0, gate_one=False,
+             x_out_stride=0, h_stride=0, hq_stride=0) -> Residual:
+    """x' = x_scale x + y_scale gate after(y) to x_out, before(x') to h and, as int8
+    codes and scales, to hq and hs; after, before: norm() or None."""
+    s = Residual(_addr(x), _addr(y), _addr(gate), int(x_stride), int(y_stride), int(gate_stride),
+                 int(bool(gate_one)), float(x_scale), float(y_scale), after or Norm(),
+                 before or Norm(), _addr(x_out), _addr(h), _addr(hq), _addr(hs),
+                 int(x_out_stride), int(h_stride), int(hq_stride))
+    s.buffers = (x, y, gate, after, before, x_out, h, hq, hs)
+    return s
+
+
+def adapters(row0, ids, scale, batch, rows, max_rows, count, rank, type) -> Adapters:
+    """Adapters of a batch: device arrays row0 [batch + 1] and ids [batch] (int32), scale
+    [count] (float32, or None); type ADAPTER_F32, _BF16 or _F16."""
+    return _kept(Adapters, (row0, ids, scale), batch, rows, max_rows, count, rank, type)
+
+
+def adapter_jobs(specs) -> ctypes.Array:
+    """[(a [count][rank][k], b [count][n][rank], n), ...] as gemma_hip_adapter_job's."""
+    arr = (AdapterJob * len(specs))(*((_addr(a), _addr(b), int(n)) for a, b, n in specs))
+    arr.buffers = specs
+    return arr
+
+
+def scores(logp=None, rank=None, entropy=None, top=None, top_logp=None) -> Scores:
+    """Where GemmaHip.logprobs' answers go: device arrays or None."""
+    return _kept(Scores, (logp, rank, entropy, top, top_logp))
 
 
 class GemmaHip:
@@ -429,6 +573,37 @@ class GemmaHip:
     def sample_work(self, rows: int, vocab: int) -> int:
         """Bytes of sample's workspace."""
         return self._size(self.lib.gemma_hip_sample_work(rows, vocab))
+
+    def rope(self, dst, dst_stride, src, src_stride, rows, heads, hdim, pos, norm=None, eps=0.0,
+             rotary=None, stream=None):
+        self._check(self.lib.gemma_hip_rope(
+            _addr(dst), dst_stride, _addr(src), src_stride, rows, heads, hdim, _addr(pos),
+            _addr(norm), eps, None if rotary is None else ctypes.byref(rotary), stream))
+
+    def cache_append(self, cache, batch, heads, stream=None):
+        self._check(self.lib.gemma_hip_cache_append(ctypes.byref(cache), ctypes.byref(batch),
+                                                    ctypes.byref(heads), stream))
+
+    def norm_residual(self, residual, rows, dim, stream=None):
+        self._check(self.lib.gemma_hip_norm_residual(ctypes.byref(residual), rows, dim, stream))
+
+    def adapters_add(self, dst, dstr, base, bstr, adapters, jobs, src, sstr, k, work=None,
+                     stream=None):
+        self._check(self.lib.gemma_hip_adapters_add(
+            _addr(dst), dstr, _addr(base), bstr, ctypes.byref(adapters), jobs, len(jobs),
+            _addr(src), sstr, k, _addr(work), _nbytes(work), stream))
+
+    def adapters_work(self, adapters, njobs: int, k: int) -> int:
+        return self._size(self.lib.gemma_hip_adapters_work(ctypes.byref(adapters), njobs, k))
+
+    def logprobs(self, scores, logits, stride, rows, vocab, temperature, ids, targets, ntop,
+                 work=None, stream=None):
+        self._check(self.lib.gemma_hip_logprobs(
+            ctypes.byref(scores), _addr(logits), stride, rows, vocab, _addr(temperature),
+            _addr(ids), targets, ntop, _addr(work), _nbytes(work), stream))
+
+    def logprobs_work(self, rows: int, vocab: int, targets: int, ntop: int) -> int:
+        return self._size(self.lib.gemma_hip_logprobs_work(rows, vocab, targets, ntop))
 
     def register_weights(self, host, nbytes: int):
         self._check(self.lib.gemma_hip_register_weights(_addr(host), nbytes))

@@ -107,7 +107,9 @@ int gemma_hip_sync(void *stream);
  * "sample_from_logits" (softcap + argmax,
  * counted in the decode phase as the reference does).  Of the entry points for
  * batches, cache_write and cache_read count as "quantize_act", cache_attention as
- * "softmax" and gemma_hip_sample as "sample_from_logits".  The decoder and the
+ * "softmax", gemma_hip_sample and gemma_hip_logprobs as "sample_from_logits", gemma_hip_rope and
+ * cache_append as "rope", norm_residual as "rmsnorm" ("layernorm" where one of its norms is) and
+ * adapters_add as "gemm_fpx" ("gemv_fpx" for single rows).  The decoder and the
  * tower set the phase themselves as the reference's forward_gemma_* do: decoder_prefill and
  * prefill_rows with mask != 0 prefill; decoder_step and decoder_generate
  * decode (run eagerly, not as the captured graph, while timing is on);
@@ -672,6 +674,182 @@ int gemma_hip_sample(int *tokens, float *probs, const float *logits, int stride,
 
 /* Bytes of gemma_hip_sample's workspace ((size_t)-1 for sizes it refuses). */
 size_t gemma_hip_sample_work(int rows, int vocab);
+
+/* ---- between the products of a served batch --------------------------------- */
+/* What a layer needs beside its products and its attention, and an answer beside its tokens, for
+ * rows of any number of requests: rotary positions, rows appended to the paged cache, norms
+ * around the residual sum, low-rank adapters, log probabilities.  As above: device buffers,
+ * nothing allocated when a workspace is given, and all may be captured then. */
+
+/* How heads turn with their positions: of a head's first `rot` values (a multiple of 4; 0: none),
+ * pair j turns by pos * freq[j] radians, (x, y) -> (x c - y s, y c + x s) with c and s `amp`
+ * times the angle's cosine and sine (0 stands for 1).  freq: rot / 2 doubles in device memory
+ * (gemma_hip_rotary_freqs; |pos * freq| below 2^31).  pairs: (j, j + rot/2), the reference's
+ * rope_apply (gemma.c:4223-4246), or neighbours (2j, 2j + 1).  Angles and values are fp64, rounded
+ * to fp32 at the end; angle32 != 0 rounds the frequency, the angle, its cosine and its sine to
+ * fp32 first, as the reference's rope_freqs_pos (gemma.c:4178-4196) and the device-resident
+ * decoder do. */
+#define GEMMA_HIP_ROPE_HALF 0
+#define GEMMA_HIP_ROPE_PAIRS 1
+typedef struct {
+  const double *freq;
+  int rot, layout, angle32;
+  float amp;
+} gemma_hip_rotary;
+
+/* Frequencies for contexts longer than the ones that were trained on, into the host array freq
+ * [rot / 2], from f_j = theta^(-2j / rot); *amp (nullable) is the amplitude that goes with them,
+ * 1 but for YARN:
+ *   NONE    f_j
+ *   LINEAR  f_j / factor
+ *   NTK     theta * factor^(rot / (rot - 2)) in theta's place
+ *   BANDS   by the turns n_j = original f_j / 2 pi that a pair makes in the original context: f_j
+ *           from n_j >= high on, f_j / factor up to n_j <= low, f_j ((1 - s) / factor + s) with s =
+ *           (n_j - low) / (high - low) between
+ *   YARN    f_j (s / factor + 1 - s), s rising from 0 to 1 between j = floor(d(high)) and
+ *           ceil(d(low)), cut to 0 .. rot - 1, where d(n) = rot ln(original / (2 pi n)) / (2 ln
+ *           theta) is the pair that makes n turns; amplitude 1 + 0.1 ln(factor)
+ * (original, low and high are read by the last two, low < high.)  Runs on the host, without a
+ * GPU. */
+#define GEMMA_HIP_ROPE_NONE 0
+#define GEMMA_HIP_ROPE_LINEAR 1
+#define GEMMA_HIP_ROPE_NTK 2
+#define GEMMA_HIP_ROPE_BANDS 3
+#define GEMMA_HIP_ROPE_YARN 4
+int gemma_hip_rotary_freqs(double *freq, float *amp, int rot, double theta, int scaling,
+                           double factor, double original, double low, double high);
+
+/* dst row r, head h = src's, through the norm x / sqrt(mean x^2 + eps) (norm + 1) where norm
+ * (device, [hdim]) is given, turned by pos[r] (device, any int).  Rows of heads * hdim floats, head
+ * h at column h * hdim, strides multiples of 4, 16-byte aligned; hdim a multiple of 4 up to
+ * 256; rows times heads at most 2^25.  dst may be src with the same stride; they don't overlap
+ * otherwise.  A NaN stays in its head, without norm in its pair. */
+int gemma_hip_rope(float *dst, int dst_stride, const float *src, int src_stride, int rows,
+                   int heads, int hdim, const int *pos, const float *norm, float eps,
+                   const gemma_hip_rotary *rotary, void *stream);
+
+/* The rows of a layer's q, k and v products on their way into its attention: q (NULL: no
+ * queries, n_heads is not read) and k as gemma_hip_rope, by norms nq and nk (device [hdim], 16-byte
+ * aligned; NULL: none), v as it is.  Row strides in floats, multiples of 4 (0: dense); rows
+ * 16-byte aligned.  The three may be columns of one buffer, and q_out may be q with its
+ * stride. */
+typedef struct {
+  const float *q, *k, *v;
+  float *q_out;
+  int q_stride, k_stride, v_stride, q_out_stride, n_heads;
+  const float *nq, *nk;
+  float eps;
+  gemma_hip_rotary rotary;
+} gemma_hip_heads;
+
+/* gemma_hip_cache_write of a batch's new rows with what comes before it: q normed and turned by
+ * the rows' positions to q_out, k so into the cache, v into the cache (gemma.c:4776-4830,
+ * 5093-5150).  A row's position is that of gemma_hip_batch, negative where its sequence is
+ * shorter than its rows: q turns by it, k and v are not written.  Keys are rounded to fp32 once
+ * and then to codes as cache_write does.  Rows of q behind the last sequence stay as they
+ * were. */
+int gemma_hip_cache_append(const gemma_hip_cache *cache, const gemma_hip_batch *batch,
+                           const gemma_hip_heads *heads, void *stream);
+
+/* A norm of rows: (v - mean) / sqrt(var + eps) (w + offset) + b, with (LAYER) or without (RMS: mean
+ * 0, var the mean square) the mean; NONE: v.  w, b: device [dim], 16-byte aligned; w NULL: 1
+ * in (w + offset)'s place; b NULL: 0.  gemma.c's rmsnorm (2508-2534) is RMS with offset 1. */
+#define GEMMA_HIP_NORM_NONE 0
+#define GEMMA_HIP_NORM_RMS 1
+#define GEMMA_HIP_NORM_LAYER 2
+typedef struct {
+  int kind;
+  const float *w, *b;
+  float offset, eps;
+} gemma_hip_norm;
+
+/* Between two blocks: x' = clamp(x_scale x + y_scale gate after(y)), h = before(x').
+ *   x [rows][dim], the residual rows; y, a block's output (NULL: x' = x_scale x); gate (NULL: 1)
+ *   a row of factors for each row, or one for all with gate_one != 0
+ *   x_out, x' (NULL: not stored; may be x); h (NULL: not stored); hq and hs (both or neither): h as
+ *   gemma_hip_quantize makes it, int8 [rows][hq_stride] and a scale per row (a row of h with a NaN
+ *   or an infinity: codes of 0 and a NaN scale)
+ * The clamp is the reference's clamp_fpx (gemma.c:2504-2506) but leaves NaN.  Sums, norms and
+ * products are fp64; x' and h are rounded to fp32 once each.  Strides in elements (0: dense),
+ * multiples of 4; fp32 rows 16-byte, hq 4-byte aligned.  Buffers that are written may be x or y
+ * with their stride, and overlap nothing else. */
+typedef struct {
+  const float *x, *y, *gate;
+  int x_stride, y_stride, gate_stride, gate_one;
+  float x_scale, y_scale;
+  gemma_hip_norm after, before;
+  float *x_out, *h;
+  int8_t *hq;
+  float *hs;
+  int x_out_stride, h_stride, hq_stride;
+} gemma_hip_residual;
+
+/* rows of dim values, dim a multiple of 4 up to 24576. */
+int gemma_hip_norm_residual(const gemma_hip_residual *residual, int rows, int dim, void *stream);
+
+/* Low-rank adapters, `count` of them, and the requests that use them.  ids [batch]: each sequence's
+ * adapter, none where it isn't 0 .. count - 1; row0 [batch + 1], rows and max_rows as in
+ * gemma_hip_batch; scale [count] (NULL: 1).  Device memory, but for the sizes.  rank: a multiple
+ * of 8 up to 128 (smaller adapters are filled up with zeros); type: that of the matrices. */
+#define GEMMA_HIP_ADAPTER_F32 0
+#define GEMMA_HIP_ADAPTER_BF16 1
+#define GEMMA_HIP_ADAPTER_F16 2
+typedef struct {
+  const int *row0, *ids;
+  const float *scale;
+  int batch, rows, max_rows, count, rank, type;
+} gemma_hip_adapters;
+
+/* The adapters of one projection: a [count][rank][k], b [count][n][rank], device, 16-byte
+ * aligned. */
+typedef struct {
+  const void *a, *b;
+  int n;
+} gemma_hip_adapter_job;
+
+/* dst = base + scale[id] b[id] (a[id] src) for the rows of a batch, beside the product that all of
+ * them share (gemma_hip_matmul_cols, gemma_hip_matmul_f32_cols): njobs (<= 3) projections of the
+ * same rows side by side, job j's columns behind those of the jobs before it.  src fp32 [rows][sstr],
+ * 16-byte aligned, sstr a multiple of 4, k a multiple of 8; base and dst fp32 [rows][bstr], [dstr]
+ * (0: dense); dst may be base with its stride, and overlaps neither otherwise.  Rows of sequences
+ * without an adapter are base; rows behind the last sequence stay as they were.  Sums are fp32, of
+ * products as exact as fp32 ones: a result is off by at most about 1e-6 of the sum of its terms'
+ * magnitudes.
+ * work: gemma_hip_adapters_work() bytes, 256-byte aligned, which one call at a time may use; NULL
+ * takes the library's for the stream (not while it is being captured). */
+int gemma_hip_adapters_add(float *dst, int dstr, const float *base, int bstr,
+                           const gemma_hip_adapters *adapters, const gemma_hip_adapter_job *jobs,
+                           int njobs, const float *src, int sstr, int k, void *work,
+                           size_t work_bytes, void *stream);
+
+/* Bytes of gemma_hip_adapters_add's workspace ((size_t)-1 for sizes it refuses). */
+size_t gemma_hip_adapters_work(const gemma_hip_adapters *adapters, int njobs, int k);
+
+/* What gemma_hip_logprobs answers; device arrays, each nullable. */
+typedef struct {
+  float *logp;     /* [rows][targets] log probabilities of the given tokens */
+  int *rank;       /* [rows][targets] their places in the order of gemma_hip_sample, from 1 */
+  float *entropy;  /* [rows] -sum p log p */
+  int *top;        /* [rows][ntop] the first tokens of that order (-1 where there are fewer) ... */
+  float *top_logp; /* [rows][ntop] ... and their log probabilities (-inf) */
+} gemma_hip_scores;
+
+/* Rows of logits [rows][stride] (vocab columns, vocab <= 524288; stride 0: dense) as distributions p
+ * = softmax(logit / temperature), temperature [rows] (NULL: 1): natural logarithms of given tokens'
+ * probabilities, ids [rows][targets] (targets <= 64), their ranks, the entropies and the ntop (<= 64)
+ * likeliest tokens, by falling logit and then rising index.  As in gemma_hip_sample, NaN counts
+ * as -inf, +inf logits share everything, and temperature 0 (or below, or NaN) puts all on the
+ * first of the largest.  An id outside 0 .. vocab - 1 has log probability -inf and rank 0; -inf
+ * logits have -inf and aren't among the likeliest; a row without a logit above -inf has entropy 0.
+ * Log probabilities and entropies are off by at most 4e-6 of the larger of 1 and
+ * themselves, mostly by 1e-7.
+ * work: gemma_hip_logprobs_work() bytes, as above. */
+int gemma_hip_logprobs(const gemma_hip_scores *scores, const float *logits, int stride, int rows,
+                       int vocab, const float *temperature, const int *ids, int targets, int ntop,
+                       void *work, size_t work_bytes, void *stream);
+
+/* Bytes of gemma_hip_logprobs' workspace ((size_t)-1 for sizes it refuses). */
+size_t gemma_hip_logprobs_work(int rows, int vocab, int targets, int ntop);
 
 #ifdef __cplusplus
 }
