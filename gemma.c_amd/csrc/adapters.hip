@@ -1,13 +1,17 @@
 // adapters.hip -- low-rank adapters of many requests on one batch of rows.
 //
-//   u = A[id] x  (rank values a job),  dst = base + scale[id] B[id] u
+//   u = scale[id] A[id] x  (rank values a job),  dst = base + B[id] u
 //
 // id is that of the row's sequence; jobs are projections side by side (q, k, v; gate, up).  A launch
-// for the first product, whose fp32 results lie in the workspace, and one for the second.
+// for the first product, whose fp32 results and whose rows' ids lie in the workspace, and one for
+// the second.
+//
+// Rows of prompts go 16 at a time through the bf16 matrix cores: an fp32 value is the sum of three
+// bf16 pieces, a bf16 weight is one, an f16 weight the sum of two and an fp32 weight of three, and
+// of the piece products those are summed whose orders add up to at most 2 (3, 5 or 6 of
+// them: what is left out is below 2^-22 of a product).  A tile with several adapters is done once
+// for each.  Single tokens take a wave for a value of u and a lane for a value of dst.
 #include <type_traits>
-
-#include <hip/hip_bf16.h>
-#include <hip/hip_fp16.h>
 
 #include "gh_arith.h"
 #include "gh_kernels.h"
@@ -16,97 +20,440 @@ namespace gh {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kNone = -1, kOutside = -2;  // a row's id: no adapter, in no sequence
 
-// eight neighbouring weights
+typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));
+
+// ---- weights ---------------------------------------------------------------------
+
 template <int TYPE>
-__device__ __forceinline__ void load8(const void *p, size_t at, float (&w)[8]) {
+constexpr int kPieces = TYPE == kAdapterBf16 ? 1 : TYPE == kAdapterF16 ? 2 : 3;
+
+// eight neighbouring weights as they lie in memory
+template <int TYPE>
+struct Raw8 {
+  u4 v[TYPE == kAdapterF32 ? 2 : 1];
+};
+template <int TYPE>
+__device__ __forceinline__ Raw8<TYPE> raw8(const void *p, size_t at) {
+  Raw8<TYPE> w;
   if (TYPE == kAdapterF32) {
-    const v4f a = *reinterpret_cast<const v4f *>((const float *)p + at);
-    const v4f b = *reinterpret_cast<const v4f *>((const float *)p + at + 4);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = a[e], w[e + 4] = b[e];
-  } else if (TYPE == kAdapterBf16) {
-    const u4 a = *reinterpret_cast<const u4 *>((const uint16_t *)p + at);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) w[2 * e] = bf16_lo(a[e]), w[2 * e + 1] = bf16_hi(a[e]);
+    w.v[0] = *reinterpret_cast<const u4 *>((const float *)p + at);
+    w.v[TYPE == kAdapterF32] = *reinterpret_cast<const u4 *>((const float *)p + at + 4);
   } else {
-    const h8 a = *reinterpret_cast<const h8 *>((const uint16_t *)p + at);
+    w.v[0] = *reinterpret_cast<const u4 *>((const uint16_t *)p + at);
+  }
+  return w;
+}
+template <int TYPE>
+__device__ __forceinline__ void floats8(const Raw8<TYPE> &w, float (&f)[8]) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = (float)a[e];
+  for (int e = 0; e < 4; ++e) {
+    if (TYPE == kAdapterF32) {
+      f[e] = __uint_as_float(w.v[0][e]);
+      f[e + 4] = __uint_as_float(w.v[TYPE == kAdapterF32][e]);
+    } else if (TYPE == kAdapterBf16) {
+      f[2 * e] = bf16_lo(w.v[0][e]);
+      f[2 * e + 1] = bf16_hi(w.v[0][e]);
+    } else {
+      const uint32_t two = w.v[0][e];  // (a cast of the element itself takes the first one's bits)
+      const h2 h = __builtin_bit_cast(h2, two);
+      f[2 * e] = (float)h[0];
+      f[2 * e + 1] = (float)h[1];
+    }
   }
 }
 
-// The adapter of row r, -1: none; -2: the row is in no sequence.
-__device__ __forceinline__ int adapter_of(const Adapters &a, int r) {
-  const KvRow row = kv_row_wave<false>(a.seq, r);
-  if (row.i < 0) return -2;
-  const int id = a.ids[row.i];
-  return (unsigned)id < (unsigned)a.count ? id : -1;
+// N bf16 pieces of eight values, each the operand of a matrix instruction
+template <int N>
+struct Split8 {
+  u4 p[N];
+};
+template <int N>
+__device__ __forceinline__ Split8<N> split8(const float (&f)[8]) {
+  Split8<N> s;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float a = f[2 * e], b = f[2 * e + 1];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      s.p[i][e] = cvt_pk_bf16(a, b);
+      a -= bf16_lo(s.p[i][e]);
+      b -= bf16_hi(s.p[i][e]);
+    }
+  }
+  return s;
+}
+template <int TYPE>
+__device__ __forceinline__ Split8<kPieces<TYPE>> pieces8(const Raw8<TYPE> &w) {
+  if constexpr (TYPE == kAdapterBf16) {
+    return Split8<1>{{w.v[0]}};
+  } else {
+    float f[8];
+    floats8<TYPE>(w, f);
+    return split8<kPieces<TYPE>>(f);
+  }
 }
 
-// a wave for one value of u
+// D[4 (lane / 16) + r][lane % 16] += W[lane % 16][8 (lane / 16) + e] . X[lane % 16][the same], the
+// small products first
+template <int N>
+__device__ __forceinline__ v4f product(const Split8<N> &w, const Split8<3> &x, v4f d) {
+#pragma unroll
+  for (int order = 2; order >= 0; --order)
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (order - i >= 0 && order - i < 3)
+        d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf8(w.p[i]), as_bf8(x.p[order - i]), d, 0,
+                                                    0, 0);
+  return d;
+}
+
+__device__ __forceinline__ const void *job_of(const void *const (&m)[kAdapterMaxJobs], int job) {
+  return job == 0 ? m[0] : job == 1 ? m[1] : m[2];
+}
+__device__ __forceinline__ float scale_of(const Adapters &a, int id) {
+  return a.scale != nullptr ? a.scale[id] : 1.0f;
+}
+
+// The workspace: u [rows][jobs * rank], then the rows' ids.
+__device__ __forceinline__ float *u_of(const Adapters &a) {
+  return reinterpret_cast<float *>(a.work);
+}
+__device__ __forceinline__ int *ids_of(const Adapters &a) {
+  return reinterpret_cast<int *>(a.work + (size_t)a.seq.rows * a.njobs * a.rank * 4);
+}
+
+// ---- single tokens ----------------------------------------------------------------
+
+// By a whole wave.
+__device__ __forceinline__ int id_of_row(const Adapters &a, int r) {
+  const KvRow row = kv_row_wave<false>(a.seq, r);
+  if (row.i < 0) return kOutside;
+  const int id = a.ids[row.i];
+  return (unsigned)id < (unsigned)a.count ? id : kNone;
+}
+
 template <int TYPE>
-__global__ __launch_bounds__(kThreads) void adapter_shrink_kernel(Adapters a) {
+__global__ __launch_bounds__(kThreads) void adapter_shrink_row_kernel(Adapters a) {
   const int all = a.njobs * a.rank, lane = threadIdx.x & 63, r = blockIdx.x;
   const int at = blockIdx.y * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int job = at / a.rank, row = at % a.rank;
   if (at >= all) return;
-  const int id = adapter_of(a, r);
+  const int id = id_of_row(a, r);
+  if (at == 0 && lane == 0) ids_of(a)[r] = id;
   if (id < 0) return;
-  const void *m = job == 0 ? a.a[0] : job == 1 ? a.a[1] : a.a[2];
+  const void *m = job_of(a.a, job);
   const size_t first = ((size_t)id * a.rank + row) * a.k;
   const float *x = a.src + r * a.src_stride;
   float s = 0.0f;
   for (int c = 8 * lane; c < a.k; c += 512) {
     float w[8];
-    load8<TYPE>(m, first + c, w);
+    floats8<TYPE>(raw8<TYPE>(m, first + c), w);
     const v4f x0 = *reinterpret_cast<const v4f *>(x + c);
     const v4f x1 = *reinterpret_cast<const v4f *>(x + c + 4);
 #pragma unroll
     for (int e = 0; e < 4; ++e) s = fmaf(x0[e], w[e], s), s = fmaf(x1[e], w[e + 4], s);
   }
   s = group_sum_f32<64>(s);
-  if (lane == 0) reinterpret_cast<float *>(a.work)[(size_t)r * all + at] = s;
+  if (lane == 0) u_of(a)[(size_t)r * all + at] = scale_of(a, id) * s;
 }
 
 template <int TYPE>
-__global__ __launch_bounds__(kThreads) void adapter_expand_kernel(Adapters a) {
+__global__ __launch_bounds__(kThreads) void adapter_expand_row_kernel(Adapters a) {
   const int n = a.end[a.njobs - 1], r = blockIdx.x;
   const int c = blockIdx.y * kThreads + threadIdx.x;
-  const int id = adapter_of(a, r);
-  if (id == -2 || c >= n) return;
+  const int id = ids_of(a)[r];
+  if (id == kOutside || c >= n) return;
   float v = a.base[r * a.base_stride + c];
   if (id >= 0) {
-    const int job = c < a.end[0] ? 0 : a.njobs > 1 && c < a.end[1] ? 1 : a.njobs > 1 ? 2 : 0;
+    const int job = c < a.end[0] ? 0 : a.njobs < 3 || c < a.end[1] ? 1 : 2;
     const int from = job == 0 ? 0 : a.end[job - 1];
-    const void *m = job == 0 ? a.b[0] : job == 1 ? a.b[1] : a.b[2];
+    const void *m = job_of(a.b, job);
     const size_t first = ((size_t)id * (a.end[job] - from) + (c - from)) * a.rank;
-    const float *u = reinterpret_cast<const float *>(a.work) +
-                     (size_t)r * a.njobs * a.rank + job * a.rank;
+    const float *u = u_of(a) + ((size_t)r * a.njobs + job) * a.rank;
     float s = 0.0f;
     for (int k = 0; k < a.rank; k += 8) {
       float w[8];
-      load8<TYPE>(m, first + k, w);
+      floats8<TYPE>(raw8<TYPE>(m, first + k), w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) s = fmaf(u[k + e], w[e], s);
     }
-    v += (a.scale != nullptr ? a.scale[id] : 1.0f) * s;
+    v += s;
   }
   a.dst[r * a.dst_stride + c] = v;
 }
 
+// ---- tiles of rows ------------------------------------------------------------------
+
+// The id of each lane's row (row, of first .. first + 15), by a whole wave: the first row's sequence,
+// and how many of the following ones begin at or before the lane's.
+__device__ __forceinline__ int ids_of_rows(const Adapters &a, int first, int row) {
+  const KvBatch &b = a.seq;
+  const int lane = threadIdx.x & 63, last = first + 15;
+  int i, n;
+  const int lo = i = kv_find_part(b, first, &n);
+  for (int from = lo + 1; from < b.batch; from += 64) {
+    const int begins = b.row0[from + lane < b.batch ? from + lane : b.batch];
+    int j = 0;
+    for (; j < 64 && from + j < b.batch; ++j) {
+      const int at = __builtin_amdgcn_readlane(begins, j);
+      if (at > last) break;
+      i += at <= row;
+    }
+    if (j < 64) break;
+  }
+  const int r0 = kv_clamp(b.row0[i], 0, b.rows);
+  int rows = kv_clamp(b.row0[i + 1], r0, b.rows) - r0;
+  if (rows > b.max_rows) rows = b.max_rows;
+  if (row < r0 || row - r0 >= rows) return kOutside;
+  const int id = a.ids[i];
+  return (unsigned)id < (unsigned)a.count ? id : kNone;
+}
+
+constexpr int kShrinkWaves = 8;  // that share a tile's inputs
+constexpr int kMostT = 4;        // 16 values of u each: a workgroup's, at most
+
+// u of 16 rows and 16 T of their values; each wave takes every eighth step of 32 inputs, the
+// partial sums meet in LDS
+template <int TYPE, int T>
+__global__ __launch_bounds__(64 * kShrinkWaves) void adapter_shrink_kernel(Adapters a) {
+  constexpr int kSteps = TYPE == kAdapterF32 ? 2 : 4;  // whose loads are in flight together
+  __shared__ v4f part[kShrinkWaves][T][64];
+  const int all = a.njobs * a.rank, lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int first = 16 * blockIdx.x, at0 = 16 * T * blockIdx.y;
+  const int row = first + (lane & 15);
+  const bool there = row < a.seq.rows;
+  const int id = ids_of_rows(a, first, row);
+  if (blockIdx.y == 0 && threadIdx.x < 16 && there) ids_of(a)[row] = id;
+  const float *x = a.src + (there ? row : a.seq.rows - 1) * a.src_stride;
+  const int steps = (a.k + 31) / 32, k0 = 8 * (lane / 16);
+  // one of the lane's 16 rows of A in each of the T groups
+  const void *m[T];
+  size_t from[T];
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    const int at = min(at0 + 16 * t + (lane & 15), all - 1), job = at / a.rank;
+    m[t] = job_of(a.a, job);
+    from[t] = (size_t)(at - job * a.rank) * a.k;
+  }
+  unsigned todo = (unsigned)__ballot(id >= 0 && there) & 0xffffu;
+  while (todo != 0) {  // adapter by adapter
+    const int cur = __builtin_amdgcn_readlane(id, __builtin_ctz(todo));
+    todo &= ~(unsigned)__ballot(id == cur);
+    const size_t skip = (size_t)cur * a.rank * a.k;
+    v4f acc[T];
+#pragma unroll
+    for (int t = 0; t < T; ++t) acc[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s0 = wave; s0 < steps; s0 += kShrinkWaves * kSteps) {
+      v4f xs[kSteps][2];
+      Raw8<TYPE> ws[kSteps][T];
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j) {
+        int k = 32 * (s0 + j * kShrinkWaves) + k0;
+        k = k < a.k ? k : 0;
+        xs[j][0] = *reinterpret_cast<const v4f *>(x + k);
+        xs[j][1] = *reinterpret_cast<const v4f *>(x + k + 4);
+#pragma unroll
+        for (int t = 0; t < T; ++t) ws[j][t] = raw8<TYPE>(m[t], skip + from[t] + k);
+      }
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j) {
+        const int s = s0 + j * kShrinkWaves;
+        if (s >= steps) break;
+        const bool in = 32 * s + k0 < a.k;  // all but the last step's last lanes are
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] = in ? xs[j][0][e] : 0.0f, f[e + 4] = in ? xs[j][1][e] : 0.0f;
+        const Split8<3> xp = split8<3>(f);
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+          Raw8<TYPE> w = ws[j][t];
+#pragma unroll
+          for (auto &v : w.v) v = in ? v : u4{0, 0, 0, 0};
+          acc[t] = product(pieces8<TYPE>(w), xp, acc[t]);
+        }
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < T; ++t) part[wave][t][lane] = acc[t];
+    __syncthreads();
+    if (wave < T) {
+      v4f sum = part[0][wave][lane];
+#pragma unroll
+      for (int w = 1; w < kShrinkWaves; ++w) sum += part[w][wave][lane];
+      const int at = at0 + 16 * wave + 4 * (lane / 16);
+      if (id == cur && there && at < all) {
+        const float sc = scale_of(a, cur);
+        *reinterpret_cast<v4f *>(u_of(a) + (size_t)row * all + at) = sum * sc;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+constexpr int kExpandRows = 32;  // of a wave
+constexpr int kExpandGroups = 2; // of 64 columns: a wave's
+
+__host__ __device__ inline int expand_units(const int (&end)[kAdapterMaxJobs], int njobs) {
+  int n = 0;
+  for (int j = 0; j < njobs; ++j) {
+    const int w = end[j] - (j == 0 ? 0 : end[j - 1]);
+    n += (w + 64 * kExpandGroups - 1) / (64 * kExpandGroups);
+  }
+  return n;
+}
+
+// dst of 32 rows and 128 columns of a job a wave; KS: steps of 32 of the rank
+template <int TYPE, int KS>
+__global__ __launch_bounds__(kThreads) void adapter_expand_kernel(Adapters a) {
+  constexpr int RT = kExpandRows / 16;
+  const int lane = threadIdx.x & 63, all = a.njobs * a.rank;
+  int unit = blockIdx.y * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  int job = 0, begin = 0, width = a.end[0];
+  for (; job < a.njobs; ++job) {
+    begin = job == 0 ? 0 : a.end[job - 1];
+    width = a.end[job] - begin;
+    const int units = (width + 64 * kExpandGroups - 1) / (64 * kExpandGroups);
+    if (unit < units) break;
+    unit -= units;
+  }
+  if (job == a.njobs) return;
+  const void *m = job_of(a.b, job);
+  const int k0 = 8 * (lane / 16);
+  int row[RT], id[RT];
+  Split8<3> u[RT][KS];
+  unsigned long long todo = 0;
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    row[i] = kExpandRows * blockIdx.x + 16 * i + (lane & 15);
+    id[i] = row[i] < a.seq.rows ? ids_of(a)[row[i]] : kOutside;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      float f[8] = {};
+      if (id[i] >= 0 && 32 * s + k0 < a.rank) {
+        const float *p = u_of(a) + (size_t)row[i] * all + job * a.rank + 32 * s + k0;
+        const v4f lo = *reinterpret_cast<const v4f *>(p);
+        const v4f hi = *reinterpret_cast<const v4f *>(p + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] = lo[e], f[e + 4] = hi[e];
+      }
+      u[i][s] = split8<3>(f);
+    }
+    todo |= (__ballot(id[i] >= 0) & 0xffffull) << (16 * i);
+  }
+  for (int g = 0; g < kExpandGroups; ++g) {
+    const int c0 = (unit * kExpandGroups + g) * 64;
+    if (c0 >= width) break;
+    v4f old[4][RT], sum[4][RT];
+    int col[4];  // the first of the lane's four, of the job's
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      col[t] = c0 + 16 * t + 4 * (lane / 16);
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        sum[t][i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        old[t][i] = sum[t][i];
+        if (id[i] == kOutside) continue;
+        const float *p = a.base + row[i] * a.base_stride + begin + col[t];
+        if (col[t] + 4 <= width)
+          old[t][i] = *reinterpret_cast<const v4f_any *>(p);
+        else
+          for (int e = 0; e < 4; ++e)
+            if (col[t] + e < width) old[t][i][e] = p[e];
+      }
+    }
+    for (unsigned long long left = todo; left != 0;) {
+      const int at = __builtin_ctzll(left);
+      int cur = __builtin_amdgcn_readlane(id[0], at & 15);
+#pragma unroll
+      for (int i = 1; i < RT; ++i) {
+        const int other = __builtin_amdgcn_readlane(id[i], at & 15);
+        cur = at / 16 == i ? other : cur;
+      }
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+        left &= ~((__ballot(id[i] == cur) & 0xffffull) << (16 * i));
+      Raw8<TYPE> w[4][KS];
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          const int c = min(c0 + 16 * t + (lane & 15), width - 1);
+          const int k = 32 * s + k0;
+          w[t][s] = raw8<TYPE>(m, ((size_t)cur * width + c) * a.rank + (k < a.rank ? k : 0));
+        }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        v4f d[RT] = {};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          Raw8<TYPE> v = w[t][s];
+#pragma unroll
+          for (auto &x : v.v) x = 32 * s + k0 < a.rank ? x : u4{0, 0, 0, 0};
+          const auto wp = pieces8<TYPE>(v);
+#pragma unroll
+          for (int i = 0; i < RT; ++i) d[i] = product(wp, u[i][s], d[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sum[t][i][e] = id[i] == cur ? d[i][e] : sum[t][i][e];
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        if (id[i] == kOutside) continue;
+        float *p = a.dst + row[i] * a.dst_stride + begin + col[t];
+        const v4f v = id[i] >= 0 ? old[t][i] + sum[t][i] : old[t][i];
+        if (col[t] + 4 <= width)
+          *reinterpret_cast<v4f_any *>(p) = v;
+        else
+          for (int e = 0; e < 4; ++e)
+            if (col[t] + e < width) p[e] = v[e];
+      }
+  }
+}
+
+// Up to so many rows a sequence go by the row.
+constexpr int kFewRows = 2;
+
 }  // namespace
 
 size_t adapters_work(int rows, int njobs, int rank) {
-  return ((size_t)rows * njobs * rank * 4 + 255) / 256 * 256;
+  return ((size_t)rows * (njobs * rank + 1) * 4 + 255) / 256 * 256;
 }
 
 hipError_t launch_adapters(const Adapters &a, const DeviceInfo &dev, hipStream_t stream) {
+  const int rows = a.seq.rows, all = a.njobs * a.rank, n = a.end[a.njobs - 1];
+  auto by_row = [&](auto type) {
+    const dim3 first(rows, (all + 3) / 4), second(rows, (n + kThreads - 1) / kThreads);
+    adapter_shrink_row_kernel<type()><<<first, kThreads, 0, stream>>>(a);
+    adapter_expand_row_kernel<type()><<<second, kThreads, 0, stream>>>(a);
+  };
+  auto shrink = [&](auto type, auto t) {
+    const dim3 grid((rows + 15) / 16, (all + 16 * t() - 1) / (16 * t()));
+    adapter_shrink_kernel<type(), t()><<<grid, 64 * kShrinkWaves, 0, stream>>>(a);
+  };
+  auto expand = [&](auto type, auto ks) {
+    const dim3 grid((rows + kExpandRows - 1) / kExpandRows,
+                    (expand_units(a.end, a.njobs) + kThreads / 64 - 1) / (kThreads / 64));
+    adapter_expand_kernel<type(), ks()><<<grid, kThreads, 0, stream>>>(a);
+  };
   auto go = [&](auto type) {
-    const dim3 first(a.seq.rows, (a.njobs * a.rank + 3) / 4);
-    adapter_shrink_kernel<type()><<<first, kThreads, 0, stream>>>(a);
-    const dim3 grid(a.seq.rows, (a.end[a.njobs - 1] + kThreads - 1) / kThreads);
-    adapter_expand_kernel<type()><<<grid, kThreads, 0, stream>>>(a);
+    using std::integral_constant;
+    if (a.seq.max_rows <= kFewRows) return by_row(type);
+    const int tiles = (all + 15) / 16;
+    tiles == 1   ? shrink(type, integral_constant<int, 1>())
+    : tiles == 2 ? shrink(type, integral_constant<int, 2>())
+    : tiles == 3 ? shrink(type, integral_constant<int, 3>())
+                 : shrink(type, integral_constant<int, kMostT>());
+    a.rank <= 32   ? expand(type, integral_constant<int, 1>())
+    : a.rank <= 64 ? expand(type, integral_constant<int, 2>())
+                   : expand(type, integral_constant<int, 4>());
   };
   a.type == kAdapterF32    ? go(std::integral_constant<int, kAdapterF32>())
   : a.type == kAdapterBf16 ? go(std::integral_constant<int, kAdapterBf16>())

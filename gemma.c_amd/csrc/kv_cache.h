@@ -103,23 +103,33 @@ __device__ __forceinline__ int kv_find_wave(const KvBatch &b, int r) {
 #endif
 
 #ifdef __HIPCC__
-// Where row r lies: sequence i, its position (rows behind their sequences' starts have negative
-// ones); i -1: in none.  By a whole wave, for one row: one load for up to 63 sequences, two for
-// up to 3969 and so on, their lengths' among them.
+// Rows' sequences are looked for by a whole wave, 63 of them at a step: a load for up to 63
+// sequences, another for up to 3969 and so on.  *n: among how many (63 at most) from the
+// returned one on the row's is.
+__device__ __forceinline__ int kv_find_part(const KvBatch &b, int r, int *n) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, left = b.batch;
+  while (left > 63) {
+    const int step = (left + 62) / 63, at = lane * step;
+    const int before = __popcll(__ballot(at < left && b.row0[lo + (at < left ? at : 0)] <= r));
+    const int skip = (before > 0 ? before - 1 : 0) * step;
+    lo += skip;
+    left = left - skip < step ? left - skip : step;
+  }
+  *n = left;
+  return lo;
+}
+
+// Where row r lies: sequence i, its position (negative for the first rows of a sequence that is
+// shorter than its rows); i -1: in none.  By a whole wave, for one row.
 struct KvRow {
   int i, pos;
 };
 template <bool POS>
 __device__ __forceinline__ KvRow kv_row_wave(const KvBatch &b, int r) {
   const int lane = threadIdx.x & 63;
-  int lo = 0, n = b.batch;  // it is one of lo .. lo + n - 1
-  while (n > 63) {
-    const int step = (n + 62) / 63, at = lane * step;
-    const int before = __popcll(__ballot(at < n && b.row0[lo + (at < n ? at : 0)] <= r));
-    const int skip = (before > 0 ? before - 1 : 0) * step;
-    lo += skip;
-    n = n - skip < step ? n - skip : step;
-  }
+  int n;
+  const int lo = kv_find_part(b, r, &n);
   const int at = lo + (lane < n ? lane : n);  // row0[lo + n] is there too
   const int first = b.row0[at];
   const int len = POS ? b.len[at < b.batch ? at : b.batch - 1] : 0;

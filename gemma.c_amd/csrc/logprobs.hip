@@ -186,13 +186,15 @@ struct TopShared {
 };
 
 // The n largest of the threads' keys (no two alike but 0), in order, 0 where there are fewer,
-// into sh.best: threads' largest are ranked, those that reach the n-th of them are listed, and
-// the list is ranked.  A thread that reaches it has `per` keys at most, and n threads do.
-template <class K>
-__device__ void top_of(TopShared &sh, int n, int per, K &&key) {
+// into sh.best: threads' largest are ranked, those of the n threads with the largest ones are
+// listed, and the list is ranked.
+template <int PER>
+__device__ __forceinline__ void top_of(TopShared &sh, int n, const u64 (&keys)[PER]) {
+  static_assert(PER <= kKeys, "the list holds n threads' keys");
   const int tid = threadIdx.x;
   u64 most = 0;
-  for (int j = 0; j < per; ++j) most = max(most, key(j));
+#pragma unroll
+  for (int j = 0; j < PER; ++j) most = max(most, keys[j]);
   __syncthreads();
   sh.most[tid] = most;
   if (tid < n) sh.best[tid] = 0;
@@ -201,10 +203,9 @@ __device__ void top_of(TopShared &sh, int n, int per, K &&key) {
   int above = 0;
   for (int j = 0; j < kThreads; ++j) above += sh.most[j] > most;
   if (most != 0 && above < n)
-    for (int j = 0; j < per; ++j) {
-      const u64 k = key(j);
-      if (k != 0) sh.list[atomicAdd(&sh.count, 1)] = k;
-    }
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (keys[j] != 0) sh.list[atomicAdd(&sh.count, 1)] = keys[j];
   __syncthreads();
   const int count = sh.count;
   for (int i = tid; i < count; i += kThreads) {
@@ -216,6 +217,8 @@ __device__ void top_of(TopShared &sh, int n, int per, K &&key) {
   __syncthreads();
 }
 
+// RUNS: of a thread, at most
+template <int RUNS>
 __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(Logprobs a, Layout at) {
   __shared__ TopShared sh;
   __shared__ double red[kThreads / 64];
@@ -226,6 +229,16 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(Logprobs a, Lay
   const float temp = a.temperature != nullptr ? a.temperature[r] : 1.0f;
   const bool drawn = temp > 0.0f;
   const double c = drawn ? fmin(0x1.71547652b82fep+0 / (double)temp, (double)FLT_MAX) : 0.0;
+  // the runs are asked for first, as they come last
+  const float *runs = reinterpret_cast<const float *>(a.work + at.runs) +
+                      (size_t)r * tiles * kTileRuns;
+  const int nruns = a.ntop > 0 ? (a.vocab + kRun - 1) / kRun : 0;
+  float most[RUNS];
+#pragma unroll
+  for (int j = 0; j < RUNS; ++j) {
+    const int i = tid + j * kThreads;
+    most[j] = i < nruns ? runs[i] : 0.0f;
+  }
   const bool in = tid < tiles;  // one part a thread
   static_assert(kMaxTiles <= kThreads, "a thread a part");
   const Part p = in ? parts[tid] : Part{-INFINITY, 0.0f, 0.0f};
@@ -263,30 +276,24 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(Logprobs a, Lay
     if (a.logp != nullptr) a.logp[to] = there ? logp(no_nan(row[id]), above == 0) : -INFINITY;
   }
   if (a.ntop == 0) return;
-  const float *runs = reinterpret_cast<const float *>(a.work + at.runs) +
-                      (size_t)r * tiles * kTileRuns;
-  const int nruns = (a.vocab + kRun - 1) / kRun;
-  top_of(sh, a.ntop, (nruns + kThreads - 1) / kThreads, [&](int j) -> u64 {
+  u64 keys[RUNS];
+#pragma unroll
+  for (int j = 0; j < RUNS; ++j) {
     const int i = tid + j * kThreads;
-    return i < nruns ? key_of(runs[i], i) : 0;
-  });
-  // a wave a run: its columns in their threads' keys
-  u64 mine[kLogprobsMaxTop / (kThreads / 64)];
-  const int per = (a.ntop + kThreads / 64 - 1) / (kThreads / 64);
-#pragma unroll
-  for (int j = 0; j < kLogprobsMaxTop / (kThreads / 64); ++j) {
-    mine[j] = 0;
-    const int i = j * (kThreads / 64) + tid / 64;
-    if (i >= a.ntop || sh.best[i] == 0) continue;
-    const int col = index_of(sh.best[i]) * kRun + (tid & 63);
-    if (col < a.vocab) mine[j] = key_of(row[col], col);
+    keys[j] = i < nruns ? key_of(most[j], i) : 0;
   }
-  top_of(sh, a.ntop, per, [&](int j) -> u64 {
-    u64 k = 0;
+  top_of(sh, a.ntop, keys);
+  // a wave a run: its columns are the threads' keys
+  constexpr int WAVES = kThreads / 64;
+  u64 mine[kLogprobsMaxTop / WAVES];
 #pragma unroll
-    for (int i = 0; i < kLogprobsMaxTop / (kThreads / 64); ++i) k = i == j ? mine[i] : k;
-    return k;
-  });
+  for (int j = 0; j < kLogprobsMaxTop / WAVES; ++j) {
+    const int i = j * WAVES + tid / 64;
+    const u64 run = i < a.ntop ? sh.best[i] : 0;
+    const int col = index_of(run) * kRun + (tid & 63);
+    mine[j] = run != 0 && col < a.vocab ? key_of(row[col], col) : 0;
+  }
+  top_of(sh, a.ntop, mine);
   if (tid < a.ntop) {
     const u64 k = sh.best[tid];
     const size_t to = (size_t)r * a.ntop + tid;
@@ -308,7 +315,12 @@ hipError_t launch_logprobs(const Logprobs &a, hipStream_t stream) {
   const unsigned grid = (unsigned)((units + 3) / 4);
   a.ntop > 0 ? logprobs_scan_kernel<true><<<grid, kThreads, 0, stream>>>(a, at)
              : logprobs_scan_kernel<false><<<grid, kThreads, 0, stream>>>(a, at);
-  logprobs_join_kernel<<<a.rows, kThreads, 0, stream>>>(a, at);
+  const auto join = [&](auto runs) {
+    logprobs_join_kernel<runs()><<<a.rows, kThreads, 0, stream>>>(a, at);
+  };
+  a.vocab <= 4 * kThreads * kRun    ? join(std::integral_constant<int, 4>())
+  : a.vocab <= 16 * kThreads * kRun ? join(std::integral_constant<int, 16>())
+                                    : join(std::integral_constant<int, kKeys>());
   return hipGetLastError();
 }
 
