@@ -14,7 +14,6 @@
 #include <float.h>
 #include <type_traits>
 
-#include "dec_common.h"
 #include "gh_arith.h"
 #include "gh_kernels.h"
 
@@ -177,59 +176,124 @@ __device__ __forceinline__ float logit_of(u64 key) {
   return __uint_as_float(up & 0x80000000u ? up & 0x7fffffffu : ~up);
 }
 
+constexpr int kWaves = kThreads / 64;
 constexpr int kKeys = kMost / kThreads;  // of a thread, at most
-struct TopShared {
+constexpr int kListed = kKeys * kLogprobsMaxTop;
+struct JoinShared {
   u64 most[kThreads];
-  u64 list[kKeys * kLogprobsMaxTop];
+  u64 list[kListed];
   u64 best[kLogprobsMaxTop];
+  double logs;
+  float top;
   int count;
+  int above[kLogprobsMaxTargets];
+  float given[kLogprobsMaxTargets];
 };
 
-// The n largest of the threads' keys (no two alike but 0), in order, 0 where there are fewer,
-// into sh.best: threads' largest are ranked, those of the n threads with the largest ones are
-// listed, and the list is ranked.
+// How many of n keys in LDS are above `mine`; sixteen are asked for at a time.
+__device__ __forceinline__ int above_in(const u64 *keys, int n, u64 mine) {
+  int above = 0, j = 0;
+  for (; j + 16 <= n; j += 16)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) above += keys[j + i] > mine;
+  for (; j < n; ++j) above += keys[j] > mine;
+  return above;
+}
+
+// Keys (no two alike but 0) of all threads into sh.list, their number into sh.count: the n largest
+// at least (all but 0 where there are fewer), and not many more.  Every wave looks for a bound that
+// n threads' largest keys reach, or a few more, bit by bit from the highest, and what reaches it is
+// listed: at most 64 threads' keys.
 template <int PER>
-__device__ __forceinline__ void top_of(TopShared &sh, int n, const u64 (&keys)[PER]) {
-  static_assert(PER <= kKeys, "the list holds n threads' keys");
+__device__ __forceinline__ void list_largest(JoinShared &sh, int n, const u64 (&keys)[PER]) {
+  static_assert(PER <= kKeys && kListed >= kLogprobsMaxTop * PER, "the list holds 64 threads' keys");
   const int tid = threadIdx.x;
   u64 most = 0;
 #pragma unroll
   for (int j = 0; j < PER; ++j) most = max(most, keys[j]);
-  __syncthreads();
   sh.most[tid] = most;
-  if (tid < n) sh.best[tid] = 0;
   if (tid == 0) sh.count = 0;
   __syncthreads();
-  int above = 0;
-  for (int j = 0; j < kThreads; ++j) above += sh.most[j] > most;
-  if (most != 0 && above < n)
+  const int enough = min(n + 8, kLogprobsMaxTop);
+  u64 other[kWaves], least = 0;
+#pragma unroll
+  for (int j = 0; j < kWaves; ++j) other[j] = sh.most[(tid & 63) + 64 * j];
+  for (int bit = 63; bit >= 0; --bit) {
+    const u64 next = least | 1ull << bit;
+    int reach = 0;
+#pragma unroll
+    for (int j = 0; j < kWaves; ++j) reach += __popcll(__ballot(other[j] >= next));
+    if (reach < n) continue;
+    least = next;
+    if (reach <= enough) break;
+  }
+  if (least == 0) least = 1;  // fewer than n
+  if (most >= least) {
+    int mine = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) mine += keys[j] >= least;
+    int at = atomicAdd(&sh.count, mine);
 #pragma unroll
     for (int j = 0; j < PER; ++j)
-      if (keys[j] != 0) sh.list[atomicAdd(&sh.count, 1)] = keys[j];
-  __syncthreads();
-  const int count = sh.count;
-  for (int i = tid; i < count; i += kThreads) {
-    const u64 mine = sh.list[i];
-    int rank = 0;
-    for (int j = 0; j < count; ++j) rank += sh.list[j] > mine;
-    if (rank < n) sh.best[rank] = mine;
+      if (keys[j] >= least) sh.list[at++] = keys[j];
   }
   __syncthreads();
 }
 
-// RUNS: of a thread, at most
+// The list's n largest, in order, into sh.best, 0 where there are fewer.
+__device__ __forceinline__ void rank_list(JoinShared &sh, int n) {
+  const int count = sh.count;
+  for (int i = threadIdx.x; i < count; i += kThreads) {
+    const u64 mine = sh.list[i];
+    const int rank = above_in(sh.list, count, mine);
+    if (rank < n) sh.best[rank] = mine;
+  }
+  if ((int)threadIdx.x >= count && (int)threadIdx.x < n) sh.best[threadIdx.x] = 0;
+  __syncthreads();
+}
+
+// S and T of the row's parts by its largest logit, by one wave.
+__device__ __forceinline__ void join_parts(JoinShared &sh, const Part *parts, int tiles, bool drawn,
+                                           double c, float *entropy) {
+  constexpr int kPer = kMaxTiles / 64;
+  static_assert(kMaxTiles % 64 == 0, "a lane has so many parts");
+  const int lane = threadIdx.x & 63;
+  Part p[kPer];
+  float top = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const int i = lane + 64 * j;
+    p[j] = i < tiles ? parts[i] : Part{-INFINITY, 0.0f, 0.0f};
+    top = fmaxf(top, p[j].m);
+  }
+  top = wave_max_dpp(top);
+  double s = 0.0, t = 0.0;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    if (!(p[j].m > -INFINITY)) continue;
+    const double x = top == p[j].m ? 0.0 : ((double)p[j].m - (double)top) * c;  // (-inf below +inf)
+    const double w = x > -1000.0 ? exp2(x) : 0.0;
+    s = fma(w, (double)p[j].s, s);
+    t += w > 0.0 ? w * ((double)p[j].t + (double)p[j].s * x) : 0.0;
+  }
+  s = wave_sum_f64(s);
+  t = wave_sum_f64(t);
+  const double ln2 = 0x1.62e42fefa39efp-1, logs = log(s);
+  if (lane != 0) return;
+  sh.top = top;
+  sh.logs = logs;
+  if (entropy != nullptr)
+    *entropy = drawn && top > -INFINITY ? (float)fmax(0.0, logs - ln2 * t / s) : 0.0f;
+}
+
+// RUNS: of a thread, at most.  Most of a row's join is waiting: everything that doesn't hang on
+// something else is asked for at once, the parts are one wave's, the given tokens the others'.
 template <int RUNS>
 __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(Logprobs a, Layout at) {
-  __shared__ TopShared sh;
-  __shared__ double red[kThreads / 64];
-  __shared__ float redf[kThreads / 64];
-  const int r = blockIdx.x, tid = threadIdx.x, tiles = tiles_of(a.vocab);
+  __shared__ JoinShared sh;
+  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, tiles = tiles_of(a.vocab);
+  const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const float *row = a.logits + r * a.stride;
-  const Part *parts = reinterpret_cast<const Part *>(a.work + at.parts) + (size_t)r * tiles;
-  const float temp = a.temperature != nullptr ? a.temperature[r] : 1.0f;
-  const bool drawn = temp > 0.0f;
-  const double c = drawn ? fmin(0x1.71547652b82fep+0 / (double)temp, (double)FLT_MAX) : 0.0;
-  // the runs are asked for first, as they come last
   const float *runs = reinterpret_cast<const float *>(a.work + at.runs) +
                       (size_t)r * tiles * kTileRuns;
   const int nruns = a.ntop > 0 ? (a.vocab + kRun - 1) / kRun : 0;
@@ -237,22 +301,37 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(Logprobs a, Lay
 #pragma unroll
   for (int j = 0; j < RUNS; ++j) {
     const int i = tid + j * kThreads;
-    most[j] = i < nruns ? runs[i] : 0.0f;
+    most[j] = i < nruns ? runs[i] : -INFINITY;
   }
-  const bool in = tid < tiles;  // one part a thread
-  static_assert(kMaxTiles <= kThreads, "a thread a part");
-  const Part p = in ? parts[tid] : Part{-INFINITY, 0.0f, 0.0f};
-  const float top = block_max<kThreads>(p.m, redf);
-  double s = 0.0, t = 0.0;
-  if (p.m > -INFINITY) {
-    const double x = top == p.m ? 0.0 : ((double)p.m - (double)top) * c;  // (-inf below +inf)
-    const double w = x > -1000.0 ? exp2(x) : 0.0;
-    s = w * (double)p.s;
-    t = w > 0.0 ? w * ((double)p.t + (double)p.s * x) : 0.0;
+  const float temp = a.temperature != nullptr ? a.temperature[r] : 1.0f;
+  const bool drawn = temp > 0.0f;
+  if (wave == kWaves - 1) {
+    const double c = drawn ? fmin(0x1.71547652b82fep+0 / (double)temp, (double)FLT_MAX) : 0.0;
+    join_parts(sh, reinterpret_cast<const Part *>(a.work + at.parts) + (size_t)r * tiles, tiles,
+               drawn, c, a.entropy != nullptr ? a.entropy + r : nullptr);
+  } else {
+    const int *counts = reinterpret_cast<const int *>(a.work + at.counts) +
+                        (size_t)r * tiles * a.targets;
+    for (int k = wave; k < a.targets; k += kWaves - 1) {
+      const int id = a.ids[(size_t)r * a.targets + k];
+      const bool there = (unsigned)id < (unsigned)a.vocab;
+      const float given = there ? no_nan(row[id]) : -INFINITY;
+      int above = 0;
+      for (int j = lane; j < tiles; j += 64) above += counts[(size_t)j * a.targets + k];
+      above = group_sum_i32<64>(above);
+      if (lane == 0) sh.above[k] = there ? above : -1, sh.given[k] = given;
+    }
   }
-  s = block_sum<kThreads>(s, red);
-  t = block_sum<kThreads>(t, red);
-  const double ln2 = 0x1.62e42fefa39efp-1, logs = log(s);
+  if (a.ntop > 0) {
+    u64 keys[RUNS];
+#pragma unroll
+    for (int j = 0; j < RUNS; ++j) keys[j] = key_of(most[j], tid + j * kThreads);
+    list_largest(sh, a.ntop, keys);
+  } else {
+    __syncthreads();
+  }
+  const float top = sh.top;
+  const double logs = sh.logs;
   // log p of a logit that isn't NaN; first: whether it is the row's first largest
   auto logp = [&](float l, bool first) -> float {
     if (!(l > -INFINITY)) return -INFINITY;
@@ -260,40 +339,34 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(Logprobs a, Lay
     if (l == top) return (float)(0.0 - logs);
     return (float)(((double)l - (double)top) / (double)temp - logs);
   };
-  if (tid == 0 && a.entropy != nullptr)
-    a.entropy[r] = drawn && top > -INFINITY ? (float)fmax(0.0, logs - ln2 * t / s) : 0.0f;
-  const int *counts = reinterpret_cast<const int *>(a.work + at.counts) +
-                      (size_t)r * tiles * a.targets;
-  for (int k = tid / 64; k < a.targets; k += kThreads / 64) {  // a wave a token
-    int above = 0;
-    for (int j = tid & 63; j < tiles; j += 64) above += counts[(size_t)j * a.targets + k];
-    above = group_sum_i32<64>(above);
-    if ((tid & 63) != 0) continue;
-    const size_t to = (size_t)r * a.targets + k;
-    const int id = a.ids[to];
-    const bool there = (unsigned)id < (unsigned)a.vocab;
-    if (a.rank != nullptr) a.rank[to] = there ? above + 1 : 0;
-    if (a.logp != nullptr) a.logp[to] = there ? logp(no_nan(row[id]), above == 0) : -INFINITY;
+  if (tid < a.targets) {
+    const size_t to = (size_t)r * a.targets + tid;
+    const int above = sh.above[tid];
+    if (a.rank != nullptr) a.rank[to] = above + 1;
+    if (a.logp != nullptr) a.logp[to] = logp(sh.given[tid], above == 0);
   }
   if (a.ntop == 0) return;
-  u64 keys[RUNS];
-#pragma unroll
-  for (int j = 0; j < RUNS; ++j) {
-    const int i = tid + j * kThreads;
-    keys[j] = i < nruns ? key_of(most[j], i) : 0;
-  }
-  top_of(sh, a.ntop, keys);
+  // the runs that matter, as they were listed unless they are too many
+  const bool few = sh.count <= kLogprobsMaxTop;
+  if (!few) rank_list(sh, a.ntop);
+  const int chosen = few ? sh.count : a.ntop;
   // a wave a run: its columns are the threads' keys
-  constexpr int WAVES = kThreads / 64;
-  u64 mine[kLogprobsMaxTop / WAVES];
+  float l[kLogprobsMaxTop / kWaves];
+  int col[kLogprobsMaxTop / kWaves];
 #pragma unroll
-  for (int j = 0; j < kLogprobsMaxTop / WAVES; ++j) {
-    const int i = j * WAVES + tid / 64;
-    const u64 run = i < a.ntop ? sh.best[i] : 0;
-    const int col = index_of(run) * kRun + (tid & 63);
-    mine[j] = run != 0 && col < a.vocab ? key_of(row[col], col) : 0;
+  for (int j = 0; j < kLogprobsMaxTop / kWaves; ++j) {
+    const int i = j * kWaves + wave;
+    l[j] = -INFINITY, col[j] = 0;
+    if (i >= chosen) continue;
+    col[j] = index_of(few ? sh.list[i] : sh.best[i]) * kRun + lane;
+    if (col[j] < a.vocab) l[j] = row[col[j]];
   }
-  top_of(sh, a.ntop, mine);
+  u64 mine[kLogprobsMaxTop / kWaves];
+#pragma unroll
+  for (int j = 0; j < kLogprobsMaxTop / kWaves; ++j) mine[j] = key_of(l[j], col[j]);
+  __syncthreads();
+  list_largest(sh, a.ntop, mine);
+  rank_list(sh, a.ntop);
   if (tid < a.ntop) {
     const u64 k = sh.best[tid];
     const size_t to = (size_t)r * a.ntop + tid;
