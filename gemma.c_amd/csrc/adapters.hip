@@ -116,12 +116,13 @@ __device__ __forceinline__ float scale_of(const Adapters &a, int id) {
   return a.scale != nullptr ? a.scale[id] : 1.0f;
 }
 
-// The workspace: u [rows][jobs * rank], then the rows' ids.
+// The workspace: u [rows][jobs * rank] as fp32 or, of tiles, [rows][3][jobs * rank] in bf16
+// pieces, then the rows' ids.
 __device__ __forceinline__ float *u_of(const Adapters &a) {
   return reinterpret_cast<float *>(a.work);
 }
 __device__ __forceinline__ int *ids_of(const Adapters &a) {
-  return reinterpret_cast<int *>(a.work + (size_t)a.seq.rows * a.njobs * a.rank * 4);
+  return reinterpret_cast<int *>(a.work + (size_t)a.seq.rows * a.njobs * a.rank * 6);
 }
 
 // ---- single tokens ----------------------------------------------------------------
@@ -191,34 +192,52 @@ __global__ __launch_bounds__(kThreads) void adapter_expand_row_kernel(Adapters a
 __device__ __forceinline__ int ids_of_rows(const Adapters &a, int first, int row) {
   const KvBatch &b = a.seq;
   const int lane = threadIdx.x & 63, last = first + 15;
-  int i, n;
-  const int lo = i = kv_find_part(b, first, &n);
-  for (int from = lo + 1; from < b.batch; from += 64) {
-    const int begins = b.row0[from + lane < b.batch ? from + lane : b.batch];
-    int j = 0;
-    for (; j < 64 && from + j < b.batch; ++j) {
-      const int at = __builtin_amdgcn_readlane(begins, j);
-      if (at > last) break;
-      i += at <= row;
+  int i, id, r0, next;
+  if (b.batch < 64) {  // a trip to memory
+    const int begins = b.row0[min(lane, b.batch)];
+    const int all = a.ids[min(lane, b.batch - 1)];
+    const unsigned long long in = ~0ull >> (64 - b.batch);
+    const int from = __popcll(__ballot(begins <= first) & in);
+    const int to = __popcll(__ballot(begins <= last) & in);
+    i = max(from - 1, 0);
+    for (int j = max(from, 1); j < to; ++j) i += __builtin_amdgcn_readlane(begins, j) <= row;
+    r0 = __shfl(begins, i, 64), next = __shfl(begins, i + 1, 64), id = __shfl(all, i, 64);
+  } else {
+    int n;
+    const int lo = i = kv_find_part(b, first, &n);
+    for (int from = lo + 1; from < b.batch; from += 64) {
+      const int begins = b.row0[from + lane < b.batch ? from + lane : b.batch];
+      int j = 0;
+      for (; j < 64 && from + j < b.batch; ++j) {
+        const int at = __builtin_amdgcn_readlane(begins, j);
+        if (at > last) break;
+        i += at <= row;
+      }
+      if (j < 64) break;
     }
-    if (j < 64) break;
+    r0 = b.row0[i], next = b.row0[i + 1], id = a.ids[i];
   }
-  const int r0 = kv_clamp(b.row0[i], 0, b.rows);
-  int rows = kv_clamp(b.row0[i + 1], r0, b.rows) - r0;
+  r0 = kv_clamp(r0, 0, b.rows);
+  int rows = kv_clamp(next, r0, b.rows) - r0;
   if (rows > b.max_rows) rows = b.max_rows;
   if (row < r0 || row - r0 >= rows) return kOutside;
-  const int id = a.ids[i];
   return (unsigned)id < (unsigned)a.count ? id : kNone;
 }
 
+// Piece p of u of a row in the workspace.
+__device__ __forceinline__ uint16_t *piece_of(const Adapters &a, int row, int p) {
+  return reinterpret_cast<uint16_t *>(a.work) + ((size_t)row * 3 + p) * (a.njobs * a.rank);
+}
+
 constexpr int kShrinkWaves = 8;  // that share a tile's inputs
-constexpr int kMostT = 4;        // 16 values of u each: a workgroup's, at most
+constexpr int kShrinkSteps = 5;  // whose loads are in flight together
+constexpr int kMostT = 3;        // 16 values of u each: a workgroup's, at most
 
 // u of 16 rows and 16 T of their values; each wave takes every eighth step of 32 inputs, the
-// partial sums meet in LDS
+// partial sums meet in LDS.  Steps behind the last are done with zeros: a branch around them would
+// take the loads with it, one after the other.
 template <int TYPE, int T>
 __global__ __launch_bounds__(64 * kShrinkWaves) void adapter_shrink_kernel(Adapters a) {
-  constexpr int kSteps = TYPE == kAdapterF32 ? 2 : 4;  // whose loads are in flight together
   __shared__ v4f part[kShrinkWaves][T][64];
   const int all = a.njobs * a.rank, lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -246,11 +265,11 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void adapter_shrink_kernel(Adapt
     v4f acc[T];
 #pragma unroll
     for (int t = 0; t < T; ++t) acc[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s0 = wave; s0 < steps; s0 += kShrinkWaves * kSteps) {
-      v4f xs[kSteps][2];
-      Raw8<TYPE> ws[kSteps][T];
+    for (int s0 = wave; s0 < steps; s0 += kShrinkWaves * kShrinkSteps) {
+      v4f xs[kShrinkSteps][2];
+      Raw8<TYPE> ws[kShrinkSteps][T];
 #pragma unroll
-      for (int j = 0; j < kSteps; ++j) {
+      for (int j = 0; j < kShrinkSteps; ++j) {
         int k = 32 * (s0 + j * kShrinkWaves) + k0;
         k = k < a.k ? k : 0;
         xs[j][0] = *reinterpret_cast<const v4f *>(x + k);
@@ -259,10 +278,8 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void adapter_shrink_kernel(Adapt
         for (int t = 0; t < T; ++t) ws[j][t] = raw8<TYPE>(m[t], skip + from[t] + k);
       }
 #pragma unroll
-      for (int j = 0; j < kSteps; ++j) {
-        const int s = s0 + j * kShrinkWaves;
-        if (s >= steps) break;
-        const bool in = 32 * s + k0 < a.k;  // all but the last step's last lanes are
+      for (int j = 0; j < kShrinkSteps; ++j) {
+        const bool in = 32 * (s0 + j * kShrinkWaves) + k0 < a.k;
         float f[8];
 #pragma unroll
         for (int e = 0; e < 4; ++e) f[e] = in ? xs[j][0][e] : 0.0f, f[e + 4] = in ? xs[j][1][e] : 0.0f;
@@ -285,107 +302,121 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void adapter_shrink_kernel(Adapt
       for (int w = 1; w < kShrinkWaves; ++w) sum += part[w][wave][lane];
       const int at = at0 + 16 * wave + 4 * (lane / 16);
       if (id == cur && there && at < all) {
-        const float sc = scale_of(a, cur);
-        *reinterpret_cast<v4f *>(u_of(a) + (size_t)row * all + at) = sum * sc;
+        sum *= scale_of(a, cur);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+          const u2 b = {cvt_pk_bf16(sum[0], sum[1]), cvt_pk_bf16(sum[2], sum[3])};
+          *reinterpret_cast<u2 *>(piece_of(a, row, p) + at) = b;
+          sum -= v4f{bf16_lo(b[0]), bf16_hi(b[0]), bf16_lo(b[1]), bf16_hi(b[1])};
+        }
       }
     }
     __syncthreads();
   }
 }
 
-constexpr int kExpandRows = 32;  // of a wave
-constexpr int kExpandGroups = 2; // of 64 columns: a wave's
+constexpr int kExpandCols = 64;                // of a wave
+constexpr int kExpandPitch = kExpandCols + 4;  // 16 rows' chunks of four in different banks
 
 __host__ __device__ inline int expand_units(const int (&end)[kAdapterMaxJobs], int njobs) {
   int n = 0;
   for (int j = 0; j < njobs; ++j) {
     const int w = end[j] - (j == 0 ? 0 : end[j - 1]);
-    n += (w + 64 * kExpandGroups - 1) / (64 * kExpandGroups);
+    n += (w + kExpandCols - 1) / kExpandCols;
   }
   return n;
 }
 
-// dst of 32 rows and 128 columns of a job a wave; KS: steps of 32 of the rank
-template <int TYPE, int KS>
-__global__ __launch_bounds__(kThreads) void adapter_expand_kernel(Adapters a) {
-  constexpr int RT = kExpandRows / 16;
-  const int lane = threadIdx.x & 63, all = a.njobs * a.rank;
-  int unit = blockIdx.y * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+// dst of 16 RT rows and 64 columns of a job a wave; KS: steps of 32 of the rank.  base and dst are
+// read and written by whole runs of 256 bytes; the products, whose lanes have a row each, go through
+// LDS.
+template <int TYPE, int KS, int RT>
+__global__ __launch_bounds__(kThreads, KS == 1 ? 4 : 3) void adapter_expand_kernel(Adapters a) {
+  __shared__ float tiles[kThreads / 64][16 * RT][kExpandPitch];
+  const int lane = threadIdx.x & 63, m = lane & 15, quarter = lane / 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  int unit = blockIdx.y * (kThreads / 64) + wave;
   int job = 0, begin = 0, width = a.end[0];
   for (; job < a.njobs; ++job) {
     begin = job == 0 ? 0 : a.end[job - 1];
     width = a.end[job] - begin;
-    const int units = (width + 64 * kExpandGroups - 1) / (64 * kExpandGroups);
+    const int units = (width + kExpandCols - 1) / kExpandCols;
     if (unit < units) break;
     unit -= units;
   }
   if (job == a.njobs) return;
-  const void *m = job_of(a.b, job);
-  const int k0 = 8 * (lane / 16);
-  int row[RT], id[RT];
+  float(&tile)[16 * RT][kExpandPitch] = tiles[wave];
+  const void *b = job_of(a.b, job);
+  const int k0 = 8 * quarter, c0 = unit * kExpandCols, row0 = 16 * RT * blockIdx.x;
+  int id[RT];
   Split8<3> u[RT][KS];
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    const int row = min(row0 + 16 * i + m, a.seq.rows - 1);
+    id[i] = ids_of(a)[row];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int k = 32 * s + k0;
+#pragma unroll
+      for (int p = 0; p < 3; ++p)
+        u[i][s].p[p] = *reinterpret_cast<const u4 *>(piece_of(a, row, p) + job * a.rank +
+                                                     (k < a.rank ? k : 0));
+    }
+  }
+  // rows 4 j + quarter, four columns of them from the lane's 4 m
+  const int left = width - c0 - 4 * m;
+  const size_t col = begin + c0 + 4 * m;
+  const bool whole = c0 + kExpandCols <= width;
+  v4f old[4 * RT];
+  if (whole) {
+#pragma unroll
+    for (int j = 0; j < 4 * RT; ++j) {
+      const int row = min(row0 + 4 * j + quarter, a.seq.rows - 1);
+      old[j] = *reinterpret_cast<const v4f_any *>(a.base + row * a.base_stride + col);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4 * RT; ++j) {
+      const int row = min(row0 + 4 * j + quarter, a.seq.rows - 1);
+      old[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < left) old[j][e] = a.base[row * a.base_stride + col + e];
+    }
+  }
   unsigned long long todo = 0;
 #pragma unroll
   for (int i = 0; i < RT; ++i) {
-    row[i] = kExpandRows * blockIdx.x + 16 * i + (lane & 15);
-    id[i] = row[i] < a.seq.rows ? ids_of(a)[row[i]] : kOutside;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      float f[8] = {};
-      if (id[i] >= 0 && 32 * s + k0 < a.rank) {
-        const float *p = u_of(a) + (size_t)row[i] * all + job * a.rank + 32 * s + k0;
-        const v4f lo = *reinterpret_cast<const v4f *>(p);
-        const v4f hi = *reinterpret_cast<const v4f *>(p + 4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f[e] = lo[e], f[e + 4] = hi[e];
-      }
-      u[i][s] = split8<3>(f);
-    }
+    if (row0 + 16 * i + m >= a.seq.rows) id[i] = kOutside;
     todo |= (__ballot(id[i] >= 0) & 0xffffull) << (16 * i);
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (auto &v : u[i][s].p) v = 32 * s + k0 < a.rank ? v : u4{0, 0, 0, 0};
   }
-  for (int g = 0; g < kExpandGroups; ++g) {
-    const int c0 = (unit * kExpandGroups + g) * 64;
-    if (c0 >= width) break;
-    v4f old[4][RT], sum[4][RT];
-    int col[4];  // the first of the lane's four, of the job's
+  while (todo != 0) {
+    const int at = __builtin_ctzll(todo);
+    int cur = __builtin_amdgcn_readlane(id[0], at & 15);
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      col[t] = c0 + 16 * t + 4 * (lane / 16);
-#pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        sum[t][i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-        old[t][i] = sum[t][i];
-        if (id[i] == kOutside) continue;
-        const float *p = a.base + row[i] * a.base_stride + begin + col[t];
-        if (col[t] + 4 <= width)
-          old[t][i] = *reinterpret_cast<const v4f_any *>(p);
-        else
-          for (int e = 0; e < 4; ++e)
-            if (col[t] + e < width) old[t][i][e] = p[e];
-      }
+    for (int i = 1; i < RT; ++i) {
+      const int other = __builtin_amdgcn_readlane(id[i], at & 15);
+      cur = at / 16 == i ? other : cur;
     }
-    for (unsigned long long left = todo; left != 0;) {
-      const int at = __builtin_ctzll(left);
-      int cur = __builtin_amdgcn_readlane(id[0], at & 15);
 #pragma unroll
-      for (int i = 1; i < RT; ++i) {
-        const int other = __builtin_amdgcn_readlane(id[i], at & 15);
-        cur = at / 16 == i ? other : cur;
-      }
+    for (int i = 0; i < RT; ++i) todo &= ~((__ballot(id[i] == cur) & 0xffffull) << (16 * i));
+    constexpr int W = KS < 4 && (KS == 1 || TYPE != kAdapterF32) ? 4 : 2;  // read together
 #pragma unroll
-      for (int i = 0; i < RT; ++i)
-        left &= ~((__ballot(id[i] == cur) & 0xffffull) << (16 * i));
-      Raw8<TYPE> w[4][KS];
+    for (int t0 = 0; t0 < 4; t0 += W) {
+      Raw8<TYPE> w[W][KS];
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+      for (int t = 0; t < W; ++t)
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-          const int c = min(c0 + 16 * t + (lane & 15), width - 1);
-          const int k = 32 * s + k0;
-          w[t][s] = raw8<TYPE>(m, ((size_t)cur * width + c) * a.rank + (k < a.rank ? k : 0));
+          const int c = min(c0 + 16 * (t0 + t) + m, width - 1), k = 32 * s + k0;
+          w[t][s] = raw8<TYPE>(b, ((size_t)cur * width + c) * a.rank + (k < a.rank ? k : 0));
         }
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
+      for (int t = 0; t < W; ++t) {
         v4f d[RT] = {};
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
@@ -398,23 +429,29 @@ __global__ __launch_bounds__(kThreads) void adapter_expand_kernel(Adapters a) {
         }
 #pragma unroll
         for (int i = 0; i < RT; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sum[t][i][e] = id[i] == cur ? d[i][e] : sum[t][i][e];
+          if (id[i] == cur)
+            *reinterpret_cast<v4f *>(&tile[16 * i + m][16 * (t0 + t) + 4 * quarter]) = d[i];
       }
     }
+  }
+  // written and read by the same wave, whose LDS accesses keep their order
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+  for (int j = 0; j < 4 * RT; ++j) {
+    const int r = 4 * j + quarter;
+    const int mine = __shfl(id[j / 4], r & 15, 64);
+    if (mine == kOutside) continue;
+    v4f v = old[j];
+    if (mine >= 0) v += *reinterpret_cast<const v4f *>(&tile[r][4 * m]);
+    float *p = a.dst + (row0 + r) * a.dst_stride + col;
+    if (whole) {
+      *reinterpret_cast<v4f_any *>(p) = v;
+    } else {
 #pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        if (id[i] == kOutside) continue;
-        float *p = a.dst + row[i] * a.dst_stride + begin + col[t];
-        const v4f v = id[i] >= 0 ? old[t][i] + sum[t][i] : old[t][i];
-        if (col[t] + 4 <= width)
-          *reinterpret_cast<v4f_any *>(p) = v;
-        else
-          for (int e = 0; e < 4; ++e)
-            if (col[t] + e < width) p[e] = v[e];
-      }
+      for (int e = 0; e < 4; ++e)
+        if (e < left) p[e] = v[e];
+    }
   }
 }
 
@@ -424,7 +461,7 @@ constexpr int kFewRows = 2;
 }  // namespace
 
 size_t adapters_work(int rows, int njobs, int rank) {
-  return ((size_t)rows * (njobs * rank + 1) * 4 + 255) / 256 * 256;
+  return ((size_t)rows * (njobs * rank * 6 + 4) + 255) / 256 * 256;
 }
 
 hipError_t launch_adapters(const Adapters &a, const DeviceInfo &dev, hipStream_t stream) {
@@ -438,22 +475,23 @@ hipError_t launch_adapters(const Adapters &a, const DeviceInfo &dev, hipStream_t
     const dim3 grid((rows + 15) / 16, (all + 16 * t() - 1) / (16 * t()));
     adapter_shrink_kernel<type(), t()><<<grid, 64 * kShrinkWaves, 0, stream>>>(a);
   };
-  auto expand = [&](auto type, auto ks) {
-    const dim3 grid((rows + kExpandRows - 1) / kExpandRows,
+  auto expand = [&](auto type, auto ks, auto rt) {
+    const dim3 grid((rows + 16 * rt() - 1) / (16 * rt()),
                     (expand_units(a.end, a.njobs) + kThreads / 64 - 1) / (kThreads / 64));
-    adapter_expand_kernel<type(), ks()><<<grid, kThreads, 0, stream>>>(a);
+    adapter_expand_kernel<type(), ks(), rt()><<<grid, kThreads, 0, stream>>>(a);
   };
   auto go = [&](auto type) {
     using std::integral_constant;
+    const integral_constant<int, 1> one;
+    const integral_constant<int, 2> two;
     if (a.seq.max_rows <= kFewRows) return by_row(type);
     const int tiles = (all + 15) / 16;
-    tiles == 1   ? shrink(type, integral_constant<int, 1>())
-    : tiles == 2 ? shrink(type, integral_constant<int, 2>())
-    : tiles == 3 ? shrink(type, integral_constant<int, 3>())
-                 : shrink(type, integral_constant<int, kMostT>());
-    a.rank <= 32   ? expand(type, integral_constant<int, 1>())
-    : a.rank <= 64 ? expand(type, integral_constant<int, 2>())
-                   : expand(type, integral_constant<int, 4>());
+    tiles == 1             ? shrink(type, one)
+    : tiles % kMostT != 0 ? shrink(type, two)
+                           : shrink(type, integral_constant<int, kMostT>());
+    a.rank <= 32   ? expand(type, one, two)
+    : a.rank <= 64 ? expand(type, two, two)
+                   : expand(type, integral_constant<int, 4>(), one);
   };
   a.type == kAdapterF32    ? go(std::integral_constant<int, kAdapterF32>())
   : a.type == kAdapterBf16 ? go(std::integral_constant<int, kAdapterBf16>())
