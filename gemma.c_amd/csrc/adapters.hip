@@ -9,8 +9,9 @@
 // Rows of prompts go 16 at a time through the bf16 matrix cores: an fp32 value is the sum of three
 // bf16 pieces, a bf16 weight is one, an f16 weight the sum of two and an fp32 weight of three, and
 // of the piece products those are summed whose orders add up to at most 2 (3, 5 or 6 of
-// them: what is left out is below 2^-22 of a product).  A tile with several adapters is done once
-// for each.  Single tokens take a wave for a value of u and a lane for a value of dst.
+// them: what is left out is below 2^-22 of a product).  A tile is one sequence's: with tiles across
+// sequences, which took a pass for each adapter, the few that had two set the time.  Single tokens
+// take a wave for a value of u and a lane for a value of dst.
 #include <type_traits>
 
 #include "gh_arith.h"
@@ -116,8 +117,7 @@ __device__ __forceinline__ float scale_of(const Adapters &a, int id) {
   return a.scale != nullptr ? a.scale[id] : 1.0f;
 }
 
-// The workspace: u [rows][jobs * rank] as fp32 or, of tiles, [rows][3][jobs * rank] in bf16
-// pieces, then the rows' ids.
+// The workspace: u [rows][jobs * rank] as fp32, then the rows' ids (of tiles: piece_of).
 __device__ __forceinline__ float *u_of(const Adapters &a) {
   return reinterpret_cast<float *>(a.work);
 }
@@ -187,131 +187,166 @@ __global__ __launch_bounds__(kThreads) void adapter_expand_row_kernel(Adapters a
 
 // ---- tiles of rows ------------------------------------------------------------------
 
-// The id of each lane's row (row, of first .. first + 15), by a whole wave: the first row's sequence,
-// and how many of the following ones begin at or before the lane's.
-__device__ __forceinline__ int ids_of_rows(const Adapters &a, int first, int row) {
+// Tiles of up to R rows of one sequence, and so of one adapter: those of sequence i begin at slot
+// row0[i] / R + i, which leaves room for all and needs no sums over the sequences before it.  A slot
+// that is left over has no rows.
+__host__ __device__ inline int tile_slots(const KvBatch &b, int r) { return b.rows / r + b.batch; }
+struct Tile {
+  int row, rows, id;  // the first row, how many, the adapter or kNone
+};
+// By a whole wave; as kv_find_part looks for rows.
+template <int R>
+__device__ __forceinline__ Tile tile_at(const Adapters &a, int slot) {
   const KvBatch &b = a.seq;
-  const int lane = threadIdx.x & 63, last = first + 15;
-  int i, id, r0, next;
-  if (b.batch < 64) {  // a trip to memory
-    const int begins = b.row0[min(lane, b.batch)];
-    const int all = a.ids[min(lane, b.batch - 1)];
-    const unsigned long long in = ~0ull >> (64 - b.batch);
-    const int from = __popcll(__ballot(begins <= first) & in);
-    const int to = __popcll(__ballot(begins <= last) & in);
-    i = max(from - 1, 0);
-    for (int j = max(from, 1); j < to; ++j) i += __builtin_amdgcn_readlane(begins, j) <= row;
-    r0 = __shfl(begins, i, 64), next = __shfl(begins, i + 1, 64), id = __shfl(all, i, 64);
-  } else {
-    int n;
-    const int lo = i = kv_find_part(b, first, &n);
-    for (int from = lo + 1; from < b.batch; from += 64) {
-      const int begins = b.row0[from + lane < b.batch ? from + lane : b.batch];
-      int j = 0;
-      for (; j < 64 && from + j < b.batch; ++j) {
-        const int at = __builtin_amdgcn_readlane(begins, j);
-        if (at > last) break;
-        i += at <= row;
-      }
-      if (j < 64) break;
-    }
-    r0 = b.row0[i], next = b.row0[i + 1], id = a.ids[i];
+  const int lane = threadIdx.x & 63;
+  int lo = 0, n = b.batch;
+  while (n > 63) {
+    const int step = (n + 62) / 63, at = lo + min(lane * step, n - 1);
+    const bool before = lane * step < n && kv_clamp(b.row0[at], 0, b.rows) / R + at <= slot;
+    const int skip = max((int)__popcll(__ballot(before)) - 1, 0) * step;
+    lo += skip;
+    n = min(n - skip, step);
   }
-  r0 = kv_clamp(r0, 0, b.rows);
-  int rows = kv_clamp(next, r0, b.rows) - r0;
-  if (rows > b.max_rows) rows = b.max_rows;
-  if (row < r0 || row - r0 >= rows) return kOutside;
-  return (unsigned)id < (unsigned)a.count ? id : kNone;
+  const int at = lo + min(lane, n);
+  const int begins = kv_clamp(b.row0[at], 0, b.rows);
+  const int ids = a.ids[min(at, b.batch - 1)];
+  const int j = max((int)__popcll(__ballot(lane < n && begins / R + at <= slot)) - 1, 0);
+  const int r0 = __builtin_amdgcn_readlane(begins, j);
+  const int rows = min(__builtin_amdgcn_readlane(begins, j + 1) - r0, b.max_rows);
+  const int id = __builtin_amdgcn_readlane(ids, j);
+  const int first = (slot - (r0 / R + lo + j)) * R;
+  return Tile{r0 + first, first < 0 ? 0 : min(rows - first, R),
+              (unsigned)id < (unsigned)a.count ? id : kNone};
 }
 
-// Piece p of u of a row in the workspace.
-__device__ __forceinline__ uint16_t *piece_of(const Adapters &a, int row, int p) {
-  return reinterpret_cast<uint16_t *>(a.work) + ((size_t)row * 3 + p) * (a.njobs * a.rank);
+// u of tiles in the workspace: a tile of up to 16 rows has their part of [rows][3][jobs * rank]
+// values, in the order in which the matrix instructions take them: [job][piece][rank / 8][rows][8].
+__device__ __forceinline__ uint16_t *piece_of(const Adapters &a, int row, int rows, int job, int p) {
+  const size_t first = (size_t)row * 3 * a.njobs * a.rank;
+  return reinterpret_cast<uint16_t *>(a.work) + first + (size_t)(job * 3 + p) * a.rank * rows;
 }
 
 constexpr int kShrinkWaves = 8;  // that share a tile's inputs
-constexpr int kShrinkSteps = 5;  // whose loads are in flight together
+constexpr int kShrinkStep = 64;  // inputs
 constexpr int kMostT = 3;        // 16 values of u each: a workgroup's, at most
 
-// u of 16 rows and 16 T of their values; each wave takes every eighth step of 32 inputs, the
-// partial sums meet in LDS.  Steps behind the last are done with zeros: a branch around them would
-// take the loads with it, one after the other.
+// A wave's steps.  A load whose neighbouring lanes are in different rows, as the matrix instructions
+// want them, takes a cycle a lane; so rows are read by runs of 16 bytes times neighbouring lanes
+// and find their lanes through LDS, the wave's own (its accesses keep their order).
+template <int TYPE, int T>
+struct ShrinkStep {
+  static constexpr int kSize = TYPE == kAdapterF32 ? 4 : 2;
+  static constexpr int kRowLanes = kShrinkStep * kSize / 16;  // of a row of A
+  static constexpr int kLoads = 16 * T * kRowLanes / 64;
+  static constexpr int kPitch = kShrinkStep + 16 / kSize;  // 16 rows' 16 bytes in different banks
+  struct Lds {
+    float x[16][kShrinkStep + 4];
+    char w[16 * T][kPitch * kSize];
+  };
+  v4f x[4];
+  u4 w[kLoads];
+
+  __device__ __forceinline__ void load(const float *const (&src)[4], const char *const (&m)[kLoads],
+                                       int k, int end) {
+    const int lane = threadIdx.x & 63, kx = k + 4 * (lane & 15);
+    const int kw = k + 16 / kSize * (lane % kRowLanes);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const v4f *>(src[j] + (kx < end ? kx : 0));
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j)
+      w[j] = *reinterpret_cast<const u4 *>(m[j] + (size_t)(kw < end ? kw : 0) * kSize);
+  }
+  // into LDS, zeros behind the last input
+  __device__ __forceinline__ void put(Lds &to, int k, int end) const {
+    const int lane = threadIdx.x & 63;
+    const bool inx = k + 4 * (lane & 15) < end;
+    const bool inw = k + 16 / kSize * (lane % kRowLanes) < end;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      *reinterpret_cast<v4f *>(&to.x[4 * j + lane / 16][4 * (lane & 15)]) =
+          inx ? x[j] : v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j)
+      *reinterpret_cast<u4 *>(
+          &to.w[64 / kRowLanes * j + lane / kRowLanes][16 * (lane % kRowLanes)]) =
+          inw ? w[j] : u4{0, 0, 0, 0};
+  }
+  __device__ __forceinline__ static void multiply(const Lds &from, v4f (&acc)[T]) {
+    const int lane = threadIdx.x & 63, m = lane & 15;
+#pragma unroll
+    for (int h = 0; h < kShrinkStep / 32; ++h) {
+      const int k0 = 32 * h + 8 * (lane / 16);
+      const v4f lo = *reinterpret_cast<const v4f *>(&from.x[m][k0]);
+      const v4f hi = *reinterpret_cast<const v4f *>(&from.x[m][k0 + 4]);
+      const float f[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      const Split8<3> xp = split8<3>(f);
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+        acc[t] = product(pieces8<TYPE>(raw8<TYPE>(from.w[16 * t + m], k0)), xp, acc[t]);
+    }
+  }
+};
+
+// u of a tile of 16 rows and 16 T of their values; each wave takes every eighth step, the partial
+// sums meet in LDS.
 template <int TYPE, int T>
 __global__ __launch_bounds__(64 * kShrinkWaves) void adapter_shrink_kernel(Adapters a) {
-  __shared__ v4f part[kShrinkWaves][T][64];
+  typedef ShrinkStep<TYPE, T> Step;
+  __shared__ union {
+    typename Step::Lds step[kShrinkWaves];
+    v4f part[kShrinkWaves][T][64];
+  } sh;
   const int all = a.njobs * a.rank, lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  const int first = 16 * blockIdx.x, at0 = 16 * T * blockIdx.y;
-  const int row = first + (lane & 15);
-  const bool there = row < a.seq.rows;
-  const int id = ids_of_rows(a, first, row);
-  if (blockIdx.y == 0 && threadIdx.x < 16 && there) ids_of(a)[row] = id;
-  const float *x = a.src + (there ? row : a.seq.rows - 1) * a.src_stride;
-  const int steps = (a.k + 31) / 32, k0 = 8 * (lane / 16);
-  // one of the lane's 16 rows of A in each of the T groups
-  const void *m[T];
-  size_t from[T];
+  const int at0 = 16 * T * blockIdx.y;
+  const Tile tile = tile_at<16>(a, blockIdx.x);
+  if (tile.rows <= 0 || tile.id < 0) return;
+  const float *x[4];
 #pragma unroll
-  for (int t = 0; t < T; ++t) {
-    const int at = min(at0 + 16 * t + (lane & 15), all - 1), job = at / a.rank;
-    m[t] = job_of(a.a, job);
-    from[t] = (size_t)(at - job * a.rank) * a.k;
+  for (int j = 0; j < 4; ++j)
+    x[j] = a.src + (tile.row + min(4 * j + lane / 16, tile.rows - 1)) * a.src_stride;
+  const char *m[Step::kLoads];
+#pragma unroll
+  for (int j = 0; j < Step::kLoads; ++j) {
+    const int at = min(at0 + (64 * j + lane) / Step::kRowLanes, all - 1), job = at / a.rank;
+    m[j] = reinterpret_cast<const char *>(job_of(a.a, job)) +
+           ((size_t)tile.id * a.rank + (at - job * a.rank)) * a.k * Step::kSize;
   }
-  unsigned todo = (unsigned)__ballot(id >= 0 && there) & 0xffffu;
-  while (todo != 0) {  // adapter by adapter
-    const int cur = __builtin_amdgcn_readlane(id, __builtin_ctz(todo));
-    todo &= ~(unsigned)__ballot(id == cur);
-    const size_t skip = (size_t)cur * a.rank * a.k;
-    v4f acc[T];
+  v4f acc[T];
 #pragma unroll
-    for (int t = 0; t < T; ++t) acc[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s0 = wave; s0 < steps; s0 += kShrinkWaves * kShrinkSteps) {
-      v4f xs[kShrinkSteps][2];
-      Raw8<TYPE> ws[kShrinkSteps][T];
+  for (int t = 0; t < T; ++t) acc[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  Step next;
+  typename Step::Lds &mine = sh.step[wave];
+  int k = kShrinkStep * wave;
+  if (k < a.k) next.load(x, m, k, a.k);
+  while (k < a.k) {
+    next.put(mine, k, a.k);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    k += kShrinkStep * kShrinkWaves;
+    next.load(x, m, k, a.k);
+    __builtin_amdgcn_sched_barrier(0);  // asked for before the products, not where they are put
+    Step::multiply(mine, acc);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+  __syncthreads();
 #pragma unroll
-      for (int j = 0; j < kShrinkSteps; ++j) {
-        int k = 32 * (s0 + j * kShrinkWaves) + k0;
-        k = k < a.k ? k : 0;
-        xs[j][0] = *reinterpret_cast<const v4f *>(x + k);
-        xs[j][1] = *reinterpret_cast<const v4f *>(x + k + 4);
+  for (int t = 0; t < T; ++t) sh.part[wave][t][lane] = acc[t];
+  __syncthreads();
+  const int at = at0 + 16 * wave + 4 * (lane / 16);
+  if (wave >= T || (lane & 15) >= tile.rows || at >= all) return;
+  v4f sum = sh.part[0][wave][lane];
 #pragma unroll
-        for (int t = 0; t < T; ++t) ws[j][t] = raw8<TYPE>(m[t], skip + from[t] + k);
-      }
+  for (int w = 1; w < kShrinkWaves; ++w) sum += sh.part[w][wave][lane];
+  sum *= scale_of(a, tile.id);
+  const int job = at / a.rank, value = at - job * a.rank;
 #pragma unroll
-      for (int j = 0; j < kShrinkSteps; ++j) {
-        const bool in = 32 * (s0 + j * kShrinkWaves) + k0 < a.k;
-        float f[8];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f[e] = in ? xs[j][0][e] : 0.0f, f[e + 4] = in ? xs[j][1][e] : 0.0f;
-        const Split8<3> xp = split8<3>(f);
-#pragma unroll
-        for (int t = 0; t < T; ++t) {
-          Raw8<TYPE> w = ws[j][t];
-#pragma unroll
-          for (auto &v : w.v) v = in ? v : u4{0, 0, 0, 0};
-          acc[t] = product(pieces8<TYPE>(w), xp, acc[t]);
-        }
-      }
-    }
-#pragma unroll
-    for (int t = 0; t < T; ++t) part[wave][t][lane] = acc[t];
-    __syncthreads();
-    if (wave < T) {
-      v4f sum = part[0][wave][lane];
-#pragma unroll
-      for (int w = 1; w < kShrinkWaves; ++w) sum += part[w][wave][lane];
-      const int at = at0 + 16 * wave + 4 * (lane / 16);
-      if (id == cur && there && at < all) {
-        sum *= scale_of(a, cur);
-#pragma unroll
-        for (int p = 0; p < 3; ++p) {
-          const u2 b = {cvt_pk_bf16(sum[0], sum[1]), cvt_pk_bf16(sum[2], sum[3])};
-          *reinterpret_cast<u2 *>(piece_of(a, row, p) + at) = b;
-          sum -= v4f{bf16_lo(b[0]), bf16_hi(b[0]), bf16_lo(b[1]), bf16_hi(b[1])};
-        }
-      }
-    }
-    __syncthreads();
+  for (int p = 0; p < 3; ++p) {
+    const u2 b = {cvt_pk_bf16(sum[0], sum[1]), cvt_pk_bf16(sum[2], sum[3])};
+    *reinterpret_cast<u2 *>(piece_of(a, tile.row, tile.rows, job, p) +
+                            (value / 8 * tile.rows + (lane & 15)) * 8 + value % 8) = b;
+    sum -= v4f{bf16_lo(b[0]), bf16_hi(b[0]), bf16_lo(b[1]), bf16_hi(b[1])};
   }
 }
 
@@ -345,24 +380,10 @@ __global__ __launch_bounds__(kThreads, KS == 1 ? 4 : 3) void adapter_expand_kern
     unit -= units;
   }
   if (job == a.njobs) return;
-  float(&tile)[16 * RT][kExpandPitch] = tiles[wave];
-  const void *b = job_of(a.b, job);
-  const int k0 = 8 * quarter, c0 = unit * kExpandCols, row0 = 16 * RT * blockIdx.x;
-  int id[RT];
-  Split8<3> u[RT][KS];
-#pragma unroll
-  for (int i = 0; i < RT; ++i) {
-    const int row = min(row0 + 16 * i + m, a.seq.rows - 1);
-    id[i] = ids_of(a)[row];
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const int k = 32 * s + k0;
-#pragma unroll
-      for (int p = 0; p < 3; ++p)
-        u[i][s].p[p] = *reinterpret_cast<const u4 *>(piece_of(a, row, p) + job * a.rank +
-                                                     (k < a.rank ? k : 0));
-    }
-  }
+  float(&sums)[16 * RT][kExpandPitch] = tiles[wave];
+  const Tile tile = tile_at<16 * RT>(a, blockIdx.x);
+  if (tile.rows <= 0) return;
+  const int k0 = 8 * quarter, c0 = unit * kExpandCols;
   // rows 4 j + quarter, four columns of them from the lane's 4 m
   const int left = width - c0 - 4 * m;
   const size_t col = begin + c0 + 4 * m;
@@ -371,39 +392,39 @@ __global__ __launch_bounds__(kThreads, KS == 1 ? 4 : 3) void adapter_expand_kern
   if (whole) {
 #pragma unroll
     for (int j = 0; j < 4 * RT; ++j) {
-      const int row = min(row0 + 4 * j + quarter, a.seq.rows - 1);
+      const int row = tile.row + min(4 * j + quarter, tile.rows - 1);
       old[j] = *reinterpret_cast<const v4f_any *>(a.base + row * a.base_stride + col);
     }
   } else {
 #pragma unroll
     for (int j = 0; j < 4 * RT; ++j) {
-      const int row = min(row0 + 4 * j + quarter, a.seq.rows - 1);
+      const int row = tile.row + min(4 * j + quarter, tile.rows - 1);
       old[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (e < left) old[j][e] = a.base[row * a.base_stride + col + e];
     }
   }
-  unsigned long long todo = 0;
+  if (tile.id >= 0) {
+    const void *b = job_of(a.b, job);
+    Split8<3> u[RT][KS];
 #pragma unroll
-  for (int i = 0; i < RT; ++i) {
-    if (row0 + 16 * i + m >= a.seq.rows) id[i] = kOutside;
-    todo |= (__ballot(id[i] >= 0) & 0xffffull) << (16 * i);
+    for (int i = 0; i < RT; ++i) {
+      const int rows = min(tile.rows - 16 * i, 16);  // of a tile of 16
+      if (rows <= 0) {
 #pragma unroll
-    for (int s = 0; s < KS; ++s)
+        for (int s = 0; s < KS; ++s) u[i][s] = u[0][s];
+        continue;
+      }
 #pragma unroll
-      for (auto &v : u[i][s].p) v = 32 * s + k0 < a.rank ? v : u4{0, 0, 0, 0};
-  }
-  while (todo != 0) {
-    const int at = __builtin_ctzll(todo);
-    int cur = __builtin_amdgcn_readlane(id[0], at & 15);
+      for (int s = 0; s < KS; ++s)
 #pragma unroll
-    for (int i = 1; i < RT; ++i) {
-      const int other = __builtin_amdgcn_readlane(id[i], at & 15);
-      cur = at / 16 == i ? other : cur;
+        for (int p = 0; p < 3; ++p) {
+          const int k = 32 * s + k0, at = (k < a.rank ? k : 0) / 8 * rows + min(m, rows - 1);
+          u[i][s].p[p] = *reinterpret_cast<const u4 *>(
+              piece_of(a, tile.row + 16 * i, rows, job, p) + at * 8);
+        }
     }
-#pragma unroll
-    for (int i = 0; i < RT; ++i) todo &= ~((__ballot(id[i] == cur) & 0xffffull) << (16 * i));
     constexpr int W = KS < 4 && (KS == 1 || TYPE != kAdapterF32) ? 4 : 2;  // read together
 #pragma unroll
     for (int t0 = 0; t0 < 4; t0 += W) {
@@ -413,44 +434,49 @@ __global__ __launch_bounds__(kThreads, KS == 1 ? 4 : 3) void adapter_expand_kern
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
           const int c = min(c0 + 16 * (t0 + t) + m, width - 1), k = 32 * s + k0;
-          w[t][s] = raw8<TYPE>(b, ((size_t)cur * width + c) * a.rank + (k < a.rank ? k : 0));
+          w[t][s] = raw8<TYPE>(b, ((size_t)tile.id * width + c) * a.rank + (k < a.rank ? k : 0));
         }
 #pragma unroll
       for (int t = 0; t < W; ++t) {
         v4f d[RT] = {};
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
+          const bool in = 32 * s + k0 < a.rank;
           Raw8<TYPE> v = w[t][s];
 #pragma unroll
-          for (auto &x : v.v) x = 32 * s + k0 < a.rank ? x : u4{0, 0, 0, 0};
+          for (auto &x : v.v) x = in ? x : u4{0, 0, 0, 0};
           const auto wp = pieces8<TYPE>(v);
 #pragma unroll
-          for (int i = 0; i < RT; ++i) d[i] = product(wp, u[i][s], d[i]);
+          for (int i = 0; i < RT; ++i) {
+            Split8<3> up = u[i][s];
+#pragma unroll
+            for (auto &x : up.p) x = in ? x : u4{0, 0, 0, 0};
+            d[i] = product(wp, up, d[i]);
+          }
         }
 #pragma unroll
         for (int i = 0; i < RT; ++i)
-          if (id[i] == cur)
-            *reinterpret_cast<v4f *>(&tile[16 * i + m][16 * (t0 + t) + 4 * quarter]) = d[i];
+          *reinterpret_cast<v4f *>(&sums[16 * i + m][16 * (t0 + t) + 4 * quarter]) = d[i];
       }
     }
+    // written and read by the same wave, whose LDS accesses keep their order
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int j = 0; j < 4 * RT; ++j)
+      old[j] += *reinterpret_cast<const v4f *>(&sums[4 * j + quarter][4 * m]);
   }
-  // written and read by the same wave, whose LDS accesses keep their order
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
 #pragma unroll
   for (int j = 0; j < 4 * RT; ++j) {
     const int r = 4 * j + quarter;
-    const int mine = __shfl(id[j / 4], r & 15, 64);
-    if (mine == kOutside) continue;
-    v4f v = old[j];
-    if (mine >= 0) v += *reinterpret_cast<const v4f *>(&tile[r][4 * m]);
-    float *p = a.dst + (row0 + r) * a.dst_stride + col;
+    if (r >= tile.rows) break;
+    float *p = a.dst + (tile.row + r) * a.dst_stride + col;
     if (whole) {
-      *reinterpret_cast<v4f_any *>(p) = v;
+      *reinterpret_cast<v4f_any *>(p) = old[j];
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (e < left) p[e] = v[e];
+        if (e < left) p[e] = old[j][e];
     }
   }
 }
@@ -471,12 +497,13 @@ hipError_t launch_adapters(const Adapters &a, const DeviceInfo &dev, hipStream_t
     adapter_shrink_row_kernel<type()><<<first, kThreads, 0, stream>>>(a);
     adapter_expand_row_kernel<type()><<<second, kThreads, 0, stream>>>(a);
   };
+  const int slots = tile_slots(a.seq, 16);
   auto shrink = [&](auto type, auto t) {
-    const dim3 grid((rows + 15) / 16, (all + 16 * t() - 1) / (16 * t()));
+    const dim3 grid(slots, (all + 16 * t() - 1) / (16 * t()));
     adapter_shrink_kernel<type(), t()><<<grid, 64 * kShrinkWaves, 0, stream>>>(a);
   };
   auto expand = [&](auto type, auto ks, auto rt) {
-    const dim3 grid((rows + 16 * rt() - 1) / (16 * rt()),
+    const dim3 grid(tile_slots(a.seq, 16 * rt()),
                     (expand_units(a.end, a.njobs) + kThreads / 64 - 1) / (kThreads / 64));
     adapter_expand_kernel<type(), ks(), rt()><<<grid, kThreads, 0, stream>>>(a);
   };
@@ -486,9 +513,9 @@ hipError_t launch_adapters(const Adapters &a, const DeviceInfo &dev, hipStream_t
     const integral_constant<int, 2> two;
     if (a.seq.max_rows <= kFewRows) return by_row(type);
     const int tiles = (all + 15) / 16;
-    tiles == 1             ? shrink(type, one)
-    : tiles % kMostT != 0 ? shrink(type, two)
-                           : shrink(type, integral_constant<int, kMostT>());
+    tiles == 1 || (long)slots * tiles <= 2 * dev.cus ? shrink(type, one)
+    : tiles % kMostT != 0                            ? shrink(type, two)
+                                                     : shrink(type, integral_constant<int, kMostT>());
     a.rank <= 32   ? expand(type, one, two)
     : a.rank <= 64 ? expand(type, two, two)
                    : expand(type, integral_constant<int, 4>(), one);
