@@ -364,13 +364,18 @@ __host__ __device__ inline int expand_units(const int (&end)[kAdapterMaxJobs], i
 
 // dst of 16 RT rows and 64 columns of a job a wave; KS: steps of 32 of the rank.  base and dst are
 // read and written by whole runs of 256 bytes; the products, whose lanes have a row each, go through
-// LDS.
-template <int TYPE, int KS, int RT>
-__global__ __launch_bounds__(kThreads, KS == 1 ? 4 : 3) void adapter_expand_kernel(Adapters a) {
-  __shared__ float tiles[kThreads / 64][16 * RT][kExpandPitch];
+// LDS.  A workgroup's four waves are WR times as many rows by 4 / WR times as many columns: 4 by 1,
+// which read B once, by whole runs, and share it in LDS, or, for short sequences, 1 by 4.
+template <int TYPE, int KS, int RT, int WR>
+__global__ __launch_bounds__(kThreads, KS == 1 && TYPE != kAdapterF32 ? 4 : 3) void adapter_expand_kernel(Adapters a) {
+  constexpr int kSize = TYPE == kAdapterF32 ? 4 : 2, kWaves = kThreads / 64;
+  constexpr int kPitch = 32 * KS * kSize + 16;  // of a row of B: 16 rows in different banks
+  constexpr int kLoads = kExpandCols * 32 * KS * kSize / 16 / kThreads;
+  __shared__ float tiles[kWaves][16 * RT][kExpandPitch];
+  __shared__ char shared[WR > 1 ? kExpandCols : 1][kPitch];
   const int lane = threadIdx.x & 63, m = lane & 15, quarter = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  int unit = blockIdx.y * (kThreads / 64) + wave;
+  int unit = WR > 1 ? blockIdx.y : blockIdx.y * kWaves + wave;
   int job = 0, begin = 0, width = a.end[0];
   for (; job < a.njobs; ++job) {
     begin = job == 0 ? 0 : a.end[job - 1];
@@ -381,33 +386,28 @@ __global__ __launch_bounds__(kThreads, KS == 1 ? 4 : 3) void adapter_expand_kern
   }
   if (job == a.njobs) return;
   float(&sums)[16 * RT][kExpandPitch] = tiles[wave];
-  const Tile tile = tile_at<16 * RT>(a, blockIdx.x);
+  Tile tile = tile_at<16 * RT * WR>(a, blockIdx.x);
   if (tile.rows <= 0) return;
   const int k0 = 8 * quarter, c0 = unit * kExpandCols;
-  // rows 4 j + quarter, four columns of them from the lane's 4 m
-  const int left = width - c0 - 4 * m;
-  const size_t col = begin + c0 + 4 * m;
-  const bool whole = c0 + kExpandCols <= width;
-  v4f old[4 * RT];
-  if (whole) {
+  const char *b = reinterpret_cast<const char *>(job_of(a.b, job)) +
+                  ((size_t)tile.id * width + c0) * a.rank * kSize;
+  const int chunks = a.rank * kSize / 16;  // of a row of B
+  u4 part[kLoads];
+  if (WR > 1 && tile.id >= 0) {
+    const int have = min(kExpandCols, width - c0) * chunks;
 #pragma unroll
-    for (int j = 0; j < 4 * RT; ++j) {
-      const int row = tile.row + min(4 * j + quarter, tile.rows - 1);
-      old[j] = *reinterpret_cast<const v4f_any *>(a.base + row * a.base_stride + col);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4 * RT; ++j) {
-      const int row = tile.row + min(4 * j + quarter, tile.rows - 1);
-      old[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (e < left) old[j][e] = a.base[row * a.base_stride + col + e];
+    for (int j = 0; j < kLoads; ++j) {
+      const int i = threadIdx.x + kThreads * j;
+      part[j] = reinterpret_cast<const u4 *>(b)[i < have ? i : 0];
     }
   }
-  if (tile.id >= 0) {
-    const void *b = job_of(a.b, job);
-    Split8<3> u[RT][KS];
+  if (WR > 1) {
+    tile.row += 16 * RT * wave;
+    tile.rows = min(tile.rows - 16 * RT * wave, 16 * RT);
+  }
+  const int last = max(tile.rows, 1) - 1;
+  Split8<3> u[RT][KS];
+  if (tile.rows > 0 && tile.id >= 0) {
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
       const int rows = min(tile.rows - 16 * i, 16);  // of a tile of 16
@@ -425,6 +425,44 @@ __global__ __launch_bounds__(kThreads, KS == 1 ? 4 : 3) void adapter_expand_kern
               piece_of(a, tile.row + 16 * i, rows, job, p) + at * 8);
         }
     }
+  }
+  // rows 4 j + quarter, four columns of them from the lane's 4 m
+  const int left = width - c0 - 4 * m;
+  const size_t col = begin + c0 + 4 * m;
+  const bool whole = c0 + kExpandCols <= width;
+  v4f old[4 * RT];
+  if (tile.rows <= 0) {
+    // (a wave that only waits for the others)
+  } else if (whole) {
+#pragma unroll
+    for (int j = 0; j < 4 * RT; ++j) {
+      const int row = tile.row + min(4 * j + quarter, last);
+      old[j] = *reinterpret_cast<const v4f_any *>(a.base + row * a.base_stride + col);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4 * RT; ++j) {
+      const int row = tile.row + min(4 * j + quarter, last);
+      old[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < left) old[j][e] = a.base[row * a.base_stride + col + e];
+    }
+  }
+  if (WR > 1) {
+    if (tile.id >= 0) {
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        const int i = threadIdx.x + kThreads * j;
+        if (i < kExpandCols * chunks)
+          *reinterpret_cast<u4 *>(&shared[i / chunks][i % chunks * 16]) = part[j];
+      }
+    }
+    lds_barrier();
+  }
+  if (tile.rows <= 0) return;
+  if (tile.id >= 0) {
+    // values behind the rank are zeros on both sides
     constexpr int W = KS < 4 && (KS == 1 || TYPE != kAdapterF32) ? 4 : 2;  // read together
 #pragma unroll
     for (int t0 = 0; t0 < 4; t0 += W) {
@@ -433,8 +471,11 @@ __global__ __launch_bounds__(kThreads, KS == 1 ? 4 : 3) void adapter_expand_kern
       for (int t = 0; t < W; ++t)
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-          const int c = min(c0 + 16 * (t0 + t) + m, width - 1), k = 32 * s + k0;
-          w[t][s] = raw8<TYPE>(b, ((size_t)tile.id * width + c) * a.rank + (k < a.rank ? k : 0));
+          const int c = 16 * (t0 + t) + m, k = 32 * s + k0 < a.rank ? 32 * s + k0 : 0;
+          if (WR > 1)
+            w[t][s] = raw8<TYPE>(shared[c], k);
+          else
+            w[t][s] = raw8<TYPE>(b, (size_t)min(c, width - c0 - 1) * a.rank + k);
         }
 #pragma unroll
       for (int t = 0; t < W; ++t) {
@@ -503,9 +544,14 @@ hipError_t launch_adapters(const Adapters &a, const DeviceInfo &dev, hipStream_t
     adapter_shrink_kernel<type(), t()><<<grid, 64 * kShrinkWaves, 0, stream>>>(a);
   };
   auto expand = [&](auto type, auto ks, auto rt) {
-    const dim3 grid(tile_slots(a.seq, 16 * rt()),
-                    (expand_units(a.end, a.njobs) + kThreads / 64 - 1) / (kThreads / 64));
-    adapter_expand_kernel<type(), ks(), rt()><<<grid, kThreads, 0, stream>>>(a);
+    constexpr int kWaves = kThreads / 64, R = 16 * rt();
+    const int units = expand_units(a.end, a.njobs);
+    if (a.seq.max_rows > 2 * R)
+      adapter_expand_kernel<type(), ks(), rt(), kWaves>
+          <<<dim3(tile_slots(a.seq, R * kWaves), units), kThreads, 0, stream>>>(a);
+    else
+      adapter_expand_kernel<type(), ks(), rt(), 1>
+          <<<dim3(tile_slots(a.seq, R), (units + kWaves - 1) / kWaves), kThreads, 0, stream>>>(a);
   };
   auto go = [&](auto type) {
     using std::integral_constant;
