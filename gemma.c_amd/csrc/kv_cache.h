@@ -142,6 +142,30 @@ __device__ __forceinline__ KvRow kv_row_wave(const KvBatch &b, int r) {
   const int ln = POS ? kv_clamp(__builtin_amdgcn_readlane(len, j), 0, b.max_len) : 0;
   return KvRow{in ? lo + j : -1, ln - rows + (r - r0)};
 }
+
+// kv_row_wave of N rows from r on, in turn to take(i, row); fewer than 64 sequences take one trip to
+// memory.
+template <int N, typename Take>
+__device__ __forceinline__ void kv_rows_wave(const KvBatch &b, int r, Take take) {
+  const int lane = threadIdx.x & 63;
+  if (b.batch > 63) {
+    for (int i = 0; i < N; ++i) take(i, kv_row_wave<true>(b, r + i));
+    return;
+  }
+  const int first = b.row0[lane < b.batch ? lane : b.batch];
+  const int len = b.len[lane < b.batch ? lane : b.batch - 1];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int before = __popcll(__ballot(lane < b.batch && first <= r + i));
+    const int j = before > 0 ? before - 1 : 0;
+    const int r0 = kv_clamp(__builtin_amdgcn_readlane(first, j), 0, b.rows);
+    int rows = kv_clamp(__builtin_amdgcn_readlane(first, j + 1), r0, b.rows) - r0;
+    if (rows > b.max_rows) rows = b.max_rows;
+    const int at = r + i - r0;
+    const int ln = kv_clamp(__builtin_amdgcn_readlane(len, j), 0, b.max_len);
+    take(i, KvRow{at >= 0 && at < rows ? j : -1, ln - rows + at});
+  }
+}
 #endif
 
 // Keys that a row at position pos sees: lo .. hi (hi < lo: none).

@@ -6,8 +6,12 @@
 // angle needs more than fp32, and the keys' codes that follow are then the exact ones but where
 // a border between two codes is hit to 1e-15 (an fp32 rounding in between moves one in 10^5).
 //
-// A head is hdim / 4 lanes' (16, 32 or 64 of them), four values a lane: pairs 2l and 2l + 1 of
-// lane l, then what doesn't turn.  A lane's two angles are those of every head of its row.
+// Few rows, and heads of any size: a head is hdim / 4 lanes' (16, 32 or 64 of them), four values a
+// lane: pairs 2l and 2l + 1 of lane l, then what doesn't turn.
+//
+// Many rows of heads of 64, 128 or 256 values: a row is hdim / 16 lanes', which take one head after
+// the other and have all the angles of their values from the start.  That is a quarter of the sums
+// over lanes, scales and addresses: 16 values a lane instead of 4.
 #include <type_traits>
 
 #include "dec_common.h"
@@ -37,6 +41,11 @@ __device__ __forceinline__ int group_max_i32(int v) {
 #pragma unroll
   for (int off = G / 2; off > 0; off >>= 1) v = max(v, __shfl_xor(v, off, 64));
   return v;
+}
+
+template <int CTRL>
+__device__ __forceinline__ int dpp_i32(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xF, 0xF, false);
 }
 
 // 1 / sqrt(v) for v > 0: the instruction's approximation and a step of third order
@@ -146,7 +155,7 @@ __device__ __forceinline__ void head_turn(float (&x)[4], bool some, bool norm,
   for (int e = 0; e < 4; ++e) d[e] = (double)x[e];
   if (some) {
     const double ss = fma(d[0], d[0], d[1] * d[1]) + fma(d[2], d[2], d[3] * d[3]);
-    const double m = rsqrt_f64(group_sum_f64<G>(ss) / (double)hdim + (double)eps);
+    const double m = rsqrt_f64(fma(group_sum_f64<G>(ss), 1.0 / (double)hdim, (double)eps));
 #pragma unroll
     for (int e = 0; e < 4; ++e) d[e] = norm ? d[e] * (m * w1[e]) : d[e];
   }
@@ -293,9 +302,233 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(KvAppend a) {
   }
 }
 
-// Heads a group of lanes does one after the other: one while that leaves the card room, so that a
-// few rows take one trip to memory, else four, which share the row's angles and table look-ups.
+// ---- many rows ---------------------------------------------------------------------
+
+// A lane's 16 values of a head: chunks of four at 4 (l + G j), G lanes a head.  NT chunks turn (4 or
+// fewer, the first ones): within themselves with PAIRS, else j with j + NT / 2, NT 2 or 4.
+template <int G, bool PAIRS>
+struct Wide {
+  static constexpr int HD = 16 * G;
+  double c[8], s[8];  // of the lane's pairs
+  int nt, lane;
+
+  __device__ __forceinline__ Wide(const Rotary &r, int pos, int lane_) : lane(lane_) {
+    nt = r.rot / (4 * G);
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      const int j = PAIRS ? n / 2 : n / 4;
+      if (j >= (PAIRS ? nt : nt / 2)) break;
+      const int f = PAIRS ? 2 * (lane + G * j) + n % 2 : 4 * (lane + G * j) + n % 4;
+      double angle = r.freq[f] * (double)pos;
+      if (r.angle32) angle = (double)((float)r.freq[f] * (float)pos);
+      cos_sin(angle, &c[n], &s[n]);
+      if (r.angle32) c[n] = (double)(float)c[n], s[n] = (double)(float)s[n];
+      c[n] *= (double)r.amp;
+      s[n] *= (double)r.amp;
+    }
+  }
+  __device__ __forceinline__ void load(const float *p, v4f (&x)[4]) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const v4f *>(p + 4 * (lane + G * j));
+  }
+  __device__ __forceinline__ void store(float *p, const v4f (&x)[4]) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) *reinterpret_cast<v4f *>(p + 4 * (lane + G * j)) = x[j];
+  }
+  // through the norm (weights w, applied as w + 1; norm is the same in the whole wave) and the turn
+  __device__ __forceinline__ void turn(v4f (&x)[4], bool norm, const v4f (&w)[4], float eps) const {
+    double d[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) d[j][e] = (double)x[j][e];
+    if (norm) {
+      double ss = 0.0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ss = fma(d[j][e], d[j][e], ss);
+      ss += dpp_f64<kDppXor1>(ss);
+      ss += dpp_f64<kDppXor2>(ss);
+      if (G >= 8) ss += dpp_f64<kDppHalfMirror>(ss);
+      if (G >= 16) ss += dpp_f64<kDppMirror>(ss);
+      const double m = rsqrt_f64(fma(ss, 1.0 / HD, (double)eps));
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[j][e] *= m * ((double)w[j][e] + 1.0);
+    }
+    auto pair = [&](double &a, double &b, int n) {
+      const double t = a * c[n] - b * s[n];
+      b = fma(b, c[n], a * s[n]);
+      a = t;
+    };
+    if (PAIRS) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < nt) {
+          pair(d[j][0], d[j][1], 2 * j);
+          pair(d[j][2], d[j][3], 2 * j + 1);
+        }
+    } else if (nt == 4) {
+#pragma unroll
+      for (int n = 0; n < 8; ++n) pair(d[n / 4][n % 4], d[n / 4 + 2][n % 4], n);
+    } else if (nt == 2) {
+#pragma unroll
+      for (int n = 0; n < 4; ++n) pair(d[0][n], d[1][n], n);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[j][e] = (float)d[j][e];
+  }
+  // As codes and a scale into the cache's row `slot` of HD codes (negative: none), as cache_write
+  // makes them.
+  template <int TYPE>
+  __device__ __forceinline__ void code(const v4f (&x)[4], uint8_t *codes, float *scales,
+                                       long slot) const {
+    int top = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = max(top, __float_as_int(x[j][e]) & 0x7fffffff);
+    top = max(top, dpp_i32<kDppXor1>(top));
+    top = max(top, dpp_i32<kDppXor2>(top));
+    if (G >= 8) top = max(top, dpp_i32<kDppHalfMirror>(top));
+    if (G >= 16) top = max(top, dpp_i32<kDppMirror>(top));
+    const bool finite = top < 0x7f800000;
+    const float amax = finite ? daz(__int_as_float(top)) : 0.0f;
+    float scale = 0.0f;
+    uint32_t q[4] = {};
+    if (TYPE == kKvI8) {
+      const QuantParams qp = quant_params(amax);
+      scale = amax > 0.0f ? qp.scale : 0.0f;
+      if (__all(finite && (amax == 0.0f || amax > 1e-30f))) {
+        // 127 / amax is finite and no code leaves -127 .. 127: quant_one without its clamps
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t t[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float y = x[j][e] * qp.inv;
+            t[e] = (uint32_t)(int)(y + copysignf(0.5f, y));
+          }
+          q[j] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(t[3], t[2], 0x0c0c0400u),
+                                       __builtin_amdgcn_perm(t[1], t[0], 0x0c0c0400u), 0x05040100u);
+        }
+      } else if (amax > 0.0f) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          q[j] = pack4(quant_one(x[j][0], qp.inv), quant_one(x[j][1], qp.inv),
+                       quant_one(x[j][2], qp.inv), quant_one(x[j][3], qp.inv));
+      }
+    } else if (amax > 0.0f) {
+      scale = mul_ftz(amax, 1.0f / 448.0f);
+      const float inv = (float)(448.0 / (double)amax);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = fmaxf(-448.0f, fminf(448.0f, daz(x[j][e]) * inv));
+        const int t = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+        q[j] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], t, true);
+      }
+    }
+    if (slot < 0) return;
+    uint32_t *dst = reinterpret_cast<uint32_t *>(codes + (size_t)slot * HD) + lane;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) dst[G * j] = q[j];
+    if (lane == 0) scales[slot] = finite ? scale : __int_as_float(0x7fc00000);
+  }
+};
+
+// Whether rows go by Wide: whole chunks turn.
+bool wide(int hdim, const Rotary &r) {
+  return (hdim == 64 || hdim == 128 || hdim == 256) && r.rot % (r.pairs ? hdim / 4 : hdim / 2) == 0;
+}
+
+// `per` heads of 64 / G rows a wave
+template <int G, bool PAIRS>
+__global__ __launch_bounds__(kThreads) void rope_wide_kernel(RopeRows a, int per) {
+  const long wave = (long)blockIdx.x * (kThreads / 64) +
+                    __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int parts = (a.heads + per - 1) / per;
+  const int h0 = (int)(wave % parts) * per, h1 = min(h0 + per, a.heads);
+  const long first = wave / parts * (64 / G);
+  if (first >= a.rows) return;
+  const int r = (int)first + threadIdx.x % 64 / G;
+  const bool there = r < a.rows;
+  const int row = there ? r : a.rows - 1;
+  const float *src = a.src + row * a.src_stride;
+  float *dst = a.dst + row * a.dst_stride;
+  const Wide<G, PAIRS> t(a.rot, a.pos[row], threadIdx.x % G);
+  v4f w[4] = {}, x[4], next[4];
+  if (a.w != nullptr) t.load(a.w, w);
+  t.load(src + h0 * (16 * G), next);
+  for (int h = h0; h < h1; ++h) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = next[j];
+    t.load(src + min(h + 1, h1 - 1) * (16 * G), next);
+    t.turn(x, a.w != nullptr, w, a.eps);
+    if (there) t.store(dst + h * (16 * G), x);
+  }
+}
+
+// `per` heads (q's, then k's, then v's) of 64 / G rows a wave
+template <int G, int TYPE, bool PAIRS>
+__global__ __launch_bounds__(kThreads) void kv_append_wide_kernel(KvAppend a, int per) {
+  constexpr int HD = 16 * G, ROWS = 64 / G;
+  const long wave = (long)blockIdx.x * (kThreads / 64) +
+                    __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int nq = a.q != nullptr ? a.n_heads : 0, nk = a.c.nkv, all = nq + 2 * nk;
+  const int parts = (all + per - 1) / per;
+  const int h0 = (int)(wave % parts) * per, h1 = min(h0 + per, all);
+  const long first = wave / parts * ROWS;
+  if (first >= a.b.rows) return;
+  const int group = threadIdx.x % 64 / G, r = min((int)first + group, a.b.rows - 1);
+  KvRow row = {-1, 0};
+  kv_rows_wave<ROWS>(a.b, (int)first, [&](int i, KvRow of) {
+    if (i == group) row = of;
+  });
+  if ((int)first + group >= a.b.rows) row.i = -1;
+  const bool there = row.i >= 0;
+  // the row's place in the first head of its page
+  const long place = there && row.pos >= 0 ? kv_slot(a.c, a.b, row.i, row.pos, 0) : -1;
+  const Wide<G, PAIRS> t(a.rot, row.pos, threadIdx.x % G);
+  const float *q = nq > 0 ? a.q + r * a.q_stride : nullptr;
+  const float *k = a.k + r * a.k_stride, *v = a.v + r * a.v_stride;
+  float *out = nq > 0 ? a.q_out + r * a.out_stride : nullptr;
+  auto from = [&](int h) {
+    return h < nq ? q + h * HD : h < nq + nk ? k + (h - nq) * HD : v + (h - nq - nk) * HD;
+  };
+  v4f w[4] = {}, x[4], next[4];
+  t.load(from(h0), next);
+  for (int h = h0; h < h1; ++h) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = next[j];
+    t.load(from(min(h + 1, h1 - 1)), next);
+    const bool isq = h < nq;
+    if (h < nq + nk) {
+      const float *norm = isq ? a.nq : a.nk;
+      if (norm != nullptr && (h == h0 || h == nq)) t.load(norm, w);
+      t.turn(x, norm != nullptr, w, a.eps);
+    }
+    if (isq) {
+      if (there) t.store(out + h * HD, x);
+    } else {
+      const bool isv = h >= nq + nk;
+      const int head = isv ? h - nq - nk : h - nq;
+      t.template code<TYPE>(x, isv ? a.c.v : a.c.k, isv ? a.c.vs : a.c.ks,
+                            place < 0 ? -1 : place + ((long)head << a.c.shift));
+    }
+  }
+}
+
+// Heads in a call up to which lanes take one each, so that a few rows are one trip to memory;
+// beyond, rows go by Wide where they can, else lanes take four heads, which share the row's angles
+// and table look-ups.
 constexpr long kFewHeads = 16384;
+constexpr int kWideHeads = 8;  // that a wave of Wide takes of its rows
 
 }  // namespace
 
@@ -306,8 +539,12 @@ hipError_t launch_rope(const RopeRows &a, hipStream_t stream) {
     rope_kernel<g(), pairs(), h()><<<(unsigned)((units + 3) / 4), kThreads, 0, stream>>>(a);
   };
   auto heads = [&](auto g, auto pairs) {
-    (long)a.rows * a.heads <= kFewHeads ? go(g, pairs, std::integral_constant<int, 1>())
-                                        : go(g, pairs, std::integral_constant<int, 4>());
+    if ((long)a.rows * a.heads <= kFewHeads) return go(g, pairs, std::integral_constant<int, 1>());
+    if (!wide(a.hdim, a.rot)) return go(g, pairs, std::integral_constant<int, 4>());
+    constexpr int G = g() / 4;
+    const long waves = (a.rows + 64 / G - 1l) / (64 / G) * ((a.heads + kWideHeads - 1) / kWideHeads);
+    rope_wide_kernel<G, pairs()>
+        <<<(unsigned)((waves + 3) / 4), kThreads, 0, stream>>>(a, kWideHeads);
   };
   auto pairs = [&](auto g) {
     a.rot.pairs ? heads(g, std::true_type()) : heads(g, std::false_type());
@@ -327,8 +564,13 @@ hipError_t launch_kv_append(const KvAppend &a, hipStream_t stream) {
         <<<(unsigned)((units + 3) / 4), kThreads, 0, stream>>>(a);
   };
   auto heads = [&](auto g, auto type, auto pairs) {
-    (long)a.b.rows * all <= kFewHeads ? go(g, type, pairs, std::integral_constant<int, 1>())
-                                      : go(g, type, pairs, std::integral_constant<int, 4>());
+    if ((long)a.b.rows * all <= kFewHeads)
+      return go(g, type, pairs, std::integral_constant<int, 1>());
+    if (!wide(a.c.hdim, a.rot)) return go(g, type, pairs, std::integral_constant<int, 4>());
+    constexpr int G = g() / 4;
+    const long waves = (a.b.rows + 64 / G - 1l) / (64 / G) * ((all + kWideHeads - 1) / kWideHeads);
+    kv_append_wide_kernel<G, type(), pairs()>
+        <<<(unsigned)((waves + 3) / 4), kThreads, 0, stream>>>(a, kWideHeads);
   };
   auto pairs = [&](auto g, auto type) {
     a.rot.pairs ? heads(g, type, std::true_type()) : heads(g, type, std::false_type());
