@@ -315,20 +315,28 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void adapter_shrink_kernel(Adapt
   v4f acc[T];
 #pragma unroll
   for (int t = 0; t < T; ++t) acc[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-  Step next;
+  // two steps are on their way while one is multiplied
+  constexpr int kNext = kShrinkStep * kShrinkWaves;
+  Step one, two;
   typename Step::Lds &mine = sh.step[wave];
-  int k = kShrinkStep * wave;
-  if (k < a.k) next.load(x, m, k, a.k);
-  while (k < a.k) {
-    next.put(mine, k, a.k);
+  auto step = [&](Step &s, int k) {
+    s.put(mine, k, a.k);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    k += kShrinkStep * kShrinkWaves;
-    next.load(x, m, k, a.k);
+    s.load(x, m, k + 2 * kNext, a.k);
     __builtin_amdgcn_sched_barrier(0);  // asked for before the products, not where they are put
     Step::multiply(mine, acc);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
+  };
+  int k = kShrinkStep * wave;
+  if (k < a.k) {
+    one.load(x, m, k, a.k);
+    two.load(x, m, k + kNext, a.k);
+  }
+  for (; k < a.k; k += 2 * kNext) {
+    step(one, k);
+    if (k + kNext < a.k) step(two, k + kNext);
   }
   __syncthreads();
 #pragma unroll
@@ -437,7 +445,8 @@ __global__ __launch_bounds__(kThreads, KS == 1 && TYPE != kAdapterF32 ? 4 : 3) v
 #pragma unroll
     for (int j = 0; j < 4 * RT; ++j) {
       const int row = tile.row + min(4 * j + quarter, last);
-      old[j] = *reinterpret_cast<const v4f_any *>(a.base + row * a.base_stride + col);
+      old[j] = __builtin_nontemporal_load(  // read once
+          reinterpret_cast<const v4f_any *>(a.base + row * a.base_stride + col));
     }
   } else {
 #pragma unroll

@@ -83,7 +83,9 @@ __global__ __launch_bounds__(kThreads) void logprobs_scan_kernel(Logprobs a, Lay
   if (c0 + kTile <= a.vocab) {
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
-      const v4f_any v = *reinterpret_cast<const v4f_any *>(row + c0 + 256 * j + 4 * lane);
+      // past the caches' order of use: read once
+      const v4f_any v = __builtin_nontemporal_load(
+          reinterpret_cast<const v4f_any *>(row + c0 + 256 * j + 4 * lane));
 #pragma unroll
       for (int e = 0; e < 4; ++e) l[j][e] = v[e];
     }

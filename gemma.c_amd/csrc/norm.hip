@@ -20,14 +20,15 @@ namespace {
 
 constexpr int kNormNone = 0, kNormLayer = 2;
 
-// rows' chunks of four: NPT a thread, chunk j of thread t is t + j NT
+// rows' chunks of four: NPT a thread, chunk j of thread t is t + j NT; read past the caches' order of
+// use, as they are read once (4096 rows of 2560: 39 -> 37 us)
 template <int NPT, int NT>
 __device__ __forceinline__ void row_load(const float *p, int n4, v4f (&v)[NPT]) {
 #pragma unroll
   for (int j = 0; j < NPT; ++j) {
     const int c = threadIdx.x + j * NT;
     v[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    if (c < n4) v[j] = reinterpret_cast<const v4f *>(p)[c];
+    if (c < n4) v[j] = __builtin_nontemporal_load(reinterpret_cast<const v4f *>(p) + c);
   }
 }
 

@@ -327,9 +327,14 @@ struct Wide {
       s[n] *= (double)r.amp;
     }
   }
+  // ONCE: past the caches' order of use, for rows that are read once and don't fit
+  template <bool ONCE = false>
   __device__ __forceinline__ void load(const float *p, v4f (&x)[4]) const {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const v4f *>(p + 4 * (lane + G * j));
+    for (int j = 0; j < 4; ++j) {
+      const v4f *at = reinterpret_cast<const v4f *>(p + 4 * (lane + G * j));
+      x[j] = ONCE ? __builtin_nontemporal_load(at) : *at;
+    }
   }
   __device__ __forceinline__ void store(float *p, const v4f (&x)[4]) const {
 #pragma unroll
@@ -502,11 +507,11 @@ __global__ __launch_bounds__(kThreads) void kv_append_wide_kernel(KvAppend a, in
     return h < nq ? q + h * HD : h < nq + nk ? k + (h - nq) * HD : v + (h - nq - nk) * HD;
   };
   v4f w[4] = {}, x[4], next[4];
-  t.load(from(h0), next);
+  t.template load<true>(from(h0), next);
   for (int h = h0; h < h1; ++h) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) x[j] = next[j];
-    t.load(from(min(h + 1, h1 - 1)), next);
+    t.template load<true>(from(min(h + 1, h1 - 1)), next);
     const bool isq = h < nq;
     if (h < nq + nk) {
       const float *norm = isq ? a.nq : a.nk;
