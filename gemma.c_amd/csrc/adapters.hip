@@ -251,7 +251,7 @@ struct ShrinkStep {
     const int lane = threadIdx.x & 63, kx = k + 4 * (lane & 15);
     const int kw = k + 16 / kSize * (lane % kRowLanes);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const v4f *>(src[j] + (kx < end ? kx : 0));
+    for (int j = 0; j < 4; ++j) x[j] = __builtin_nontemporal_load(reinterpret_cast<const v4f *>(src[j] + (kx < end ? kx : 0)));
 #pragma unroll
     for (int j = 0; j < kLoads; ++j)
       w[j] = *reinterpret_cast<const u4 *>(m[j] + (size_t)(kw < end ? kw : 0) * kSize);
@@ -568,7 +568,7 @@ hipError_t launch_adapters(const Adapters &a, const DeviceInfo &dev, hipStream_t
     const integral_constant<int, 2> two;
     if (a.seq.max_rows <= kFewRows) return by_row(type);
     const int tiles = (all + 15) / 16;
-    tiles == 1 || (long)slots * tiles <= 2 * dev.cus ? shrink(type, one)
+    tiles == 1 || (long)slots * tiles <= dev.cus ? shrink(type, one)
     : tiles % kMostT != 0                            ? shrink(type, two)
                                                      : shrink(type, integral_constant<int, kMostT>());
     a.rank <= 32   ? expand(type, one, two)
