@@ -178,13 +178,17 @@ __device__ __forceinline__ float logit_of(u64 key) {
   return __uint_as_float(up & 0x80000000u ? up & 0x7fffffffu : ~up);
 }
 
-constexpr int kWaves = kThreads / 64;
-constexpr int kKeys = kMost / kThreads;  // of a thread, at most
-constexpr int kListed = kKeys * kLogprobsMaxTop;
+// The join's workgroups.  One row's has the card to itself, and what it takes is the length of a
+// wave's program: 1024 threads' is a third of 256 threads' (10 us).
+constexpr int kJoin = 1024, kWaves = kJoin / 64;
+constexpr int kKeys = kMost / kJoin;  // of a thread, at most
+constexpr int kFours = kJoin / 4;
+constexpr int kListed = 4 * kKeys * kLogprobsMaxTop;
 struct JoinShared {
-  u64 most[kThreads];
-  u64 list[kListed];
+  u64 most[kFours];
+  u64 list[kListed + 16];
   u64 best[kLogprobsMaxTop];
+  u64 least;
   double logs;
   float top;
   int count;
@@ -192,45 +196,69 @@ struct JoinShared {
   float given[kLogprobsMaxTargets];
 };
 
-// How many of n keys in LDS are above `mine`; sixteen are asked for at a time.
+// How many of n keys in LDS are above `mine`; sixteen are asked for at a time, behind the last too.
 __device__ __forceinline__ int above_in(const u64 *keys, int n, u64 mine) {
-  int above = 0, j = 0;
-  for (; j + 16 <= n; j += 16)
+  int above = 0;
+  for (int j = 0; j < n; j += 16)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) above += keys[j + i] > mine;
-  for (; j < n; ++j) above += keys[j] > mine;
+    for (int i = 0; i < 16; ++i) above += keys[j + i] > mine && j + i < n;
   return above;
 }
 
+template <int CTRL>
+__device__ __forceinline__ u64 dpp_u64(u64 v) {
+  return (u64)__double_as_longlong(dpp_f64<CTRL>(__longlong_as_double((long long)v)));
+}
+
 // Keys (no two alike but 0) of all threads into sh.list, their number into sh.count: the n largest
-// at least (all but 0 where there are fewer), and not many more.  Every wave looks for a bound that
-// n threads' largest keys reach, or a few more, bit by bit from the highest, and what reaches it is
-// listed: at most 64 threads' keys.
+// at least (all but 0 where there are fewer), and not many more.  One wave looks for a bound that the
+// largest keys of n groups of four threads reach, or a few more, bit by bit from the highest (with
+// every wave doing so, 3 us went by instead of 1), and what reaches it is listed: at most 64
+// groups' keys.
 template <int PER>
 __device__ __forceinline__ void list_largest(JoinShared &sh, int n, const u64 (&keys)[PER]) {
-  static_assert(PER <= kKeys && kListed >= kLogprobsMaxTop * PER, "the list holds 64 threads' keys");
+  static_assert(kListed >= kLogprobsMaxTop * 4 * PER, "the list holds 64 groups' keys");
   const int tid = threadIdx.x;
-  u64 most = 0;
+  u64 own = 0;
 #pragma unroll
-  for (int j = 0; j < PER; ++j) most = max(most, keys[j]);
-  sh.most[tid] = most;
+  for (int j = 0; j < PER; ++j) own = max(own, keys[j]);
+  u64 most = max(own, dpp_u64<kDppXor1>(own));
+  most = max(most, dpp_u64<kDppXor2>(most));
+  if ((tid & 3) == 0) sh.most[tid / 4] = most;
   if (tid == 0) sh.count = 0;
   __syncthreads();
-  const int enough = min(n + 8, kLogprobsMaxTop);
-  u64 other[kWaves], least = 0;
+  if (tid < 64) {
+    const int enough = min(n + 8, kLogprobsMaxTop);
+    u64 other[kFours / 64];
+    uint32_t high[kFours / 64], bound = 0;
 #pragma unroll
-  for (int j = 0; j < kWaves; ++j) other[j] = sh.most[(tid & 63) + 64 * j];
-  for (int bit = 63; bit >= 0; --bit) {
-    const u64 next = least | 1ull << bit;
-    int reach = 0;
+    for (int j = 0; j < kFours / 64; ++j) {
+      other[j] = sh.most[tid + 64 * j];
+      high[j] = (uint32_t)(other[j] >> 32);
+    }
+    bool found = false;
+    for (int bit = 31; bit >= 0 && !found; --bit) {
+      const uint32_t next = bound | 1u << bit;
+      int reach = 0;
 #pragma unroll
-    for (int j = 0; j < kWaves; ++j) reach += __popcll(__ballot(other[j] >= next));
-    if (reach < n) continue;
-    least = next;
-    if (reach <= enough) break;
+      for (int j = 0; j < kFours / 64; ++j) reach += __popcll(__ballot(high[j] >= next));
+      bound = reach >= n ? next : bound;
+      found = reach >= n && reach <= enough;
+    }
+    u64 least = (u64)bound << 32;
+    for (int bit = 31; bit >= 0 && !found; --bit) {  // equals, by their indices
+      const u64 next = least | 1ull << bit;
+      int reach = 0;
+#pragma unroll
+      for (int j = 0; j < kFours / 64; ++j) reach += __popcll(__ballot(other[j] >= next));
+      least = reach >= n ? next : least;
+      found = reach >= n && reach <= enough;
+    }
+    if (tid == 0) sh.least = max(least, (u64)1);  // (0: fewer than n)
   }
-  if (least == 0) least = 1;  // fewer than n
-  if (most >= least) {
+  __syncthreads();
+  const u64 least = sh.least;
+  if (own >= least) {
     int mine = 0;
 #pragma unroll
     for (int j = 0; j < PER; ++j) mine += keys[j] >= least;
@@ -245,7 +273,7 @@ __device__ __forceinline__ void list_largest(JoinShared &sh, int n, const u64 (&
 // The list's n largest, in order, into sh.best, 0 where there are fewer.
 __device__ __forceinline__ void rank_list(JoinShared &sh, int n) {
   const int count = sh.count;
-  for (int i = threadIdx.x; i < count; i += kThreads) {
+  for (int i = threadIdx.x; i < count; i += kJoin) {
     const u64 mine = sh.list[i];
     const int rank = above_in(sh.list, count, mine);
     if (rank < n) sh.best[rank] = mine;
@@ -254,104 +282,85 @@ __device__ __forceinline__ void rank_list(JoinShared &sh, int n) {
   __syncthreads();
 }
 
-// S and T of the row's parts by its largest logit, by one wave.
-__device__ __forceinline__ void join_parts(JoinShared &sh, const Part *parts, int tiles, bool drawn,
+// S and T of the row's parts by its largest logit, by one wave; c: octaves a logit.
+template <int PARTS>
+__device__ __forceinline__ void join_parts(JoinShared &sh, const Part (&p)[PARTS], bool drawn,
                                            double c, float *entropy) {
-  constexpr int kPer = kMaxTiles / 64;
-  static_assert(kMaxTiles % 64 == 0, "a lane has so many parts");
-  const int lane = threadIdx.x & 63;
-  Part p[kPer];
   float top = -INFINITY;
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    const int i = lane + 64 * j;
-    p[j] = i < tiles ? parts[i] : Part{-INFINITY, 0.0f, 0.0f};
-    top = fmaxf(top, p[j].m);
-  }
+  for (int j = 0; j < PARTS; ++j) top = fmaxf(top, p[j].m);
   top = wave_max_dpp(top);
   double s = 0.0, t = 0.0;
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) {
+  for (int j = 0; j < PARTS; ++j) {
     if (!(p[j].m > -INFINITY)) continue;
-    const double x = top == p[j].m ? 0.0 : ((double)p[j].m - (double)top) * c;  // (-inf below +inf)
-    const double w = x > -1000.0 ? exp2(x) : 0.0;
+    double x = top == p[j].m ? 0.0 : ((double)p[j].m - (double)top) * c;  // (-inf below +inf)
+    x = fmax(x, -1000.0);
+    // 2^x: e^y for what is left of the nearest whole number, by Taylor's polynomial (y^9 / 9! is
+    // below 3e-10)
+    const double whole = rint(x), y = (x - whole) * 0x1.62e42fefa39efp-1;
+    double e = fma(y, 1.0 / 40320.0, 1.0 / 5040.0);
+    e = fma(y, e, 1.0 / 720.0);
+    e = fma(y, e, 1.0 / 120.0);
+    e = fma(y, e, 1.0 / 24.0);
+    e = fma(y, e, 1.0 / 6.0);
+    e = fma(y, e, 0.5);
+    e = fma(y, e, 1.0);
+    const double w = ldexp(fma(y, e, 1.0), (int)whole);
     s = fma(w, (double)p[j].s, s);
-    t += w > 0.0 ? w * ((double)p[j].t + (double)p[j].s * x) : 0.0;
+    t = fma(w, (double)p[j].t + (double)p[j].s * x, t);
   }
   s = wave_sum_f64(s);
   t = wave_sum_f64(t);
   const double ln2 = 0x1.62e42fefa39efp-1, logs = log(s);
-  if (lane != 0) return;
+  if ((threadIdx.x & 63) != 0) return;
   sh.top = top;
   sh.logs = logs;
   if (entropy != nullptr)
     *entropy = drawn && top > -INFINITY ? (float)fmax(0.0, logs - ln2 * t / s) : 0.0f;
 }
 
-// RUNS: of a thread, at most.  Most of a row's join is waiting: everything that doesn't hang on
-// something else is asked for at once, the parts are one wave's, the given tokens the others'.
+// RUNS: of a thread, at most.  A row's join is mostly waiting, so it takes two trips to memory: for
+// the runs and what else is there, and then for the columns of the runs that matter, while one wave
+// joins the parts and the others look up the given tokens.
 template <int RUNS>
-__global__ __launch_bounds__(kThreads) void logprobs_join_kernel(Logprobs a, Layout at) {
+__global__ __launch_bounds__(kJoin) void logprobs_join_kernel(Logprobs a, Layout at) {
   __shared__ JoinShared sh;
   const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, tiles = tiles_of(a.vocab);
   const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const float *row = a.logits + r * a.stride;
   const float *runs = reinterpret_cast<const float *>(a.work + at.runs) +
                       (size_t)r * tiles * kTileRuns;
+  const Part *parts = reinterpret_cast<const Part *>(a.work + at.parts) + (size_t)r * tiles;
   const int nruns = a.ntop > 0 ? (a.vocab + kRun - 1) / kRun : 0;
   float most[RUNS];
 #pragma unroll
   for (int j = 0; j < RUNS; ++j) {
-    const int i = tid + j * kThreads;
+    const int i = tid + j * kJoin;
     most[j] = i < nruns ? runs[i] : -INFINITY;
   }
   const float temp = a.temperature != nullptr ? a.temperature[r] : 1.0f;
-  const bool drawn = temp > 0.0f;
-  if (wave == kWaves - 1) {
-    const double c = drawn ? fmin(0x1.71547652b82fep+0 / (double)temp, (double)FLT_MAX) : 0.0;
-    join_parts(sh, reinterpret_cast<const Part *>(a.work + at.parts) + (size_t)r * tiles, tiles,
-               drawn, c, a.entropy != nullptr ? a.entropy + r : nullptr);
-  } else {
-    const int *counts = reinterpret_cast<const int *>(a.work + at.counts) +
-                        (size_t)r * tiles * a.targets;
-    for (int k = wave; k < a.targets; k += kWaves - 1) {
-      const int id = a.ids[(size_t)r * a.targets + k];
-      const bool there = (unsigned)id < (unsigned)a.vocab;
-      const float given = there ? no_nan(row[id]) : -INFINITY;
-      int above = 0;
-      for (int j = lane; j < tiles; j += 64) above += counts[(size_t)j * a.targets + k];
-      above = group_sum_i32<64>(above);
-      if (lane == 0) sh.above[k] = there ? above : -1, sh.given[k] = given;
-    }
+  const bool drawn = temp > 0.0f, joins = wave == kWaves - 1;
+  constexpr int kParts = (RUNS * kJoin / kTileRuns + 63) / 64;  // of a lane
+  Part part[kParts];
+#pragma unroll
+  for (int j = 0; j < kParts; ++j) {
+    const int i = lane + 64 * j;
+    part[j] = joins && i < tiles ? parts[i] : Part{-INFINITY, 0.0f, 0.0f};
   }
+  int id = !joins && wave < a.targets ? a.ids[(size_t)r * a.targets + wave] : -1;
+  // the runs that matter, as they were listed unless they are too many
+  int chosen = 0;
+  bool few = true;
   if (a.ntop > 0) {
     u64 keys[RUNS];
 #pragma unroll
-    for (int j = 0; j < RUNS; ++j) keys[j] = key_of(most[j], tid + j * kThreads);
+    for (int j = 0; j < RUNS; ++j) keys[j] = key_of(most[j], tid + j * kJoin);
     list_largest(sh, a.ntop, keys);
-  } else {
-    __syncthreads();
+    few = sh.count <= kLogprobsMaxTop;
+    if (!few) rank_list(sh, a.ntop);
+    chosen = few ? sh.count : a.ntop;
   }
-  const float top = sh.top;
-  const double logs = sh.logs;
-  // log p of a logit that isn't NaN; first: whether it is the row's first largest
-  auto logp = [&](float l, bool first) -> float {
-    if (!(l > -INFINITY)) return -INFINITY;
-    if (!drawn) return first ? 0.0f : -INFINITY;
-    if (l == top) return (float)(0.0 - logs);
-    return (float)(((double)l - (double)top) / (double)temp - logs);
-  };
-  if (tid < a.targets) {
-    const size_t to = (size_t)r * a.targets + tid;
-    const int above = sh.above[tid];
-    if (a.rank != nullptr) a.rank[to] = above + 1;
-    if (a.logp != nullptr) a.logp[to] = logp(sh.given[tid], above == 0);
-  }
-  if (a.ntop == 0) return;
-  // the runs that matter, as they were listed unless they are too many
-  const bool few = sh.count <= kLogprobsMaxTop;
-  if (!few) rank_list(sh, a.ntop);
-  const int chosen = few ? sh.count : a.ntop;
   // a wave a run: its columns are the threads' keys
   float l[kLogprobsMaxTop / kWaves];
   int col[kLogprobsMaxTop / kWaves];
@@ -363,12 +372,46 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(Logprobs a, Lay
     col[j] = index_of(few ? sh.list[i] : sh.best[i]) * kRun + lane;
     if (col[j] < a.vocab) l[j] = row[col[j]];
   }
-  u64 mine[kLogprobsMaxTop / kWaves];
-#pragma unroll
-  for (int j = 0; j < kLogprobsMaxTop / kWaves; ++j) mine[j] = key_of(l[j], col[j]);
+  if (joins) {
+    const double c = drawn ? fmin(0x1.71547652b82fep+0 / (double)temp, (double)FLT_MAX) : 0.0;
+    join_parts(sh, part, drawn, c, a.entropy != nullptr ? a.entropy + r : nullptr);
+  } else {
+    const int *counts = reinterpret_cast<const int *>(a.work + at.counts) +
+                        (size_t)r * tiles * a.targets;
+    for (int k = wave; k < a.targets; k += kWaves - 1) {
+      if (k != wave) id = a.ids[(size_t)r * a.targets + k];
+      const bool there = (unsigned)id < (unsigned)a.vocab;
+      const float given = there ? no_nan(row[id]) : -INFINITY;
+      int above = 0;
+      for (int j = lane; j < tiles; j += 64) above += counts[(size_t)j * a.targets + k];
+      above = group_sum_i32<64>(above);
+      if (lane == 0) sh.above[k] = there ? above : -1, sh.given[k] = given;
+    }
+  }
   __syncthreads();
-  list_largest(sh, a.ntop, mine);
-  rank_list(sh, a.ntop);
+  if (a.ntop > 0) {
+    u64 mine[kLogprobsMaxTop / kWaves];
+#pragma unroll
+    for (int j = 0; j < kLogprobsMaxTop / kWaves; ++j) mine[j] = key_of(l[j], col[j]);
+    list_largest(sh, a.ntop, mine);
+    rank_list(sh, a.ntop);
+  }
+  const float top = sh.top;
+  const double logs = sh.logs;
+  const double per = 1.0 / (double)temp;
+  // log p of a logit that isn't NaN; first: whether it is the row's first largest
+  auto logp = [&](float l, bool first) -> float {
+    if (!(l > -INFINITY)) return -INFINITY;
+    if (!drawn) return first ? 0.0f : -INFINITY;
+    if (l == top) return (float)(0.0 - logs);
+    return (float)(((double)l - (double)top) * per - logs);
+  };
+  if (tid < a.targets) {
+    const size_t to = (size_t)r * a.targets + tid;
+    const int above = sh.above[tid];
+    if (a.rank != nullptr) a.rank[to] = above + 1;
+    if (a.logp != nullptr) a.logp[to] = logp(sh.given[tid], above == 0);
+  }
   if (tid < a.ntop) {
     const u64 k = sh.best[tid];
     const size_t to = (size_t)r * a.ntop + tid;
@@ -391,11 +434,11 @@ hipError_t launch_logprobs(const Logprobs &a, hipStream_t stream) {
   a.ntop > 0 ? logprobs_scan_kernel<true><<<grid, kThreads, 0, stream>>>(a, at)
              : logprobs_scan_kernel<false><<<grid, kThreads, 0, stream>>>(a, at);
   const auto join = [&](auto runs) {
-    logprobs_join_kernel<runs()><<<a.rows, kThreads, 0, stream>>>(a, at);
+    logprobs_join_kernel<runs()><<<a.rows, kJoin, 0, stream>>>(a, at);
   };
-  a.vocab <= 4 * kThreads * kRun    ? join(std::integral_constant<int, 4>())
-  : a.vocab <= 16 * kThreads * kRun ? join(std::integral_constant<int, 16>())
-                                    : join(std::integral_constant<int, kKeys>());
+  a.vocab <= kJoin * kRun       ? join(std::integral_constant<int, 1>())
+  : a.vocab <= 4 * kJoin * kRun ? join(std::integral_constant<int, 4>())
+                                : join(std::integral_constant<int, kKeys>());
   return hipGetLastError();
 }
 
