@@ -11,7 +11,7 @@
 // of the piece products those are summed whose orders add up to at most 2 (3, 5 or 6 of
 // them: what is left out is below 2^-22 of a product).  A tile is one sequence's: with tiles across
 // sequences, which took a pass for each adapter, the few that had two set the time.  Single tokens
-// take a wave for a value of u and a lane for a value of dst.
+// take a wave for a value of u and a wave for 64 of dst.
 #include <type_traits>
 
 #include "gh_arith.h"
@@ -158,31 +158,6 @@ __global__ __launch_bounds__(kThreads) void adapter_shrink_row_kernel(Adapters a
   }
   s = group_sum_f32<64>(s);
   if (lane == 0) u_of(a)[(size_t)r * all + at] = scale_of(a, id) * s;
-}
-
-template <int TYPE>
-__global__ __launch_bounds__(kThreads) void adapter_expand_row_kernel(Adapters a) {
-  const int n = a.end[a.njobs - 1], r = blockIdx.x;
-  const int c = blockIdx.y * kThreads + threadIdx.x;
-  const int id = ids_of(a)[r];
-  if (id == kOutside || c >= n) return;
-  float v = a.base[r * a.base_stride + c];
-  if (id >= 0) {
-    const int job = c < a.end[0] ? 0 : a.njobs < 3 || c < a.end[1] ? 1 : 2;
-    const int from = job == 0 ? 0 : a.end[job - 1];
-    const void *m = job_of(a.b, job);
-    const size_t first = ((size_t)id * (a.end[job] - from) + (c - from)) * a.rank;
-    const float *u = u_of(a) + ((size_t)r * a.njobs + job) * a.rank;
-    float s = 0.0f;
-    for (int k = 0; k < a.rank; k += 8) {
-      float w[8];
-      floats8<TYPE>(raw8<TYPE>(m, first + k), w);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s = fmaf(u[k + e], w[e], s);
-    }
-    v += s;
-  }
-  a.dst[r * a.dst_stride + c] = v;
 }
 
 // ---- tiles of rows ------------------------------------------------------------------
@@ -370,6 +345,84 @@ __host__ __device__ inline int expand_units(const int (&end)[kAdapterMaxJobs], i
   return n;
 }
 
+// Where unit u's 64 columns lie: a job, its columns' first and how many it has, the unit's first of
+// them.
+struct ExpandUnit {
+  int job, begin, width, c0;
+};
+__device__ __forceinline__ ExpandUnit expand_unit(const Adapters &a, int unit) {
+  ExpandUnit u = {0, 0, a.end[0], 0};
+  for (; u.job < a.njobs; ++u.job) {
+    u.begin = u.job == 0 ? 0 : a.end[u.job - 1];
+    u.width = a.end[u.job] - u.begin;
+    const int units = (u.width + kExpandCols - 1) / kExpandCols;
+    if (unit < units) break;
+    unit -= units;
+  }
+  u.c0 = unit * kExpandCols;
+  return u;
+}
+
+// dst of a row and 64 columns of a job a wave.  B's part is one run of memory, read 16 bytes a lane
+// (CHUNKS a row of it at most); their products with u meet in LDS, where a lane has a column.
+template <int TYPE, int CHUNKS>
+__global__ __launch_bounds__(kThreads) void adapter_expand_row_kernel(Adapters a) {
+  constexpr int kSize = TYPE == kAdapterF32 ? 4 : 2, kOf = 16 / kSize;  // weights a chunk
+  constexpr int kFlight = CHUNKS < 8 ? CHUNKS : 8;  // read together
+  constexpr int kNowhere = kExpandCols * (CHUNKS + 1);
+  __shared__ float sums[kThreads / 64][kNowhere + 1];
+  const int lane = threadIdx.x & 63, r = blockIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const ExpandUnit x = expand_unit(a, blockIdx.y * (kThreads / 64) + wave);
+  if (x.job == a.njobs) return;
+  const int id = ids_of(a)[r], c = x.c0 + lane;
+  if (id == kOutside) return;
+  float v = c < x.width ? a.base[r * a.base_stride + x.begin + c] : 0.0f;
+  if (id >= 0) {
+    const int chunks = a.rank / kOf, all = min(kExpandCols, x.width - x.c0) * chunks;
+    const unsigned share = (65536 + chunks - 1) / chunks;  // i / chunks is i share / 65536
+    const u4 *b = reinterpret_cast<const u4 *>(
+        reinterpret_cast<const char *>(job_of(a.b, x.job)) +
+        ((size_t)id * x.width + x.c0) * a.rank * kSize);
+    const float *u = u_of(a) + ((size_t)r * a.njobs + x.job) * a.rank;
+    for (int j0 = 0; j0 < chunks; j0 += kFlight) {
+      u4 w[kFlight];
+#pragma unroll
+      for (int j = 0; j < kFlight; ++j) {
+        const int i = lane + 64 * (j0 + j);
+        w[j] = b[i < all ? i : 0];
+      }
+#pragma unroll
+      for (int j = 0; j < kFlight; ++j) {
+        const int i = lane + 64 * (j0 + j);
+        const int col = (int)(i * share >> 16), p = i - col * chunks;
+        float s = 0.0f;
+        if constexpr (TYPE == kAdapterF32) {
+          const v4f at = *reinterpret_cast<const v4f *>(u + kOf * p);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s = fmaf(at[e], __uint_as_float(w[j][e]), s);
+        } else {
+          float f[8];
+          floats8<TYPE>(Raw8<TYPE>{{w[j]}}, f);
+          const v4f lo = *reinterpret_cast<const v4f *>(u + kOf * p);
+          const v4f hi = *reinterpret_cast<const v4f *>(u + kOf * p + 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s = fmaf(lo[e], f[e], s), s = fmaf(hi[e], f[e + 4], s);
+        }
+        // (no branch, which would take the loads with it, one after the other)
+        sums[wave][j0 + j < chunks ? col * (chunks + 1) + p : kNowhere] = s;
+      }
+    }
+    // written and read by the same wave, whose LDS accesses keep their order
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    float s = 0.0f;
+    for (int p = 0; p < chunks; ++p) s += sums[wave][lane * (chunks + 1) + p];
+    v += s;
+  }
+  if (c < x.width) a.dst[r * a.dst_stride + x.begin + c] = v;
+}
+
 // dst of 16 RT rows and 64 columns of a job a wave; KS: steps of 32 of the rank.  base and dst are
 // read and written by whole runs of 256 bytes; the products, whose lanes have a row each, go through
 // LDS.  A workgroup's four waves are WR times as many rows by 4 / WR times as many columns: 4 by 1,
@@ -383,20 +436,13 @@ __global__ __launch_bounds__(kThreads, KS == 1 && TYPE != kAdapterF32 ? 4 : 3) v
   __shared__ char shared[WR > 1 ? kExpandCols : 1][kPitch];
   const int lane = threadIdx.x & 63, m = lane & 15, quarter = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  int unit = WR > 1 ? blockIdx.y : blockIdx.y * kWaves + wave;
-  int job = 0, begin = 0, width = a.end[0];
-  for (; job < a.njobs; ++job) {
-    begin = job == 0 ? 0 : a.end[job - 1];
-    width = a.end[job] - begin;
-    const int units = (width + kExpandCols - 1) / kExpandCols;
-    if (unit < units) break;
-    unit -= units;
-  }
+  const ExpandUnit x = expand_unit(a, WR > 1 ? blockIdx.y : blockIdx.y * kWaves + wave);
+  const int job = x.job, begin = x.begin, width = x.width, c0 = x.c0;
   if (job == a.njobs) return;
   float(&sums)[16 * RT][kExpandPitch] = tiles[wave];
   Tile tile = tile_at<16 * RT * WR>(a, blockIdx.x);
   if (tile.rows <= 0) return;
-  const int k0 = 8 * quarter, c0 = unit * kExpandCols;
+  const int k0 = 8 * quarter;
   const char *b = reinterpret_cast<const char *>(job_of(a.b, job)) +
                   ((size_t)tile.id * width + c0) * a.rank * kSize;
   const int chunks = a.rank * kSize / 16;  // of a row of B
@@ -541,11 +587,18 @@ size_t adapters_work(int rows, int njobs, int rank) {
 }
 
 hipError_t launch_adapters(const Adapters &a, const DeviceInfo &dev, hipStream_t stream) {
-  const int rows = a.seq.rows, all = a.njobs * a.rank, n = a.end[a.njobs - 1];
+  const int rows = a.seq.rows, all = a.njobs * a.rank;
   auto by_row = [&](auto type) {
-    const dim3 first(rows, (all + 3) / 4), second(rows, (n + kThreads - 1) / kThreads);
+    constexpr int kSize = type() == kAdapterF32 ? 4 : 2;
+    const dim3 first(rows, (all + 3) / 4);
+    const dim3 second(rows, (expand_units(a.end, a.njobs) + 3) / 4);
     adapter_shrink_row_kernel<type()><<<first, kThreads, 0, stream>>>(a);
-    adapter_expand_row_kernel<type()><<<second, kThreads, 0, stream>>>(a);
+    auto expand_row = [&](auto chunks) {
+      adapter_expand_row_kernel<type(), chunks()><<<second, kThreads, 0, stream>>>(a);
+    };
+    a.rank * kSize <= 32    ? expand_row(std::integral_constant<int, 2>())
+    : a.rank * kSize <= 128 ? expand_row(std::integral_constant<int, 8>())
+                            : expand_row(std::integral_constant<int, kAdapterMaxRank * kSize / 16>());
   };
   const int slots = tile_slots(a.seq, 16);
   auto shrink = [&](auto type, auto t) {

@@ -1339,7 +1339,7 @@ int gemma_hip_rope(float *dst, int dst_stride, const float *src, int src_stride,
   const gh::Rotary rot = a.rot;
   a = gh::RopeRows{dst, src, pos, norm, dst_stride, src_stride, rows, heads, hdim, eps, rot};
   PerfScope perf(kOpRope, pick_stream(stream));
-  GH_CHECK("gemma_hip_rope: launch", gh::launch_rope(a, pick_stream(stream)));
+  GH_CHECK("gemma_hip_rope: launch", gh::launch_rope(a, g.info, pick_stream(stream)));
   return 0;
 }
 
@@ -1374,7 +1374,7 @@ int gemma_hip_cache_append(const gemma_hip_cache *cache, const gemma_hip_batch *
   a.q_stride = qs, a.k_stride = ks, a.v_stride = vs, a.out_stride = os;
   a.n_heads = nq, a.nq = heads->nq, a.nk = heads->nk, a.eps = heads->eps;
   PerfScope perf(kOpRope, pick_stream(stream));
-  GH_CHECK("gemma_hip_cache_append: launch", gh::launch_kv_append(a, pick_stream(stream)));
+  GH_CHECK("gemma_hip_cache_append: launch", gh::launch_kv_append(a, g.info, pick_stream(stream)));
   return 0;
 }
 
@@ -1427,7 +1427,7 @@ int gemma_hip_norm_residual(const gemma_hip_residual *residual, int rows, int di
   a.rows = rows, a.dim = dim;
   const bool layer = v.before.kind == GEMMA_HIP_NORM_LAYER || v.after.kind == GEMMA_HIP_NORM_LAYER;
   PerfScope perf(layer ? kOpLayernorm : kOpRmsnorm, pick_stream(stream));
-  GH_CHECK("gemma_hip_norm_residual: launch", gh::launch_norm_residual(a, pick_stream(stream)));
+  GH_CHECK("gemma_hip_norm_residual: launch", gh::launch_norm_residual(a, g.info, pick_stream(stream)));
   return 0;
 }
 
@@ -1548,7 +1548,7 @@ int gemma_hip_logprobs(const gemma_hip_scores *scores, const float *logits, int 
     return 1;
   {
     PerfScope perf(kOpSample, s);
-    GH_CHECK("gemma_hip_logprobs: launch", gh::launch_logprobs(a, s));
+    GH_CHECK("gemma_hip_logprobs: launch", gh::launch_logprobs(a, g.info, s));
   }
   if (hold) GH_CHECK("gemma_hip_logprobs", hold->done());
   return 0;

@@ -440,7 +440,7 @@ struct RopeRows {
   float eps;
   Rotary rot;
 };
-hipError_t launch_rope(const RopeRows &a, hipStream_t stream);
+hipError_t launch_rope(const RopeRows &a, const DeviceInfo &dev, hipStream_t stream);
 // the batch's new rows of q into q_out, of k and v into the cache, q by the norm of nq and the
 // turn, k by those of nk; q may be null
 struct KvAppend {
@@ -454,7 +454,7 @@ struct KvAppend {
   KvCache c;
   KvBatch b;
 };
-hipError_t launch_kv_append(const KvAppend &a, hipStream_t stream);
+hipError_t launch_kv_append(const KvAppend &a, const DeviceInfo &dev, hipStream_t stream);
 
 // norm.hip: per row x' = clamp(cx x + cy gate after(y)), h = before(x') as fp32 and, when hq is
 // given, as codes.  A norm's kind: 0 none, 1 by the root of the mean square, 2 with the mean taken
@@ -475,7 +475,7 @@ struct NormResidual {
   int rows, dim;
 };
 constexpr int kNormMaxDim = 24576;
-hipError_t launch_norm_residual(const NormResidual &a, hipStream_t stream);
+hipError_t launch_norm_residual(const NormResidual &a, const DeviceInfo &dev, hipStream_t stream);
 
 // adapters.hip: dst row = base row + scale[id] B[id] (A[id] src row), id that of the row's
 // sequence; rows whose id is none of 0 .. count - 1 are base.  Job j: a [count][rank][k],
@@ -514,7 +514,7 @@ struct Logprobs {
   char *work;
 };
 size_t logprobs_work(int rows, int vocab, int targets, int ntop);
-hipError_t launch_logprobs(const Logprobs &a, hipStream_t stream);
+hipError_t launch_logprobs(const Logprobs &a, const DeviceInfo &dev, hipStream_t stream);
 
 // sample.hip: one token per row of logits.  Settings are device arrays of a value
 // per row, or null.

@@ -178,14 +178,12 @@ __device__ __forceinline__ float logit_of(u64 key) {
   return __uint_as_float(up & 0x80000000u ? up & 0x7fffffffu : ~up);
 }
 
-// The join's workgroups.  One row's has the card to itself, and what it takes is the length of a
-// wave's program: 1024 threads' is a third of 256 threads' (10 us).
-constexpr int kJoin = 1024, kWaves = kJoin / 64;
-constexpr int kKeys = kMost / kJoin;  // of a thread, at most
-constexpr int kFours = kJoin / 4;
-constexpr int kListed = 4 * kKeys * kLogprobsMaxTop;
+// The join's workgroups have 1024 threads, as one row's time is the length of a wave's program, or
+// 256 where rows are many and their sum counts; keys are looked at by 256 groups of one or four.
+constexpr int kGroups = 256;
+constexpr int kListed = kMost / kGroups * kLogprobsMaxTop;
 struct JoinShared {
-  u64 most[kFours];
+  u64 most[kGroups];
   u64 list[kListed + 16];
   u64 best[kLogprobsMaxTop];
   u64 least;
@@ -212,27 +210,32 @@ __device__ __forceinline__ u64 dpp_u64(u64 v) {
 
 // Keys (no two alike but 0) of all threads into sh.list, their number into sh.count: the n largest
 // at least (all but 0 where there are fewer), and not many more.  One wave looks for a bound that the
-// largest keys of n groups of four threads reach, or a few more, bit by bit from the highest (with
+// largest keys of n groups reach, or a few more, bit by bit from the highest (with
 // every wave doing so, 3 us went by instead of 1), and what reaches it is listed: at most 64
 // groups' keys.
-template <int PER>
+template <int NT, int PER>
 __device__ __forceinline__ void list_largest(JoinShared &sh, int n, const u64 (&keys)[PER]) {
-  static_assert(kListed >= kLogprobsMaxTop * 4 * PER, "the list holds 64 groups' keys");
+  constexpr int GROUP = NT / kGroups;
+  static_assert(GROUP == 1 || GROUP == 4, "a group is a lane or a quad");
+  static_assert(kListed >= kLogprobsMaxTop * GROUP * PER, "the list holds 64 groups' keys");
   const int tid = threadIdx.x;
   u64 own = 0;
 #pragma unroll
   for (int j = 0; j < PER; ++j) own = max(own, keys[j]);
-  u64 most = max(own, dpp_u64<kDppXor1>(own));
-  most = max(most, dpp_u64<kDppXor2>(most));
-  if ((tid & 3) == 0) sh.most[tid / 4] = most;
+  u64 most = own;
+  if (GROUP == 4) {
+    most = max(most, dpp_u64<kDppXor1>(most));
+    most = max(most, dpp_u64<kDppXor2>(most));
+  }
+  if (tid % GROUP == 0) sh.most[tid / GROUP] = most;
   if (tid == 0) sh.count = 0;
   __syncthreads();
   if (tid < 64) {
     const int enough = min(n + 8, kLogprobsMaxTop);
-    u64 other[kFours / 64];
-    uint32_t high[kFours / 64], bound = 0;
+    u64 other[kGroups / 64];
+    uint32_t high[kGroups / 64], bound = 0;
 #pragma unroll
-    for (int j = 0; j < kFours / 64; ++j) {
+    for (int j = 0; j < kGroups / 64; ++j) {
       other[j] = sh.most[tid + 64 * j];
       high[j] = (uint32_t)(other[j] >> 32);
     }
@@ -241,7 +244,7 @@ __device__ __forceinline__ void list_largest(JoinShared &sh, int n, const u64 (&
       const uint32_t next = bound | 1u << bit;
       int reach = 0;
 #pragma unroll
-      for (int j = 0; j < kFours / 64; ++j) reach += __popcll(__ballot(high[j] >= next));
+      for (int j = 0; j < kGroups / 64; ++j) reach += __popcll(__ballot(high[j] >= next));
       bound = reach >= n ? next : bound;
       found = reach >= n && reach <= enough;
     }
@@ -250,7 +253,7 @@ __device__ __forceinline__ void list_largest(JoinShared &sh, int n, const u64 (&
       const u64 next = least | 1ull << bit;
       int reach = 0;
 #pragma unroll
-      for (int j = 0; j < kFours / 64; ++j) reach += __popcll(__ballot(other[j] >= next));
+      for (int j = 0; j < kGroups / 64; ++j) reach += __popcll(__ballot(other[j] >= next));
       least = reach >= n ? next : least;
       found = reach >= n && reach <= enough;
     }
@@ -271,9 +274,10 @@ __device__ __forceinline__ void list_largest(JoinShared &sh, int n, const u64 (&
 }
 
 // The list's n largest, in order, into sh.best, 0 where there are fewer.
+template <int NT>
 __device__ __forceinline__ void rank_list(JoinShared &sh, int n) {
   const int count = sh.count;
-  for (int i = threadIdx.x; i < count; i += kJoin) {
+  for (int i = threadIdx.x; i < count; i += NT) {
     const u64 mine = sh.list[i];
     const int rank = above_in(sh.list, count, mine);
     if (rank < n) sh.best[rank] = mine;
@@ -323,8 +327,9 @@ __device__ __forceinline__ void join_parts(JoinShared &sh, const Part (&p)[PARTS
 // RUNS: of a thread, at most.  A row's join is mostly waiting, so it takes two trips to memory: for
 // the runs and what else is there, and then for the columns of the runs that matter, while one wave
 // joins the parts and the others look up the given tokens.
-template <int RUNS>
-__global__ __launch_bounds__(kJoin) void logprobs_join_kernel(Logprobs a, Layout at) {
+template <int NT, int RUNS>
+__global__ __launch_bounds__(NT) void logprobs_join_kernel(Logprobs a, Layout at) {
+  constexpr int kWaves = NT / 64;
   __shared__ JoinShared sh;
   const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, tiles = tiles_of(a.vocab);
   const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
@@ -336,12 +341,12 @@ __global__ __launch_bounds__(kJoin) void logprobs_join_kernel(Logprobs a, Layout
   float most[RUNS];
 #pragma unroll
   for (int j = 0; j < RUNS; ++j) {
-    const int i = tid + j * kJoin;
+    const int i = tid + j * NT;
     most[j] = i < nruns ? runs[i] : -INFINITY;
   }
   const float temp = a.temperature != nullptr ? a.temperature[r] : 1.0f;
   const bool drawn = temp > 0.0f, joins = wave == kWaves - 1;
-  constexpr int kParts = (RUNS * kJoin / kTileRuns + 63) / 64;  // of a lane
+  constexpr int kParts = (RUNS * NT / kTileRuns + 63) / 64;  // of a lane
   Part part[kParts];
 #pragma unroll
   for (int j = 0; j < kParts; ++j) {
@@ -355,10 +360,10 @@ __global__ __launch_bounds__(kJoin) void logprobs_join_kernel(Logprobs a, Layout
   if (a.ntop > 0) {
     u64 keys[RUNS];
 #pragma unroll
-    for (int j = 0; j < RUNS; ++j) keys[j] = key_of(most[j], tid + j * kJoin);
-    list_largest(sh, a.ntop, keys);
+    for (int j = 0; j < RUNS; ++j) keys[j] = key_of(most[j], tid + j * NT);
+    list_largest<NT>(sh, a.ntop, keys);
     few = sh.count <= kLogprobsMaxTop;
-    if (!few) rank_list(sh, a.ntop);
+    if (!few) rank_list<NT>(sh, a.ntop);
     chosen = few ? sh.count : a.ntop;
   }
   // a wave a run: its columns are the threads' keys
@@ -393,8 +398,8 @@ __global__ __launch_bounds__(kJoin) void logprobs_join_kernel(Logprobs a, Layout
     u64 mine[kLogprobsMaxTop / kWaves];
 #pragma unroll
     for (int j = 0; j < kLogprobsMaxTop / kWaves; ++j) mine[j] = key_of(l[j], col[j]);
-    list_largest(sh, a.ntop, mine);
-    rank_list(sh, a.ntop);
+    list_largest<NT>(sh, a.ntop, mine);
+    rank_list<NT>(sh, a.ntop);
   }
   const float top = sh.top;
   const double logs = sh.logs;
@@ -427,18 +432,24 @@ size_t logprobs_work(int rows, int vocab, int targets, int ntop) {
   return layout_of(rows, vocab, targets, ntop).all;
 }
 
-hipError_t launch_logprobs(const Logprobs &a, hipStream_t stream) {
+hipError_t launch_logprobs(const Logprobs &a, const DeviceInfo &dev, hipStream_t stream) {
   const Layout at = layout_of(a.rows, a.vocab, a.targets, a.ntop);
   const long units = (long)a.rows * tiles_of(a.vocab);
   const unsigned grid = (unsigned)((units + 3) / 4);
   a.ntop > 0 ? logprobs_scan_kernel<true><<<grid, kThreads, 0, stream>>>(a, at)
              : logprobs_scan_kernel<false><<<grid, kThreads, 0, stream>>>(a, at);
-  const auto join = [&](auto runs) {
-    logprobs_join_kernel<runs()><<<a.rows, kJoin, 0, stream>>>(a, at);
+  using std::integral_constant;
+  const auto join = [&](auto nt, auto runs) {
+    logprobs_join_kernel<nt(), runs()><<<a.rows, nt(), 0, stream>>>(a, at);
   };
-  a.vocab <= kJoin * kRun       ? join(std::integral_constant<int, 1>())
-  : a.vocab <= 4 * kJoin * kRun ? join(std::integral_constant<int, 4>())
-                                : join(std::integral_constant<int, kKeys>());
+  const auto by = [&](auto nt) {
+    const int runs = (a.vocab + kRun * nt() - 1) / (kRun * nt());
+    runs <= 1               ? join(nt, integral_constant<int, 1>())
+    : runs <= 4             ? join(nt, integral_constant<int, 4>())
+    : runs <= kMost / 1024 ? join(nt, integral_constant<int, kMost / 1024>())
+                            : join(nt, integral_constant<int, kMost / nt()>());
+  };
+  a.rows > 2 * dev.cus ? by(integral_constant<int, 256>()) : by(integral_constant<int, 1024>());
   return hipGetLastError();
 }
 

@@ -7,8 +7,8 @@
 // fp64 between the roundings of x' and of h to fp32, so that h's codes are the exact ones but where
 // a border between two is hit to 1e-15.
 //
-// A workgroup has a row, which stays in registers from its loads to its stores: each value is
-// read and written once.
+// A wave or a workgroup has a row, which stays in registers from its loads to its stores: each value
+// is read and written once.
 #include <type_traits>
 
 #include "dec_common.h"
@@ -19,6 +19,17 @@ namespace gh {
 namespace {
 
 constexpr int kNormNone = 0, kNormLayer = 2;
+constexpr int kThreads = 256;  // of a workgroup whose waves have a row each
+
+// Sum and largest over a row's NT threads.
+template <int NT>
+__device__ __forceinline__ double row_sum(double v, double *red) {
+  return NT == 64 ? wave_sum_f64(v) : block_sum<NT>(v, red);
+}
+template <int NT>
+__device__ __forceinline__ float row_max(float v, float *red) {
+  return NT == 64 ? wave_max_dpp(v) : block_max<NT>(v, red);
+}
 
 // rows' chunks of four: NPT a thread, chunk j of thread t is t + j NT; read past the caches' order of
 // use, as they are read once (4096 rows of 2560: 39 -> 37 us)
@@ -26,7 +37,7 @@ template <int NPT, int NT>
 __device__ __forceinline__ void row_load(const float *p, int n4, v4f (&v)[NPT]) {
 #pragma unroll
   for (int j = 0; j < NPT; ++j) {
-    const int c = threadIdx.x + j * NT;
+    const int c = threadIdx.x % NT + j * NT;
     v[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     if (c < n4) v[j] = __builtin_nontemporal_load(reinterpret_cast<const v4f *>(p) + c);
   }
@@ -46,18 +57,18 @@ __device__ Moments moments(const v4f (&v)[NPT], const NormOf &n, int dim, double
     for (int j = 0; j < NPT; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) s += (double)v[j][e];
-    r.mean = block_sum<NT>(s, red) / (double)dim;
+    r.mean = row_sum<NT>(s, red) / (double)dim;
     s = 0.0;
   }
 #pragma unroll
   for (int j = 0; j < NPT; ++j)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const bool there = 4 * (int)(threadIdx.x + j * NT) < dim;
+      const bool there = 4 * (int)(threadIdx.x % NT + j * NT) < dim;
       const double d = there ? (double)v[j][e] - r.mean : 0.0;
       s = fma(d, d, s);
     }
-  r.m = rms_of(block_sum<NT>(s, red), dim, n.eps);
+  r.m = rms_of(row_sum<NT>(s, red), dim, n.eps);
   return r;
 }
 
@@ -71,11 +82,17 @@ __device__ __forceinline__ float clamped(double v) {
   return v > (double)FLT_MAX ? FLT_MAX : v < -(double)FLT_MAX ? -FLT_MAX : (float)v;
 }
 
+// NT threads a row: 64, a wave, without barriers, or a workgroup
 template <int NPT, int NT>
-__global__ __launch_bounds__(NT) void norm_residual_kernel(NormResidual a) {
+__global__ __launch_bounds__(NT == 64 ? kThreads : NT) void norm_residual_kernel(NormResidual a) {
   __shared__ double red[NT / 64];
   __shared__ float redf[NT / 64];
-  const int r = blockIdx.x, tid = threadIdx.x, n4 = a.dim >> 2;
+  const int tid = threadIdx.x % NT, n4 = a.dim >> 2;
+  int r = blockIdx.x;
+  if (NT == 64) {
+    r = r * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    if (r >= a.rows) return;
+  }
   v4f x[NPT], y[NPT];
   row_load<NPT, NT>(a.x + r * a.x_stride, n4, x);
   if (a.y != nullptr) {
@@ -141,7 +158,7 @@ __global__ __launch_bounds__(NT) void norm_residual_kernel(NormResidual a) {
       finite = finite && fabsf(x[j][e]) <= FLT_MAX;
       amax = fmaxf(amax, abs_daz(x[j][e]));
     }
-  amax = block_max<NT>(finite ? amax : INFINITY, redf);
+  amax = row_max<NT>(finite ? amax : INFINITY, redf);
   finite = amax <= FLT_MAX;
   const QuantParams qp = quant_params(finite ? amax : 0.0f);
 #pragma unroll
@@ -158,19 +175,39 @@ __global__ __launch_bounds__(NT) void norm_residual_kernel(NormResidual a) {
 
 }  // namespace
 
-hipError_t launch_norm_residual(const NormResidual &a, hipStream_t stream) {
-  auto go = [&](auto npt, auto nt) {
-    norm_residual_kernel<npt(), nt()><<<a.rows, nt(), 0, stream>>>(a);
-  };
+hipError_t launch_norm_residual(const NormResidual &a, const DeviceInfo &dev,
+                                hipStream_t stream) {
+  using std::integral_constant;
   const int n4 = a.dim / 4;
-  auto by = [&](auto nt) {
-    const int npt = (n4 + nt() - 1) / nt();
-    npt <= 1   ? go(std::integral_constant<int, 1>(), nt)
-    : npt == 2 ? go(std::integral_constant<int, 2>(), nt)
-    : npt == 3 ? go(std::integral_constant<int, 3>(), nt)
-               : go(std::integral_constant<int, 6>(), nt);
+  auto go = [&](auto npt, auto nt) {
+    constexpr int rows = nt() == 64 ? kThreads / 64 : 1;
+    norm_residual_kernel<npt(), nt()>
+        <<<(a.rows + rows - 1) / rows, nt() == 64 ? kThreads : nt(), 0, stream>>>(a);
   };
-  n4 <= 6 * 256 ? by(std::integral_constant<int, 256>()) : by(std::integral_constant<int, 1024>());
+  auto by = [&](auto nt, auto least) {
+    const int npt = (n4 + nt() - 1) / nt();
+    constexpr int kLeast = least(), kMost = nt() < 256 ? 3 : 6;
+    if constexpr (kLeast <= 1) {
+      if (npt <= 1) return go(integral_constant<int, 1>(), nt);
+    }
+    if (npt <= 2) return go(integral_constant<int, 2>(), nt);
+    if (npt <= 3 || kMost == 3) return go(integral_constant<int, 3>(), nt);
+    if constexpr (kMost > 3)
+      npt <= 4   ? go(integral_constant<int, 4>(), nt)
+      : npt <= 5 ? go(integral_constant<int, 5>(), nt)
+                 : go(integral_constant<int, kMost>(), nt);
+  };
+  // Few rows have a workgroup each, so that a row takes as little time as it can.  Of many, threads
+  // have three chunks at most, which leaves room for other rows' waves, and few are without any:
+  // us of 20000 rows of 256 with 64, 128 and 256 threads a row 22, 29, 43, of 8192 rows of 1152 42,
+  // 34, 38, of 4096 rows of 2560 (128 and 256) 46, 37.
+  const bool many = a.rows > 4 * dev.cus;
+  const integral_constant<int, 1> one;
+  const integral_constant<int, 2> two;
+  many && n4 <= 3 * 64     ? by(integral_constant<int, 64>(), one)
+  : many && n4 <= 3 * 128 ? by(integral_constant<int, 128>(), two)
+  : n4 <= 6 * 256         ? by(integral_constant<int, 256>(), one)
+                          : by(integral_constant<int, 1024>(), two);
   return hipGetLastError();
 }
 

@@ -529,27 +529,45 @@ __global__ __launch_bounds__(kThreads) void kv_append_wide_kernel(KvAppend a, in
   }
 }
 
-// Heads in a call up to which lanes take one each, so that a few rows are one trip to memory;
-// beyond, rows go by Wide where they can, else lanes take four heads, which share the row's angles
-// and table look-ups.
-constexpr long kFewHeads = 16384;
-constexpr int kWideHeads = 8;  // that a wave of Wide takes of its rows
+// Heads in a call up to which lanes take one each, so that a few rows are one trip to memory; beyond,
+// rows go by Wide where they can and if that leaves every SIMD two heads to do, else lanes take four
+// heads, which share the row's angles and table look-ups.  us of q, k and v appended (16 heads of
+// 256 a row) by one, by four and by Wide: 512 rows 8.7, 8.5, 6.8, 2048 rows 26, 18, 18, 8192 rows 96,
+// 57, 50; of 1024 rows (8 heads of 128) 5.6, 5.5, 6.5, 2048 rows 8.7, 7.4, 7.4.
+constexpr long kFewHeads = 8192;
+// Calls of Wide: `rows` waves' worth of rows, `per` heads of them a wave, `waves` in all.
+struct WideCall {
+  long waves;
+  int per;
+};
+// most: heads a wave, if that leaves every SIMD two waves.  Rows for the cache take up to 8, as each
+// wave looks their places up; rope two (32768 rows of 8 heads of 256: 51 us, with eight 57).
+WideCall wide_call(int nrows, int heads, int g, int most, const DeviceInfo &dev) {
+  const long rows = (nrows + 64 / g - 1l) / (64 / g), all = rows * heads;
+  if (all < 8l * dev.cus) return WideCall{0, 0};
+  const long per = all / (8l * dev.cus);
+  const int p = (int)(per < 2 ? 2 : per > most ? most : per);
+  return WideCall{rows * ((heads + p - 1) / p), p};
+}
 
 }  // namespace
 
-hipError_t launch_rope(const RopeRows &a, hipStream_t stream) {
+hipError_t launch_rope(const RopeRows &a, const DeviceInfo &dev, hipStream_t stream) {
   auto go = [&](auto g, auto pairs, auto h) {
     constexpr int PER = 64 / g() * h();
     const long units = (long)a.rows * ((a.heads + PER - 1) / PER);
     rope_kernel<g(), pairs(), h()><<<(unsigned)((units + 3) / 4), kThreads, 0, stream>>>(a);
   };
   auto heads = [&](auto g, auto pairs) {
-    if ((long)a.rows * a.heads <= kFewHeads) return go(g, pairs, std::integral_constant<int, 1>());
-    if (!wide(a.hdim, a.rot)) return go(g, pairs, std::integral_constant<int, 4>());
     constexpr int G = g() / 4;
-    const long waves = (a.rows + 64 / G - 1l) / (64 / G) * ((a.heads + kWideHeads - 1) / kWideHeads);
-    rope_wide_kernel<G, pairs()>
-        <<<(unsigned)((waves + 3) / 4), kThreads, 0, stream>>>(a, kWideHeads);
+    const WideCall w = wide_call(a.rows, a.heads, G, 2, dev);
+    if (w.waves > 0 && wide(a.hdim, a.rot))
+      rope_wide_kernel<G, pairs()>
+          <<<(unsigned)((w.waves + 3) / 4), kThreads, 0, stream>>>(a, w.per);
+    else if ((long)a.rows * a.heads <= kFewHeads)
+      go(g, pairs, std::integral_constant<int, 1>());
+    else
+      go(g, pairs, std::integral_constant<int, 4>());
   };
   auto pairs = [&](auto g) {
     a.rot.pairs ? heads(g, std::true_type()) : heads(g, std::false_type());
@@ -560,7 +578,7 @@ hipError_t launch_rope(const RopeRows &a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-hipError_t launch_kv_append(const KvAppend &a, hipStream_t stream) {
+hipError_t launch_kv_append(const KvAppend &a, const DeviceInfo &dev, hipStream_t stream) {
   const int all = (a.q != nullptr ? a.n_heads : 0) + 2 * a.c.nkv;
   auto go = [&](auto g, auto type, auto pairs, auto h) {
     constexpr int PER = 64 / g() * h();
@@ -569,13 +587,15 @@ hipError_t launch_kv_append(const KvAppend &a, hipStream_t stream) {
         <<<(unsigned)((units + 3) / 4), kThreads, 0, stream>>>(a);
   };
   auto heads = [&](auto g, auto type, auto pairs) {
-    if ((long)a.b.rows * all <= kFewHeads)
-      return go(g, type, pairs, std::integral_constant<int, 1>());
-    if (!wide(a.c.hdim, a.rot)) return go(g, type, pairs, std::integral_constant<int, 4>());
     constexpr int G = g() / 4;
-    const long waves = (a.b.rows + 64 / G - 1l) / (64 / G) * ((all + kWideHeads - 1) / kWideHeads);
-    kv_append_wide_kernel<G, type(), pairs()>
-        <<<(unsigned)((waves + 3) / 4), kThreads, 0, stream>>>(a, kWideHeads);
+    const WideCall w = wide_call(a.b.rows, all, G, 8, dev);
+    if (w.waves > 0 && wide(a.c.hdim, a.rot))
+      kv_append_wide_kernel<G, type(), pairs()>
+          <<<(unsigned)((w.waves + 3) / 4), kThreads, 0, stream>>>(a, w.per);
+    else if ((long)a.b.rows * all <= kFewHeads)
+      go(g, type, pairs, std::integral_constant<int, 1>());
+    else
+      go(g, type, pairs, std::integral_constant<int, 4>());
   };
   auto pairs = [&](auto g, auto type) {
     a.rot.pairs ? heads(g, type, std::true_type()) : heads(g, type, std::false_type());
