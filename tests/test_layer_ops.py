@@ -330,7 +330,10 @@ ROPES = [  # rows, heads, hdim, rot, layout, norm, angle32, stride
     (33, 4, 256, 256, ROPE_HALF, True, False, 1032), (2, 7, 96, 0, ROPE_HALF, True, False, 0),
     (9, 1, 256, 64, ROPE_PAIRS, True, True, 0), (40, 3, 68, 68, ROPE_PAIRS, False, False, 0),
     (6000, 3, 128, 64, ROPE_HALF, True, False, 384), (4099, 5, 256, 256, ROPE_PAIRS, True, False, 0),
-    (1500, 17, 32, 32, ROPE_HALF, True, False, 0)]
+    (1500, 17, 32, 32, ROPE_HALF, True, False, 0),
+    (9000, 4, 64, 64, ROPE_HALF, True, True, 0), (5003, 7, 64, 16, ROPE_PAIRS, False, False, 452),
+    (3001, 6, 256, 0, ROPE_HALF, True, False, 0), (8203, 3, 128, 96, ROPE_PAIRS, True, False, 0),
+    (2601, 5, 256, 128, ROPE_HALF, True, True, 1284), (9001, 4, 64, 32, ROPE_HALF, False, False, 0)]
 
 
 @pytest.mark.gpu
@@ -392,6 +395,10 @@ APPENDS = {  # sequences (new rows, positions), q heads, kv heads, head dim, pag
     "many": ([(1 + b % 3, 3 + b % 20) for b in range(200)], 2, 1, 128, 16, 128, ROPE_PAIRS, False),
     "prompt": ([(1500, 1600), (1, 5)], 8, 4, 256, 64, 256, ROPE_HALF, True),
     "prompt128": ([(2100, 2100)], 7, 1, 128, 256, 128, ROPE_PAIRS, True),
+    "chunks": ([(1 + b % 19, 2 + b % 23) for b in range(220)], 7, 1, 128, 16, 64, ROPE_HALF, True),
+    "chunks256": ([(40 + b, 45 + 3 * b % 70) for b in range(12)], 4, 2, 256, 32, 64, ROPE_PAIRS,
+                  True),
+    "keys256": ([(700, 800), (0, 5), (900, 900)], 0, 4, 256, 64, 256, ROPE_HALF, False),
 }
 
 
@@ -437,6 +444,8 @@ def test_append(gh, name, kind):
     p, rows, x, wq, wk, f = append_inputs(case, kind, 2)
     if name == "ragged":
         p.table[3, 1] = -1  # a page that isn't there
+    if name in ("chunks", "keys256"):
+        p.table[2, 0] = 1 << 30
     c, b = p.device(), None
     b = p.batch(rows=rows)
     dx, wqd, wkd = cuda(x), None if wq is None else cuda(wq), None if wk is None else cuda(wk)
@@ -500,6 +509,74 @@ def test_append_of_rows_that_are_not_finite(gh):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("hd,layout", [(128, ROPE_HALF), (256, ROPE_PAIRS)])
+def test_many_rows_of_any_size_of_values(gh, kind, hd, layout):
+    """Heads of zeros, subnormals, values at both ends of fp32, NaN and infinities among many rows:
+    codes and scales to the bit those of rope and cache_write, other heads untouched by them."""
+    import torch
+
+    nq, kv, page, n = 3, 2, 64, 3000
+    rng = np.random.default_rng(17)
+    x = rng.standard_normal((n, nq + 2 * kv, hd)).astype(F32)
+    sizes = np.array([1.0, 0.0, 1e-42, 1e-39, 1e-36, 1e-31, 1e-29, 1e30, 3e37], F32)
+    x *= rng.choice(sizes, (n, nq + 2 * kv, 1))
+    bad = rng.random((n, nq + 2 * kv)) < 0.1
+    x[bad, 5] = rng.choice(np.array([np.nan, np.inf, -np.inf], F32), bad.sum())
+    f, _ = gemma_hip.rotary_freqs(hd, 10000.0)
+    r = gemma_hip.rotary(cuda(f), hd, layout)
+    w = (nq + 2 * kv) * hd
+    p = Paged([(n, n)], kv, hd, page, KINDS[kind], rng)
+    pos = cuda(np.arange(n, dtype=np.int32))
+    out = []
+    for one in (False, True):
+        c, b, dx = p.device(), p.batch(), cuda(x.reshape(n, w))
+        if one:
+            gh.cache_append(c, b, gemma_hip.heads(dx, w, dx[:, nq * hd:], w, dx[:, (nq + kv) * hd:],
+                                                  w, dx, w, nq, None, None, EPS, r), stream())
+            out.append([dx[:, :nq * hd].contiguous()])
+        else:  # 64 rows at a time: by the kernel of few rows
+            for i in range(0, n, 64):
+                m = min(64, n - i)
+                gh.rope(dx[i:], w, dx[i:], w, m, nq + kv, hd, pos[i:], None, EPS, r, stream())
+            gh.cache_write(c, b, dx[:, nq * hd:], w, dx[:, (nq + kv) * hd:], w, stream())
+            out.append([dx[:, :nq * hd].contiguous()])
+        out[-1] += [t.clone() for k in "kv" for t in p.d[k]]
+    for a, b in zip(*out):
+        same = a.contiguous().view(torch.uint8) == b.contiguous().view(torch.uint8)
+        if a.dtype == torch.float32:  # NaN is NaN
+            same = same.view(*a.shape, 4).all(-1) | (a.isnan() & b.isnan())
+        assert same.all()
+
+
+@pytest.mark.gpu
+def test_append_behind_four_gigabytes(gh):
+    """Codes of pages whose addresses pass 32 bits, by one row and by many."""
+    import torch
+
+    kv, hd, page, npages = 4, 256, 64, 70000  # 4.6e9 codes of keys
+    codes = torch.zeros((2, npages, kv, page, hd), dtype=torch.int8, device="cuda")
+    scales = torch.zeros((2, npages, kv, page), device="cuda")
+    c = gemma_hip.cache(codes[0], codes[1], scales[0], scales[1], CACHE_I8, npages, page, kv, hd)
+    for n in (1, 1024):
+        pages = -(-n // page)
+        table = torch.arange(npages - pages, npages, device="cuda", dtype=torch.int32)[None]
+        row0 = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+        b = gemma_hip.batch(table, row0[1:], row0, 1, pages, n, n, n)
+        x = torch.randn((n, 2 * kv * hd), device="cuda")
+        gh.cache_append(c, b, gemma_hip.heads(None, 0, x, 2 * kv * hd, x[:, kv * hd:], 2 * kv * hd,
+                                              None, 0, 0), stream())
+        for i in range(2):
+            got = codes[i, npages - pages:].float() * scales[i, npages - pages:, :, :, None]
+            got = got.permute(0, 2, 1, 3).reshape(-1, kv * hd)[:n]
+            off = (got - x[:, i * kv * hd:(i + 1) * kv * hd]).abs().view(n, kv, hd).amax(-1)
+            # half a step of 1/127 of the head's largest, and a rounding of each side
+            top = x[:, i * kv * hd:(i + 1) * kv * hd].abs().view(n, kv, hd).amax(-1)
+            assert (off <= top / 254 * (1 + 1e-5)).all()
+        assert not codes[:, :1000].any()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("batch", [1, 62, 63, 64, 65, 200, 4000, 10000])
 def test_rows_find_their_sequences(gh, batch):
     """Single rows, none and several, in batches around the search's steps."""
@@ -536,7 +613,11 @@ NORMS = [  # rows, dim, after, before, gate, stride
     (700, 640, NORM_LAYER, NORM_RMS, "rows", 0), (4, 2564, NORM_RMS, NORM_LAYER, None, 0),
     (3, 6144, NORM_LAYER, NORM_LAYER, "one", 0), (2, 6148, NORM_RMS, NORM_RMS, "rows", 6152),
     (2, 24576, NORM_RMS, NORM_RMS, None, 0), (9, 512, NORM_NONE, NORM_NONE, None, 0),
-    (3000, 256, NORM_RMS, NORM_RMS, None, 0)]
+    (3000, 256, NORM_RMS, NORM_RMS, None, 0), (1101, 704, NORM_LAYER, NORM_RMS, "rows", 712),
+    (1030, 768, NORM_RMS, NORM_LAYER, "one", 0), (1027, 772, NORM_LAYER, NORM_LAYER, "rows", 0),
+    (1300, 1152, NORM_RMS, NORM_RMS, "one", 1160), (1026, 1536, NORM_NONE, NORM_LAYER, None, 0),
+    (1025, 2560, NORM_RMS, NORM_RMS, "rows", 0), (2, 5000, NORM_RMS, NORM_RMS, "one", 0),
+    (2, 17000, NORM_LAYER, NORM_RMS, "rows", 0), (4100, 208, NORM_RMS, NORM_RMS, None, 216)]
 
 
 def codes_of_rows(h):
@@ -638,6 +719,10 @@ ADAPTERS = {  # rows of the sequences, k, outputs, rank, adapters
     "wide": ([17, 64], 640, [300, 44, 8], 64, 2), "most": ([130], 72, [515], 128, 1),
     "prompts": ([300, 77, 0, 260], 2560, [512, 256, 256], 16, 3),
     "long": ([40], 10240, [65], 32, 2), "few": ([3, 4, 2], 1152, [1024, 256, 256], 16, 4),
+    "three": ([900, 700], 264, [64, 100, 64], 16, 2), "two": ([300, 270], 200, [96, 40], 64, 2),
+    "tiles": ([1 + i * 7 % 40 for i in range(90)], 72, [70, 3], 40, 4),
+    "rank128": ([20, 3], 136, [130, 64], 128, 2), "tokens128": ([1] * 5, 200, [70, 130], 128, 3),
+    "pairs": ([1, 2, 0, 1], 1000, [65], 24, 2), "tall": ([129, 65, 64], 512, [129], 72, 2),
 }
 
 
@@ -710,6 +795,46 @@ def test_adapters(gh, name, kind):
     work = torch.empty(gh.adapters_work(ad, len(ns), k), dtype=torch.uint8, device="cuda")
     gh.adapters_add(mine, n + 3, mine, n + 3, ad, jobs, src, k + 4, k, work, stream())
     assert torch.equal(mine, out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", TYPES)
+def test_adapters_leave_rows_in_no_sequence(gh, kind):
+    """Rows before the first sequence, behind max_rows of one and behind the last, and a table that
+    falls: the others as if they weren't there; nothing that an adapter of another row holds, NaN and
+    infinities among it, comes into a row."""
+    import torch
+
+    k, n, rank, count = 72, 70, 16, 3
+    case = ([100], k, [n], rank, count)
+    a, b, x, base, scale, _ = adapter_inputs(case, TYPES[kind], 12)
+    a[0][2], b[0][2] = math.nan, math.inf
+    for row0, max_rows in (([3, 20, 50, 52, 90], 18), ([3, 4, 5, 7, 9], 2)):
+        ids = np.array([1, 2, 0, 1], np.int32)
+        ad = gemma_hip.adapters(cuda(np.array(row0, np.int32)), cuda(ids), scale.cuda(), 4, 100,
+                                max_rows, count, rank, TYPES[kind])
+        out = torch.full((100, n), 4.0, device="cuda")
+        jobs = gemma_hip.adapter_jobs([(a[0].cuda(), b[0].cuda(), n)])
+        gh.adapters_add(out, 0, base.cuda(), 0, ad, jobs, x.cuda(), 0, k, None, stream())
+        got = out.cpu().double().numpy()
+        room = (math.sqrt(3 * k) + math.sqrt(3 * rank) + 8) * HALF
+        left = np.ones(100, bool)
+        for i, id in enumerate(ids):
+            r = slice(row0[i], min(row0[i + 1], row0[i] + max_rows))
+            left[r] = False
+            if id == 2:
+                assert not np.isfinite(got[r]).any()
+                continue
+            one = ([r.stop - r.start], k, [n], rank, count)
+            want, size = adapters_expected(one, a, b, x[r], base[r], scale, [id])
+            assert (np.abs(got[r] - want) <= room * size).all()
+        assert (got[left] == 4.0).all()
+    # a table that falls: no row outside of 0 .. 99 is touched (guards on both sides)
+    out = torch.full((300, n), 4.0, device="cuda")
+    ad = gemma_hip.adapters(cuda(np.array([50, 90, 10, -7, 1 << 30], np.int32)), cuda(ids),
+                            scale.cuda(), 4, 100, 18, count, rank, TYPES[kind])
+    gh.adapters_add(out[100:], 0, base.cuda(), 0, ad, jobs, x.cuda(), 0, k, None, stream())
+    assert (out[:100] == 4.0).all() and (out[200:] == 4.0).all()
 
 
 @pytest.mark.gpu
@@ -853,6 +978,39 @@ def test_logprobs_of_a_whole_vocabulary(gh):
             p, k, e, first, _ = describe(l[r], 1.0, ids[r], 64)
             assert np.array_equal(top[r].cpu().numpy(), first) and rank[r].item() == k[0]
             assert close_logs(logp[r].cpu().numpy(), p) and close_logs(h[r].item(), e)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab,ntop,targets", [(70, 64, 1), (3023, 12, 2), (20000, 64, 0),
+                                                (70000, 5, 1), (270000, 64, 1)])
+def test_logprobs_of_many_rows(gh, vocab, ntop, targets):
+    """More rows than compute units: rows that are repeated have the same answers, to the bit, and
+    the first ones the definition's."""
+    import torch
+
+    rng = np.random.default_rng(vocab)
+    kinds = [n for n in ROWS if n in ("normal", "ties", "equal", "holes", "falling", "nothing")]
+    l = np.stack([row_of(n, vocab, rng) for n in kinds])
+    ids = rng.integers(0, vocab, (len(l), targets)).astype(np.int32)
+    t = np.array([1.0, 0.7, 0.0, 1.5, 1.0, 1.0], F32)
+    times = 90  # 540 rows
+    rows = len(l) * times
+    out = dict(logp=torch.empty((rows, targets), device="cuda"),
+               rank=torch.empty((rows, targets), dtype=torch.int32, device="cuda"),
+               entropy=torch.empty(rows, device="cuda"),
+               top=torch.empty((rows, ntop), dtype=torch.int32, device="cuda"),
+               top_logp=torch.empty((rows, ntop), device="cuda"))
+    gh.logprobs(gemma_hip.scores(**out), cuda(l).repeat(times, 1), 0, rows, vocab,
+                cuda(t).repeat(times), cuda(ids).repeat(times, 1), targets, ntop, None, stream())
+    for v in out.values():
+        again = v.view(times, -1)
+        assert torch.equal(again, again[:1].expand_as(again))
+    got = {k: v[:len(l)].cpu().numpy() for k, v in out.items()}
+    for r in range(len(l)):
+        logp, rank, h, top, tl = describe(l[r], F64(t[r]), ids[r], ntop)
+        assert np.array_equal(got["rank"][r], rank) and np.array_equal(got["top"][r], top), kinds[r]
+        assert close_logs(got["logp"][r], logp) and close_logs(got["top_logp"][r], tl), kinds[r]
+        assert close_logs(got["entropy"][r], h), kinds[r]
 
 
 # ---- together ---------------------------------------------------------------------
