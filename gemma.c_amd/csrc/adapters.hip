@@ -363,64 +363,145 @@ __device__ __forceinline__ ExpandUnit expand_unit(const Adapters &a, int unit) {
   return u;
 }
 
-// dst of a row and 64 columns of a job a wave.  B's part is one run of memory, read 16 bytes a lane
-// (CHUNKS a row of it at most); their products with u meet in LDS, where a lane has a column.
+// dst of a row and a unit's 64 columns, by a wave; u: the row's values of the unit's job, in memory or
+// LDS.  B's part is one run of memory, read 16 bytes a lane (CHUNKS a row of it at most); their
+// products with u meet in LDS, where a lane has a column.
+template <int TYPE, int CHUNKS>
+struct ExpandRow {
+  static constexpr int kSize = TYPE == kAdapterF32 ? 4 : 2, kOf = 16 / kSize;  // weights a chunk
+  static constexpr int kFlight = CHUNKS < 8 ? CHUNKS : 8;                      // read together
+  static constexpr int kNowhere = kExpandCols * (CHUNKS + 1), kSums = kNowhere + 1;
+
+  u4 w[kFlight];
+  float v;
+
+  __device__ __forceinline__ void weights(const Adapters &a, const ExpandUnit &x, int id, int j0) {
+    const int all = min(kExpandCols, x.width - x.c0) * (a.rank / kOf);
+    const u4 *b = reinterpret_cast<const u4 *>(reinterpret_cast<const char *>(job_of(a.b, x.job)) +
+                                               ((size_t)id * x.width + x.c0) * a.rank * kSize);
+#pragma unroll
+    for (int j = 0; j < kFlight; ++j) {
+      const int i = (threadIdx.x & 63) + 64 * (j0 + j);
+      w[j] = b[i < all ? i : 0];
+    }
+  }
+  __device__ __forceinline__ void load(const Adapters &a, const ExpandUnit &x, int r, int id) {
+    const int c = x.c0 + (threadIdx.x & 63);
+    v = c < x.width ? a.base[r * a.base_stride + x.begin + c] : 0.0f;
+    if (id >= 0) weights(a, x, id, 0);
+  }
+  __device__ __forceinline__ void finish(const Adapters &a, const ExpandUnit &x, int r, int id,
+                                         const float *u, float (&sums)[kSums]) {
+    const int lane = threadIdx.x & 63, c = x.c0 + lane;
+    if (id >= 0) {
+      const int chunks = a.rank / kOf;
+      const unsigned share = (65536 + chunks - 1) / chunks;  // i / chunks is i share / 65536
+      for (int j0 = 0;;) {
+#pragma unroll
+        for (int j = 0; j < kFlight; ++j) {
+          const int i = lane + 64 * (j0 + j);
+          const int col = (int)(i * share >> 16), p = i - col * chunks;
+          float s = 0.0f;
+          if constexpr (TYPE == kAdapterF32) {
+            const v4f at = *reinterpret_cast<const v4f *>(u + kOf * p);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s = fmaf(at[e], __uint_as_float(w[j][e]), s);
+          } else {
+            float f[8];
+            floats8<TYPE>(Raw8<TYPE>{{w[j]}}, f);
+            const v4f lo = *reinterpret_cast<const v4f *>(u + kOf * p);
+            const v4f hi = *reinterpret_cast<const v4f *>(u + kOf * p + 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s = fmaf(lo[e], f[e], s), s = fmaf(hi[e], f[e + 4], s);
+          }
+          // (no branch, which would take the loads with it, one after the other)
+          sums[j0 + j < chunks ? col * (chunks + 1) + p : kNowhere] = s;
+        }
+        j0 += kFlight;
+        if (j0 >= chunks) break;
+        weights(a, x, id, j0);
+      }
+      // written and read by the same wave, whose LDS accesses keep their order
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      float s = 0.0f;
+      for (int p = 0; p < chunks; ++p) s += sums[lane * (chunks + 1) + p];
+      v += s;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+    if (c < x.width) a.dst[r * a.dst_stride + x.begin + c] = v;
+  }
+};
+
 template <int TYPE, int CHUNKS>
 __global__ __launch_bounds__(kThreads) void adapter_expand_row_kernel(Adapters a) {
-  constexpr int kSize = TYPE == kAdapterF32 ? 4 : 2, kOf = 16 / kSize;  // weights a chunk
-  constexpr int kFlight = CHUNKS < 8 ? CHUNKS : 8;  // read together
-  constexpr int kNowhere = kExpandCols * (CHUNKS + 1);
-  __shared__ float sums[kThreads / 64][kNowhere + 1];
-  const int lane = threadIdx.x & 63, r = blockIdx.x;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  typedef ExpandRow<TYPE, CHUNKS> Expand;
+  __shared__ float sums[kThreads / 64][Expand::kSums];
+  const int r = blockIdx.x, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const ExpandUnit x = expand_unit(a, blockIdx.y * (kThreads / 64) + wave);
   if (x.job == a.njobs) return;
-  const int id = ids_of(a)[r], c = x.c0 + lane;
+  const int id = ids_of(a)[r];
   if (id == kOutside) return;
-  float v = c < x.width ? a.base[r * a.base_stride + x.begin + c] : 0.0f;
+  Expand e;
+  e.load(a, x, r, id);
+  e.finish(a, x, r, id, u_of(a) + ((size_t)r * a.njobs + x.job) * a.rank, sums[wave]);
+}
+
+// Both products of a row by one workgroup, u in LDS: a launch less (of 3.7 us on the host), where a row
+// has little to read.
+constexpr int kRowWaves = 16, kRowValues = 4;  // values of u a wave has in flight
+template <int TYPE, int CHUNKS>
+__global__ __launch_bounds__(64 * kRowWaves) void adapter_row_kernel(Adapters a, int units) {
+  typedef ExpandRow<TYPE, CHUNKS> Expand;
+  __shared__ float u[kAdapterMaxJobs * kAdapterMaxRank];
+  __shared__ float sums[kRowWaves][Expand::kSums];
+  const int r = blockIdx.x, all = a.njobs * a.rank, lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int id = id_of_row(a, r);
+  if (id == kOutside) return;
   if (id >= 0) {
-    const int chunks = a.rank / kOf, all = min(kExpandCols, x.width - x.c0) * chunks;
-    const unsigned share = (65536 + chunks - 1) / chunks;  // i / chunks is i share / 65536
-    const u4 *b = reinterpret_cast<const u4 *>(
-        reinterpret_cast<const char *>(job_of(a.b, x.job)) +
-        ((size_t)id * x.width + x.c0) * a.rank * kSize);
-    const float *u = u_of(a) + ((size_t)r * a.njobs + x.job) * a.rank;
-    for (int j0 = 0; j0 < chunks; j0 += kFlight) {
-      u4 w[kFlight];
+    const float *x = a.src + r * a.src_stride;
+    for (int at0 = wave; at0 < all; at0 += kRowWaves * kRowValues) {
+      const void *m[kRowValues];
+      size_t first[kRowValues];
+      float s[kRowValues];
 #pragma unroll
-      for (int j = 0; j < kFlight; ++j) {
-        const int i = lane + 64 * (j0 + j);
-        w[j] = b[i < all ? i : 0];
+      for (int t = 0; t < kRowValues; ++t) {
+        const int at = min(at0 + t * kRowWaves, all - 1), job = at / a.rank;
+        m[t] = job_of(a.a, job);
+        first[t] = ((size_t)id * a.rank + (at - job * a.rank)) * a.k;
+        s[t] = 0.0f;
+      }
+      for (int c = 8 * lane; c < a.k; c += 512) {
+        const v4f x0 = *reinterpret_cast<const v4f *>(x + c);
+        const v4f x1 = *reinterpret_cast<const v4f *>(x + c + 4);
+        Raw8<TYPE> w[kRowValues];
+#pragma unroll
+        for (int t = 0; t < kRowValues; ++t) w[t] = raw8<TYPE>(m[t], first[t] + c);
+#pragma unroll
+        for (int t = 0; t < kRowValues; ++t) {
+          float f[8];
+          floats8<TYPE>(w[t], f);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[t] = fmaf(x0[e], f[e], s[t]), s[t] = fmaf(x1[e], f[e + 4], s[t]);
+        }
       }
 #pragma unroll
-      for (int j = 0; j < kFlight; ++j) {
-        const int i = lane + 64 * (j0 + j);
-        const int col = (int)(i * share >> 16), p = i - col * chunks;
-        float s = 0.0f;
-        if constexpr (TYPE == kAdapterF32) {
-          const v4f at = *reinterpret_cast<const v4f *>(u + kOf * p);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s = fmaf(at[e], __uint_as_float(w[j][e]), s);
-        } else {
-          float f[8];
-          floats8<TYPE>(Raw8<TYPE>{{w[j]}}, f);
-          const v4f lo = *reinterpret_cast<const v4f *>(u + kOf * p);
-          const v4f hi = *reinterpret_cast<const v4f *>(u + kOf * p + 4);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s = fmaf(lo[e], f[e], s), s = fmaf(hi[e], f[e + 4], s);
-        }
-        // (no branch, which would take the loads with it, one after the other)
-        sums[wave][j0 + j < chunks ? col * (chunks + 1) + p : kNowhere] = s;
+      for (int t = 0; t < kRowValues; ++t) {
+        s[t] = group_sum_f32<64>(s[t]);
+        const int at = at0 + t * kRowWaves;
+        if (lane == 0 && at < all) u[at] = scale_of(a, id) * s[t];
       }
     }
-    // written and read by the same wave, whose LDS accesses keep their order
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    float s = 0.0f;
-    for (int p = 0; p < chunks; ++p) s += sums[wave][lane * (chunks + 1) + p];
-    v += s;
   }
-  if (c < x.width) a.dst[r * a.dst_stride + x.begin + c] = v;
+  __syncthreads();
+  for (int unit = wave; unit < units; unit += kRowWaves) {
+    const ExpandUnit x = expand_unit(a, unit);
+    Expand e;
+    e.load(a, x, r, id);
+    e.finish(a, x, r, id, u + x.job * a.rank, sums[wave]);
+  }
 }
 
 // dst of 16 RT rows and 64 columns of a job a wave; KS: steps of 32 of the rank.  base and dst are
@@ -579,6 +660,10 @@ __global__ __launch_bounds__(kThreads, KS == 1 && TYPE != kAdapterF32 ? 4 : 3) v
 
 // Up to so many rows a sequence go by the row.
 constexpr int kFewRows = 2;
+// Bytes of an adapter's matrices up to which a row is one workgroup's.  us a call, in a row of eager
+// ones and in a graph, by two launches and by one: 32 rows of 156 KiB 11.6 and 5.6, 8.7 and 7.0; of
+// 368 KiB 11.2 and 7.7, 12.8 and 12.8.
+constexpr long kRowBytes = 192 << 10;
 
 }  // namespace
 
@@ -590,15 +675,20 @@ hipError_t launch_adapters(const Adapters &a, const DeviceInfo &dev, hipStream_t
   const int rows = a.seq.rows, all = a.njobs * a.rank;
   auto by_row = [&](auto type) {
     constexpr int kSize = type() == kAdapterF32 ? 4 : 2;
-    const dim3 first(rows, (all + 3) / 4);
-    const dim3 second(rows, (expand_units(a.end, a.njobs) + 3) / 4);
-    adapter_shrink_row_kernel<type()><<<first, kThreads, 0, stream>>>(a);
-    auto expand_row = [&](auto chunks) {
-      adapter_expand_row_kernel<type(), chunks()><<<second, kThreads, 0, stream>>>(a);
+    const int units = expand_units(a.end, a.njobs);
+    const bool one = ((long)all * a.k + (long)a.end[a.njobs - 1] * a.rank) * kSize <= kRowBytes;
+    auto go = [&](auto chunks) {
+      if (one) {
+        adapter_row_kernel<type(), chunks()><<<rows, 64 * kRowWaves, 0, stream>>>(a, units);
+      } else {
+        const dim3 first(rows, (all + 3) / 4), second(rows, (units + 3) / 4);
+        adapter_shrink_row_kernel<type()><<<first, kThreads, 0, stream>>>(a);
+        adapter_expand_row_kernel<type(), chunks()><<<second, kThreads, 0, stream>>>(a);
+      }
     };
-    a.rank * kSize <= 32    ? expand_row(std::integral_constant<int, 2>())
-    : a.rank * kSize <= 128 ? expand_row(std::integral_constant<int, 8>())
-                            : expand_row(std::integral_constant<int, kAdapterMaxRank * kSize / 16>());
+    a.rank * kSize <= 32    ? go(std::integral_constant<int, 2>())
+    : a.rank * kSize <= 128 ? go(std::integral_constant<int, 8>())
+                            : go(std::integral_constant<int, kAdapterMaxRank * kSize / 16>());
   };
   const int slots = tile_slots(a.seq, 16);
   auto shrink = [&](auto type, auto t) {
