@@ -3,15 +3,21 @@
 //   u = scale[id] A[id] x  (rank values a job),  dst = base + B[id] u
 //
 // id is that of the row's sequence; jobs are projections side by side (q, k, v; gate, up).  A launch
-// for the first product, whose fp32 results and whose rows' ids lie in the workspace, and one for
-// the second.
+// for the first product, whose results lie in the workspace, and one for the second; single tokens
+// with little to read take both in one.
 //
 // Rows of prompts go 16 at a time through the bf16 matrix cores: an fp32 value is the sum of three
 // bf16 pieces, a bf16 weight is one, an f16 weight the sum of two and an fp32 weight of three, and
 // of the piece products those are summed whose orders add up to at most 2 (3, 5 or 6 of
 // them: what is left out is below 2^-22 of a product).  A tile is one sequence's: with tiles across
-// sequences, which took a pass for each adapter, the few that had two set the time.  Single tokens
-// take a wave for a value of u and a wave for 64 of dst.
+// sequences, which took a pass for each adapter, the few that had two set the time.
+//
+// The products are small; what bounds these kernels is how x, base and dst get in and out.  A load
+// whose neighbouring lanes have a row each, as the matrix instructions want them, takes 64 cycles
+// (1024 rows by 2560 inputs so: 23 us, by whole runs and LDS 15), so all tiles but B's of short
+// sequences are read by runs and turned in LDS.  4096 rows of 2560 by rank 16 on 4096 columns: first
+// product 15 us (42 MB, 8 at a copy's rate), second 25 (134 MB, 26); 851 rows of 2560 by rank 64 on
+// 20480 columns, f16: 14 and 35 (139 MB, 27).
 #include <type_traits>
 
 #include "gh_arith.h"
@@ -507,14 +513,17 @@ __global__ __launch_bounds__(64 * kRowWaves) void adapter_row_kernel(Adapters a,
 // dst of 16 RT rows and 64 columns of a job a wave; KS: steps of 32 of the rank.  base and dst are
 // read and written by whole runs of 256 bytes; the products, whose lanes have a row each, go through
 // LDS.  A workgroup's four waves are WR times as many rows by 4 / WR times as many columns: 4 by 1,
-// which read B once, by whole runs, and share it in LDS, or, for short sequences, 1 by 4.
+// which read B once, by whole runs, and share its pieces in LDS, or, for short sequences, 1 by 4.
 template <int TYPE, int KS, int RT, int WR>
-__global__ __launch_bounds__(kThreads, KS == 1 && TYPE != kAdapterF32 ? 4 : 3) void adapter_expand_kernel(Adapters a) {
+__global__ __launch_bounds__(kThreads, TYPE == kAdapterF32               ? (WR > 1 ? 2 : 3)
+                                       : KS == 1 && TYPE == kAdapterBf16 ? 4
+                                                                         : 3)
+void adapter_expand_kernel(Adapters a) {
   constexpr int kSize = TYPE == kAdapterF32 ? 4 : 2, kWaves = kThreads / 64;
-  constexpr int kPitch = 32 * KS * kSize + 16;  // of a row of B: 16 rows in different banks
+  constexpr int kP = kPieces<TYPE>, kPitch = 64 * KS + 16;  // of a row of B's pieces: 16 in all banks
   constexpr int kLoads = kExpandCols * 32 * KS * kSize / 16 / kThreads;
   __shared__ float tiles[kWaves][16 * RT][kExpandPitch];
-  __shared__ char shared[WR > 1 ? kExpandCols : 1][kPitch];
+  __shared__ char shared[WR > 1 ? kP : 1][WR > 1 ? kExpandCols : 1][kPitch];
   const int lane = threadIdx.x & 63, m = lane & 15, quarter = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const ExpandUnit x = expand_unit(a, WR > 1 ? blockIdx.y : blockIdx.y * kWaves + wave);
@@ -590,8 +599,26 @@ __global__ __launch_bounds__(kThreads, KS == 1 && TYPE != kAdapterF32 ? 4 : 3) v
 #pragma unroll
       for (int j = 0; j < kLoads; ++j) {
         const int i = threadIdx.x + kThreads * j;
-        if (i < kExpandCols * chunks)
-          *reinterpret_cast<u4 *>(&shared[i / chunks][i % chunks * 16]) = part[j];
+        if (i >= kExpandCols * chunks) continue;
+        const int row = i / chunks, at = i - row * chunks;
+        if constexpr (TYPE == kAdapterF32) {
+          v4f left = __builtin_bit_cast(v4f, part[j]);
+#pragma unroll
+          for (int p = 0; p < kP; ++p) {
+            const u2 q = {cvt_pk_bf16(left[0], left[1]), cvt_pk_bf16(left[2], left[3])};
+            *reinterpret_cast<u2 *>(&shared[p][row][8 * at]) = q;
+            left -= v4f{bf16_lo(q[0]), bf16_hi(q[0]), bf16_lo(q[1]), bf16_hi(q[1])};
+          }
+        } else {
+          const Split8<kP> q = pieces8<TYPE>(Raw8<TYPE>{{part[j]}});
+#pragma unroll
+          for (int p = 0; p < kP; ++p) *reinterpret_cast<u4 *>(&shared[p][row][16 * at]) = q.p[p];
+        }
+      }
+      const int pads = 4 * KS - a.rank / 8;  // of 16 bytes, behind the rank
+      for (int i = threadIdx.x; i < kP * kExpandCols * pads; i += kThreads) {
+        const int row = i / pads, at = a.rank / 8 + i - row * pads;
+        *reinterpret_cast<u4 *>(&shared[row / kExpandCols][row % kExpandCols][16 * at]) = u4{0, 0, 0, 0};
       }
     }
     lds_barrier();
@@ -601,35 +628,42 @@ __global__ __launch_bounds__(kThreads, KS == 1 && TYPE != kAdapterF32 ? 4 : 3) v
     // values behind the rank are zeros on both sides
     constexpr int W = KS < 4 && (KS == 1 || TYPE != kAdapterF32) ? 4 : 2;  // read together
 #pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (auto &v : u[i][s].p) v = 32 * s + k0 < a.rank ? v : u4{0, 0, 0, 0};
+#pragma unroll
     for (int t0 = 0; t0 < 4; t0 += W) {
       Raw8<TYPE> w[W][KS];
+      if (WR == 1) {
 #pragma unroll
-      for (int t = 0; t < W; ++t)
+        for (int t = 0; t < W; ++t)
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          const int c = 16 * (t0 + t) + m, k = 32 * s + k0 < a.rank ? 32 * s + k0 : 0;
-          if (WR > 1)
-            w[t][s] = raw8<TYPE>(shared[c], k);
-          else
+          for (int s = 0; s < KS; ++s) {
+            const int c = 16 * (t0 + t) + m, k = 32 * s + k0 < a.rank ? 32 * s + k0 : 0;
             w[t][s] = raw8<TYPE>(b, (size_t)min(c, width - c0 - 1) * a.rank + k);
-        }
+          }
+      }
 #pragma unroll
       for (int t = 0; t < W; ++t) {
         v4f d[RT] = {};
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-          const bool in = 32 * s + k0 < a.rank;
-          Raw8<TYPE> v = w[t][s];
+          Split8<kP> wp;
+          if (WR > 1) {
 #pragma unroll
-          for (auto &x : v.v) x = in ? x : u4{0, 0, 0, 0};
-          const auto wp = pieces8<TYPE>(v);
+            for (int p = 0; p < kP; ++p)
+              wp.p[p] = *reinterpret_cast<const u4 *>(
+                  &shared[p][16 * (t0 + t) + m][64 * s + 16 * quarter]);
+          } else {
+            Raw8<TYPE> v = w[t][s];
 #pragma unroll
-          for (int i = 0; i < RT; ++i) {
-            Split8<3> up = u[i][s];
-#pragma unroll
-            for (auto &x : up.p) x = in ? x : u4{0, 0, 0, 0};
-            d[i] = product(wp, up, d[i]);
+            for (auto &x : v.v) x = 32 * s + k0 < a.rank ? x : u4{0, 0, 0, 0};
+            wp = pieces8<TYPE>(v);
           }
+#pragma unroll
+          for (int i = 0; i < RT; ++i) d[i] = product(wp, u[i][s], d[i]);
         }
 #pragma unroll
         for (int i = 0; i < RT; ++i)
@@ -658,7 +692,7 @@ __global__ __launch_bounds__(kThreads, KS == 1 && TYPE != kAdapterF32 ? 4 : 3) v
   }
 }
 
-// Up to so many rows a sequence go by the row.
+// Up to so many rows a sequence go by the row: with more, a tile's 16 rows share what is read.
 constexpr int kFewRows = 2;
 // Bytes of an adapter's matrices up to which a row is one workgroup's.  us a call, in a row of eager
 // ones and in a graph, by two launches and by one: 32 rows of 156 KiB 11.6 and 5.6, 8.7 and 7.0; of
@@ -710,6 +744,8 @@ hipError_t launch_adapters(const Adapters &a, const DeviceInfo &dev, hipStream_t
     const integral_constant<int, 1> one;
     const integral_constant<int, 2> two;
     if (a.seq.max_rows <= kFewRows) return by_row(type);
+    // 16 values of u a workgroup until there is one for every compute unit, then more, which share x
+    // (864 rows with 128 values: 16 each 13.9 us, 32 each 12.9)
     const int tiles = (all + 15) / 16;
     tiles == 1 || (long)slots * tiles <= dev.cus ? shrink(type, one)
     : tiles % kMostT != 0                            ? shrink(type, two)
