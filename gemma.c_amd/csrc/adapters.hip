@@ -14,7 +14,7 @@
 //
 // The products are small; what bounds these kernels is how x, base and dst get in and out.  A load
 // whose neighbouring lanes have a row each, as the matrix instructions want them, takes 64 cycles
-// (1024 rows by 2560 inputs so: 23 us, by whole runs and LDS 15), so all tiles but B's of short
+// (4096 rows of 2560 with 48 values of u so: 23 us, by whole runs and LDS 15), so all tiles but B's of short
 // sequences are read by runs and turned in LDS.  4096 rows of 2560 by rank 16 on 4096 columns: first
 // product 15 us (42 MB, 8 at a copy's rate), second 25 (134 MB, 26); 851 rows of 2560 by rank 64 on
 // 20480 columns, f16: 14 and 35 (139 MB, 27).
@@ -745,7 +745,7 @@ hipError_t launch_adapters(const Adapters &a, const DeviceInfo &dev, hipStream_t
     const integral_constant<int, 2> two;
     if (a.seq.max_rows <= kFewRows) return by_row(type);
     // 16 values of u a workgroup until there is one for every compute unit, then more, which share x
-    // (864 rows with 128 values: 16 each 13.9 us, 32 each 12.9)
+    // (851 rows with 128 values: 16 each 13.9 us, 32 each 12.9)
     const int tiles = (all + 15) / 16;
     tiles == 1 || (long)slots * tiles <= dev.cus ? shrink(type, one)
     : tiles % kMostT != 0                            ? shrink(type, two)

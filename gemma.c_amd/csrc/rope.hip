@@ -12,8 +12,8 @@
 // Many rows of heads of 64, 128 or 256 values: a row is hdim / 16 lanes', which take one head after
 // the other and have all the angles of their values from the start.  That is a quarter of the sums
 // over lanes, scales and addresses: 16 values a lane instead of 4.  9342 rows of 8 + 4 + 4 heads of
-// 256 (249 MB) take 55 us, 4.5 TB/s, with 66 instructions a head; with 4 values a lane 199, and
-// the 66 us were theirs.
+// 256 (249 MB) take 55 us, 4.5 TB/s, with 76 vector instructions a head; with 4 values a lane
+// 199, which bounded it (66 us).
 #include <type_traits>
 
 #include "dec_common.h"
