@@ -14,8 +14,8 @@
 //
 // The products are small; what bounds these kernels is how x, base and dst get in and out.  A load
 // whose neighbouring lanes have a row each, as the matrix instructions want them, takes 64 cycles
-// (4096 rows of 2560 with 48 values of u so: 23 us, by whole runs and LDS 15), so all tiles but B's of short
-// sequences are read by runs and turned in LDS.  4096 rows of 2560 by rank 16 on 4096 columns: first
+// (4096 rows of 2560 with 48 values of u so: 23 us, by whole runs and LDS 15), so all tiles but B's of
+// short sequences are read by runs and turned in LDS.  4096 rows of 2560 by rank 16 on 4096 columns: first
 // product 15 us (42 MB, 8 at a copy's rate), second 25 (134 MB, 26); 851 rows of 2560 by rank 64 on
 // 20480 columns, f16: 14 and 35 (139 MB, 27).
 #include <type_traits>
@@ -232,7 +232,9 @@ struct ShrinkStep {
     const int lane = threadIdx.x & 63, kx = k + 4 * (lane & 15);
     const int kw = k + 16 / kSize * (lane % kRowLanes);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = __builtin_nontemporal_load(reinterpret_cast<const v4f *>(src[j] + (kx < end ? kx : 0)));
+    for (int j = 0; j < 4; ++j)  // past the caches' order of use: read once, or by few workgroups
+      x[j] = __builtin_nontemporal_load(
+          reinterpret_cast<const v4f *>(src[j] + (kx < end ? kx : 0)));
 #pragma unroll
     for (int j = 0; j < kLoads; ++j)
       w[j] = *reinterpret_cast<const u4 *>(m[j] + (size_t)(kw < end ? kw : 0) * kSize);
@@ -490,7 +492,10 @@ __global__ __launch_bounds__(64 * kRowWaves) void adapter_row_kernel(Adapters a,
           float f[8];
           floats8<TYPE>(w[t], f);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[t] = fmaf(x0[e], f[e], s[t]), s[t] = fmaf(x1[e], f[e + 4], s[t]);
+          for (int e = 0; e < 4; ++e) {
+            s[t] = fmaf(x0[e], f[e], s[t]);
+            s[t] = fmaf(x1[e], f[e + 4], s[t]);
+          }
         }
       }
 #pragma unroll
@@ -710,7 +715,8 @@ hipError_t launch_adapters(const Adapters &a, const DeviceInfo &dev, hipStream_t
   auto by_row = [&](auto type) {
     constexpr int kSize = type() == kAdapterF32 ? 4 : 2;
     const int units = expand_units(a.end, a.njobs);
-    const bool one = ((long)all * a.k + (long)a.end[a.njobs - 1] * a.rank) * kSize <= kRowBytes;
+    const bool one = ((long)all * a.k + (long)a.end[a.njobs - 1] * a.rank) * kSize <= kRowBytes &&
+                     rows <= 1 << 21;  // (a grid has 2^32 - 1 threads at most)
     auto go = [&](auto chunks) {
       if (one) {
         adapter_row_kernel<type(), chunks()><<<rows, 64 * kRowWaves, 0, stream>>>(a, units);

@@ -1399,7 +1399,7 @@ int gemma_hip_norm_residual(const gemma_hip_residual *residual, int rows, int di
   const char *name = "gemma_hip_norm_residual";
   if (residual == nullptr) return fail("%s: null pointer", name);
   gemma_hip_residual v = *residual;
-  if (rows < 0 || dim < 4 || dim % 4 != 0 || dim > gh::kNormMaxDim)
+  if (rows < 0 || rows > gh::kNormMaxRows || dim < 4 || dim % 4 != 0 || dim > gh::kNormMaxDim)
     return fail("%s: unsupported shape: %d rows of %d", name, rows, dim);
   gh::NormResidual a{};
   if (norm_args(name, v.after, &a.after) || norm_args(name, v.before, &a.before)) return 1;

@@ -474,7 +474,7 @@ struct NormResidual {
   float *hs;
   int rows, dim;
 };
-constexpr int kNormMaxDim = 24576;
+constexpr int kNormMaxDim = 24576, kNormMaxRows = 1 << 21;  // (a grid has 2^32 - 1 threads)
 hipError_t launch_norm_residual(const NormResidual &a, const DeviceInfo &dev, hipStream_t stream);
 
 // adapters.hip: dst row = base row + scale[id] B[id] (A[id] src row), id that of the row's

@@ -410,6 +410,7 @@ __global__ __launch_bounds__(NT) void logprobs_join_kernel(Logprobs a, Layout at
     if (!(l > -INFINITY)) return -INFINITY;
     if (!drawn) return first ? 0.0f : -INFINITY;
     if (l == top) return (float)(0.0 - logs);
+    if (top == INFINITY) return -INFINITY;
     return (float)(((double)l - (double)top) * per - logs);
   };
   if (tid < a.targets) {

@@ -784,7 +784,7 @@ typedef struct {
   int x_out_stride, h_stride, hq_stride;
 } gemma_hip_residual;
 
-/* rows of dim values, dim a multiple of 4 up to 24576. */
+/* rows (at most 2^21) of dim values, dim a multiple of 4 up to 24576. */
 int gemma_hip_norm_residual(const gemma_hip_residual *residual, int rows, int dim, void *stream);
 
 /* Low-rank adapters, `count` of them, and the requests that use them.  ids [batch]: each sequence's

@@ -263,7 +263,7 @@ def test_bad_norms_are_refused():
 
     for kw, word in ((dict(null=True), "null"), (dict(rows=-1), "shape"), (dict(dim=66), "shape"),
                      (dict(dim=0), "shape"), (dict(dim=24580), "shape"), (dict(x=None), "null"),
-                     (dict(y=fake(4)), "aligned"), (dict(x_stride=60), "stride"),
+                     (dict(rows=(1 << 21) + 1), "shape"), (dict(y=fake(4)), "aligned"), (dict(x_stride=60), "stride"),
                      (dict(gate=fake(8)), "aligned"), (dict(h=fake(4)), "aligned"),
                      (dict(x_out=fake(), x_out_stride=66), "multiple"),
                      (dict(hq=fake()), "together"), (dict(hs=fake()), "together"),
@@ -842,6 +842,29 @@ def test_adapters_leave_rows_in_no_sequence(gh, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1 << 21, 1 << 22])
+def test_adapters_of_the_last_of_many_rows(gh, rows):
+    """As many rows as there may be, two of them in sequences."""
+    import torch
+
+    case = ([1, 1], 8, [8], 8, 2)
+    a, b, x, base, scale, _ = adapter_inputs(case, ADAPTER_BF16, 15)
+    ids = np.array([1, 0], np.int32)
+    row0 = np.array([rows - 2, rows - 1, rows], np.int32)
+    src, out = torch.zeros((2, rows, 8), device="cuda").unbind(0)
+    src[rows - 2:], old = x.cuda(), torch.zeros((rows, 8), device="cuda")
+    old[rows - 2:] = base.cuda()
+    ad = gemma_hip.adapters(cuda(row0), cuda(ids), scale.cuda(), 2, rows, 1, 2, 8, ADAPTER_BF16)
+    jobs = gemma_hip.adapter_jobs([(a[0].cuda(), b[0].cuda(), 8)])
+    work = torch.empty(gh.adapters_work(ad, 1, 8), dtype=torch.uint8, device="cuda")
+    gh.adapters_add(out, 0, old, 0, ad, jobs, src, 0, 8, work, stream())
+    want, size = adapters_expected(case, a, b, x, base, scale, ids)
+    room = (math.sqrt(24) + math.sqrt(24) + 8) * HALF
+    assert (np.abs(out[rows - 2:].cpu().double().numpy() - want) <= room * size).all()
+    assert not out[:rows - 2].any()
+
+
+@pytest.mark.gpu
 def test_adapters_without_scales_and_with_ids_that_lie(gh):
     import torch
 
@@ -957,6 +980,25 @@ def test_logprobs(gh, vocab, stride, targets, ntop, seed):
         assert close_logs(got["logp"][r], logp), (where, got["logp"][r], logp)
         assert close_logs(got["top_logp"][r], tl), where
         assert close_logs(got["entropy"][r], h), (where, got["entropy"][r], h)
+
+
+@pytest.mark.gpu
+def test_infinite_logits_at_any_temperature(gh):
+    """They share everything, also where the temperature is infinite and differences count nothing."""
+    import torch
+
+    rng = np.random.default_rng(3)
+    l = np.stack([row_of("infinite", 5000, rng) for _ in range(3)])
+    t, ids = np.array([np.inf, 1e-40, 3.0], F32), rng.integers(0, 5000, (3, 2)).astype(np.int32)
+    ids[:, 0] = l.argmax(1)
+    out = dict(logp=torch.empty((3, 2), device="cuda"), entropy=torch.empty(3, device="cuda"),
+               top_logp=torch.empty((3, 8), device="cuda"))
+    gh.logprobs(gemma_hip.scores(**out), cuda(l), 0, 3, 5000, cuda(t), cuda(ids), 2, 8, None,
+                stream())
+    for r in range(3):
+        logp, _, h, _, tl = describe(l[r], F64(t[r]), ids[r], 8)
+        assert close_logs(out["logp"][r].cpu(), logp) and close_logs(out["top_logp"][r].cpu(), tl)
+        assert close_logs(out["entropy"][r].item(), h)
 
 
 @pytest.mark.gpu
