@@ -72,13 +72,11 @@ __device__ __forceinline__ float next_up(float l) {
   return __int_as_float(b > 0 ? b + 1 : b - 1);
 }
 
+// A tile of row r by a wave; its part, runs (if TOP) and counts.
 template <bool TOP>
-__global__ __launch_bounds__(kThreads) void logprobs_scan_kernel(Logprobs a, Layout at) {
-  const int lane = threadIdx.x & 63, tiles = tiles_of(a.vocab);
-  const long unit = (long)blockIdx.x * (kThreads / 64) +
-                    __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  const int r = (int)(unit / tiles), tile = (int)(unit % tiles), c0 = tile * kTile;
-  if (r >= a.rows) return;
+__device__ __forceinline__ void scan_tile(const Logprobs &a, int r, int tile, Part *part,
+                                          float *runs, int *counts) {
+  const int lane = threadIdx.x & 63, c0 = tile * kTile;
   const float *row = a.logits + r * a.stride;
   float l[kLoads][4];
   if (c0 + kTile <= a.vocab) {
@@ -110,8 +108,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_scan_kernel(Logprobs a, Lay
       top = fmaxf(top, dpp_f32<kDppXor2>(top));
       top = fmaxf(top, dpp_f32<kDppHalfMirror>(top));
       top = fmaxf(top, dpp_f32<kDppMirror>(top));
-      if ((lane & 15) == 0)
-        reinterpret_cast<float *>(a.work + at.runs)[unit * kTileRuns + 4 * j + lane / 16] = top;
+      if ((lane & 15) == 0) runs[4 * j + lane / 16] = top;
     }
   }
   // S and T of a lane by its largest, then of the wave by the wave's
@@ -140,7 +137,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_scan_kernel(Logprobs a, Lay
   }
   s = group_sum_f32<64>(s);
   t = group_sum_f32<64>(t);
-  if (lane == 0) reinterpret_cast<Part *>(a.work + at.parts)[unit] = Part{top, s, t};
+  if (lane == 0) *part = Part{top, s, t};
   for (int k = 0; k < a.targets; ++k) {
     const int id = a.ids[(size_t)r * a.targets + k];
     int above = 0;
@@ -161,8 +158,20 @@ __global__ __launch_bounds__(kThreads) void logprobs_scan_kernel(Logprobs a, Lay
         }
       }
     }
-    if (lane == 0) reinterpret_cast<int *>(a.work + at.counts)[unit * a.targets + k] = above;
+    if (lane == 0) counts[k] = above;
   }
+}
+
+template <bool TOP>
+__global__ __launch_bounds__(kThreads) void logprobs_scan_kernel(Logprobs a, Layout at) {
+  const int tiles = tiles_of(a.vocab);
+  const long unit = (long)blockIdx.x * (kThreads / 64) +
+                    __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int r = (int)(unit / tiles), tile = (int)(unit % tiles);
+  if (r >= a.rows) return;
+  scan_tile<TOP>(a, r, tile, reinterpret_cast<Part *>(a.work + at.parts) + unit,
+                 reinterpret_cast<float *>(a.work + at.runs) + unit * kTileRuns,
+                 reinterpret_cast<int *>(a.work + at.counts) + unit * a.targets);
 }
 
 // Tokens and runs in the order of falling logit, then rising index, as falling whole numbers;
@@ -325,19 +334,18 @@ __device__ __forceinline__ void join_parts(JoinShared &sh, const Part (&p)[PARTS
     *entropy = drawn && top > -INFINITY ? (float)fmax(0.0, logs - ln2 * t / s) : 0.0f;
 }
 
-// RUNS: of a thread, at most.  A row's join is mostly waiting, so it takes two trips to memory: for
-// the runs and what else is there, and then for the columns of the runs that matter, while one wave
-// joins the parts and the others look up the given tokens.
+// A row's answers from its tiles' parts, runs and counts; RUNS: of a thread, at most.  It is mostly
+// waiting, so it takes two trips to memory: for the runs and what else is there, and then for the
+// columns of the runs that matter, while one wave joins the parts and the others look up the given
+// tokens.
 template <int NT, int RUNS>
-__global__ __launch_bounds__(NT) void logprobs_join_kernel(Logprobs a, Layout at) {
+__device__ __forceinline__ void join_row(const Logprobs &a, int r, JoinShared &sh,
+                                         const Part *parts, const float *runs,
+                                         const int *counts) {
   constexpr int kWaves = NT / 64;
-  __shared__ JoinShared sh;
-  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, tiles = tiles_of(a.vocab);
+  const int tid = threadIdx.x, lane = tid & 63, tiles = tiles_of(a.vocab);
   const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const float *row = a.logits + r * a.stride;
-  const float *runs = reinterpret_cast<const float *>(a.work + at.runs) +
-                      (size_t)r * tiles * kTileRuns;
-  const Part *parts = reinterpret_cast<const Part *>(a.work + at.parts) + (size_t)r * tiles;
   const int nruns = a.ntop > 0 ? (a.vocab + kRun - 1) / kRun : 0;
   float most[RUNS];
 #pragma unroll
@@ -382,8 +390,6 @@ __global__ __launch_bounds__(NT) void logprobs_join_kernel(Logprobs a, Layout at
     const double c = drawn ? fmin(0x1.71547652b82fep+0 / (double)temp, (double)FLT_MAX) : 0.0;
     join_parts(sh, part, drawn, c, a.entropy != nullptr ? a.entropy + r : nullptr);
   } else {
-    const int *counts = reinterpret_cast<const int *>(a.work + at.counts) +
-                        (size_t)r * tiles * a.targets;
     for (int k = wave; k < a.targets; k += kWaves - 1) {
       if (k != wave) id = a.ids[(size_t)r * a.targets + k];
       const bool there = (unsigned)id < (unsigned)a.vocab;
@@ -428,6 +434,32 @@ __global__ __launch_bounds__(NT) void logprobs_join_kernel(Logprobs a, Layout at
   }
 }
 
+template <int NT, int RUNS>
+__global__ __launch_bounds__(NT) void logprobs_join_kernel(Logprobs a, Layout at) {
+  __shared__ JoinShared sh;
+  const int r = blockIdx.x;
+  const size_t first = (size_t)r * tiles_of(a.vocab);
+  join_row<NT, RUNS>(a, r, sh, reinterpret_cast<const Part *>(a.work + at.parts) + first,
+                     reinterpret_cast<const float *>(a.work + at.runs) + first * kTileRuns,
+                     reinterpret_cast<const int *>(a.work + at.counts) + first * a.targets);
+}
+
+// Short rows by one workgroup, which keeps in LDS what the tiles leave: a launch (3.7 us on the host)
+// and a trip less.
+constexpr int kShortTiles = 16, kShortVocab = kShortTiles * kTile;
+template <int NT>
+__global__ __launch_bounds__(NT) void logprobs_short_kernel(Logprobs a) {
+  __shared__ JoinShared sh;
+  __shared__ Part parts[kShortTiles];
+  __shared__ float runs[kShortTiles * kTileRuns];
+  __shared__ int counts[kShortTiles * kLogprobsMaxTargets];
+  const int r = blockIdx.x, tiles = tiles_of(a.vocab);
+  for (int i = __builtin_amdgcn_readfirstlane(threadIdx.x / 64); i < tiles; i += NT / 64)
+    scan_tile<true>(a, r, i, parts + i, runs + i * kTileRuns, counts + i * a.targets);
+  __syncthreads();
+  join_row<NT, (kShortTiles * kTileRuns + NT - 1) / NT>(a, r, sh, parts, runs, counts);
+}
+
 }  // namespace
 
 size_t logprobs_work(int rows, int vocab, int targets, int ntop) {
@@ -435,6 +467,15 @@ size_t logprobs_work(int rows, int vocab, int targets, int ntop) {
 }
 
 hipError_t launch_logprobs(const Logprobs &a, const DeviceInfo &dev, hipStream_t stream) {
+  const bool many = a.rows > 2 * dev.cus;
+  // Short rows by one launch, but not many that leave most of a workgroup's waves without a tile: us by
+  // two launches and by one, 11 rows of 2511 10.4, 8.5, 256 of 32000 17.7, 14.4, 2048 of 32000 74, 61,
+  // 600 of 8000 19.6, 16.8, 2433 of 3023 32, 35.
+  if (a.vocab <= kShortVocab && (!many || tiles_of(a.vocab) >= 4)) {
+    many ? logprobs_short_kernel<256><<<a.rows, 256, 0, stream>>>(a)
+         : logprobs_short_kernel<1024><<<a.rows, 1024, 0, stream>>>(a);
+    return hipGetLastError();
+  }
   const Layout at = layout_of(a.rows, a.vocab, a.targets, a.ntop);
   const long units = (long)a.rows * tiles_of(a.vocab);
   const unsigned grid = (unsigned)((units + 3) / 4);
@@ -446,12 +487,14 @@ hipError_t launch_logprobs(const Logprobs &a, const DeviceInfo &dev, hipStream_t
   };
   const auto by = [&](auto nt) {
     const int runs = (a.vocab + kRun * nt() - 1) / (kRun * nt());
-    runs <= 1               ? join(nt, integral_constant<int, 1>())
-    : runs <= 4             ? join(nt, integral_constant<int, 4>())
+    if constexpr (nt() > 256) {
+      if (runs <= 1) return join(nt, integral_constant<int, 1>());
+    }
+    runs <= 4              ? join(nt, integral_constant<int, 4>())
     : runs <= kMost / 1024 ? join(nt, integral_constant<int, kMost / 1024>())
-                            : join(nt, integral_constant<int, kMost / nt()>());
+                           : join(nt, integral_constant<int, kMost / nt()>());
   };
-  a.rows > 2 * dev.cus ? by(integral_constant<int, 256>()) : by(integral_constant<int, 1024>());
+  many ? by(integral_constant<int, 256>()) : by(integral_constant<int, 1024>());
   return hipGetLastError();
 }
 

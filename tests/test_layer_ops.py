@@ -947,7 +947,7 @@ ROWS = ("normal", "ties", "equal", "peaked", "holes", "lowest", "infinite", "not
 @pytest.mark.parametrize("vocab,stride,targets,ntop", [
     (1, 0, 1, 1), (2, 3, 2, 64), (63, 0, 1, 5), (64, 65, 3, 64), (65, 0, 1, 20), (1000, 1003, 8, 0),
     (2047, 0, 0, 7), (2048, 2048, 1, 64), (2049, 0, 2, 1), (16000, 16001, 64, 33),
-    (70001, 0, 1, 64)])
+    (70001, 0, 1, 64), (32768, 32769, 3, 64), (32769, 0, 3, 9), (66000, 0, 1, 0)])
 @pytest.mark.parametrize("seed", [0, 1])
 def test_logprobs(gh, vocab, stride, targets, ntop, seed):
     import torch
@@ -1028,6 +1028,7 @@ def test_logprobs_of_a_whole_vocabulary(gh):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("vocab,ntop,targets", [(70, 64, 1), (3023, 12, 2), (20000, 64, 0),
+                                                (6145, 3, 0), (8000, 20, 1), (32768, 64, 2),
                                                 (70000, 5, 1), (270000, 64, 1)])
 def test_logprobs_of_many_rows(gh, vocab, ntop, targets):
     """More rows than compute units: rows that are repeated have the same answers, to the bit, and
@@ -1225,6 +1226,37 @@ def test_captured_calls_follow_the_tables(gh):
                 assert torch.equal(ly.st["p"].d[n][0], ref.st["p"].d[n][0])
             for k in o:
                 assert torch.equal(o[k], outs[i][0][k]), k
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,vocab", [(3, 40000), (600, 3000)])
+def test_captured_log_probabilities_of_two_launches(gh, rows, vocab):
+    """Replays on new logits, with eager work between, against eager calls."""
+    import torch
+
+    logits = torch.randn((rows, vocab), device="cuda")
+    ids = torch.zeros((rows, 2), dtype=torch.int32, device="cuda")
+    work = [torch.empty(gh.logprobs_work(rows, vocab, 2, 9), dtype=torch.uint8, device="cuda")
+            for _ in "ab"]
+    out = [dict(logp=torch.empty((rows, 2), device="cuda"), entropy=torch.empty(rows, device="cuda"),
+                rank=torch.empty((rows, 2), dtype=torch.int32, device="cuda"),
+                top=torch.empty((rows, 9), dtype=torch.int32, device="cuda")) for _ in "ab"]
+
+    def call(i, s):
+        gh.logprobs(gemma_hip.scores(**out[i]), logits, 0, rows, vocab, None, ids, 2, 9, work[i], s)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        call(0, s.cuda_stream)
+    for step in range(4):
+        logits.copy_(torch.randn((rows, vocab), device="cuda"))
+        ids.fill_(step * 7)
+        g.replay()
+        call(1, stream())
+        torch.cuda.synchronize()
+        assert all(torch.equal(out[0][k], out[1][k]) for k in out[0])
 
 
 @pytest.mark.gpu
