@@ -117,11 +117,14 @@ __global__ __launch_bounds__(NT == 64 ? kThreads : NT) void norm_residual_kernel
         x[j][e] = clamped(sum);
       }
     }
-  } else if (a.cx != 1.0f) {
+  } else {
 #pragma unroll
     for (int j = 0; j < NPT; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[j][e] = clamped((double)a.cx * (double)x[j][e]);
+      for (int e = 0; e < 4; ++e)
+        x[j][e] = a.cx != 1.0f                    ? clamped((double)a.cx * (double)x[j][e])
+                  : fabsf(x[j][e]) == INFINITY ? copysignf(FLT_MAX, x[j][e])
+                                               : x[j][e];
   }
   if (a.x_out != nullptr)
 #pragma unroll
