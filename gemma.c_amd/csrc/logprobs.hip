@@ -59,10 +59,24 @@ __host__ __device__ inline Layout layout_of(int rows, int vocab, int targets, in
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float no_nan(float l) { return fmaxf(l, -INFINITY); }
 
-// log2(e) / temperature; 0 where the temperature is 0 or none: all on the largest
-__device__ __forceinline__ float octaves_of(const float *temperature, int r) {
+// How many octaves l lies above m (l <= m) by a temperature: fma(h, l, -h m) c, h a power of two that
+// keeps both factors in fp32.  Finite logits may lie more than FLT_MAX apart, so where a logit is less
+// than an octave they are halved.  Where it is more than FLT_MAX octaves, h is 2^64 as long as m is
+// below 2^60: what this takes past FLT_MAX is further below m than any weight reaches; so is all that
+// isn't m itself about larger m, where FLT_MAX will do.  Anywhere else the bits are those of (l - m) c.
+struct Octaves {
+  float h, c;
+  __device__ __forceinline__ Octaves about(float m) const {
+    return h > 1.0f && !(fabsf(m) < 0x1p60f) ? Octaves{1.0f, FLT_MAX} : *this;
+  }
+};
+// c 0 where the temperature is 0 or none: all on the largest
+__device__ __forceinline__ Octaves octaves_of(const float *temperature, int r) {
   const float t = temperature != nullptr ? temperature[r] : 1.0f;
-  return t > 0.0f ? (float)fmin(0x1.71547652b82fep+0 / (double)t, (double)FLT_MAX) : 0.0f;
+  if (!(t > 0.0f)) return Octaves{1.0f, 0.0f};
+  const double c = 0x1.71547652b82fep+0 / (double)t;
+  const float h = c < 1.0 ? 0.5f : c > (double)FLT_MAX ? 0x1p64f : 1.0f;
+  return Octaves{h, (float)(c * (h == 0.5f ? 2.0 : h > 1.0f ? 0x1p-64 : 1.0))};
 }
 
 // The least float above l (l not NaN); of +inf: NaN, which nothing reaches.
@@ -97,7 +111,7 @@ __device__ __forceinline__ void scan_tile(const Logprobs &a, int r, int tile, Pa
         l[j][e] = c < a.vocab ? row[c] : -INFINITY;
       }
   }
-  const float c = octaves_of(a.temperature, r);
+  const Octaves octaves = octaves_of(a.temperature, r);
   float m = -INFINITY;
 #pragma unroll
   for (int j = 0; j < kLoads; ++j) {
@@ -113,11 +127,13 @@ __device__ __forceinline__ void scan_tile(const Logprobs &a, int r, int tile, Pa
   }
   // S and T of a lane by its largest, then of the wave by the wave's
   float s = 0.0f, t = 0.0f;
+  const Octaves by = octaves.about(m);
+  const float hm = by.h * m;
 #pragma unroll
   for (int j = 0; j < kLoads; ++j)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float x = fmaxf((l[j][e] - m) * c, kFar);  // NaN and -inf are far off
+      const float x = fmaxf(fmaf(by.h, l[j][e], -hm) * by.c, kFar);  // NaN and -inf are far off
       const float w = exp2_fast(x);
       s += w;
       t = fmaf(w, x, t);
@@ -130,7 +146,8 @@ __device__ __forceinline__ void scan_tile(const Logprobs &a, int r, int tile, Pa
 #pragma unroll
       for (int e = 0; e < 4; ++e) s += l[j][e] == INFINITY ? 1.0f : 0.0f;
   } else {
-    const float x = fmaxf((m - top) * c, kFar);
+    const Octaves by = octaves.about(top);
+    const float x = fmaxf(fmaf(by.h, m, -(by.h * top)) * by.c, kFar);
     const float w = exp2_fast(x);
     t = w * fmaf(s, x, t);
     s = w * s;
@@ -387,7 +404,7 @@ __device__ __forceinline__ void join_row(const Logprobs &a, int r, JoinShared &s
     if (col[j] < a.vocab) l[j] = row[col[j]];
   }
   if (joins) {
-    const double c = drawn ? fmin(0x1.71547652b82fep+0 / (double)temp, (double)FLT_MAX) : 0.0;
+    const double c = drawn ? 0x1.71547652b82fep+0 / (double)temp : 0.0;
     join_parts(sh, part, drawn, c, a.entropy != nullptr ? a.entropy + r : nullptr);
   } else {
     for (int k = wave; k < a.targets; k += kWaves - 1) {

@@ -8,7 +8,7 @@ import pytest
 
 import gemma_hip
 from gemma_hip import NORM_LAYER, NORM_RMS
-from test_layer_ops import F32, F64, codes_of_rows, normed, once
+from test_layer_ops import F32, F64, close_logs, codes_of_rows, describe, normed, once
 from test_serving import cuda, stream
 
 TOP = np.finfo(F32).max
@@ -46,3 +46,71 @@ def test_a_sum_without_a_block_is_clamped(gh, rows, dim, kind, x_scale):
     code, scale = codes_of_rows(got[fine])
     assert np.array_equal(q[fine], code) and np.array_equal(s[fine], scale)
     assert np.isnan(got[2]).all() and np.isnan(s[2]) and not q[2].any()
+
+
+# ---- log probabilities --------------------------------------------------------------
+
+
+def far_apart(vocab, t, rng, kind):
+    """Rows of finite logits whose differences pass FLT_MAX, or are no more than some temperatures
+    that fp32 holds as subnormals."""
+    if kind == "ends":
+        return rng.choice(np.array([-TOP, -3e38, 3e38, TOP], F32), vocab)
+    if kind == "two":
+        l = np.full(vocab, -3e38, F32)
+        l[rng.integers(0, vocab, 1 + vocab // 3)] = 3e38
+        return l
+    if kind == "spread":
+        return (rng.uniform(-1, 1, vocab) * F64(TOP)).astype(F32)
+    if kind == "holes":
+        l = (rng.uniform(-1, 1, vocab) * F64(TOP)).astype(F32)
+        l[rng.random(vocab) < 0.3] = -np.inf
+        l[rng.random(vocab) < 0.1] = np.nan
+        return l
+    if kind == "small":  # some temperatures apart
+        return (rng.standard_normal(vocab) * 3 * F64(t)).astype(F32)
+    l = (rng.standard_normal(vocab) * 3 * F64(t)).astype(F32)  # "mixed": far below as well
+    l[rng.random(vocab) < 0.5] = -1e30
+    return l
+
+
+FAR = [(k, t) for k in ("ends", "two", "spread", "holes")
+       for t in (np.inf, float(TOP), 3e38, 1e38, 1e37, 1.5, 1.0, 1e-40)] + \
+      [(k, t) for k in ("small", "mixed") for t in (1e-45, 1e-42, 1e-40, 4e-39, 1e-38, 1e30)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab,ntop,times", [(2, 2, 1), (70, 9, 1), (2100, 64, 1), (5000, 5, 1),
+                                              (40000, 12, 1), (3000, 4, 14), (9000, 7, 14)])
+def test_logits_at_any_distance(gh, vocab, ntop, times):
+    """Every kind of row at temperatures of its size, in one launch and in two; many rows are the
+    same ones repeated."""
+    import torch
+
+    rng = np.random.default_rng(vocab)
+    l = np.stack([far_apart(vocab, F32(t), rng, k) for k, t in FAR])
+    t = np.array([t for _, t in FAR], F32)
+    n = len(FAR)
+    rows, targets = n * times, 3
+    ids = rng.integers(0, vocab, (n, targets)).astype(np.int32)
+    ids[:, 0], ids[:, 1] = np.nan_to_num(l, nan=-np.inf, posinf=np.inf).argmax(1), \
+        np.nan_to_num(l, nan=np.inf).argmin(1)
+    out = dict(logp=torch.empty((rows, targets), device="cuda"),
+               rank=torch.empty((rows, targets), dtype=torch.int32, device="cuda"),
+               entropy=torch.empty(rows, device="cuda"),
+               top=torch.empty((rows, ntop), dtype=torch.int32, device="cuda"),
+               top_logp=torch.empty((rows, ntop), device="cuda"))
+    gh.logprobs(gemma_hip.scores(**out), cuda(l).repeat(times, 1), 0, rows, vocab,
+                cuda(t).repeat(times), cuda(ids).repeat(times, 1), targets, ntop, None, stream())
+    for v in out.values():
+        again = v.view(times, -1)
+        assert torch.equal(again, again[:1].expand_as(again))
+    got = {k: v[:n].cpu().numpy() for k, v in out.items()}
+    bad = []
+    for r in range(n):
+        logp, rank, h, top, tl = describe(l[r], F64(t[r]), ids[r], ntop)
+        assert np.array_equal(got["rank"][r], rank) and np.array_equal(got["top"][r], top), FAR[r]
+        if not (close_logs(got["logp"][r], logp) and close_logs(got["top_logp"][r], tl) and
+                close_logs(got["entropy"][r], h)):
+            bad.append((FAR[r], got["logp"][r], logp, got["entropy"][r], h))
+    assert not bad, bad
