@@ -9,7 +9,9 @@
 // Rows of prompts go 16 at a time through the bf16 matrix cores: an fp32 value is the sum of three
 // bf16 pieces, a bf16 weight is one, an f16 weight the sum of two and an fp32 weight of three, and
 // of the piece products those are summed whose orders add up to at most 2 (3, 5 or 6 of
-// them: what is left out is below 2^-22 of a product).  A tile is one sequence's: with tiles across
+// them: what is left out is below 2^-22 of a product).  Where pieces can't make a value up, an
+// infinity or one that rounds to an infinite bf16, the sums with it aren't finite, and such sums are
+// done over in fp32 as they are for single tokens.  A tile is one sequence's: with tiles across
 // sequences, which took a pass for each adapter, the few that had two set the time.
 //
 // The products are small; what bounds these kernels is how x, base and dst get in and out.  A load
@@ -28,8 +30,17 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kNone = -1, kOutside = -2;  // a row's id: no adapter, in no sequence
+constexpr float kBf16Most = 0x1.fep127f;
 
 typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));
+
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) < INFINITY; }
+// the largest magnitude of x and v; NaN if there is one
+__device__ __forceinline__ float largest(float x, v4f v) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x = __builtin_elementwise_maximum(x, fabsf(v[e]));
+  return x;
+}
 
 // ---- weights ---------------------------------------------------------------------
 
@@ -141,6 +152,33 @@ __device__ __forceinline__ int id_of_row(const Adapters &a, int r) {
   return (unsigned)id < (unsigned)a.count ? id : kNone;
 }
 
+// Sums of a row's inputs times N rows of weights, in fp32, by a whole wave, in all its lanes.
+template <int TYPE, int N>
+__device__ __forceinline__ void row_sums(const float *x, const void *const (&m)[N],
+                                         const size_t (&first)[N], int k, float (&s)[N]) {
+#pragma unroll
+  for (int t = 0; t < N; ++t) s[t] = 0.0f;
+  for (int c = 8 * (threadIdx.x & 63); c < k; c += 512) {
+    const v4f x0 = *reinterpret_cast<const v4f *>(x + c);
+    const v4f x1 = *reinterpret_cast<const v4f *>(x + c + 4);
+    Raw8<TYPE> w[N];
+#pragma unroll
+    for (int t = 0; t < N; ++t) w[t] = raw8<TYPE>(m[t], first[t] + c);
+#pragma unroll
+    for (int t = 0; t < N; ++t) {
+      float f[8];
+      floats8<TYPE>(w[t], f);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[t] = fmaf(x0[e], f[e], s[t]);
+        s[t] = fmaf(x1[e], f[e + 4], s[t]);
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < N; ++t) s[t] = group_sum_f32<64>(s[t]);
+}
+
 template <int TYPE>
 __global__ __launch_bounds__(kThreads) void adapter_shrink_row_kernel(Adapters a) {
   const int all = a.njobs * a.rank, lane = threadIdx.x & 63, r = blockIdx.x;
@@ -150,20 +188,11 @@ __global__ __launch_bounds__(kThreads) void adapter_shrink_row_kernel(Adapters a
   const int id = id_of_row(a, r);
   if (at == 0 && lane == 0) ids_of(a)[r] = id;
   if (id < 0) return;
-  const void *m = job_of(a.a, job);
-  const size_t first = ((size_t)id * a.rank + row) * a.k;
-  const float *x = a.src + r * a.src_stride;
-  float s = 0.0f;
-  for (int c = 8 * lane; c < a.k; c += 512) {
-    float w[8];
-    floats8<TYPE>(raw8<TYPE>(m, first + c), w);
-    const v4f x0 = *reinterpret_cast<const v4f *>(x + c);
-    const v4f x1 = *reinterpret_cast<const v4f *>(x + c + 4);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) s = fmaf(x0[e], w[e], s), s = fmaf(x1[e], w[e + 4], s);
-  }
-  s = group_sum_f32<64>(s);
-  if (lane == 0) u_of(a)[(size_t)r * all + at] = scale_of(a, id) * s;
+  const void *const m[1] = {job_of(a.a, job)};
+  const size_t first[1] = {((size_t)id * a.rank + row) * a.k};
+  float s[1];
+  row_sums<TYPE, 1>(a.src + r * a.src_stride, m, first, a.k, s);
+  if (lane == 0) u_of(a)[(size_t)r * all + at] = scale_of(a, id) * s[0];
 }
 
 // ---- tiles of rows ------------------------------------------------------------------
@@ -325,19 +354,47 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void adapter_shrink_kernel(Adapt
 #pragma unroll
   for (int t = 0; t < T; ++t) sh.part[wave][t][lane] = acc[t];
   __syncthreads();
-  const int at = at0 + 16 * wave + 4 * (lane / 16);
-  if (wave >= T || (lane & 15) >= tile.rows || at >= all) return;
+  if (wave >= T) return;
+  const int at = at0 + 16 * wave + 4 * (lane / 16), m16 = lane & 15;
   v4f sum = sh.part[0][wave][lane];
 #pragma unroll
   for (int w = 1; w < kShrinkWaves; ++w) sum += sh.part[w][wave][lane];
+  const bool has = m16 < tile.rows && at < all;
+  // Pieces don't make up an infinity, nor a value that rounds to an infinite bf16; sums of such ones
+  // are never finite, and are done over without pieces, one after the other.
+  if (__any(has && !finite(largest(0.0f, sum)))) {
+    for (int e = 0; e < 4; ++e) {
+      const float mine = e == 0 ? sum[0] : e == 1 ? sum[1] : e == 2 ? sum[2] : sum[3];
+      for (uint64_t bad = __ballot(has && !finite(mine)); bad != 0; bad &= bad - 1) {
+        const int of = __ffsll((unsigned long long)bad) - 1;
+        const int u = at0 + 16 * wave + 4 * (of / 16) + e, job = u / a.rank;
+        const void *const m[1] = {job_of(a.a, job)};
+        const size_t first[1] = {((size_t)tile.id * a.rank + (u - job * a.rank)) * a.k};
+        float s[1];
+        row_sums<TYPE, 1>(a.src + (tile.row + of % 16) * a.src_stride, m, first, a.k, s);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] = lane == of && i == e ? s[0] : sum[i];
+      }
+    }
+  }
+  if (!has) return;
   sum *= scale_of(a, tile.id);
   const int job = at / a.rank, value = at - job * a.rank;
+  // u is the sum of its pieces whatever it is: the first one of a finite value is finite, and those
+  // behind the first of another are zeros
+  v4f first = sum;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (finite(sum[e])) first[e] = fminf(fmaxf(sum[e], -kBf16Most), kBf16Most);
 #pragma unroll
   for (int p = 0; p < 3; ++p) {
-    const u2 b = {cvt_pk_bf16(sum[0], sum[1]), cvt_pk_bf16(sum[2], sum[3])};
+    const v4f of = p == 0 ? first : sum;
+    const u2 b = {cvt_pk_bf16(of[0], of[1]), cvt_pk_bf16(of[2], of[3])};
     *reinterpret_cast<u2 *>(piece_of(a, tile.row, tile.rows, job, p) +
-                            (value / 8 * tile.rows + (lane & 15)) * 8 + value % 8) = b;
+                            (value / 8 * tile.rows + m16) * 8 + value % 8) = b;
     sum -= v4f{bf16_lo(b[0]), bf16_hi(b[0]), bf16_lo(b[1]), bf16_hi(b[1])};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[e] = finite(of[e]) ? sum[e] : 0.0f;
   }
 }
 
@@ -479,28 +536,10 @@ __global__ __launch_bounds__(64 * kRowWaves) void adapter_row_kernel(Adapters a,
         const int at = min(at0 + t * kRowWaves, all - 1), job = at / a.rank;
         m[t] = job_of(a.a, job);
         first[t] = ((size_t)id * a.rank + (at - job * a.rank)) * a.k;
-        s[t] = 0.0f;
       }
-      for (int c = 8 * lane; c < a.k; c += 512) {
-        const v4f x0 = *reinterpret_cast<const v4f *>(x + c);
-        const v4f x1 = *reinterpret_cast<const v4f *>(x + c + 4);
-        Raw8<TYPE> w[kRowValues];
-#pragma unroll
-        for (int t = 0; t < kRowValues; ++t) w[t] = raw8<TYPE>(m[t], first[t] + c);
-#pragma unroll
-        for (int t = 0; t < kRowValues; ++t) {
-          float f[8];
-          floats8<TYPE>(w[t], f);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            s[t] = fmaf(x0[e], f[e], s[t]);
-            s[t] = fmaf(x1[e], f[e + 4], s[t]);
-          }
-        }
-      }
+      row_sums<TYPE, kRowValues>(x, m, first, a.k, s);
 #pragma unroll
       for (int t = 0; t < kRowValues; ++t) {
-        s[t] = group_sum_f32<64>(s[t]);
         const int at = at0 + t * kRowWaves;
         if (lane == 0 && at < all) u[at] = scale_of(a, id) * s[t];
       }
@@ -632,6 +671,7 @@ void adapter_expand_kernel(Adapters a) {
   if (tile.id >= 0) {
     // values behind the rank are zeros on both sides
     constexpr int W = KS < 4 && (KS == 1 || TYPE != kAdapterF32) ? 4 : 2;  // read together
+    float most = 0.0f;  // of the products' magnitudes
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
@@ -671,13 +711,44 @@ void adapter_expand_kernel(Adapters a) {
           for (int i = 0; i < RT; ++i) d[i] = product(wp, u[i][s], d[i]);
         }
 #pragma unroll
-        for (int i = 0; i < RT; ++i)
+        for (int i = 0; i < RT; ++i) {
           *reinterpret_cast<v4f *>(&sums[16 * i + m][16 * (t0 + t) + 4 * quarter]) = d[i];
+          most = largest(most, d[i]);
+        }
       }
     }
     // written and read by the same wave, whose LDS accesses keep their order
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
+    if (__any(!finite(most))) {  // as in the first product; a lane a column
+      for (int r = 0; r < tile.rows; ++r) {
+        const bool bad = c0 + lane < width && !finite(sums[r][lane]);
+        if (!__any(bad)) continue;
+        const int rows = min(tile.rows - r / 16 * 16, 16);
+        const size_t row = (size_t)(bad ? lane : 0) * a.rank;
+        float s = 0.0f;
+        for (int k = 0; k < a.rank; k += 8) {
+          float w[8];
+          floats8<TYPE>(raw8<TYPE>(b, row + k), w);
+          Split8<3> v;
+#pragma unroll
+          for (int p = 0; p < 3; ++p)
+            v.p[p] = *reinterpret_cast<const u4 *>(
+                piece_of(a, tile.row + r / 16 * 16, rows, job, p) + (k / 8 * rows + r % 16) * 8);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            float x = 0.0f;
+#pragma unroll
+            for (int p = 2; p >= 0; --p)
+              x += e % 2 ? bf16_hi(v.p[p][e / 2]) : bf16_lo(v.p[p][e / 2]);
+            s = fmaf(x, w[e], s);
+          }
+        }
+        if (bad) sums[r][lane] = s;
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
 #pragma unroll
     for (int j = 0; j < 4 * RT; ++j)
       old[j] += *reinterpret_cast<const v4f *>(&sums[4 * j + quarter][4 * m]);

@@ -3,12 +3,15 @@ are those of test_layer_ops.py, or stand beside the test."""
 
 from __future__ import annotations
 
+import math
+
 import numpy as np
 import pytest
 
 import gemma_hip
-from gemma_hip import NORM_LAYER, NORM_RMS
-from test_layer_ops import F32, F64, close_logs, codes_of_rows, describe, normed, once
+from gemma_hip import ADAPTER_BF16, ADAPTER_F16, ADAPTER_F32, NORM_LAYER, NORM_RMS
+from test_layer_ops import (F32, F64, HALF, TYPES, adapters_expected, close_logs, codes_of_rows,
+                            describe, normed, once)
 from test_serving import cuda, stream
 
 TOP = np.finfo(F32).max
@@ -114,3 +117,97 @@ def test_logits_at_any_distance(gh, vocab, ntop, times):
                 close_logs(got["entropy"][r], h)):
             bad.append((FAR[r], got["logp"][r], logp, got["entropy"][r], h))
     assert not bad, bad
+
+
+# ---- adapters ---------------------------------------------------------------------
+
+
+def one_adapter(gh, kind, a, b, x, scale=1.0, most=None):
+    """A sequence's rows of zeros through one adapter, on the GPU: (result, definition in fp64, sums
+    of the terms' magnitudes)."""
+    import torch
+
+    dt = {ADAPTER_F32: torch.float32, ADAPTER_BF16: torch.bfloat16, ADAPTER_F16: torch.float16}[kind]
+    a, b, x = torch.from_numpy(a)[None].to(dt), torch.from_numpy(b)[None].to(dt), torch.from_numpy(x)
+    (rows, k), (n, rank) = x.shape, b.shape[1:]
+    base, scale = torch.zeros((rows, n)), torch.tensor([scale], dtype=torch.float32)
+    ad = gemma_hip.adapters(cuda(np.array([0, rows], np.int32)), cuda(np.zeros(1, np.int32)),
+                            scale.cuda(), 1, rows, most or rows, 1, rank, kind)
+    jobs = gemma_hip.adapter_jobs([(a.cuda(), b.cuda(), n)])
+    out = torch.full((rows, n), 7.0, device="cuda")
+    gh.adapters_add(out, 0, base.cuda(), 0, ad, jobs, x.cuda(), 0, k, None, stream())
+    with np.errstate(all="ignore"):
+        want, size = adapters_expected(([rows], k, [n], rank, 1), [a], [b], x, base, scale, [0])
+    return out.cpu().numpy().astype(F64), want, size
+
+
+def agree(got, want, size, k, rank):
+    """Within the bar where the definition is finite, the same infinity or NaN elsewhere."""
+    room = (math.sqrt(3 * k) + math.sqrt(3 * rank) + 8) * HALF
+    fine = np.isfinite(want)
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    assert np.array_equal(got[np.isinf(want)], want[np.isinf(want)])
+    with np.errstate(invalid="ignore"):
+        assert (np.abs(got - want)[fine] <= room * size[fine]).all()
+
+
+# by the row in one launch and in two (n), by tiles, by tiles whose waves share the matrices
+ENDS = [(2, 70), (2, 9000), (3, 70), (40, 70), (100, 70), (100, 64)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows,n", ENDS)
+@pytest.mark.parametrize("rank", [8, 40, 128])
+@pytest.mark.parametrize("where", ["x", "u", "a", "b"])
+def test_adapters_at_the_largest_values(gh, kind, rows, n, rank, where):
+    """Values from the largest that rounds to a finite bf16 up to FLT_MAX, among the inputs, the
+    first product's results and the matrices, beside ones that leave the answers finite."""
+    k, rng = 136, np.random.default_rng(rows + n)
+    ends = np.array([TOP, -TOP, 3.3961775e38, 3.3961777e38, -3.4e38, 1e38], F32)
+    a, b = rng.standard_normal((rank, k)), rng.standard_normal((n, rank))
+    x = rng.standard_normal((rows, k))
+    if where == "x":
+        a, b = a * 2.0 ** -10, b * 2.0 ** -10
+    elif where == "u":  # the first inputs, as they are
+        a, b = np.eye(rank, k), b * 2.0 ** -10
+    else:
+        x *= 2.0 ** -20
+        a = a if where == "a" else np.eye(rank, k)
+        b = b * 2.0 ** -10 if where == "a" else b
+    a, b, x = a.astype(F32), b.astype(F32), x.astype(F32)
+    if where in "xu":
+        x[0, 1], x[-1, 2:8] = TOP, ends
+        x[rows // 2, :6] = ends
+    else:  # f16 ends at 65504, bf16 at 3.39e38
+        m = a if where == "a" else b
+        top = {"f32": 1.0, "bf16": 0.99, "f16": 65504 / F64(TOP)}[kind]
+        m[1, 2:8], m[-1, 0] = (ends * top).astype(F32), F32(TOP * top)
+    got, want, size = one_adapter(gh, TYPES[kind], a, b, x)
+    assert np.isfinite(want).all() and size.max() < F64(TOP)
+    agree(got, want, size, k, rank)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows,n", ENDS)
+@pytest.mark.parametrize("rank", [8, 40, 128])
+def test_adapters_of_infinities(gh, kind, rows, n, rank):
+    """One infinity or NaN in the inputs or the matrices comes out where it belongs, and nowhere
+    else."""
+    k, rng = 136, np.random.default_rng(rows + n)
+    a, b = (rng.random(s).astype(F32) + F32(0.5) for s in ((rank, k), (n, rank)))
+    x = rng.random((rows, k)).astype(F32) + F32(0.5)
+    for where in range(4):
+        p, q, y = a.copy(), b.copy(), x.copy()
+        if where == 0:
+            y[0, 3], y[-1, k - 1] = np.inf, -np.inf
+        elif where == 1:
+            y[rows // 2, 7], q[5] = np.nan, -q[5]
+        elif where == 2:
+            p[rank - 1, 9], q[:, rank - 1] = np.inf, np.where(np.arange(n) % 3 == 0, 0.0, 1.0)
+        else:
+            q[5, 2], q[n - 1, rank - 1], q[6, 1] = np.inf, -np.inf, np.nan
+        got, want, size = one_adapter(gh, TYPES[kind], p, q, y)
+        assert not np.isfinite(want).all()
+        agree(got, want, size, k, rank)
