@@ -152,34 +152,49 @@ __device__ __forceinline__ int id_of_row(const Adapters &a, int r) {
   return (unsigned)id < (unsigned)a.count ? id : kNone;
 }
 
-// Sums of a row's inputs times N rows of weights, in fp32, by a whole wave, in all its lanes.
-template <int TYPE, int N>
+// Inputs whose products are summed in fp32; sums of more (LONG) meet in fp64.  One product is added
+// after the other, and where the roundings all point one way, as those of equal products do, sums of
+// 10240 inputs were up to 4.5e-6 off and of 2^20 up to 1.5e-4; both 2e-6 so.  The fp64 sums take
+// registers, so kernels for fewer inputs go without.
+constexpr int kSpan = 4096;
+
+// Sums of a row's inputs times N rows of weights, by a whole wave, in all its lanes.
+template <int TYPE, bool LONG, int N>
 __device__ __forceinline__ void row_sums(const float *x, const void *const (&m)[N],
                                          const size_t (&first)[N], int k, float (&s)[N]) {
+  double far[N] = {};
+  for (int k0 = 0; k0 < k; k0 += kSpan) {
 #pragma unroll
-  for (int t = 0; t < N; ++t) s[t] = 0.0f;
-  for (int c = 8 * (threadIdx.x & 63); c < k; c += 512) {
-    const v4f x0 = *reinterpret_cast<const v4f *>(x + c);
-    const v4f x1 = *reinterpret_cast<const v4f *>(x + c + 4);
-    Raw8<TYPE> w[N];
+    for (int t = 0; t < N; ++t) s[t] = 0.0f;
+    for (int c = k0 + 8 * (threadIdx.x & 63); c < (LONG ? min(k, k0 + kSpan) : k); c += 512) {
+      const v4f x0 = *reinterpret_cast<const v4f *>(x + c);
+      const v4f x1 = *reinterpret_cast<const v4f *>(x + c + 4);
+      Raw8<TYPE> w[N];
 #pragma unroll
-    for (int t = 0; t < N; ++t) w[t] = raw8<TYPE>(m[t], first[t] + c);
+      for (int t = 0; t < N; ++t) w[t] = raw8<TYPE>(m[t], first[t] + c);
+#pragma unroll
+      for (int t = 0; t < N; ++t) {
+        float f[8];
+        floats8<TYPE>(w[t], f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[t] = fmaf(x0[e], f[e], s[t]);
+          s[t] = fmaf(x1[e], f[e + 4], s[t]);
+        }
+      }
+    }
+    if (!LONG) break;
 #pragma unroll
     for (int t = 0; t < N; ++t) {
-      float f[8];
-      floats8<TYPE>(w[t], f);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[t] = fmaf(x0[e], f[e], s[t]);
-        s[t] = fmaf(x1[e], f[e + 4], s[t]);
-      }
+      far[t] += (double)s[t];
+      s[t] = (float)far[t];
     }
   }
 #pragma unroll
   for (int t = 0; t < N; ++t) s[t] = group_sum_f32<64>(s[t]);
 }
 
-template <int TYPE>
+template <int TYPE, bool LONG>
 __global__ __launch_bounds__(kThreads) void adapter_shrink_row_kernel(Adapters a) {
   const int all = a.njobs * a.rank, lane = threadIdx.x & 63, r = blockIdx.x;
   const int at = blockIdx.y * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -191,7 +206,7 @@ __global__ __launch_bounds__(kThreads) void adapter_shrink_row_kernel(Adapters a
   const void *const m[1] = {job_of(a.a, job)};
   const size_t first[1] = {((size_t)id * a.rank + row) * a.k};
   float s[1];
-  row_sums<TYPE, 1>(a.src + r * a.src_stride, m, first, a.k, s);
+  row_sums<TYPE, LONG, 1>(a.src + r * a.src_stride, m, first, a.k, s);
   if (lane == 0) u_of(a)[(size_t)r * all + at] = scale_of(a, id) * s[0];
 }
 
@@ -301,7 +316,7 @@ struct ShrinkStep {
 
 // u of a tile of 16 rows and 16 T of their values; each wave takes every eighth step, the partial
 // sums meet in LDS.
-template <int TYPE, int T>
+template <int TYPE, int T, bool LONG>
 __global__ __launch_bounds__(64 * kShrinkWaves) void adapter_shrink_kernel(Adapters a) {
   typedef ShrinkStep<TYPE, T> Step;
   __shared__ union {
@@ -346,9 +361,20 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void adapter_shrink_kernel(Adapt
     one.load(x, m, k, a.k);
     two.load(x, m, k + kNext, a.k);
   }
-  for (; k < a.k; k += 2 * kNext) {
-    step(one, k);
-    if (k + kNext < a.k) step(two, k + kNext);
+  double far[T][4] = {};
+  for (int end = kSpan; k < a.k; end += kSpan) {
+    for (; k < (LONG ? min(a.k, end) : a.k); k += 2 * kNext) {
+      step(one, k);
+      if (k + kNext < a.k) step(two, k + kNext);
+    }
+    if (!LONG) break;
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        far[t][e] += (double)acc[t][e];
+        acc[t][e] = k < a.k ? 0.0f : (float)far[t][e];
+      }
   }
   __syncthreads();
 #pragma unroll
@@ -371,7 +397,7 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void adapter_shrink_kernel(Adapt
         const void *const m[1] = {job_of(a.a, job)};
         const size_t first[1] = {((size_t)tile.id * a.rank + (u - job * a.rank)) * a.k};
         float s[1];
-        row_sums<TYPE, 1>(a.src + (tile.row + of % 16) * a.src_stride, m, first, a.k, s);
+        row_sums<TYPE, LONG, 1>(a.src + (tile.row + of % 16) * a.src_stride, m, first, a.k, s);
 #pragma unroll
         for (int i = 0; i < 4; ++i) sum[i] = lane == of && i == e ? s[0] : sum[i];
       }
@@ -516,7 +542,7 @@ __global__ __launch_bounds__(kThreads) void adapter_expand_row_kernel(Adapters a
 // Both products of a row by one workgroup, u in LDS: a launch less (of 3.7 us on the host), where a row
 // has little to read.
 constexpr int kRowWaves = 16, kRowValues = 4;  // values of u a wave has in flight
-template <int TYPE, int CHUNKS>
+template <int TYPE, int CHUNKS, bool LONG>
 __global__ __launch_bounds__(64 * kRowWaves) void adapter_row_kernel(Adapters a, int units) {
   typedef ExpandRow<TYPE, CHUNKS> Expand;
   __shared__ float u[kAdapterMaxJobs * kAdapterMaxRank];
@@ -537,7 +563,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void adapter_row_kernel(Adapters a,
         m[t] = job_of(a.a, job);
         first[t] = ((size_t)id * a.rank + (at - job * a.rank)) * a.k;
       }
-      row_sums<TYPE, kRowValues>(x, m, first, a.k, s);
+      row_sums<TYPE, LONG, kRowValues>(x, m, first, a.k, s);
 #pragma unroll
       for (int t = 0; t < kRowValues; ++t) {
         const int at = at0 + t * kRowWaves;
@@ -790,10 +816,14 @@ hipError_t launch_adapters(const Adapters &a, const DeviceInfo &dev, hipStream_t
                      rows <= 1 << 21;  // (a grid has 2^32 - 1 threads at most)
     auto go = [&](auto chunks) {
       if (one) {
-        adapter_row_kernel<type(), chunks()><<<rows, 64 * kRowWaves, 0, stream>>>(a, units);
+        a.k > kSpan ? adapter_row_kernel<type(), chunks(), true>
+                          <<<rows, 64 * kRowWaves, 0, stream>>>(a, units)
+                    : adapter_row_kernel<type(), chunks(), false>
+                          <<<rows, 64 * kRowWaves, 0, stream>>>(a, units);
       } else {
         const dim3 first(rows, (all + 3) / 4), second(rows, (units + 3) / 4);
-        adapter_shrink_row_kernel<type()><<<first, kThreads, 0, stream>>>(a);
+        a.k > kSpan ? adapter_shrink_row_kernel<type(), true><<<first, kThreads, 0, stream>>>(a)
+                    : adapter_shrink_row_kernel<type(), false><<<first, kThreads, 0, stream>>>(a);
         adapter_expand_row_kernel<type(), chunks()><<<second, kThreads, 0, stream>>>(a);
       }
     };
@@ -804,7 +834,9 @@ hipError_t launch_adapters(const Adapters &a, const DeviceInfo &dev, hipStream_t
   const int slots = tile_slots(a.seq, 16);
   auto shrink = [&](auto type, auto t) {
     const dim3 grid(slots, (all + 16 * t() - 1) / (16 * t()));
-    adapter_shrink_kernel<type(), t()><<<grid, 64 * kShrinkWaves, 0, stream>>>(a);
+    a.k > kSpan
+        ? adapter_shrink_kernel<type(), t(), true><<<grid, 64 * kShrinkWaves, 0, stream>>>(a)
+        : adapter_shrink_kernel<type(), t(), false><<<grid, 64 * kShrinkWaves, 0, stream>>>(a);
   };
   auto expand = [&](auto type, auto ks, auto rt) {
     constexpr int kWaves = kThreads / 64, R = 16 * rt();

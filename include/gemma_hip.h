@@ -812,9 +812,10 @@ typedef struct {
  * same rows side by side, job j's columns behind those of the jobs before it.  src fp32 [rows][sstr],
  * 16-byte aligned, sstr a multiple of 4, k a multiple of 8; base and dst fp32 [rows][bstr], [dstr]
  * (0: dense); dst may be base with its stride, and overlaps neither otherwise.  Rows of sequences
- * without an adapter are base; rows behind the last sequence stay as they were.  Sums are fp32, of
- * products as exact as fp32 ones: a result is off by at most about 1e-6 of the sum of its terms'
- * magnitudes.
+ * without an adapter are base; rows behind the last sequence stay as they were.  Sums are fp32, over
+ * 4096 inputs at most and fp64 beyond, of products as exact as fp32 ones: a result is off by at most
+ * 1e-5 of the sum of its terms' magnitudes, by 2e-6 where equal terms are all rounded one way, mostly
+ * by 1e-7.
  * work: gemma_hip_adapters_work() bytes, 256-byte aligned, which one call at a time may use; NULL
  * takes the library's for the stream (not while it is being captured). */
 int gemma_hip_adapters_add(float *dst, int dstr, const float *base, int bstr,

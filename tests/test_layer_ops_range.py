@@ -211,3 +211,20 @@ def test_adapters_of_infinities(gh, kind, rows, n, rank):
         got, want, size = one_adapter(gh, TYPES[kind], p, q, y)
         assert not np.isfinite(want).all()
         agree(got, want, size, k, rank)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows,k", [(1, 10240), (3, 10240), (1, 1 << 20), (3, 1 << 20)])
+def test_adapters_of_many_inputs(gh, kind, rows, k):
+    """Sums of equal terms, whose roundings all point one way.  Sums are fp32 over 4096 inputs at
+    most and fp64 beyond.  By the row: 64 products to a lane's sum, 6 sums of lanes; by the tile 8
+    steps of 2 times up to 6 products, 8 sums of waves; then the scale, u B of rank 8 in up to 9
+    additions (6 products) and the base: 96 + 8 + 1 + 9 + 1 roundings of 2^-24 at most, and products
+    off by 2^-22 twice: 7.4e-6 of the sum of magnitudes, below the 1e-5 that is promised."""
+    rank, n, rng = 8, 24, np.random.default_rng(k)
+    a = np.repeat((rng.random((rank, 1)) + 0.5).astype(F32), k, 1)
+    b = np.repeat((rng.random((n, 1)) + 0.5).astype(F32), rank, 1)
+    x = np.repeat((rng.random((rows, 1)) + 0.5).astype(F32), k, 1)
+    got, want, size = one_adapter(gh, TYPES[kind], a, b, x)
+    assert (np.abs(got - want) <= 1e-5 * size).all(), (np.abs(got - want) / size).max()
