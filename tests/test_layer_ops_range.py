@@ -228,3 +228,36 @@ def test_adapters_of_many_inputs(gh, kind, rows, k):
     x = np.repeat((rng.random((rows, 1)) + 0.5).astype(F32), k, 1)
     got, want, size = one_adapter(gh, TYPES[kind], a, b, x)
     assert (np.abs(got - want) <= 1e-5 * size).all(), (np.abs(got - want) / size).max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows", [2, 3, 100])
+@pytest.mark.parametrize("where", ["x", "u", "a"])
+def test_adapters_of_the_smallest_values(gh, kind, rows, where):
+    """bf16 pieces reach down to 2^-133, so in tiles a value counts to half that; its partner's
+    magnitudes and the other matrix make of it what they do."""
+    import torch
+
+    k, n, rank, rng = 136, 70, 16, np.random.default_rng(rows)
+    a, b = (rng.standard_normal(s).astype(F32) for s in ((rank, k), (n, rank)))
+    x = rng.standard_normal((rows, k)).astype(F32)
+    scale = 1.0
+    if where == "x":
+        x, scale = x * F32(1e-36), 1e30
+    elif where == "u":
+        scale = 1e-36
+    elif kind == "f16":
+        a = a * F32(1e-7)
+    else:
+        a, scale = a * F32(1e-36), 1e30
+    got, want, size = one_adapter(gh, TYPES[kind], a, b, x, scale)
+    dt = {"f32": F32, "f16": np.float16}.get(kind)
+    p, q = (torch.from_numpy(m).to(torch.bfloat16).double().numpy() if dt is None else
+            m.astype(dt).astype(F64) for m in (a, b))
+    s, step = F64(F32(scale)), 2.0 ** -134
+    # halves of the last piece's step: of the inputs, of A (its pieces), of u
+    floor = s * step * (np.abs(p).sum(1) + np.abs(x.astype(F64)).sum(1)[:, None]) @ np.abs(q).T
+    floor += step * np.abs(q).sum(1)
+    room = (math.sqrt(3 * k) + math.sqrt(3 * rank) + 8) * HALF
+    assert (np.abs(got - want) <= room * size + 1.01 * floor).all()
