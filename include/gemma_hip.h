@@ -815,8 +815,9 @@ typedef struct {
  * without an adapter are base; rows behind the last sequence stay as they were.  Sums are fp32, over
  * 4096 inputs at most and fp64 beyond, of products as exact as fp32 ones: a result is off by at most
  * 1e-5 of the sum of its terms' magnitudes, by 2e-6 where equal terms are all rounded one way, mostly
- * by 1e-7.  Where max_rows passes 2, a value of src, of an fp32 matrix or of scale[id] a[id] src
- * counts to 2^-134, which is less exact than that below 2^-110.
+ * by 1e-7, as long as terms and sums are normal numbers.  Where max_rows passes 2, a value of src, of
+ * an fp32 matrix or of scale[id] a[id] src counts to 2^-134, which is less exact than that below
+ * 2^-110.
  * work: gemma_hip_adapters_work() bytes, 256-byte aligned, which one call at a time may use; NULL
  * takes the library's for the stream (not while it is being captured). */
 int gemma_hip_adapters_add(float *dst, int dstr, const float *base, int bstr,
