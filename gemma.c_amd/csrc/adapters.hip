@@ -807,15 +807,19 @@ size_t adapters_work(int rows, int njobs, int rank) {
   return ((size_t)rows * (njobs * rank * 6 + 4) + 255) / 256 * 256;
 }
 
+bool adapters_one_launch(const Adapters &a) {
+  const long weights = (long)a.njobs * a.rank * a.k + (long)a.end[a.njobs - 1] * a.rank;
+  return a.seq.max_rows <= kFewRows && weights * (a.type == kAdapterF32 ? 4 : 2) <= kRowBytes &&
+         a.seq.rows <= 1 << 21;  // (a grid has 2^32 - 1 threads at most)
+}
+
 hipError_t launch_adapters(const Adapters &a, const DeviceInfo &dev, hipStream_t stream) {
   const int rows = a.seq.rows, all = a.njobs * a.rank;
   auto by_row = [&](auto type) {
     constexpr int kSize = type() == kAdapterF32 ? 4 : 2;
     const int units = expand_units(a.end, a.njobs);
-    const bool one = ((long)all * a.k + (long)a.end[a.njobs - 1] * a.rank) * kSize <= kRowBytes &&
-                     rows <= 1 << 21;  // (a grid has 2^32 - 1 threads at most)
     auto go = [&](auto chunks) {
-      if (one) {
+      if (adapters_one_launch(a)) {
         a.k > kSpan ? adapter_row_kernel<type(), chunks(), true>
                           <<<rows, 64 * kRowWaves, 0, stream>>>(a, units)
                     : adapter_row_kernel<type(), chunks(), false>

@@ -1103,9 +1103,10 @@ int attn_args(const char *name, const gemma_hip_cache *cache, const gemma_hip_ba
 }
 
 // The workspace of a call: the caller's, or the one kept for the stream, which alone is held:
-// a call that needs none, or has its own, waits for no other thread's.
+// a call that needs none, or has its own, waits for no other thread's.  unused: the call writes to
+// none at these sizes, so the library's isn't taken; what else holds for it stays.
 int call_workspace(const char *name, size_t need, void *work, size_t work_bytes, hipStream_t s,
-                   std::optional<AttnHold> *hold, char **out) {
+                   std::optional<AttnHold> *hold, char **out, bool unused = false) {
   *out = (char *)work;
   if (need == 0) return 0;
   if (work != nullptr) {
@@ -1116,6 +1117,7 @@ int call_workspace(const char *name, size_t need, void *work, size_t work_bytes,
   }
   if (capturing(s))
     return fail("%s: a call that is captured needs a workspace of its own (%zu bytes)", name, need);
+  if (unused) return 0;
   hold->emplace(s);
   GH_CHECK(name, (*hold)->get(need, out));
   return 0;
@@ -1496,7 +1498,7 @@ int gemma_hip_adapters_add(float *dst, int dstr, const float *base, int bstr,
   hipStream_t s = pick_stream(stream);
   std::optional<AttnHold> hold;
   if (call_workspace(name, gh::adapters_work(adapters->rows, njobs, adapters->rank), work,
-                     work_bytes, s, &hold, &a.work))
+                     work_bytes, s, &hold, &a.work, gh::adapters_one_launch(a)))
     return 1;
   {
     PerfScope perf(adapters->max_rows > 1 ? kOpGemmFpx : kOpGemvFpx, s);
@@ -1544,7 +1546,7 @@ int gemma_hip_logprobs(const gemma_hip_scores *scores, const float *logits, int 
   hipStream_t s = pick_stream(stream);
   std::optional<AttnHold> hold;
   if (call_workspace(name, gh::logprobs_work(rows, vocab, targets, ntop), work, work_bytes, s,
-                     &hold, &a.work))
+                     &hold, &a.work, gh::logprobs_one_launch(rows, vocab, g.info)))
     return 1;
   {
     PerfScope perf(kOpSample, s);

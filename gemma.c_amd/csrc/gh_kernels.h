@@ -495,6 +495,7 @@ struct Adapters {
   char *work;
 };
 size_t adapters_work(int rows, int njobs, int rank);
+bool adapters_one_launch(const Adapters &a);  // which writes nothing to work
 hipError_t launch_adapters(const Adapters &a, const DeviceInfo &dev, hipStream_t stream);
 
 // logprobs.hip: what logits say of given tokens, and the likeliest ones.
@@ -514,6 +515,7 @@ struct Logprobs {
   char *work;
 };
 size_t logprobs_work(int rows, int vocab, int targets, int ntop);
+bool logprobs_one_launch(int rows, int vocab, const DeviceInfo &dev);  // which writes nothing to work
 hipError_t launch_logprobs(const Logprobs &a, const DeviceInfo &dev, hipStream_t stream);
 
 // sample.hip: one token per row of logits.  Settings are device arrays of a value

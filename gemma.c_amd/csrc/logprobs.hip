@@ -483,12 +483,20 @@ size_t logprobs_work(int rows, int vocab, int targets, int ntop) {
   return layout_of(rows, vocab, targets, ntop).all;
 }
 
+namespace {
+bool many_rows(int rows, const DeviceInfo &dev) { return rows > 2 * dev.cus; }
+}  // namespace
+
+// Short rows by one launch, but not many that leave most of a workgroup's waves without a tile: us by
+// two launches and by one, 11 rows of 2511 10.4, 8.5, 256 of 32000 17.7, 14.4, 2048 of 32000 74, 61,
+// 600 of 8000 19.6, 16.8, 2433 of 3023 32, 35.
+bool logprobs_one_launch(int rows, int vocab, const DeviceInfo &dev) {
+  return vocab <= kShortVocab && (!many_rows(rows, dev) || tiles_of(vocab) >= 4);
+}
+
 hipError_t launch_logprobs(const Logprobs &a, const DeviceInfo &dev, hipStream_t stream) {
-  const bool many = a.rows > 2 * dev.cus;
-  // Short rows by one launch, but not many that leave most of a workgroup's waves without a tile: us by
-  // two launches and by one, 11 rows of 2511 10.4, 8.5, 256 of 32000 17.7, 14.4, 2048 of 32000 74, 61,
-  // 600 of 8000 19.6, 16.8, 2433 of 3023 32, 35.
-  if (a.vocab <= kShortVocab && (!many || tiles_of(a.vocab) >= 4)) {
+  const bool many = many_rows(a.rows, dev);
+  if (logprobs_one_launch(a.rows, a.vocab, dev)) {
     many ? logprobs_short_kernel<256><<<a.rows, 256, 0, stream>>>(a)
          : logprobs_short_kernel<1024><<<a.rows, 1024, 0, stream>>>(a);
     return hipGetLastError();

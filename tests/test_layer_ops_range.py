@@ -1,9 +1,11 @@
-"""The operators between the products of a served batch where fp32 ends.  Definitions and bars
-are those of test_layer_ops.py, or stand beside the test."""
+"""The operators between the products of a served batch where fp32 ends, at sums of many
+terms, and calls that need none of the library's memory.  Definitions and bars are those of
+test_layer_ops.py, or stand beside the test."""
 
 from __future__ import annotations
 
 import math
+import threading
 
 import numpy as np
 import pytest
@@ -261,3 +263,72 @@ def test_adapters_of_the_smallest_values(gh, kind, rows, where):
     floor += step * np.abs(q).sum(1)
     room = (math.sqrt(3 * k) + math.sqrt(3 * rank) + 8) * HALF
     assert (np.abs(got - want) <= room * size + 1.01 * floor).all()
+
+
+# ---- workspaces ---------------------------------------------------------------------
+
+
+@pytest.mark.gpu
+def test_calls_of_one_launch_wait_for_no_other_s_workspace(gh):
+    """Short rows' log probabilities and single tokens' small adapters write no workspace: without
+    one of their own they go on while another thread waits for the library's to grow."""
+    import torch
+
+    from test_serving_limits import attention_call
+
+    small, need0 = attention_call(gh, 1, [3000])
+    large, need1 = attention_call(gh, 2, [4000] * 40)
+    assert 0 < need0 < need1
+    busy, free = torch.cuda.Stream(), torch.cuda.Stream()
+    logits, h = torch.randn((2, 3000), device="cuda"), torch.zeros(2, device="cuda")
+    x, out = torch.randn((2, 64), device="cuda"), torch.zeros((2, 24), device="cuda")
+    a, b = torch.randn((1, 8, 64), device="cuda"), torch.randn((1, 24, 8), device="cuda")
+    row0, ids = cuda(np.array([0, 1, 2], np.int32)), cuda(np.zeros(2, np.int32))
+    ad = gemma_hip.adapters(row0, ids, None, 2, 2, 1, 1, 8, ADAPTER_F32)
+    jobs = gemma_hip.adapter_jobs([(a, b, 24)])
+    zeros = torch.zeros_like(out)
+
+    def calls():
+        gh.logprobs(gemma_hip.scores(entropy=h), logits, 0, 2, 3000, None, None, 0, 0, None,
+                    free.cuda_stream)
+        gh.adapters_add(out, 0, zeros, 0, ad, jobs, x, 0, 64, None, free.cuda_stream)
+
+    m = torch.randn((8192, 8192), device="cuda")
+    to = torch.empty_like(m)
+    torch.mm(m, m, out=to)
+    small(None, busy.cuda_stream)
+    torch.cuda.synchronize()
+    calls()
+    torch.cuda.synchronize()
+    want = h.clone(), out.clone()
+    h.zero_()
+    out.zero_()
+    torch.cuda.synchronize()
+    begun, errors = threading.Event(), []
+
+    def grow():
+        try:
+            begun.set()
+            large(None, busy.cuda_stream)
+        except Exception as e:  # (shown by the main thread)
+            errors.append(e)
+
+    with torch.cuda.stream(busy):
+        for _ in range(200):
+            torch.mm(m, m, out=to)
+        done = torch.cuda.Event()
+        done.record()
+    t = threading.Thread(target=grow)
+    t.start()
+    begun.wait()
+    t.join(0.2)  # time to take the lock and to wait
+    waiting = t.is_alive()
+    calls()
+    early = not done.query()
+    free.synchronize()
+    t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    assert waiting, "the other thread's call was not waiting: this shows nothing"
+    assert early, "a call that needs no workspace waited for another thread's"
+    assert torch.equal(h, want[0]) and torch.equal(out, want[1])
