@@ -332,3 +332,30 @@ def test_calls_of_one_launch_wait_for_no_other_s_workspace(gh):
     assert waiting, "the other thread's call was not waiting: this shows nothing"
     assert early, "a call that needs no workspace waited for another thread's"
     assert torch.equal(h, want[0]) and torch.equal(out, want[1])
+
+
+@pytest.mark.gpu
+def test_log_probabilities_of_two_launches_on_two_streams(gh):
+    """The library's own workspaces are a stream's: rows that take two launches, and so one, on two
+    streams at once."""
+    import torch
+
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    logits = [torch.randn((3, 40000 + i), device="cuda") for i in range(2)]
+
+    def one(i, s):
+        o = dict(entropy=torch.empty(3, device="cuda"),
+                 top=torch.empty((3, 12), dtype=torch.int32, device="cuda"))
+        gh.logprobs(gemma_hip.scores(**o), logits[i], 0, 3, 40000 + i, None, None, 0, 12, None, s)
+        return [o["entropy"], o["top"]]
+
+    want = [one(i, stream()) for i in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(40):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append((i, one(i, s.cuda_stream)))
+    torch.cuda.synchronize()
+    for i, g in got:
+        assert all(torch.equal(x, y) for x, y in zip(g, want[i]))
