@@ -389,9 +389,22 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void adapter_shrink_kernel(Adapt
   // Pieces don't make up an infinity, nor a value that rounds to an infinite bf16; sums of such ones
   // are never finite, and are done over without pieces, one after the other.
   if (__any(has && !finite(largest(0.0f, sum)))) {
+    uint64_t rows = __ballot(has && !finite(largest(0.0f, sum)));
+    rows = (rows | rows >> 16 | rows >> 32 | rows >> 48) & 0xffff;
+    uint64_t nan = 0;  // rows with NaN among the inputs, whose sums are what they should be
+    for (; rows != 0; rows &= rows - 1) {
+      const int r = __ffsll((unsigned long long)rows) - 1;
+      const float *x = a.src + (tile.row + r) * a.src_stride;
+      float most = 0.0f;
+#pragma unroll 4
+      for (int c = 4 * lane; c < a.k; c += 256)
+        most = largest(most, *reinterpret_cast<const v4f *>(x + c));
+      if (__any(most != most)) nan |= 1ull << r;
+    }
     for (int e = 0; e < 4; ++e) {
       const float mine = e == 0 ? sum[0] : e == 1 ? sum[1] : e == 2 ? sum[2] : sum[3];
-      for (uint64_t bad = __ballot(has && !finite(mine)); bad != 0; bad &= bad - 1) {
+      uint64_t bad = __ballot(has && !finite(mine) && (nan >> m16 & 1) == 0);
+      for (; bad != 0; bad &= bad - 1) {
         const int of = __ffsll((unsigned long long)bad) - 1;
         const int u = at0 + 16 * wave + 4 * (of / 16) + e, job = u / a.rank;
         const void *const m[1] = {job_of(a.a, job)};
@@ -747,8 +760,23 @@ void adapter_expand_kernel(Adapters a) {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
     if (__any(!finite(most))) {  // as in the first product; a lane a column
+      uint64_t nan = 0;  // rows with NaN among u
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        const int rows = min(tile.rows - 16 * i, 16);
+        bool some = false;
+        for (int k = k0; k < a.rank && m < rows; k += 32) {
+          const u4 p = *reinterpret_cast<const u4 *>(piece_of(a, tile.row + 16 * i, rows, job, 0) +
+                                                     (k / 8 * rows + m) * 8);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            some = some || bf16_lo(p[e]) != bf16_lo(p[e]) || bf16_hi(p[e]) != bf16_hi(p[e]);
+        }
+        const uint64_t all = __ballot(some);
+        nan |= ((all | all >> 16 | all >> 32 | all >> 48) & 0xffff) << 16 * i;
+      }
       for (int r = 0; r < tile.rows; ++r) {
-        const bool bad = c0 + lane < width && !finite(sums[r][lane]);
+        const bool bad = c0 + lane < width && !finite(sums[r][lane]) && (nan >> r & 1) == 0;
         if (!__any(bad)) continue;
         const int rows = min(tile.rows - r / 16 * 16, 16);
         const size_t row = (size_t)(bad ? lane : 0) * a.rank;

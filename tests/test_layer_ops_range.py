@@ -195,12 +195,12 @@ def test_adapters_at_the_largest_values(gh, kind, rows, n, rank, where):
 @pytest.mark.parametrize("rows,n", ENDS)
 @pytest.mark.parametrize("rank", [8, 40, 128])
 def test_adapters_of_infinities(gh, kind, rows, n, rank):
-    """One infinity or NaN in the inputs or the matrices comes out where it belongs, and nowhere
-    else."""
+    """An infinity or NaN in the inputs or the matrices comes out where it belongs, and nowhere
+    else, a row of one beside a row of the other too."""
     k, rng = 136, np.random.default_rng(rows + n)
     a, b = (rng.random(s).astype(F32) + F32(0.5) for s in ((rank, k), (n, rank)))
     x = rng.random((rows, k)).astype(F32) + F32(0.5)
-    for where in range(4):
+    for where in range(5):
         p, q, y = a.copy(), b.copy(), x.copy()
         if where == 0:
             y[0, 3], y[-1, k - 1] = np.inf, -np.inf
@@ -210,6 +210,8 @@ def test_adapters_of_infinities(gh, kind, rows, n, rank):
             p[rank - 1, 9], q[:, rank - 1] = np.inf, np.where(np.arange(n) % 3 == 0, 0.0, 1.0)
         else:
             q[5, 2], q[n - 1, rank - 1], q[6, 1] = np.inf, -np.inf, np.nan
+        if where == 4:
+            y[0, 3], y[-1, 1] = np.nan, np.inf
         got, want, size = one_adapter(gh, TYPES[kind], p, q, y)
         assert not np.isfinite(want).all()
         agree(got, want, size, k, rank)
