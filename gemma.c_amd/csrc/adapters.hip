@@ -18,8 +18,10 @@
 // whose neighbouring lanes have a row each, as the matrix instructions want them, takes 64 cycles
 // (4096 rows of 2560 with 48 values of u so: 23 us, by whole runs and LDS 15), so all tiles but B's of
 // short sequences are read by runs and turned in LDS.  4096 rows of 2560 by rank 16 on 4096 columns: first
-// product 15 us (42 MB, 8 at a copy's rate), second 25 (134 MB, 26); 851 rows of 2560 by rank 64 on
-// 20480 columns, f16: 14 and 35 (139 MB, 27).
+// product 16 us (42 MB, 8 at a copy's rate), second 26 (134 MB, 26), 42 a call in bf16, 45 in f16 and
+// 52 in fp32; 851 rows of 2560 by rank 64 on 20480 columns, f16: 14 and 36 (139 MB, 27).  Single
+// tokens beside a chunk of a prompt each have a tile, which a workgroup takes for itself: 63 beside
+// 512 rows by rank 16 on 20480 columns 84 us (106 MB, 21).
 #include <type_traits>
 
 #include "gh_arith.h"
@@ -824,9 +826,13 @@ void adapter_expand_kernel(Adapters a) {
 
 // Up to so many rows a sequence go by the row: with more, a tile's 16 rows share what is read.
 constexpr int kFewRows = 2;
-// Bytes of an adapter's matrices up to which a row is one workgroup's.  us a call, in a row of eager
-// ones and in a graph, by two launches and by one: 32 rows of 156 KiB 11.6 and 5.6, 8.7 and 7.0; of
-// 368 KiB 11.2 and 7.7, 12.8 and 12.8.
+// Bytes of an adapter's matrices up to which a row is one workgroup's.  The rule is for eager calls,
+// where the host's launches set the time; a graph of few tokens pays for it.  us a call by two launches
+// and by one, in a row of eager ones: 1 row of 80 KiB 11.0, 8.8, of 156 KiB 10.7, 8.8, of 234 KiB
+// 10.4, 9.5; 32 rows 10.3, 8.3, then 10.2, 8.4, then 10.1, 10.4; 64 rows 10.1, 8.3, then 10.2, 8.3, then
+// 10.0, 11.6; 200 rows 10.0, 8.4, then 11.1, 9.0, then 15.2, 12.2.  In a graph: 1 row 5.4, 6.7, then
+// 5.4, 6.8, then 6.0, 9.1; 32 rows 5.6, 7.0, then 5.7, 7.1, then 6.9, 10.1; 64 rows 6.0, 7.2, then
+// 6.6, 7.4, then 9.1, 11.4; 200 rows 7.7, 7.7, then 11.1, 8.9, then 15.2, 12.2.
 constexpr long kRowBytes = 192 << 10;
 
 }  // namespace

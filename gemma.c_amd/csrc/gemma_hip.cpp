@@ -1437,7 +1437,7 @@ int gemma_hip_norm_residual(const gemma_hip_residual *residual, int rows, int di
 
 namespace {
 
-// Rows times columns, or times values of u, of a call of the adapters', at most.
+// Rows of a call of the adapters', at most: a grid of 256 threads a row holds them.
 constexpr long kAdapterMostRows = 1l << 22;
 
 int adapter_args(const char *name, const gemma_hip_adapters *ad, int njobs, int k) {

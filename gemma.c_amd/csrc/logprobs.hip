@@ -10,8 +10,9 @@
 // So one reading does: a wave takes 2048 columns, 32 a lane in registers, and leaves S and T by
 // its own largest logit (fp32, the exponents' errors below 2^-22), the given tokens' counts and its 32
 // runs' largest logits.  A second launch joins a row's (fp64) and looks into the n runs that
-// matter.  256 rows of 262144 (268 MB) take 49 + 8 us: the reading at 5.4 TB/s, the join a chain of
-// two trips to memory and two searches; one row 5 + 7.
+// matter.  256 rows of 262144 (268 MB) take 56 + 9 us by themselves: the reading at 4.8 TB/s, the join
+// a chain of two trips to memory and two searches; one row 5 + 9.  Short rows are bound by that chain,
+// not by their bytes: 4000 rows of 1500 38 us (24 MB, 5 at a copy's rate), 256 of 32000 14.4 (33, 6).
 #include <float.h>
 #include <type_traits>
 

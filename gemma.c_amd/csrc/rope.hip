@@ -3,8 +3,10 @@
 // Pair j of a head's first `rot` values (x, y) becomes (x c - y s, y c + x s), c and s amp times
 // the cosine and sine of pos f_j; the others stay.  Before that comes, if asked for, the head's
 // norm x / sqrt(mean x^2 + eps) (w + 1).  Both in fp64, rounded to fp32 once: a far position's
-// angle needs more than fp32, and the keys' codes that follow are then the exact ones but where
-// a border between two codes is hit to 1e-15 (an fp32 rounding in between moves one in 10^5).
+// angle needs more than fp32.  What is off before that is 1e-15 of the head's largest value and
+// the rounding of pos f_j, 2^-53 of the angle: up to 7e-12 by position 131071.  The keys' codes that
+// follow are the exact ones but where a border between two codes is hit to that (an fp32 rounding
+// in between moves one in 10^5).
 //
 // Few rows, and heads of any size: a head is hdim / 4 lanes' (16, 32 or 64 of them), four values a
 // lane: pairs 2l and 2l + 1 of lane l, then what doesn't turn.
@@ -12,8 +14,10 @@
 // Many rows of heads of 64, 128 or 256 values: a row is hdim / 16 lanes', which take one head after
 // the other and have all the angles of their values from the start.  That is a quarter of the sums
 // over lanes, scales and addresses: 16 values a lane instead of 4.  9342 rows of 8 + 4 + 4 heads of
-// 256 (249 MB) take 55 us, 4.5 TB/s, with 76 vector instructions a head; with 4 values a lane
-// 199, which bounded it (66 us).
+// 256 (249 MB) take 59 us, 4.2 TB/s, with 76 vector instructions a head; with 4 values a lane
+// 199, which bounded it (66 us).  Other heads and rotations take four values a lane however many rows
+// there are, 24 or 18 of 32 lanes at work for heads of 96 or 72: 4096 rows of 16 heads 13 us (96, 50
+// MB) and 12 (72, 38 MB).
 #include <type_traits>
 
 #include "dec_common.h"
